@@ -38,6 +38,26 @@ void flash_attn_fwd_tc(torch::Tensor qkv, torch::Tensor o, torch::Tensor lse, in
 void flash_attn_bwd_tc(torch::Tensor qkv, torch::Tensor o, torch::Tensor dout, torch::Tensor lse, torch::Tensor dqkv,
                        torch::Tensor dq_acc, torch::Tensor delta, int64_t n_head, double scale, torch::Tensor status);
 void exp2_poly_eval(torch::Tensor x, torch::Tensor y);
+// generation.cpp
+void copy_pages(torch::Tensor kv, torch::Tensor src, torch::Tensor dst, torch::Tensor status);
+void fork_sequences(torch::Tensor kv, torch::Tensor page_table, torch::Tensor lens, torch::Tensor refs,
+                    torch::Tensor parents, torch::Tensor children, torch::Tensor status);
+void reserve_pages(torch::Tensor page_table, torch::Tensor lens, torch::Tensor refs, torch::Tensor slots,
+                   torch::Tensor counts, int64_t page_size, torch::Tensor status);
+void free_sequences(torch::Tensor page_table, torch::Tensor lens, torch::Tensor refs, torch::Tensor slots,
+                    torch::Tensor status);
+std::tuple<torch::Tensor, torch::Tensor> compact_pages(torch::Tensor kv, torch::Tensor page_table, torch::Tensor refs,
+                                                       torch::Tensor status);
+void append_kv(torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor k, torch::Tensor v, torch::Tensor page_table,
+               torch::Tensor positions, c10::optional<torch::Tensor> slots, torch::Tensor status);
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>> sample(
+    torch::Tensor logits, torch::Tensor noise, c10::optional<torch::Tensor> temperature, double temperature_all,
+    c10::optional<torch::Tensor> top_k, int64_t top_k_all, c10::optional<torch::Tensor> top_p, double top_p_all,
+    c10::optional<torch::Tensor> min_p, double min_p_all, bool return_logprob);
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(
+    torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor prefix_pages, int64_t prefix_len,
+    torch::Tensor page_table, torch::Tensor seq_lens, c10::optional<torch::Tensor> q_offsets, int64_t max_q_len,
+    int64_t max_seq_len, double scale, bool return_lse, torch::Tensor status);
 // comm.cu
 void register_comm(pybind11::module_& m);
 }  // namespace mnb
@@ -63,5 +83,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("flash_attn_fwd_tc", &mnb::flash_attn_fwd_tc, "tcgen05 flash attention forward");
   m.def("flash_attn_bwd_tc", &mnb::flash_attn_bwd_tc, "tcgen05 flash attention backward");
   m.def("exp2_poly_eval", &mnb::exp2_poly_eval, "the attention softmax's FMA-pipe exp2, over a tensor");
+  m.def("copy_pages", &mnb::copy_pages);
+  m.def("fork_sequences", &mnb::fork_sequences);
+  m.def("reserve_pages", &mnb::reserve_pages);
+  m.def("free_sequences", &mnb::free_sequences);
+  m.def("compact_pages", &mnb::compact_pages);
+  m.def("append_kv", &mnb::append_kv);
+  m.def("sample", &mnb::sample, "temperature / top-k / top-p / min-p sampling from given noise");
+  m.def("shared_prefix_attention", &mnb::shared_prefix_attention,
+        "paged attention over a shared prefix and each sequence's own tokens");
   mnb::register_comm(m);
 }

@@ -1,0 +1,391 @@
+// Page operations of the paged key / value cache.
+//
+// The pool is one tensor [..., num_pages, page_size, kv_heads, head_dim]; the
+// leading axes (layers, keys / values) are "planes" that every page id names
+// at once.  The bookkeeping lives on the device, so no operation waits for
+// the host: page_table [sequences, columns] (int32, -1 past a sequence's last
+// page), lens [sequences] and refs [num_pages], the number of sequences that
+// hold each page.  refs is the only record of what is free; a page is free
+// when its count is zero, and the lowest free ids are handed out first, in
+// the order of the requests, so results do not depend on scheduling.
+//
+// Bookkeeping kernels are one block (a few thousand counts); they leave a
+// list of copies that a second kernel with many blocks carries out.  Bad
+// indices and a pool without room set the status word and leave the request
+// out; nothing is read or written out of range.
+#include <algorithm>
+
+#include "common.cuh"
+#include "generation.h"
+
+namespace mnb {
+
+namespace cache {
+
+constexpr int kThreads = 1024;
+
+MNB_DEVICE void flag(int* status, int code) { atomicCAS(status, 0, code); }
+
+// Exclusive scan over the block; *total gets the sum.  `sh` holds 33 ints.
+MNB_DEVICE int block_scan(int v, int* sh, int* total) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) sh[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int s = lane < blockDim.x / 32 ? sh[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += y;
+    }
+    sh[lane] = s;
+  }
+  __syncthreads();
+  const int before = warp == 0 ? 0 : sh[warp - 1];
+  *total = sh[blockDim.x / 32 - 1];
+  __syncthreads();
+  return before + x - v;
+}
+
+// The first `want` free pages in ascending order into ids[]; returns how many there are (at most want).
+MNB_DEVICE int find_free(const int* refs, int pages, int want, int* ids, int* sh) {
+  int found = 0;
+  for (int p0 = 0; p0 < pages && found < want; p0 += kThreads) {
+    const int p = p0 + threadIdx.x;
+    const int is_free = p < pages && refs[p] == 0;
+    int total;
+    const int rank = found + block_scan(is_free, sh, &total);
+    if (is_free && rank < want) ids[rank] = p;
+    found += total;
+  }
+  __syncthreads();
+  return min(found, want);
+}
+
+// Marks in owner[slot] the first request that names each slot (requests that
+// name it again are refused).
+MNB_DEVICE void claim(const int* slot_of, int n, int slots, int* owner) {
+  for (int s = threadIdx.x; s < slots; s += kThreads) owner[s] = 0x7fffffff;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const int s = slot_of[i];
+    if (s >= 0 && s < slots) atomicMin(owner + s, i);
+  }
+  __syncthreads();
+}
+
+// fork: child i gets parent i's table row; full pages are shared, the
+// part-filled last one gets a page of its own (src / dst / tokens name the copy).
+__global__ void __launch_bounds__(kThreads) fork_plan_kernel(Table t, const int* __restrict__ parents,
+                                                             const int* __restrict__ children, int n, int* owner,
+                                                             int* ids, int* src, int* dst, int* tokens, int* status) {
+  __shared__ int sh[33];
+  claim(children, n, t.slots, owner);
+  // which requests are sound, and which need a page (ids' rank parked in dst)
+  int base = 0;
+  for (int i0 = 0; i0 < n; i0 += kThreads) {
+    const int i = i0 + threadIdx.x;
+    int need = 0, part = -1;
+    if (i < n) {
+      const int p = parents[i], c = children[i];
+      bool ok = p >= 0 && p < t.slots && c >= 0 && c < t.slots && owner[c] == i && t.lens[c] == 0;
+      ok = ok && owner[p] == 0x7fffffff;  // a parent is nobody's child in the same call
+      if (ok) {
+        const int len = t.lens[p];
+        ok = len >= 0 && len <= t.columns * static_cast<long long>(t.page_size);
+        if (ok) {
+          part = len % t.page_size;
+          need = part > 0;
+        }
+      }
+      if (!ok) flag(status, kErrBadIndex);
+    }
+    int total;
+    const int rank = base + block_scan(need, sh, &total);
+    if (i < n) {
+      tokens[i] = part;
+      dst[i] = need ? rank : -1;
+    }
+    base += total;
+  }
+  const int have = find_free(t.refs, t.pages, base, ids, sh);
+  if (base > have && threadIdx.x == 0) flag(status, kErrNoPages);
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    src[i] = -1;
+    if (dst[i] >= have) tokens[i] = dst[i] = -1;  // no page left: the child stays empty
+  }
+  __syncthreads();
+  for (long long x = threadIdx.x; x < static_cast<long long>(n) * t.columns; x += kThreads) {
+    const int i = static_cast<int>(x / t.columns), col = static_cast<int>(x % t.columns);
+    if (tokens[i] < 0) continue;
+    const int full = t.lens[parents[i]] / t.page_size;
+    int page = -1;
+    if (col <= full) {
+      page = t.table[parents[i] * t.ld + col];
+      if (col == full) {
+        if (tokens[i] > 0 && page >= 0 && page < t.pages) src[i] = page;
+        page = tokens[i] > 0 ? ids[dst[i]] : -1;
+        if (page >= 0) t.refs[page] = 1;
+      } else if (page < 0 || page >= t.pages) {
+        flag(status, kErrBadIndex);
+        page = -1;
+      } else {
+        atomicAdd(t.refs + page, 1);
+      }
+    }
+    t.table[children[i] * t.ld + col] = page;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    if (tokens[i] < 0) continue;
+    if (dst[i] >= 0) dst[i] = ids[dst[i]];
+    if (dst[i] >= 0 && src[i] < 0) flag(status, kErrBadIndex);  // the parent's last page is not in the pool
+    t.lens[children[i]] = t.lens[parents[i]];
+  }
+}
+
+// reserve: slot i grows by counts[i] tokens; new pages fill its row.
+__global__ void __launch_bounds__(kThreads) reserve_kernel(Table t, const int* __restrict__ slot_of,
+                                                           const int* __restrict__ counts, int n, int* owner, int* ids,
+                                                           int most, int* rank_of, int* status) {
+  __shared__ int sh[33];
+  claim(slot_of, n, t.slots, owner);
+  int base = 0;
+  for (int i0 = 0; i0 < n; i0 += kThreads) {
+    const int i = i0 + threadIdx.x;
+    int need = 0;
+    if (i < n) {
+      const int s = slot_of[i], more = counts[i];
+      bool ok = s >= 0 && s < t.slots && owner[s] == i && more >= 0;
+      if (ok) {
+        const long long len = t.lens[s], to = len + more;
+        ok = len >= 0 && to <= t.columns * static_cast<long long>(t.page_size);
+        if (ok) need = static_cast<int>((to + t.page_size - 1) / t.page_size - (len + t.page_size - 1) / t.page_size);
+      }
+      if (!ok) {
+        flag(status, kErrBadIndex);
+        need = -1;
+      }
+    }
+    int total;
+    const int rank = base + block_scan(max(need, 0), sh, &total);
+    if (i < n) rank_of[i] = need < 0 ? -1 : rank;
+    base += total;
+  }
+  const int have = find_free(t.refs, t.pages, min(base, most), ids, sh);
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    if (rank_of[i] < 0) continue;
+    const int s = slot_of[i], len = t.lens[s];
+    const int c0 = (len + t.page_size - 1) / t.page_size, c1 = (len + counts[i] + t.page_size - 1) / t.page_size;
+    if (c1 > c0 && rank_of[i] + (c1 - c0) > have) {
+      flag(status, kErrNoPages);
+      continue;
+    }
+    for (int c = c0; c < c1; ++c) {
+      const int page = ids[rank_of[i] + c - c0];
+      t.table[s * t.ld + c] = page;
+      t.refs[page] = 1;
+    }
+    t.lens[s] = len + counts[i];
+  }
+}
+
+// free: every page of the slots' rows loses one holder.  The exchange hands
+// each entry to one thread, so naming a slot twice frees it once.
+__global__ void __launch_bounds__(256) free_kernel(Table t, const int* __restrict__ slot_of, int n, int* status) {
+  const long long all = static_cast<long long>(n) * t.columns;
+  for (long long x = blockIdx.x * 256ll + threadIdx.x; x < all; x += gridDim.x * 256ll) {
+    const int i = static_cast<int>(x / t.columns), col = static_cast<int>(x % t.columns);
+    const int s = slot_of[i];
+    if (s < 0 || s >= t.slots) {
+      flag(status, kErrBadIndex);
+      continue;
+    }
+    const int page = atomicExch(t.table + s * t.ld + col, -1);
+    if (col == 0) t.lens[s] = 0;
+    if (page < 0) continue;
+    if (page >= t.pages) {
+      flag(status, kErrBadIndex);
+    } else if (atomicSub(t.refs + page, 1) <= 0) {  // nobody held it: put the count back
+      atomicAdd(t.refs + page, 1);
+      flag(status, kErrBadIndex);
+    }
+  }
+}
+
+// compact: with n pages in use, those with ids >= n move, in ascending order,
+// into the free ids below n.  Writes the moves, the new counts and, for every
+// old id, the new one.
+__global__ void __launch_bounds__(kThreads) compact_plan_kernel(const int* __restrict__ refs, int pages,
+                                                                int* __restrict__ new_refs, int* __restrict__ to,
+                                                                int* __restrict__ src, int* __restrict__ dst,
+                                                                int* __restrict__ moves) {
+  __shared__ int sh[33];
+  int live = 0;
+  for (int p0 = 0; p0 < pages; p0 += kThreads) {
+    const int p = p0 + threadIdx.x;
+    live += __syncthreads_count(p < pages && refs[p] > 0);
+  }
+  int movers = 0, holes = 0;
+  for (int p0 = 0; p0 < pages; p0 += kThreads) {
+    const int p = p0 + threadIdx.x;
+    const int r = p < pages ? refs[p] : 0;
+    const bool mover = p < pages && r > 0 && p >= live, hole = p < live && r <= 0;
+    int total;
+    const int rank = block_scan((mover ? 1 << 16 : 0) | (hole ? 1 : 0), sh, &total);
+    if (mover) src[movers + (rank >> 16)] = p;
+    if (hole) dst[holes + (rank & 0xffff)] = p;
+    if (p < pages) {
+      new_refs[p] = p < live ? r : 0;
+      to[p] = r > 0 ? p : -1;
+    }
+    movers += total >> 16;
+    holes += total & 0xffff;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < movers; i += kThreads) {
+    new_refs[dst[i]] = refs[src[i]];
+    to[src[i]] = dst[i];
+  }
+  if (threadIdx.x == 0) *moves = movers;
+}
+
+// 16-byte chunks of the named pages, in every plane: [moves][planes][chunks].
+// `tokens` (or null) gives the leading tokens of each page that hold data.
+__global__ void __launch_bounds__(256) copy_pages_kernel(uint4* __restrict__ pool, long long plane_chunks,
+                                                         int page_chunks, int token_chunks, int planes, int pages,
+                                                         const int* __restrict__ src, const int* __restrict__ dst,
+                                                         const int* __restrict__ tokens, const int* __restrict__ count,
+                                                         int n_max, int* status) {
+  constexpr int kPer = 4;  // independent 16-byte loads per thread
+  const int n = count ? min(*count, n_max) : n_max;
+  const int runs = (page_chunks + 256 * kPer - 1) / (256 * kPer);
+  const long long all = static_cast<long long>(n) * planes * runs;
+  for (long long x = blockIdx.x; x < all; x += gridDim.x) {
+    const int run = static_cast<int>(x % runs);
+    const int plane = static_cast<int>((x / runs) % planes);
+    const int i = static_cast<int>(x / (static_cast<long long>(runs) * planes));
+    const int a = src[i], b = dst[i];
+    if (a < 0 || b < 0) continue;
+    if (a >= pages || b >= pages) {
+      if (threadIdx.x == 0) flag(status, kErrBadIndex);
+      continue;
+    }
+    const int valid = tokens ? min(tokens[i] * token_chunks, page_chunks) : page_chunks;
+    const uint4* from = pool + plane * plane_chunks + static_cast<long long>(a) * page_chunks;
+    uint4* into = pool + plane * plane_chunks + static_cast<long long>(b) * page_chunks;
+    uint4 w[kPer];
+    const int c0 = run * 256 * kPer + threadIdx.x;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+      if (c0 + k * 256 < valid) w[k] = from[c0 + k * 256];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+      if (c0 + k * 256 < valid) into[c0 + k * 256] = w[k];
+  }
+}
+
+// Table entries under the new ids.
+__global__ void __launch_bounds__(256) remap_kernel(const int* __restrict__ table, long long ld, int columns, long long all,
+                                                    const int* __restrict__ to, int pages, int* __restrict__ out) {
+  const long long x = blockIdx.x * 256ll + threadIdx.x;
+  if (x >= all) return;
+  const int p = table[(x / columns) * ld + x % columns];
+  out[x] = p >= 0 && p < pages ? to[p] : -1;
+}
+
+// One 16-byte chunk of one token's keys or values per thread and step.
+__global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ Append a, int* status) {
+  const int per = a.heads * a.chunks;
+  const long long all = static_cast<long long>(a.n) * per;
+  for (long long x = blockIdx.x * 256ll + threadIdx.x; x < all; x += gridDim.x * 256ll) {
+    const int i = static_cast<int>(x / per), r = static_cast<int>(x % per);
+    const int pos = a.positions[i];
+    if (pos < 0) continue;  // padding
+    const int s = a.slot_of ? a.slot_of[i] : i;
+    const int col = pos / a.page_size;
+    if (s < 0 || s >= a.slots || col >= a.columns) {
+      flag(status, kErrBadIndex);
+      continue;
+    }
+    const int page = a.table[s * a.table_ld + col];
+    if (page < 0 || page >= a.pages) {
+      flag(status, kErrBadIndex);
+      continue;
+    }
+    const int h = r / a.chunks, c = (r % a.chunks) * 8;
+    const long long to = page * a.page_ld + (pos % a.page_size) * a.token_ld + h * a.head_ld + c;
+    const uint4 wk = ld_v4(a.k + i * a.k_ld + h * a.k_head + c), wv = ld_v4(a.v + i * a.v_ld + h * a.v_head + c);
+    st_v4(a.k_pool + to, wk);
+    st_v4(a.v_pool + to, wv);
+  }
+}
+
+
+namespace {
+int copy_blocks(long long units) {
+  // 148 SMs x 8 blocks of 256 threads cover the memory latency of a copy
+  return static_cast<int>(std::max<long long>(1, std::min<long long>(units, 148 * 8)));
+}
+}  // namespace
+
+cudaError_t launch_copy(const Pool& p, const int* src, const int* dst, const int* tokens, const int* count, int n, int* status,
+                        cudaStream_t stream) {
+  if (n == 0) return cudaSuccess;
+  const long long runs = (p.page_chunks + 1023) / 1024;
+  copy_pages_kernel<<<copy_blocks(static_cast<long long>(n) * p.planes * runs), 256, 0, stream>>>(
+      static_cast<uint4*>(p.base), p.plane_chunks, p.page_chunks, p.token_chunks, p.planes, p.pages, src, dst, tokens, count,
+      n, status);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_fork(const Pool& p, const Table& t, const int* parents, const int* children, int n, int* scratch,
+                        int* status, cudaStream_t stream) {
+  int* s = scratch;
+  fork_plan_kernel<<<1, kThreads, 0, stream>>>(t, parents, children, n, s + 4 * n, s, s + n, s + 2 * n, s + 3 * n, status);
+  if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
+  return launch_copy(p, s + n, s + 2 * n, s + 3 * n, nullptr, n, status, stream);
+}
+
+cudaError_t launch_reserve(const Table& t, const int* slots, const int* counts, int n, int* scratch, int* status,
+                           cudaStream_t stream) {
+  int* s = scratch;
+  reserve_kernel<<<1, kThreads, 0, stream>>>(t, slots, counts, n, s + t.pages + n, s, t.pages, s + t.pages, status);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_free(const Table& t, const int* slots, int n, int* status, cudaStream_t stream) {
+  const long long all = static_cast<long long>(n) * t.columns;
+  free_kernel<<<copy_blocks((all + 255) / 256), 256, 0, stream>>>(t, slots, n, status);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_compact(const Pool& p, const int* table, long long table_ld, int rows, int columns, const int* refs,
+                           int* new_table, int* new_refs, int* scratch, int* status, cudaStream_t stream) {
+  int* s = scratch;
+  compact_plan_kernel<<<1, kThreads, 0, stream>>>(refs, p.pages, new_refs, s, s + p.pages, s + 2 * p.pages, s + 3 * p.pages);
+  if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
+  const long long all = static_cast<long long>(rows) * columns;
+  if (all > 0) {
+    remap_kernel<<<static_cast<unsigned>((all + 255) / 256), 256, 0, stream>>>(table, table_ld, columns, all, s, p.pages,
+                                                                               new_table);
+    if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
+  }
+  return launch_copy(p, s + p.pages, s + 2 * p.pages, nullptr, s + 3 * p.pages, p.pages, status, stream);
+}
+
+cudaError_t launch_append(const Append& a, int* status, cudaStream_t stream) {
+  const long long all = static_cast<long long>(a.n) * a.heads * a.chunks;
+  append_kernel<<<copy_blocks((all + 255) / 256), 256, 0, stream>>>(a, status);
+  return cudaGetLastError();
+}
+
+}  // namespace cache
+
+}  // namespace mnb

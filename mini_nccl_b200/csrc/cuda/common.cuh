@@ -23,6 +23,8 @@ enum : int {
   kErrPeerTimeout = 1,     // a peer's signal did not arrive before the deadline
   kErrPipelineTimeout = 2, // an intra-CTA mbarrier wait exceeded its budget
   kErrBadArgument = 3,
+  kErrNoPages = 4,         // the key / value cache's pool has too few free pages
+  kErrBadIndex = 5,        // a page, slot, position or length outside its tensor
 };
 
 // ---------------------------------------------------------------------------

@@ -1,0 +1,336 @@
+// Torch entry points of the generation operators: checks of the tensors, their
+// workspaces, and the launches (cache.cu, sampling.cu, prefix_attention.cu).
+#include "generation.h"
+
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <algorithm>
+
+namespace mnb {
+
+namespace {
+
+constexpr double kLog2e = 1.4426950408889634;
+
+void check_int32(const torch::Tensor& t, int64_t dim, const torch::Tensor& like, const char* what) {
+  TORCH_CHECK_VALUE(t.is_cuda() && t.device() == like.device() && t.scalar_type() == at::kInt && t.dim() == dim &&
+                        (t.numel() == 0 || t.stride(dim - 1) == 1),
+                    what, ": a ", dim, "-d int32 tensor on ", like.device(), " with its last axis contiguous");
+  TORCH_CHECK_VALUE(t.numel() < (1ll << 31), what, ": too many entries");
+}
+
+void check_status_word(const torch::Tensor& status) {
+  TORCH_CHECK(status.is_cuda() && status.scalar_type() == at::kInt && status.numel() >= 1, "status: int32 on the device");
+}
+
+// 16-byte accesses along the last axis work at every index.
+bool rows_aligned(const torch::Tensor& t) {
+  bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
+  return ok;
+}
+
+__nv_bfloat16* bf16(const torch::Tensor& t) { return reinterpret_cast<__nv_bfloat16*>(t.data_ptr()); }
+
+cache::Pool pool_of(const torch::Tensor& kv) {
+  TORCH_CHECK_VALUE(kv.is_cuda() && kv.dim() >= 4 && kv.is_contiguous(),
+                    "kv: a contiguous CUDA tensor [..., num_pages, page_size, kv_heads, head_dim]");
+  TORCH_CHECK_VALUE(kv.numel() > 0, "kv: an empty pool");
+  const int64_t d = kv.dim();
+  const int64_t token = kv.size(d - 1) * kv.size(d - 2) * kv.element_size();
+  const int64_t page = token * kv.size(d - 3), pages = kv.size(d - 4);
+  TORCH_CHECK_VALUE(token % 16 == 0 && reinterpret_cast<uintptr_t>(kv.data_ptr()) % 16 == 0,
+                    "kv: a token's keys must be a multiple of 16 bytes, 16-byte aligned (got ", token, " bytes)");
+  TORCH_CHECK_VALUE(page / 16 < (1 << 30) && pages < (1 << 29), "kv: pages too large");
+  cache::Pool p;
+  p.base = kv.data_ptr();
+  p.plane_chunks = pages * (page / 16);
+  p.page_chunks = static_cast<int>(page / 16);
+  p.token_chunks = static_cast<int>(token / 16);
+  p.planes = static_cast<int>(kv.numel() * kv.element_size() / (page * pages));
+  p.pages = static_cast<int>(pages);
+  p.page_size = static_cast<int>(kv.size(d - 3));
+  return p;
+}
+
+cache::Table table_of(const torch::Tensor& page_table, const torch::Tensor& lens, const torch::Tensor& refs, int page_size) {
+  check_int32(page_table, 2, page_table, "page_table");
+  check_int32(lens, 1, page_table, "lens");
+  check_int32(refs, 1, page_table, "refs");
+  TORCH_CHECK_VALUE(lens.size(0) == page_table.size(0), "lens: one entry for each row of page_table");
+  return cache::Table{page_table.data_ptr<int>(), lens.data_ptr<int>(), refs.data_ptr<int>(), page_table.stride(0),
+                      static_cast<int>(page_table.size(0)), static_cast<int>(page_table.size(1)),
+                      static_cast<int>(refs.size(0)), page_size};
+}
+
+template <typename S>
+S setting(const c10::optional<torch::Tensor>& each, double all, int64_t rows, at::ScalarType type, const torch::Tensor& like,
+          const char* what) {
+  S s{nullptr, static_cast<decltype(S::all)>(all)};
+  if (each) {
+    TORCH_CHECK_VALUE(each->device() == like.device() && each->scalar_type() == type && each->dim() == 1 &&
+                          each->size(0) == rows && each->is_contiguous(),
+                      what, ": a number, or a contiguous ", type, " tensor with one entry for each of the ", rows, " rows");
+    s.each = each->data_ptr<decltype(S::all)>();
+  }
+  return s;
+}
+
+}  // namespace
+
+void copy_pages(torch::Tensor kv, torch::Tensor src, torch::Tensor dst, torch::Tensor status) {
+  const auto p = pool_of(kv);
+  check_int32(src, 1, kv, "src");
+  check_int32(dst, 1, kv, "dst");
+  check_status_word(status);
+  TORCH_CHECK_VALUE(src.size(0) == dst.size(0), "src and dst: one destination for each source");
+  const c10::cuda::CUDAGuard guard(kv.device());
+  C10_CUDA_CHECK(cache::launch_copy(p, src.data_ptr<int>(), dst.data_ptr<int>(), nullptr, nullptr,
+                                    static_cast<int>(src.size(0)), status.data_ptr<int>(), at::cuda::getCurrentCUDAStream()));
+}
+
+void fork_sequences(torch::Tensor kv, torch::Tensor page_table, torch::Tensor lens, torch::Tensor refs,
+                    torch::Tensor parents, torch::Tensor children, torch::Tensor status) {
+  const auto p = pool_of(kv);
+  const auto t = table_of(page_table, lens, refs, p.page_size);
+  check_int32(parents, 1, kv, "parents");
+  check_int32(children, 1, kv, "children");
+  check_status_word(status);
+  TORCH_CHECK_VALUE(page_table.device() == kv.device(), "page_table and kv: on one device");
+  TORCH_CHECK_VALUE(refs.size(0) == p.pages, "refs: one count for each page of kv");
+  TORCH_CHECK_VALUE(parents.size(0) == children.size(0), "parents and children: one parent for each child");
+  const int64_t n = parents.size(0);
+  if (n == 0 || t.slots == 0) return;
+  TORCH_CHECK_VALUE(n < (1 << 28), "children: too many");
+  const c10::cuda::CUDAGuard guard(kv.device());
+  auto scratch = torch::empty({4 * n + t.slots}, parents.options());
+  C10_CUDA_CHECK(cache::launch_fork(p, t, parents.data_ptr<int>(), children.data_ptr<int>(), static_cast<int>(n),
+                                    scratch.data_ptr<int>(), status.data_ptr<int>(), at::cuda::getCurrentCUDAStream()));
+}
+
+void reserve_pages(torch::Tensor page_table, torch::Tensor lens, torch::Tensor refs, torch::Tensor slots,
+                   torch::Tensor counts, int64_t page_size, torch::Tensor status) {
+  TORCH_CHECK_VALUE(page_size >= 1 && page_size < (1 << 30), "page_size: at least 1");
+  const auto t = table_of(page_table, lens, refs, static_cast<int>(page_size));
+  check_int32(slots, 1, page_table, "slots");
+  check_int32(counts, 1, page_table, "counts");
+  check_status_word(status);
+  TORCH_CHECK_VALUE(slots.size(0) == counts.size(0), "slots and counts: one count for each slot");
+  const int64_t n = slots.size(0);
+  if (n == 0) return;
+  const c10::cuda::CUDAGuard guard(page_table.device());
+  auto scratch = torch::empty({t.pages + n + t.slots}, slots.options());
+  C10_CUDA_CHECK(cache::launch_reserve(t, slots.data_ptr<int>(), counts.data_ptr<int>(), static_cast<int>(n),
+                                       scratch.data_ptr<int>(), status.data_ptr<int>(), at::cuda::getCurrentCUDAStream()));
+}
+
+void free_sequences(torch::Tensor page_table, torch::Tensor lens, torch::Tensor refs, torch::Tensor slots,
+                    torch::Tensor status) {
+  const auto t = table_of(page_table, lens, refs, 1);
+  check_int32(slots, 1, page_table, "slots");
+  check_status_word(status);
+  const int n = static_cast<int>(slots.size(0));
+  if (n == 0 || t.columns == 0) return;
+  const c10::cuda::CUDAGuard guard(page_table.device());
+  C10_CUDA_CHECK(cache::launch_free(t, slots.data_ptr<int>(), n, status.data_ptr<int>(), at::cuda::getCurrentCUDAStream()));
+}
+
+std::tuple<torch::Tensor, torch::Tensor> compact_pages(torch::Tensor kv, torch::Tensor page_table, torch::Tensor refs,
+                                                       torch::Tensor status) {
+  const auto p = pool_of(kv);
+  check_int32(page_table, 2, kv, "page_table");
+  check_int32(refs, 1, kv, "refs");
+  check_status_word(status);
+  TORCH_CHECK_VALUE(refs.size(0) == p.pages, "refs: one count for each page of kv");
+  const c10::cuda::CUDAGuard guard(kv.device());
+  auto new_table = torch::empty(page_table.sizes(), page_table.options());
+  auto new_refs = torch::empty(refs.sizes(), refs.options());
+  auto scratch = torch::empty({3 * static_cast<int64_t>(p.pages) + 1}, refs.options());
+  C10_CUDA_CHECK(cache::launch_compact(p, page_table.data_ptr<int>(), page_table.stride(0),
+                                       static_cast<int>(page_table.size(0)), static_cast<int>(page_table.size(1)),
+                                       refs.data_ptr<int>(), new_table.data_ptr<int>(), new_refs.data_ptr<int>(),
+                                       scratch.data_ptr<int>(), status.data_ptr<int>(), at::cuda::getCurrentCUDAStream()));
+  return {new_table, new_refs};
+}
+
+void append_kv(torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor k, torch::Tensor v, torch::Tensor page_table,
+               torch::Tensor positions, c10::optional<torch::Tensor> slots, torch::Tensor status) {
+  TORCH_CHECK_VALUE(k_pages.is_cuda() && k_pages.dim() == 4 && k_pages.scalar_type() == at::kBFloat16 &&
+                        v_pages.scalar_type() == at::kBFloat16 && v_pages.sizes() == k_pages.sizes() &&
+                        v_pages.strides() == k_pages.strides() && v_pages.device() == k_pages.device(),
+                    "k_pages and v_pages: bf16 CUDA tensors [num_pages, page_size, kv_heads, head_dim] of one layout");
+  TORCH_CHECK_VALUE(k.dim() == 3 && v.dim() == 3 && k.sizes() == v.sizes() && k.scalar_type() == at::kBFloat16 &&
+                        v.scalar_type() == at::kBFloat16 && k.device() == k_pages.device() && v.device() == k.device(),
+                    "k and v: bf16 tensors [tokens, kv_heads, head_dim] on the pages' device");
+  const int64_t H = k_pages.size(2), D = k_pages.size(3), n = k.size(0);
+  TORCH_CHECK_VALUE(k.size(1) == H && k.size(2) == D, "k and v: ", H, " heads of ", D, " as in the pages");
+  TORCH_CHECK_VALUE(D % 8 == 0, "head_dim: a multiple of 8");
+  TORCH_CHECK_VALUE(n == 0 || k_pages.numel() == 0 ||
+                        (rows_aligned(k) && rows_aligned(v) && rows_aligned(k_pages) && rows_aligned(v_pages)),
+                    "k, v and the pages: last axis contiguous, rows 16-byte aligned");
+  check_int32(page_table, 2, k_pages, "page_table");
+  check_int32(positions, 1, k_pages, "positions");
+  check_status_word(status);
+  TORCH_CHECK_VALUE(positions.size(0) == n, "positions: one for each token");
+  if (slots) {
+    check_int32(*slots, 1, k_pages, "slots");
+    TORCH_CHECK_VALUE(slots->size(0) == n, "slots: one for each token");
+  } else {
+    TORCH_CHECK_VALUE(n <= page_table.size(0), "without slots, token i belongs to row i of page_table: too many tokens");
+  }
+  if (n * H * D == 0 || k_pages.size(1) == 0) return;
+  const c10::cuda::CUDAGuard guard(k_pages.device());
+  cache::Append a{};
+  a.k_pool = bf16(k_pages);
+  a.v_pool = bf16(v_pages);
+  a.page_ld = k_pages.stride(0);
+  a.token_ld = k_pages.stride(1);
+  a.head_ld = k_pages.stride(2);
+  a.k = bf16(k);
+  a.v = bf16(v);
+  a.k_ld = k.stride(0);
+  a.k_head = k.stride(1);
+  a.v_ld = v.stride(0);
+  a.v_head = v.stride(1);
+  a.table = page_table.data_ptr<int>();
+  a.table_ld = page_table.stride(0);
+  a.slots = static_cast<int>(page_table.size(0));
+  a.columns = static_cast<int>(page_table.size(1));
+  a.pages = static_cast<int>(k_pages.size(0));
+  a.page_size = static_cast<int>(k_pages.size(1));
+  a.positions = positions.data_ptr<int>();
+  a.slot_of = slots ? slots->data_ptr<int>() : nullptr;
+  a.n = static_cast<int>(n);
+  a.heads = static_cast<int>(H);
+  a.chunks = static_cast<int>(D / 8);
+  C10_CUDA_CHECK(cache::launch_append(a, status.data_ptr<int>(), at::cuda::getCurrentCUDAStream()));
+}
+
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>> sample(
+    torch::Tensor logits, torch::Tensor noise, c10::optional<torch::Tensor> temperature, double temperature_all,
+    c10::optional<torch::Tensor> top_k, int64_t top_k_all, c10::optional<torch::Tensor> top_p, double top_p_all,
+    c10::optional<torch::Tensor> min_p, double min_p_all, bool return_logprob) {
+  using sampling::Setting;
+  TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() == 2 &&
+                        (logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kFloat),
+                    "logits: a bf16 or fp32 tensor [rows, vocabulary]");
+  const int64_t R = logits.size(0), V = logits.size(1);
+  TORCH_CHECK_VALUE(V >= 1 && V <= (1 << sampling::kIndexBits), "vocabulary: 1 to 1048576 tokens, got ", V);
+  TORCH_CHECK_VALUE(logits.stride(1) == 1 || V == 1, "logits: last axis contiguous");
+  TORCH_CHECK_VALUE(noise.device() == logits.device() && noise.scalar_type() == at::kFloat && noise.sizes() == logits.sizes() &&
+                        (noise.stride(1) == 1 || V == 1),
+                    "noise: an fp32 tensor of the logits' shape, last axis contiguous");
+  TORCH_CHECK_VALUE(R < (1ll << 31), "too many rows");
+  sampling::Sample a{};
+  a.temperature = setting<Setting>(temperature, temperature_all, R, at::kFloat, logits, "temperature");
+  a.top_k = setting<sampling::WholeSetting>(top_k, static_cast<double>(std::clamp<int64_t>(top_k_all, 0, V)), R, at::kInt,
+                                            logits, "top_k");
+  a.top_p = setting<Setting>(top_p, top_p_all, R, at::kFloat, logits, "top_p");
+  a.min_p = setting<Setting>(min_p, min_p_all, R, at::kFloat, logits, "min_p");
+  const c10::cuda::CUDAGuard guard(logits.device());
+  auto token = torch::empty({R}, logits.options().dtype(at::kLong));
+  c10::optional<torch::Tensor> logprob;
+  if (return_logprob) logprob = torch::empty({R}, logits.options().dtype(at::kFloat));
+  if (R == 0) return {token, logprob};
+  a.logits = logits.data_ptr();
+  a.bf16 = logits.scalar_type() == at::kBFloat16;
+  a.ld = logits.stride(0);
+  a.noise = noise.data_ptr<float>();
+  a.noise_ld = noise.stride(0);
+  a.rows = static_cast<int>(R);
+  a.vocab = static_cast<int>(V);
+  a.token = reinterpret_cast<long long*>(token.data_ptr<int64_t>());
+  a.logprob = logprob ? logprob->data_ptr<float>() : nullptr;
+  C10_CUDA_CHECK(sampling::launch_sample(a, at::cuda::getCurrentCUDAStream()));
+  return {token, logprob};
+}
+
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(
+    torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor prefix_pages, int64_t prefix_len,
+    torch::Tensor page_table, torch::Tensor seq_lens, c10::optional<torch::Tensor> q_offsets, int64_t max_q_len,
+    int64_t max_seq_len, double scale, bool return_lse, torch::Tensor status) {
+  TORCH_CHECK_VALUE(q.is_cuda() && q.scalar_type() == at::kBFloat16 && q.dim() == 3,
+                    "q: a bf16 CUDA tensor [tokens, heads, head_dim]");
+  TORCH_CHECK_VALUE(k_pages.device() == q.device() && v_pages.device() == q.device() &&
+                        k_pages.scalar_type() == at::kBFloat16 && v_pages.scalar_type() == at::kBFloat16 &&
+                        k_pages.dim() == 4 && k_pages.sizes() == v_pages.sizes() && k_pages.strides() == v_pages.strides(),
+                    "k_pages and v_pages: bf16 tensors [num_pages, page_size, kv_heads, head_dim] of one layout, on q's device");
+  const int64_t N = q.size(0), H = q.size(1), D = q.size(2);
+  const int64_t pages = k_pages.size(0), page = k_pages.size(1), Hk = k_pages.size(2);
+  TORCH_CHECK_VALUE(D == 32 || D == 64 || D == 128, "head_dim: 32, 64 or 128, got ", D);
+  TORCH_CHECK_VALUE(k_pages.size(3) == D, "k_pages: head_dim ", D, " as in q, got ", k_pages.size(3));
+  TORCH_CHECK_VALUE(Hk > 0 && H > 0 && H % Hk == 0, "heads: a multiple of the pages' ", Hk, " kv heads, got ", H);
+  TORCH_CHECK_VALUE(page >= 8 && page <= 256 && (page & (page - 1)) == 0, "page_size: a power of two from 8 to 256, got ", page);
+  TORCH_CHECK_VALUE(N == 0 || rows_aligned(q), "q: last axis contiguous, rows 16-byte aligned");
+  TORCH_CHECK_VALUE(pages == 0 || (rows_aligned(k_pages) && rows_aligned(v_pages)),
+                    "pages: last axis contiguous, rows 16-byte aligned");
+  check_int32(prefix_pages, 1, q, "prefix_pages");
+  check_int32(page_table, 2, q, "page_table");
+  check_int32(seq_lens, 1, q, "seq_lens");
+  check_status_word(status);
+  const int64_t B = page_table.size(0);
+  TORCH_CHECK_VALUE(seq_lens.size(0) == B, "seq_lens: one length for each row of page_table");
+  TORCH_CHECK_VALUE(prefix_len >= 0 && prefix_len <= prefix_pages.size(0) * page, "prefix_len: 0 to the ",
+                    prefix_pages.size(0) * page, " tokens of prefix_pages, got ", prefix_len);
+  const int64_t room = page_table.size(1) * page;
+  if (max_seq_len < 0) max_seq_len = room;
+  TORCH_CHECK_VALUE(max_seq_len <= room, "max_seq_len: at most the ", room, " tokens of a row of page_table, got ", max_seq_len);
+  if (q_offsets) {
+    check_int32(*q_offsets, 1, q, "q_offsets");
+    TORCH_CHECK_VALUE(q_offsets->size(0) == B + 1, "q_offsets: one more entry than page_table has rows");
+    TORCH_CHECK_VALUE(max_q_len >= 0, "max_q_len: needed with q_offsets");
+  } else {
+    TORCH_CHECK_VALUE(N == B, "without q_offsets there is one token for each of the ", B, " sequences, got ", N);
+    max_q_len = 1;
+  }
+  TORCH_CHECK_VALUE(N * H < (1ll << 31) && prefix_len < (1ll << 30) && room < (1ll << 30), "too many rows or keys");
+
+  const c10::cuda::CUDAGuard guard(q.device());
+  auto o = torch::empty({N, H, D}, q.options());
+  c10::optional<torch::Tensor> lse;
+  if (return_lse) lse = torch::empty({N, H}, q.options().dtype(at::kFloat));
+  if (N == 0) return {o, lse};
+
+  prefix::Args a{};
+  a.q = bf16(q);
+  a.q_ld = q.stride(0);
+  a.q_head = q.stride(1);
+  a.k = bf16(k_pages);
+  a.v = bf16(v_pages);
+  a.page_ld = k_pages.stride(0);
+  a.token_ld = k_pages.stride(1);
+  a.head_ld = k_pages.stride(2);
+  a.pages = static_cast<int>(pages);
+  a.page_shift = __builtin_ctzll(static_cast<uint64_t>(page));
+  a.prefix_pages = prefix_pages.data_ptr<int>();
+  a.prefix_len = static_cast<int>(prefix_len);
+  a.page_table = page_table.data_ptr<int>();
+  a.table_ld = page_table.stride(0);
+  a.seq_lens = seq_lens.data_ptr<int>();
+  a.q_offsets = q_offsets ? q_offsets->data_ptr<int>() : nullptr;
+  a.n = static_cast<int>(N);
+  a.batch = static_cast<int>(B);
+  a.kv_heads = static_cast<int>(Hk);
+  a.heads = static_cast<int>(H);
+  a.group = static_cast<int>(H / Hk);
+  a.max_q = static_cast<int>(std::min(max_q_len, N));
+  a.max_len = static_cast<int>(max_seq_len);
+  a.scale_log2 = static_cast<float>(scale * kLog2e);
+  a.status = status.data_ptr<int>();
+  a.o = bf16(o);
+  a.lse = lse ? lse->data_ptr<float>() : nullptr;
+  const int64_t pieces = prefix::plan(a), rows = N * H;
+  TORCH_CHECK_VALUE(B * a.own_tiles * a.own_splits * Hk < (1ll << 31), "too many sequences times max_q_len");
+  torch::Tensor part;
+  if (pieces > 0) {
+    part = torch::empty({pieces * rows * (D + 2)}, q.options().dtype(at::kFloat));
+    a.part_o = part.data_ptr<float>();
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + pieces * rows * D);
+  }
+  C10_CUDA_CHECK(prefix::launch_attention(a, static_cast<int>(D), at::cuda::getCurrentCUDAStream()));
+  return {o, lse};
+}
+
+}  // namespace mnb

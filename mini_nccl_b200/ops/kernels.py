@@ -66,14 +66,21 @@ def fold_accumulator(device: torch.device, n: int) -> torch.Tensor:
     return buf
 
 
+#: Status codes of the page operations and the paged attention (csrc/cuda/common.cuh).
+_CACHE_STATUS = {4: "the key / value cache's pool has too few free pages",
+                 5: "a page, slot, position or length outside its tensor"}
+
+
 def check_status(device: torch.device | None = None) -> None:
-    """Raise if a GEMM pipeline wait ran out of budget (device sync)."""
+    """Raise if a GEMM pipeline wait ran out of budget, or a cache operation left a request out (device sync)."""
     for idx, st in _STATUS.items():
         if device is not None and device.index not in (None, idx):
             continue
         v = int(st[0].item())
         if v:
             st.zero_()
+            if v in _CACHE_STATUS:
+                raise RuntimeError(f"cache operation on cuda:{idx}: {_CACHE_STATUS[v]}")
             raise RuntimeError(f"GEMM kernel on cuda:{idx} reported pipeline status {v}")
 
 

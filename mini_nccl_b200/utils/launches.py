@@ -30,6 +30,14 @@ KERNELS_PER_CALL = {
     "flash_attn_fwd_tc": 1,
     "flash_attn_bwd": 3,
     "flash_attn_bwd_tc": 3,
+    "copy_pages": 1,
+    "fork_sequences": 2,
+    "reserve_pages": 1,
+    "free_sequences": 1,
+    "compact_pages": 3,
+    "append_kv": 1,
+    "sample": 1,
+    "shared_prefix_attention": 3,
     "all_reduce": 1,
     "reduce_scatter": 1,
     "move": 1,
