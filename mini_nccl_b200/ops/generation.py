@@ -167,8 +167,8 @@ def sample(
     Order a row by logit, equal logits by index.  ``top_k`` keeps the first k
     tokens (0, or a k of at least the vocabulary: all); ``top_p`` those before
     which less than p of the remaining probability lies (1 or more: all; the
-    first token always stays); ``min_p`` those with at least ``min_p`` times
-    the first one's probability.  The token with the largest
+    first token always stays); ``min_p`` (at most 1) those with at least
+    ``min_p`` times the first one's probability.  The token with the largest
     ``logit / temperature + noise`` among what is left is returned, of equals
     the one with the lowest index: with ``noise`` from the standard Gumbel
     distribution, fp32 ``[rows, vocabulary]``, that is a draw from the
@@ -203,7 +203,7 @@ def sample(
         return torch.full((R, 1), x, dtype=dtype)
 
     T, k = column(temperature, torch.float32, "temperature"), column(top_k, torch.int32, "top_k")
-    p, least = column(top_p, torch.float32, "top_p"), column(min_p, torch.float32, "min_p")
+    p, least = column(top_p, torch.float32, "top_p"), column(min_p, torch.float32, "min_p").clamp(max=1)
     x = logits.float()
     x = torch.where(x.isnan(), -math.inf, x)
     xs, order = torch.sort(x, dim=-1, descending=True, stable=True)
@@ -216,7 +216,7 @@ def sample(
     w = torch.where(left, torch.exp(delta), 0.0)
     before = torch.cumsum(w, -1) - w
     keep = left & ((p >= 1) | (before < p * w.sum(-1, keepdim=True))) & (w >= least)
-    keep |= (rank == 0) & (top > -math.inf)
+    keep |= left & (rank == 0)
     total = torch.where(keep, w, 0.0).sum(-1)
     kept = torch.zeros_like(keep).scatter_(1, order, keep)
     score = torch.where(kept, x / heat + noise, -math.inf)
