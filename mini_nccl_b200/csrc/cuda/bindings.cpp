@@ -53,7 +53,7 @@ void append_kv(torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor k, to
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>> sample(
     torch::Tensor logits, torch::Tensor noise, c10::optional<torch::Tensor> temperature, double temperature_all,
     c10::optional<torch::Tensor> top_k, int64_t top_k_all, c10::optional<torch::Tensor> top_p, double top_p_all,
-    c10::optional<torch::Tensor> min_p, double min_p_all, bool return_logprob);
+    c10::optional<torch::Tensor> min_p, double min_p_all, bool return_logprob, torch::Tensor status);
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(
     torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor prefix_pages, int64_t prefix_len,
     torch::Tensor page_table, torch::Tensor seq_lens, c10::optional<torch::Tensor> q_offsets, int64_t max_q_len,

@@ -211,7 +211,7 @@ void append_kv(torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor k, to
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>> sample(
     torch::Tensor logits, torch::Tensor noise, c10::optional<torch::Tensor> temperature, double temperature_all,
     c10::optional<torch::Tensor> top_k, int64_t top_k_all, c10::optional<torch::Tensor> top_p, double top_p_all,
-    c10::optional<torch::Tensor> min_p, double min_p_all, bool return_logprob) {
+    c10::optional<torch::Tensor> min_p, double min_p_all, bool return_logprob, torch::Tensor status) {
   using sampling::Setting;
   TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() == 2 &&
                         (logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kFloat),
@@ -223,7 +223,9 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> sample(
                         (noise.stride(1) == 1 || V == 1),
                     "noise: an fp32 tensor of the logits' shape, last axis contiguous");
   TORCH_CHECK_VALUE(R < (1ll << 31), "too many rows");
+  check_status_word(status);
   sampling::Sample a{};
+  a.status = status.data_ptr<int>();
   a.temperature = setting<Setting>(temperature, temperature_all, R, at::kFloat, logits, "temperature");
   a.top_k = setting<sampling::WholeSetting>(top_k, static_cast<double>(std::clamp<int64_t>(top_k_all, 0, V)), R, at::kInt,
                                             logits, "top_k");

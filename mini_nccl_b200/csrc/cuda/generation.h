@@ -79,6 +79,7 @@ struct Sample {
   Setting top_p, min_p;
   long long* token;
   float* logprob;  // or null
+  int* status;
 };
 
 cudaError_t launch_sample(const Sample& a, cudaStream_t stream);

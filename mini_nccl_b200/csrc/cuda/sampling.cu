@@ -8,9 +8,10 @@
 // p times the weight of the first k; min-p those with w_i >= min_p.  So a
 // row is described by one cut, the last (logit, index) pair that stays.
 //
-// One block of 512 threads per row, two or three blocks per SM so that one
-// row's loads run under another's arithmetic; every pass reads the row in
-// 16-byte pieces, after the first one from L2.  No pass sorts the row:
+// A cluster of 1 to 8 blocks of 256 threads takes a row.  Each block brings
+// its slice of the row into shared memory once, by bulk copies, and the passes
+// below read it there; block results meet through distributed shared memory.
+// No pass sorts the row:
 //   - pass 1 finds the maximum.  Greedy rows end there.
 //   - rows without top-k and top-p need one more pass (sum and best score).
 //   - a small top-k takes the k-th largest of the threads' own maxima as a
@@ -24,7 +25,11 @@
 //   - what is left (thousands of equal logits at the cut, infinite logits) is
 //     found by bisection over the pairs, slowly.
 // Weights and sums are fp32, in a fixed order, so results do not depend on
-// scheduling; the scores are IEEE fp32 division and addition.
+// scheduling; the winning score is IEEE fp32 division and addition.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
 #include "common.cuh"
 #include "generation.h"
 
@@ -32,11 +37,18 @@ namespace mnb {
 
 namespace sampling {
 
-constexpr int kThreads = 512;
+namespace cg = cooperative_groups;
+
+constexpr int kMaxCluster = 8;
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kList = 1024;        // tokens a list can hold
-constexpr int kSmallK = 384;       // top-k by the threads' maxima: 3/4 of the threads bound about 1.4 x 512 tokens
+constexpr int kPlaces = kList / kThreads;
+constexpr int kSmallK = 3 * kThreads / 4;  // top-k by the threads' maxima: those of one block bound about 1.4 x 256 tokens
+constexpr int kMostK = 600;                // 2048 maxima bound about 700 tokens then, which a list holds
+constexpr int kChunk = 4 * kThreads;       // pieces of 16 bytes per bulk copy
+constexpr int kChunks = 8;
 constexpr float kRange = 36.f;     // bins cover weights down to 2^-36 of the largest
 constexpr int kLevels = 3;         // times a band is divided
 constexpr uint32_t kIndexMask = (1u << kIndexBits) - 1;
@@ -56,6 +68,11 @@ MNB_DEVICE uint64_t pair_of(uint32_t key, int i) {
 MNB_DEVICE int index_of(uint64_t pair) { return static_cast<int>(kIndexMask - (static_cast<uint32_t>(pair) & kIndexMask)); }
 MNB_DEVICE float logit_of(uint64_t pair) { return value_of(static_cast<uint32_t>(pair >> kIndexBits)); }
 
+template <bool B>
+struct Flag {
+  static constexpr bool value = B;
+};
+
 // One value for all rows, or one for each.
 template <typename S>
 MNB_DEVICE auto at(const S& s, int r) {
@@ -68,11 +85,25 @@ struct Shared {
     float f32[kWarps];
     int i32[kWarps];
   } red;
-  int n_list;
+  // one value of every block of the cluster, in turn in two places
+  union {
+    uint64_t u64[kMaxCluster];
+    float f32[kMaxCluster];
+    int i32[kMaxCluster];
+  } from[2];
+  uint64_t arrived[kChunks];  // mbarriers of the bulk copies
+  int n_mine;
   int bin_from, bin_to, bin_count;
   uint64_t cut;
-  int hist[kBins];
-  uint64_t list[kList];
+  uint64_t mine[kList];  // this block's part of the list
+  union {
+    float maxima[kMaxCluster][kThreads];
+    struct {
+      int bins[kBins];      // this block's counts
+      int hist[kBins];      // the cluster's
+    };
+    uint64_t list[kList];   // the cluster's list
+  };
 };
 
 template <typename V, typename F>
@@ -87,17 +118,63 @@ MNB_DEVICE V block_reduce(V v, V* sh, F f) {
   __syncthreads();
   return s;
 }
+// The same over the cluster: every block sends its value to all, and joins what it got in the blocks' order.
+struct Team {
+  Shared& sh;
+  int size, rank;
+  int phase = 0;
+  MNB_DEVICE void sync() const {
+    if (size > 1) cg::this_cluster().sync();
+    else __syncthreads();
+  }
+  template <typename T>
+  MNB_DEVICE T* peer(T* p, int q) const {
+    return size > 1 ? cg::this_cluster().map_shared_rank(p, q) : p;
+  }
+  template <typename V, typename F>
+  MNB_DEVICE V join(V v, V* red, V* from, F f) {
+    v = block_reduce(v, red, f);
+    if (size == 1) return v;
+    if (threadIdx.x < size) *peer(from + rank, threadIdx.x) = v;
+    sync();
+    V s = from[0];
+    for (int q = 1; q < size; ++q) s = f(s, from[q]);
+    phase ^= 1;
+    return s;
+  }
+  MNB_DEVICE float sum(float v) {
+    return join(v, sh.red.f32, sh.from[phase].f32, [](float a, float b) { return a + b; });
+  }
+  MNB_DEVICE int sum(int v) {
+    return join(v, sh.red.i32, sh.from[phase].i32, [](int a, int b) { return a + b; });
+  }
+  MNB_DEVICE float max(float v) {
+    return join(v, sh.red.f32, sh.from[phase].f32, [](float a, float b) { return fmaxf(a, b); });
+  }
+  MNB_DEVICE uint64_t max(uint64_t v) {
+    return join(v, sh.red.u64, sh.from[phase].u64, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+  }
+  // The blocks' lists into everybody's `list`; returns the length, more than kList if they do not fit.
+  // The next change of `mine` has to lie behind another exchange.
+  MNB_DEVICE int gather_list() {
+    sync();
+    int n = 0;
+    for (int q = 0; q < size; ++q) {
+      const int m = *peer(&sh.n_mine, q);
+      const uint64_t* from = peer(sh.mine, q);
+      if (n + m <= kList)
+        for (int i = threadIdx.x; i < m; i += kThreads) sh.list[n + i] = from[i];
+      n += m;
+    }
+    __syncthreads();
+    return n;
+  }
+};
 MNB_DEVICE float block_sum(float v, Shared& sh) {
   return block_reduce(v, sh.red.f32, [](float a, float b) { return a + b; });
 }
 MNB_DEVICE int block_sum(int v, Shared& sh) {
   return block_reduce(v, sh.red.i32, [](int a, int b) { return a + b; });
-}
-MNB_DEVICE float block_max(float v, Shared& sh) {
-  return block_reduce(v, sh.red.f32, [](float a, float b) { return fmaxf(a, b); });
-}
-MNB_DEVICE uint64_t block_max(uint64_t v, Shared& sh) {
-  return block_reduce(v, sh.red.u64, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
 }
 // Sum over the threads before this one.
 template <typename V>
@@ -117,56 +194,124 @@ MNB_DEVICE V block_before(V v, V* sh) {
   return base + (x - v);
 }
 
-// A row read in 16-byte pieces.  The first and last piece may reach past the
-// row; elements outside it read as NaN, which no filter keeps.
-template <typename T>
-struct Row {
-  static constexpr int kVec = 16 / sizeof(T);
-  const T* x;
-  int V, lead, pieces;
-  MNB_DEVICE Row(const T* p, int n) : x(p), V(n) {
-    lead = static_cast<int>(reinterpret_cast<uintptr_t>(p) % 16 / sizeof(T));
-    pieces = (n + lead + kVec - 1) / kVec;
-  }
-  MNB_DEVICE float one(int i) const;
-  MNB_DEVICE void piece(int c, float* v) const {
-    const int i0 = c * kVec - lead;
-    if (i0 >= 0 && i0 + kVec <= V) {
-      const uint4 w = *reinterpret_cast<const uint4*>(x + i0);
-      unpack(w, v);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) v[j] = i0 + j >= 0 && i0 + j < V ? one(i0 + j) : __uint_as_float(0x7fc00000u);
-    }
-  }
-  MNB_DEVICE static void unpack(uint4 w, float* v);
-  // f(values, index of the first) over the thread's pieces
-  template <typename F>
-  MNB_DEVICE void scan(F f) const {
-#pragma unroll 2
-    for (int c = threadIdx.x; c < pieces; c += kThreads) {
-      float v[kVec];
-      piece(c, v);
-      f(v, c * kVec - lead);
-    }
-  }
-};
-template <>
-MNB_DEVICE float Row<float>::one(int i) const { return x[i]; }
-template <>
-MNB_DEVICE float Row<__nv_bfloat16>::one(int i) const { return bf16_to_f32(x[i]); }
-template <>
-MNB_DEVICE void Row<float>::unpack(uint4 w, float* v) {
+MNB_DEVICE float to_float(float v) { return v; }
+MNB_DEVICE float to_float(__nv_bfloat16 v) { return bf16_to_f32(v); }
+MNB_DEVICE void unpack_piece(uint4 w, float (&v)[4]) {
   v[0] = __uint_as_float(w.x), v[1] = __uint_as_float(w.y), v[2] = __uint_as_float(w.z), v[3] = __uint_as_float(w.w);
 }
-template <>
-MNB_DEVICE void Row<__nv_bfloat16>::unpack(uint4 w, float* v) {
+MNB_DEVICE void unpack_piece(uint4 w, float (&v)[8]) {
   const uint32_t a[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     v[2 * j] = __uint_as_float(a[j] << 16);
     v[2 * j + 1] = __uint_as_float(a[j] & 0xffff0000u);
   }
+}
+MNB_DEVICE float widest_of(uint4 w, float m, float) {
+  return max3f(max3f(__uint_as_float(w.x), __uint_as_float(w.y), m), __uint_as_float(w.z), __uint_as_float(w.w));
+}
+MNB_DEVICE float widest_of(uint4 w, float m, __nv_bfloat16) {
+  auto pair = [](uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); };
+  const __nv_bfloat162 a = __hmax2(__hmax2(pair(w.x), pair(w.y)), __hmax2(pair(w.z), pair(w.w)));
+  return max3f(m, __low2float(a), __high2float(a));
+}
+MNB_DEVICE uint4 pack_piece(const float* x, int i0, int V) {
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = i0 + j >= 0 && i0 + j < V ? __float_as_uint(x[i0 + j]) : 0x7fc00000u;
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+MNB_DEVICE uint4 pack_piece(const __nv_bfloat16* x, int i0, int V) {
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int i = i0 + 2 * j;
+    const uint32_t lo = i >= 0 && i < V ? __bfloat16_as_ushort(x[i]) : 0x7fc0u;
+    const uint32_t hi = i + 1 >= 0 && i + 1 < V ? __bfloat16_as_ushort(x[i + 1]) : 0x7fc0u;
+    w[j] = lo | hi << 16;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// This block's slice of a row, in 16-byte pieces.  The row's first and last
+// piece may reach past it; elements outside read as NaN, which no filter keeps.
+template <typename T, bool Staged>
+struct Row {
+  static constexpr int kVec = 16 / sizeof(T);
+  const T* x;
+  int V, lead;
+  int first, count;  // pieces
+  uint4* slice;      // in shared memory, if Staged; otherwise every pass reads global memory (L2)
+  MNB_DEVICE Row(const T* p, int n, int rank, int size, uint4* smem) : x(p), V(n), slice(smem) {
+    lead = static_cast<int>(reinterpret_cast<uintptr_t>(p) % 16 / sizeof(T));
+    const int all = (n + lead + kVec - 1) / kVec, per = (all + size - 1) / size;
+    first = min(all, rank * per);
+    count = min(all - first, per);
+  }
+  MNB_DEVICE int start(int c) const { return (first + c) * kVec - lead; }  // element of piece c
+  MNB_DEVICE bool whole(int c) const { return start(c) >= 0 && start(c) + kVec <= V; }
+  // One thread starts the copies of the whole pieces; the thread that reads a row's edge fills it in.
+  MNB_DEVICE void stage(uint64_t* arrived) const {
+    if (!Staged || count == 0) return;
+    const int from = whole(0) ? 0 : 1, to = whole(count - 1) ? count : count - 1;
+    if (threadIdx.x == 0)
+      for (int j = 0; j * kChunk < count; ++j) {
+        const int a = max(j * kChunk, from), b = min((j + 1) * kChunk, to);
+        const uint32_t bar = smem_u32(arrived + j), bytes = a < b ? static_cast<uint32_t>(b - a) * 16 : 0;
+        mbar_arrive_expect_tx(bar, bytes);
+        if (bytes) bulk_load(smem_u32(slice + a), x + start(a), bytes, bar);
+      }
+    if (from == 1 && threadIdx.x == 0) slice[0] = edge(start(0));
+    if (to < count && count > from && (count - 1) % kThreads == threadIdx.x) slice[count - 1] = edge(start(count - 1));
+  }
+  MNB_DEVICE static void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(bar)
+                 : "memory");
+  }
+  MNB_DEVICE uint4 piece(int c) const {
+    if (Staged) return slice[c];
+    return whole(c) ? *reinterpret_cast<const uint4*>(x + start(c)) : edge(start(c));
+  }
+  MNB_DEVICE float one(int i) const { return to_float(x[i]); }
+  // the largest of m and the piece's elements (NaN does not count)
+  MNB_DEVICE static float widest(uint4 w, float m) { return widest_of(w, m, T{}); }
+  // a piece that reaches past the row
+  MNB_DEVICE uint4 edge(int i0) const { return pack_piece(x, i0, V); }
+  // f(values, index of the first) over the thread's pieces
+  template <typename F>
+  MNB_DEVICE void scan(F f) const {
+#pragma unroll 2
+    for (int c = threadIdx.x; c < count; c += kThreads) {
+      float v[kVec];
+      unpack_piece(piece(c), v);
+      f(v, start(c));
+    }
+  }
+  // the same over the pieces with an element of at least `least`
+  template <typename F>
+  MNB_DEVICE void scan_from(float least, F f) const {
+#pragma unroll 4
+    for (int c = threadIdx.x; c < count; c += kThreads) {
+      const uint4 w = piece(c);
+      if (!(widest(w, -INFINITY) >= least)) continue;
+      float v[kVec];
+      unpack_piece(w, v);
+      f(v, start(c));
+    }
+  }
+};
+// v / t, rounded as IEEE division rounds it, from the reciprocal inv_t = 1 / t (itself rounded to nearest): two
+// steps q += (v - q t) inv_t with the remainder exact by fused multiply-add, after which the quotient is the correctly
+// rounded one (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", 1990).  Where
+// a step could overflow, underflow or meet an infinity the division itself is called.
+MNB_DEVICE float divide(float v, float t, float inv_t) {
+  float q = v * inv_t;
+  q = fmaf(fmaf(-q, t, v), inv_t, q);
+  q = fmaf(fmaf(-q, t, v), inv_t, q);
+  const float m = fabsf(q);
+  if (!(m > 1e-25f && m < 1e25f)) q = __fdiv_rn(v, t);
+  return q;
 }
 
 // The best score so far of the tokens that a thread has seen.
@@ -175,12 +320,20 @@ struct Best {
   int index = -1;
   const float* noise;
   MNB_DEVICE void see(float v, float g, int i) {
-    // the division is only needed where the product, good to 2^-22 of either term, comes near the best
-    const float a = v * inv_t;
-    if (index >= 0 && a + g < score - 1e-6f * (fabsf(a) + fabsf(g))) return;
-    float s = __fadd_rn(__fdiv_rn(v, t), g);
-    if (s != s) s = -INFINITY;
-    if (index < 0 || s > score || (s == score && i < index)) score = s, index = i;
+    float s = __fadd_rn(divide(v, t, inv_t), g);
+    s = s != s ? -INFINITY : s;
+    const bool better = s > score || index < 0 || (s == score && i < index);
+    score = better ? s : score;
+    index = better ? i : index;
+  }
+  // The same for v * inv_t + g: the best and the second best, for a thread's own ranking.
+  float near_score = -INFINITY, near_second = -INFINITY, near_v = 0.f, near_g = 0.f;
+  int near_index = -1;
+  MNB_DEVICE void see_nearly(bool counts, float v, float g, int i) {
+    const float s = counts ? fmaf(v, inv_t, g) : -INFINITY;
+    near_second = fmaxf(near_second, fminf(near_score, s));
+    if (s > near_score) near_v = v, near_g = g, near_index = i;
+    near_score = fmaxf(near_score, s);
   }
   MNB_DEVICE uint64_t pair() const { return index < 0 ? 0 : pair_of(key_of(score), index); }
 };
@@ -195,8 +348,8 @@ MNB_DEVICE int sort_list(Shared& sh, int n) {
   if (!one_warp || threadIdx.x < 32) {
     for (int size = 2; size <= n2; size <<= 1)
       for (int stride = size / 2; stride > 0; stride >>= 1) {
-        if (threadIdx.x < n2 / 2) {
-          const int i = 2 * threadIdx.x - (threadIdx.x & (stride - 1)), j = i + stride;
+        for (int t = threadIdx.x; t < n2 / 2; t += one_warp ? 32 : kThreads) {
+          const int i = 2 * t - (t & (stride - 1)), j = i + stride;
           const uint64_t a = sh.list[i], b = sh.list[j];
           if ((a < b) == ((i & size) == 0)) sh.list[i] = b, sh.list[j] = a;
         }
@@ -209,16 +362,16 @@ MNB_DEVICE int sort_list(Shared& sh, int n) {
 }
 
 // Bisection over the pairs: right for every row, some 50 passes.
-template <typename T>
-__device__ __noinline__ uint64_t slow_cut(const Row<T>& row, float mx, float scale, int k, float p, Shared& sh) {
+template <typename T, bool Staged>
+__device__ __noinline__ uint64_t slow_cut(const Row<T, Staged>& row, float mx, float scale, int k, float p, Team& team) {
   auto weight = [&](float v) { return v == mx ? 1.f : ex2_approx((v - mx) * scale); };  // an infinite maximum takes all
   uint64_t best = 0;
   row.scan([&](const float* v, int i0) {
 #pragma unroll
-    for (int j = 0; j < Row<T>::kVec; ++j)
+    for (int j = 0; j < Row<T, Staged>::kVec; ++j)
       if (v[j] == mx) best = max(best, pair_of(key_of(v[j]), i0 + j));
   });
-  best = block_max(best, sh);
+  best = team.max(best);
   uint64_t cut = static_cast<uint64_t>(kKeyNegInf + 1) << kIndexBits;
   if (k > 0 && k < row.V) {
     uint64_t lo = cut, hi = best;  // smallest pair with fewer than k before it
@@ -227,9 +380,9 @@ __device__ __noinline__ uint64_t slow_cut(const Row<T>& row, float mx, float sca
       int n = 0;
       row.scan([&](const float* v, int i0) {
 #pragma unroll
-        for (int j = 0; j < Row<T>::kVec; ++j) n += v[j] == v[j] && pair_of(key_of(v[j]), i0 + j) > mid;
+        for (int j = 0; j < Row<T, Staged>::kVec; ++j) n += v[j] == v[j] && pair_of(key_of(v[j]), i0 + j) > mid;
       });
-      if (block_sum(n, sh) < k) hi = mid;
+      if (team.sum(n) < k) hi = mid;
       else lo = mid + 1;
     }
     cut = lo;
@@ -239,10 +392,10 @@ __device__ __noinline__ uint64_t slow_cut(const Row<T>& row, float mx, float sca
       float s = 0.f;
       row.scan([&](const float* v, int i0) {
 #pragma unroll
-        for (int j = 0; j < Row<T>::kVec; ++j)
+        for (int j = 0; j < Row<T, Staged>::kVec; ++j)
           if (v[j] == v[j] && pair_of(key_of(v[j]), i0 + j) > from) s += weight(v[j]);
       });
-      return block_sum(s, sh);
+      return team.sum(s);
     };
     const float limit = p * mass(cut - 1);
     uint64_t lo = cut, hi = best;  // smallest pair with less than the limit before it
@@ -256,19 +409,34 @@ __device__ __noinline__ uint64_t slow_cut(const Row<T>& row, float mx, float sca
   return cut;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ Sample a) {
-  constexpr int kVec = Row<T>::kVec;
+template <typename T, bool Staged>
+__global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_constant__ Sample a, int cluster) {
+  using R = Row<T, Staged>;
+  constexpr int kVec = R::kVec;
+  extern __shared__ uint4 slice[];
   __shared__ Shared sh;
-  const int r = blockIdx.x, tid = threadIdx.x;
-  const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.vocab);
+  const int r = blockIdx.x / cluster, tid = threadIdx.x;
+  Team team{sh, cluster, static_cast<int>(blockIdx.x) % cluster};
+  if (cluster > 1) cg::this_cluster().barrier_arrive();  // a block's shared memory is there once the block runs
+  const R row(static_cast<const T*>(a.logits) + r * a.ld, a.vocab, team.rank, cluster, slice);
+  if (Staged) {
+    if (tid == 0) {
+      for (int j = 0; j < kChunks; ++j) mbar_init(smem_u32(sh.arrived + j), 1);
+      fence_mbar_init();
+    }
+    __syncthreads();
+    row.stage(sh.arrived);
+  }
 
   float mine = -INFINITY;
-  row.scan([&](const float* v, int) {
+  for (int c = tid, j = 0; c < row.count; ++j) {  // a chunk holds four of a thread's pieces
+    if (Staged && !mbar_wait(smem_u32(sh.arrived + j), 0, a.status)) break;
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) mine = fmaxf(mine, v[j]);
-  });
-  const float mx = block_max(mine, sh);
+    for (int e = 0; e < kChunk / kThreads; ++e, c += kThreads)
+      if (c < row.count) mine = R::widest(row.piece(c), mine);
+  }
+  if (cluster > 1) cg::this_cluster().barrier_wait();
+  const float mx = team.max(mine);
   const float t = at(a.temperature, r);
   if (mx == -INFINITY || !(t > 0.f)) {  // no token left, or the first one
     uint64_t first = 0;
@@ -278,8 +446,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         for (int j = 0; j < kVec; ++j)
           if (v[j] == mx) first = max(first, pair_of(1, i0 + j));
       });
-    first = block_max(first, sh);
-    if (tid == 0) {
+    first = team.max(first);
+    if (tid == 0 && team.rank == 0) {
       a.token[r] = first ? index_of(first) : -1;
       if (a.logprob) a.logprob[r] = first ? 0.f : -INFINITY;
     }
@@ -294,28 +462,28 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   best.noise = a.noise + r * a.noise_ld;
   float z = 0.f;  // weight of the kept tokens that this thread has seen
 
-  // Keeps the elements of a piece that `kept` accepts and that pass min-p.
+  // The noise of the elements of a piece whose weight w[j] is not negative.
   const bool noise_vec = (reinterpret_cast<uintptr_t>(best.noise - row.lead) & 15) == 0;
-  auto keep = [&](const float* v, int i0, auto kept) {
-    float w[kVec];
-    bool any = false;
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) {
-      w[j] = -1.f;
-      if (kept(v[j], i0 + j)) {
-        const float x = v[j] == mx ? 1.f : ex2_approx((v[j] - mx) * scale);
-        if (x >= least) w[j] = x, any = true;
-      }
-    }
-    if (!any) return;
-    float g[kVec];
+  auto fetch = [&](float* g, const float* w, int i0) {
     if (noise_vec && i0 >= 0 && i0 + kVec <= a.vocab) {
 #pragma unroll
-      for (int j = 0; j < kVec; j += 4) *reinterpret_cast<float4*>(g + j) = *reinterpret_cast<const float4*>(best.noise + i0 + j);
+      for (int j = 0; j < kVec; j += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(best.noise + i0 + j);
+        g[j] = f.x, g[j + 1] = f.y, g[j + 2] = f.z, g[j + 3] = f.w;
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < kVec; ++j) g[j] = w[j] >= 0.f ? best.noise[i0 + j] : 0.f;
     }
+  };
+  // Scores those elements.
+  auto score = [&](const float* v, const float* w, int i0) {
+    bool any = false;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) any |= w[j] >= 0.f;
+    if (!any) return;
+    float g[kVec];
+    fetch(g, w, i0);
 #pragma unroll
     for (int j = 0; j < kVec; ++j)
       if (w[j] >= 0.f) {
@@ -323,10 +491,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         best.see(v[j], g[j], i0 + j);
       }
   };
+  // Keeps the elements of a piece that `kept` accepts and that pass min-p.
+  auto keep = [&](const float* v, int i0, auto kept) {
+    float w[kVec];
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      const float x = v[j] == mx ? 1.f : ex2_approx((v[j] - mx) * scale);
+      w[j] = kept(v[j], i0 + j) && x >= least ? x : -1.f;
+    }
+    score(v, w, i0);
+  };
   auto finish = [&]() {
-    const uint64_t chosen = block_max(best.pair(), sh);
-    const float total = block_sum(z, sh);
-    if (tid == 0) {
+    const uint64_t chosen = team.max(best.pair());
+    const float total = team.sum(z);
+    if (tid == 0 && team.rank == 0) {
       const int i = index_of(chosen);
       a.token[r] = i;
       if (a.logprob) {
@@ -338,7 +516,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 
   const bool cut_by_mass = p < 1.f;
   if (!k && !cut_by_mass) {
-    row.scan([&](const float* v, int i0) { keep(v, i0, [&](float x, int) { return x > -INFINITY; }); });
+    // what min-p drops is far enough below this bound to be skipped by the piece
+    const float bound = least > 0.f ? mx - (0.01f - 1.0001f * log2f(least)) / scale : -3.402823466e38f;
+    row.scan_from(mx < INFINITY && scale < 1e30f ? bound : -3.402823466e38f, [&](const float* v, int i0) {
+      keep(v, i0, [&](float x, int) { return x > -INFINITY; });
+    });
     finish();
     return;
   }
@@ -346,15 +528,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   uint64_t cut = static_cast<uint64_t>(kKeyNegInf + 1) << kIndexBits;
   bool settled = false;
   if (mx < INFINITY && scale < 1e30f) {
-    if (k && (k <= kSmallK || a.vocab <= kList)) {
+    if (k && (k <= min(kSmallK * cluster, kMostK) || a.vocab <= kList)) {
       // the bound: the k-th largest of the threads' maxima, or a little less
       uint32_t lo = kKeyNegInf + 1;
       if (a.vocab > kList) {
-        const uint32_t key = key_of(mine);
+        // every block gets all the maxima, so the search needs no further exchange
+        for (int q = 0; q < cluster; ++q) team.peer(&sh.maxima[team.rank][tid], q)[0] = mine;
+        team.sync();
+        uint32_t key[kMaxCluster];
+#pragma unroll
+        for (int q = 0; q < kMaxCluster; ++q) key[q] = q < cluster ? key_of(sh.maxima[q][tid]) : 0u;
         uint32_t hi = key_of(mx);
         while (lo < hi) {  // the largest bound that at least k maxima reach
           const uint32_t mid = lo + (hi - lo + 1) / 2;
-          const int n = __syncthreads_count(key >= mid);
+          int n = 0;
+#pragma unroll
+          for (int q = 0; q < kMaxCluster; ++q)
+            if (q < cluster) n += __syncthreads_count(key[q] >= mid);
           if (n >= k) {
             lo = mid;
             if (n <= k + k / 8) break;
@@ -364,27 +554,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         }
       }
       const float bound = value_of(lo);
-      if (tid == 0) sh.n_list = 0;
+      if (tid == 0) sh.n_mine = 0;
       __syncthreads();
-      row.scan([&](const float* v, int i0) {
+      row.scan_from(bound, [&](const float* v, int i0) {
 #pragma unroll
         for (int j = 0; j < kVec; ++j)
           if (v[j] >= bound) {
-            const int n = atomicAdd(&sh.n_list, 1);
-            if (n < kList) sh.list[n] = pair_of(key_of(v[j]), i0 + j);
+            const int n = atomicAdd(&sh.n_mine, 1);
+            if (n < kList) sh.mine[n] = pair_of(key_of(v[j]), i0 + j);
           }
       });
-      __syncthreads();
-      const int n = sh.n_list;
+      const int n = team.gather_list();
       if (n <= kList) {
         sort_list(sh, n);
         const int have = min(n, k);
-        // two neighbouring places per thread
-        float w[2], sum = 0.f;
-        uint64_t pair[2];
+        // neighbouring places per thread
+        float w[kPlaces], sum = 0.f;
+        uint64_t pair[kPlaces];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int i = 2 * tid + e;
+        for (int e = 0; e < kPlaces; ++e) {
+          const int i = kPlaces * tid + e;
           pair[e] = i < have ? sh.list[i] : 0;
           const float v = logit_of(pair[e]);
           w[e] = i < have ? (v == mx ? 1.f : ex2_approx((v - mx) * scale)) : 0.f;
@@ -393,9 +582,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         float before = block_before(sum, sh.red.f32);
         const float limit = cut_by_mass ? p * block_sum(sum, sh) : INFINITY;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int i = 2 * tid + e;
-          if (i < have && (i == 0 || before < limit) && w[e] >= least) {
+        for (int e = 0; e < kPlaces; ++e) {
+          const int i = kPlaces * tid + e;
+          if (team.rank == 0 && i < have && (i == 0 || before < limit) && w[e] >= least) {
             z += w[e];
             best.see(logit_of(pair[e]), best.noise[index_of(pair[e])], index_of(pair[e]));
           }
@@ -406,6 +595,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       }
     }
     // Count and mass bands: first the cut of top-k (if any), then that of top-p.
+    using Yes = Flag<true>;
+    using No = Flag<false>;
     bool ok = true;
     float limit = 0.f;
     for (int stage = k ? 0 : 1; stage < (cut_by_mass ? 2 : 1) && ok; ++stage) {
@@ -414,31 +605,42 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       float y0 = 0.f, y1 = kRange;
       ok = false;
       for (int level = 0; level < kLevels && !ok; ++level) {
-        for (int b = tid; b < kBins; b += kThreads) sh.hist[b] = 0;
+        if (level) team.sync();  // everybody has read the last level's counts
+        for (int b = tid; b < kBins; b += kThreads) sh.bins[b] = 0;
         __syncthreads();
         const float per = kBins / (y1 - y0);
         float mass = 0.f;  // level 0: of everything; later: of what lies above the band
         int above = 0;
-        row.scan([&](const float* v, int i0) {
+        // At first the last bin also takes what lies beyond the range, and NaN.
+        auto tally = [&](auto filter, auto masses, auto first) {
+          row.scan([&](const float* v, int i0) {
 #pragma unroll
-          for (int j = 0; j < kVec; ++j) {
-            const float y = (mx - v[j]) * scale;
-            if (filtered && !(v[j] > -INFINITY && pair_of(key_of(v[j]), i0 + j) >= cut)) continue;
-            if (level == 0) {
-              if (by_mass && v[j] > -INFINITY) mass += ex2_approx(-y);
-            } else if (y < y0) {
-              ++above;
-              if (by_mass) mass += ex2_approx(-y);
-            }
-            if (y >= y0 && y <= y1) {
+            for (int j = 0; j < kVec; ++j) {
+              const float y = (mx - v[j]) * scale;
+              if (filter.value && !(v[j] > -INFINITY && pair_of(key_of(v[j]), i0 + j) >= cut)) continue;
+              if (masses.value) {
+                const float w = ex2_approx(-y);
+                mass += (first.value ? y < INFINITY : y < y0) ? w : 0.f;
+              } else if (!first.value && y < y0) {
+                ++above;
+              }
               // adding 2^23 leaves the bin, rounded to the nearest, in the low bits
-              const float b = fminf(fmaxf((y - y0) * per, 0.f), kBins - 1.f) + 8388608.f;
-              atomicAdd(&sh.hist[__float_as_uint(b) & (kBins - 1)], 1);
+              const float b = fminf(first.value ? y * per : (y - y0) * per, kBins - 1.f) + 8388608.f;
+              if (first.value || (y >= y0 && y <= y1)) atomicAdd(&sh.bins[__float_as_uint(b) & (kBins - 1)], 1);
             }
-          }
-        });
-        mass = block_sum(mass, sh);
-        if (!by_mass && level) above = block_sum(above, sh);
+          });
+        };
+        if (filtered) level ? tally(Yes{}, Yes{}, No{}) : tally(Yes{}, Yes{}, Yes{});
+        else if (by_mass) level ? tally(No{}, Yes{}, No{}) : tally(No{}, Yes{}, Yes{});
+        else level ? tally(No{}, No{}, No{}) : tally(No{}, No{}, Yes{});
+        mass = team.sum(mass);
+        above = team.sum(above);  // (these exchanges also tell that every block's counts are there)
+        for (int b = tid; b < kBins; b += kThreads) {
+          int c = 0;
+          for (int q = 0; q < cluster; ++q) c += *team.peer(&sh.bins[b], q);
+          sh.hist[b] = c;
+        }
+        __syncthreads();
         if (by_mass && level == 0) limit = p * mass;
         // this thread's bins, in order
         constexpr int kPer = kBins / kThreads;
@@ -447,7 +649,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         float sum_hi = 0.f, sum_lo = 0.f;  // with every token at the bin's upper / lower weight
         const float step = 1.f / per;
         auto upper = [&](int b) { return ex2_approx(-(y0 + (b - 0.5f) * step)); };
-        auto lower = [&](int b) { return ex2_approx(-(y0 + (b + (b == kBins - 1 ? 1.f : 0.5f)) * step)); };
+        auto lower = [&](int b) {
+          return b < kBins - 1 ? ex2_approx(-(y0 + (b + 0.5f) * step)) : level ? ex2_approx(-(y0 + kBins * step)) : 0.f;
+        };
 #pragma unroll
         for (int e = 0; e < kPer; ++e) {
           const int b = tid * kPer + e;
@@ -468,9 +672,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           __syncthreads();
         } else {
           float hi = head + block_before(sum_hi, sh.red.f32), lo = head + block_before(sum_lo, sh.red.f32);
-          // from the other end too: behind a bin lie at most the upper weights of the later bins and of what no bin counts
+          // from the other end too: behind a bin lie at most the upper weights of the later bins
           const float all_hi = block_sum(sum_hi, sh);
-          float behind = level == 0 ? all_hi - (hi - head) + a.vocab * ex2_approx(-kRange) : INFINITY;
+          float behind = level == 0 ? all_hi - (hi - head) : INFINITY;
           const float all = level == 0 ? mass * (1.f - 2e-6f) : 0.f;
 #pragma unroll
           for (int e = 0; e < kPer; ++e) {
@@ -497,7 +701,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         }
         const int from = sh.bin_from, to = sh.bin_to, count = sh.bin_count;
         __syncthreads();
-        if (from >= kBins) break;  // the cut lies below the range
+        if (from >= kBins || (to == kBins - 1 && level == 0)) break;  // the cut may lie below the range
         const float wide = 1e-6f * (y0 + to * step) + 1e-6f * step;
         y1 = to == kBins - 1 ? y1 : y0 + (to + 0.5f) * step + wide;
         y0 = fmaxf(y0, y0 + (from - 0.5f) * step - wide);
@@ -505,45 +709,71 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       }
       if (!ok) break;
       // what lies above the band, and the band itself as a list
-      if (tid == 0) sh.n_list = 0;
+      if (tid == 0) sh.n_mine = 0;
       __syncthreads();
       float mass = 0.f;
       int above = 0;
-      auto inside = [&](float x, int i) {
-        return x > -INFINITY && !(filtered && pair_of(key_of(x), i) < cut);
-      };
-      row.scan([&](const float* v, int i0) {
-        bool any = false;
+      const float bound = mx - (y1 * 1.0001f + 0.01f) / scale;  // what lies below the band is skipped by the piece
+      const bool rough = last && !(least > 0.f);
+      auto split = [&](auto filter, auto roughly) {
+        row.scan_from(bound, [&](const float* v, int i0) {
+          float w[kVec];
+          bool any = false;
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) {
-          const float y = (mx - v[j]) * scale;
-          if (!(y <= y1) || !inside(v[j], i0 + j)) continue;
-          if (y < y0) {
-            any = true;
-            ++above;
-            if (cut_by_mass) mass += ex2_approx(-y);
-          } else {
-            const int n = atomicAdd(&sh.n_list, 1);
-            if (n < kList) sh.list[n] = pair_of(key_of(v[j]), i0 + j);
+          for (int j = 0; j < kVec; ++j) {
+            const float y = (mx - v[j]) * scale;
+            bool in = y <= y1;
+            if (filter.value) in = in && pair_of(key_of(v[j]), i0 + j) >= cut;
+            const bool over = in && y < y0;
+            const float x = ex2_approx(-y);
+            mass += over ? x : 0.f;
+            above += over;
+            w[j] = over && x >= least ? x : -1.f;
+            any |= over;
+            if (in && !over) {
+              const int n = atomicAdd(&sh.n_mine, 1);
+              if (n < kList) sh.mine[n] = pair_of(key_of(v[j]), i0 + j);
+            }
           }
+          if (!any || !last) return;
+          if (!roughly.value) return score(v, w, i0);
+          float g[kVec];
+          fetch(g, w, i0);
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) best.see_nearly(w[j] >= 0.f, v[j], g[j], i0 + j);
+        });
+      };
+      if (filtered) split(Yes{}, No{});
+      else if (rough) split(No{}, Yes{});
+      else split(No{}, No{});
+      if (rough && !filtered) {
+        // Scores by a product are off by less than this; whoever is that near the top is scored exactly, and if a
+        // thread's second best is too, all are.
+        const float top = team.max(best.near_score);
+        const float off = 1e-6f * (fabsf(mx * best.inv_t) + y1 + fabsf(top));
+        const bool unclear = best.near_second >= top - off || !(fabsf(top) < 1e30f);
+        if (team.sum(static_cast<int>(unclear))) {
+          row.scan_from(bound, [&](const float* v, int i0) {
+            keep(v, i0, [&](float x, int) { return (mx - x) * scale < y0; });
+          });
+        } else if (best.near_score >= top - off) {
+          best.see(best.near_v, best.near_g, best.near_index);
         }
-        if (last && any)
-          keep(v, i0, [&](float x, int i) { return (mx - x) * scale < y0 && inside(x, i); });
-      });
-      mass = block_sum(mass, sh);
-      above = block_sum(above, sh);
-      const int n = sh.n_list;
-      __syncthreads();
+        z = mass;
+      }
+      mass = team.sum(mass);
+      above = team.sum(above);
+      const int n = team.gather_list();
       if (n > kList) {
         ok = false;
         break;
       }
       sort_list(sh, n);
-      float w[2], sum = 0.f;
-      uint64_t pair[2];
+      float w[kPlaces], sum = 0.f;
+      uint64_t pair[kPlaces];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int i = 2 * tid + e;
+      for (int e = 0; e < kPlaces; ++e) {
+        const int i = kPlaces * tid + e;
         pair[e] = i < n ? sh.list[i] : 0;
         const float v = logit_of(pair[e]);
         w[e] = i < n ? (v == mx ? 1.f : ex2_approx((v - mx) * scale)) : 0.f;
@@ -559,10 +789,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       if (tid == 0) sh.cut = 0;
       __syncthreads();
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int i = 2 * tid + e;
+      for (int e = 0; e < kPlaces; ++e) {
+        const int i = kPlaces * tid + e;
         const bool stays = i < n && (by_mass ? before < limit || above + i == 0 : above + i < k);
-        if (stays && last && w[e] >= least) {
+        if (team.rank == 0 && stays && last && w[e] >= least) {
           z += w[e];
           best.see(logit_of(pair[e]), best.noise[index_of(pair[e])], index_of(pair[e]));
         }
@@ -578,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   if (!settled) {
     z = 0.f;
     best.index = -1, best.score = -INFINITY;
-    cut = slow_cut(row, mx, scale, k, p, sh);
+    cut = slow_cut(row, mx, scale, k, p, team);
     row.scan([&](const float* v, int i0) {
       keep(v, i0, [&](float x, int i) { return x == x && pair_of(key_of(x), i) >= cut; });
     });
@@ -586,10 +816,38 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   finish();
 }
 
+template <typename T, bool Staged>
+static cudaError_t launch_with(const Sample& a, int cluster, int bytes, cudaStream_t stream) {
+  if (Staged)
+    if (const cudaError_t e = cudaFuncSetAttribute(sample_kernel<T, Staged>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        e != cudaSuccess)
+      return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.rows) * cluster);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, sample_kernel<T, Staged>, a, cluster);
+}
+
 template <typename T>
 static cudaError_t launch(const Sample& a, cudaStream_t stream) {
-  sample_kernel<T><<<static_cast<unsigned>(a.rows), kThreads, 0, stream>>>(a);
-  return cudaGetLastError();
+  // Blocks per row: the fewest whose slices leave room for three blocks on an SM, more while the rows alone do not
+  // fill the GPU and every thread still gets two pieces.
+  constexpr int kSlice = (227 * 1024 / 3 - static_cast<int>(sizeof(Shared)) - 1024) / 16;  // pieces
+  const int pieces = static_cast<int>((static_cast<long long>(a.vocab) * sizeof(T) + 15) / 16 + 1);
+  int cluster = 1;
+  while (cluster < kMaxCluster && (pieces > cluster * kSlice || (a.rows * cluster < 148 && pieces > 2 * cluster * kThreads)))
+    cluster *= 2;
+  const int slice = (pieces + cluster - 1) / cluster;
+  if (slice <= kChunk * kChunks && slice * 16 <= 160 * 1024) return launch_with<T, true>(a, cluster, slice * 16, stream);
+  return launch_with<T, false>(a, cluster, 0, stream);
 }
 
 cudaError_t launch_sample(const Sample& a, cudaStream_t stream) {

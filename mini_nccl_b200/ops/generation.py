@@ -186,9 +186,10 @@ def sample(
         def split(x, whole):
             return (x, whole(0)) if isinstance(x, torch.Tensor) else (None, whole(x))
 
-        token, logprob = _kernels().ext().sample(
+        K = _kernels()
+        token, logprob = K.ext().sample(
             logits, noise, *split(temperature, float), *split(top_k, int), *split(top_p, float), *split(min_p, float),
-            return_logprob)
+            return_logprob, K.status_word(logits.device))
         return (token, logprob) if return_logprob else token
     _need(logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32),
           "logits: a bf16 or fp32 tensor [rows, vocabulary]")
