@@ -8,7 +8,7 @@
 // p times the weight of the first k; min-p those with w_i >= min_p.  So a
 // row is described by one cut, the last (logit, index) pair that stays.
 //
-// A cluster of 1 to 8 blocks of 256 threads takes a row.  Each block brings
+// A cluster of 1 to 8 blocks of 512 threads takes a row.  Each block brings
 // its slice of the row into shared memory once, by bulk copies, and the passes
 // below read it there; block results meet through distributed shared memory.
 // No pass sorts the row:
@@ -40,14 +40,14 @@ namespace sampling {
 namespace cg = cooperative_groups;
 
 constexpr int kMaxCluster = 8;
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kList = 1024;        // tokens a list can hold
 constexpr int kPlaces = kList / kThreads;
-constexpr int kSmallK = 3 * kThreads / 4;  // top-k by the threads' maxima: those of one block bound about 1.4 x 256 tokens
-constexpr int kMostK = 600;                // 2048 maxima bound about 700 tokens then, which a list holds
-constexpr int kChunk = 4 * kThreads;       // pieces of 16 bytes per bulk copy
+constexpr int kSmallK = 3 * kThreads / 4;  // top-k by the threads' maxima: those of one block bound about 1.4 x 512 tokens
+constexpr int kMostK = 600;                // more maxima than 512 bound under 700 tokens then, which a list holds
+constexpr int kChunk = 2 * kThreads;       // pieces of 16 bytes per bulk copy
 constexpr int kChunks = 8;
 constexpr float kRange = 36.f;     // bins cover weights down to 2^-36 of the largest
 constexpr int kLevels = 3;         // times a band is divided
@@ -79,31 +79,46 @@ MNB_DEVICE auto at(const S& s, int r) {
   return s.each ? s.each[r] : s.all;
 }
 
-struct Shared {
+// A block on its own counts and lists in place; the blocks of a cluster have parts of their own.
+template <bool Multi>
+struct Lists;
+template <>
+struct Lists<false> {
+  union {
+    int hist[kBins];
+    uint64_t list[kList];
+  };
+  MNB_DEVICE int* bins() { return hist; }
+  MNB_DEVICE uint64_t* mine() { return list; }
+};
+template <>
+struct Lists<true> {
+  uint64_t part[kList];
+  union {
+    float maxima[kMaxCluster][kThreads];
+    struct {
+      int counts[kBins];
+      int hist[kBins];
+    };
+    uint64_t list[kList];
+  };
+  MNB_DEVICE int* bins() { return counts; }
+  MNB_DEVICE uint64_t* mine() { return part; }
+};
+
+template <bool Multi>
+struct Shared : Lists<Multi> {
   union {
     uint64_t u64[kWarps];
     float f32[kWarps];
     int i32[kWarps];
   } red;
-  // one value of every block of the cluster, in turn in two places
-  union {
-    uint64_t u64[kMaxCluster];
-    float f32[kMaxCluster];
-    int i32[kMaxCluster];
-  } from[2];
-  uint64_t arrived[kChunks];  // mbarriers of the bulk copies
+  uint64_t from[2][kMaxCluster];  // one value of every block of the cluster, in turn in two places
+  uint64_t joined[2];             // mbarriers of these exchanges
+  uint64_t arrived[kChunks];      // mbarriers of the bulk copies
   int n_mine;
   int bin_from, bin_to, bin_count;
   uint64_t cut;
-  uint64_t mine[kList];  // this block's part of the list
-  union {
-    float maxima[kMaxCluster][kThreads];
-    struct {
-      int bins[kBins];      // this block's counts
-      int hist[kBins];      // the cluster's
-    };
-    uint64_t list[kList];   // the cluster's list
-  };
 };
 
 template <typename V, typename F>
@@ -118,50 +133,74 @@ MNB_DEVICE V block_reduce(V v, V* sh, F f) {
   __syncthreads();
   return s;
 }
-// The same over the cluster: every block sends its value to all, and joins what it got in the blocks' order.
+// The same over the cluster: every block sends its value to all by asynchronous remote stores, which the receivers'
+// mbarriers count, and joins what it got in the blocks' order.
+template <bool Multi>
 struct Team {
-  Shared& sh;
+  Shared<Multi>& sh;
   int size, rank;
-  int phase = 0;
+  int* status;
+  int exchanges = 0;
+  // everything written to shared memory before is there for every block after
   MNB_DEVICE void sync() const {
-    if (size > 1) cg::this_cluster().sync();
+    if (Multi) cg::this_cluster().sync();
     else __syncthreads();
   }
   template <typename T>
   MNB_DEVICE T* peer(T* p, int q) const {
-    return size > 1 ? cg::this_cluster().map_shared_rank(p, q) : p;
+    return Multi ? cg::this_cluster().map_shared_rank(p, q) : p;
   }
+  MNB_DEVICE static uint64_t bits(float v) { return __float_as_uint(v); }
+  MNB_DEVICE static uint64_t bits(int v) { return static_cast<uint32_t>(v); }
+  MNB_DEVICE static uint64_t bits(uint64_t v) { return v; }
+  MNB_DEVICE static void of_bits(uint64_t b, float& v) { v = __uint_as_float(static_cast<uint32_t>(b)); }
+  MNB_DEVICE static void of_bits(uint64_t b, int& v) { v = static_cast<int>(static_cast<uint32_t>(b)); }
+  MNB_DEVICE static void of_bits(uint64_t b, uint64_t& v) { v = b; }
   template <typename V, typename F>
-  MNB_DEVICE V join(V v, V* red, V* from, F f) {
+  MNB_DEVICE V join(V v, V* red, F f) {
     v = block_reduce(v, red, f);
-    if (size == 1) return v;
-    if (threadIdx.x < size) *peer(from + rank, threadIdx.x) = v;
-    sync();
-    V s = from[0];
-    for (int q = 1; q < size; ++q) s = f(s, from[q]);
-    phase ^= 1;
+    if (!Multi) return v;
+    const int turn = exchanges & 1;
+    const uint32_t bar = smem_u32(sh.joined + turn);
+    if (threadIdx.x == 0) mbar_arrive_expect_tx(bar, 8 * size);
+    if (threadIdx.x < size) {
+      uint32_t to, to_bar;
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(&sh.from[turn][rank])), "r"(threadIdx.x));
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to_bar) : "r"(bar), "r"(threadIdx.x));
+      asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(to), "l"(bits(v)), "r"(to_bar)
+                   : "memory");
+    }
+    mbar_wait(bar, (exchanges >> 1) & 1, status);
+    ++exchanges;
+    V s, x;
+    of_bits(*const_cast<volatile uint64_t*>(&sh.from[turn][0]), s);
+    for (int q = 1; q < size; ++q) {
+      of_bits(*const_cast<volatile uint64_t*>(&sh.from[turn][q]), x);
+      s = f(s, x);
+    }
     return s;
   }
   MNB_DEVICE float sum(float v) {
-    return join(v, sh.red.f32, sh.from[phase].f32, [](float a, float b) { return a + b; });
+    return join(v, sh.red.f32, [](float a, float b) { return a + b; });
   }
   MNB_DEVICE int sum(int v) {
-    return join(v, sh.red.i32, sh.from[phase].i32, [](int a, int b) { return a + b; });
+    return join(v, sh.red.i32, [](int a, int b) { return a + b; });
   }
   MNB_DEVICE float max(float v) {
-    return join(v, sh.red.f32, sh.from[phase].f32, [](float a, float b) { return fmaxf(a, b); });
+    return join(v, sh.red.f32, [](float a, float b) { return fmaxf(a, b); });
   }
   MNB_DEVICE uint64_t max(uint64_t v) {
-    return join(v, sh.red.u64, sh.from[phase].u64, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+    return join(v, sh.red.u64, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
   }
   // The blocks' lists into everybody's `list`; returns the length, more than kList if they do not fit.
-  // The next change of `mine` has to lie behind another exchange.
+  // The next change of a part has to lie behind another sync().
   MNB_DEVICE int gather_list() {
     sync();
+    if (!Multi) return sh.n_mine;
     int n = 0;
     for (int q = 0; q < size; ++q) {
       const int m = *peer(&sh.n_mine, q);
-      const uint64_t* from = peer(sh.mine, q);
+      const uint64_t* from = peer(sh.mine(), q);
       if (n + m <= kList)
         for (int i = threadIdx.x; i < m; i += kThreads) sh.list[n + i] = from[i];
       n += m;
@@ -170,10 +209,12 @@ struct Team {
     return n;
   }
 };
-MNB_DEVICE float block_sum(float v, Shared& sh) {
+template <typename S>
+MNB_DEVICE float block_sum(float v, S& sh) {
   return block_reduce(v, sh.red.f32, [](float a, float b) { return a + b; });
 }
-MNB_DEVICE int block_sum(int v, Shared& sh) {
+template <typename S>
+MNB_DEVICE int block_sum(int v, S& sh) {
   return block_reduce(v, sh.red.i32, [](int a, int b) { return a + b; });
 }
 // Sum over the threads before this one.
@@ -326,20 +367,12 @@ struct Best {
     score = better ? s : score;
     index = better ? i : index;
   }
-  // The same for v * inv_t + g: the best and the second best, for a thread's own ranking.
-  float near_score = -INFINITY, near_second = -INFINITY, near_v = 0.f, near_g = 0.f;
-  int near_index = -1;
-  MNB_DEVICE void see_nearly(bool counts, float v, float g, int i) {
-    const float s = counts ? fmaf(v, inv_t, g) : -INFINITY;
-    near_second = fmaxf(near_second, fminf(near_score, s));
-    if (s > near_score) near_v = v, near_g = g, near_index = i;
-    near_score = fmaxf(near_score, s);
-  }
   MNB_DEVICE uint64_t pair() const { return index < 0 ? 0 : pair_of(key_of(score), index); }
 };
 
 // The list in descending order (bitonic, n <= kList, one compare per thread and step).
-MNB_DEVICE int sort_list(Shared& sh, int n) {
+template <typename S>
+MNB_DEVICE int sort_list(S& sh, int n) {
   int n2 = 32;
   while (n2 < n) n2 <<= 1;
   for (int i = n + threadIdx.x; i < n2; i += kThreads) sh.list[i] = 0;
@@ -362,8 +395,8 @@ MNB_DEVICE int sort_list(Shared& sh, int n) {
 }
 
 // Bisection over the pairs: right for every row, some 50 passes.
-template <typename T, bool Staged>
-__device__ __noinline__ uint64_t slow_cut(const Row<T, Staged>& row, float mx, float scale, int k, float p, Team& team) {
+template <typename T, bool Staged, bool Multi>
+__device__ __noinline__ uint64_t slow_cut(const Row<T, Staged>& row, float mx, float scale, int k, float p, Team<Multi>& team) {
   auto weight = [&](float v) { return v == mx ? 1.f : ex2_approx((v - mx) * scale); };  // an infinite maximum takes all
   uint64_t best = 0;
   row.scan([&](const float* v, int i0) {
@@ -409,22 +442,24 @@ __device__ __noinline__ uint64_t slow_cut(const Row<T, Staged>& row, float mx, f
   return cut;
 }
 
-template <typename T, bool Staged>
-__global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_constant__ Sample a, int cluster) {
+template <typename T, bool Staged, bool Multi>
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ Sample a, int cluster) {
   using R = Row<T, Staged>;
   constexpr int kVec = R::kVec;
   extern __shared__ uint4 slice[];
-  __shared__ Shared sh;
+  __shared__ Shared<Multi> sh;
   const int r = blockIdx.x / cluster, tid = threadIdx.x;
-  Team team{sh, cluster, static_cast<int>(blockIdx.x) % cluster};
-  if (cluster > 1) cg::this_cluster().barrier_arrive();  // a block's shared memory is there once the block runs
+  if (!Multi) cluster = 1;
+  Team<Multi> team{sh, cluster, static_cast<int>(blockIdx.x) % cluster, a.status};
   const R row(static_cast<const T*>(a.logits) + r * a.ld, a.vocab, team.rank, cluster, slice);
-  if (Staged) {
+  if (Staged || Multi) {
     if (tid == 0) {
       for (int j = 0; j < kChunks; ++j) mbar_init(smem_u32(sh.arrived + j), 1);
+      for (int j = 0; j < 2; ++j) mbar_init(smem_u32(sh.joined + j), 1);
       fence_mbar_init();
     }
     __syncthreads();
+    if (Multi) cg::this_cluster().barrier_arrive();  // this block runs and its mbarriers are there
     row.stage(sh.arrived);
   }
 
@@ -435,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
     for (int e = 0; e < kChunk / kThreads; ++e, c += kThreads)
       if (c < row.count) mine = R::widest(row.piece(c), mine);
   }
-  if (cluster > 1) cg::this_cluster().barrier_wait();
+  if (Multi) cg::this_cluster().barrier_wait();
   const float mx = team.max(mine);
   const float t = at(a.temperature, r);
   if (mx == -INFINITY || !(t > 0.f)) {  // no token left, or the first one
@@ -462,9 +497,9 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
   best.noise = a.noise + r * a.noise_ld;
   float z = 0.f;  // weight of the kept tokens that this thread has seen
 
-  // The noise of the elements of a piece whose weight w[j] is not negative.
+  // The noise of the wanted elements of a piece.
   const bool noise_vec = (reinterpret_cast<uintptr_t>(best.noise - row.lead) & 15) == 0;
-  auto fetch = [&](float* g, const float* w, int i0) {
+  auto fetch = [&](float* g, int i0, auto wanted) {
     if (noise_vec && i0 >= 0 && i0 + kVec <= a.vocab) {
 #pragma unroll
       for (int j = 0; j < kVec; j += 4) {
@@ -473,17 +508,17 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) g[j] = w[j] >= 0.f ? best.noise[i0 + j] : 0.f;
+      for (int j = 0; j < kVec; ++j) g[j] = wanted(j) ? best.noise[i0 + j] : 0.f;
     }
   };
-  // Scores those elements.
+  // Scores the elements of a piece whose weight is not negative.
   auto score = [&](const float* v, const float* w, int i0) {
     bool any = false;
 #pragma unroll
     for (int j = 0; j < kVec; ++j) any |= w[j] >= 0.f;
     if (!any) return;
     float g[kVec];
-    fetch(g, w, i0);
+    fetch(g, i0, [&](int j) { return w[j] >= 0.f; });
 #pragma unroll
     for (int j = 0; j < kVec; ++j)
       if (w[j] >= 0.f) {
@@ -532,18 +567,21 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
       // the bound: the k-th largest of the threads' maxima, or a little less
       uint32_t lo = kKeyNegInf + 1;
       if (a.vocab > kList) {
-        // every block gets all the maxima, so the search needs no further exchange
-        for (int q = 0; q < cluster; ++q) team.peer(&sh.maxima[team.rank][tid], q)[0] = mine;
-        team.sync();
-        uint32_t key[kMaxCluster];
+        constexpr int kSets = Multi ? kMaxCluster : 1;
+        uint32_t key[kSets];
+        key[0] = key_of(mine);
+        if constexpr (Multi) {  // every block gets all the maxima, so the search needs no further exchange
+          for (int q = 0; q < cluster; ++q) team.peer(&sh.maxima[team.rank][tid], q)[0] = mine;
+          team.sync();
 #pragma unroll
-        for (int q = 0; q < kMaxCluster; ++q) key[q] = q < cluster ? key_of(sh.maxima[q][tid]) : 0u;
+          for (int q = 0; q < kSets; ++q) key[q] = q < cluster ? key_of(sh.maxima[q][tid]) : 0u;
+        }
         uint32_t hi = key_of(mx);
         while (lo < hi) {  // the largest bound that at least k maxima reach
           const uint32_t mid = lo + (hi - lo + 1) / 2;
           int n = 0;
 #pragma unroll
-          for (int q = 0; q < kMaxCluster; ++q)
+          for (int q = 0; q < kSets; ++q)
             if (q < cluster) n += __syncthreads_count(key[q] >= mid);
           if (n >= k) {
             lo = mid;
@@ -561,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
         for (int j = 0; j < kVec; ++j)
           if (v[j] >= bound) {
             const int n = atomicAdd(&sh.n_mine, 1);
-            if (n < kList) sh.mine[n] = pair_of(key_of(v[j]), i0 + j);
+            if (n < kList) sh.mine()[n] = pair_of(key_of(v[j]), i0 + j);
           }
       });
       const int n = team.gather_list();
@@ -606,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
       ok = false;
       for (int level = 0; level < kLevels && !ok; ++level) {
         if (level) team.sync();  // everybody has read the last level's counts
-        for (int b = tid; b < kBins; b += kThreads) sh.bins[b] = 0;
+        for (int b = tid; b < kBins; b += kThreads) sh.bins()[b] = 0;
         __syncthreads();
         const float per = kBins / (y1 - y0);
         float mass = 0.f;  // level 0: of everything; later: of what lies above the band
@@ -614,33 +652,42 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
         // At first the last bin also takes what lies beyond the range, and NaN.
         auto tally = [&](auto filter, auto masses, auto first) {
           row.scan([&](const float* v, int i0) {
+            const float2 mx2 = splat2(mx), scale2 = splat2(scale), per2 = splat2(per), y02 = splat2(y0);
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) {
-              const float y = (mx - v[j]) * scale;
-              if (filter.value && !(v[j] > -INFINITY && pair_of(key_of(v[j]), i0 + j) >= cut)) continue;
-              if (masses.value) {
-                const float w = ex2_approx(-y);
-                mass += (first.value ? y < INFINITY : y < y0) ? w : 0.f;
-              } else if (!first.value && y < y0) {
-                ++above;
+            for (int j = 0; j < kVec; j += 2) {
+              const float2 y2 = mul2(sub2(mx2, make_float2(v[j], v[j + 1])), scale2);
+              const float2 b2 = mul2(first.value ? y2 : sub2(y2, y02), per2);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float y = e ? y2.y : y2.x;
+                if (filter.value && !(v[j + e] > -INFINITY && pair_of(key_of(v[j + e]), i0 + j + e) >= cut)) continue;
+                if (masses.value) {
+                  const float w = ex2_approx(-y);
+                  if (first.value ? y < INFINITY : y < y0) mass += w;
+                } else if (!first.value) {
+                  above += y < y0;
+                }
+                // adding 2^23 leaves the bin, rounded to the nearest, in the low bits
+                const float b = fminf(e ? b2.y : b2.x, kBins - 1.f) + 8388608.f;
+                if (first.value || (y >= y0 && y <= y1)) atomicAdd(sh.bins() + (__float_as_uint(b) & (kBins - 1)), 1);
               }
-              // adding 2^23 leaves the bin, rounded to the nearest, in the low bits
-              const float b = fminf(first.value ? y * per : (y - y0) * per, kBins - 1.f) + 8388608.f;
-              if (first.value || (y >= y0 && y <= y1)) atomicAdd(&sh.bins[__float_as_uint(b) & (kBins - 1)], 1);
             }
           });
         };
         if (filtered) level ? tally(Yes{}, Yes{}, No{}) : tally(Yes{}, Yes{}, Yes{});
         else if (by_mass) level ? tally(No{}, Yes{}, No{}) : tally(No{}, Yes{}, Yes{});
         else level ? tally(No{}, No{}, No{}) : tally(No{}, No{}, Yes{});
-        mass = team.sum(mass);
-        above = team.sum(above);  // (these exchanges also tell that every block's counts are there)
-        for (int b = tid; b < kBins; b += kThreads) {
-          int c = 0;
-          for (int q = 0; q < cluster; ++q) c += *team.peer(&sh.bins[b], q);
-          sh.hist[b] = c;
+        if (by_mass) mass = team.sum(mass);
+        else if (level) above = team.sum(above);
+        team.sync();
+        if constexpr (Multi) {
+          for (int b = tid; b < kBins; b += kThreads) {
+            int c = 0;
+            for (int q = 0; q < cluster; ++q) c += *team.peer(sh.bins() + b, q);
+            sh.hist[b] = c;
+          }
+          __syncthreads();
         }
-        __syncthreads();
         if (by_mass && level == 0) limit = p * mass;
         // this thread's bins, in order
         constexpr int kPer = kBins / kThreads;
@@ -648,17 +695,18 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
         int c[kPer], sum_c = 0;
         float sum_hi = 0.f, sum_lo = 0.f;  // with every token at the bin's upper / lower weight
         const float step = 1.f / per;
-        auto upper = [&](int b) { return ex2_approx(-(y0 + (b - 0.5f) * step)); };
-        auto lower = [&](int b) {
-          return b < kBins - 1 ? ex2_approx(-(y0 + (b + 0.5f) * step)) : level ? ex2_approx(-(y0 + kBins * step)) : 0.f;
-        };
+        const float w0 = ex2_approx(-(y0 + (tid * kPer - 0.5f) * step)), ratio = ex2_approx(-step);
+        // (the last bin of the first level has no lower end)
+        auto lower = [&](int b, float upper) { return b == kBins - 1 && !level ? 0.f : upper * ratio * (b == kBins - 1 ? ratio : 1.f); };
+        float upper = w0;
 #pragma unroll
         for (int e = 0; e < kPer; ++e) {
           const int b = tid * kPer + e;
           c[e] = sh.hist[b];
           sum_c += c[e];
-          sum_hi += c[e] * upper(b);
-          sum_lo += c[e] * lower(b);
+          sum_hi += c[e] * upper;
+          sum_lo += c[e] * lower(b, upper);
+          upper *= ratio;
         }
         if (tid == 0) sh.bin_from = kBins, sh.bin_to = kBins, sh.bin_count = 0;
         int n = block_before(sum_c, sh.red.i32);
@@ -676,12 +724,14 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
           const float all_hi = block_sum(sum_hi, sh);
           float behind = level == 0 ? all_hi - (hi - head) : INFINITY;
           const float all = level == 0 ? mass * (1.f - 2e-6f) : 0.f;
+          upper = w0;
 #pragma unroll
           for (int e = 0; e < kPer; ++e) {
             const int b = tid * kPer + e;
-            hi += c[e] * upper(b);
-            lo += c[e] * lower(b);
-            behind -= c[e] * upper(b);
+            hi += c[e] * upper;
+            lo += c[e] * lower(b, upper);
+            behind -= c[e] * upper;
+            upper *= ratio;
             if (c[e] && hi >= limit * (1.f - 1e-5f)) atomicMin(&sh.bin_from, b);
             if (c[e] && (lo >= limit * (1.f + 1e-5f) || all - behind * (1.f + 1e-4f) >= limit * (1.f + 1e-5f)))
               atomicMin(&sh.bin_to, b);
@@ -714,55 +764,90 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
       float mass = 0.f;
       int above = 0;
       const float bound = mx - (y1 * 1.0001f + 0.01f) / scale;  // what lies below the band is skipped by the piece
-      const bool rough = last && !(least > 0.f);
-      auto split = [&](auto filter, auto roughly) {
+      const bool rough = by_mass && !filtered && !(least > 0.f);
+      // The usual case, top-p alone: scores by a product, of which a thread keeps the best and second best piece.
+      float near = -INFINITY, second = -INFINITY;
+      int near_at = -1;
+      if (rough) {
         row.scan_from(bound, [&](const float* v, int i0) {
-          float w[kVec];
-          bool any = false;
+          const float2 mx2 = splat2(mx), scale2 = splat2(scale);
+          float y[kVec];
+          bool any = false, band = false;
+#pragma unroll
+          for (int j = 0; j < kVec; j += 2) {
+            const float2 y2 = mul2(sub2(mx2, make_float2(v[j], v[j + 1])), scale2);
+            y[j] = y2.x, y[j + 1] = y2.y;
+          }
 #pragma unroll
           for (int j = 0; j < kVec; ++j) {
-            const float y = (mx - v[j]) * scale;
-            bool in = y <= y1;
-            if (filter.value) in = in && pair_of(key_of(v[j]), i0 + j) >= cut;
-            const bool over = in && y < y0;
-            const float x = ex2_approx(-y);
-            mass += over ? x : 0.f;
-            above += over;
-            w[j] = over && x >= least ? x : -1.f;
-            any |= over;
-            if (in && !over) {
-              const int n = atomicAdd(&sh.n_mine, 1);
-              if (n < kList) sh.mine[n] = pair_of(key_of(v[j]), i0 + j);
-            }
+            const float w = ex2_approx(-y[j]);
+            if (y[j] < y0) mass += w;
+            any |= y[j] < y0;
+            band |= y[j] >= y0 && y[j] <= y1;
           }
-          if (!any || !last) return;
-          if (!roughly.value) return score(v, w, i0);
-          float g[kVec];
-          fetch(g, w, i0);
+          if (band) {
 #pragma unroll
-          for (int j = 0; j < kVec; ++j) best.see_nearly(w[j] >= 0.f, v[j], g[j], i0 + j);
+            for (int j = 0; j < kVec; ++j)
+              if (y[j] >= y0 && y[j] <= y1) {
+                const int n = atomicAdd(&sh.n_mine, 1);
+                if (n < kList) sh.mine()[n] = pair_of(key_of(v[j]), i0 + j);
+              }
+          }
+          if (!any) return;
+          float g[kVec], s = -INFINITY;
+          fetch(g, i0, [&](int j) { return y[j] < y0; });
+#pragma unroll
+          for (int j = 0; j < kVec; j += 2)
+            s = max3f(s, fmaf(v[j], best.inv_t, y[j] < y0 ? g[j] : -INFINITY),
+                      fmaf(v[j + 1], best.inv_t, y[j + 1] < y0 ? g[j + 1] : -INFINITY));
+          second = fmaxf(second, fminf(near, s));
+          near_at = s > near ? i0 : near_at;
+          near = fmaxf(near, s);
         });
-      };
-      if (filtered) split(Yes{}, No{});
-      else if (rough) split(No{}, Yes{});
-      else split(No{}, No{});
-      if (rough && !filtered) {
-        // Scores by a product are off by less than this; whoever is that near the top is scored exactly, and if a
-        // thread's second best is too, all are.
-        const float top = team.max(best.near_score);
+        // A product is off by less than `off`; a piece that comes that near the top is scored exactly, and if a
+        // thread's second best does too (or a noise is infinite or NaN), all are.
+        const float top = team.max(near);
         const float off = 1e-6f * (fabsf(mx * best.inv_t) + y1 + fabsf(top));
-        const bool unclear = best.near_second >= top - off || !(fabsf(top) < 1e30f);
+        const bool unclear = second >= top - off || !(fabsf(top) < 1e30f);
         if (team.sum(static_cast<int>(unclear))) {
           row.scan_from(bound, [&](const float* v, int i0) {
             keep(v, i0, [&](float x, int) { return (mx - x) * scale < y0; });
           });
-        } else if (best.near_score >= top - off) {
-          best.see(best.near_v, best.near_g, best.near_index);
+        } else if (near >= top - off) {
+          for (int j = 0; j < kVec; ++j)
+            if (near_at + j >= 0 && near_at + j < a.vocab) {
+              const float x = row.one(near_at + j);
+              if ((mx - x) * scale < y0) best.see(x, best.noise[near_at + j], near_at + j);
+            }
         }
         z = mass;
+      } else {
+        auto split = [&](auto filter) {
+          row.scan_from(bound, [&](const float* v, int i0) {
+            float w[kVec];
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) {
+              const float y = (mx - v[j]) * scale;
+              bool in = y <= y1;
+              if (filter.value) in = in && pair_of(key_of(v[j]), i0 + j) >= cut;
+              const bool over = in && y < y0;
+              const float x = ex2_approx(-y);
+              if (over) mass += x;
+              above += over;
+              w[j] = over && x >= least ? x : -1.f;
+              if (in && !over) {
+                const int n = atomicAdd(&sh.n_mine, 1);
+                if (n < kList) sh.mine()[n] = pair_of(key_of(v[j]), i0 + j);
+              }
+            }
+            if (last) score(v, w, i0);
+          });
+        };
+        if (filtered) split(Yes{});
+        else split(No{});
       }
       mass = team.sum(mass);
-      above = team.sum(above);
+      above = rough ? mass > 0.f : team.sum(above);  // (top-p asks only whether there is any)
       const int n = team.gather_list();
       if (n > kList) {
         ok = false;
@@ -816,10 +901,10 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
   finish();
 }
 
-template <typename T, bool Staged>
+template <typename T, bool Staged, bool Multi>
 static cudaError_t launch_with(const Sample& a, int cluster, int bytes, cudaStream_t stream) {
   if (Staged)
-    if (const cudaError_t e = cudaFuncSetAttribute(sample_kernel<T, Staged>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (const cudaError_t e = cudaFuncSetAttribute(sample_kernel<T, Staged, Multi>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
         e != cudaSuccess)
       return e;
   cudaLaunchConfig_t cfg{};
@@ -833,21 +918,22 @@ static cudaError_t launch_with(const Sample& a, int cluster, int bytes, cudaStre
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sample_kernel<T, Staged>, a, cluster);
+  return cudaLaunchKernelEx(&cfg, sample_kernel<T, Staged, Multi>, a, cluster);
 }
 
 template <typename T>
 static cudaError_t launch(const Sample& a, cudaStream_t stream) {
-  // Blocks per row: the fewest whose slices leave room for three blocks on an SM, more while the rows alone do not
+  // Blocks per row: the fewest whose slices leave room for two blocks on an SM, more while the rows alone do not
   // fill the GPU and every thread still gets two pieces.
-  constexpr int kSlice = (227 * 1024 / 3 - static_cast<int>(sizeof(Shared)) - 1024) / 16;  // pieces
+  auto room = [](size_t shared) { return (227 * 1024 / 2 - static_cast<int>(shared) - 1024) / 16; };  // pieces
   const int pieces = static_cast<int>((static_cast<long long>(a.vocab) * sizeof(T) + 15) / 16 + 1);
   int cluster = 1;
-  while (cluster < kMaxCluster && (pieces > cluster * kSlice || (a.rows * cluster < 148 && pieces > 2 * cluster * kThreads)))
-    cluster *= 2;
+  auto fits = [&](int c) { return (pieces + c - 1) / c <= room(c > 1 ? sizeof(Shared<true>) : sizeof(Shared<false>)); };
+  while (cluster < kMaxCluster && (!fits(cluster) || (a.rows * cluster < 148 && pieces > 2 * cluster * kThreads))) cluster *= 2;
   const int slice = (pieces + cluster - 1) / cluster;
-  if (slice <= kChunk * kChunks && slice * 16 <= 160 * 1024) return launch_with<T, true>(a, cluster, slice * 16, stream);
-  return launch_with<T, false>(a, cluster, 0, stream);
+  const bool staged = slice <= kChunk * kChunks;
+  if (cluster == 1) return launch_with<T, true, false>(a, 1, slice * 16, stream);
+  return staged ? launch_with<T, true, true>(a, cluster, slice * 16, stream) : launch_with<T, false, true>(a, cluster, 0, stream);
 }
 
 cudaError_t launch_sample(const Sample& a, cudaStream_t stream) {
