@@ -48,7 +48,7 @@ constexpr int kPlaces = kList / kThreads;
 constexpr int kSmallK = 3 * kThreads / 4;  // top-k by the threads' maxima: those of one block bound about 1.4 x 512 tokens
 constexpr int kMostK = 600;                // more maxima than 512 bound under 700 tokens then, which a list holds
 constexpr int kChunk = 2 * kThreads;       // pieces of 16 bytes per bulk copy
-constexpr int kChunks = 8;
+constexpr int kChunks = 14;
 constexpr float kRange = 36.f;     // bins cover weights down to 2^-36 of the largest
 constexpr int kLevels = 3;         // times a band is divided
 constexpr uint32_t kIndexMask = (1u << kIndexBits) - 1;
@@ -112,8 +112,13 @@ struct Shared : Lists<Multi> {
     uint64_t u64[kWarps];
     float f32[kWarps];
     int i32[kWarps];
+    struct {
+      int n[kWarps];
+      float hi[kWarps], lo[kWarps];
+    } sums;
   } red;
   uint64_t from[2][kMaxCluster];  // one value of every block of the cluster, in turn in two places
+  uint64_t from_too[2][kMaxCluster];
   uint64_t joined[2];             // mbarriers of these exchanges
   uint64_t arrived[kChunks];      // mbarriers of the bulk copies
   int n_mine;
@@ -156,6 +161,14 @@ struct Team {
   MNB_DEVICE static void of_bits(uint64_t b, float& v) { v = __uint_as_float(static_cast<uint32_t>(b)); }
   MNB_DEVICE static void of_bits(uint64_t b, int& v) { v = static_cast<int>(static_cast<uint32_t>(b)); }
   MNB_DEVICE static void of_bits(uint64_t b, uint64_t& v) { v = b; }
+  // 8 bytes to the same place in block q, counted by its mbarrier
+  MNB_DEVICE static void send(uint64_t* place, uint64_t v, uint32_t bar, int q) {
+    uint32_t to, to_bar;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(place)), "r"(q));
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to_bar) : "r"(bar), "r"(q));
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(to), "l"(v), "r"(to_bar)
+                 : "memory");
+  }
   template <typename V, typename F>
   MNB_DEVICE V join(V v, V* red, F f) {
     v = block_reduce(v, red, f);
@@ -163,13 +176,7 @@ struct Team {
     const int turn = exchanges & 1;
     const uint32_t bar = smem_u32(sh.joined + turn);
     if (threadIdx.x == 0) mbar_arrive_expect_tx(bar, 8 * size);
-    if (threadIdx.x < size) {
-      uint32_t to, to_bar;
-      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(&sh.from[turn][rank])), "r"(threadIdx.x));
-      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to_bar) : "r"(bar), "r"(threadIdx.x));
-      asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(to), "l"(bits(v)), "r"(to_bar)
-                   : "memory");
-    }
+    if (threadIdx.x < size) send(&sh.from[turn][rank], bits(v), bar, threadIdx.x);
     mbar_wait(bar, (exchanges >> 1) & 1, status);
     ++exchanges;
     V s, x;
@@ -192,6 +199,29 @@ struct Team {
   MNB_DEVICE uint64_t max(uint64_t v) {
     return join(v, sh.red.u64, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
   }
+  // The largest `best` and the sum of `z` of all threads, in one exchange.
+  MNB_DEVICE uint64_t max_and_sum(uint64_t best, float* z) {
+    best = block_reduce(best, sh.red.u64, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+    *z = block_reduce(*z, sh.red.f32, [](float a, float b) { return a + b; });
+    if (!Multi) return best;
+    const int turn = exchanges & 1;
+    const uint32_t bar = smem_u32(sh.joined + turn);
+    if (threadIdx.x == 0) mbar_arrive_expect_tx(bar, 16 * size);
+    if (threadIdx.x < size) {
+      send(&sh.from[turn][rank], best, bar, threadIdx.x);
+      send(&sh.from_too[turn][rank], bits(*z), bar, threadIdx.x);
+    }
+    mbar_wait(bar, (exchanges >> 1) & 1, status);
+    ++exchanges;
+    *z = 0.f;
+    for (int q = 0; q < size; ++q) {
+      best = ::max(best, *const_cast<volatile uint64_t*>(&sh.from[turn][q]));
+      float x;
+      of_bits(*const_cast<volatile uint64_t*>(&sh.from_too[turn][q]), x);
+      *z += x;
+    }
+    return best;
+  }
   // The blocks' lists into everybody's `list`; returns the length, more than kList if they do not fit.
   // The next change of a part has to lie behind another sync().
   MNB_DEVICE int gather_list() {
@@ -209,30 +239,38 @@ struct Team {
     return n;
   }
 };
+// Sums over the threads before this one, and over all.
+struct Sums {
+  int n;
+  float hi, lo;
+};
 template <typename S>
-MNB_DEVICE float block_sum(float v, S& sh) {
-  return block_reduce(v, sh.red.f32, [](float a, float b) { return a + b; });
-}
-template <typename S>
-MNB_DEVICE int block_sum(int v, S& sh) {
-  return block_reduce(v, sh.red.i32, [](int a, int b) { return a + b; });
-}
-// Sum over the threads before this one.
-template <typename V>
-MNB_DEVICE V block_before(V v, V* sh) {
+MNB_DEVICE Sums sums_before(Sums v, S& sh, Sums* total) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  V x = v;
+  auto scan = [&](auto x) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const V y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  if (lane == 31) sh[warp] = x;
+    for (int o = 1; o < 32; o <<= 1) {
+      const auto y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    return x;
+  };
+  const Sums x{scan(v.n), scan(v.hi), scan(v.lo)};
+  if (lane == 31) sh.red.sums.n[warp] = x.n, sh.red.sums.hi[warp] = x.hi, sh.red.sums.lo[warp] = x.lo;
   __syncthreads();
-  V base = 0;
-  for (int i = 0; i < warp; ++i) base += sh[i];
+  const bool in = lane < kWarps;
+  const Sums w{in ? sh.red.sums.n[lane % kWarps] : 0, in ? sh.red.sums.hi[lane % kWarps] : 0.f,
+               in ? sh.red.sums.lo[lane % kWarps] : 0.f};
+  const Sums p{scan(w.n), scan(w.hi), scan(w.lo)};
+  auto at = [](auto x, int i) { return __shfl_sync(0xffffffffu, x, i); };
+  *total = {at(p.n, 31), at(p.hi, 31), at(p.lo, 31)};
+  const Sums head{at(p.n, (warp + 31) % 32), at(p.hi, (warp + 31) % 32), at(p.lo, (warp + 31) % 32)};
   __syncthreads();
-  return base + (x - v);
+  // (x - v would lose what cancels: shift the scan by a lane instead)
+  Sums before{__shfl_up_sync(0xffffffffu, x.n, 1), __shfl_up_sync(0xffffffffu, x.hi, 1), __shfl_up_sync(0xffffffffu, x.lo, 1)};
+  if (lane == 0) before = {0, 0.f, 0.f};
+  if (warp > 0) before = {before.n + head.n, before.hi + head.hi, before.lo + head.lo};
+  return before;
 }
 
 MNB_DEVICE float to_float(float v) { return v; }
@@ -329,7 +367,45 @@ struct Row {
       f(v, start(c));
     }
   }
-  // the same over the pieces with an element of at least `least`
+  // f(values, noise, index of the first) over the pieces with an element of at least `least`.  The next piece's noise
+  // is on its way while this one is worked on, in two sets of registers by turns (a copy from one to the other would
+  // wait for the loads).
+  template <typename F>
+  MNB_DEVICE void scan_noise(float least, const float* noise, F f) const {
+    const bool vec = (reinterpret_cast<uintptr_t>(noise - lead) & 15) == 0;
+    auto fetch = [&](int c, float (&g)[kVec]) {
+      if (c >= count || !(widest(piece(c), -INFINITY) >= least)) return false;
+      const int i0 = start(c);
+      if (vec && whole(c)) {
+#pragma unroll
+        for (int j = 0; j < kVec; j += 4) {
+          const float4 t = *reinterpret_cast<const float4*>(noise + i0 + j);
+          g[j] = t.x, g[j + 1] = t.y, g[j + 2] = t.z, g[j + 3] = t.w;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) g[j] = i0 + j >= 0 && i0 + j < V ? noise[i0 + j] : 0.f;
+      }
+      return true;
+    };
+    auto work = [&](int c, const float (&g)[kVec]) {
+      float v[kVec];
+      unpack_piece(piece(c), v);
+#pragma unroll
+      for (int j = 0; j < kVec; j += 4) f(v + j, g + j, start(c) + j);  // four at a time: fewer values held at once
+    };
+    float g0[kVec], g1[kVec];
+    int c = threadIdx.x;
+    bool have0 = fetch(c, g0), have1;
+    while (c < count) {
+      have1 = fetch(c + kThreads, g1);
+      if (have0) work(c, g0);
+      have0 = fetch(c + 2 * kThreads, g0);
+      if (have1) work(c + kThreads, g1);
+      c += 2 * kThreads;
+    }
+  }
+  // f(values, index of the first) over those pieces
   template <typename F>
   MNB_DEVICE void scan_from(float least, F f) const {
 #pragma unroll 4
@@ -370,33 +446,74 @@ struct Best {
   MNB_DEVICE uint64_t pair() const { return index < 0 ? 0 : pair_of(key_of(score), index); }
 };
 
-// The list in descending order (bitonic, n <= kList, one compare per thread and step).
+// Puts the n <= kList pairs of the list in descending order; the log-weights lie between y0 and y1.  A counting sort by
+// finer bins of the log-weight, after which each pair is ranked among those of its own bin.  (The list and the counts
+// may share their memory: the pairs wait in registers.)
 template <typename S>
-MNB_DEVICE int sort_list(S& sh, int n) {
-  int n2 = 32;
-  while (n2 < n) n2 <<= 1;
-  for (int i = n + threadIdx.x; i < n2; i += kThreads) sh.list[i] = 0;
-  __syncthreads();
-  const bool one_warp = n2 <= 64;  // only warp 0 has work: its steps need no block barrier
-  if (!one_warp || threadIdx.x < 32) {
-    for (int size = 2; size <= n2; size <<= 1)
-      for (int stride = size / 2; stride > 0; stride >>= 1) {
-        for (int t = threadIdx.x; t < n2 / 2; t += one_warp ? 32 : kThreads) {
-          const int i = 2 * t - (t & (stride - 1)), j = i + stride;
-          const uint64_t a = sh.list[i], b = sh.list[j];
-          if ((a < b) == ((i & size) == 0)) sh.list[i] = b, sh.list[j] = a;
-        }
-        if (one_warp) __syncwarp();
-        else __syncthreads();
-      }
+MNB_DEVICE void sort_list(S& sh, int n, float mx, float scale, float y0, float y1) {
+  const float per = y1 > y0 ? kBins / (y1 - y0) : 0.f;
+  uint64_t pair[kPlaces];
+  int bin[kPlaces], start[kPlaces], end[kPlaces], slot[kPlaces];
+#pragma unroll
+  for (int e = 0; e < kPlaces; ++e) {
+    const int i = threadIdx.x + e * kThreads;
+    pair[e] = i < n ? sh.list[i] : 0;
+    const float y = (mx - logit_of(pair[e])) * scale;
+    bin[e] = static_cast<int>(fminf(fmaxf((y - y0) * per, 0.f), kBins - 1.f));
   }
   __syncthreads();
-  return n2;
+  for (int b = threadIdx.x; b < kBins; b += kThreads) sh.hist[b] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < kPlaces; ++e)
+    if (pair[e]) atomicAdd(sh.hist + bin[e], 1);
+  __syncthreads();
+  constexpr int kPer = kBins / kThreads;
+  int c[kPer], sum = 0;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) sum += c[e] = sh.hist[threadIdx.x * kPer + e];
+  Sums all;
+  int at = sums_before(Sums{sum, 0.f, 0.f}, sh, &all).n;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    sh.hist[threadIdx.x * kPer + e] = at;
+    at += c[e];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < kPlaces; ++e) {
+    start[e] = sh.hist[bin[e]];
+    end[e] = bin[e] + 1 < kBins ? sh.hist[bin[e] + 1] : n;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < kPlaces; ++e) slot[e] = pair[e] ? atomicAdd(sh.hist + bin[e], 1) : 0;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < kPlaces; ++e)
+    if (pair[e]) sh.list[slot[e]] = pair[e];
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < kPlaces; ++e) {
+    slot[e] = start[e];
+    if (pair[e])
+      for (int i = start[e]; i < end[e]; ++i) slot[e] += sh.list[i] > pair[e];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < kPlaces; ++e)
+    if (pair[e]) sh.list[slot[e]] = pair[e];
+  __syncthreads();
 }
 
 // Bisection over the pairs: right for every row, some 50 passes.
+// (By value: a reference would keep the row and the team in memory, not in registers, wherever the kernel uses them.)
+struct Cut {
+  uint64_t pair;
+  int exchanges;
+};
 template <typename T, bool Staged, bool Multi>
-__device__ __noinline__ uint64_t slow_cut(const Row<T, Staged>& row, float mx, float scale, int k, float p, Team<Multi>& team) {
+__device__ __noinline__ Cut slow_cut(Row<T, Staged> row, float mx, float scale, int k, float p, Team<Multi> team) {
   auto weight = [&](float v) { return v == mx ? 1.f : ex2_approx((v - mx) * scale); };  // an infinite maximum takes all
   uint64_t best = 0;
   row.scan([&](const float* v, int i0) {
@@ -439,7 +556,7 @@ __device__ __noinline__ uint64_t slow_cut(const Row<T, Staged>& row, float mx, f
     }
     cut = lo;
   }
-  return cut;
+  return {cut, team.exchanges};
 }
 
 template <typename T, bool Staged, bool Multi>
@@ -495,50 +612,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   Best best;
   best.t = t, best.inv_t = 1.f / t;
   best.noise = a.noise + r * a.noise_ld;
-  float z = 0.f;  // weight of the kept tokens that this thread has seen
-
-  // The noise of the wanted elements of a piece.
-  const bool noise_vec = (reinterpret_cast<uintptr_t>(best.noise - row.lead) & 15) == 0;
-  auto fetch = [&](float* g, int i0, auto wanted) {
-    if (noise_vec && i0 >= 0 && i0 + kVec <= a.vocab) {
-#pragma unroll
-      for (int j = 0; j < kVec; j += 4) {
-        const float4 f = *reinterpret_cast<const float4*>(best.noise + i0 + j);
-        g[j] = f.x, g[j + 1] = f.y, g[j + 2] = f.z, g[j + 3] = f.w;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) g[j] = wanted(j) ? best.noise[i0 + j] : 0.f;
-    }
-  };
-  // Scores the elements of a piece whose weight is not negative.
-  auto score = [&](const float* v, const float* w, int i0) {
-    bool any = false;
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) any |= w[j] >= 0.f;
-    if (!any) return;
-    float g[kVec];
-    fetch(g, i0, [&](int j) { return w[j] >= 0.f; });
-#pragma unroll
-    for (int j = 0; j < kVec; ++j)
-      if (w[j] >= 0.f) {
-        z += w[j];
-        best.see(v[j], g[j], i0 + j);
-      }
-  };
-  // Keeps the elements of a piece that `kept` accepts and that pass min-p.
-  auto keep = [&](const float* v, int i0, auto kept) {
-    float w[kVec];
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) {
-      const float x = v[j] == mx ? 1.f : ex2_approx((v[j] - mx) * scale);
-      w[j] = kept(v[j], i0 + j) && x >= least ? x : -1.f;
-    }
-    score(v, w, i0);
-  };
-  auto finish = [&]() {
-    const uint64_t chosen = team.max(best.pair());
-    const float total = team.sum(z);
+  // `z`, summed over the threads, is added to the weight of the kept
+  auto finish = [&](float total, float z) {
+    const uint64_t chosen = team.max_and_sum(best.pair(), &z);
+    total += z;
     if (tid == 0 && team.rank == 0) {
       const int i = index_of(chosen);
       a.token[r] = i;
@@ -550,19 +627,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   };
 
   const bool cut_by_mass = p < 1.f;
-  if (!k && !cut_by_mass) {
-    // what min-p drops is far enough below this bound to be skipped by the piece
-    const float bound = least > 0.f ? mx - (0.01f - 1.0001f * log2f(least)) / scale : -3.402823466e38f;
-    row.scan_from(mx < INFINITY && scale < 1e30f ? bound : -3.402823466e38f, [&](const float* v, int i0) {
-      keep(v, i0, [&](float x, int) { return x > -INFINITY; });
-    });
-    finish();
-    return;
-  }
-
-  uint64_t cut = static_cast<uint64_t>(kKeyNegInf + 1) << kIndexBits;
-  bool settled = false;
-  if (mx < INFINITY && scale < 1e30f) {
+  float total = 0.f;  // weight of what the cut keeps
+  uint64_t cut = static_cast<uint64_t>(kKeyNegInf + 1) << kIndexBits;  // keeps all but -inf and NaN
+  bool settled = !k && !cut_by_mass;
+  if (!settled && mx < INFINITY && scale < 1e30f) {
     if (k && (k <= min(kSmallK * cluster, kMostK) || a.vocab <= kList)) {
       // the bound: the k-th largest of the threads' maxima, or a little less
       uint32_t lo = kKeyNegInf + 1;
@@ -604,7 +672,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       });
       const int n = team.gather_list();
       if (n <= kList) {
-        sort_list(sh, n);
+        sort_list(sh, n, mx, scale, 0.f, (mx - bound) * scale);
         const int have = min(n, k);
         // neighbouring places per thread
         float w[kPlaces], sum = 0.f;
@@ -617,18 +685,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           w[e] = i < have ? (v == mx ? 1.f : ex2_approx((v - mx) * scale)) : 0.f;
           sum += w[e];
         }
-        float before = block_before(sum, sh.red.f32);
-        const float limit = cut_by_mass ? p * block_sum(sum, sh) : INFINITY;
+        Sums all;
+        float before = sums_before(Sums{0, sum, 0.f}, sh, &all).hi;
+        const float limit = cut_by_mass ? p * all.hi : INFINITY;
+        float z = 0.f;
 #pragma unroll
         for (int e = 0; e < kPlaces; ++e) {
           const int i = kPlaces * tid + e;
-          if (team.rank == 0 && i < have && (i == 0 || before < limit) && w[e] >= least) {
+          if (i < have && (i == 0 || before < limit) && w[e] >= least) {
             z += w[e];
             best.see(logit_of(pair[e]), best.noise[index_of(pair[e])], index_of(pair[e]));
           }
           before += w[e];
         }
-        finish();
+        sums_before(Sums{0, z, 0.f}, sh, &all);  // (every block of a cluster has the whole list)
+        finish(all.hi, 0.f);
         return;
       }
     }
@@ -638,7 +709,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     bool ok = true;
     float limit = 0.f;
     for (int stage = k ? 0 : 1; stage < (cut_by_mass ? 2 : 1) && ok; ++stage) {
-      const bool by_mass = stage == 1, last = by_mass || !cut_by_mass;
+      const bool by_mass = stage == 1;
       const bool filtered = by_mass && k;  // only what top-k left
       float y0 = 0.f, y1 = kRange;
       ok = false;
@@ -708,10 +779,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           sum_lo += c[e] * lower(b, upper);
           upper *= ratio;
         }
-        if (tid == 0) sh.bin_from = kBins, sh.bin_to = kBins, sh.bin_count = 0;
-        int n = block_before(sum_c, sh.red.i32);
+        if (tid == 0) sh.bin_from = kBins, sh.bin_to = kBins - 1, sh.bin_count = 0;
+        Sums all;
+        const Sums before = sums_before(Sums{sum_c, sum_hi, sum_lo}, sh, &all);
         if (!by_mass) {
-          n += level ? above : 0;
+          int n = before.n + (level ? above : 0);
 #pragma unroll
           for (int e = 0; e < kPer; ++e) {
             if (n < k && n + c[e] >= k) sh.bin_from = sh.bin_to = tid * kPer + e, sh.bin_count = c[e];
@@ -719,25 +791,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           }
           __syncthreads();
         } else {
-          float hi = head + block_before(sum_hi, sh.red.f32), lo = head + block_before(sum_lo, sh.red.f32);
-          // from the other end too: behind a bin lie at most the upper weights of the later bins
-          const float all_hi = block_sum(sum_hi, sh);
-          float behind = level == 0 ? all_hi - (hi - head) : INFINITY;
-          const float all = level == 0 ? mass * (1.f - 2e-6f) : 0.f;
+          // The mass down to and with a bin is bounded from above and below by the weights at its bins' ends, and,
+          // where everything is counted (level 0), by the whole mass less such bounds of the bins behind it, which is
+          // far sharper where little lies behind.
+          float hi = head + before.hi, lo = head + before.lo;
+          float behind_hi = all.hi - before.hi, behind_lo = all.lo - before.lo;
+          const float slack = 3e-6f * mass;
           upper = w0;
 #pragma unroll
           for (int e = 0; e < kPer; ++e) {
             const int b = tid * kPer + e;
             hi += c[e] * upper;
             lo += c[e] * lower(b, upper);
-            behind -= c[e] * upper;
+            behind_hi -= c[e] * upper;
+            behind_lo -= c[e] * lower(b, upper);
             upper *= ratio;
-            if (c[e] && hi >= limit * (1.f - 1e-5f)) atomicMin(&sh.bin_from, b);
-            if (c[e] && (lo >= limit * (1.f + 1e-5f) || all - behind * (1.f + 1e-4f) >= limit * (1.f + 1e-5f)))
-              atomicMin(&sh.bin_to, b);
+            const float most = level ? hi : fminf(hi, mass - behind_lo * (1.f - 1e-4f));
+            const float fewest = level ? lo : fmaxf(lo, mass - behind_hi * (1.f + 1e-4f));
+            if (c[e] && most + slack >= limit) atomicMin(&sh.bin_from, b);
+            if (c[e] && fewest - slack >= limit) atomicMin(&sh.bin_to, b);
           }
-          __syncthreads();
-          if (sh.bin_to == kBins && tid == 0) sh.bin_to = kBins - 1;
           __syncthreads();
           int inside = 0;
 #pragma unroll
@@ -745,8 +818,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
             const int b = tid * kPer + e;
             if (b >= sh.bin_from && b <= sh.bin_to) inside += c[e];
           }
-          inside = block_sum(inside, sh);
-          if (tid == 0) sh.bin_count = inside;
+          inside = __reduce_add_sync(0xffffffffu, inside);
+          if (tid % 32 == 0 && inside) atomicAdd(&sh.bin_count, inside);
           __syncthreads();
         }
         const int from = sh.bin_from, to = sh.bin_to, count = sh.bin_count;
@@ -764,15 +837,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       float mass = 0.f;
       int above = 0;
       const float bound = mx - (y1 * 1.0001f + 0.01f) / scale;  // what lies below the band is skipped by the piece
-      const bool rough = by_mass && !filtered && !(least > 0.f);
-      // The usual case, top-p alone: scores by a product, of which a thread keeps the best and second best piece.
-      float near = -INFINITY, second = -INFINITY;
-      int near_at = -1;
-      if (rough) {
+      auto split = [&](auto filter, auto masses) {
         row.scan_from(bound, [&](const float* v, int i0) {
           const float2 mx2 = splat2(mx), scale2 = splat2(scale);
           float y[kVec];
-          bool any = false, band = false;
+          int in = 0;
 #pragma unroll
           for (int j = 0; j < kVec; j += 2) {
             const float2 y2 = mul2(sub2(mx2, make_float2(v[j], v[j + 1])), scale2);
@@ -780,80 +849,39 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           }
 #pragma unroll
           for (int j = 0; j < kVec; ++j) {
-            const float w = ex2_approx(-y[j]);
-            if (y[j] < y0) mass += w;
-            any |= y[j] < y0;
-            band |= y[j] >= y0 && y[j] <= y1;
+            if (filter.value && !(v[j] > -INFINITY && pair_of(key_of(v[j]), i0 + j) >= cut)) y[j] = INFINITY;
+            if (masses.value) {
+              const float w = ex2_approx(-y[j]);
+              if (y[j] < y0) mass += w;
+            } else {
+              above += y[j] < y0;
+            }
+            in += y[j] >= y0 && y[j] <= y1;
           }
-          if (band) {
+          // the last pass will want this noise
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(best.noise + min(max(i0, 0), a.vocab - 1)));
+          if (in) {  // one place in the list for all of them: the counter's answer takes long
+            int n = atomicAdd(&sh.n_mine, in);
 #pragma unroll
             for (int j = 0; j < kVec; ++j)
               if (y[j] >= y0 && y[j] <= y1) {
-                const int n = atomicAdd(&sh.n_mine, 1);
                 if (n < kList) sh.mine()[n] = pair_of(key_of(v[j]), i0 + j);
+                ++n;
               }
           }
-          if (!any) return;
-          float g[kVec], s = -INFINITY;
-          fetch(g, i0, [&](int j) { return y[j] < y0; });
-#pragma unroll
-          for (int j = 0; j < kVec; j += 2)
-            s = max3f(s, fmaf(v[j], best.inv_t, y[j] < y0 ? g[j] : -INFINITY),
-                      fmaf(v[j + 1], best.inv_t, y[j + 1] < y0 ? g[j + 1] : -INFINITY));
-          second = fmaxf(second, fminf(near, s));
-          near_at = s > near ? i0 : near_at;
-          near = fmaxf(near, s);
         });
-        // A product is off by less than `off`; a piece that comes that near the top is scored exactly, and if a
-        // thread's second best does too (or a noise is infinite or NaN), all are.
-        const float top = team.max(near);
-        const float off = 1e-6f * (fabsf(mx * best.inv_t) + y1 + fabsf(top));
-        const bool unclear = second >= top - off || !(fabsf(top) < 1e30f);
-        if (team.sum(static_cast<int>(unclear))) {
-          row.scan_from(bound, [&](const float* v, int i0) {
-            keep(v, i0, [&](float x, int) { return (mx - x) * scale < y0; });
-          });
-        } else if (near >= top - off) {
-          for (int j = 0; j < kVec; ++j)
-            if (near_at + j >= 0 && near_at + j < a.vocab) {
-              const float x = row.one(near_at + j);
-              if ((mx - x) * scale < y0) best.see(x, best.noise[near_at + j], near_at + j);
-            }
-        }
-        z = mass;
-      } else {
-        auto split = [&](auto filter) {
-          row.scan_from(bound, [&](const float* v, int i0) {
-            float w[kVec];
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) {
-              const float y = (mx - v[j]) * scale;
-              bool in = y <= y1;
-              if (filter.value) in = in && pair_of(key_of(v[j]), i0 + j) >= cut;
-              const bool over = in && y < y0;
-              const float x = ex2_approx(-y);
-              if (over) mass += x;
-              above += over;
-              w[j] = over && x >= least ? x : -1.f;
-              if (in && !over) {
-                const int n = atomicAdd(&sh.n_mine, 1);
-                if (n < kList) sh.mine()[n] = pair_of(key_of(v[j]), i0 + j);
-              }
-            }
-            if (last) score(v, w, i0);
-          });
-        };
-        if (filtered) split(Yes{});
-        else split(No{});
-      }
-      mass = team.sum(mass);
-      above = rough ? mass > 0.f : team.sum(above);  // (top-p asks only whether there is any)
+      };
+      if (filtered) split(Yes{}, Yes{});
+      else if (by_mass) split(No{}, Yes{});
+      else split(No{}, No{});
+      if (by_mass) mass = team.sum(mass);
+      else above = team.sum(above);
       const int n = team.gather_list();
       if (n > kList) {
         ok = false;
         break;
       }
-      sort_list(sh, n);
+      sort_list(sh, n, mx, scale, y0, y1);
       float w[kPlaces], sum = 0.f;
       uint64_t pair[kPlaces];
 #pragma unroll
@@ -864,41 +892,97 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         w[e] = i < n ? (v == mx ? 1.f : ex2_approx((v - mx) * scale)) : 0.f;
         sum += w[e];
       }
-      float before = mass + block_before(sum, sh.red.f32);
-      const float total = mass + block_sum(sum, sh);
-      // The first token that goes has to be in the list, and the tokens above it have to stay.
-      if (by_mass ? !(mass < limit || above == 0) || !(total >= limit * (1.f - 1e-6f)) : !(above < k && above + n >= k)) {
+      Sums all;
+      float before = mass + sums_before(Sums{0, sum, 0.f}, sh, &all).hi;
+      // What lies above the band has to stay, and the last that stays has to be in it.
+      if (by_mass ? !(mass < limit || mass == 0.f) || !(mass + all.hi >= limit * (1.f - 1e-6f)) : !(above < k && above + n >= k)) {
         ok = false;
         break;
       }
-      if (tid == 0) sh.cut = 0;
+      if (tid == 0) sh.bin_count = 0;
       __syncthreads();
+      float z = 0.f;
 #pragma unroll
       for (int e = 0; e < kPlaces; ++e) {
         const int i = kPlaces * tid + e;
-        const bool stays = i < n && (by_mass ? before < limit || above + i == 0 : above + i < k);
-        if (team.rank == 0 && stays && last && w[e] >= least) {
+        const bool stays = i < n && (by_mass ? before < limit || (mass == 0.f && i == 0) : above + i < k);
+        if (stays) {
           z += w[e];
-          best.see(logit_of(pair[e]), best.noise[index_of(pair[e])], index_of(pair[e]));
+          atomicMax(&sh.bin_count, i);
         }
-        if (!by_mass && above + i == k - 1 && i < n) sh.cut = pair[e];
         before += w[e];
       }
-      __syncthreads();
-      if (!last) cut = sh.cut;
+      sums_before(Sums{0, z, 0.f}, sh, &all);
+      cut = sh.list[sh.bin_count];
+      total = mass + all.hi;
       __syncthreads();
     }
     settled = ok;
   }
   if (!settled) {
-    z = 0.f;
-    best.index = -1, best.score = -INFINITY;
-    cut = slow_cut(row, mx, scale, k, p, team);
-    row.scan([&](const float* v, int i0) {
-      keep(v, i0, [&](float x, int i) { return x == x && pair_of(key_of(x), i) >= cut; });
-    });
+    const Cut found = slow_cut(row, mx, scale, k, p, team);
+    cut = found.pair;
+    team.exchanges = found.exchanges;
   }
-  finish();
+
+  // The best score of what is kept: by a product with 1 / T at first, of which a thread keeps the best and the second
+  // best group of four.
+  const float cut_x = logit_of(cut), next_x = value_of(static_cast<uint32_t>(cut >> kIndexBits) + 1);
+  const int cut_i = index_of(cut);
+  const bool weigh = least > 0.f || !settled || !cut_by_mass;  // min-p, or a total that is not known yet
+  // what min-p drops is far enough below this bound to be skipped by the piece
+  const float least_x = least > 0.f && mx < INFINITY && scale < 1e30f ? mx - (0.01f - 1.0001f * log2f(least)) / scale : cut_x;
+  float z = 0.f, near = -INFINITY, second = -INFINITY, widest_noise = 0.f;
+  int near_at = -1;
+  auto kept = [&](float v, int i) { return v > cut_x || (v == cut_x && i <= cut_i); };
+  auto weight = [&](float v) { return v == mx ? 1.f : ex2_approx((v - mx) * scale); };
+  auto rank = [&](auto weighs) {
+    row.scan_noise(fmaxf(cut_x, least_x), best.noise, [&](const float* x, const float* g, int i0) {
+      const float from = i0 <= cut_i ? cut_x : next_x;  // equal logits stay up to the cut's index
+      float v[4], s = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = x[j];
+      if (i0 <= cut_i && cut_i < i0 + 3) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (i0 + j > cut_i && v[j] == cut_x) v[j] = -INFINITY;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        bool in = v[j] >= from;
+        if (weighs.value) {
+          const float w = weight(v[j]);
+          in = in && w >= least;
+          if (in) z += w;
+        }
+        s = fmaxf(s, fmaf(v[j], best.inv_t, in ? g[j] : -INFINITY));
+        widest_noise = fmaxf(widest_noise, fabsf(g[j]));
+      }
+      second = fmaxf(second, fminf(near, s));
+      near_at = s > near ? i0 : near_at;
+      near = fmaxf(near, s);
+    });
+  };
+  if (weigh) rank(Flag<true>{});
+  else rank(Flag<false>{});
+  // A product is off by less than `off`; a group that comes that near the block's top is scored exactly, and if a
+  // thread's second best does too (or a score is infinite), all of the block's are.
+  const auto larger = [](float a, float b) { return fmaxf(a, b); };
+  const float top = block_reduce(near, sh.red.f32, larger);
+  const float off = 2e-6f * (fabsf(mx * best.inv_t) + fabsf(top) + block_reduce(widest_noise, sh.red.f32, larger));
+  const bool unclear = second >= top - off || !(fabsf(top) < 1e30f) || !(off < 1e30f);
+  if (__syncthreads_or(unclear)) {
+    row.scan_noise(fmaxf(cut_x, least_x), best.noise, [&](const float* v, const float* g, int i0) {
+      for (int j = 0; j < 4; ++j)
+        if (kept(v[j], i0 + j) && weight(v[j]) >= least) best.see(v[j], g[j], i0 + j);
+    });
+  } else if (near >= top - off) {
+    for (int i = max(near_at, 0); i < min(near_at + 4, a.vocab); ++i) {
+      const float v = row.one(i);
+      if (kept(v, i) && weight(v) >= least) best.see(v, best.noise[i], i);
+    }
+  }
+  finish(weigh ? 0.f : total, z);
 }
 
 template <typename T, bool Staged, bool Multi>
@@ -923,15 +1007,19 @@ static cudaError_t launch_with(const Sample& a, int cluster, int bytes, cudaStre
 
 template <typename T>
 static cudaError_t launch(const Sample& a, cudaStream_t stream) {
-  // Blocks per row: the fewest whose slices leave room for two blocks on an SM, more while the rows alone do not
-  // fill the GPU and every thread still gets two pieces.
-  auto room = [](size_t shared) { return (227 * 1024 / 2 - static_cast<int>(shared) - 1024) / 16; };  // pieces
+  // Blocks per row: as few as hold it, because what the blocks of a cluster exchange costs several microseconds a row;
+  // a block has an SM to itself while there are at most 148, then half of one.  More only while SMs are idle and a
+  // thread has over 16 pieces to go through.
+  auto room = [](size_t shared, int per_sm) { return (227 * 1024 / per_sm - static_cast<int>(shared) - 1024) / 16; };  // pieces
   const int pieces = static_cast<int>((static_cast<long long>(a.vocab) * sizeof(T) + 15) / 16 + 1);
-  int cluster = 1;
-  auto fits = [&](int c) { return (pieces + c - 1) / c <= room(c > 1 ? sizeof(Shared<true>) : sizeof(Shared<false>)); };
-  while (cluster < kMaxCluster && (!fits(cluster) || (a.rows * cluster < 148 && pieces > 2 * cluster * kThreads))) cluster *= 2;
-  const int slice = (pieces + cluster - 1) / cluster;
-  const bool staged = slice <= kChunk * kChunks;
+  int cluster = 1, slice = pieces;
+  for (;; cluster *= 2) {
+    slice = (pieces + cluster - 1) / cluster;
+    const long long blocks = static_cast<long long>(a.rows) * cluster;
+    const bool fits = slice <= room(cluster > 1 ? sizeof(Shared<true>) : sizeof(Shared<false>), blocks <= 148 ? 1 : 2);
+    if (cluster == kMaxCluster || (fits && (2 * blocks > 148 || slice <= 16 * kThreads))) break;
+  }
+  const bool staged = slice <= std::min(kChunk * kChunks, room(sizeof(Shared<true>), 1));
   if (cluster == 1) return launch_with<T, true, false>(a, 1, slice * 16, stream);
   return staged ? launch_with<T, true, true>(a, cluster, slice * 16, stream) : launch_with<T, false, true>(a, cluster, 0, stream);
 }
