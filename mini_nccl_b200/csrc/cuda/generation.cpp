@@ -323,7 +323,7 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(
   a.status = status.data_ptr<int>();
   a.o = bf16(o);
   a.lse = lse ? lse->data_ptr<float>() : nullptr;
-  const int64_t pieces = prefix::plan(a), rows = N * H;
+  const int64_t pieces = prefix::plan(a, static_cast<int>(D)), rows = N * H;
   TORCH_CHECK_VALUE(B * a.own_tiles * a.own_splits * Hk < (1ll << 31), "too many sequences times max_q_len");
   torch::Tensor part;
   if (pieces > 0) {

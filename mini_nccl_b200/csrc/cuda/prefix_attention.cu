@@ -31,6 +31,7 @@ namespace prefix {
 constexpr int kThreads = 128;
 constexpr int kKeys = 64;  // keys per tile
 constexpr int kStages = 3;
+constexpr int kTensorCoreRows = 32;  // more rows of a kv head than this go to the tensor-core kernel
 constexpr float kLn2 = 0.6931471805599453f;
 
 template <int D, int WR>
@@ -341,28 +342,57 @@ static cudaError_t launch_own(const Args& a, cudaStream_t stream) {
 template <int D>
 static cudaError_t launch_for(const Args& a, cudaStream_t stream) {
   cudaError_t e = cudaSuccess;
-  if (a.prefix_splits > 0) {
-    const int w = row_warps(a.n * a.group);
-    e = w == 1 ? launch_prefix<D, 1>(a, stream) : w == 2 ? launch_prefix<D, 2>(a, stream) : launch_prefix<D, 4>(a, stream);
-  }
-  if (e == cudaSuccess && a.own_splits > 0) {
+  if (a.own_splits > 0) {
     const int w = row_warps(a.max_q * a.group);
     e = w == 1 ? launch_own<D, 1>(a, stream) : w == 2 ? launch_own<D, 2>(a, stream) : launch_own<D, 4>(a, stream);
+  }
+  if (e == cudaSuccess && a.prefix_splits > 0) {
+    if (a.tensor_cores) {
+      e = launch_prefix_tc(a, D, stream);
+      if (a.prefix_splits == 1) return e;
+    } else {
+      const int w = row_warps(a.n * a.group);
+      e = w == 1 ? launch_prefix<D, 1>(a, stream) : w == 2 ? launch_prefix<D, 2>(a, stream) : launch_prefix<D, 4>(a, stream);
+    }
   }
   if (e != cudaSuccess) return e;
   join_kernel<D><<<ceil_div(static_cast<long long>(a.n) * a.heads, 8), 256, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
-int plan(Args& a) {
+// Splits of the tensor-core kernel: whole waves of one block per SM, each taking its tiles and a fixed part, and the
+// partial outputs written and read when there are several.
+static int tc_splits(int blocks, int tiles, long long rows, int head_dim, bool wide) {
+  const double tile_us = wide ? 1.5 : 0.8, fixed_us = 4.0;
+  int best = 1;
+  double least = 1e30;
+  for (int s = 1; s <= std::min(tiles, 64); ++s) {
+    const int per = ceil_div(tiles, s), pieces = ceil_div(tiles, per);
+    double us = ceil_div(static_cast<long long>(blocks) * pieces, 148) * (per * tile_us + fixed_us);
+    if (pieces > 1) us += 3.0 + pieces * rows * head_dim * 8 / 6.5e6;
+    if (us < least * 0.999) least = us, best = s;
+  }
+  return best;
+}
+
+int plan(Args& a, int head_dim) {
   // Two blocks fit an SM (64 KB of tiles each); split until there are about two waves of them.
   constexpr int kWant = 148 * 2 * 2;
   a.prefix_splits = a.own_splits = 0;
   if (a.prefix_len > 0) {
-    a.row_tiles = ceil_div(static_cast<long long>(a.n) * a.group, 16 * row_warps(a.n * a.group));
-    const int tiles = ceil_div(a.prefix_len, kKeys);
-    const int splits = std::max(1, std::min({tiles, 64, ceil_div(kWant, static_cast<long long>(a.row_tiles) * a.kv_heads)}));
-    a.prefix_chunk = ceil_div(tiles, splits) * kKeys;
+    const long long rows = static_cast<long long>(a.n) * a.group;
+    a.tensor_cores = head_dim != 32 && rows > kTensorCoreRows && a.scale_log2 >= 0.f && a.head_ld > 0 && a.token_ld > 0 && a.page_ld > 0;
+    if (a.tensor_cores) {
+      a.row_tiles = ceil_div(rows, 256);
+      const int tiles = ceil_div(a.prefix_len, 128);
+      const int splits = tc_splits(a.row_tiles * a.kv_heads, tiles, rows * a.kv_heads, head_dim, rows > 128);
+      a.prefix_chunk = ceil_div(tiles, splits) * 128;
+    } else {
+      a.row_tiles = ceil_div(rows, 16 * row_warps(a.n * a.group));
+      const int tiles = ceil_div(a.prefix_len, kKeys);
+      const int splits = std::max(1, std::min({tiles, 64, ceil_div(kWant, static_cast<long long>(a.row_tiles) * a.kv_heads)}));
+      a.prefix_chunk = ceil_div(tiles, splits) * kKeys;
+    }
     a.prefix_splits = ceil_div(a.prefix_len, a.prefix_chunk);
   }
   if (a.max_len > 0 && a.max_q > 0 && a.batch > 0) {
