@@ -27,6 +27,7 @@
 
 #include "common.cuh"
 #include "generation.h"
+#include "warp_mma.cuh"
 
 namespace mnb {
 
@@ -46,7 +47,7 @@ struct Smem {
   static constexpr int stages = D == 128 ? 5 : 8;
   static constexpr uint32_t q_off = 0, kv_off = 2 * q_tile;
   static constexpr uint32_t bar_off = kv_off + stages * kv_tile;
-  static constexpr int n_bars = 2 * stages + 7;
+  static constexpr int n_bars = 2 * stages + 9;
   static constexpr uint32_t total = bar_off + n_bars * 8 + 16 + 1024;
 };
 
@@ -57,7 +58,72 @@ MNB_DEVICE void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, 
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
       : "memory");
 }
+// 2^x of a pair on the FMA and integer pipes.  x = n + f with n the nearest whole number (adding and subtracting
+// 1.5 * 2^23 rounds to it; shifted left by 23 the sum's bits are n in the exponent's place, the rest shifted out) and
+// 2^f from 1 + c1 f + ... + c5 f^5, a least-squares fit of the relative error on [-1/2, 1/2] reweighted until level
+// (computed for this kernel; off by at most 1e-7).  Below -126 the result is about 2^-126 where 0 would be right.
+MNB_DEVICE float2 exp2_fma(float2 x) {
+  x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+  const float2 round = splat2(12582912.f);
+  const float2 t = add2(x, round), f = sub2(x, sub2(t, round));
+  float2 p = fma2(f, splat2(0.001326472614891827f), splat2(0.009671512991189957f));
+  p = fma2(p, f, splat2(0.05550733581185341f));
+  p = fma2(p, f, splat2(0.24022242426872253f));
+  p = fma2(p, f, splat2(0.6931470036506653f));
+  p = fma2(p, f, splat2(1.f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
+// 128 consecutive columns of this thread's TMEM lane, with one wait.
+MNB_DEVICE void tmem_ld_128(uint32_t taddr, float* out) {
+  uint32_t r[128];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t* q = r + 32 * c;
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]), "=r"(q[8]),
+          "=r"(q[9]), "=r"(q[10]), "=r"(q[11]), "=r"(q[12]), "=r"(q[13]), "=r"(q[14]), "=r"(q[15]), "=r"(q[16]),
+          "=r"(q[17]), "=r"(q[18]), "=r"(q[19]), "=r"(q[20]), "=r"(q[21]), "=r"(q[22]), "=r"(q[23]), "=r"(q[24]),
+          "=r"(q[25]), "=r"(q[26]), "=r"(q[27]), "=r"(q[28]), "=r"(q[29]), "=r"(q[30]), "=r"(q[31])
+        : "r"(taddr + 32 * c));
+  }
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  // the values exist only after the wait: no use may move above it
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    uint32_t* q = r + 16 * c;
+    asm volatile(""
+                 : "+r"(q[0]), "+r"(q[1]), "+r"(q[2]), "+r"(q[3]), "+r"(q[4]), "+r"(q[5]), "+r"(q[6]), "+r"(q[7]),
+                   "+r"(q[8]), "+r"(q[9]), "+r"(q[10]), "+r"(q[11]), "+r"(q[12]), "+r"(q[13]), "+r"(q[14]), "+r"(q[15]));
+  }
+#pragma unroll
+  for (int i = 0; i < 128; ++i) out[i] = __uint_as_float(r[i]);
+}
+MNB_DEVICE void tmem_st_8(uint32_t taddr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+// One lane of a converged warp, the same one every time: the products are issued from warp-uniform code, so their
+// descriptors stay in uniform registers (a `lane == 0` branch moved them there one by one: 110 cycles a product
+// instead of the 64 it takes).
+MNB_DEVICE bool elected() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
 MNB_DEVICE void softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// A lane's part of a row, moved at once.
+template <int N>
+struct Vec {
+  struct alignas(4 * N) type {
+    float v[N];
+  };
+};
 
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -73,7 +139,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + S::bar_off);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + S::n_bars);
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * kStages, q_full = empty0 + 8 * kStages,
-                 s_full0 = q_full + 8, p_full0 = s_full0 + 16, o_full0 = p_full0 + 16;
+                 s_full0 = q_full + 8, o_full0 = s_full0 + 16, p_full0 = o_full0 + 16;  // (p_full: two halves per stream)
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int rt = blockIdx.x % a.row_tiles;
@@ -93,7 +159,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(q_full, 256);
     for (int s = 0; s < 2; ++s) {
       mbar_init(s_full0 + 8 * s, 1);
-      mbar_init(p_full0 + 8 * s, 128);
+      mbar_init(p_full0 + 16 * s, 128);
+      mbar_init(p_full0 + 16 * s + 8, 128);
       mbar_init(o_full0 + 8 * s, 1);
     }
     fence_mbar_init();
@@ -109,151 +176,163 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;  // S_0, S_1: 128 columns each, then O_0, O_1
 
-  if (warp == 0) {
-    int pos = 0;
-    auto load = [&](const CUtensorMap* map, int tile) -> bool {
-      const int st = pos % kStages;
-      if (!mbar_wait(empty0 + 8 * st, ((pos / kStages) & 1) ^ 1, a.status)) return false;
-      ++pos;
-      const int j0 = k0 + tile * kTile;
-      const int per = min(1 << a.page_shift, kTile);  // tokens of a box
-      const int boxes = (min(kTile, k1 - j0) + per - 1) / per;
-      if (lane == 0) mbar_arrive_expect_tx(full0 + 8 * st, boxes * per * D * 2);
-      __syncwarp();
-      if (lane < boxes) {
-        const int j = j0 + lane * per;
-        int page = a.prefix_pages[j >> a.page_shift];
-        if (page < 0 || page >= a.pages) {
-          atomicCAS(a.status, 0, kErrBadIndex);
-          page = a.pages;  // outside the map: reads as zeros
+  // A softmax thread holds a row of scores: registers move there from the other four warps.  4 x 40 + 8 x 224 per
+  // lane are within the 12 x 168 of the launch.
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 0) {
+      int pos = 0;
+      auto load = [&](const CUtensorMap* map, int tile) -> bool {
+        const int st = pos % kStages;
+        if (!mbar_wait(empty0 + 8 * st, ((pos / kStages) & 1) ^ 1, a.status)) return false;
+        ++pos;
+        const int j0 = k0 + tile * kTile;
+        const int per = min(1 << a.page_shift, kTile);  // tokens of a box
+        const int boxes = (min(kTile, k1 - j0) + per - 1) / per;
+        if (lane == 0) mbar_arrive_expect_tx(full0 + 8 * st, boxes * per * D * 2);
+        __syncwarp();
+        if (lane < boxes) {
+          const int j = j0 + lane * per;
+          int page = a.prefix_pages[j >> a.page_shift];
+          if (page < 0 || page >= a.pages) {
+            atomicCAS(a.status, 0, kErrBadIndex);
+            page = a.pages;  // outside the map: reads as zeros
+          }
+  #pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+            tma_load_4d(sbase + S::kv_off + st * S::kv_tile + c * (kTile * 128) + lane * per * 128, map, c * 64, h,
+                        j & ((1 << a.page_shift) - 1), page, full0 + 8 * st);
         }
-#pragma unroll
+        return true;
+      };
+      bool ok = true;
+      if (shared) {
+        for (int t = 0; t < n_tiles && ok; ++t) ok = load(&map_k, t) && load(&map_v, t);
+      } else {
+        ok = load(&map_k, 0) && (n_tiles < 2 || load(&map_k, 1));
+        for (int t = 0; t < n_tiles && ok; ++t) ok = load(&map_v, t) && (t + 2 >= n_tiles || load(&map_k, t + 2));
+      }
+    } else if (warp == 1) {
+      int pos = 0;
+      auto wait_full = [&](int p) { return mbar_wait(full0 + 8 * (p % kStages), (p / kStages) & 1, a.status); };
+      // (adding bytes / 16 to a descriptor moves its address: the tiles lie below 256 KB, so nothing carries)
+      const uint64_t q_desc = smem_desc_sw128(sbase + S::q_off, 16, 1024);
+      const uint64_t k_desc = smem_desc_sw128(sbase + S::kv_off, 16, 1024);
+      const uint64_t v_desc = smem_desc_sw128(sbase + S::kv_off, kTile * 128, 1024);
+      auto tile_of = [&](int p) { return static_cast<uint64_t>(p % kStages) * (S::kv_tile / 16); };
+      // S_s = Q_s K^T
+      auto scores = [&](int s, int p) {
+        const uint64_t qa = q_desc + (shared ? s : 0) * (S::q_tile / 16), kb = k_desc + tile_of(p);
+        if (elected()) {
+  #pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t at = ((kk / 4) * (kTile * 128) + (kk % 4) * 32) / 16;
+            tc_mma(tmem + s * kTile, qa + at, kb + at, kIdescS, kk > 0 ? 1u : 0u);
+          }
+          tc_commit(s_full0 + 8 * s);
+        }
+        __syncwarp();
+      };
+      // O_s (+)= P_s V, the first half of the keys while the second half's probabilities are still computed
+      auto values = [&](int s, int p, int step) -> bool {
+        const uint64_t vb = v_desc + tile_of(p);
+  #pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if (!mbar_wait(p_full0 + 16 * s + 8 * half, step & 1, a.status)) return false;
+          tc_fence_after();
+          if (elected()) {
+  #pragma unroll
+            for (int kk = half * kTile / 32; kk < (half + 1) * kTile / 32; ++kk)
+              tc_mma_tmem_a(tmem + 2 * kTile + s * D, tmem + s * kTile + kk * 8, vb + kk * (2048 / 16), kIdescO,
+                            step == 0 && kk == 0 ? 0u : 1u);
+          }
+          __syncwarp();
+        }
+        return true;
+      };
+      auto done_with = [&](int p) {
+        if (elected()) tc_commit(empty0 + 8 * (p % kStages));
+        __syncwarp();
+      };
+      // rows of V past the end of the keys
+      auto clean = [&](int tile, int p) {
+        const int valid = k1 - k0 - tile * kTile;
+        if (valid >= kTile) return;
+        uint8_t* v = sm + S::kv_off + (p % kStages) * S::kv_tile;
+  #pragma unroll
         for (int c = 0; c < D / 64; ++c)
-          tma_load_4d(sbase + S::kv_off + st * S::kv_tile + c * (kTile * 128) + lane * per * 128, map, c * 64, h,
-                      j & ((1 << a.page_shift) - 1), page, full0 + 8 * st);
-      }
-      return true;
-    };
-    bool ok = true;
-    if (shared) {
-      for (int t = 0; t < n_tiles && ok; ++t) ok = load(&map_k, t) && load(&map_v, t);
-    } else {
-      ok = load(&map_k, 0) && (n_tiles < 2 || load(&map_k, 1));
-      for (int t = 0; t < n_tiles && ok; ++t) ok = load(&map_v, t) && (t + 2 >= n_tiles || load(&map_k, t + 2));
-    }
-  } else if (warp == 1) {
-    int pos = 0;
-    auto stage_of = [&](int p) { return sbase + S::kv_off + (p % kStages) * S::kv_tile; };
-    auto wait_full = [&](int p) { return mbar_wait(full0 + 8 * (p % kStages), (p / kStages) & 1, a.status); };
-    // S_s = Q_s K^T
-    auto scores = [&](int s, int p) {
-      if (lane == 0) {
-        const uint32_t qa = sbase + S::q_off + (shared ? s : 0) * S::q_tile, kb = stage_of(p);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          tc_mma(tmem + s * kTile, smem_desc_sw128(qa + (kk / 4) * (kTile * 128) + (kk % 4) * 32, 16, 1024),
-                 smem_desc_sw128(kb + (kk / 4) * (kTile * 128) + (kk % 4) * 32, 16, 1024), kIdescS, kk > 0 ? 1u : 0u);
-        tc_commit(s_full0 + 8 * s);
-      }
-    };
-    // O_s (+)= P_s V
-    auto values = [&](int s, int p, bool first) {
-      if (lane == 0) {
-        const uint32_t vb = stage_of(p);
-#pragma unroll
-        for (int kk = 0; kk < kTile / 16; ++kk)
-          tc_mma_tmem_a(tmem + 2 * kTile + s * D, tmem + s * kTile + kk * 8, smem_desc_sw128(vb + kk * 2048, kTile * 128, 1024),
-                        kIdescO, first && kk == 0 ? 0u : 1u);
-      }
-    };
-    auto done_with = [&](int p) {
-      if (lane == 0) tc_commit(empty0 + 8 * (p % kStages));
-    };
-    // rows of V past the end of the keys
-    auto clean = [&](int tile, int p) {
-      const int valid = k1 - k0 - tile * kTile;
-      if (valid >= kTile) return;
-      uint8_t* v = sm + S::kv_off + (p % kStages) * S::kv_tile;
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c)
-        for (int i = valid * 8 + lane; i < kTile * 8; i += 32)
-          *reinterpret_cast<uint4*>(v + c * (kTile * 128) + i * 16) = make_uint4(0, 0, 0, 0);
-      fence_async_smem();
-      __syncwarp();
-    };
-    bool ok = mbar_wait(q_full, 0, a.status);
-    tc_fence_after();
-    if (shared) {
-      if (ok && (ok = wait_full(pos))) {
-        scores(0, pos);
-        scores(1, pos);
-        done_with(pos++);
-      }
-      for (int t = 0; t < n_tiles && ok; ++t) {
-        const int v = pos++, k = pos;
-        const bool more = t + 1 < n_tiles;
-        if (more) ++pos;
-        if (!(ok = wait_full(v))) break;
-        clean(t, v);
-        if (!(ok = mbar_wait(p_full0, t & 1, a.status))) break;
-        tc_fence_after();
-        values(0, v, t == 0);
-        if (more) {
-          if (!(ok = wait_full(k))) break;
-          scores(0, k);
-        } else if (lane == 0) {
-          tc_commit(o_full0);
-        }
-        if (!(ok = mbar_wait(p_full0 + 8, t & 1, a.status))) break;
-        tc_fence_after();
-        values(1, v, t == 0);
-        done_with(v);
-        if (more) {
-          scores(1, k);
-          done_with(k);
-        } else if (lane == 0) {
-          tc_commit(o_full0 + 8);
-        }
-      }
-    } else {
-      for (int s = 0; s < 2 && s < n_tiles && ok; ++s)
-        if ((ok = wait_full(pos))) {
-          scores(s, pos);
+          for (int i = valid * 8 + lane; i < kTile * 8; i += 32)
+            *reinterpret_cast<uint4*>(v + c * (kTile * 128) + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_async_smem();
+        __syncwarp();
+      };
+      bool ok = mbar_wait(q_full, 0, a.status);
+      tc_fence_after();
+      if (shared) {
+        if (ok && (ok = wait_full(pos))) {
+          scores(0, pos);
+          scores(1, pos);
           done_with(pos++);
         }
-      for (int t = 0; t < n_tiles && ok; ++t) {
-        const int s = t & 1;
-        if (!(ok = wait_full(pos))) break;
-        clean(t, pos);
-        if (!(ok = mbar_wait(p_full0 + 8 * s, (t >> 1) & 1, a.status))) break;
-        tc_fence_after();
-        values(s, pos, t < 2);
-        done_with(pos++);
-        if (t + 2 < n_tiles) {
+        for (int t = 0; t < n_tiles && ok; ++t) {
+          const int v = pos++, k = pos;
+          const bool more = t + 1 < n_tiles;
+          if (more) ++pos;
+          if (!(ok = wait_full(v))) break;
+          clean(t, v);
+          if (!(ok = values(0, v, t))) break;
+          if (more) {
+            if (!(ok = wait_full(k))) break;
+            scores(0, k);
+          } else if (elected()) {
+            tc_commit(o_full0);
+          }
+          if (!(ok = values(1, v, t))) break;
+          done_with(v);
+          if (more) {
+            scores(1, k);
+            done_with(k);
+          } else if (elected()) {
+            tc_commit(o_full0 + 8);
+          }
+        }
+      } else {
+        for (int s = 0; s < 2 && s < n_tiles && ok; ++s)
+          if ((ok = wait_full(pos))) {
+            scores(s, pos);
+            done_with(pos++);
+          }
+        for (int t = 0; t < n_tiles && ok; ++t) {
+          const int s = t & 1;
           if (!(ok = wait_full(pos))) break;
-          scores(s, pos);
+          clean(t, pos);
+          if (!(ok = values(s, pos, t >> 1))) break;
           done_with(pos++);
-        } else if (lane == 0) {
-          tc_commit(o_full0 + 8 * s);
+          if (t + 2 < n_tiles) {
+            if (!(ok = wait_full(pos))) break;
+            scores(s, pos);
+            done_with(pos++);
+          } else if (elected()) {
+            tc_commit(o_full0 + 8 * s);
+          }
         }
       }
     }
-  } else if (warp >= 4) {
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int s = (warp - 4) / 4, quad = warp % 4;
     const int r = quad * 32 + lane;                 // row of the stream's tile
-    const int row = shared ? s * kTile + r : r;     // row of the block
-    auto token_of = [&](int i) { return (r0 + i) / a.group; };
-    auto head_of = [&](int i) { return h * a.group + (r0 + i) % a.group; };
     {  // Q, swizzled as TMA would leave it; rows past the last are zeros
-      const int t = threadIdx.x - 128;
-      const int q_rows = shared ? 2 * kTile : kTile;
-      for (int i = t; i < q_rows * (D / 8); i += 256) {
-        const int qr = i / (D / 8), c = i % (D / 8);
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (qr < n_rows) w = ld_v4(a.q + token_of(qr) * a.q_ld + head_of(qr) * a.q_head + c * 8);
-        const int qt = qr / kTile, x = qr % kTile;
-        st_v4(sm + S::q_off + qt * S::q_tile + (c / 8) * (kTile * 128) + x * 128 + (((c % 8) ^ (x % 8)) << 4), w);
+      constexpr int kChunks = D / 8, kStep = 256 / kChunks;  // a thread keeps its chunk and goes through the rows
+      const int c = (threadIdx.x - 128) % kChunks, end = shared ? 2 * kTile : kTile;
+      for (int i = (threadIdx.x - 128) / kChunks; i < end; i += kStep) {
+        const bool in = i < n_rows;
+        const int x = i % kTile, j = in ? r0 + i : r0;
+        cp_async16(sbase + S::q_off + (i / kTile) * S::q_tile + (c / 8) * (kTile * 128) + x * 128 + (((c % 8) ^ (x % 8)) << 4),
+                   a.q + (j / a.group) * a.q_ld + (h * a.group + j % a.group) * a.q_head + c * 8, in);
       }
+      cp_async_commit();
+      cp_async_wait_all();
       fence_async_smem();
       mbar_arrive(q_full);
     }
@@ -267,20 +346,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       tc_fence_after();
       const int valid = k1 - k0 - (shared ? t : 2 * t + s) * kTile;  // keys of this tile (or more)
-      float mx = -INFINITY;
+      float v[kTile];
+      tmem_ld_128(t_s, v);
+      if (valid < kTile) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float v[64];
-        tmem_ld_64(t_s + c * 64, v);
-        if (valid < kTile) {
-#pragma unroll
-          for (int i = 0; i < 64; ++i) mx = fmaxf(mx, c * 64 + i < valid ? v[i] : -INFINITY);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 64; i += 2) mx = max3f(mx, v[i], v[i + 1]);
-        }
+        for (int i = 0; i < kTile; ++i)
+          if (i >= valid) v[i] = -INFINITY;
       }
-      mx *= a.scale_log2;
+      float mx = v[0], mx2 = v[1];
+#pragma unroll
+      for (int i = 2; i < kTile; i += 4) {
+        mx = max3f(mx, v[i], v[i + 1]);
+        if (i + 3 < kTile) mx2 = max3f(mx2, v[i + 2], v[i + 3]);
+      }
+      mx = fmaxf(mx, mx2) * a.scale_log2;
       const bool grows = mx > m + kRescale || m == -INFINITY;
       if (__any_sync(0xffffffffu, grows)) {
         const float to = grows ? mx : m;
@@ -289,147 +368,143 @@ __global__ void __launch_bounds__(kThreads, 1)
           // every product issued so far has finished: S of this step was issued after them
 #pragma unroll
           for (int c = 0; c < D / 16; ++c) {
-            float v[16];
+            float x[16];
             uint32_t w[16];
-            tmem_ld_16(t_o + c * 16, v);
+            tmem_ld_16(t_o + c * 16, x);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[i] * alpha);
+            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(x[i] * alpha);
             tmem_st_16(t_o + c * 16, w);
           }
         }
         l *= alpha;
         m = to;
       }
-      const float base = m == -INFINITY ? 0.f : m;
-      const float2 scale2 = splat2(a.scale_log2), base2 = splat2(-base);
-      float2 sum = make_float2(0.f, 0.f);
+      const float2 scale2 = splat2(a.scale_log2), base2 = splat2(m == -INFINITY ? 0.f : -m);
+      float2 sum = make_float2(0.f, 0.f), sum2 = sum;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float v[32];
-        uint32_t w[16];
-        tmem_ld_32(t_s + c * 32, v);
+      for (int c = 0; c < 8; ++c) {
+        uint32_t w[8];
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          const float2 y = fma2(make_float2(v[i], v[i + 1]), scale2, base2);
-          float2 p = make_float2(ex2_approx(y.x), ex2_approx(y.y));
-          if (valid < kTile) {
-            if (c * 32 + i >= valid) p.x = 0.f;
-            if (c * 32 + i + 1 >= valid) p.y = 0.f;
-          }
-          sum = add2(sum, p);
+        for (int i = 0; i < 16; i += 2) {
+          const float2 y = fma2(make_float2(v[c * 16 + i], v[c * 16 + i + 1]), scale2, base2);
+          // three pairs of eight on the FMA pipe: the exponential unit alone takes as long as the products
+          const float2 p = i % 16 == 2 || i % 16 == 8 || i % 16 == 12 ? exp2_fma(y) : make_float2(ex2_approx(y.x), ex2_approx(y.y));
+          if (i & 2) sum2 = add2(sum2, p);
+          else sum = add2(sum, p);
           w[i / 2] = pack_bf16x2(p.x, p.y);
         }
-        tmem_st_16(t_s + c * 16, w);  // over columns whose scores have been read
+        tmem_st_8(t_s + c * 8, w);  // over scores that are in registers
+        if (c % 4 == 3) {
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(p_full0 + 16 * s + 8 * (c / 4));
+        }
       }
+      sum = add2(sum, sum2);
       l += sum.x + sum.y;
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(p_full0 + 8 * s);
     }
     if (ok && steps > 0) {
       ok = __all_sync(0xffffffffu, mbar_wait(o_full0 + 8 * s, 0, a.status));
       tc_fence_after();
     }
-    // Streams of the same rows meet in the ring, which nobody uses any more once both have their outputs.
-    constexpr int kPitch = D + 4;
+    // Outputs, maxima and sums pass through the ring, which nobody uses any more once both streams have theirs, so that
+    // a warp can write whole rows; streams of the same rows meet there.
+    constexpr int kPitch = D + 4, kPer = D / 32;
     float* meet = reinterpret_cast<float*>(sm + S::kv_off);
-    float2* meet_ml = reinterpret_cast<float2*>(meet + kTile * kPitch);
-    static_assert((kTile * kPitch * 4 + kTile * 8) <= S::stages * S::kv_tile, "the meeting place fits the ring");
-    if (!shared) {
-      softmax_sync();
-      if (s == 1) {
+    float2* meet_ml = reinterpret_cast<float2*>(meet + 2 * kTile * kPitch);
+    struct Row {  // where a row goes, and the factors of its parts
+      int at;
+      float top, mine, met, inv;
+    };
+    Row* info = reinterpret_cast<Row*>(meet_ml + 2 * kTile);
+    static_assert(2 * kTile * (kPitch * 4 + 8 + sizeof(Row)) <= S::stages * S::kv_tile, "the meeting place fits the ring");
+    softmax_sync();
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-          float v[16];
-          if (steps > 0) tmem_ld_16(t_o + c * 16, v);
+    for (int c = 0; c < D / 16; ++c) {
+      float v[16];
+      if (steps > 0) tmem_ld_16(t_o + c * 16, v);
 #pragma unroll
-          for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<float4*>(meet + r * kPitch + c * 16 + i) =
-                steps > 0 ? make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-        meet_ml[r] = make_float2(m, l);
-      }
-      softmax_sync();
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<float4*>(meet + (s * kTile + r) * kPitch + c * 16 + i) =
+            steps > 0 ? make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    if (ok && (shared || s == 0)) {
-      float f_mine = 1.f, f_met = 0.f;
+    meet_ml[s * kTile + r] = make_float2(m, l);
+    softmax_sync();
+    using Part = typename Vec<kPer>::type;
+    const long long rows = static_cast<long long>(a.n) * a.heads;
+    const bool alone = a.prefix_splits == 1;  // then this block joins the rows with their own keys' pieces and finishes them
+    if (const int i = s * kTile + r; i < n_rows) {  // (without `shared`, the first stream's threads)
+      const int j = r0 + i, token = j / a.group;
+      Row x{token * a.heads + h * a.group + j - token * a.group, m, 1.f, 0.f, 1.f};
       if (!shared) {
-        const float2 met = meet_ml[r];
-        const float to = fmaxf(m, met.x), base = to == -INFINITY ? 0.f : to;
-        f_mine = ex2_approx(m - base);
-        f_met = ex2_approx(met.x - base);
-        l = l * f_mine + met.y * f_met;
-        m = to;
+        const float2 other = meet_ml[kTile + i];
+        x.top = fmaxf(m, other.x);
+        const float base = x.top == -INFINITY ? 0.f : x.top;
+        x.mine = ex2_approx(m - base), x.met = ex2_approx(other.x - base);
+        l = l * x.mine + other.y * x.met;
       }
-      const bool mine = row < n_rows;
-      const long long at = static_cast<long long>(token_of(mine ? row : 0)) * a.heads + head_of(mine ? row : 0);
-      const long long rows = static_cast<long long>(a.n) * a.heads;
-      if (a.prefix_splits > 1) {
-        float* out = a.part_o + (split * rows + at) * D;
-#pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-          float v[16];
-          tmem_ld_16(t_o + c * 16, v);
-#pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            float4 o = make_float4(v[i] * f_mine, v[i + 1] * f_mine, v[i + 2] * f_mine, v[i + 3] * f_mine);
-            if (!shared) {
-              const float4 x = *reinterpret_cast<const float4*>(meet + r * kPitch + c * 16 + i);
-              o = make_float4(fmaf(x.x, f_met, o.x), fmaf(x.y, f_met, o.y), fmaf(x.z, f_met, o.z), fmaf(x.w, f_met, o.w));
-            }
-            if (mine) *reinterpret_cast<float4*>(out + c * 16 + i) = o;
-          }
-        }
-        if (mine) a.part_ml[split * rows + at] = make_float2(m, l);
-      } else {
-        // the prefix in one piece: this block joins the rows with their own keys' pieces and finishes them
-        float to = m;
-        for (int p = 1; p < 1 + a.own_splits; ++p) to = fmaxf(to, mine ? a.part_ml[p * rows + at].x : -INFINITY);
-        const float base = to == -INFINITY ? 0.f : to;
-        const float f = ex2_approx(m - base);
+      if (alone) {
+        const float prefix_top = x.top;
+        for (int p = 1; p < 1 + a.own_splits; ++p) x.top = fmaxf(x.top, a.part_ml[p * rows + x.at].x);
+        const float base = x.top == -INFINITY ? 0.f : x.top, f = ex2_approx(prefix_top - base);
         l *= f;
-        f_mine *= f;
-        f_met *= f;
-        for (int p = 1; p < 1 + a.own_splits; ++p)
-          if (mine) {
-            const float2 ml = a.part_ml[p * rows + at];
-            l = fmaf(ex2_approx(ml.x - base), ml.y, l);
-          }
-        const float inv = l > 0.f ? 1.f / l : 0.f;
-#pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-          float v[16];
-          tmem_ld_16(t_o + c * 16, v);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] *= f_mine;
-          if (!shared) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = fmaf(meet[r * kPitch + c * 16 + i], f_met, v[i]);
-          }
-          if (mine) {
-            for (int p = 1; p < 1 + a.own_splits; ++p) {
-              const float mp = a.part_ml[p * rows + at].x;
-              if (mp == -INFINITY) continue;
-              const float g = ex2_approx(mp - base);
-              const float4* x = reinterpret_cast<const float4*>(a.part_o + (p * rows + at) * D + c * 16);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float4 y = x[i];
-                v[4 * i] = fmaf(g, y.x, v[4 * i]);
-                v[4 * i + 1] = fmaf(g, y.y, v[4 * i + 1]);
-                v[4 * i + 2] = fmaf(g, y.z, v[4 * i + 2]);
-                v[4 * i + 3] = fmaf(g, y.w, v[4 * i + 3]);
-              }
-            }
-            uint4 w[2];
-            uint32_t* u = reinterpret_cast<uint32_t*>(w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) u[i] = pack_bf16x2(v[2 * i] * inv, v[2 * i + 1] * inv);
-            st_v4(a.o + at * D + c * 16, w[0]);
-            st_v4(a.o + at * D + c * 16 + 8, w[1]);
-          }
+        for (int p = 1; p < 1 + a.own_splits; ++p) {
+          const float2 ml = a.part_ml[p * rows + x.at];
+          l = fmaf(ex2_approx(ml.x - base), ml.y, l);
         }
-        if (mine && a.lse) a.lse[at] = l > 0.f ? kLn2 * (to + log2f(l)) : -INFINITY;
+        x.inv = l > 0.f ? 1.f / l : 0.f;
+        x.mine *= f * x.inv, x.met *= f * x.inv;
+        if (a.lse) a.lse[x.at] = l > 0.f ? kLn2 * (x.top + log2f(l)) : -INFINITY;
+      } else {
+        a.part_ml[split * rows + x.at] = make_float2(x.top, l);
+      }
+      info[i] = x;
+    }
+    softmax_sync();
+    constexpr int kBatch = 4;  // rows whose loads are under way together
+    for (int i0 = (warp - 4) * kBatch; i0 < n_rows; i0 += 8 * kBatch) {
+      Part o[kBatch];
+      Row x[kBatch];
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e) {
+        const int i = min(i0 + e, n_rows - 1);
+        x[e] = info[i];
+        o[e] = *reinterpret_cast<const Part*>(meet + i * kPitch + lane * kPer);
+        Part met;
+        if (!shared) met = *reinterpret_cast<const Part*>(meet + (kTile + i) * kPitch + lane * kPer);
+#pragma unroll
+        for (int d = 0; d < kPer; ++d) o[e].v[d] = o[e].v[d] * x[e].mine + (shared ? 0.f : met.v[d] * x[e].met);
+      }
+      if (!alone) {
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e)
+          if (i0 + e < n_rows) *reinterpret_cast<Part*>(a.part_o + (split * rows + x[e].at) * D + lane * kPer) = o[e];
+        continue;
+      }
+      for (int p = 1; p < 1 + a.own_splits; ++p) {
+        float top[kBatch];
+        Part y[kBatch];
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+          top[e] = a.part_ml[p * rows + x[e].at].x;
+          y[e] = *reinterpret_cast<const Part*>(a.part_o + (p * rows + x[e].at) * D + lane * kPer);
+        }
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+          const float g = top[e] == -INFINITY ? 0.f : ex2_approx(top[e] - x[e].top) * x[e].inv;
+#pragma unroll
+          for (int d = 0; d < kPer; ++d) o[e].v[d] += g > 0.f ? y[e].v[d] * g : 0.f;  // (nothing was written without keys)
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e) {
+        if (i0 + e >= n_rows) break;
+        uint32_t w[kPer / 2];
+#pragma unroll
+        for (int d = 0; d < kPer; d += 2) w[d / 2] = pack_bf16x2(o[e].v[d], o[e].v[d + 1]);
+        uint32_t* out = reinterpret_cast<uint32_t*>(a.o + static_cast<long long>(x[e].at) * D) + lane * (kPer / 2);
+        if constexpr (kPer == 4) *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+        else *out = w[0];
       }
     }
     tc_fence_before();
