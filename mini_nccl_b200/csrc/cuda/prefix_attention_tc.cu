@@ -36,7 +36,8 @@ namespace prefix {
 namespace tc {
 
 constexpr int kTile = 128;             // rows per stream and keys per tile
-constexpr int kThreads = 32 * 12;      // producer, MMA, two idle warps, two softmax warpgroups
+constexpr int kSoftmax = 512;            // threads: two warpgroups for each stream, each with half the keys of a tile
+constexpr int kThreads = 64 + kSoftmax;  // and the producer and MMA warps
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kRescale = 8.f;        // log2 units that the scores may pass the running maximum by
 
@@ -48,7 +49,9 @@ struct Smem {
   static constexpr uint32_t q_off = 0, kv_off = 2 * q_tile;
   static constexpr uint32_t bar_off = kv_off + stages * kv_tile;
   static constexpr int n_bars = 2 * stages + 9;
-  static constexpr uint32_t total = bar_off + n_bars * 8 + 16 + 1024;
+  static constexpr uint32_t max_off = bar_off + n_bars * 8 + 16;  // row maxima: [stream][half][row], bf16
+  static constexpr uint32_t total = max_off + 4 * kTile * 2 + 1024;
+  static_assert(total <= 227 * 1024, "a block's shared memory");
 };
 
 MNB_DEVICE void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -74,34 +77,6 @@ MNB_DEVICE float2 exp2_fma(float2 x) {
   return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
                      __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
-// 128 consecutive columns of this thread's TMEM lane, with one wait.
-MNB_DEVICE void tmem_ld_128(uint32_t taddr, float* out) {
-  uint32_t r[128];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    uint32_t* q = r + 32 * c;
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]), "=r"(q[8]),
-          "=r"(q[9]), "=r"(q[10]), "=r"(q[11]), "=r"(q[12]), "=r"(q[13]), "=r"(q[14]), "=r"(q[15]), "=r"(q[16]),
-          "=r"(q[17]), "=r"(q[18]), "=r"(q[19]), "=r"(q[20]), "=r"(q[21]), "=r"(q[22]), "=r"(q[23]), "=r"(q[24]),
-          "=r"(q[25]), "=r"(q[26]), "=r"(q[27]), "=r"(q[28]), "=r"(q[29]), "=r"(q[30]), "=r"(q[31])
-        : "r"(taddr + 32 * c));
-  }
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-  // the values exist only after the wait: no use may move above it
-#pragma unroll
-  for (int c = 0; c < 8; ++c) {
-    uint32_t* q = r + 16 * c;
-    asm volatile(""
-                 : "+r"(q[0]), "+r"(q[1]), "+r"(q[2]), "+r"(q[3]), "+r"(q[4]), "+r"(q[5]), "+r"(q[6]), "+r"(q[7]),
-                   "+r"(q[8]), "+r"(q[9]), "+r"(q[10]), "+r"(q[11]), "+r"(q[12]), "+r"(q[13]), "+r"(q[14]), "+r"(q[15]));
-  }
-#pragma unroll
-  for (int i = 0; i < 128; ++i) out[i] = __uint_as_float(r[i]);
-}
 MNB_DEVICE void tmem_st_8(uint32_t taddr, const uint32_t* v) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
                "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
@@ -115,7 +90,8 @@ MNB_DEVICE bool elected() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
   return one != 0;
 }
-MNB_DEVICE void softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+MNB_DEVICE void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kSoftmax) : "memory"); }
+MNB_DEVICE void stream_sync(int s) { asm volatile("bar.sync %0, %1;" ::"r"(2 + s), "n"(kSoftmax / 2) : "memory"); }
 
 // A lane's part of a row, moved at once.
 template <int N>
@@ -156,7 +132,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(full0 + 8 * s, 1);
       mbar_init(empty0 + 8 * s, 1);
     }
-    mbar_init(q_full, 256);
+    mbar_init(q_full, kSoftmax);
     for (int s = 0; s < 2; ++s) {
       mbar_init(s_full0 + 8 * s, 1);
       mbar_init(p_full0 + 16 * s, 128);
@@ -176,156 +152,150 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;  // S_0, S_1: 128 columns each, then O_0, O_1
 
-  // A softmax thread holds a row of scores: registers move there from the other four warps.  4 x 40 + 8 x 224 per
-  // lane are within the 12 x 168 of the launch.
-  if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (warp == 0) {
-      int pos = 0;
-      auto load = [&](const CUtensorMap* map, int tile) -> bool {
-        const int st = pos % kStages;
-        if (!mbar_wait(empty0 + 8 * st, ((pos / kStages) & 1) ^ 1, a.status)) return false;
-        ++pos;
-        const int j0 = k0 + tile * kTile;
-        const int per = min(1 << a.page_shift, kTile);  // tokens of a box
-        const int boxes = (min(kTile, k1 - j0) + per - 1) / per;
-        if (lane == 0) mbar_arrive_expect_tx(full0 + 8 * st, boxes * per * D * 2);
-        __syncwarp();
-        if (lane < boxes) {
-          const int j = j0 + lane * per;
-          int page = a.prefix_pages[j >> a.page_shift];
-          if (page < 0 || page >= a.pages) {
-            atomicCAS(a.status, 0, kErrBadIndex);
-            page = a.pages;  // outside the map: reads as zeros
-          }
-  #pragma unroll
-          for (int c = 0; c < D / 64; ++c)
-            tma_load_4d(sbase + S::kv_off + st * S::kv_tile + c * (kTile * 128) + lane * per * 128, map, c * 64, h,
-                        j & ((1 << a.page_shift) - 1), page, full0 + 8 * st);
+  if (warp == 0) {
+    int pos = 0;
+    auto load = [&](const CUtensorMap* map, int tile) -> bool {
+      const int st = pos % kStages;
+      if (!mbar_wait(empty0 + 8 * st, ((pos / kStages) & 1) ^ 1, a.status)) return false;
+      ++pos;
+      const int j0 = k0 + tile * kTile;
+      const int per = min(1 << a.page_shift, kTile);  // tokens of a box
+      const int boxes = (min(kTile, k1 - j0) + per - 1) / per;
+      if (lane == 0) mbar_arrive_expect_tx(full0 + 8 * st, boxes * per * D * 2);
+      __syncwarp();
+      if (lane < boxes) {
+        const int j = j0 + lane * per;
+        int page = a.prefix_pages[j >> a.page_shift];
+        if (page < 0 || page >= a.pages) {
+          atomicCAS(a.status, 0, kErrBadIndex);
+          page = a.pages;  // outside the map: reads as zeros
         }
-        return true;
-      };
-      bool ok = true;
-      if (shared) {
-        for (int t = 0; t < n_tiles && ok; ++t) ok = load(&map_k, t) && load(&map_v, t);
-      } else {
-        ok = load(&map_k, 0) && (n_tiles < 2 || load(&map_k, 1));
-        for (int t = 0; t < n_tiles && ok; ++t) ok = load(&map_v, t) && (t + 2 >= n_tiles || load(&map_k, t + 2));
-      }
-    } else if (warp == 1) {
-      int pos = 0;
-      auto wait_full = [&](int p) { return mbar_wait(full0 + 8 * (p % kStages), (p / kStages) & 1, a.status); };
-      // (adding bytes / 16 to a descriptor moves its address: the tiles lie below 256 KB, so nothing carries)
-      const uint64_t q_desc = smem_desc_sw128(sbase + S::q_off, 16, 1024);
-      const uint64_t k_desc = smem_desc_sw128(sbase + S::kv_off, 16, 1024);
-      const uint64_t v_desc = smem_desc_sw128(sbase + S::kv_off, kTile * 128, 1024);
-      auto tile_of = [&](int p) { return static_cast<uint64_t>(p % kStages) * (S::kv_tile / 16); };
-      // S_s = Q_s K^T
-      auto scores = [&](int s, int p) {
-        const uint64_t qa = q_desc + (shared ? s : 0) * (S::q_tile / 16), kb = k_desc + tile_of(p);
-        if (elected()) {
-  #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t at = ((kk / 4) * (kTile * 128) + (kk % 4) * 32) / 16;
-            tc_mma(tmem + s * kTile, qa + at, kb + at, kIdescS, kk > 0 ? 1u : 0u);
-          }
-          tc_commit(s_full0 + 8 * s);
-        }
-        __syncwarp();
-      };
-      // O_s (+)= P_s V, the first half of the keys while the second half's probabilities are still computed
-      auto values = [&](int s, int p, int step) -> bool {
-        const uint64_t vb = v_desc + tile_of(p);
-  #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (!mbar_wait(p_full0 + 16 * s + 8 * half, step & 1, a.status)) return false;
-          tc_fence_after();
-          if (elected()) {
-  #pragma unroll
-            for (int kk = half * kTile / 32; kk < (half + 1) * kTile / 32; ++kk)
-              tc_mma_tmem_a(tmem + 2 * kTile + s * D, tmem + s * kTile + kk * 8, vb + kk * (2048 / 16), kIdescO,
-                            step == 0 && kk == 0 ? 0u : 1u);
-          }
-          __syncwarp();
-        }
-        return true;
-      };
-      auto done_with = [&](int p) {
-        if (elected()) tc_commit(empty0 + 8 * (p % kStages));
-        __syncwarp();
-      };
-      // rows of V past the end of the keys
-      auto clean = [&](int tile, int p) {
-        const int valid = k1 - k0 - tile * kTile;
-        if (valid >= kTile) return;
-        uint8_t* v = sm + S::kv_off + (p % kStages) * S::kv_tile;
-  #pragma unroll
+#pragma unroll
         for (int c = 0; c < D / 64; ++c)
-          for (int i = valid * 8 + lane; i < kTile * 8; i += 32)
-            *reinterpret_cast<uint4*>(v + c * (kTile * 128) + i * 16) = make_uint4(0, 0, 0, 0);
-        fence_async_smem();
+          tma_load_4d(sbase + S::kv_off + st * S::kv_tile + c * (kTile * 128) + lane * per * 128, map, c * 64, h,
+                      j & ((1 << a.page_shift) - 1), page, full0 + 8 * st);
+      }
+      return true;
+    };
+    bool ok = true;
+    if (shared) {
+      for (int t = 0; t < n_tiles && ok; ++t) ok = load(&map_k, t) && load(&map_v, t);
+    } else {
+      ok = load(&map_k, 0) && (n_tiles < 2 || load(&map_k, 1));
+      for (int t = 0; t < n_tiles && ok; ++t) ok = load(&map_v, t) && (t + 2 >= n_tiles || load(&map_k, t + 2));
+    }
+  } else if (warp == 1) {
+    int pos = 0;
+    auto wait_full = [&](int p) { return mbar_wait(full0 + 8 * (p % kStages), (p / kStages) & 1, a.status); };
+    // (adding bytes / 16 to a descriptor moves its address: the tiles lie below 256 KB, so nothing carries)
+    const uint64_t q_desc = smem_desc_sw128(sbase + S::q_off, 16, 1024);
+    const uint64_t k_desc = smem_desc_sw128(sbase + S::kv_off, 16, 1024);
+    const uint64_t v_desc = smem_desc_sw128(sbase + S::kv_off, kTile * 128, 1024);
+    auto tile_of = [&](int p) { return static_cast<uint64_t>(p % kStages) * (S::kv_tile / 16); };
+    // S_s = Q_s K^T
+    auto scores = [&](int s, int p) {
+      const uint64_t qa = q_desc + (shared ? s : 0) * (S::q_tile / 16), kb = k_desc + tile_of(p);
+      if (elected()) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t at = ((kk / 4) * (kTile * 128) + (kk % 4) * 32) / 16;
+          tc_mma(tmem + s * kTile, qa + at, kb + at, kIdescS, kk > 0 ? 1u : 0u);
+        }
+        tc_commit(s_full0 + 8 * s);
+      }
+      __syncwarp();
+    };
+    // O_s (+)= P_s V, the first half of the keys while the second half's probabilities are still computed
+    auto values = [&](int s, int p, int step) -> bool {
+      const uint64_t vb = v_desc + tile_of(p);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (!mbar_wait(p_full0 + 16 * s + 8 * half, step & 1, a.status)) return false;
+        tc_fence_after();
+        if (elected()) {
+#pragma unroll
+          for (int kk = half * kTile / 32; kk < (half + 1) * kTile / 32; ++kk)
+            tc_mma_tmem_a(tmem + 2 * kTile + s * D, tmem + s * kTile + kk * 8, vb + kk * (2048 / 16), kIdescO,
+                          step == 0 && kk == 0 ? 0u : 1u);
+        }
         __syncwarp();
-      };
-      bool ok = mbar_wait(q_full, 0, a.status);
-      tc_fence_after();
-      if (shared) {
-        if (ok && (ok = wait_full(pos))) {
-          scores(0, pos);
-          scores(1, pos);
+      }
+      return true;
+    };
+    auto done_with = [&](int p) {
+      if (elected()) tc_commit(empty0 + 8 * (p % kStages));
+      __syncwarp();
+    };
+    // rows of V past the end of the keys
+    auto clean = [&](int tile, int p) {
+      const int valid = k1 - k0 - tile * kTile;
+      if (valid >= kTile) return;
+      uint8_t* v = sm + S::kv_off + (p % kStages) * S::kv_tile;
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c)
+        for (int i = valid * 8 + lane; i < kTile * 8; i += 32)
+          *reinterpret_cast<uint4*>(v + c * (kTile * 128) + i * 16) = make_uint4(0, 0, 0, 0);
+      fence_async_smem();
+      __syncwarp();
+    };
+    bool ok = mbar_wait(q_full, 0, a.status);
+    tc_fence_after();
+    if (shared) {
+      if (ok && (ok = wait_full(pos))) {
+        scores(0, pos);
+        scores(1, pos);
+        done_with(pos++);
+      }
+      for (int t = 0; t < n_tiles && ok; ++t) {
+        const int v = pos++, k = pos;
+        const bool more = t + 1 < n_tiles;
+        if (more) ++pos;
+        if (!(ok = wait_full(v))) break;
+        clean(t, v);
+        if (!(ok = values(0, v, t))) break;
+        if (more) {
+          if (!(ok = wait_full(k))) break;
+          scores(0, k);
+        } else if (elected()) {
+          tc_commit(o_full0);
+        }
+        if (!(ok = values(1, v, t))) break;
+        done_with(v);
+        if (more) {
+          scores(1, k);
+          done_with(k);
+        } else if (elected()) {
+          tc_commit(o_full0 + 8);
+        }
+      }
+    } else {
+      for (int s = 0; s < 2 && s < n_tiles && ok; ++s)
+        if ((ok = wait_full(pos))) {
+          scores(s, pos);
           done_with(pos++);
         }
-        for (int t = 0; t < n_tiles && ok; ++t) {
-          const int v = pos++, k = pos;
-          const bool more = t + 1 < n_tiles;
-          if (more) ++pos;
-          if (!(ok = wait_full(v))) break;
-          clean(t, v);
-          if (!(ok = values(0, v, t))) break;
-          if (more) {
-            if (!(ok = wait_full(k))) break;
-            scores(0, k);
-          } else if (elected()) {
-            tc_commit(o_full0);
-          }
-          if (!(ok = values(1, v, t))) break;
-          done_with(v);
-          if (more) {
-            scores(1, k);
-            done_with(k);
-          } else if (elected()) {
-            tc_commit(o_full0 + 8);
-          }
-        }
-      } else {
-        for (int s = 0; s < 2 && s < n_tiles && ok; ++s)
-          if ((ok = wait_full(pos))) {
-            scores(s, pos);
-            done_with(pos++);
-          }
-        for (int t = 0; t < n_tiles && ok; ++t) {
-          const int s = t & 1;
+      for (int t = 0; t < n_tiles && ok; ++t) {
+        const int s = t & 1;
+        if (!(ok = wait_full(pos))) break;
+        clean(t, pos);
+        if (!(ok = values(s, pos, t >> 1))) break;
+        done_with(pos++);
+        if (t + 2 < n_tiles) {
           if (!(ok = wait_full(pos))) break;
-          clean(t, pos);
-          if (!(ok = values(s, pos, t >> 1))) break;
+          scores(s, pos);
           done_with(pos++);
-          if (t + 2 < n_tiles) {
-            if (!(ok = wait_full(pos))) break;
-            scores(s, pos);
-            done_with(pos++);
-          } else if (elected()) {
-            tc_commit(o_full0 + 8 * s);
-          }
+        } else if (elected()) {
+          tc_commit(o_full0 + 8 * s);
         }
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-    const int s = (warp - 4) / 4, quad = warp % 4;
+    const int s = (warp - 2) / 8, half = (warp - 2) / 4 % 2, quad = warp % 4;
     const int r = quad * 32 + lane;                 // row of the stream's tile
     {  // Q, swizzled as TMA would leave it; rows past the last are zeros
-      constexpr int kChunks = D / 8, kStep = 256 / kChunks;  // a thread keeps its chunk and goes through the rows
-      const int c = (threadIdx.x - 128) % kChunks, end = shared ? 2 * kTile : kTile;
-      for (int i = (threadIdx.x - 128) / kChunks; i < end; i += kStep) {
+      constexpr int kChunks = D / 8, kStep = kSoftmax / kChunks;  // a thread keeps its chunk and goes through the rows
+      const int c = (threadIdx.x - 64) % kChunks, end = shared ? 2 * kTile : kTile;
+      for (int i = (threadIdx.x - 64) / kChunks; i < end; i += kStep) {
         const bool in = i < n_rows;
         const int x = i % kTile, j = in ? r0 + i : r0;
         cp_async16(sbase + S::q_off + (i / kTile) * S::q_tile + (c / 8) * (kTile * 128) + x * 128 + (((c % 8) ^ (x % 8)) << 4),
@@ -337,35 +307,53 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_arrive(q_full);
     }
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    __nv_bfloat16* seen = reinterpret_cast<__nv_bfloat16*>(sm + S::max_off) + s * 2 * kTile + r;
     const uint32_t t_s = tmem + s * kTile + lanes, t_o = tmem + 2 * kTile + s * D + lanes;
     const int steps = shared ? n_tiles : (n_tiles - s + 1) / 2;
+    const bool padding = (shared ? s * kTile : 0) + quad * 32 >= n_rows;  // a warp without rows leaves P as it is
     float m = -INFINITY, l = 0.f;
-    bool ok = true;
     for (int t = 0; t < steps; ++t) {
-      ok = __all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * s, t & 1, a.status));
-      if (!ok) break;
+      // (a wait that gave up is in the status word; the loop goes on, because the other warps meet this one at barriers)
+      mbar_wait(s_full0 + 8 * s, t & 1, a.status);
+      __syncwarp();
       tc_fence_after();
-      const int valid = k1 - k0 - (shared ? t : 2 * t + s) * kTile;  // keys of this tile (or more)
-      float v[kTile];
-      tmem_ld_128(t_s, v);
-      if (valid < kTile) {
+      if (padding) {
+        tc_fence_before();
+        stream_sync(s);
+        mbar_arrive(p_full0 + 16 * s + 8 * half);
+        continue;
+      }
+      const int valid = k1 - k0 - (shared ? t : 2 * t + s) * kTile - half * 64;  // keys of this half tile (or more, or none)
+      float v[64];
+      tmem_ld_64(t_s + half * 64, v);
+      if (valid < 64) {
 #pragma unroll
-        for (int i = 0; i < kTile; ++i)
+        for (int i = 0; i < 64; ++i)
           if (i >= valid) v[i] = -INFINITY;
       }
       float mx = v[0], mx2 = v[1];
 #pragma unroll
-      for (int i = 2; i < kTile; i += 4) {
+      for (int i = 2; i < 64; i += 4) {
         mx = max3f(mx, v[i], v[i + 1]);
-        if (i + 3 < kTile) mx2 = max3f(mx2, v[i + 2], v[i + 3]);
+        if (i + 3 < 64) mx2 = max3f(mx2, v[i + 2], v[i + 3]);
       }
-      mx = fmaxf(mx, mx2) * a.scale_log2;
+      mx = fmaxf(mx, mx2);
+      // The halves' maxima meet, rounded up to bf16: any base that both use will do.  Past this barrier both halves'
+      // scores are in registers, so P may go over them.  (Each step's places are free again: its S was issued after both
+      // halves of the last step had read theirs and written P.)
+      const __nv_bfloat16 up = __float2bfloat16_ru(mx * a.scale_log2);
+      seen[half * kTile] = up;
+      tc_fence_before();
+      stream_sync(s);
+      tc_fence_after();
+      mx = fmaxf(bf16_to_f32(up), bf16_to_f32(seen[(half ^ 1) * kTile]));
       const bool grows = mx > m + kRescale || m == -INFINITY;
       if (__any_sync(0xffffffffu, grows)) {
         const float to = grows ? mx : m;
         const float alpha = ex2_approx(m - (to == -INFINITY ? 0.f : to));
-        if (t > 0) {
-          // every product issued so far has finished: S of this step was issued after them
+        if (t > 0 && half == 0) {
+          // The first half's threads rescale O: the products of this step wait for their probabilities.  Every product
+          // issued so far has finished: S of this step was issued after them.
 #pragma unroll
           for (int c = 0; c < D / 16; ++c) {
             float x[16];
@@ -380,31 +368,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         m = to;
       }
       const float2 scale2 = splat2(a.scale_log2), base2 = splat2(m == -INFINITY ? 0.f : -m);
-      float2 sum = make_float2(0.f, 0.f), sum2 = sum;
+      float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
+      for (int c = 0; c < 4; ++c) {
         uint32_t w[8];
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
           const float2 y = fma2(make_float2(v[c * 16 + i], v[c * 16 + i + 1]), scale2, base2);
-          // three pairs of eight on the FMA pipe: the exponential unit alone takes as long as the products
-          const float2 p = i % 16 == 2 || i % 16 == 8 || i % 16 == 12 ? exp2_fma(y) : make_float2(ex2_approx(y.x), ex2_approx(y.y));
-          if (i & 2) sum2 = add2(sum2, p);
-          else sum = add2(sum, p);
+          // one pair of eight on the FMA pipe: the exponential unit alone takes as long as the products (none of eight
+          // measured 3 % slower, two equal)
+          const float2 p = i == 6 ? exp2_fma(y) : make_float2(ex2_approx(y.x), ex2_approx(y.y));
+          sum = add2(sum, p);
           w[i / 2] = pack_bf16x2(p.x, p.y);
         }
-        tmem_st_8(t_s + c * 8, w);  // over scores that are in registers
-        if (c % 4 == 3) {
-          tmem_st_wait();
-          tc_fence_before();
-          mbar_arrive(p_full0 + 16 * s + 8 * (c / 4));
-        }
+        tmem_st_8(t_s + half * 32 + c * 8, w);
       }
-      sum = add2(sum, sum2);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(p_full0 + 16 * s + 8 * half);
       l += sum.x + sum.y;
     }
-    if (ok && steps > 0) {
-      ok = __all_sync(0xffffffffu, mbar_wait(o_full0 + 8 * s, 0, a.status));
+    if (steps > 0) {
+      mbar_wait(o_full0 + 8 * s, 0, a.status);
+      __syncwarp();
       tc_fence_after();
     }
     // Outputs, maxima and sums pass through the ring, which nobody uses any more once both streams have theirs, so that
@@ -417,10 +403,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       float top, mine, met, inv;
     };
     Row* info = reinterpret_cast<Row*>(meet_ml + 2 * kTile);
-    static_assert(2 * kTile * (kPitch * 4 + 8 + sizeof(Row)) <= S::stages * S::kv_tile, "the meeting place fits the ring");
+    float* meet_l = reinterpret_cast<float*>(info + 2 * kTile);  // the second half's sums
+    static_assert(2 * kTile * (kPitch * 4 + 8 + sizeof(Row) + 4) <= S::stages * S::kv_tile, "the meeting place fits the ring");
     softmax_sync();
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
+    for (int c = half * D / 32; c < (half + 1) * D / 32; ++c) {
       float v[16];
       if (steps > 0) tmem_ld_16(t_o + c * 16, v);
 #pragma unroll
@@ -428,12 +415,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         *reinterpret_cast<float4*>(meet + (s * kTile + r) * kPitch + c * 16 + i) =
             steps > 0 ? make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    meet_ml[s * kTile + r] = make_float2(m, l);
+    if (half == 1) meet_l[s * kTile + r] = l;
+    softmax_sync();
+    if (half == 0) {
+      l += meet_l[s * kTile + r];
+      meet_ml[s * kTile + r] = make_float2(m, l);
+    }
     softmax_sync();
     using Part = typename Vec<kPer>::type;
     const long long rows = static_cast<long long>(a.n) * a.heads;
     const bool alone = a.prefix_splits == 1;  // then this block joins the rows with their own keys' pieces and finishes them
-    if (const int i = s * kTile + r; i < n_rows) {  // (without `shared`, the first stream's threads)
+    if (const int i = s * kTile + r; i < n_rows && half == 0) {  // (without `shared`, the first stream's threads)
       const int j = r0 + i, token = j / a.group;
       Row x{token * a.heads + h * a.group + j - token * a.group, m, 1.f, 0.f, 1.f};
       if (!shared) {
@@ -461,8 +453,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       info[i] = x;
     }
     softmax_sync();
-    constexpr int kBatch = 4;  // rows whose loads are under way together
-    for (int i0 = (warp - 4) * kBatch; i0 < n_rows; i0 += 8 * kBatch) {
+    constexpr int kBatch = 2;  // rows whose loads are under way together
+    for (int i0 = (warp - 2) * kBatch; i0 < n_rows; i0 += kSoftmax / 32 * kBatch) {
       Part o[kBatch];
       Row x[kBatch];
 #pragma unroll
