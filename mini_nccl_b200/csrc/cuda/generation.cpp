@@ -268,6 +268,9 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(
   TORCH_CHECK_VALUE(N == 0 || rows_aligned(q), "q: last axis contiguous, rows 16-byte aligned");
   TORCH_CHECK_VALUE(pages == 0 || (rows_aligned(k_pages) && rows_aligned(v_pages)),
                     "pages: last axis contiguous, rows 16-byte aligned");
+  for (int64_t i = 0; i < 3; ++i)
+    TORCH_CHECK_VALUE(k_pages.size(i) <= 1 || (k_pages.stride(i) > 0 && k_pages.stride(i) < (1ll << 39)),
+                      "pages: an axis with a stride that a tensor map cannot hold (expanded?)");
   check_int32(prefix_pages, 1, q, "prefix_pages");
   check_int32(page_table, 2, q, "page_table");
   check_int32(seq_lens, 1, q, "seq_lens");

@@ -3,6 +3,7 @@
 // fills these in.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -105,6 +106,7 @@ struct Args {
   float scale_log2;  // the scores' factor times log2(e)
   // the pieces (plan)
   bool tensor_cores;  // the prefix by prefix_attention_tc.cu
+  int tile_rows;      // rows that a block of the other kernel takes at once
   int row_tiles, prefix_splits, prefix_chunk;
   int own_tiles, own_splits, own_chunk;
   float* part_o;    // [pieces][n][heads][head_dim]
@@ -117,7 +119,7 @@ struct Args {
 // Splits the keys into pieces; returns how many partial results each row gets.
 int plan(Args& a, int head_dim);
 // head dims 64 and 128; with one prefix piece, joins the rows and finishes them
-cudaError_t launch_prefix_tc(const Args& a, int head_dim, cudaStream_t stream);
+cudaError_t launch_prefix_tc(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, int head_dim, cudaStream_t stream);
 cudaError_t launch_attention(const Args& a, int head_dim, cudaStream_t stream);
 
 }  // namespace prefix

@@ -12,13 +12,21 @@
 // own keys are another part, and both are split along the keys into enough
 // pieces to fill the GPU.  A second kernel joins the pieces.
 //
-// Decoding is bound by the bytes of keys and values; one block keeps two
-// 64-key tiles of K and V in flight with cp.async while warps work on a third
-// (mma.sync m16n8k16, scores and probabilities in registers).  Query rows of
-// the heads of one kv head (grouped heads) share a tile of 16, 32 or 64 rows.
+// Decoding is bound by the bytes of keys and values.  Blocks of four working
+// warps and a loading one go through a list of pieces: the loading warp fills
+// a ring of 64-key stages of K and V through a TMA map of the pool (page by
+// page, 128-byte swizzle), on into the next piece while the others still work
+// on this one, so loads never wait for a piece to end.  The working warps hold
+// scores and probabilities in registers (mma.sync m16n8k16); the query rows of
+// the heads of one kv head (grouped heads) share a tile of 16, 32 or 64 rows,
+// and warps without rows of their own split the keys of a stage.
 // Scores, maxima, sums and outputs are fp32; only the probabilities are
-// rounded to bf16, as the operand of the product with V.
+// rounded to bf16, as the operand of the product with V.  Many rows go to the
+// tensor-core kernel of prefix_attention_tc.cu, which follows the same scheme.
+#include <cudaTypedefs.h>
+
 #include <algorithm>
+#include <mutex>
 
 #include "common.cuh"
 #include "generation.h"
@@ -28,335 +36,405 @@ namespace mnb {
 
 namespace prefix {
 
-constexpr int kThreads = 128;
-constexpr int kKeys = 64;  // keys per tile
-constexpr int kStages = 3;
+constexpr int kWorkers = 128;
+constexpr int kThreads = kWorkers + 32;
+constexpr int kKeys = 64;            // keys per stage
 constexpr int kTensorCoreRows = 32;  // more rows of a kv head than this go to the tensor-core kernel
 constexpr float kLn2 = 0.6931471805599453f;
 
-template <int D, int WR>
-struct Smem {
-  static constexpr int rows = 16 * WR;
-  static constexpr uint32_t q_bytes = rows * D * 2;
-  static constexpr uint32_t tile = kKeys * D * 2;
-  static constexpr uint32_t total = q_bytes + kStages * 2 * tile;
+template <int D>
+struct Ring {
+  static constexpr int stages = D == 128 ? 2 : D == 64 ? 3 : 4;  // three blocks of head dim 128 fit an SM, four of 64
+  static constexpr uint32_t tile = kKeys * D * 2;                // of K; V follows
+  static constexpr uint32_t bytes = stages * 2 * tile;
+  // 16-byte chunk c of row r, as TMA's swizzle leaves it
+  MNB_DEVICE static uint32_t at(int r, int c) {
+    if (D == 32) return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+    return (c / 8) * (kKeys * 128) + r * 128 + (((c % 8) ^ (r % 8)) << 4);
+  }
 };
 
-// One piece: rows [0, n_rows) of a tile (row r is token n0 + r / group, head
-// h * group + r % group), keys [k0, k1) named by `ids`.  Row r sees all of
-// them, or (own tokens) those below limit0 + r / group.
-template <int D, int WR, bool Causal>
-MNB_DEVICE void attend(const Args& a, uint8_t* sm, int piece, int h, int n0, int r0, int n_rows, const int* ids, int k0,
-                       int k1, int limit0) {
-  using S = Smem<D, WR>;
-  constexpr int WK = 4 / WR;         // key groups: warps that share rows
-  constexpr int KW = kKeys / WK;     // keys of a tile per warp
-  constexpr int chunks = D / 8;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int wr = warp % WR, wk = warp / WR;
-  const int gq = lane / 4, tg = lane % 4;
-  const uint32_t sQ = smem_u32(sm);
-  const uint32_t sKV = sQ + S::q_bytes;
-
-  auto row_token = [&](int r) { return n0 + (r0 + r) / a.group; };
-  auto row_head = [&](int r) { return h * a.group + (r0 + r) % a.group; };
-
-  for (int i = threadIdx.x; i < S::rows * chunks; i += kThreads) {
-    const int r = i / chunks, c = i % chunks;
-    const bool ok = r < n_rows;
-    const int rr = ok ? r : 0;
-    cp_async16(sQ + swz<D>(r, c), a.q + row_token(rr) * a.q_ld + row_head(rr) * a.q_head + c * 8, ok);
-  }
-  auto load_tile = [&](int stage, int j0) {
-    const uint32_t sK = sKV + stage * 2 * S::tile, sV = sK + S::tile;
-    for (int i = threadIdx.x; i < kKeys * chunks; i += kThreads) {
-      const int r = i / chunks, c = i % chunks;
-      const int j = j0 + r;
-      bool ok = j < k1;
-      long long at = 0;
-      if (ok) {
-        const int page = ids[j >> a.page_shift];
-        ok = page >= 0 && page < a.pages;
-        if (ok)
-          at = page * a.page_ld + (j & ((1 << a.page_shift) - 1)) * a.token_ld + h * a.head_ld + c * 8;
-        else
-          atomicCAS(a.status, 0, kErrBadIndex);
-      }
-      cp_async16(sK + swz<D>(r, c), a.k + at, ok);
-      cp_async16(sV + swz<D>(r, c), a.v + at, ok);
-    }
-  };
-  const int tiles = (k1 - k0 + kKeys - 1) / kKeys;
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) {
-    if (s < tiles) load_tile(s, k0 + s * kKeys);
-    cp_async_commit();
-  }
-
-  float acc[D / 8][4];
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-  float m_r[2] = {-INFINITY, -INFINITY}, l_r[2] = {0.f, 0.f};
-  uint32_t qf[D / 16][4];
-  // keys below lim[i] are visible to this thread's row i
-  int lim[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = wr * 16 + gq + 8 * i;
-    lim[i] = Causal ? min(k1, limit0 + (r0 + r) / a.group) : k1;
-  }
-
-  for (int t = 0; t < tiles; ++t) {
-    cp_async_wait<kStages - 2>();
-    __syncthreads();
-    if (t + kStages - 1 < tiles) load_tile((t + kStages - 1) % kStages, k0 + (t + kStages - 1) * kKeys);
-    cp_async_commit();
-    if (t == 0) {
-#pragma unroll
-      for (int kc = 0; kc < D / 16; ++kc)
-        ldsm_x4(qf[kc], sQ + swz<D>(wr * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, kc * 2 + (lane >> 4)));
-    }
-    const uint32_t sK = sKV + (t % kStages) * 2 * S::tile, sV = sK + S::tile;
-    float s[KW / 8][4];
-#pragma unroll
-    for (int n = 0; n < KW / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
-    for (int kc = 0; kc < D / 16; ++kc)
-#pragma unroll
-      for (int n = 0; n < KW / 16; ++n) {
-        uint32_t b[4];
-        ldsm_x4(b, sK + swz<D>(wk * KW + n * 16 + (lane & 7) + (lane >> 4) * 8, kc * 2 + ((lane >> 3) & 1)));
-        mma_bf16(s[2 * n], qf[kc], b);
-        mma_bf16(s[2 * n + 1], qf[kc], b + 2);
-      }
-    const int j0 = k0 + t * kKeys + wk * KW + 2 * tg;
-    float mx[2] = {m_r[0], m_r[1]};
-#pragma unroll
-    for (int n = 0; n < KW / 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = j0 + n * 8 + (e & 1);
-        s[n][e] = j < lim[e >> 1] ? s[n][e] * a.scale_log2 : -INFINITY;
-        mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
-      }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-      const float base = mx[i] == -INFINITY ? 0.f : mx[i];  // no key yet: every weight is exp2(-inf) = 0
-      const float alpha = ex2_approx(m_r[i] - base);
-      m_r[i] = mx[i];
-      l_r[i] *= alpha;
-#pragma unroll
-      for (int d = 0; d < D / 8; ++d) {
-        acc[d][2 * i] *= alpha;
-        acc[d][2 * i + 1] *= alpha;
-      }
-#pragma unroll
-      for (int n = 0; n < KW / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float p = ex2_approx(s[n][2 * i + e] - base);
-          s[n][2 * i + e] = p;
-          l_r[i] += p;
-        }
-    }
-#pragma unroll
-    for (int n = 0; n < KW / 16; ++n) {
-      const uint32_t pa[4] = {pack_bf16x2(s[2 * n][0], s[2 * n][1]), pack_bf16x2(s[2 * n][2], s[2 * n][3]),
-                              pack_bf16x2(s[2 * n + 1][0], s[2 * n + 1][1]), pack_bf16x2(s[2 * n + 1][2], s[2 * n + 1][3])};
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) {
-        uint32_t b[4];
-        ldsm_x4_t(b, sV + swz<D>(wk * KW + n * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, d * 2 + (lane >> 4)));
-        mma_bf16(acc[2 * d], pa, b);
-        mma_bf16(acc[2 * d + 1], pa, b + 2);
-      }
-    }
-  }
-  cp_async_wait_all();
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    l_r[i] += __shfl_xor_sync(0xffffffffu, l_r[i], 1);
-    l_r[i] += __shfl_xor_sync(0xffffffffu, l_r[i], 2);
-  }
-  // The key groups of a row join through shared memory (the K / V stages are free now).
-  if constexpr (WK > 1) {
-    float* so = reinterpret_cast<float*>(sm + S::q_bytes);        // [4 warps][16][D + 4]
-    float2* sml = reinterpret_cast<float2*>(so + 4 * 16 * (D + 4));  // [4 warps][16]
-    static_assert(4 * 16 * (D + 4) * 4 + 4 * 16 * 8 <= kStages * 2 * S::tile, "the join fits the stages");
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = gq + 8 * i;
-      if (tg == 0) sml[warp * 16 + r] = make_float2(m_r[i], l_r[i]);
-#pragma unroll
-      for (int d = 0; d < D / 8; ++d)
-        *reinterpret_cast<float2*>(so + (warp * 16 + r) * (D + 4) + d * 8 + 2 * tg) = make_float2(acc[d][2 * i], acc[d][2 * i + 1]);
-    }
-    __syncthreads();
-    for (int x = threadIdx.x; x < n_rows * (D / 4); x += kThreads) {
-      const int r = x / (D / 4), c = x % (D / 4) * 4;
-      const int w0 = r / 16;  // warps w0 + g * WR hold this row
-      float m = -INFINITY;
-#pragma unroll
-      for (int g = 0; g < WK; ++g) m = fmaxf(m, sml[(w0 + g * WR) * 16 + r % 16].x);
-      const float base = m == -INFINITY ? 0.f : m;
-      float l = 0.f;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int g = 0; g < WK; ++g) {
-        const int at = (w0 + g * WR) * 16 + r % 16;
-        const float f = ex2_approx(sml[at].x - base);
-        const float4 p = *reinterpret_cast<const float4*>(so + at * (D + 4) + c);
-        l = fmaf(f, sml[at].y, l);
-        o.x = fmaf(f, p.x, o.x);
-        o.y = fmaf(f, p.y, o.y);
-        o.z = fmaf(f, p.z, o.z);
-        o.w = fmaf(f, p.w, o.w);
-      }
-      const long long out = (static_cast<long long>(piece) * a.n + row_token(r)) * a.heads + row_head(r);
-      *reinterpret_cast<float4*>(a.part_o + out * D + c) = o;
-      if (c == 0) a.part_ml[out] = make_float2(m, l);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = wr * 16 + gq + 8 * i;
-      if (r >= n_rows) continue;
-      const long long out = (static_cast<long long>(piece) * a.n + row_token(r)) * a.heads + row_head(r);
-#pragma unroll
-      for (int d = 0; d < D / 8; ++d)
-        *reinterpret_cast<float2*>(a.part_o + out * D + d * 8 + 2 * tg) = make_float2(acc[d][2 * i], acc[d][2 * i + 1]);
-      if (tg == 0) a.part_ml[out] = make_float2(m_r[i], l_r[i]);
-    }
-  }
+MNB_DEVICE void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
 }
+MNB_DEVICE void workers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory"); }
 
-// Prefix pieces: (split, kv head, row tile), row tiles of the same keys side by side.
-template <int D, int WR>
-__global__ void __launch_bounds__(kThreads) prefix_kernel(const __grid_constant__ Args a) {
-  extern __shared__ __align__(128) uint8_t sm[];
-  const int rt = blockIdx.x % a.row_tiles;
-  const int h = (blockIdx.x / a.row_tiles) % a.kv_heads;
-  const int split = blockIdx.x / (a.row_tiles * a.kv_heads);
-  const int r0 = rt * 16 * WR;
-  const int k0 = split * a.prefix_chunk;
-  attend<D, WR, false>(a, sm, split, h, 0, r0, min(16 * WR, a.n * a.group - r0), a.prefix_pages, k0,
-                min(a.prefix_len, k0 + a.prefix_chunk), 0);
-}
+// One piece: rows r0 .. r0 + n_rows of the rows that start at token n0 (row r is token n0 + r / group, head
+// h * group + r % group) over keys [k0, k1) in the pages `ids`.  Row r sees those below limit0 + r / group.
+struct Piece {
+  int h, n0, r0, n_rows, k0, k1, slot, limit0;
+  const int* ids;
+};
+constexpr int kUnlimited = 1 << 30;
 
-// Own pieces: (sequence, row tile, split, kv head).
-template <int D, int WR>
-__global__ void __launch_bounds__(kThreads) own_kernel(const __grid_constant__ Args a) {
-  extern __shared__ __align__(128) uint8_t sm[];
-  const int h = blockIdx.x % a.kv_heads;
-  const int split = (blockIdx.x / a.kv_heads) % a.own_splits;
-  const int rt = (blockIdx.x / (a.kv_heads * a.own_splits)) % a.own_tiles;
-  const int b = blockIdx.x / (a.kv_heads * a.own_splits * a.own_tiles);
-  int n0 = b, q_len = 1;
+MNB_DEVICE void flag(const Args& a) { atomicCAS(a.status, 0, kErrBadIndex); }
+
+// Item i of the list: first the prefix's (split, kv head, row tile; the row tiles of the same keys side by side), then
+// the sequences' own (sequence, row tile, split, kv head).
+MNB_DEVICE Piece piece_of(const Args& a, int i, int tile_rows) {
+  Piece p;
+  const int of_prefix = a.tensor_cores ? 0 : a.row_tiles * a.kv_heads * a.prefix_splits;
+  if (i < of_prefix) {
+    const int split = i / (a.row_tiles * a.kv_heads);
+    p.h = (i / a.row_tiles) % a.kv_heads;
+    p.n0 = 0;
+    p.r0 = (i % a.row_tiles) * tile_rows;
+    p.n_rows = min(tile_rows, a.n * a.group - p.r0);
+    p.k0 = split * a.prefix_chunk;
+    p.k1 = min(a.prefix_len, p.k0 + a.prefix_chunk);
+    p.slot = split;
+    p.limit0 = kUnlimited;
+    p.ids = a.prefix_pages;
+    return p;
+  }
+  i -= of_prefix;
+  p.h = i % a.kv_heads;
+  const int split = (i / a.kv_heads) % a.own_splits;
+  const int rt = (i / (a.kv_heads * a.own_splits)) % a.own_tiles;
+  const int b = i / (a.kv_heads * a.own_splits * a.own_tiles);
+  p.n0 = b;
+  int q_len = 1;
   if (a.q_offsets) {
-    n0 = min(max(a.q_offsets[b], 0), a.n);
-    q_len = min(max(a.q_offsets[b + 1] - n0, 0), a.n - n0);
+    p.n0 = min(max(a.q_offsets[b], 0), a.n);
+    q_len = min(max(a.q_offsets[b + 1] - p.n0, 0), a.n - p.n0);
     if (q_len > a.max_q) {
-      if (threadIdx.x == 0) atomicCAS(a.status, 0, kErrBadIndex);
+      flag(a);
       q_len = a.max_q;
     }
   }
-  const int r0 = rt * 16 * WR;
-  const int n_rows = min(16 * WR, q_len * a.group - r0);
-  if (n_rows <= 0) return;
+  p.r0 = rt * tile_rows;
+  p.n_rows = min(tile_rows, q_len * a.group - p.r0);
   int len = a.seq_lens[b];
   if (len < 0 || len > a.max_len) {
-    if (threadIdx.x == 0) atomicCAS(a.status, 0, kErrBadIndex);
+    flag(a);
     len = min(max(len, 0), a.max_len);
   }
-  const int k0 = split * a.own_chunk;
+  p.limit0 = len - q_len + 1;
+  p.k0 = split * a.own_chunk;
   // the newest row of the tile sees the most keys
-  const int seen = max(0, len - q_len + 1 + (r0 + n_rows - 1) / a.group);
-  const int k1 = min(min(len, seen), k0 + a.own_chunk);
-  const int piece = a.prefix_splits + split;
-  if (k1 <= k0) {  // nothing here: the join skips the piece
-    for (int r = threadIdx.x; r < n_rows; r += kThreads)
-      a.part_ml[(static_cast<long long>(piece) * a.n + n0 + (r0 + r) / a.group) * a.heads + h * a.group + (r0 + r) % a.group] =
-          make_float2(-INFINITY, 0.f);
-    return;
-  }
-  attend<D, WR, true>(a, sm, piece, h, n0, r0, n_rows, a.page_table + b * a.table_ld, k0, k1, len - q_len + 1);
+  p.k1 = p.n_rows > 0 ? min(min(len, max(0, p.limit0 + (p.r0 + p.n_rows - 1) / a.group)), p.k0 + a.own_chunk) : p.k0;
+  p.slot = a.prefix_splits + split;
+  p.ids = a.page_table + b * a.table_ld;
+  return p;
 }
 
-// One warp joins the pieces of one (token, head).
+// WR: warps that take rows of their own (16 each); the 4 / WR groups of warps split the keys of a stage.
+template <int D, int WR>
+__global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
+    pieces_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap map_k,
+                  const __grid_constant__ CUtensorMap map_v, int items, int join_rows) {
+  using R = Ring<D>;
+  constexpr int WK = 4 / WR, KW = kKeys / WK, kStages = R::stages, kPitch = D + 4;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t bars[2 * kStages];
+  const uint32_t ring = smem_u32(sm), full0 = smem_u32(bars), empty0 = full0 + 8 * kStages;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full0 + 8 * s, 1);
+      mbar_init(empty0 + 8 * s, 4);
+    }
+    fence_mbar_init();
+  }
+  __syncthreads();
+  int pos = 0;  // stages filled, or used, so far
+
+  if (warp == 4) {
+    const int per = min(1 << a.page_shift, kKeys);  // tokens of a box
+    for (int i = blockIdx.x; i < items; i += gridDim.x) {
+      const Piece p = piece_of(a, i, 16 * WR);
+      for (int j0 = p.k0; j0 < p.k1; j0 += kKeys, ++pos) {
+        const int st = pos % kStages, boxes = (min(kKeys, p.k1 - j0) + per - 1) / per;
+        int page = 0;
+        const int j = j0 + lane * per;
+        if (lane < boxes) {
+          page = p.ids[j >> a.page_shift];
+          if (page < 0 || page >= a.pages) {
+            flag(a);
+            page = a.pages;  // outside the map: reads as zeros
+          }
+        }
+        if (!mbar_wait(empty0 + 8 * st, ((pos / kStages) & 1) ^ 1, a.status)) return;
+        if (lane == 0) mbar_arrive_expect_tx(full0 + 8 * st, boxes * per * D * 4);
+        __syncwarp();
+        if (lane < boxes) {
+          const uint32_t to = ring + st * 2 * R::tile + lane * per * (D == 32 ? 64 : 128);
+#pragma unroll
+          for (int c = 0; c < (D + 63) / 64; ++c) {
+            const int token = j & ((1 << a.page_shift) - 1);
+            tma_load_4d(to + c * (kKeys * 128), &map_k, c * 64, p.h, token, page, full0 + 8 * st);
+            tma_load_4d(to + R::tile + c * (kKeys * 128), &map_v, c * 64, p.h, token, page, full0 + 8 * st);
+          }
+        }
+      }
+    }
+    return;
+  }
+
+  const int wr = warp % WR, wk = warp / WR, gq = lane / 4, tg = lane % 4;
+  for (int i = blockIdx.x; i < items; i += gridDim.x) {
+    const Piece p = piece_of(a, i, 16 * WR);
+    if (p.n_rows <= 0) continue;
+    auto out_of = [&](int r) {
+      const int j = p.r0 + r, token = j / a.group;
+      return (static_cast<long long>(p.slot) * a.n + p.n0 + token) * a.heads + p.h * a.group + j - token * a.group;
+    };
+    if (p.k1 <= p.k0) {  // nothing here: the join skips the piece
+      for (int r = threadIdx.x; r < p.n_rows; r += kWorkers) a.part_ml[out_of(r)] = make_float2(-INFINITY, 0.f);
+      continue;
+    }
+    // Q as the products' first operand, straight from memory
+    uint32_t qf[D / 16][4];
+    int lim[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = wr * 16 + gq + 8 * e, j = p.r0 + r, token = j / a.group;
+      const bool in = r < p.n_rows;
+      lim[e] = min(p.k1, p.limit0 + token);
+      const __nv_bfloat16* q = a.q + (p.n0 + token) * a.q_ld + (p.h * a.group + j - token * a.group) * a.q_head + 2 * tg;
+#pragma unroll
+      for (int kc = 0; kc < D / 16; ++kc) {
+        qf[kc][e] = in ? *reinterpret_cast<const uint32_t*>(q + kc * 16) : 0u;
+        qf[kc][e + 2] = in ? *reinterpret_cast<const uint32_t*>(q + kc * 16 + 8) : 0u;
+      }
+    }
+    float acc[D / 8][4];
+#pragma unroll
+    for (int d = 0; d < D / 8; ++d) acc[d][0] = acc[d][1] = acc[d][2] = acc[d][3] = 0.f;
+    float m_r[2] = {-INFINITY, -INFINITY}, l_r[2] = {0.f, 0.f};
+
+    for (int t0 = p.k0; t0 < p.k1; t0 += kKeys, ++pos) {
+      const int st = pos % kStages;
+      mbar_wait(full0 + 8 * st, (pos / kStages) & 1, a.status);  // (a wait that gave up is in the status word)
+      __syncwarp();
+      const uint32_t sK = ring + st * 2 * R::tile, sV = sK + R::tile;
+      const bool part = p.k1 - t0 < kKeys;
+      if (part) {  // V rows past the end hold anything: this warp's become zeros
+        for (int x = lane; x < KW * (D / 8); x += 32) {
+          const int r = wk * KW + x / (D / 8);
+          if (t0 + r >= p.k1) st_v4(sm + st * 2 * R::tile + R::tile + R::at(r, x % (D / 8)), make_uint4(0, 0, 0, 0));
+        }
+        __syncwarp();
+      }
+      float s[KW / 8][4];
+#pragma unroll
+      for (int n = 0; n < KW / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+      for (int kc = 0; kc < D / 16; ++kc)
+#pragma unroll
+        for (int n = 0; n < KW / 16; ++n) {
+          uint32_t b[4];
+          ldsm_x4(b, sK + R::at(wk * KW + n * 16 + (lane & 7) + (lane >> 4) * 8, kc * 2 + ((lane >> 3) & 1)));
+          mma_bf16(s[2 * n], qf[kc], b);
+          mma_bf16(s[2 * n + 1], qf[kc], b + 2);
+        }
+      const int j0 = t0 + wk * KW + 2 * tg;
+      float mx[2] = {m_r[0], m_r[1]};
+#pragma unroll
+      for (int n = 0; n < KW / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = j0 + n * 8 + (e & 1);
+          s[n][e] = j < lim[e >> 1] ? s[n][e] * a.scale_log2 : -INFINITY;
+          mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
+        }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
+        mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
+        const float base = mx[e] == -INFINITY ? 0.f : mx[e];  // no key yet: every weight is exp2(-inf) = 0
+        const float alpha = ex2_approx(m_r[e] - base);
+        m_r[e] = mx[e];
+        l_r[e] *= alpha;
+#pragma unroll
+        for (int d = 0; d < D / 8; ++d) {
+          acc[d][2 * e] *= alpha;
+          acc[d][2 * e + 1] *= alpha;
+        }
+#pragma unroll
+        for (int n = 0; n < KW / 8; ++n)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float w = ex2_approx(s[n][2 * e + x] - base);
+            s[n][2 * e + x] = w;
+            l_r[e] += w;
+          }
+      }
+#pragma unroll
+      for (int n = 0; n < KW / 16; ++n) {
+        const uint32_t pa[4] = {pack_bf16x2(s[2 * n][0], s[2 * n][1]), pack_bf16x2(s[2 * n][2], s[2 * n][3]),
+                                pack_bf16x2(s[2 * n + 1][0], s[2 * n + 1][1]), pack_bf16x2(s[2 * n + 1][2], s[2 * n + 1][3])};
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+          uint32_t b[4];
+          ldsm_x4_t(b, sV + R::at(wk * KW + n * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, d * 2 + (lane >> 4)));
+          mma_bf16(acc[2 * d], pa, b);
+          mma_bf16(acc[2 * d + 1], pa, b + 2);
+        }
+      }
+      if (part) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // TMA writes over the zeros next
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty0 + 8 * st);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      l_r[e] += __shfl_xor_sync(0xffffffffu, l_r[e], 1);
+      l_r[e] += __shfl_xor_sync(0xffffffffu, l_r[e], 2);
+    }
+    if constexpr (WK > 1) {
+      // the key groups of a row join through shared memory
+      float* so = reinterpret_cast<float*>(sm + R::bytes);                     // [WK][join_rows][kPitch]
+      float2* sml = reinterpret_cast<float2*>(so + WK * join_rows * kPitch);  // [WK][join_rows]
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = wr * 16 + gq + 8 * e;
+        if (r >= p.n_rows) continue;
+        if (tg == 0) sml[wk * join_rows + r] = make_float2(m_r[e], l_r[e]);
+#pragma unroll
+        for (int d = 0; d < D / 8; ++d)
+          *reinterpret_cast<float2*>(so + (wk * join_rows + r) * kPitch + d * 8 + 2 * tg) = make_float2(acc[d][2 * e], acc[d][2 * e + 1]);
+      }
+      workers_sync();
+      for (int x = threadIdx.x; x < p.n_rows * (D / 4); x += kWorkers) {
+        const int r = x / (D / 4), c = x % (D / 4) * 4;
+        float m = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < WK; ++g) m = fmaxf(m, sml[g * join_rows + r].x);
+        const float base = m == -INFINITY ? 0.f : m;
+        float l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int g = 0; g < WK; ++g) {
+          const float2 ml = sml[g * join_rows + r];
+          const float f = ex2_approx(ml.x - base);
+          const float4 v = *reinterpret_cast<const float4*>(so + (g * join_rows + r) * kPitch + c);
+          l = fmaf(f, ml.y, l);
+          o = make_float4(fmaf(f, v.x, o.x), fmaf(f, v.y, o.y), fmaf(f, v.z, o.z), fmaf(f, v.w, o.w));
+        }
+        const long long out = out_of(r);
+        *reinterpret_cast<float4*>(a.part_o + out * D + c) = o;
+        if (c == 0) a.part_ml[out] = make_float2(m, l);
+      }
+      workers_sync();
+    } else {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = wr * 16 + gq + 8 * e;
+        if (r >= p.n_rows) continue;
+        const long long out = out_of(r);
+#pragma unroll
+        for (int d = 0; d < D / 8; ++d)
+          *reinterpret_cast<float2*>(a.part_o + out * D + d * 8 + 2 * tg) = make_float2(acc[d][2 * e], acc[d][2 * e + 1]);
+        if (tg == 0) a.part_ml[out] = make_float2(m_r[e], l_r[e]);
+      }
+    }
+  }
+}
+
+// One block joins the pieces of one (token, head), its warps taking them in turn.
 template <int D>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args a) {
-  const long long row = blockIdx.x * 8ll + threadIdx.x / 32;
-  const int lane = threadIdx.x % 32;
-  const long long rows = static_cast<long long>(a.n) * a.heads;
-  if (row >= rows) return;
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args a) {
+  constexpr int kPer = D / 32;
+  __shared__ float so[4][D];
+  __shared__ float sl[4];
+  const long long row = blockIdx.x, rows = static_cast<long long>(a.n) * a.heads;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int pieces = a.prefix_splits + a.own_splits;
   float m = -INFINITY;
   for (int p = lane; p < pieces; p += 32) m = fmaxf(m, a.part_ml[p * rows + row].x);
   m = warp_max(m);
   const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  constexpr int per = D / 32;
-  float o[per];
-#pragma unroll
-  for (int i = 0; i < per; ++i) o[i] = 0.f;
-  for (int p = 0; p < pieces; ++p) {
+  float l = 0.f, o[kPer] = {};
+#pragma unroll 4
+  for (int p = warp; p < pieces; p += 4) {
     const float2 ml = a.part_ml[p * rows + row];
-    if (ml.x == -INFINITY) continue;
     const float f = ex2_approx(ml.x - base);
     l = fmaf(f, ml.y, l);
-    const float* po = a.part_o + (p * rows + row) * D + lane * per;
+    const float* po = a.part_o + (p * rows + row) * D + lane * kPer;
 #pragma unroll
-    for (int i = 0; i < per; ++i) o[i] = fmaf(f, po[i], o[i]);
+    for (int i = 0; i < kPer; ++i) o[i] = fmaf(f, ml.x == -INFINITY ? 0.f : po[i], o[i]);  // (a piece without keys is not written)
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;  // a row without keys is zero
 #pragma unroll
-  for (int i = 0; i < per; ++i) a.o[row * D + lane * per + i] = f32_to_bf16(o[i] * inv);
-  if (a.lse && lane == 0) a.lse[row] = l > 0.f ? kLn2 * (m + log2f(l)) : -INFINITY;
+  for (int i = 0; i < kPer; ++i) so[warp][lane * kPer + i] = o[i];
+  if (lane == 0) sl[warp] = l;
+  __syncthreads();
+  l = sl[0] + sl[1] + sl[2] + sl[3];
+  const float inv = l > 0.f ? 1.f / l : 0.f;  // a row without keys is zero
+  if (threadIdx.x < D / 2) {
+    const int c = 2 * threadIdx.x;
+    auto sum = [&](int i) { return so[0][i] + so[1][i] + so[2][i] + so[3][i]; };
+    *reinterpret_cast<uint32_t*>(a.o + row * D + c) = pack_bf16x2(sum(c) * inv, sum(c + 1) * inv);
+  }
+  if (a.lse && threadIdx.x == 0) a.lse[row] = l > 0.f ? kLn2 * (m + log2f(l)) : -INFINITY;
 }
 
 int row_warps(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 int ceil_div(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 
-template <int D, int WR>
-static cudaError_t launch_prefix(const Args& a, cudaStream_t stream) {
-  constexpr int bytes = Smem<D, WR>::total;
-  if (const cudaError_t e = cudaFuncSetAttribute(prefix_kernel<D, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-      e != cudaSuccess)
-    return e;
-  prefix_kernel<D, WR><<<a.row_tiles * a.kv_heads * a.prefix_splits, kThreads, bytes, stream>>>(a);
-  return cudaGetLastError();
+static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    cudaDriverEntryPointQueryResult q;
+    void* p = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
 }
+
+// A pool as (head_dim, heads, tokens, pages) in boxes of 64 values (or the head) and up to 64 tokens of one page.
+static bool pool_map(CUtensorMap* map, const __nv_bfloat16* base, const Args& a, int head_dim) {
+  if (!encode_fn()) return false;
+  const int page = 1 << a.page_shift;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(a.kv_heads),
+                              static_cast<cuuint64_t>(page), static_cast<cuuint64_t>(std::max(1, a.pages))};
+  // an axis of one entry may have any stride: give the map one that it accepts
+  auto stride = [](long long n, long long ld) { return static_cast<cuuint64_t>(n > 1 ? ld * 2 : 16); };
+  const cuuint64_t strides[3] = {stride(a.kv_heads, a.head_ld), stride(page, a.token_ld), stride(a.pages, a.page_ld)};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(std::min(64, head_dim)), 1, static_cast<cuuint32_t>(std::min(page, kKeys)), 1};
+  const cuuint32_t each[4] = {1, 1, 1, 1};
+  return encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<__nv_bfloat16*>(base), dims, strides, box, each,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, head_dim == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D, int WR>
-static cudaError_t launch_own(const Args& a, cudaStream_t stream) {
-  constexpr int bytes = Smem<D, WR>::total;
-  if (const cudaError_t e = cudaFuncSetAttribute(own_kernel<D, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+static cudaError_t launch_pieces(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
+  const int rows_most = std::max(a.tensor_cores ? 0 : a.n * a.group, a.own_splits > 0 ? a.max_q * a.group : 0);
+  const int join_rows = WR == 4 ? 0 : std::min(16 * WR, rows_most);
+  const int bytes = Ring<D>::bytes + (4 / WR) * join_rows * ((D + 4) * 4 + 8) + 1024;
+  const int items = (a.tensor_cores ? 0 : a.row_tiles * a.kv_heads * a.prefix_splits) +
+                    a.batch * a.own_tiles * a.own_splits * a.kv_heads;
+  if (const cudaError_t e = cudaFuncSetAttribute(pieces_kernel<D, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
       e != cudaSuccess)
     return e;
-  own_kernel<D, WR><<<a.batch * a.own_tiles * a.own_splits * a.kv_heads, kThreads, bytes, stream>>>(a);
+  const int per_sm = std::max(1, std::min(WR == 4 ? 2 : 3, 227 * 1024 / (bytes + 1024 + 64)));
+  pieces_kernel<D, WR><<<std::min(items, 148 * per_sm), kThreads, bytes, stream>>>(a, mk, mv, items, join_rows);
   return cudaGetLastError();
 }
 
 template <int D>
 static cudaError_t launch_for(const Args& a, cudaStream_t stream) {
   cudaError_t e = cudaSuccess;
-  if (a.own_splits > 0) {
-    const int w = row_warps(a.max_q * a.group);
-    e = w == 1 ? launch_own<D, 1>(a, stream) : w == 2 ? launch_own<D, 2>(a, stream) : launch_own<D, 4>(a, stream);
+  CUtensorMap mk, mv;
+  const bool by_warps = a.own_splits > 0 || (a.prefix_splits > 0 && !a.tensor_cores);
+  if (a.prefix_splits + a.own_splits > 0 && (!pool_map(&mk, a.k, a, D) || !pool_map(&mv, a.v, a, D))) return cudaErrorInvalidValue;
+  if (by_warps) {
+    const int w = a.tile_rows / 16;
+    e = w == 1 ? launch_pieces<D, 1>(a, mk, mv, stream) : w == 2 ? launch_pieces<D, 2>(a, mk, mv, stream) : launch_pieces<D, 4>(a, mk, mv, stream);
+    if (e != cudaSuccess) return e;
   }
-  if (e == cudaSuccess && a.prefix_splits > 0) {
-    if (a.tensor_cores) {
-      e = launch_prefix_tc(a, D, stream);
-      if (a.prefix_splits == 1) return e;
-    } else {
-      const int w = row_warps(a.n * a.group);
-      e = w == 1 ? launch_prefix<D, 1>(a, stream) : w == 2 ? launch_prefix<D, 2>(a, stream) : launch_prefix<D, 4>(a, stream);
-    }
+  if (a.tensor_cores && a.prefix_splits > 0) {
+    e = launch_prefix_tc(a, mk, mv, D, stream);
+    if (e != cudaSuccess || a.prefix_splits == 1) return e;
   }
-  if (e != cudaSuccess) return e;
-  join_kernel<D><<<ceil_div(static_cast<long long>(a.n) * a.heads, 8), 256, 0, stream>>>(a);
+  join_kernel<D><<<a.n * a.heads, 128, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
@@ -376,19 +454,20 @@ static int tc_splits(int blocks, int tiles, long long rows, int head_dim, bool w
 }
 
 int plan(Args& a, int head_dim) {
-  // Two blocks fit an SM (64 KB of tiles each); split until there are about two waves of them.
-  constexpr int kWant = 148 * 2 * 2;
+  // Without tensor cores, pieces until every SM has about six, so that the last ones are short against the whole.
+  constexpr int kWant = 148 * 6;
   a.prefix_splits = a.own_splits = 0;
+  const long long rows = static_cast<long long>(a.n) * a.group;
+  a.tensor_cores = a.prefix_len > 0 && head_dim != 32 && rows > kTensorCoreRows && a.scale_log2 >= 0.f;
+  a.tile_rows = 16 * row_warps(static_cast<int>(a.tensor_cores || a.prefix_len == 0 ? static_cast<long long>(a.max_q) * a.group : rows));
   if (a.prefix_len > 0) {
-    const long long rows = static_cast<long long>(a.n) * a.group;
-    a.tensor_cores = head_dim != 32 && rows > kTensorCoreRows && a.scale_log2 >= 0.f && a.head_ld > 0 && a.token_ld > 0 && a.page_ld > 0;
     if (a.tensor_cores) {
       a.row_tiles = ceil_div(rows, 256);
       const int tiles = ceil_div(a.prefix_len, 128);
       const int splits = tc_splits(a.row_tiles * a.kv_heads, tiles, rows * a.kv_heads, head_dim, rows > 128);
       a.prefix_chunk = ceil_div(tiles, splits) * 128;
     } else {
-      a.row_tiles = ceil_div(rows, 16 * row_warps(a.n * a.group));
+      a.row_tiles = ceil_div(rows, a.tile_rows);
       const int tiles = ceil_div(a.prefix_len, kKeys);
       const int splits = std::max(1, std::min({tiles, 64, ceil_div(kWant, static_cast<long long>(a.row_tiles) * a.kv_heads)}));
       a.prefix_chunk = ceil_div(tiles, splits) * kKeys;
@@ -396,7 +475,7 @@ int plan(Args& a, int head_dim) {
     a.prefix_splits = ceil_div(a.prefix_len, a.prefix_chunk);
   }
   if (a.max_len > 0 && a.max_q > 0 && a.batch > 0) {
-    a.own_tiles = ceil_div(static_cast<long long>(a.max_q) * a.group, 16 * row_warps(a.max_q * a.group));
+    a.own_tiles = ceil_div(static_cast<long long>(a.max_q) * a.group, a.tile_rows);
     const int tiles = ceil_div(a.max_len, kKeys);
     const int splits =
         std::max(1, std::min({tiles, 64, ceil_div(kWant, static_cast<long long>(a.batch) * a.own_tiles * a.kv_heads)}));

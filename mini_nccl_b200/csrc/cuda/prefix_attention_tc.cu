@@ -21,10 +21,6 @@
 // (head_dim, heads, tokens, pages) into a ring of 128-byte-swizzled stages, in
 // the order in which the products use them.  The MMA warp zeroes V rows past
 // the prefix's end (pages hold anything there); keys past it are masked.
-#include <cudaTypedefs.h>
-
-#include <mutex>
-
 #include "common.cuh"
 #include "generation.h"
 #include "warp_mma.cuh"
@@ -159,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!mbar_wait(empty0 + 8 * st, ((pos / kStages) & 1) ^ 1, a.status)) return false;
       ++pos;
       const int j0 = k0 + tile * kTile;
-      const int per = min(1 << a.page_shift, kTile);  // tokens of a box
+      const int per = min(1 << a.page_shift, 64);  // tokens of a box
       const int boxes = (min(kTile, k1 - j0) + per - 1) / per;
       if (lane == 0) mbar_arrive_expect_tx(full0 + 8 * st, boxes * per * D * 2);
       __syncwarp();
@@ -508,39 +504,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    cudaDriverEntryPointQueryResult q;
-    void* p = nullptr;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  });
-  return fn;
-}
-
-// The pool as (head_dim, heads, tokens, pages); boxes of 64 x 1 x min(page, 128) x 1.
-bool pool_map(CUtensorMap* map, const __nv_bfloat16* base, const Args& a, int head_dim) {
-  if (!encode_fn()) return false;
-  const int page = 1 << a.page_shift;
-  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(a.kv_heads),
-                              static_cast<cuuint64_t>(page), static_cast<cuuint64_t>(a.pages)};
-  // an axis of one entry may have any stride: give the map one that it accepts
-  auto stride = [](long long n, long long ld) { return static_cast<cuuint64_t>(n > 1 ? ld * 2 : 16); };
-  const cuuint64_t strides[3] = {stride(a.kv_heads, a.head_ld), stride(page, a.token_ld), stride(a.pages, a.page_ld)};
-  const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(page < kTile ? page : kTile), 1};
-  const cuuint32_t each[4] = {1, 1, 1, 1};
-  return encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<__nv_bfloat16*>(base), dims, strides, box, each,
-                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int D>
-cudaError_t launch(const Args& a, cudaStream_t stream) {
-  CUtensorMap mk, mv;
-  if (!pool_map(&mk, a.k, a, D) || !pool_map(&mv, a.v, a, D)) return cudaErrorInvalidValue;
+static cudaError_t launch(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
   constexpr int bytes = Smem<D>::total;
   if (const cudaError_t e = cudaFuncSetAttribute(prefix_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
       e != cudaSuccess)
@@ -551,8 +516,8 @@ cudaError_t launch(const Args& a, cudaStream_t stream) {
 
 }  // namespace tc
 
-cudaError_t launch_prefix_tc(const Args& a, int head_dim, cudaStream_t stream) {
-  return head_dim == 64 ? tc::launch<64>(a, stream) : tc::launch<128>(a, stream);
+cudaError_t launch_prefix_tc(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, int head_dim, cudaStream_t stream) {
+  return head_dim == 64 ? tc::launch<64>(a, mk, mv, stream) : tc::launch<128>(a, mk, mv, stream);
 }
 
 }  // namespace prefix
