@@ -30,6 +30,7 @@
 
 #include "common.cuh"
 #include "generation.h"
+#include "launch.cuh"
 #include "warp_mma.cuh"
 
 namespace mnb {
@@ -42,9 +43,10 @@ constexpr int kKeys = 64;            // keys per stage
 constexpr int kTensorCoreRows = 32;  // more rows of a kv head than this go to the tensor-core kernel
 constexpr float kLn2 = 0.6931471805599453f;
 
-template <int D>
+template <int D, int WR>
 struct Ring {
-  static constexpr int stages = D == 128 ? 2 : D == 64 ? 3 : 4;  // three blocks of head dim 128 fit an SM, four of 64
+  // Head dim 128: three blocks with two stages fit an SM, or two (tiles of 64 rows need the registers) with three.
+  static constexpr int stages = D == 128 ? (WR == 4 ? 3 : 2) : D == 64 ? 3 : 4;
   static constexpr uint32_t tile = kKeys * D * 2;                // of K; V follows
   static constexpr uint32_t bytes = stages * 2 * tile;
   // 16-byte chunk c of row r, as TMA's swizzle leaves it
@@ -126,7 +128,7 @@ template <int D, int WR>
 __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
     pieces_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, int items, int join_rows) {
-  using R = Ring<D>;
+  using R = Ring<D, WR>;
   constexpr int WK = 4 / WR, KW = kKeys / WK, kStages = R::stages, kPitch = D + 4;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -142,6 +144,7 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
   }
   __syncthreads();
   int pos = 0;  // stages filled, or used, so far
+  let_next_start();
 
   if (warp == 4) {
     const int per = min(1 << a.page_shift, kKeys);  // tokens of a box
@@ -343,6 +346,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args 
   __shared__ float sl[4];
   const long long row = blockIdx.x, rows = static_cast<long long>(a.n) * a.heads;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  wait_for_previous();
   const int pieces = a.prefix_splits + a.own_splits;
   float m = -INFINITY;
   for (int p = lane; p < pieces; p += 32) m = fmaxf(m, a.part_ml[p * rows + row].x);
@@ -408,12 +412,11 @@ template <int D, int WR>
 static cudaError_t launch_pieces(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
   const int rows_most = std::max(a.tensor_cores ? 0 : a.n * a.group, a.own_splits > 0 ? a.max_q * a.group : 0);
   const int join_rows = WR == 4 ? 0 : std::min(16 * WR, rows_most);
-  const int bytes = Ring<D>::bytes + (4 / WR) * join_rows * ((D + 4) * 4 + 8) + 1024;
+  const int bytes = Ring<D, WR>::bytes + (4 / WR) * join_rows * ((D + 4) * 4 + 8) + 1024;
   const int items = (a.tensor_cores ? 0 : a.row_tiles * a.kv_heads * a.prefix_splits) +
                     a.batch * a.own_tiles * a.own_splits * a.kv_heads;
-  if (const cudaError_t e = cudaFuncSetAttribute(pieces_kernel<D, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-      e != cudaSuccess)
-    return e;
+  static SharedMemory allowed;
+  if (const cudaError_t e = allowed.at_least(reinterpret_cast<const void*>(pieces_kernel<D, WR>), bytes); e != cudaSuccess) return e;
   const int per_sm = std::max(1, std::min(WR == 4 ? 2 : 3, 227 * 1024 / (bytes + 1024 + 64)));
   pieces_kernel<D, WR><<<std::min(items, 148 * per_sm), kThreads, bytes, stream>>>(a, mk, mv, items, join_rows);
   return cudaGetLastError();
@@ -434,8 +437,7 @@ static cudaError_t launch_for(const Args& a, cudaStream_t stream) {
     e = launch_prefix_tc(a, mk, mv, D, stream);
     if (e != cudaSuccess || a.prefix_splits == 1) return e;
   }
-  join_kernel<D><<<a.n * a.heads, 128, 0, stream>>>(a);
-  return cudaGetLastError();
+  return launch_after(join_kernel<D>, a.n * a.heads, 128, 0, stream, a);
 }
 
 // Splits of the tensor-core kernel: whole waves of one block per SM, each taking its tiles and a fixed part, and the

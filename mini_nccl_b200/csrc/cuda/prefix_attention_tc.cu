@@ -23,6 +23,7 @@
 // the prefix's end (pages hold anything there); keys past it are masked.
 #include "common.cuh"
 #include "generation.h"
+#include "launch.cuh"
 #include "warp_mma.cuh"
 
 namespace mnb {
@@ -146,6 +147,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  let_next_start();
   const uint32_t tmem = *tmem_slot;  // S_0, S_1: 128 columns each, then O_0, O_1
 
   if (warp == 0) {
@@ -420,6 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     softmax_sync();
     using Part = typename Vec<kPer>::type;
     const long long rows = static_cast<long long>(a.n) * a.heads;
+    wait_for_previous();  // the own keys' pieces
     const bool alone = a.prefix_splits == 1;  // then this block joins the rows with their own keys' pieces and finishes them
     if (const int i = s * kTile + r; i < n_rows && half == 0) {  // (without `shared`, the first stream's threads)
       const int j = r0 + i, token = j / a.group;
@@ -507,10 +510,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <int D>
 static cudaError_t launch(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
   constexpr int bytes = Smem<D>::total;
-  if (const cudaError_t e = cudaFuncSetAttribute(prefix_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-      e != cudaSuccess)
-    return e;
-  prefix_tc_kernel<D><<<a.row_tiles * a.kv_heads * a.prefix_splits, kThreads, bytes, stream>>>(a, mk, mv);
+  static SharedMemory allowed;
+  if (const cudaError_t e = allowed.at_least(reinterpret_cast<const void*>(prefix_tc_kernel<D>), bytes); e != cudaSuccess) return e;
+  const int blocks = a.row_tiles * a.kv_heads * a.prefix_splits;
+  if (a.own_splits > 0) return launch_after(prefix_tc_kernel<D>, blocks, kThreads, bytes, stream, a, mk, mv);
+  prefix_tc_kernel<D><<<blocks, kThreads, bytes, stream>>>(a, mk, mv);
   return cudaGetLastError();
 }
 
