@@ -17,6 +17,7 @@
 
 #include "common.cuh"
 #include "generation.h"
+#include "launch.cuh"
 
 namespace mnb {
 
@@ -54,11 +55,12 @@ MNB_DEVICE int block_scan(int v, int* sh, int* total) {
 }
 
 // The first `want` free pages in ascending order into ids[]; returns how many there are (at most want).
-MNB_DEVICE int find_free(const int* refs, int pages, int want, int* ids, int* sh) {
+// (`first`: this thread's count of the first kThreads, already read.)
+MNB_DEVICE int find_free(const int* refs, int pages, int want, int* ids, int* sh, int first) {
   int found = 0;
   for (int p0 = 0; p0 < pages && found < want; p0 += kThreads) {
     const int p = p0 + threadIdx.x;
-    const int is_free = p < pages && refs[p] == 0;
+    const int is_free = p < pages && (p0 == 0 ? first : refs[p]) == 0;
     int total;
     const int rank = found + block_scan(is_free, sh, &total);
     if (is_free && rank < want) ids[rank] = p;
@@ -82,55 +84,73 @@ MNB_DEVICE void claim(const int* slot_of, int n, int slots, int* owner) {
 
 // fork: child i gets parent i's table row; full pages are shared, the
 // part-filled last one gets a page of its own (src / dst / tokens name the copy).
+// Few requests keep their state in shared memory: what is left of the time is
+// three trips to memory, one after another (the requests, their lengths, the rows).
+constexpr int kFew = 256;
 __global__ void __launch_bounds__(kThreads) fork_plan_kernel(Table t, const int* __restrict__ parents,
                                                              const int* __restrict__ children, int n, int* owner,
                                                              int* ids, int* src, int* dst, int* tokens, int* status) {
   __shared__ int sh[33];
-  claim(children, n, t.slots, owner);
-  // which requests are sound, and which need a page (ids' rank parked in dst)
+  __shared__ int few_ids[kFew], few_src[kFew], few_dst[kFew], few_tokens[kFew], few_len[kFew], few_parent[kFew], few_child[kFew];
+  const bool few = n <= kFew;
+  int* const of_ids = few ? few_ids : ids;
+  int* const of_src = few ? few_src : src;
+  int* const of_dst = few ? few_dst : dst;
+  int* const of_tokens = few ? few_tokens : tokens;
+  const int first_refs = threadIdx.x < t.pages ? t.refs[threadIdx.x] : 1;  // on its way with the requests
+  let_next_start();
+  if (!few) claim(children, n, t.slots, owner);
+  // which requests are sound, and which need a page (its rank is parked in dst)
   int base = 0;
   for (int i0 = 0; i0 < n; i0 += kThreads) {
     const int i = i0 + threadIdx.x;
     int need = 0, part = -1;
+    int p = -1, c = -1;
+    if (i < n) p = parents[i], c = children[i];
+    bool ok = p >= 0 && p < t.slots && c >= 0 && c < t.slots;
+    const int len = ok ? t.lens[p] : 0, child_len = ok ? t.lens[c] : 0;
+    if (few) {
+      if (i < n) few_parent[i] = p, few_child[i] = c, few_len[i] = len;
+      __syncthreads();
+      if (ok)
+        for (int j = 0; j < n; ++j) ok = ok && few_child[j] != p && (few_child[j] != c || j >= i);
+    } else if (ok) {
+      ok = owner[c] == i && owner[p] == 0x7fffffff;  // the child's first request, and a parent that is nobody's child
+    }
     if (i < n) {
-      const int p = parents[i], c = children[i];
-      bool ok = p >= 0 && p < t.slots && c >= 0 && c < t.slots && owner[c] == i && t.lens[c] == 0;
-      ok = ok && owner[p] == 0x7fffffff;  // a parent is nobody's child in the same call
+      ok = ok && child_len == 0 && len >= 0 && len <= t.columns * static_cast<long long>(t.page_size);
       if (ok) {
-        const int len = t.lens[p];
-        ok = len >= 0 && len <= t.columns * static_cast<long long>(t.page_size);
-        if (ok) {
-          part = len % t.page_size;
-          need = part > 0;
-        }
+        part = len % t.page_size;
+        need = part > 0;
+      } else {
+        flag(status, kErrBadIndex);
       }
-      if (!ok) flag(status, kErrBadIndex);
     }
     int total;
     const int rank = base + block_scan(need, sh, &total);
     if (i < n) {
-      tokens[i] = part;
-      dst[i] = need ? rank : -1;
+      of_tokens[i] = part;
+      of_dst[i] = need ? rank : -1;
     }
     base += total;
   }
-  const int have = find_free(t.refs, t.pages, base, ids, sh);
+  const int have = find_free(t.refs, t.pages, base, of_ids, sh, first_refs);
   if (base > have && threadIdx.x == 0) flag(status, kErrNoPages);
   for (int i = threadIdx.x; i < n; i += kThreads) {
-    src[i] = -1;
-    if (dst[i] >= have) tokens[i] = dst[i] = -1;  // no page left: the child stays empty
+    of_src[i] = -1;
+    if (of_dst[i] >= have) of_tokens[i] = of_dst[i] = -1;  // no page left: the child stays empty
   }
   __syncthreads();
   for (long long x = threadIdx.x; x < static_cast<long long>(n) * t.columns; x += kThreads) {
     const int i = static_cast<int>(x / t.columns), col = static_cast<int>(x % t.columns);
-    if (tokens[i] < 0) continue;
-    const int full = t.lens[parents[i]] / t.page_size;
+    if (of_tokens[i] < 0) continue;
+    const int p = few ? few_parent[i] : parents[i], full = (few ? few_len[i] : t.lens[p]) / t.page_size;
     int page = -1;
     if (col <= full) {
-      page = t.table[parents[i] * t.ld + col];
+      page = t.table[p * t.ld + col];
       if (col == full) {
-        if (tokens[i] > 0 && page >= 0 && page < t.pages) src[i] = page;
-        page = tokens[i] > 0 ? ids[dst[i]] : -1;
+        if (of_tokens[i] > 0 && page >= 0 && page < t.pages) of_src[i] = page;
+        page = of_tokens[i] > 0 ? of_ids[of_dst[i]] : -1;
         if (page >= 0) t.refs[page] = 1;
       } else if (page < 0 || page >= t.pages) {
         flag(status, kErrBadIndex);
@@ -139,14 +159,16 @@ __global__ void __launch_bounds__(kThreads) fork_plan_kernel(Table t, const int*
         atomicAdd(t.refs + page, 1);
       }
     }
-    t.table[children[i] * t.ld + col] = page;
+    t.table[(few ? few_child[i] : children[i]) * t.ld + col] = page;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += kThreads) {
-    if (tokens[i] < 0) continue;
-    if (dst[i] >= 0) dst[i] = ids[dst[i]];
-    if (dst[i] >= 0 && src[i] < 0) flag(status, kErrBadIndex);  // the parent's last page is not in the pool
-    t.lens[children[i]] = t.lens[parents[i]];
+    const int to = of_tokens[i] >= 0 && of_dst[i] >= 0 ? of_ids[of_dst[i]] : -1;
+    if (to >= 0 && of_src[i] < 0) flag(status, kErrBadIndex);  // the parent's last page is not in the pool
+    if (of_tokens[i] >= 0) t.lens[few ? few_child[i] : children[i]] = few ? few_len[i] : t.lens[parents[i]];
+    src[i] = of_src[i];
+    dst[i] = to;
+    tokens[i] = of_tokens[i];
   }
 }
 
@@ -155,6 +177,7 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(Table t, const int* _
                                                            const int* __restrict__ counts, int n, int* owner, int* ids,
                                                            int most, int* rank_of, int* status) {
   __shared__ int sh[33];
+  const int first_refs = threadIdx.x < t.pages ? t.refs[threadIdx.x] : 1;
   claim(slot_of, n, t.slots, owner);
   int base = 0;
   for (int i0 = 0; i0 < n; i0 += kThreads) {
@@ -178,7 +201,7 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(Table t, const int* _
     if (i < n) rank_of[i] = need < 0 ? -1 : rank;
     base += total;
   }
-  const int have = find_free(t.refs, t.pages, min(base, most), ids, sh);
+  const int have = find_free(t.refs, t.pages, min(base, most), ids, sh, first_refs);
   for (int i = threadIdx.x; i < n; i += kThreads) {
     if (rank_of[i] < 0) continue;
     const int s = slot_of[i], len = t.lens[s];
@@ -220,13 +243,16 @@ __global__ void __launch_bounds__(256) free_kernel(Table t, const int* __restric
 }
 
 // compact: with n pages in use, those with ids >= n move, in ascending order,
-// into the free ids below n.  Writes the moves, the new counts and, for every
-// old id, the new one.
+// into the free ids below n.  Writes the moves, the new counts, for every old
+// id the new one, and the first `entries` of the table under the new ids.
 __global__ void __launch_bounds__(kThreads) compact_plan_kernel(const int* __restrict__ refs, int pages,
                                                                 int* __restrict__ new_refs, int* __restrict__ to,
                                                                 int* __restrict__ src, int* __restrict__ dst,
-                                                                int* __restrict__ moves) {
+                                                                int* __restrict__ moves, const int* __restrict__ table,
+                                                                long long ld, int columns, int entries,
+                                                                int* __restrict__ new_table) {
   __shared__ int sh[33];
+  let_next_start();
   int live = 0;
   for (int p0 = 0; p0 < pages; p0 += kThreads) {
     const int p = p0 + threadIdx.x;
@@ -254,23 +280,31 @@ __global__ void __launch_bounds__(kThreads) compact_plan_kernel(const int* __res
     to[src[i]] = dst[i];
   }
   if (threadIdx.x == 0) *moves = movers;
+  __syncthreads();
+  for (int x = threadIdx.x; x < entries; x += kThreads) {
+    const int p = table[(x / columns) * ld + x % columns];
+    new_table[x] = p >= 0 && p < pages ? to[p] : -1;
+  }
 }
 
-// 16-byte chunks of the named pages, in every plane: [moves][planes][chunks].
+// 16-byte chunks of the named pages, in every plane: [planes][moves][chunks].
+// Eight loads in flight per thread: 83 us for 477 MB (5.8 TB/s; four 97, two 88).
 // `tokens` (or null) gives the leading tokens of each page that hold data.
+constexpr int kPer = 8;
 __global__ void __launch_bounds__(256) copy_pages_kernel(uint4* __restrict__ pool, long long plane_chunks,
                                                          int page_chunks, int token_chunks, int planes, int pages,
                                                          const int* __restrict__ src, const int* __restrict__ dst,
                                                          const int* __restrict__ tokens, const int* __restrict__ count,
                                                          int n_max, int* status) {
-  constexpr int kPer = 4;  // independent 16-byte loads per thread
+  wait_for_previous();
   const int n = count ? min(*count, n_max) : n_max;
   const int runs = (page_chunks + 256 * kPer - 1) / (256 * kPer);
   const long long all = static_cast<long long>(n) * planes * runs;
   for (long long x = blockIdx.x; x < all; x += gridDim.x) {
+    // plane by plane, so that a page that several children copy is still in L2 for the next one
     const int run = static_cast<int>(x % runs);
-    const int plane = static_cast<int>((x / runs) % planes);
-    const int i = static_cast<int>(x / (static_cast<long long>(runs) * planes));
+    const int i = static_cast<int>((x / runs) % n);
+    const int plane = static_cast<int>(x / (static_cast<long long>(runs) * n));
     const int a = src[i], b = dst[i];
     if (a < 0 || b < 0) continue;
     if (a >= pages || b >= pages) {
@@ -338,11 +372,10 @@ int copy_blocks(long long units) {
 cudaError_t launch_copy(const Pool& p, const int* src, const int* dst, const int* tokens, const int* count, int n, int* status,
                         cudaStream_t stream) {
   if (n == 0) return cudaSuccess;
-  const long long runs = (p.page_chunks + 1023) / 1024;
-  copy_pages_kernel<<<copy_blocks(static_cast<long long>(n) * p.planes * runs), 256, 0, stream>>>(
-      static_cast<uint4*>(p.base), p.plane_chunks, p.page_chunks, p.token_chunks, p.planes, p.pages, src, dst, tokens, count,
-      n, status);
-  return cudaGetLastError();
+  const long long runs = (p.page_chunks + 256 * kPer - 1) / (256 * kPer);
+  return launch_after(copy_pages_kernel, copy_blocks(static_cast<long long>(n) * p.planes * runs), 256, 0, stream,
+                      static_cast<uint4*>(p.base), p.plane_chunks, p.page_chunks, p.token_chunks, p.planes, p.pages, src, dst,
+                      tokens, count, n, status);
 }
 
 cudaError_t launch_fork(const Pool& p, const Table& t, const int* parents, const int* children, int n, int* scratch,
@@ -369,10 +402,13 @@ cudaError_t launch_free(const Table& t, const int* slots, int n, int* status, cu
 cudaError_t launch_compact(const Pool& p, const int* table, long long table_ld, int rows, int columns, const int* refs,
                            int* new_table, int* new_refs, int* scratch, int* status, cudaStream_t stream) {
   int* s = scratch;
-  compact_plan_kernel<<<1, kThreads, 0, stream>>>(refs, p.pages, new_refs, s, s + p.pages, s + 2 * p.pages, s + 3 * p.pages);
-  if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
   const long long all = static_cast<long long>(rows) * columns;
-  if (all > 0) {
+  constexpr int kSmallTable = 16 * kThreads;  // the planning block does 16 entries a thread in less time than a launch takes
+  const bool small = all <= kSmallTable;
+  compact_plan_kernel<<<1, kThreads, 0, stream>>>(refs, p.pages, new_refs, s, s + p.pages, s + 2 * p.pages, s + 3 * p.pages,
+                                                  table, table_ld, columns, small ? static_cast<int>(all) : 0, new_table);
+  if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
+  if (!small) {
     remap_kernel<<<static_cast<unsigned>((all + 255) / 256), 256, 0, stream>>>(table, table_ld, columns, all, s, p.pages,
                                                                                new_table);
     if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
