@@ -76,7 +76,7 @@ MNB_DEVICE void flag(const Args& a) { atomicCAS(a.status, 0, kErrBadIndex); }
 
 // Item i of the list: first the prefix's (split, kv head, row tile; the row tiles of the same keys side by side), then
 // the sequences' own (sequence, row tile, split, kv head).
-MNB_DEVICE Piece piece_of(const Args& a, int i, int tile_rows) {
+MNB_DEVICE Piece piece_of(const Args& a, const int* seq_lens, const int* q_offsets, int i, int tile_rows) {
   Piece p;
   const int of_prefix = a.tensor_cores ? 0 : a.row_tiles * a.kv_heads * a.prefix_splits;
   if (i < of_prefix) {
@@ -100,8 +100,8 @@ MNB_DEVICE Piece piece_of(const Args& a, int i, int tile_rows) {
   p.n0 = b;
   int q_len = 1;
   if (a.q_offsets) {
-    p.n0 = min(max(a.q_offsets[b], 0), a.n);
-    q_len = min(max(a.q_offsets[b + 1] - p.n0, 0), a.n - p.n0);
+    p.n0 = min(max(q_offsets[b], 0), a.n);
+    q_len = min(max(q_offsets[b + 1] - p.n0, 0), a.n - p.n0);
     if (q_len > a.max_q) {
       flag(a);
       q_len = a.max_q;
@@ -109,7 +109,7 @@ MNB_DEVICE Piece piece_of(const Args& a, int i, int tile_rows) {
   }
   p.r0 = rt * tile_rows;
   p.n_rows = min(tile_rows, q_len * a.group - p.r0);
-  int len = a.seq_lens[b];
+  int len = seq_lens[b];
   if (len < 0 || len > a.max_len) {
     flag(a);
     len = min(max(len, 0), a.max_len);
@@ -127,7 +127,7 @@ MNB_DEVICE Piece piece_of(const Args& a, int i, int tile_rows) {
 template <int D, int WR>
 __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
     pieces_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap map_k,
-                  const __grid_constant__ CUtensorMap map_v, int items, int join_rows) {
+                  const __grid_constant__ CUtensorMap map_v, int items, int join_rows, int known) {
   using R = Ring<D, WR>;
   constexpr int WK = 4 / WR, KW = kKeys / WK, kStages = R::stages, kPitch = D + 4;
   extern __shared__ uint8_t smem_raw[];
@@ -142,6 +142,14 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
     }
     fence_mbar_init();
   }
+  // The sequences' lengths, for short lists (`known` of them): finding a piece then costs no trip to memory.
+  int* lens = reinterpret_cast<int*>(sm + R::bytes + WK * join_rows * (kPitch * 4 + 8));
+  int* offsets = lens + known;
+  for (int b = threadIdx.x; b < known; b += kThreads) lens[b] = a.seq_lens[b];
+  if (a.q_offsets)
+    for (int b = threadIdx.x; b < known + (known > 0); b += kThreads) offsets[b] = a.q_offsets[b];
+  const int* const seq_lens = known ? lens : a.seq_lens;
+  const int* const q_offsets = known ? offsets : a.q_offsets;
   __syncthreads();
   int pos = 0;  // stages filled, or used, so far
   let_next_start();
@@ -149,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
   if (warp == 4) {
     const int per = min(1 << a.page_shift, kKeys);  // tokens of a box
     for (int i = blockIdx.x; i < items; i += gridDim.x) {
-      const Piece p = piece_of(a, i, 16 * WR);
+      const Piece p = piece_of(a, seq_lens, q_offsets, i, 16 * WR);
       for (int j0 = p.k0; j0 < p.k1; j0 += kKeys, ++pos) {
         const int st = pos % kStages, boxes = (min(kKeys, p.k1 - j0) + per - 1) / per;
         int page = 0;
@@ -180,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
 
   const int wr = warp % WR, wk = warp / WR, gq = lane / 4, tg = lane % 4;
   for (int i = blockIdx.x; i < items; i += gridDim.x) {
-    const Piece p = piece_of(a, i, 16 * WR);
+    const Piece p = piece_of(a, seq_lens, q_offsets, i, 16 * WR);
     if (p.n_rows <= 0) continue;
     auto out_of = [&](int r) {
       const int j = p.r0 + r, token = j / a.group;
@@ -412,13 +420,14 @@ template <int D, int WR>
 static cudaError_t launch_pieces(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
   const int rows_most = std::max(a.tensor_cores ? 0 : a.n * a.group, a.own_splits > 0 ? a.max_q * a.group : 0);
   const int join_rows = WR == 4 ? 0 : std::min(16 * WR, rows_most);
-  const int bytes = Ring<D, WR>::bytes + (4 / WR) * join_rows * ((D + 4) * 4 + 8) + 1024;
+  const int known = a.own_splits > 0 && a.batch <= 1024 ? a.batch : 0;
+  const int bytes = Ring<D, WR>::bytes + (4 / WR) * join_rows * ((D + 4) * 4 + 8) + (known ? (2 * known + 1) * 4 : 0) + 1024;
   const int items = (a.tensor_cores ? 0 : a.row_tiles * a.kv_heads * a.prefix_splits) +
                     a.batch * a.own_tiles * a.own_splits * a.kv_heads;
   static SharedMemory allowed;
   if (const cudaError_t e = allowed.at_least(reinterpret_cast<const void*>(pieces_kernel<D, WR>), bytes); e != cudaSuccess) return e;
   const int per_sm = std::max(1, std::min(WR == 4 ? 2 : 3, 227 * 1024 / (bytes + 1024 + 64)));
-  pieces_kernel<D, WR><<<std::min(items, 148 * per_sm), kThreads, bytes, stream>>>(a, mk, mv, items, join_rows);
+  pieces_kernel<D, WR><<<std::min(items, 148 * per_sm), kThreads, bytes, stream>>>(a, mk, mv, items, join_rows, known);
   return cudaGetLastError();
 }
 
@@ -443,12 +452,15 @@ static cudaError_t launch_for(const Args& a, cudaStream_t stream) {
 // Splits of the tensor-core kernel: whole waves of one block per SM, each taking its tiles and a fixed part, and the
 // partial outputs written and read when there are several.
 static int tc_splits(int blocks, int tiles, long long rows, int head_dim, bool wide) {
-  const double tile_us = wide ? 1.5 : 0.8, fixed_us = 4.0;
+  const double tile_us = wide ? 1.9 : 0.95, fixed_us = 6.0;  // measured: a 128-key tile for 256 rows or for 128, and the rest
   int best = 1;
   double least = 1e30;
   for (int s = 1; s <= std::min(tiles, 64); ++s) {
     const int per = ceil_div(tiles, s), pieces = ceil_div(tiles, per);
-    double us = ceil_div(static_cast<long long>(blocks) * pieces, 148) * (per * tile_us + fixed_us);
+    const int units = blocks * pieces, last = units % 148;
+    double waves = units / 148 + (last > 0);
+    if (pieces == 1 && last > 0 && 2 * last <= 148) waves -= 0.4;  // the last one in half the time (prefix_attention_tc.cu)
+    double us = waves * (per * tile_us + fixed_us);
     if (pieces > 1) us += 3.0 + pieces * rows * head_dim * 8 / 6.5e6;
     if (us < least * 0.999) least = us, best = s;
   }

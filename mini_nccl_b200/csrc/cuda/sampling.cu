@@ -373,36 +373,49 @@ struct Row {
   template <typename F>
   MNB_DEVICE void scan_noise(float least, const float* noise, F f) const {
     const bool vec = (reinterpret_cast<uintptr_t>(noise - lead) & 15) == 0;
-    auto fetch = [&](int c, float (&g)[kVec]) {
-      if (c >= count || !(widest(piece(c), -INFINITY) >= least)) return false;
-      const int i0 = start(c);
-      if (vec && whole(c)) {
+    constexpr int kUnit = 8 / kVec, kStep = kUnit * kThreads;  // pieces per turn: eight values
+    auto fetch = [&](int c0, float (&g)[8]) {
+      unsigned have = 0;
 #pragma unroll
-        for (int j = 0; j < kVec; j += 4) {
-          const float4 t = *reinterpret_cast<const float4*>(noise + i0 + j);
-          g[j] = t.x, g[j + 1] = t.y, g[j + 2] = t.z, g[j + 3] = t.w;
+      for (int u = 0; u < kUnit; ++u) {
+        const int c = c0 + u * kThreads;
+        if (c >= count || !(widest(piece(c), -INFINITY) >= least)) continue;
+        const int i0 = start(c);
+        if (vec && whole(c)) {
+#pragma unroll
+          for (int j = 0; j < kVec; j += 4) {
+            const float4 t = *reinterpret_cast<const float4*>(noise + i0 + j);
+            float* to = g + u * kVec + j;
+            to[0] = t.x, to[1] = t.y, to[2] = t.z, to[3] = t.w;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) g[u * kVec + j] = i0 + j >= 0 && i0 + j < V ? noise[i0 + j] : 0.f;
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) g[j] = i0 + j >= 0 && i0 + j < V ? noise[i0 + j] : 0.f;
+        have |= 1u << u;
       }
-      return true;
+      return have;
     };
-    auto work = [&](int c, const float (&g)[kVec]) {
-      float v[kVec];
-      unpack_piece(piece(c), v);
+    auto work = [&](int c0, const float (&g)[8], unsigned have) {
 #pragma unroll
-      for (int j = 0; j < kVec; j += 4) f(v + j, g + j, start(c) + j);  // four at a time: fewer values held at once
+      for (int u = 0; u < kUnit; ++u) {
+        if (!(have >> u & 1)) continue;
+        const int c = c0 + u * kThreads;
+        float v[kVec];
+        unpack_piece(piece(c), v);
+#pragma unroll
+        for (int j = 0; j < kVec; j += 4) f(v + j, g + u * kVec + j, start(c) + j);  // four at a time: fewer values held at once
+      }
     };
-    float g0[kVec], g1[kVec];
+    float g0[8], g1[8];
     int c = threadIdx.x;
-    bool have0 = fetch(c, g0), have1;
+    unsigned have0 = fetch(c, g0), have1;
     while (c < count) {
-      have1 = fetch(c + kThreads, g1);
-      if (have0) work(c, g0);
-      have0 = fetch(c + 2 * kThreads, g0);
-      if (have1) work(c + kThreads, g1);
-      c += 2 * kThreads;
+      have1 = fetch(c + kStep, g1);
+      work(c, g0, have0);
+      have0 = fetch(c + 2 * kStep, g0);
+      work(c + kStep, g1, have1);
+      c += 2 * kStep;
     }
   }
   // f(values, index of the first) over those pieces

@@ -29,10 +29,16 @@ from collections.abc import Sequence
 import torch
 
 
-def _kernels():
-    from . import kernels
+_KERNELS = None
 
-    return kernels
+
+def _kernels():
+    global _KERNELS
+    if _KERNELS is None:
+        from . import kernels
+
+        _KERNELS = kernels
+    return _KERNELS
 
 
 def _need(ok: bool, message: str) -> None:
