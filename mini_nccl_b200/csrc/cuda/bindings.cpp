@@ -39,25 +39,25 @@ void flash_attn_bwd_tc(torch::Tensor qkv, torch::Tensor o, torch::Tensor dout, t
                        torch::Tensor dq_acc, torch::Tensor delta, int64_t n_head, double scale, torch::Tensor status);
 void exp2_poly_eval(torch::Tensor x, torch::Tensor y);
 // generation.cpp
-void copy_pages(torch::Tensor kv, torch::Tensor src, torch::Tensor dst, torch::Tensor status);
-void fork_sequences(torch::Tensor kv, torch::Tensor page_table, torch::Tensor lens, torch::Tensor refs,
-                    torch::Tensor parents, torch::Tensor children, torch::Tensor status);
-void reserve_pages(torch::Tensor page_table, torch::Tensor lens, torch::Tensor refs, torch::Tensor slots,
-                   torch::Tensor counts, int64_t page_size, torch::Tensor status);
-void free_sequences(torch::Tensor page_table, torch::Tensor lens, torch::Tensor refs, torch::Tensor slots,
-                    torch::Tensor status);
-std::tuple<torch::Tensor, torch::Tensor> compact_pages(torch::Tensor kv, torch::Tensor page_table, torch::Tensor refs,
-                                                       torch::Tensor status);
-void append_kv(torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor k, torch::Tensor v, torch::Tensor page_table,
-               torch::Tensor positions, c10::optional<torch::Tensor> slots, torch::Tensor status);
+void copy_pages(const torch::Tensor& kv, const torch::Tensor& src, const torch::Tensor& dst, const torch::Tensor& status);
+void fork_sequences(const torch::Tensor& kv, const torch::Tensor& page_table, const torch::Tensor& lens, const torch::Tensor& refs,
+                    const torch::Tensor& parents, const torch::Tensor& children, const torch::Tensor& status);
+void reserve_pages(const torch::Tensor& page_table, const torch::Tensor& lens, const torch::Tensor& refs, const torch::Tensor& slots,
+                   const torch::Tensor& counts, int64_t page_size, const torch::Tensor& status);
+void free_sequences(const torch::Tensor& page_table, const torch::Tensor& lens, const torch::Tensor& refs, const torch::Tensor& slots,
+                    const torch::Tensor& status);
+std::tuple<torch::Tensor, torch::Tensor> compact_pages(const torch::Tensor& kv, const torch::Tensor& page_table, const torch::Tensor& refs,
+                                                       const torch::Tensor& status);
+void append_kv(const torch::Tensor& k_pages, const torch::Tensor& v_pages, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& page_table,
+               const torch::Tensor& positions, const c10::optional<torch::Tensor>& slots, const torch::Tensor& status);
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>> sample(
-    torch::Tensor logits, torch::Tensor noise, c10::optional<torch::Tensor> temperature, double temperature_all,
-    c10::optional<torch::Tensor> top_k, int64_t top_k_all, c10::optional<torch::Tensor> top_p, double top_p_all,
-    c10::optional<torch::Tensor> min_p, double min_p_all, bool return_logprob, torch::Tensor status);
+    const torch::Tensor& logits, const torch::Tensor& noise, const c10::optional<torch::Tensor>& temperature, double temperature_all,
+    const c10::optional<torch::Tensor>& top_k, int64_t top_k_all, const c10::optional<torch::Tensor>& top_p, double top_p_all,
+    const c10::optional<torch::Tensor>& min_p, double min_p_all, bool return_logprob, const torch::Tensor& status);
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(
-    torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor prefix_pages, int64_t prefix_len,
-    torch::Tensor page_table, torch::Tensor seq_lens, c10::optional<torch::Tensor> q_offsets, int64_t max_q_len,
-    int64_t max_seq_len, double scale, bool return_lse, torch::Tensor status);
+    const torch::Tensor& q, const torch::Tensor& k_pages, const torch::Tensor& v_pages, const torch::Tensor& prefix_pages, int64_t prefix_len,
+    const torch::Tensor& page_table, const torch::Tensor& seq_lens, const c10::optional<torch::Tensor>& q_offsets, int64_t max_q_len,
+    int64_t max_seq_len, double scale, bool return_lse, const torch::Tensor& status);
 // comm.cu
 void register_comm(pybind11::module_& m);
 }  // namespace mnb

@@ -80,7 +80,7 @@ S setting(const c10::optional<torch::Tensor>& each, double all, int64_t rows, at
 
 }  // namespace
 
-void copy_pages(torch::Tensor kv, torch::Tensor src, torch::Tensor dst, torch::Tensor status) {
+void copy_pages(const torch::Tensor& kv, const torch::Tensor& src, const torch::Tensor& dst, const torch::Tensor& status) {
   const auto p = pool_of(kv);
   check_int32(src, 1, kv, "src");
   check_int32(dst, 1, kv, "dst");
@@ -91,8 +91,8 @@ void copy_pages(torch::Tensor kv, torch::Tensor src, torch::Tensor dst, torch::T
                                     static_cast<int>(src.size(0)), status.data_ptr<int>(), at::cuda::getCurrentCUDAStream()));
 }
 
-void fork_sequences(torch::Tensor kv, torch::Tensor page_table, torch::Tensor lens, torch::Tensor refs,
-                    torch::Tensor parents, torch::Tensor children, torch::Tensor status) {
+void fork_sequences(const torch::Tensor& kv, const torch::Tensor& page_table, const torch::Tensor& lens, const torch::Tensor& refs,
+                    const torch::Tensor& parents, const torch::Tensor& children, const torch::Tensor& status) {
   const auto p = pool_of(kv);
   const auto t = table_of(page_table, lens, refs, p.page_size);
   check_int32(parents, 1, kv, "parents");
@@ -105,13 +105,13 @@ void fork_sequences(torch::Tensor kv, torch::Tensor page_table, torch::Tensor le
   if (n == 0 || t.slots == 0) return;
   TORCH_CHECK_VALUE(n < (1 << 28), "children: too many");
   const c10::cuda::CUDAGuard guard(kv.device());
-  auto scratch = torch::empty({4 * n + t.slots}, parents.options());
+  auto scratch = at::empty({4 * n + t.slots}, parents.options());
   C10_CUDA_CHECK(cache::launch_fork(p, t, parents.data_ptr<int>(), children.data_ptr<int>(), static_cast<int>(n),
                                     scratch.data_ptr<int>(), status.data_ptr<int>(), at::cuda::getCurrentCUDAStream()));
 }
 
-void reserve_pages(torch::Tensor page_table, torch::Tensor lens, torch::Tensor refs, torch::Tensor slots,
-                   torch::Tensor counts, int64_t page_size, torch::Tensor status) {
+void reserve_pages(const torch::Tensor& page_table, const torch::Tensor& lens, const torch::Tensor& refs, const torch::Tensor& slots,
+                   const torch::Tensor& counts, int64_t page_size, const torch::Tensor& status) {
   TORCH_CHECK_VALUE(page_size >= 1 && page_size < (1 << 30), "page_size: at least 1");
   const auto t = table_of(page_table, lens, refs, static_cast<int>(page_size));
   check_int32(slots, 1, page_table, "slots");
@@ -121,13 +121,13 @@ void reserve_pages(torch::Tensor page_table, torch::Tensor lens, torch::Tensor r
   const int64_t n = slots.size(0);
   if (n == 0) return;
   const c10::cuda::CUDAGuard guard(page_table.device());
-  auto scratch = torch::empty({t.pages + n + t.slots}, slots.options());
+  auto scratch = at::empty({t.pages + n + t.slots}, slots.options());
   C10_CUDA_CHECK(cache::launch_reserve(t, slots.data_ptr<int>(), counts.data_ptr<int>(), static_cast<int>(n),
                                        scratch.data_ptr<int>(), status.data_ptr<int>(), at::cuda::getCurrentCUDAStream()));
 }
 
-void free_sequences(torch::Tensor page_table, torch::Tensor lens, torch::Tensor refs, torch::Tensor slots,
-                    torch::Tensor status) {
+void free_sequences(const torch::Tensor& page_table, const torch::Tensor& lens, const torch::Tensor& refs, const torch::Tensor& slots,
+                    const torch::Tensor& status) {
   const auto t = table_of(page_table, lens, refs, 1);
   check_int32(slots, 1, page_table, "slots");
   check_status_word(status);
@@ -137,17 +137,17 @@ void free_sequences(torch::Tensor page_table, torch::Tensor lens, torch::Tensor 
   C10_CUDA_CHECK(cache::launch_free(t, slots.data_ptr<int>(), n, status.data_ptr<int>(), at::cuda::getCurrentCUDAStream()));
 }
 
-std::tuple<torch::Tensor, torch::Tensor> compact_pages(torch::Tensor kv, torch::Tensor page_table, torch::Tensor refs,
-                                                       torch::Tensor status) {
+std::tuple<torch::Tensor, torch::Tensor> compact_pages(const torch::Tensor& kv, const torch::Tensor& page_table, const torch::Tensor& refs,
+                                                       const torch::Tensor& status) {
   const auto p = pool_of(kv);
   check_int32(page_table, 2, kv, "page_table");
   check_int32(refs, 1, kv, "refs");
   check_status_word(status);
   TORCH_CHECK_VALUE(refs.size(0) == p.pages, "refs: one count for each page of kv");
   const c10::cuda::CUDAGuard guard(kv.device());
-  auto new_table = torch::empty(page_table.sizes(), page_table.options());
-  auto new_refs = torch::empty(refs.sizes(), refs.options());
-  auto scratch = torch::empty({3 * static_cast<int64_t>(p.pages) + 1}, refs.options());
+  auto new_table = at::empty(page_table.sizes(), page_table.options());
+  auto new_refs = at::empty(refs.sizes(), refs.options());
+  auto scratch = at::empty({3 * static_cast<int64_t>(p.pages) + 1}, refs.options());
   C10_CUDA_CHECK(cache::launch_compact(p, page_table.data_ptr<int>(), page_table.stride(0),
                                        static_cast<int>(page_table.size(0)), static_cast<int>(page_table.size(1)),
                                        refs.data_ptr<int>(), new_table.data_ptr<int>(), new_refs.data_ptr<int>(),
@@ -155,8 +155,8 @@ std::tuple<torch::Tensor, torch::Tensor> compact_pages(torch::Tensor kv, torch::
   return {new_table, new_refs};
 }
 
-void append_kv(torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor k, torch::Tensor v, torch::Tensor page_table,
-               torch::Tensor positions, c10::optional<torch::Tensor> slots, torch::Tensor status) {
+void append_kv(const torch::Tensor& k_pages, const torch::Tensor& v_pages, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& page_table,
+               const torch::Tensor& positions, const c10::optional<torch::Tensor>& slots, const torch::Tensor& status) {
   TORCH_CHECK_VALUE(k_pages.is_cuda() && k_pages.dim() == 4 && k_pages.scalar_type() == at::kBFloat16 &&
                         v_pages.scalar_type() == at::kBFloat16 && v_pages.sizes() == k_pages.sizes() &&
                         v_pages.strides() == k_pages.strides() && v_pages.device() == k_pages.device(),
@@ -209,9 +209,9 @@ void append_kv(torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor k, to
 }
 
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>> sample(
-    torch::Tensor logits, torch::Tensor noise, c10::optional<torch::Tensor> temperature, double temperature_all,
-    c10::optional<torch::Tensor> top_k, int64_t top_k_all, c10::optional<torch::Tensor> top_p, double top_p_all,
-    c10::optional<torch::Tensor> min_p, double min_p_all, bool return_logprob, torch::Tensor status) {
+    const torch::Tensor& logits, const torch::Tensor& noise, const c10::optional<torch::Tensor>& temperature, double temperature_all,
+    const c10::optional<torch::Tensor>& top_k, int64_t top_k_all, const c10::optional<torch::Tensor>& top_p, double top_p_all,
+    const c10::optional<torch::Tensor>& min_p, double min_p_all, bool return_logprob, const torch::Tensor& status) {
   using sampling::Setting;
   TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() == 2 &&
                         (logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kFloat),
@@ -232,9 +232,9 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> sample(
   a.top_p = setting<Setting>(top_p, top_p_all, R, at::kFloat, logits, "top_p");
   a.min_p = setting<Setting>(min_p, min_p_all, R, at::kFloat, logits, "min_p");
   const c10::cuda::CUDAGuard guard(logits.device());
-  auto token = torch::empty({R}, logits.options().dtype(at::kLong));
+  auto token = at::empty({R}, logits.options().dtype(at::kLong));
   c10::optional<torch::Tensor> logprob;
-  if (return_logprob) logprob = torch::empty({R}, logits.options().dtype(at::kFloat));
+  if (return_logprob) logprob = at::empty({R}, logits.options().dtype(at::kFloat));
   if (R == 0) return {token, logprob};
   a.logits = logits.data_ptr();
   a.bf16 = logits.scalar_type() == at::kBFloat16;
@@ -250,9 +250,9 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> sample(
 }
 
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(
-    torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor prefix_pages, int64_t prefix_len,
-    torch::Tensor page_table, torch::Tensor seq_lens, c10::optional<torch::Tensor> q_offsets, int64_t max_q_len,
-    int64_t max_seq_len, double scale, bool return_lse, torch::Tensor status) {
+    const torch::Tensor& q, const torch::Tensor& k_pages, const torch::Tensor& v_pages, const torch::Tensor& prefix_pages, int64_t prefix_len,
+    const torch::Tensor& page_table, const torch::Tensor& seq_lens, const c10::optional<torch::Tensor>& q_offsets, int64_t max_q_len,
+    int64_t max_seq_len, double scale, bool return_lse, const torch::Tensor& status) {
   TORCH_CHECK_VALUE(q.is_cuda() && q.scalar_type() == at::kBFloat16 && q.dim() == 3,
                     "q: a bf16 CUDA tensor [tokens, heads, head_dim]");
   TORCH_CHECK_VALUE(k_pages.device() == q.device() && v_pages.device() == q.device() &&
@@ -293,9 +293,9 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(
   TORCH_CHECK_VALUE(N * H < (1ll << 31) && prefix_len < (1ll << 30) && room < (1ll << 30), "too many rows or keys");
 
   const c10::cuda::CUDAGuard guard(q.device());
-  auto o = torch::empty({N, H, D}, q.options());
+  auto o = at::empty({N, H, D}, q.options());
   c10::optional<torch::Tensor> lse;
-  if (return_lse) lse = torch::empty({N, H}, q.options().dtype(at::kFloat));
+  if (return_lse) lse = at::empty({N, H}, q.options().dtype(at::kFloat));
   if (N == 0) return {o, lse};
 
   prefix::Args a{};
@@ -330,7 +330,7 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(
   TORCH_CHECK_VALUE(B * a.own_tiles * a.own_splits * Hk < (1ll << 31), "too many sequences times max_q_len");
   torch::Tensor part;
   if (pieces > 0) {
-    part = torch::empty({pieces * rows * (D + 2)}, q.options().dtype(at::kFloat));
+    part = at::empty({pieces * rows * (D + 2)}, q.options().dtype(at::kFloat));
     a.part_o = part.data_ptr<float>();
     a.part_ml = reinterpret_cast<float2*>(a.part_o + pieces * rows * D);
   }
