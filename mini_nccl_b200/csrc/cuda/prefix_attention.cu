@@ -217,6 +217,7 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
 #pragma unroll
     for (int d = 0; d < D / 8; ++d) acc[d][0] = acc[d][1] = acc[d][2] = acc[d][3] = 0.f;
     float m_r[2] = {-INFINITY, -INFINITY}, l_r[2] = {0.f, 0.f};
+    const bool lower = p.n_rows > wr * 16 + 8;  // whether the tile's rows 8 to 15 are any of ours
 
     for (int t0 = p.k0; t0 < p.k1; t0 += kKeys, ++pos) {
       const int st = pos % kStages;
@@ -255,16 +256,19 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
         }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
+        if (e == 1 && !lower) break;  // (their weights stay at the scores, which nobody reads)
         mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
         mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
         const float base = mx[e] == -INFINITY ? 0.f : mx[e];  // no key yet: every weight is exp2(-inf) = 0
         const float alpha = ex2_approx(m_r[e] - base);
         m_r[e] = mx[e];
-        l_r[e] *= alpha;
+        if (__any_sync(0xffffffffu, alpha != 1.f)) {  // some row of the warp has a new maximum
+          l_r[e] *= alpha;
 #pragma unroll
-        for (int d = 0; d < D / 8; ++d) {
-          acc[d][2 * e] *= alpha;
-          acc[d][2 * e + 1] *= alpha;
+          for (int d = 0; d < D / 8; ++d) {
+            acc[d][2 * e] *= alpha;
+            acc[d][2 * e + 1] *= alpha;
+          }
         }
 #pragma unroll
         for (int n = 0; n < KW / 8; ++n)
@@ -346,15 +350,17 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
   }
 }
 
-// One block joins the pieces of one (token, head), its warps taking them in turn.
-template <int D>
+// Joins the pieces of each (token, head).  With many pieces a block takes a row and its warps the pieces in turn, because
+// one warp would wait for one piece after another; with few a warp takes a row (76,000 rows of two pieces: see below).
+template <int D, bool Together>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args a) {
-  constexpr int kPer = D / 32;
+  constexpr int kPer = D / 32, kStep = Together ? 4 : 1;
   __shared__ float so[4][D];
   __shared__ float sl[4];
-  const long long row = blockIdx.x, rows = static_cast<long long>(a.n) * a.heads;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const long long row = Together ? blockIdx.x : blockIdx.x * 4ll + warp, rows = static_cast<long long>(a.n) * a.heads;
   wait_for_previous();
+  if (row >= rows) return;
   const int pieces = a.prefix_splits + a.own_splits;
   float m = -INFINITY;
   for (int p = lane; p < pieces; p += 32) m = fmaxf(m, a.part_ml[p * rows + row].x);
@@ -362,7 +368,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args 
   const float base = m == -INFINITY ? 0.f : m;
   float l = 0.f, o[kPer] = {};
 #pragma unroll 4
-  for (int p = warp; p < pieces; p += 4) {
+  for (int p = Together ? warp : 0; p < pieces; p += kStep) {
     const float2 ml = a.part_ml[p * rows + row];
     const float f = ex2_approx(ml.x - base);
     l = fmaf(f, ml.y, l);
@@ -370,18 +376,22 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args 
 #pragma unroll
     for (int i = 0; i < kPer; ++i) o[i] = fmaf(f, ml.x == -INFINITY ? 0.f : po[i], o[i]);  // (a piece without keys is not written)
   }
+  if (Together) {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) so[warp][lane * kPer + i] = o[i];
-  if (lane == 0) sl[warp] = l;
-  __syncthreads();
-  l = sl[0] + sl[1] + sl[2] + sl[3];
-  const float inv = l > 0.f ? 1.f / l : 0.f;  // a row without keys is zero
-  if (threadIdx.x < D / 2) {
-    const int c = 2 * threadIdx.x;
-    auto sum = [&](int i) { return so[0][i] + so[1][i] + so[2][i] + so[3][i]; };
-    *reinterpret_cast<uint32_t*>(a.o + row * D + c) = pack_bf16x2(sum(c) * inv, sum(c + 1) * inv);
+    for (int i = 0; i < kPer; ++i) so[warp][lane * kPer + i] = o[i];
+    if (lane == 0) sl[warp] = l;
+    __syncthreads();
+    if (warp > 0) return;
+    l = sl[0] + sl[1] + sl[2] + sl[3];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) o[i] = so[0][lane * kPer + i] + so[1][lane * kPer + i] + so[2][lane * kPer + i] + so[3][lane * kPer + i];
   }
-  if (a.lse && threadIdx.x == 0) a.lse[row] = l > 0.f ? kLn2 * (m + log2f(l)) : -INFINITY;
+  const float inv = l > 0.f ? 1.f / l : 0.f;  // a row without keys is zero
+  __nv_bfloat16* out = a.o + row * D + lane * kPer;
+  if constexpr (kPer == 1) *out = f32_to_bf16(o[0] * inv);
+#pragma unroll
+  for (int i = 0; i + 1 < kPer; i += 2) *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2(o[i] * inv, o[i + 1] * inv);
+  if (a.lse && lane == 0) a.lse[row] = l > 0.f ? kLn2 * (m + log2f(l)) : -INFINITY;
 }
 
 int row_warps(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
@@ -446,7 +456,9 @@ static cudaError_t launch_for(const Args& a, cudaStream_t stream) {
     e = launch_prefix_tc(a, mk, mv, D, stream);
     if (e != cudaSuccess || a.prefix_splits == 1) return e;
   }
-  return launch_after(join_kernel<D>, a.n * a.heads, 128, 0, stream, a);
+  const int rows = a.n * a.heads;
+  if (a.prefix_splits + a.own_splits > 4) return launch_after(join_kernel<D, true>, rows, 128, 0, stream, a);
+  return launch_after(join_kernel<D, false>, ceil_div(rows, 4), 128, 0, stream, a);
 }
 
 // Splits of the tensor-core kernel: whole waves of one block per SM, each taking its tiles and a fixed part, and the
