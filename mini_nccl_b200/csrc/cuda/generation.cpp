@@ -102,7 +102,7 @@ void fork_sequences(const torch::Tensor& kv, const torch::Tensor& page_table, co
   TORCH_CHECK_VALUE(refs.size(0) == p.pages, "refs: one count for each page of kv");
   TORCH_CHECK_VALUE(parents.size(0) == children.size(0), "parents and children: one parent for each child");
   const int64_t n = parents.size(0);
-  if (n == 0 || t.slots == 0) return;
+  if (n == 0 || t.slots == 0 || t.columns == 0) return;
   TORCH_CHECK_VALUE(n < (1 << 28), "children: too many");
   const c10::cuda::CUDAGuard guard(kv.device());
   auto scratch = at::empty({4 * n + t.slots}, parents.options());

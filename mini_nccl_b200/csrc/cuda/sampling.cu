@@ -24,6 +24,15 @@
 //     exact cut.  A band with too many tokens is counted again in finer bins.
 //   - what is left (thousands of equal logits at the cut, infinite logits) is
 //     found by bisection over the pairs, slowly.
+// Measured (GPU time): 1 x 50304 bf16, top-k 50: 11 us; 64 x 50304 fp32 with
+// mixed settings 26 us; 512 x 50304 bf16, top-p 0.9 to 0.95: 80 us (52 MB of
+// logits and about as much noise); 129 x 130003 fp32, min-p: 43 us (67 MB).
+// None is bound by its bytes: a row is a chain of passes, and the instructions
+// of the passes (12 an element to count, 13 to split, 11 to score) fill the
+// issue slots of the two blocks that share an SM.  A row's blocks exchange
+// values four to eight times at about a microsecond each, so a row gets the
+// fewest blocks that hold it: 512 rows of 50304 in clusters of 1, 2, 4 and 8
+// blocks took 112, 171, 298 and 562 us.
 // Weights and sums are fp32, in a fixed order, so results do not depend on
 // scheduling; the winning score is IEEE fp32 division and addition.
 #include <cooperative_groups.h>
