@@ -34,10 +34,10 @@ KERNELS_PER_CALL = {
     "fork_sequences": 2,
     "reserve_pages": 1,
     "free_sequences": 1,
-    "compact_pages": 3,
+    "compact_pages": 2,
     "append_kv": 1,
     "sample": 1,
-    "shared_prefix_attention": 3,
+    "shared_prefix_attention": 2,
     "all_reduce": 1,
     "reduce_scatter": 1,
     "move": 1,
