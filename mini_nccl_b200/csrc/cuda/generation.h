@@ -107,6 +107,7 @@ struct Args {
   // the pieces (plan)
   bool tensor_cores;  // the prefix by prefix_attention_tc.cu
   int tile_rows;      // rows that a block of the other kernel takes at once
+  bool quad;          // it takes four kv heads of a sequence at once
   int row_tiles, prefix_splits, prefix_chunk;
   int own_tiles, own_splits, own_chunk;
   float* part_o;    // [pieces][n][heads][head_dim]

@@ -76,7 +76,8 @@ MNB_DEVICE void flag(const Args& a) { atomicCAS(a.status, 0, kErrBadIndex); }
 
 // Item i of the list: first the prefix's (split, kv head, row tile; the row tiles of the same keys side by side), then
 // the sequences' own (sequence, row tile, split, kv head).
-MNB_DEVICE Piece piece_of(const Args& a, const int* seq_lens, const int* q_offsets, int i, int tile_rows) {
+// With `heads` of 4 an own piece is that of four kv heads, from p.h on.
+MNB_DEVICE Piece piece_of(const Args& a, const int* seq_lens, const int* q_offsets, int i, int tile_rows, int heads) {
   Piece p;
   const int of_prefix = a.tensor_cores ? 0 : a.row_tiles * a.kv_heads * a.prefix_splits;
   if (i < of_prefix) {
@@ -93,10 +94,11 @@ MNB_DEVICE Piece piece_of(const Args& a, const int* seq_lens, const int* q_offse
     return p;
   }
   i -= of_prefix;
-  p.h = i % a.kv_heads;
-  const int split = (i / a.kv_heads) % a.own_splits;
-  const int rt = (i / (a.kv_heads * a.own_splits)) % a.own_tiles;
-  const int b = i / (a.kv_heads * a.own_splits * a.own_tiles);
+  const int groups = (a.kv_heads + heads - 1) / heads;
+  p.h = i % groups * heads;
+  const int split = (i / groups) % a.own_splits;
+  const int rt = (i / (groups * a.own_splits)) % a.own_tiles;
+  const int b = i / (groups * a.own_splits * a.own_tiles);
   p.n0 = b;
   int q_len = 1;
   if (a.q_offsets) {
@@ -130,12 +132,17 @@ MNB_DEVICE Piece piece_of(const Args& a, const int* seq_lens, const int* q_offse
 // as a full one (some 400 instructions at 1.5 a cycle).  Blocks fetching their pieces from the hardware's work queue
 // instead of in turn were no faster, and neither were keys laid out head by head.  2388 rows of 24 sequences in tiles
 // of 64 (masked triangles, 14 GFLOP as computed): 80 us, bound by the latency of eight working warps per SM.
-template <int D, int WR>
+//
+// Quad: a piece is four kv heads of one sequence, a stage 16 keys of each, and every warp works on a head of its own,
+// without a join: what a piece costs beside its keys is spent once for four heads, which decides where many sequences
+// are short (2048 sequences of 4 tokens, 16 heads: QUADBEFORE us without, QUADAFTER with).
+template <int D, int WR, bool Quad>
 __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
     pieces_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, int items, int join_rows, int known) {
   using R = Ring<D, WR>;
-  constexpr int WK = 4 / WR, KW = kKeys / WK, kStages = R::stages, kPitch = D + 4;
+  constexpr int WK = Quad ? 1 : 4 / WR, KW = Quad ? 16 : kKeys / WK, kStages = R::stages, kPitch = D + 4;
+  constexpr int kStep = Quad ? 16 : kKeys, kHeads = Quad ? 4 : 1;  // keys and heads of a stage; head y's keys are rows 16 y on
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t bars[2 * kStages];
@@ -161,14 +168,17 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
   let_next_start();
 
   if (warp == 4) {
-    const int per = min(1 << a.page_shift, kKeys);  // tokens of a box
+    const int per = min(1 << a.page_shift, kStep);  // tokens of a box
+    const int box = lane / kHeads, head = lane % kHeads;
     for (int i = blockIdx.x; i < items; i += gridDim.x) {
-      const Piece p = piece_of(a, seq_lens, q_offsets, i, 16 * WR);
-      for (int j0 = p.k0; j0 < p.k1; j0 += kKeys, ++pos) {
-        const int st = pos % kStages, boxes = (min(kKeys, p.k1 - j0) + per - 1) / per;
+      const Piece p = piece_of(a, seq_lens, q_offsets, i, 16 * WR, kHeads);
+      const int heads = min(kHeads, a.kv_heads - p.h);
+      for (int j0 = p.k0; j0 < p.k1; j0 += kStep, ++pos) {
+        const int st = pos % kStages, boxes = (min(kStep, p.k1 - j0) + per - 1) / per;
         int page = 0;
-        const int j = j0 + lane * per;
-        if (lane < boxes) {
+        const int j = j0 + box * per;
+        const bool mine = box < boxes && head < heads;
+        if (mine) {
           page = p.ids[j >> a.page_shift];
           if (page < 0 || page >= a.pages) {
             flag(a);
@@ -176,15 +186,15 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
           }
         }
         if (!mbar_wait(empty0 + 8 * st, ((pos / kStages) & 1) ^ 1, a.status)) return;
-        if (lane == 0) mbar_arrive_expect_tx(full0 + 8 * st, boxes * per * D * 4);
+        if (lane == 0) mbar_arrive_expect_tx(full0 + 8 * st, boxes * per * heads * D * 4);
         __syncwarp();
-        if (lane < boxes) {
-          const uint32_t to = ring + st * 2 * R::tile + lane * per * (D == 32 ? 64 : 128);
+        if (mine) {
+          const uint32_t to = ring + st * 2 * R::tile + (head * kStep + box * per) * (D == 32 ? 64 : 128);
 #pragma unroll
           for (int c = 0; c < (D + 63) / 64; ++c) {
             const int token = j & ((1 << a.page_shift) - 1);
-            tma_load_4d(to + c * (kKeys * 128), &map_k, c * 64, p.h, token, page, full0 + 8 * st);
-            tma_load_4d(to + R::tile + c * (kKeys * 128), &map_v, c * 64, p.h, token, page, full0 + 8 * st);
+            tma_load_4d(to + c * (kKeys * 128), &map_k, c * 64, p.h + head, token, page, full0 + 8 * st);
+            tma_load_4d(to + R::tile + c * (kKeys * 128), &map_v, c * 64, p.h + head, token, page, full0 + 8 * st);
           }
         }
       }
@@ -192,16 +202,20 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
     return;
   }
 
-  const int wr = warp % WR, wk = warp / WR, gq = lane / 4, tg = lane % 4;
+  const int wr = Quad ? 0 : warp % WR, wk = Quad ? 0 : warp / WR, gq = lane / 4, tg = lane % 4;
+  const int row0 = Quad ? warp * 16 : wk * KW;  // of this warp's keys in a stage
   for (int i = blockIdx.x; i < items; i += gridDim.x) {
-    const Piece p = piece_of(a, seq_lens, q_offsets, i, 16 * WR);
+    const Piece p = piece_of(a, seq_lens, q_offsets, i, 16 * WR, kHeads);
     if (p.n_rows <= 0) continue;
+    const int head = Quad ? p.h + warp : p.h;
+    const bool idle = Quad && head >= a.kv_heads;  // the last four heads may be fewer
     auto out_of = [&](int r) {
       const int j = p.r0 + r, token = j / a.group;
-      return (static_cast<long long>(p.slot) * a.n + p.n0 + token) * a.heads + p.h * a.group + j - token * a.group;
+      return (static_cast<long long>(p.slot) * a.n + p.n0 + token) * a.heads + head * a.group + j - token * a.group;
     };
     if (p.k1 <= p.k0) {  // nothing here: the join skips the piece
-      for (int r = threadIdx.x; r < p.n_rows; r += kWorkers) a.part_ml[out_of(r)] = make_float2(-INFINITY, 0.f);
+      if (!idle)
+        for (int r = Quad ? lane : threadIdx.x; r < p.n_rows; r += Quad ? 32 : kWorkers) a.part_ml[out_of(r)] = make_float2(-INFINITY, 0.f);
       continue;
     }
     // Q as the products' first operand, straight from memory
@@ -210,9 +224,9 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int r = wr * 16 + gq + 8 * e, j = p.r0 + r, token = j / a.group;
-      const bool in = r < p.n_rows;
+      const bool in = r < p.n_rows && !idle;
       lim[e] = min(p.k1, p.limit0 + token);
-      const __nv_bfloat16* q = a.q + (p.n0 + token) * a.q_ld + (p.h * a.group + j - token * a.group) * a.q_head + 2 * tg;
+      const __nv_bfloat16* q = a.q + (p.n0 + token) * a.q_ld + (head * a.group + j - token * a.group) * a.q_head + 2 * tg;
 #pragma unroll
       for (int kc = 0; kc < D / 16; ++kc) {
         qf[kc][e] = in ? *reinterpret_cast<const uint32_t*>(q + kc * 16) : 0u;
@@ -225,16 +239,21 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
     float m_r[2] = {-INFINITY, -INFINITY}, l_r[2] = {0.f, 0.f};
     const bool lower = p.n_rows > wr * 16 + 8;  // whether the tile's rows 8 to 15 are any of ours
 
-    for (int t0 = p.k0; t0 < p.k1; t0 += kKeys, ++pos) {
+    for (int t0 = p.k0; t0 < p.k1; t0 += kStep, ++pos) {
       const int st = pos % kStages;
       mbar_wait(full0 + 8 * st, (pos / kStages) & 1, a.status);  // (a wait that gave up is in the status word)
       __syncwarp();
       const uint32_t sK = ring + st * 2 * R::tile, sV = sK + R::tile;
-      const bool part = p.k1 - t0 < kKeys;
+      if (idle) {
+        if (lane == 0) mbar_arrive(empty0 + 8 * st);
+        continue;
+      }
+      const bool part = p.k1 - t0 < kStep;
+      const int key0 = Quad ? t0 : t0 + wk * KW;  // this warp's first key
       if (part) {  // V rows past the end hold anything: this warp's become zeros
         for (int x = lane; x < KW * (D / 8); x += 32) {
-          const int r = wk * KW + x / (D / 8);
-          if (t0 + r >= p.k1) st_v4(sm + st * 2 * R::tile + R::tile + R::at(r, x % (D / 8)), make_uint4(0, 0, 0, 0));
+          const int r = x / (D / 8);
+          if (key0 + r >= p.k1) st_v4(sm + st * 2 * R::tile + R::tile + R::at(row0 + r, x % (D / 8)), make_uint4(0, 0, 0, 0));
         }
         __syncwarp();
       }
@@ -246,11 +265,11 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
 #pragma unroll
         for (int n = 0; n < KW / 16; ++n) {
           uint32_t b[4];
-          ldsm_x4(b, sK + R::at(wk * KW + n * 16 + (lane & 7) + (lane >> 4) * 8, kc * 2 + ((lane >> 3) & 1)));
+          ldsm_x4(b, sK + R::at(row0 + n * 16 + (lane & 7) + (lane >> 4) * 8, kc * 2 + ((lane >> 3) & 1)));
           mma_bf16(s[2 * n], qf[kc], b);
           mma_bf16(s[2 * n + 1], qf[kc], b + 2);
         }
-      const int j0 = t0 + wk * KW + 2 * tg;
+      const int j0 = key0 + 2 * tg;
       float mx[2] = {m_r[0], m_r[1]};
 #pragma unroll
       for (int n = 0; n < KW / 8; ++n)
@@ -292,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
           uint32_t b[4];
-          ldsm_x4_t(b, sV + R::at(wk * KW + n * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, d * 2 + (lane >> 4)));
+          ldsm_x4_t(b, sV + R::at(row0 + n * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, d * 2 + (lane >> 4)));
           mma_bf16(acc[2 * d], pa, b);
           mma_bf16(acc[2 * d + 1], pa, b + 2);
         }
@@ -345,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = wr * 16 + gq + 8 * e;
-        if (r >= p.n_rows) continue;
+        if (r >= p.n_rows || idle) continue;
         const long long out = out_of(r);
 #pragma unroll
         for (int d = 0; d < D / 8; ++d)
@@ -417,8 +436,8 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// A pool as (head_dim, heads, tokens, pages) in boxes of 64 values (or the head) and up to 64 tokens of one page.
-static bool pool_map(CUtensorMap* map, const __nv_bfloat16* base, const Args& a, int head_dim) {
+// A pool as (head_dim, heads, tokens, pages) in boxes of 64 values (or the head) and up to `tokens` of one page.
+static bool pool_map(CUtensorMap* map, const __nv_bfloat16* base, const Args& a, int head_dim, int tokens) {
   if (!encode_fn()) return false;
   const int page = 1 << a.page_shift;
   const cuuint64_t dims[4] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(a.kv_heads),
@@ -426,25 +445,25 @@ static bool pool_map(CUtensorMap* map, const __nv_bfloat16* base, const Args& a,
   // an axis of one entry may have any stride: give the map one that it accepts
   auto stride = [](long long n, long long ld) { return static_cast<cuuint64_t>(n > 1 ? ld * 2 : 16); };
   const cuuint64_t strides[3] = {stride(a.kv_heads, a.head_ld), stride(page, a.token_ld), stride(a.pages, a.page_ld)};
-  const cuuint32_t box[4] = {static_cast<cuuint32_t>(std::min(64, head_dim)), 1, static_cast<cuuint32_t>(std::min(page, kKeys)), 1};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(std::min(64, head_dim)), 1, static_cast<cuuint32_t>(std::min(page, tokens)), 1};
   const cuuint32_t each[4] = {1, 1, 1, 1};
   return encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<__nv_bfloat16*>(base), dims, strides, box, each,
                      CU_TENSOR_MAP_INTERLEAVE_NONE, head_dim == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D, int WR>
+template <int D, int WR, bool Quad>
 static cudaError_t launch_pieces(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
   const int rows_most = std::max(a.tensor_cores ? 0 : a.n * a.group, a.own_splits > 0 ? a.max_q * a.group : 0);
-  const int join_rows = WR == 4 ? 0 : std::min(16 * WR, rows_most);
+  const int join_rows = WR == 4 || Quad ? 0 : std::min(16 * WR, rows_most);
   const int known = a.own_splits > 0 && a.batch <= 1024 ? a.batch : 0;
   const int bytes = Ring<D, WR>::bytes + (4 / WR) * join_rows * ((D + 4) * 4 + 8) + (known ? (2 * known + 1) * 4 : 0) + 1024;
   const int items = (a.tensor_cores ? 0 : a.row_tiles * a.kv_heads * a.prefix_splits) +
-                    a.batch * a.own_tiles * a.own_splits * a.kv_heads;
+                    a.batch * a.own_tiles * a.own_splits * (Quad ? ceil_div(a.kv_heads, 4) : a.kv_heads);
   static SharedMemory allowed;
-  if (const cudaError_t e = allowed.at_least(reinterpret_cast<const void*>(pieces_kernel<D, WR>), bytes); e != cudaSuccess) return e;
+  if (const cudaError_t e = allowed.at_least(reinterpret_cast<const void*>(pieces_kernel<D, WR, Quad>), bytes); e != cudaSuccess) return e;
   const int per_sm = std::max(1, std::min(WR == 4 ? 2 : 3, 227 * 1024 / (bytes + 1024 + 64)));
-  pieces_kernel<D, WR><<<std::min(items, 148 * per_sm), kThreads, bytes, stream>>>(a, mk, mv, items, join_rows, known);
+  pieces_kernel<D, WR, Quad><<<std::min(items, 148 * per_sm), kThreads, bytes, stream>>>(a, mk, mv, items, join_rows, known);
   return cudaGetLastError();
 }
 
@@ -453,13 +472,17 @@ static cudaError_t launch_for(const Args& a, cudaStream_t stream) {
   cudaError_t e = cudaSuccess;
   CUtensorMap mk, mv;
   const bool by_warps = a.own_splits > 0 || (a.prefix_splits > 0 && !a.tensor_cores);
-  if (a.prefix_splits + a.own_splits > 0 && (!pool_map(&mk, a.k, a, D) || !pool_map(&mv, a.v, a, D))) return cudaErrorInvalidValue;
   if (by_warps) {
-    const int w = a.tile_rows / 16;
-    e = w == 1 ? launch_pieces<D, 1>(a, mk, mv, stream) : w == 2 ? launch_pieces<D, 2>(a, mk, mv, stream) : launch_pieces<D, 4>(a, mk, mv, stream);
+    const int w = a.tile_rows / 16, tokens = a.quad ? 16 : kKeys;
+    if (!pool_map(&mk, a.k, a, D, tokens) || !pool_map(&mv, a.v, a, D, tokens)) return cudaErrorInvalidValue;
+    e = a.quad ? launch_pieces<D, 1, true>(a, mk, mv, stream)
+        : w == 1 ? launch_pieces<D, 1, false>(a, mk, mv, stream)
+        : w == 2 ? launch_pieces<D, 2, false>(a, mk, mv, stream)
+                 : launch_pieces<D, 4, false>(a, mk, mv, stream);
     if (e != cudaSuccess) return e;
   }
   if (a.tensor_cores && a.prefix_splits > 0) {
+    if ((!by_warps || a.quad) && (!pool_map(&mk, a.k, a, D, kKeys) || !pool_map(&mv, a.v, a, D, kKeys))) return cudaErrorInvalidValue;
     e = launch_prefix_tc(a, mk, mv, D, stream);
     if (e != cudaSuccess || a.prefix_splits == 1) return e;
   }
@@ -477,9 +500,9 @@ static int tc_splits(int blocks, int tiles, long long rows, int head_dim, bool w
   for (int s = 1; s <= std::min(tiles, 64); ++s) {
     const int per = ceil_div(tiles, s), pieces = ceil_div(tiles, per);
     const int units = blocks * pieces, last = units % 148;
-    double waves = units / 148 + (last > 0);
-    if (pieces == 1 && last > 0 && 2 * last <= 148) waves -= 0.4;  // the last one in half the time (prefix_attention_tc.cu)
-    double us = waves * (per * tile_us + fixed_us);
+    double us = units / 148 * (per * tile_us + fixed_us);
+    // (a short last wave of a prefix in one piece has half the rows to a block: prefix_attention_tc.cu)
+    if (last > 0) us += per * (pieces == 1 && 2 * last <= 148 ? std::min(tile_us, 0.95) : tile_us) + fixed_us;
     if (pieces > 1) us += 3.0 + pieces * rows * head_dim * 8 / 6.5e6;
     if (us < least * 0.999) least = us, best = s;
   }
@@ -490,6 +513,7 @@ int plan(Args& a, int head_dim) {
   // Without tensor cores, pieces until every SM has about six, so that the last ones are short against the whole.
   constexpr int kWant = 148 * 6;
   a.prefix_splits = a.own_splits = 0;
+  a.quad = false;
   const long long rows = static_cast<long long>(a.n) * a.group;
   a.tensor_cores = a.prefix_len > 0 && head_dim != 32 && rows > kTensorCoreRows && a.scale_log2 >= 0.f;
   a.tile_rows = 16 * row_warps(static_cast<int>(a.tensor_cores || a.prefix_len == 0 ? static_cast<long long>(a.max_q) * a.group : rows));
@@ -514,6 +538,9 @@ int plan(Args& a, int head_dim) {
         std::max(1, std::min({tiles, 64, ceil_div(kWant, static_cast<long long>(a.batch) * a.own_tiles * a.kv_heads)}));
     a.own_chunk = ceil_div(tiles, splits) * kKeys;
     a.own_splits = ceil_div(a.max_len, a.own_chunk);
+    // Four heads to a piece where that still leaves every block (three on an SM) two pieces, and no prefix piece is there.
+    a.quad = (a.tensor_cores || a.prefix_len == 0) && a.tile_rows == 16 && a.kv_heads >= 3 &&
+             static_cast<long long>(a.batch) * a.own_tiles * a.own_splits * ceil_div(a.kv_heads, 4) >= 2 * 3 * 148;
   }
   return a.prefix_splits + a.own_splits;
 }

@@ -123,6 +123,10 @@ SHAPES = [
     ([40] * 9, [30] * 9, 1, 1, 128, 16, 400),  # 270 rows
     ([3] * 150, [1] * 150, 2, 1, 64, 32, 2000),
     ([31, 90, 500], [31, 77, 200], 1, 4, 64, 64, 191),
+    # many short sequences: four kv heads at a time, the last of them fewer
+    ([i % 37 for i in range(230)], [1] * 230, 13, 1, 64, 8, 70),
+    ([(7 * i) % 50 for i in range(225)], [1] * 225, 16, 2, 128, 32, 0),
+    ([(5 * i) % 21 for i in range(450)], [i % 3 for i in range(450)], 6, 3, 32, 16, 40),
 ]
 
 
