@@ -135,7 +135,8 @@ MNB_DEVICE Piece piece_of(const Args& a, const int* seq_lens, const int* q_offse
 //
 // Quad: a piece is four kv heads of one sequence, a stage 16 keys of each, and every warp works on a head of its own,
 // without a join: what a piece costs beside its keys is spent once for four heads, which decides where many sequences
-// are short (2048 sequences of 4 tokens, 16 heads: QUADBEFORE us without, QUADAFTER with).
+// are short (2048 sequences of 4 tokens, 16 heads, behind a prefix of 64: the
+// call 261 us without, 86 with).
 template <int D, int WR, bool Quad>
 __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
     pieces_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap map_k,
@@ -538,9 +539,12 @@ int plan(Args& a, int head_dim) {
         std::max(1, std::min({tiles, 64, ceil_div(kWant, static_cast<long long>(a.batch) * a.own_tiles * a.kv_heads)}));
     a.own_chunk = ceil_div(tiles, splits) * kKeys;
     a.own_splits = ceil_div(a.max_len, a.own_chunk);
-    // Four heads to a piece where that still leaves every block (three on an SM) two pieces, and no prefix piece is there.
+    // Four heads to a piece, where no prefix piece is in the list.  Short sequences (two stages of 64 keys and less) gain
+    // as soon as every SM has such a piece: 192 of 4 tokens, 16 heads, 34 us without and 19 with.  Long ones need two for
+    // each of an SM's three blocks: 192 of 201 tokens on average, 768 such pieces, lost 4 %.
+    const long long quads = static_cast<long long>(a.batch) * a.own_tiles * a.own_splits * ceil_div(a.kv_heads, 4);
     a.quad = (a.tensor_cores || a.prefix_len == 0) && a.tile_rows == 16 && a.kv_heads >= 3 &&
-             static_cast<long long>(a.batch) * a.own_tiles * a.own_splits * ceil_div(a.kv_heads, 4) >= 2 * 3 * 148;
+             quads >= (a.max_len <= 2 * kKeys ? 148 : 2 * 3 * 148);
   }
   return a.prefix_splits + a.own_splits;
 }
