@@ -22,8 +22,13 @@ void check_int32(const torch::Tensor& t, int64_t dim, const torch::Tensor& like,
 }
 
 void check_status_word(const torch::Tensor& status) {
-  TORCH_CHECK(status.is_cuda() && status.scalar_type() == at::kInt && status.numel() >= 1, "status: int32 on the device");
+  TORCH_CHECK(status.is_cuda() && status.scalar_type() == at::kInt && status.numel() >= 3, "status: int32 on the device");
 }
+
+// A device's status: word 0 is a pipeline wait that ran out, which makes every other wait give up too; word 2 a request
+// that a kernel left out, which must not.
+int* waits_of(const torch::Tensor& status) { return status.data_ptr<int>(); }
+int* errors_of(const torch::Tensor& status) { return status.data_ptr<int>() + 2; }
 
 // 16-byte accesses along the last axis work at every index.
 bool rows_aligned(const torch::Tensor& t) {
@@ -88,7 +93,7 @@ void copy_pages(const torch::Tensor& kv, const torch::Tensor& src, const torch::
   TORCH_CHECK_VALUE(src.size(0) == dst.size(0), "src and dst: one destination for each source");
   const c10::cuda::CUDAGuard guard(kv.device());
   C10_CUDA_CHECK(cache::launch_copy(p, src.data_ptr<int>(), dst.data_ptr<int>(), nullptr, nullptr,
-                                    static_cast<int>(src.size(0)), status.data_ptr<int>(), at::cuda::getCurrentCUDAStream()));
+                                    static_cast<int>(src.size(0)), errors_of(status), at::cuda::getCurrentCUDAStream()));
 }
 
 void fork_sequences(const torch::Tensor& kv, const torch::Tensor& page_table, const torch::Tensor& lens, const torch::Tensor& refs,
@@ -107,7 +112,7 @@ void fork_sequences(const torch::Tensor& kv, const torch::Tensor& page_table, co
   const c10::cuda::CUDAGuard guard(kv.device());
   auto scratch = at::empty({4 * n + t.slots}, parents.options());
   C10_CUDA_CHECK(cache::launch_fork(p, t, parents.data_ptr<int>(), children.data_ptr<int>(), static_cast<int>(n),
-                                    scratch.data_ptr<int>(), status.data_ptr<int>(), at::cuda::getCurrentCUDAStream()));
+                                    scratch.data_ptr<int>(), errors_of(status), at::cuda::getCurrentCUDAStream()));
 }
 
 void reserve_pages(const torch::Tensor& page_table, const torch::Tensor& lens, const torch::Tensor& refs, const torch::Tensor& slots,
@@ -123,7 +128,7 @@ void reserve_pages(const torch::Tensor& page_table, const torch::Tensor& lens, c
   const c10::cuda::CUDAGuard guard(page_table.device());
   auto scratch = at::empty({t.pages + n + t.slots}, slots.options());
   C10_CUDA_CHECK(cache::launch_reserve(t, slots.data_ptr<int>(), counts.data_ptr<int>(), static_cast<int>(n),
-                                       scratch.data_ptr<int>(), status.data_ptr<int>(), at::cuda::getCurrentCUDAStream()));
+                                       scratch.data_ptr<int>(), errors_of(status), at::cuda::getCurrentCUDAStream()));
 }
 
 void free_sequences(const torch::Tensor& page_table, const torch::Tensor& lens, const torch::Tensor& refs, const torch::Tensor& slots,
@@ -134,7 +139,7 @@ void free_sequences(const torch::Tensor& page_table, const torch::Tensor& lens, 
   const int n = static_cast<int>(slots.size(0));
   if (n == 0 || t.columns == 0) return;
   const c10::cuda::CUDAGuard guard(page_table.device());
-  C10_CUDA_CHECK(cache::launch_free(t, slots.data_ptr<int>(), n, status.data_ptr<int>(), at::cuda::getCurrentCUDAStream()));
+  C10_CUDA_CHECK(cache::launch_free(t, slots.data_ptr<int>(), n, errors_of(status), at::cuda::getCurrentCUDAStream()));
 }
 
 std::tuple<torch::Tensor, torch::Tensor> compact_pages(const torch::Tensor& kv, const torch::Tensor& page_table, const torch::Tensor& refs,
@@ -151,7 +156,7 @@ std::tuple<torch::Tensor, torch::Tensor> compact_pages(const torch::Tensor& kv, 
   C10_CUDA_CHECK(cache::launch_compact(p, page_table.data_ptr<int>(), page_table.stride(0),
                                        static_cast<int>(page_table.size(0)), static_cast<int>(page_table.size(1)),
                                        refs.data_ptr<int>(), new_table.data_ptr<int>(), new_refs.data_ptr<int>(),
-                                       scratch.data_ptr<int>(), status.data_ptr<int>(), at::cuda::getCurrentCUDAStream()));
+                                       scratch.data_ptr<int>(), errors_of(status), at::cuda::getCurrentCUDAStream()));
   return {new_table, new_refs};
 }
 
@@ -205,7 +210,7 @@ void append_kv(const torch::Tensor& k_pages, const torch::Tensor& v_pages, const
   a.n = static_cast<int>(n);
   a.heads = static_cast<int>(H);
   a.chunks = static_cast<int>(D / 8);
-  C10_CUDA_CHECK(cache::launch_append(a, status.data_ptr<int>(), at::cuda::getCurrentCUDAStream()));
+  C10_CUDA_CHECK(cache::launch_append(a, errors_of(status), at::cuda::getCurrentCUDAStream()));
 }
 
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>> sample(
@@ -225,7 +230,7 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> sample(
   TORCH_CHECK_VALUE(R < (1ll << 31), "too many rows");
   check_status_word(status);
   sampling::Sample a{};
-  a.status = status.data_ptr<int>();
+  a.status = waits_of(status);
   a.temperature = setting<Setting>(temperature, temperature_all, R, at::kFloat, logits, "temperature");
   a.top_k = setting<sampling::WholeSetting>(top_k, static_cast<double>(std::clamp<int64_t>(top_k_all, 0, V)), R, at::kInt,
                                             logits, "top_k");
@@ -323,7 +328,8 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(
   a.max_q = static_cast<int>(std::min(max_q_len, N));
   a.max_len = static_cast<int>(max_seq_len);
   a.scale_log2 = static_cast<float>(scale * kLog2e);
-  a.status = status.data_ptr<int>();
+  a.status = waits_of(status);
+  a.errors = errors_of(status);
   a.o = bf16(o);
   a.lse = lse ? lse->data_ptr<float>() : nullptr;
   const int64_t pieces = prefix::plan(a, static_cast<int>(D)), rows = N * H;

@@ -114,7 +114,8 @@ struct Args {
   float2* part_ml;  // [pieces][n][heads]: maximum (log2 units) and sum
   __nv_bfloat16* o;
   float* lse;  // or null
-  int* status;
+  int* status;  // of waits
+  int* errors;  // of bad indices
 };
 
 // Splits the keys into pieces; returns how many partial results each row gets.

@@ -72,7 +72,7 @@ struct Piece {
 };
 constexpr int kUnlimited = 1 << 30;
 
-MNB_DEVICE void flag(const Args& a) { atomicCAS(a.status, 0, kErrBadIndex); }
+MNB_DEVICE void flag(const Args& a) { atomicCAS(a.errors, 0, kErrBadIndex); }
 
 // Item i of the list: first the prefix's (split, kv head, row tile; the row tiles of the same keys side by side), then
 // the sequences' own (sequence, row tile, split, kv head).

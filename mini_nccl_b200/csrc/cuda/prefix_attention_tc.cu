@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int j = j0 + lane * per;
         int page = a.prefix_pages[j >> a.page_shift];
         if (page < 0 || page >= a.pages) {
-          atomicCAS(a.status, 0, kErrBadIndex);
+          atomicCAS(a.errors, 0, kErrBadIndex);
           page = a.pages;  // outside the map: reads as zeros
         }
 #pragma unroll

@@ -76,11 +76,12 @@ def check_status(device: torch.device | None = None) -> None:
     for idx, st in _STATUS.items():
         if device is not None and device.index not in (None, idx):
             continue
-        v = int(st[0].item())
-        if v:
+        v, _, left_out, _ = st.tolist()
+        if v or left_out:
             st.zero_()
-            if v in _CACHE_STATUS:
-                raise RuntimeError(f"cache operation on cuda:{idx}: {_CACHE_STATUS[v]}")
+        if left_out:
+            raise RuntimeError(f"cache operation on cuda:{idx}: {_CACHE_STATUS.get(left_out, left_out)}")
+        if v:
             raise RuntimeError(f"GEMM kernel on cuda:{idx} reported pipeline status {v}")
 
 

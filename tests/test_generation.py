@@ -624,3 +624,59 @@ def test_cache_class(device):
                  lambda: G.PagedKVCache(1, 4, 12, 1, 32, max_seqs=1, max_seq_len=8, device=device)):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(4))
+def test_page_operations_agree_bit_for_bit_with_the_plain_ones(seed):
+    """A run of random operations on both: every value of the pool and the books stays the same, unused pages included."""
+    rng = random.Random(seed)
+    page, heads, dim = rng.choice([(8, 3, 16), (16, 2, 64), (5, 1, 8)])
+    kv = torch.randn(3, 2, 400, page, heads, dim).to(torch.bfloat16)
+    S, W = 300, 9
+    sides = []
+    for device in ("cpu", "cuda"):
+        sides.append([kv.clone().to(device), ints([[-1] * W] * S, device), ints([0] * S, device), ints([0] * 400, device)])
+    lens = [0] * S
+    for _ in range(25):
+        live = [s for s in range(S) if lens[s]]
+        op = rng.choice(["grow", "grow", "fork", "free", "compact", "append"])
+        if op == "grow":
+            slots = rng.sample(range(S), rng.randrange(1, 12))
+            counts = [rng.randrange(0, min(2 * page, W * page - lens[s]) + 1) for s in slots]
+            if sum(-(-c // page) + 1 for c in counts) > int((sides[0][3] == 0).sum()):
+                continue
+            for k, t, n, r in sides:
+                G.reserve_pages(t, n, r, ints(slots, t.device), ints(counts, t.device), page)
+            for s, c in zip(slots, counts):
+                lens[s] += c
+        elif op == "fork" and live:
+            empty = [s for s in range(S) if not lens[s]]
+            children = rng.sample(empty, min(len(empty), rng.choice([1, 5, 270])))
+            children = children[: int((sides[0][3] == 0).sum())]
+            parents = [rng.choice(live) for _ in children]
+            for k, t, n, r in sides:
+                G.fork_sequences(k, t, n, r, ints(parents, t.device), ints(children, t.device))
+            for p, c in zip(parents, children):
+                lens[c] = lens[p]
+        elif op == "free" and live:
+            gone = rng.sample(live, max(1, len(live) // 2))
+            for k, t, n, r in sides:
+                G.free_sequences(t, n, r, ints(gone, t.device))
+            for s in gone:
+                lens[s] = 0
+        elif op == "compact":
+            for side in sides:
+                side[1], side[3] = G.compact_pages(side[0], side[1], side[3])
+        elif op == "append" and live:
+            # only pages with one holder may be written
+            alone = [s for s in live if int(sides[0][3][int(sides[0][1][s, (lens[s] - 1) // page])]) == 1]
+            if not alone:
+                continue
+            new = torch.randn(len(alone), 2, heads, dim).to(torch.bfloat16)
+            for k, t, n, r in sides:
+                x = new.to(t.device)
+                G.append_kv(k[1, 0], k[1, 1], x[:, 0], x[:, 1], t, ints([lens[s] - 1 for s in alone], t.device), ints(alone, t.device))
+        settle("cuda")
+        for a, b in zip(*sides):
+            assert torch.equal(a, b.cpu()), op
