@@ -143,6 +143,10 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
                   const __grid_constant__ CUtensorMap map_v, int items, int join_rows, int known) {
   using R = Ring<D, WR>;
   constexpr int WK = Quad ? 1 : 4 / WR, KW = Quad ? 16 : kKeys / WK, kStages = R::stages, kPitch = D + 4;
+  // Tiles of 64 rows of one kv head hold triangles: a warp leaves out the keys that none of its 16 rows sees (16 x 512
+  // tokens, 16 heads of 128: 65.6 us with, 69.2 without; 9 x 65 tokens of 24 heads 26.2 and 28.8).  Not at head dim 64
+  // (44.8 and 43.6) nor in smaller tiles, where it costs registers (192 single tokens 99 and 95).
+  constexpr bool kSkip = WR == 4 && D == 128;
   constexpr int kStep = Quad ? 16 : kKeys, kHeads = Quad ? 4 : 1;  // keys and heads of a stage; head y's keys are rows 16 y on
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -203,11 +207,12 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
     return;
   }
 
-  const int wr = Quad ? 0 : warp % WR, wk = Quad ? 0 : warp / WR, gq = lane / 4, tg = lane % 4;
+  const int wk = Quad ? 0 : warp / WR, gq = lane / 4, tg = lane % 4;
   const int row0 = Quad ? warp * 16 : wk * KW;  // of this warp's keys in a stage
   for (int i = blockIdx.x; i < items; i += gridDim.x) {
     const Piece p = piece_of(a, seq_lens, q_offsets, i, 16 * WR, kHeads);
     if (p.n_rows <= 0) continue;
+    const int wr = Quad ? 0 : (kSkip ? warp + pos : warp) % WR;  // rows in turn: a triangle's last ones have the most keys
     const int head = Quad ? p.h + warp : p.h;
     const bool idle = Quad && head >= a.kv_heads;  // the last four heads may be fewer
     auto out_of = [&](int r) {
@@ -238,6 +243,8 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
 #pragma unroll
     for (int d = 0; d < D / 8; ++d) acc[d][0] = acc[d][1] = acc[d][2] = acc[d][3] = 0.f;
     float m_r[2] = {-INFINITY, -INFINITY}, l_r[2] = {0.f, 0.f};
+    // the end of the keys that any of this warp's rows sees
+    const int top = !kSkip ? p.k1 : wr * 16 < p.n_rows ? min(p.k1, p.limit0 + (p.r0 + min(wr * 16 + 15, p.n_rows - 1)) / a.group) : p.k0;
     const bool lower = p.n_rows > wr * 16 + 8;  // whether the tile's rows 8 to 15 are any of ours
 
     for (int t0 = p.k0; t0 < p.k1; t0 += kStep, ++pos) {
@@ -245,12 +252,13 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
       mbar_wait(full0 + 8 * st, (pos / kStages) & 1, a.status);  // (a wait that gave up is in the status word)
       __syncwarp();
       const uint32_t sK = ring + st * 2 * R::tile, sV = sK + R::tile;
-      if (idle) {
+      const int key0 = Quad ? t0 : t0 + wk * KW;  // this warp's first key
+      const int live = top - key0;
+      if (idle || (kSkip && live <= 0)) {
         if (lane == 0) mbar_arrive(empty0 + 8 * st);
         continue;
       }
       const bool part = p.k1 - t0 < kStep;
-      const int key0 = Quad ? t0 : t0 + wk * KW;  // this warp's first key
       if (part) {  // V rows past the end hold anything: this warp's become zeros
         for (int x = lane; x < KW * (D / 8); x += 32) {
           const int r = x / (D / 8);
@@ -262,14 +270,16 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
 #pragma unroll
       for (int n = 0; n < KW / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
-      for (int kc = 0; kc < D / 16; ++kc)
+      for (int n = 0; n < KW / 16; ++n) {
+        if (kSkip && n * 16 >= live) break;
 #pragma unroll
-        for (int n = 0; n < KW / 16; ++n) {
+        for (int kc = 0; kc < D / 16; ++kc) {
           uint32_t b[4];
           ldsm_x4(b, sK + R::at(row0 + n * 16 + (lane & 7) + (lane >> 4) * 8, kc * 2 + ((lane >> 3) & 1)));
           mma_bf16(s[2 * n], qf[kc], b);
           mma_bf16(s[2 * n + 1], qf[kc], b + 2);
         }
+      }
       const int j0 = key0 + 2 * tg;
       float mx[2] = {m_r[0], m_r[1]};
 #pragma unroll
@@ -307,6 +317,7 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
       }
 #pragma unroll
       for (int n = 0; n < KW / 16; ++n) {
+        if (kSkip && n * 16 >= live) break;
         const uint32_t pa[4] = {pack_bf16x2(s[2 * n][0], s[2 * n][1]), pack_bf16x2(s[2 * n][2], s[2 * n][3]),
                                 pack_bf16x2(s[2 * n + 1][0], s[2 * n + 1][1]), pack_bf16x2(s[2 * n + 1][2], s[2 * n + 1][3])};
 #pragma unroll
