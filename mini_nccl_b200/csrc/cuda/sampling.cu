@@ -30,8 +30,8 @@
 // None is bound by its bytes: a row is a chain of passes, and the instructions
 // of the passes (12 an element to count, 13 to split, 11 to score) fill the
 // issue slots of the two blocks that share an SM.  A row's blocks exchange
-// values four to eight times at about a microsecond each, so a row gets the
-// fewest blocks that hold it: 512 rows of 50304 in clusters of 1, 2, 4 and 8
+// values four to eight times at about a microsecond each, so where
+// rows fill the GPU each gets the fewest blocks that hold it: 512 rows of 50304 in clusters of 1, 2, 4 and 8
 // blocks took 112, 171, 298 and 562 us.
 // Weights and sums are fp32, in a fixed order, so results do not depend on
 // scheduling; the winning score is IEEE fp32 division and addition.
@@ -128,6 +128,7 @@ struct Shared : Lists<Multi> {
   } red;
   uint64_t from[2][kMaxCluster];  // one value of every block of the cluster, in turn in two places
   uint64_t from_too[2][kMaxCluster];
+  int counted[2][kWarps];         // warps' counts, in turn in two places
   uint64_t joined[2];             // mbarriers of these exchanges
   uint64_t arrived[kChunks];      // mbarriers of the bulk copies
   int n_mine;
@@ -146,6 +147,14 @@ MNB_DEVICE V block_reduce(V v, V* sh, F f) {
   for (int o = kWarps / 2; o > 0; o >>= 1) s = f(s, __shfl_xor_sync(0xffffffffu, s, o));
   __syncthreads();
   return s;
+}
+// The sum with one barrier; the next call takes other places.
+MNB_DEVICE int block_count(int n, int* sh) {
+  n = __reduce_add_sync(0xffffffffu, n);
+  if (threadIdx.x % 32 == 0) sh[threadIdx.x / 32] = n;
+  __syncthreads();
+  const int lane = threadIdx.x % 32;
+  return __reduce_add_sync(0xffffffffu, lane < kWarps ? sh[lane] : 0);
 }
 // The same over the cluster: every block sends its value to all by asynchronous remote stores, which the receivers'
 // mbarriers count, and joins what it got in the blocks' order.
@@ -667,12 +676,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           for (int q = 0; q < kSets; ++q) key[q] = q < cluster ? key_of(sh.maxima[q][tid]) : 0u;
         }
         uint32_t hi = key_of(mx);
+        int turn = 0;
         while (lo < hi) {  // the largest bound that at least k maxima reach
           const uint32_t mid = lo + (hi - lo + 1) / 2;
-          int n = 0;
+          int n;
+          if constexpr (Multi) {
+            n = 0;
 #pragma unroll
-          for (int q = 0; q < kSets; ++q)
-            if (q < cluster) n += __syncthreads_count(key[q] >= mid);
+            for (int q = 0; q < kSets; ++q) n += key[q] >= mid;  // (mid is above the 0 of blocks that are not there)
+            n = block_count(n, sh.counted[turn]);
+            turn ^= 1;
+          } else {
+            n = __syncthreads_count(key[0] >= mid);
+          }
           if (n >= k) {
             lo = mid;
             if (n <= k + k / 8) break;
@@ -1031,15 +1047,20 @@ template <typename T>
 static cudaError_t launch(const Sample& a, cudaStream_t stream) {
   // Blocks per row: as few as hold it, because what the blocks of a cluster exchange costs several microseconds a row;
   // a block has an SM to itself while there are at most 148, then half of one.  More only while SMs are idle and a
-  // thread has over 16 pieces to go through.
+  // thread has over 16 pieces to go through.  Where no row asks for top-k (whose exchange is the dearest) and a thread
+  // would have over 6 of the whole row, as many as fit 128 SMs: 1 x 50304 bf16, 1 and 8 blocks, takes 13.7 and 7.6 us
+  // without filters, 26.7 and 21.9 with top-p, 10.5 and 14.5 with top-k 50; 1 x 16384 with top-p 15.9 and 19.9; 18
+  // rows of 32000 in 8 blocks (144, which clusters of 8 do not fill in one wave) 24.7, in 4 19.9.
   auto room = [](size_t shared, int per_sm) { return (227 * 1024 / per_sm - static_cast<int>(shared) - 1024) / 16; };  // pieces
   const int pieces = static_cast<int>((static_cast<long long>(a.vocab) * sizeof(T) + 15) / 16 + 1);
+  const bool spread = !a.top_k.each && !a.top_k.all && pieces > 6 * kThreads;
   int cluster = 1, slice = pieces;
   for (;; cluster *= 2) {
     slice = (pieces + cluster - 1) / cluster;
     const long long blocks = static_cast<long long>(a.rows) * cluster;
     const bool fits = slice <= room(cluster > 1 ? sizeof(Shared<true>) : sizeof(Shared<false>), blocks <= 148 ? 1 : 2);
-    if (cluster == kMaxCluster || (fits && (2 * blocks > 148 || slice <= 16 * kThreads))) break;
+    const bool more = (slice > 16 * kThreads && 2 * blocks <= 148) || (spread && 2 * blocks <= 128);
+    if (cluster == kMaxCluster || (fits && !more)) break;
   }
   const bool staged = slice <= std::min(kChunk * kChunks, room(sizeof(Shared<true>), 1));
   if (cluster == 1) return launch_with<T, true, false>(a, 1, slice * 16, stream);

@@ -179,7 +179,9 @@ def sample(
     the one with the lowest index: with ``noise`` from the standard Gumbel
     distribution, fp32 ``[rows, vocabulary]``, that is a draw from the
     filtered softmax, and the same noise gives the same token whatever the
-    batch.  A temperature of 0 (or less) takes the first token.  Each setting
+    batch (except that ``top_p`` compares fp32 sums, whose order depends on the
+    number of rows: a token within their rounding of the cut may fall on either
+    side).  A temperature of 0 (or less) takes the first token.  Each setting
     is a number or a tensor with one entry for each row (fp32; ``top_k``
     int32).  Logits of ``-inf`` and NaN are never drawn, and a row without any
     other returns token -1.

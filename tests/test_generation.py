@@ -329,6 +329,19 @@ def test_sample_row_splits(device, rows, vocab):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("rows,vocab,dtype", [(1, 12288, torch.float32), (1, 25013, torch.bfloat16), (9, 17001, torch.float32),
+                                              (17, 26000, torch.bfloat16), (35, 13001, torch.float32)])
+def test_sample_few_rows_without_top_k(device, rows, vocab, dtype):
+    # settings as numbers, so that a row may be spread over more blocks than hold it
+    x, noise = logits_of(rows, vocab, dtype, seed=vocab)
+    x[0, 5:] = x[0, 5]  # ties across the blocks' slices
+    if rows > 1:
+        x[1] = -math.inf
+    for T, p, least in ((0.8, 1.0, 0.0), (1.0, 0.9, 0.0), (1.3, 0.99, 0.02), (0.0, 1.0, 0.0)):
+        check_sample(device, x, noise, T, 0, p, least, tensors=False)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("spread", [1e-3, 0.1])
 def test_sample_nearly_flat_rows(device, spread):
     # thousands of tokens within one bin of the log-weight, a far maximum, and the type's lowest value as a mask
