@@ -131,7 +131,8 @@ MNB_DEVICE Piece piece_of(const Args& a, const int* seq_lens, const int* q_offse
 // long (604 MB): 104 us, 5.8 TB/s, so what short sequences lose is the last stage of each, which costs a warp as much
 // as a full one (some 400 instructions at 1.5 a cycle).  Blocks fetching their pieces from the hardware's work queue
 // instead of in turn were no faster, and neither were keys laid out head by head.  2388 rows of 24 sequences in tiles
-// of 64 (masked triangles, 14 GFLOP as computed): 80 us, bound by the latency of eight working warps per SM.
+// of 64 (masked triangles): 78 us under ncu (88 with the keys
+// that a warp's rows do not see computed too), bound by the latency of eight working warps per SM.
 //
 // Quad: a piece is four kv heads of one sequence, a stage 16 keys of each, and every warp works on a head of its own,
 // without a join: what a piece costs beside its keys is spent once for four heads, which decides where many sequences
