@@ -19,7 +19,7 @@ int colsum_row_blocks(int rows);
 void bias_grad(torch::Tensor g, torch::Tensor out, torch::Tensor partials, bool accumulate);
 void gelu_fwd(torch::Tensor x, torch::Tensor y);
 void gelu_bwd(torch::Tensor x, torch::Tensor dy, torch::Tensor dx);
-void embed_fwd(torch::Tensor idx, torch::Tensor wte, torch::Tensor wpe, torch::Tensor y);
+void embed_fwd(torch::Tensor idx, torch::Tensor wte, torch::Tensor wpe, torch::Tensor y, torch::Tensor status);
 void embed_bwd(torch::Tensor idx, torch::Tensor dy, torch::Tensor dwte, torch::Tensor dwpe, bool accumulate_pos);
 void xent_fwd_bwd(torch::Tensor logits, torch::Tensor targets, torch::Tensor loss, double grad_scale,
                   int64_t ignore_index);

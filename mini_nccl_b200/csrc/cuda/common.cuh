@@ -24,7 +24,7 @@ enum : int {
   kErrPipelineTimeout = 2, // an intra-CTA mbarrier wait exceeded its budget
   kErrBadArgument = 3,
   kErrNoPages = 4,         // the key / value cache's pool has too few free pages
-  kErrBadIndex = 5,        // a page, slot, position or length outside its tensor
+  kErrBadIndex = 5,        // a token, page, slot, position or length outside its tensor
 };
 
 // ---------------------------------------------------------------------------

@@ -645,18 +645,22 @@ __global__ void gelu_bwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_
 
 // ---------------------------------------------------------------------------
 // Embedding: y[b, t] = wte[idx[b, t]] + wpe[t]
+// An id that is no row of wte (the sampler's -1 for a row of logits with nothing to draw) reads as a zero vector, gets no
+// gradient and is reported in `errors`.
 // ---------------------------------------------------------------------------
 __global__ void embed_fwd_kernel(const int64_t* __restrict__ idx, const __nv_bfloat16* __restrict__ wte,
                                  const __nv_bfloat16* __restrict__ wpe, __nv_bfloat16* __restrict__ y, int tokens,
-                                 int T, int C) {
+                                 int T, int C, int64_t vocab, int* errors) {
   const int row = blockIdx.x * kRowWarps + threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
   if (row >= tokens) return;
   const long long tok = idx[row];
+  const bool known = tok >= 0 && tok < vocab;
+  if (!known && lane == 0) atomicCAS(errors, 0, kErrBadIndex);
   const int t = row % T;
   for (int c = lane * 8; c < C; c += 256) {
-    float a[8], p[8];
-    load8(wte + tok * C + c, a);
+    float a[8] = {0, 0, 0, 0, 0, 0, 0, 0}, p[8];
+    if (known) load8(wte + tok * C + c, a);
     load8(wpe + static_cast<long long>(t) * C + c, p);
 #pragma unroll
     for (int j = 0; j < 8; ++j) a[j] += p[j];
@@ -666,11 +670,12 @@ __global__ void embed_fwd_kernel(const int64_t* __restrict__ idx, const __nv_bfl
 
 // dwte[idx] += dy (bf16x2 atomics, collisions are rare for real token streams);
 __global__ void embed_bwd_tok_kernel(const int64_t* __restrict__ idx, const __nv_bfloat16* __restrict__ dy,
-                                     __nv_bfloat16* __restrict__ dwte, int tokens, int C) {
+                                     __nv_bfloat16* __restrict__ dwte, int tokens, int C, int64_t vocab) {
   const int row = blockIdx.x * kRowWarps + threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
   if (row >= tokens) return;
   const long long tok = idx[row];
+  if (tok < 0 || tok >= vocab) return;
   for (int c = lane * 2; c < C; c += 64) {
     __nv_bfloat162 g = *reinterpret_cast<const __nv_bfloat162*>(dy + static_cast<long long>(row) * C + c);
     atomicAdd(reinterpret_cast<__nv_bfloat162*>(dwte + tok * C + c), g);
@@ -1215,10 +1220,11 @@ void gelu_bwd(torch::Tensor x, torch::Tensor dy, torch::Tensor dx) {
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-void embed_fwd(torch::Tensor idx, torch::Tensor wte, torch::Tensor wpe, torch::Tensor y) {
+void embed_fwd(torch::Tensor idx, torch::Tensor wte, torch::Tensor wpe, torch::Tensor y, torch::Tensor status) {
   check_bf16(wte, "wte");
   check_bf16(wpe, "wpe");
   TORCH_CHECK(idx.scalar_type() == at::kLong && idx.is_contiguous(), "idx must be int64");
+  TORCH_CHECK(status.is_cuda() && status.scalar_type() == at::kInt && status.numel() >= 3, "status: int32 on the device");
   const int T = static_cast<int>(idx.size(-1));
   const int C = static_cast<int>(wte.size(1));
   const int tokens = static_cast<int>(idx.numel());
@@ -1226,7 +1232,7 @@ void embed_fwd(torch::Tensor idx, torch::Tensor wte, torch::Tensor wpe, torch::T
   embed_fwd_kernel<<<(tokens + kRowWarps - 1) / kRowWarps, kRowWarps * 32, 0, at::cuda::getCurrentCUDAStream()>>>(
       idx.data_ptr<int64_t>(), reinterpret_cast<const __nv_bfloat16*>(wte.data_ptr()),
       reinterpret_cast<const __nv_bfloat16*>(wpe.data_ptr()), reinterpret_cast<__nv_bfloat16*>(y.data_ptr()), tokens,
-      T, C);
+      T, C, wte.size(0), status.data_ptr<int>() + 2);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
@@ -1240,7 +1246,7 @@ void embed_bwd(torch::Tensor idx, torch::Tensor dy, torch::Tensor dwte, torch::T
   auto stream = at::cuda::getCurrentCUDAStream();
   embed_bwd_tok_kernel<<<(tokens + kRowWarps - 1) / kRowWarps, kRowWarps * 32, 0, stream>>>(
       idx.data_ptr<int64_t>(), reinterpret_cast<const __nv_bfloat16*>(dy.data_ptr()),
-      reinterpret_cast<__nv_bfloat16*>(dwte.data_ptr()), tokens, C);
+      reinterpret_cast<__nv_bfloat16*>(dwte.data_ptr()), tokens, C, dwte.size(0));
   embed_bwd_pos_kernel<<<T, 128, 0, stream>>>(reinterpret_cast<const __nv_bfloat16*>(dy.data_ptr()),
                                              reinterpret_cast<__nv_bfloat16*>(dwpe.data_ptr()), B, T, C,
                                              accumulate_pos ? 1 : 0);

@@ -66,13 +66,13 @@ def fold_accumulator(device: torch.device, n: int) -> torch.Tensor:
     return buf
 
 
-#: Status codes of the page operations and the paged attention (csrc/cuda/common.cuh).
-_CACHE_STATUS = {4: "the key / value cache's pool has too few free pages",
-                 5: "a page, slot, position or length outside its tensor"}
+#: Status codes of the page operations, the paged attention and the embedding (csrc/cuda/common.cuh).
+_REQUEST_STATUS = {4: "the key / value cache's pool has too few free pages",
+                   5: "a token, page, slot, position or length outside its tensor"}
 
 
 def check_status(device: torch.device | None = None) -> None:
-    """Raise if a GEMM pipeline wait ran out of budget, or a cache operation left a request out (device sync)."""
+    """Raise if a GEMM pipeline wait ran out of budget, or an operation left a request out (device sync)."""
     for idx, st in _STATUS.items():
         if device is not None and device.index not in (None, idx):
             continue
@@ -80,7 +80,7 @@ def check_status(device: torch.device | None = None) -> None:
         if v or left_out:
             st.zero_()
         if left_out:
-            raise RuntimeError(f"cache operation on cuda:{idx}: {_CACHE_STATUS.get(left_out, left_out)}")
+            raise RuntimeError(f"request left out on cuda:{idx}: {_REQUEST_STATUS.get(left_out, left_out)}")
         if v:
             raise RuntimeError(f"GEMM kernel on cuda:{idx} reported pipeline status {v}")
 
@@ -475,13 +475,16 @@ class HeadCrossEntropy(torch.autograd.Function):
 
 
 class Embedding(torch.autograd.Function):
-    """``wte[idx] + wpe[:T]`` for ``idx`` of shape ``[B, T]``."""
+    """``wte[idx] + wpe[:T]`` for ``idx`` of shape ``[B, T]``.
+
+    An id outside ``wte`` reads as a zero vector and is reported by :func:`check_status`.
+    """
 
     @staticmethod
     def forward(ctx, idx, wte, wpe):
         B, T = idx.shape
         y = torch.empty((B, T, wte.shape[1]), dtype=wte.dtype, device=wte.device)
-        ext().embed_fwd(idx.contiguous(), wte, wpe, y)
+        ext().embed_fwd(idx.contiguous(), wte, wpe, y, status_word(wte.device))
         ctx.save_for_backward(idx)
         ctx.shapes = (wte.shape, wpe.shape)
         return y

@@ -1,0 +1,67 @@
+"""Edges of the generation operators: special values, damaged requests, bounds, and forms that few calls reach.
+
+The references are in 64 bits; tolerances as in ``test_generation.py``.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from mini_nccl_b200.ops import generation as G
+from test_generation import DEVICES, Books, Problem, ints, logits_of, settle
+
+
+def out_of_range(device, call, match="outside its tensor"):
+    """The call raises (CPU), or is reported afterwards (GPU); returns what it returned on the GPU."""
+    if device == "cpu":
+        with pytest.raises((RuntimeError, IndexError)):
+            call()
+        return None
+    from mini_nccl_b200.ops import kernels as K
+
+    out = call()
+    with pytest.raises(RuntimeError, match=match):
+        K.check_status()
+    return out
+
+
+# ---- tokens that are none ----------------------------------------------------------------
+
+
+@pytest.mark.gpu
+def test_embedding_reports_ids_outside_the_table():
+    from mini_nccl_b200.ops import kernels as K
+
+    wte = torch.randn(40, 24, device="cuda").to(torch.bfloat16).requires_grad_()
+    wpe = torch.randn(4, 24, device="cuda").to(torch.bfloat16).requires_grad_()
+    idx = torch.tensor([[3, -1, 39, 40], [1 << 40, 0, -(1 << 50), 7]], device="cuda")
+    y = out_of_range("cuda", lambda: K.Embedding.apply(idx, wte, wpe))
+    known = (idx >= 0) & (idx < 40)
+    want = torch.where(known[..., None], wte[idx.clamp(0, 39)].float(), 0.0) + wpe.float()
+    assert torch.equal(y, want.to(torch.bfloat16))
+    y.backward(torch.ones_like(y))
+    count = torch.bincount(idx[known], minlength=40)
+    assert torch.equal(wte.grad.float(), count[:, None].float().expand(40, 24))
+    assert torch.all(wpe.grad == 2)
+    settle("cuda")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_model_of_nan_is_reported(device):
+    """Its logits are NaN, nothing can be drawn from them (-1), and -1 is no token that could be fed back."""
+    from mini_nccl_b200.models.generation import sample_continuations
+    from mini_nccl_b200.models.gpt import GPT
+
+    torch.manual_seed(0)
+    m = GPT(96, 64, 2, 2, 64)
+    m.blocks[1].proj.bias.data[5] = math.nan
+    m = m.to(device, torch.bfloat16) if device == "cuda" else m
+    prompt = torch.arange(20, device=device)
+    tokens, logprobs = sample_continuations(m, prompt, 3, 1)
+    settle(device)
+    assert torch.all(tokens == -1) and torch.all(logprobs == -math.inf)
+    out = out_of_range(device, lambda: sample_continuations(m, prompt, 3, 5))
+    assert out is None or torch.all(out[0] == -1)
