@@ -301,12 +301,13 @@ __global__ void __launch_bounds__(kThreads) compact_plan_kernel(const int* __res
 // 16-byte chunks of the named pages, in every plane: [planes][moves][chunks].
 // Eight loads in flight per thread: 83 us for 477 MB (5.8 TB/s; four 97, two 88).
 // `tokens` (or null) gives the leading tokens of each page that hold data.
+// The kernel may start while the one that plans the copies still writes src,
+// dst, tokens and count, so those are neither const nor __restrict__: nothing
+// may read them ahead of wait_for_previous().
 constexpr int kPer = 8;
 __global__ void __launch_bounds__(256) copy_pages_kernel(uint4* __restrict__ pool, long long plane_chunks,
                                                          int page_chunks, int token_chunks, int planes, int pages,
-                                                         const int* __restrict__ src, const int* __restrict__ dst,
-                                                         const int* __restrict__ tokens, const int* __restrict__ count,
-                                                         int n_max, int* status) {
+                                                         int* src, int* dst, int* tokens, int* count, int n_max, int* status) {
   wait_for_previous();
   const int n = count ? min(*count, n_max) : n_max;
   const int runs = (page_chunks + 256 * kPer - 1) / (256 * kPer);
@@ -381,8 +382,7 @@ int copy_blocks(long long units) {
 }
 }  // namespace
 
-cudaError_t launch_copy(const Pool& p, const int* src, const int* dst, const int* tokens, const int* count, int n, int* status,
-                        cudaStream_t stream) {
+cudaError_t launch_copy(const Pool& p, int* src, int* dst, int* tokens, int* count, int n, int* status, cudaStream_t stream) {
   if (n == 0) return cudaSuccess;
   const long long runs = (p.page_chunks + 256 * kPer - 1) / (256 * kPer);
   return launch_after(copy_pages_kernel, copy_blocks(static_cast<long long>(n) * p.planes * runs), 256, 0, stream,

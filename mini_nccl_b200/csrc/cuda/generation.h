@@ -39,8 +39,7 @@ struct Append {
   int n, heads, chunks;
 };
 
-cudaError_t launch_copy(const Pool& p, const int* src, const int* dst, const int* tokens, const int* count, int n, int* status,
-                        cudaStream_t stream);
+cudaError_t launch_copy(const Pool& p, int* src, int* dst, int* tokens, int* count, int n, int* status, cudaStream_t stream);
 // scratch: 4 n + slots ints
 cudaError_t launch_fork(const Pool& p, const Table& t, const int* parents, const int* children, int n, int* scratch,
                         int* status, cudaStream_t stream);

@@ -65,3 +65,33 @@ def test_a_model_of_nan_is_reported(device):
     assert torch.all(tokens == -1) and torch.all(logprobs == -math.inf)
     out = out_of_range(device, lambda: sample_continuations(m, prompt, 3, 5))
     assert out is None or torch.all(out[0] == -1)
+
+
+# ---- pages -------------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+def test_page_plans_are_read_when_they_are_there():
+    """Calls back to back, each with other requests in the same workspace: a copy named by the last plan would show."""
+    page, S, pages = 8, 64, 600
+    kv = torch.randn(2, 2, pages, page, 2, 64).to(torch.bfloat16).cuda()
+    table, lens, refs = ints([[-1] * 5] * S, "cuda"), ints([0] * S, "cuda"), ints([0] * pages, "cuda")
+    G.reserve_pages(table, lens, refs, ints(range(S // 2), "cuda"), ints([9 + i % 20 for i in range(S // 2)], "cuda"), page)
+    gen = torch.Generator().manual_seed(0)
+    plans = []
+    for _ in range(40):
+        n = int(torch.randint(1, S // 2, (1,), generator=gen))
+        plans.append((torch.randint(0, S // 2, (n,), generator=gen).int().cuda(), (S // 2 + torch.randperm(S // 2, generator=gen)[:n]).int().cuda()))
+    parents_of, copies = [], []
+    for parents, children in plans:
+        G.fork_sequences(kv, table, lens, refs, parents, children)
+        rows = table[children.long()].long().clamp(min=0)
+        copies.append((kv[:, :, rows].clone(), lens[children.long()].clone()))
+        rows = table[parents.long()].long().clamp(min=0)
+        parents_of.append(kv[:, :, rows].clone())
+        G.free_sequences(table, lens, refs, children)
+        table, refs = G.compact_pages(kv, table, refs)
+    settle("cuda")
+    for (got, n), want in zip(copies, parents_of):
+        inside = (torch.arange(5 * page, device="cuda") < n[:, None]).view(1, 1, -1, 5, page, 1, 1)
+        assert torch.equal(torch.where(inside, got, 0), torch.where(inside, want, 0))
