@@ -307,12 +307,13 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(
   a.q = bf16(q);
   a.q_ld = q.stride(0);
   a.q_head = q.stride(1);
-  a.k = bf16(k_pages);
-  a.v = bf16(v_pages);
+  a.k = bf16(pages > 0 ? k_pages : q);  // (a map needs an address, also where nothing will be read)
+  a.v = bf16(pages > 0 ? v_pages : q);
   a.page_ld = k_pages.stride(0);
   a.token_ld = k_pages.stride(1);
   a.head_ld = k_pages.stride(2);
   a.pages = static_cast<int>(pages);
+  a.no_page = std::max(1, a.pages);  // (a map has at least one page)
   a.page_shift = __builtin_ctzll(static_cast<uint64_t>(page));
   a.prefix_pages = prefix_pages.data_ptr<int>();
   a.prefix_len = static_cast<int>(prefix_len);

@@ -94,6 +94,7 @@ struct Args {
   const __nv_bfloat16 *k, *v;
   long long page_ld, token_ld, head_ld;  // of the page pools, in elements
   int pages, page_shift;
+  int no_page;  // an index outside the pool's tensor map, where TMA reads zeros: for ids that name no page
   const int* prefix_pages;
   int prefix_len;
   const int* page_table;

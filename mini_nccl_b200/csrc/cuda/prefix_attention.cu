@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
           page = p.ids[j >> a.page_shift];
           if (page < 0 || page >= a.pages) {
             flag(a);
-            page = a.pages;  // outside the map: reads as zeros
+            page = a.no_page;
           }
         }
         if (!mbar_wait(empty0 + 8 * st, ((pos / kStages) & 1) ^ 1, a.status)) return;

@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int page = a.prefix_pages[j >> a.page_shift];
         if (page < 0 || page >= a.pages) {
           atomicCAS(a.errors, 0, kErrBadIndex);
-          page = a.pages;  // outside the map: reads as zeros
+          page = a.no_page;
         }
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)

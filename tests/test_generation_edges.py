@@ -95,3 +95,27 @@ def test_page_plans_are_read_when_they_are_there():
     for (got, n), want in zip(copies, parents_of):
         inside = (torch.arange(5 * page, device="cuda") < n[:, None]).view(1, 1, -1, 5, page, 1, 1)
         assert torch.equal(torch.where(inside, got, 0), torch.where(inside, want, 0))
+
+
+# ---- attention: memory -------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_attention_on_a_pool_without_pages(device):
+    """No page can be read, not even of the tensor that the pool is a part of."""
+    for rows in (3, 60):
+        q = torch.randn(rows, 2, 64).to(torch.bfloat16).to(device)
+        whole = torch.full((2, 6, 8, 2, 64), math.nan, dtype=torch.bfloat16, device=device)
+        for pool in (whole[:, 3:3], torch.empty(2, 0, 8, 2, 64, dtype=torch.bfloat16, device=device)):
+            table = ints([[0, -1]] * rows, device)
+
+            def call(prefix, lens):
+                return G.shared_prefix_attention(q, pool[0], pool[1], ints([0] * 17, device), prefix, table, ints(lens, device),
+                                                 return_lse=True)
+
+            o, lse = call(0, [0] * rows)
+            settle(device)
+            assert torch.all(o == 0) and torch.all(lse == -math.inf)
+            for prefix, lens in ((130, [0] * rows), (0, [1] * rows), (130, [5] * rows)):
+                out = out_of_range(device, lambda: call(prefix, lens))
+                assert out is None or torch.all(out[0] == 0), "the keys that are not there read as zeros"
