@@ -181,7 +181,8 @@ __global__ void __launch_bounds__(kThreads) fork_plan_kernel(Table t, const int*
   }
 }
 
-// reserve: slot i grows by counts[i] tokens; new pages fill its row.
+// reserve: slot i grows by counts[i] tokens; new pages fill its row.  (A row may hold more tokens than an int32 length
+// can say: a sequence ends at 2^31 - 1.)
 __global__ void __launch_bounds__(kThreads) reserve_kernel(Table t, const int* __restrict__ slot_of,
                                                            const int* __restrict__ counts, int n, int* owner, int* ids,
                                                            int most, int* rank_of, int* status) {
@@ -197,7 +198,7 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(Table t, const int* _
       bool ok = s >= 0 && s < t.slots && owner[s] == i && more >= 0;
       if (ok) {
         const long long len = t.lens[s], to = len + more;
-        ok = len >= 0 && to <= t.columns * static_cast<long long>(t.page_size);
+        ok = len >= 0 && to <= min(t.columns * static_cast<long long>(t.page_size), 0x7fffffffll);
         if (ok) need = static_cast<int>((to + t.page_size - 1) / t.page_size - (len + t.page_size - 1) / t.page_size);
       }
       if (!ok) {
@@ -213,8 +214,9 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(Table t, const int* _
   const int have = find_free(t.refs, t.pages, min(base, most), ids, sh, first_refs);
   for (int i = threadIdx.x; i < n; i += kThreads) {
     if (rank_of[i] < 0) continue;
-    const int s = slot_of[i], len = t.lens[s];
-    const int c0 = (len + t.page_size - 1) / t.page_size, c1 = (len + counts[i] + t.page_size - 1) / t.page_size;
+    const int s = slot_of[i];
+    const long long len = t.lens[s], to = len + counts[i];
+    const int c0 = static_cast<int>((len + t.page_size - 1) / t.page_size), c1 = static_cast<int>((to + t.page_size - 1) / t.page_size);
     if (c1 > c0 && rank_of[i] + (c1 - c0) > have) {
       flag(status, kErrNoPages);
       continue;
@@ -224,7 +226,7 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(Table t, const int* _
       t.table[s * t.ld + c] = page;
       t.refs[page] = 1;
     }
-    t.lens[s] = len + counts[i];
+    t.lens[s] = static_cast<int>(to);
   }
 }
 

@@ -396,7 +396,7 @@ def reserve_pages(
     ss, ns = _ids((slots, "slots"), (counts, "counts"))
     S, W = page_table.shape
     for i, (s, n) in enumerate(zip(ss, ns)):
-        if not (0 <= s < S and n >= 0 and ss.index(s) == i and int(lens[s]) + n <= W * page_size):
+        if not (0 <= s < S and n >= 0 and ss.index(s) == i and int(lens[s]) + n <= min(W * page_size, 2 ** 31 - 1)):
             raise RuntimeError(f"reserve {i}: {n} tokens for sequence {s}")
     free = _free_ids(refs)
     for s, n in zip(ss, ns):

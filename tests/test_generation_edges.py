@@ -119,3 +119,20 @@ def test_attention_on_a_pool_without_pages(device):
             for prefix, lens in ((130, [0] * rows), (0, [1] * rows), (130, [5] * rows)):
                 out = out_of_range(device, lambda: call(prefix, lens))
                 assert out is None or torch.all(out[0] == 0), "the keys that are not there read as zeros"
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_reserve_past_the_range_of_lengths(device):
+    """A row whose pages hold more than 2^31 tokens: lengths are int32, so it ends before."""
+    page, columns, last = 1 << 20, 2100, (1 << 31) - 1
+    table, lens, refs = ints([[-1] * columns], device), ints([last - 50], device), ints([0] * 4, device)
+    before = table.clone()
+    out_of_range(device, lambda: G.reserve_pages(table, lens, refs, ints([0], device), ints([60], device), page), match=".")
+    assert torch.equal(table, before) and lens.tolist() == [last - 50] and refs.tolist() == [0] * 4
+    G.reserve_pages(table, lens, refs, ints([0], device), ints([50], device), page)  # up to the last length
+    settle(device)
+    assert lens.tolist() == [last] and torch.equal(table, before)
+    lens.fill_(last - page - 7)
+    G.reserve_pages(table, lens, refs, ints([0], device), ints([page], device), page)
+    settle(device)
+    assert lens.tolist() == [last - 7] and table[0, 2047].item() == 0 and int(refs.sum()) == 1
