@@ -187,6 +187,12 @@ struct Team {
     asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(to), "l"(v), "r"(to_bar)
                  : "memory");
   }
+  // Until every block's values are there.  Not given up because another wait of the device has run out: the blocks of a
+  // cluster have to agree on every value, or one would end while another still reads its memory.
+  MNB_DEVICE void receive(uint32_t bar) {
+    if (!mbar_wait(bar, (exchanges >> 1) & 1, nullptr)) atomicCAS(status, 0, kErrPipelineTimeout);
+    ++exchanges;
+  }
   template <typename V, typename F>
   MNB_DEVICE V join(V v, V* red, F f) {
     v = block_reduce(v, red, f);
@@ -195,8 +201,7 @@ struct Team {
     const uint32_t bar = smem_u32(sh.joined + turn);
     if (threadIdx.x == 0) mbar_arrive_expect_tx(bar, 8 * size);
     if (threadIdx.x < size) send(&sh.from[turn][rank], bits(v), bar, threadIdx.x);
-    mbar_wait(bar, (exchanges >> 1) & 1, status);
-    ++exchanges;
+    receive(bar);
     V s, x;
     of_bits(*const_cast<volatile uint64_t*>(&sh.from[turn][0]), s);
     for (int q = 1; q < size; ++q) {
@@ -229,8 +234,7 @@ struct Team {
       send(&sh.from[turn][rank], best, bar, threadIdx.x);
       send(&sh.from_too[turn][rank], bits(*z), bar, threadIdx.x);
     }
-    mbar_wait(bar, (exchanges >> 1) & 1, status);
-    ++exchanges;
+    receive(bar);
     *z = 0.f;
     for (int q = 0; q < size; ++q) {
       best = ::max(best, *const_cast<volatile uint64_t*>(&sh.from[turn][q]));
@@ -612,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   }
 
   float mine = -INFINITY;
-  for (int c = tid, j = 0; c < row.count; ++j) {  // a chunk holds four of a thread's pieces
+  for (int c = tid, j = 0; c < row.count; ++j) {  // a chunk holds two of a thread's pieces
     if (Staged && !mbar_wait(smem_u32(sh.arrived + j), 0, a.status)) break;
 #pragma unroll
     for (int e = 0; e < kChunk / kThreads; ++e, c += kThreads)
@@ -648,10 +652,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     const uint64_t chosen = team.max_and_sum(best.pair(), &z);
     total += z;
     if (tid == 0 && team.rank == 0) {
-      const int i = index_of(chosen);
+      const int i = chosen ? index_of(chosen) : -1;  // (nothing: the row did not arrive in time, which is in the status word)
       a.token[r] = i;
       if (a.logprob) {
-        const float v = row.one(i);
+        const float v = i >= 0 ? row.one(i) : -INFINITY;
         a.logprob[r] = (v == mx ? 0.f : __fdiv_rn(v - mx, t)) - logf(total);
       }
     }
