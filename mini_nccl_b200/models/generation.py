@@ -29,17 +29,31 @@ def _add_linear(x: torch.Tensor, layer: torch.nn.Linear, resid: torch.Tensor) ->
     return resid + F.linear(x, layer.weight, layer.bias)
 
 
+def _plain_blocks(model: GPT) -> list[Block]:
+    """The model's blocks, which are run layer by layer here; a wrapped or changed one would not be what the model runs."""
+    blocks = list(getattr(model, "blocks", ()))
+    for b in blocks:
+        if getattr(type(b), "forward", None) is not Block.forward or getattr(type(b), "_forward_cuda", None) is not Block._forward_cuda:
+            raise ValueError(f"generation with a cache runs the layers of GPT's own Block, not of {type(b).__name__} "
+                             "(of a sharded model, load the full weights into a plain GPT)")
+    if not blocks:
+        raise ValueError(f"a GPT with blocks, not {type(model).__name__}")
+    return blocks
+
+
 class BranchedGeneration:
     """The state of up to ``max_branches`` continuations of one prompt, which grow in step.
 
     ``logits`` holds the scores of the next token, one row for each of
     ``branches``; at first there is one branch, which holds nothing yet.
+    The model is a plain :class:`GPT`: one whose blocks are wrapped (sharded
+    by ``FullyShardedDataParallel``) is refused with ``ValueError``.
     """
 
     @torch.no_grad()
     def __init__(self, model: GPT, prompt: torch.Tensor, *, max_branches: int, max_new_tokens: int, page_size: int = 16) -> None:
         prompt = prompt.reshape(-1)
-        P, blocks = prompt.numel(), [b for b in model.blocks if isinstance(b, Block)]
+        P, self._blocks = prompt.numel(), _plain_blocks(model)
         if P < 1 or max_branches < 1 or max_new_tokens < 1:
             raise ValueError("a prompt of at least one token, one branch and one new token")
         if P + max_new_tokens > model.block_size:
@@ -57,7 +71,7 @@ class BranchedGeneration:
         self.cache.extend([0], [P])
         places = torch.arange(P, dtype=torch.int32, device=w.device)
         x = _embed(model, prompt[None], 0)
-        for layer, block in enumerate(blocks):
+        for layer, block in enumerate(self._blocks):
             h = F.layer_norm(x, block.ln1.weight, block.ln1.bias, block.ln1.eps)
             qkv = F.linear(h, block.qkv.weight, block.qkv.bias)
             _, k, v = qkv[0].view(P, 3, self.heads, self.head_dim).unbind(1)
@@ -99,7 +113,7 @@ class BranchedGeneration:
         prefix = c.page_table[0, : -(-P // c.page_size)]
         x = _embed(self.model, tokens[:, None], P + self.length)[:, 0]
         self.length += 1
-        for layer, block in enumerate(self.model.blocks):
+        for layer, block in enumerate(self._blocks):
             h = F.layer_norm(x, block.ln1.weight, block.ln1.bias, block.ln1.eps)
             q, k, v = F.linear(h, block.qkv.weight, block.qkv.bias).view(n, 3, self.heads, self.head_dim).unbind(1)
             c.append(layer, k, v, place, ids)

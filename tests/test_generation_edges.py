@@ -136,3 +136,64 @@ def test_reserve_past_the_range_of_lengths(device):
     G.reserve_pages(table, lens, refs, ints([0], device), ints([page], device), page)
     settle(device)
     assert lens.tolist() == [last - 7] and table[0, 2047].item() == 0 and int(refs.sum()) == 1
+
+
+# ---- models ------------------------------------------------------------------------------
+
+
+def _sharded_gpt_is_refused(pg):
+    from mini_nccl_b200.fsdp import FullyShardedDataParallel
+    from mini_nccl_b200.models.generation import BranchedGeneration, sample_continuations
+    from mini_nccl_b200.models.gpt import GPT, Block
+
+    torch.manual_seed(0)
+    model, prompt = GPT(96, 64, 2, 2, 64), torch.arange(20)
+    with torch.no_grad():
+        want = model(prompt[None])[0][:, -1]
+    plain = GPT(96, 64, 2, 2, 64)
+    fsdp = FullyShardedDataParallel(model, pg, unit_cls=Block)
+    for m in (model, fsdp):
+        with pytest.raises(ValueError, match="Block|blocks"):
+            sample_continuations(m, prompt, 2, 1)
+        with pytest.raises(ValueError, match="Block|blocks"):
+            BranchedGeneration(m, prompt, max_branches=1, max_new_tokens=3)
+    plain.load_state_dict(fsdp.full_state_dict(), strict=False)
+    assert torch.allclose(BranchedGeneration(plain, prompt, max_branches=1, max_new_tokens=3).logits, want, atol=1e-4)
+
+
+@pytest.mark.parametrize("ranks", [1, 2])
+def test_generation_refuses_a_sharded_model(ranks):
+    from mini_nccl_b200.launcher import run
+
+    run(_sharded_gpt_is_refused, ranks)
+
+
+def test_generation_refuses_blocks_that_do_something_else():
+    from mini_nccl_b200.models.generation import BranchedGeneration
+    from mini_nccl_b200.models.gpt import GPT, Block
+
+    class Scaled(Block):
+        def forward(self, x):
+            return super().forward(x) * 0.5
+
+    class Named(Block):
+        pass
+
+    class Around(torch.nn.Module):
+        def __init__(self, block):
+            super().__init__()
+            self.block = block
+
+        def forward(self, x):
+            return self.block(x)
+
+    for change, ok in ((lambda b: Scaled(64, 2), False), (Around, False), (lambda b: Named(64, 2), True), (lambda b: b, True)):
+        m = GPT(96, 64, 2, 2, 64)
+        m.blocks[1] = change(m.blocks[1])
+        call = lambda: BranchedGeneration(m, torch.arange(9), max_branches=1, max_new_tokens=3)  # noqa: E731
+        if not ok:
+            with pytest.raises(ValueError, match="Block"):
+                call()
+            continue
+        with torch.no_grad():
+            assert torch.allclose(call().logits, m(torch.arange(9)[None])[0][:, -1], atol=1e-4)
