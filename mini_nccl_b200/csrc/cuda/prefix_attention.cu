@@ -528,7 +528,8 @@ int plan(Args& a, int head_dim) {
   a.prefix_splits = a.own_splits = 0;
   a.quad = false;
   const long long rows = static_cast<long long>(a.n) * a.group;
-  a.tensor_cores = a.prefix_len > 0 && head_dim != 32 && rows > kTensorCoreRows && a.scale_log2 >= 0.f;
+  // (that kernel masks scores before they are scaled, and -inf times a scale of 0 or below is not -inf)
+  a.tensor_cores = a.prefix_len > 0 && head_dim != 32 && rows > kTensorCoreRows && a.scale_log2 > 0.f;
   a.tile_rows = 16 * row_warps(static_cast<int>(a.tensor_cores || a.prefix_len == 0 ? static_cast<long long>(a.max_q) * a.group : rows));
   if (a.prefix_len > 0) {
     if (a.tensor_cores) {

@@ -197,3 +197,19 @@ def test_generation_refuses_blocks_that_do_something_else():
             continue
         with torch.no_grad():
             assert torch.allclose(call().logits, m(torch.arange(9)[None])[0][:, -1], atol=1e-4)
+
+
+# ---- attention: values -------------------------------------------------------------------
+
+
+# few and many rows of a kv head, prefixes that end inside a tile and behind one
+ROWS = [([60, 3, 0], [1, 1, 1], 1, 129), ([40] * 50, [1] * 50, 1, 129), ([70, 90], [60, 90], 2, 333), ([5] * 70, [1] * 70, 4, 256)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("lens,new,group,prefix", ROWS)
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+def test_attention_scale_of_zero_and_below(device, dim, lens, new, group, prefix, scale):
+    p = Problem(lens, new, kv_heads=2, group=group, dim=dim, page=16, prefix=prefix, device=device)
+    p.check(*p.run(scale=scale), scale=scale)
