@@ -13,9 +13,12 @@
 //     tiles s, s + 2, ...; they are joined through shared memory at the end.
 // Per 128-key tile and stream:  S = Q K^T (TMEM) -> softmax: thread = row, no
 // exchange between threads; P (bf16) goes over S in TMEM -> O += P V with P as
-// the TMEM operand.  The running maximum only moves when a row's scores pass
-// it by 2^8, so O is rarely rescaled (exact either way: the final division
-// uses the same maximum); sums are fp32.
+// the TMEM operand.  The base that scores are taken relative to is a running
+// maximum that only moves when a row's scores pass it by 2^8, so O is rarely
+// rescaled (exact either way: the final division uses the same base); it is
+// held in fp32, because a rounded one lies up to a 2^-8th of itself above the
+// scores, which for large ones is more than any weight survives.  Sums are
+// fp32.
 //
 // Measured: 16 sequences of 4 grouped heads (64 rows) over 65,537 keys of 8 kv
 // heads, 268 MB: 48 us, 5.6 TB/s, bound by the bytes.  2388 rows of 32 heads
@@ -56,8 +59,8 @@ struct Smem {
   static constexpr uint32_t q_off = 0, kv_off = 2 * q_tile;
   static constexpr uint32_t bar_off = kv_off + stages * kv_tile;
   static constexpr int n_bars = 2 * stages + 9;
-  static constexpr uint32_t max_off = bar_off + n_bars * 8 + 16;  // row maxima: [stream][half][row], bf16
-  static constexpr uint32_t total = max_off + 4 * kTile * 2 + 1024;
+  static constexpr uint32_t max_off = bar_off + n_bars * 8 + 16;  // row maxima so far: [stream][row], as order_of()
+  static constexpr uint32_t total = max_off + 2 * kTile * 4 + 1024;
   static_assert(total <= 227 * 1024, "a block's shared memory");
 };
 
@@ -97,6 +100,12 @@ MNB_DEVICE bool elected() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
   return one != 0;
 }
+// Whole numbers in the floats' order (and back): what atomicMax on shared memory takes.
+MNB_DEVICE int order_of(float x) {
+  const int i = __float_as_int(x);
+  return i ^ ((i >> 31) & 0x7fffffff);
+}
+MNB_DEVICE float of_order(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
 MNB_DEVICE void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kSoftmax) : "memory"); }
 MNB_DEVICE void stream_sync(int s) { asm volatile("bar.sync %0, %1;" ::"r"(2 + s), "n"(kSoftmax / 2) : "memory"); }
 
@@ -160,6 +169,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&map_k);
     tma_prefetch_desc(&map_v);
   }
+  if (threadIdx.x < 2 * kTile) reinterpret_cast<int*>(sm + S::max_off)[threadIdx.x] = order_of(-INFINITY);
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
@@ -325,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_arrive(q_full);
     }
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-    __nv_bfloat16* seen = reinterpret_cast<__nv_bfloat16*>(sm + S::max_off) + s * 2 * kTile + r;
+    volatile int* seen = reinterpret_cast<int*>(sm + S::max_off) + s * kTile + r;
     const uint32_t t_s = tmem + s * kTile + lanes, t_o = tmem + 2 * kTile + s * D + lanes;
     const int steps = shared ? n_tiles : (n_tiles - s + 1) / 2;
     const bool padding = (shared ? s * kTile : 0) + quad * 32 >= n_rows;  // a warp without rows leaves P as it is
@@ -356,15 +366,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (i + 3 < 64) mx2 = max3f(mx2, v[i + 2], v[i + 3]);
       }
       mx = fmaxf(mx, mx2);
-      // The halves' maxima meet, rounded up to bf16: any base that both use will do.  Past this barrier both halves'
-      // scores are in registers, so P may go over them.  (Each step's places are free again: its S was issued after both
-      // halves of the last step had read theirs and written P.)
-      const __nv_bfloat16 up = __float2bfloat16_ru(mx * a.scale_log2);
-      seen[half * kTile] = up;
+      // The halves' maxima meet in the row's maximum so far.  Past this barrier both halves' scores are in registers, so
+      // P may go over them.  (Neither half is ahead: S of a step was issued after both halves of the last one had read
+      // their maximum and written P.)
+      atomicMax(const_cast<int*>(seen), order_of(mx * a.scale_log2));
       tc_fence_before();
       stream_sync(s);
       tc_fence_after();
-      mx = fmaxf(bf16_to_f32(up), bf16_to_f32(seen[(half ^ 1) * kTile]));
+      mx = of_order(*seen);
       const bool grows = mx > m + kRescale || m == -INFINITY;
       if (__any_sync(0xffffffffu, grows)) {
         const float to = grows ? mx : m;
@@ -385,7 +394,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         l *= alpha;
         m = to;
       }
-      const float2 scale2 = splat2(a.scale_log2), base2 = splat2(m == -INFINITY ? 0.f : -m);
+      float2 scale2 = splat2(a.scale_log2);
+      const float2 base2 = splat2(m == -INFINITY ? 0.f : -m);
+      if (__any_sync(0xffffffffu, fabsf(m) >= 16777216.f)) {
+        // Here rounding a scaled score moves it by whole units, and by more than a float's range later: round the scores as
+        // their maximum was.
+#pragma unroll
+        for (int i = 0; i < 64; ++i) v[i] *= a.scale_log2;
+        scale2 = splat2(1.f);
+      }
       float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {

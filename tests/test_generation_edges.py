@@ -213,3 +213,33 @@ ROWS = [([60, 3, 0], [1, 1, 1], 1, 129), ([40] * 50, [1] * 50, 1, 129), ([70, 90
 def test_attention_scale_of_zero_and_below(device, dim, lens, new, group, prefix, scale):
     p = Problem(lens, new, kv_heads=2, group=group, dim=dim, page=16, prefix=prefix, device=device)
     p.check(*p.run(scale=scale), scale=scale)
+
+
+def aligned_problem(device, dim, size, rows, prefix, group=1, lens=None, new=None):
+    """Every query and key lies along one direction, so scores are products of two bf16 numbers: +-`size` and near it."""
+    lens = [3] * rows if lens is None else lens
+    p = Problem(lens, [1] * len(lens) if new is None else new, kv_heads=1, group=group, dim=dim, page=16, prefix=prefix, device=device)
+    p.q = torch.zeros_like(p.q)
+    p.q[..., 0] = 128.0
+    keys = p.pool[0]
+    g = torch.Generator().manual_seed(1)
+    along = (size / 128 + torch.randn(keys.shape[:3], generator=g).mul_(abs(size) * 2.0 ** -15)).to(torch.bfloat16)
+    keys[:] = 0
+    keys[..., 0] = along.to(device)
+    p.head[0].zero_()
+    ids = torch.tensor(p.prefix_pages)
+    p.head[0][..., 0] = along[ids].reshape(-1, 1)[:prefix].double()
+    for own, row, m in zip(p.own, p.rows, lens):
+        own[0].zero_()
+        own[0][..., 0] = along[torch.tensor(row[: -(-m // 16)], dtype=torch.long)].reshape(-1, 1)[:m].double()
+    return p
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("size", [1.2e4, -1.2e4, 2.9e4, 1.5e5, -3e6, 2e9, 1e12, -1e15, 1e30])
+@pytest.mark.parametrize("rows,prefix", [(2, 300), (40, 300), (40, 500), (200, 2100)])
+def test_attention_scores_far_from_zero(device, dim, size, rows, prefix):
+    # log2 units: size / ln 2.  Beyond 2^14 a step of bf16 is 128 and more, beyond 2^31 one of fp32 is
+    p = aligned_problem(device, dim, size, rows, prefix)
+    p.check(*p.run(scale=1.0), scale=1.0)
