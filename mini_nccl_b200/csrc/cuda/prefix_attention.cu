@@ -425,12 +425,12 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args 
 #pragma unroll
     for (int i = 0; i < kPer; ++i) o[i] = so[0][lane * kPer + i] + so[1][lane * kPer + i] + so[2][lane * kPer + i] + so[3][lane * kPer + i];
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;  // a row without keys is zero
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // a row without keys is zero; one with a score of NaN stays NaN
   __nv_bfloat16* out = a.o + row * D + lane * kPer;
   if constexpr (kPer == 1) *out = f32_to_bf16(o[0] * inv);
 #pragma unroll
   for (int i = 0; i + 1 < kPer; i += 2) *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2(o[i] * inv, o[i + 1] * inv);
-  if (a.lse && lane == 0) a.lse[row] = l > 0.f ? kLn2 * (m + log2f(l)) : -INFINITY;
+  if (a.lse && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : kLn2 * (m + log2f(l));
 }
 
 int row_warps(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }

@@ -100,7 +100,13 @@ MNB_DEVICE bool elected() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
   return one != 0;
 }
-// Whole numbers in the floats' order (and back): what atomicMax on shared memory takes.
+// The largest of three, or NaN where one is.
+MNB_DEVICE float max3_or_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Whole numbers in the floats' order (and back): what atomicMax on shared memory takes.  NaN (as the maximum gives it) comes last.
 MNB_DEVICE int order_of(float x) {
   const int i = __float_as_int(x);
   return i ^ ((i >> 31) & 0x7fffffff);
@@ -362,10 +368,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       float mx = v[0], mx2 = v[1];
 #pragma unroll
       for (int i = 2; i < 64; i += 4) {
-        mx = max3f(mx, v[i], v[i + 1]);
-        if (i + 3 < 64) mx2 = max3f(mx2, v[i + 2], v[i + 3]);
+        mx = max3_or_nan(mx, v[i], v[i + 1]);
+        if (i + 3 < 64) mx2 = max3_or_nan(mx2, v[i + 2], v[i + 3]);
       }
-      mx = fmaxf(mx, mx2);
+      mx = max3_or_nan(mx, mx2, mx2);  // (a score of NaN makes the row NaN, by its base)
       // The halves' maxima meet in the row's maximum so far.  Past this barrier both halves' scores are in registers, so
       // P may go over them.  (Neither half is ahead: S of a step was issued after both halves of the last one had read
       // their maximum and written P.)
@@ -374,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       stream_sync(s);
       tc_fence_after();
       mx = of_order(*seen);
-      const bool grows = mx > m + kRescale || m == -INFINITY;
+      const bool grows = !(mx <= m + kRescale) || m == -INFINITY;
       if (__any_sync(0xffffffffu, grows)) {
         const float to = grows ? mx : m;
         const float alpha = ex2_approx(m - (to == -INFINITY ? 0.f : to));
@@ -480,9 +486,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float2 ml = a.part_ml[p * rows + x.at];
           l = fmaf(ex2_approx(ml.x - base), ml.y, l);
         }
-        x.inv = l > 0.f ? 1.f / l : 0.f;
+        x.inv = l == 0.f ? 0.f : 1.f / l;  // (NaN stays NaN)
         x.mine *= f * x.inv, x.met *= f * x.inv;
-        if (a.lse) a.lse[x.at] = l > 0.f ? kLn2 * (x.top + log2f(l)) : -INFINITY;
+        if (a.lse) a.lse[x.at] = l == 0.f ? -INFINITY : kLn2 * (x.top + log2f(l));
       } else {
         a.part_ml[split * rows + x.at] = make_float2(x.top, l);
       }
@@ -521,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 0; e < kBatch; ++e) {
           const float g = top[e] == -INFINITY ? 0.f : ex2_approx(top[e] - x[e].top) * x[e].inv;
 #pragma unroll
-          for (int d = 0; d < kPer; ++d) o[e].v[d] += g > 0.f ? y[e].v[d] * g : 0.f;  // (nothing was written without keys)
+          for (int d = 0; d < kPer; ++d) o[e].v[d] += g == 0.f ? 0.f : y[e].v[d] * g;  // (nothing was written without keys)
         }
       }
 #pragma unroll

@@ -243,3 +243,35 @@ def test_attention_scores_far_from_zero(device, dim, size, rows, prefix):
     # log2 units: size / ln 2.  Beyond 2^14 a step of bf16 is 128 and more, beyond 2^31 one of fp32 is
     p = aligned_problem(device, dim, size, rows, prefix)
     p.check(*p.run(scale=1.0), scale=1.0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("rows,prefix", [(3, 140), (3, 0), (50, 140), (50, 0), (50, 1300), (300, 700)])
+def test_attention_shows_nan_in_queries_and_visible_keys(device, dim, rows, prefix):
+    def fresh():
+        return Problem([4] * rows, [1] * rows, kv_heads=2, group=1, dim=dim, page=16, prefix=prefix, device=device)
+
+    p = fresh()
+    p.q[1, 1] = math.nan
+    o, lse = (t.cpu() for t in p.run())
+    assert torch.all(o[1, 1].isnan()) and lse[1, 1].isnan(), "a query of NaN"
+    p.q[1, 1] = 0
+    rest, rest_lse = (t.cpu() for t in p.run())
+    others = torch.ones(rows, 2, dtype=torch.bool)
+    others[1, 1] = False
+    assert torch.equal(o[others], rest[others]) and torch.equal(lse[others], rest_lse[others])
+    # one key of the prefix: every row of its head sees it, wherever it lies in its tile
+    for at in range(0, min(prefix, 140), 1 if rows == 50 and dim == 64 else 23):
+        p = fresh()
+        p.pool[0, p.prefix_pages[at // 16], at % 16, 1, 3] = math.nan
+        o, lse = p.run()
+        assert torch.all(o[:, 1].isnan()) and torch.all(lse[:, 1].isnan()), at
+        assert not o[:, 0].isnan().any() and not lse[:, 0].isnan().any()
+    # one key of a sequence's own
+    p = fresh()
+    p.pool[0, p.rows[2][0], 3, 0, 0] = math.nan
+    o, lse = p.run()
+    hit = torch.zeros(rows, 2, dtype=torch.bool)
+    hit[2, 0] = True
+    assert torch.equal(o.isnan().all(-1).cpu(), hit) and torch.equal(lse.isnan().cpu(), hit)
