@@ -125,6 +125,42 @@ MNB_DEVICE Piece piece_of(const Args& a, const int* seq_lens, const int* q_offse
   return p;
 }
 
+// The outputs of a warp's 16 rows from row0 on once more, key by key: keys first to first + width - 1 of every `step`.  A
+// product over a tile gives a hidden key weight 0, and 0 times a value that is no number is NaN; here each row takes
+// only what it sees.  `m0` and `m1` are the maxima of this lane's rows (lane / 4, and 8 more); the rows are those of
+// `rows` in shared memory, `pitch` apart, or without it their places among the partial results.
+template <int D>
+__device__ __noinline__ void rows_key_by_key(const Args& a, Piece p, int head, int row0, int first, int width, int step, float m0,
+                                             float m1, float* rows, int pitch) {
+  constexpr int kPer = D / 32;
+  const int lane = threadIdx.x % 32;
+  __syncwarp();
+  for (int x = 0; x < 16; ++x) {
+    const int r = row0 + x;
+    if (r >= p.n_rows) break;
+    const float m = __shfl_sync(0xffffffffu, x < 8 ? m0 : m1, x % 8 * 4), base = m == -INFINITY ? 0.f : m;
+    const int j = p.r0 + r, token = j / a.group, limit = min(p.k1, p.limit0 + token), in_group = j - token * a.group;
+    const __nv_bfloat16* q = a.q + (p.n0 + token) * a.q_ld + (head * a.group + in_group) * a.q_head + lane * kPer;
+    float o[kPer] = {};
+    for (int t0 = p.k0 + first; t0 < limit; t0 += step)
+      for (int key = t0; key < min(t0 + width, limit); ++key) {
+        const int page = p.ids[key >> a.page_shift];
+        if (page < 0 || page >= a.pages) continue;  // reads as zeros
+        const long long at = page * a.page_ld + (key & ((1 << a.page_shift) - 1)) * a.token_ld + head * a.head_ld + lane * kPer;
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) s = fmaf(bf16_to_f32(q[i]), bf16_to_f32(a.k[at + i]), s);
+        const float w = ex2_approx(warp_sum(s) * a.scale_log2 - base);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) o[i] = fmaf(w, bf16_to_f32(a.v[at + i]), o[i]);
+      }
+    const long long out = (static_cast<long long>(p.slot) * a.n + p.n0 + token) * a.heads + head * a.group + in_group;
+    float* to = rows ? rows + r * pitch : a.part_o + out * D;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) to[lane * kPer + i] = o[i];
+  }
+}
+
 // WR: warps that take rows of their own (16 each); the 4 / WR groups of warps split the keys of a stage.
 //
 // Measured: 192 sequences of 1 to 401 tokens, 16 heads of 128, one row each (314 MB): 72 us, 4.4 TB/s; all of them 384
@@ -138,7 +174,10 @@ MNB_DEVICE Piece piece_of(const Args& a, const int* seq_lens, const int* q_offse
 // without a join: what a piece costs beside its keys is spent once for four heads, which decides where many sequences
 // are short (2048 sequences of 4 tokens, 16 heads, behind a prefix of 64: the
 // call 261 us without, 86 with).
-template <int D, int WR, bool Quad>
+//
+// Chunk: sequences may have several new tokens, and rows not see all the keys of their piece.  (Its own kernel because the
+// registers for rows_key_by_key cost single tokens 1 %.)
+template <int D, int WR, bool Quad, bool Chunk>
 __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
     pieces_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, int items, int join_rows, int known) {
@@ -338,6 +377,18 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
       l_r[e] += __shfl_xor_sync(0xffffffffu, l_r[e], 1);
       l_r[e] += __shfl_xor_sync(0xffffffffu, l_r[e], 2);
     }
+    // Whether some row does not see all the keys here, and the warp's outputs hold something that is no number.
+    bool again = false;
+    if (Chunk && p.limit0 + p.r0 / a.group < p.k1 && !idle) {
+      float zero = 0.f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (e == 1 && !lower) break;
+#pragma unroll
+        for (int d = 0; d < D / 8; ++d) zero = fmaf(acc[d][2 * e], 0.f, fmaf(acc[d][2 * e + 1], 0.f, zero));
+      }
+      again = __any_sync(0xffffffffu, zero != 0.f);
+    }
     if constexpr (WK > 1) {
       // the key groups of a row join through shared memory
       float* so = reinterpret_cast<float*>(sm + R::bytes);                     // [WK][join_rows][kPitch]
@@ -351,6 +402,7 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
         for (int d = 0; d < D / 8; ++d)
           *reinterpret_cast<float2*>(so + (wk * join_rows + r) * kPitch + d * 8 + 2 * tg) = make_float2(acc[d][2 * e], acc[d][2 * e + 1]);
       }
+      if (again) rows_key_by_key<D>(a, p, head, wr * 16, wk * KW, KW, kStep, m_r[0], m_r[1], so + wk * join_rows * kPitch, kPitch);
       workers_sync();
       for (int x = threadIdx.x; x < p.n_rows * (D / 4); x += kWorkers) {
         const int r = x / (D / 4), c = x % (D / 4) * 4;
@@ -384,6 +436,7 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
           *reinterpret_cast<float2*>(a.part_o + out * D + d * 8 + 2 * tg) = make_float2(acc[d][2 * e], acc[d][2 * e + 1]);
         if (tg == 0) a.part_ml[out] = make_float2(m_r[e], l_r[e]);
       }
+      if (again) rows_key_by_key<D>(a, p, head, wr * 16, 0, kStep, kStep, m_r[0], m_r[1], nullptr, 0);
     }
   }
 }
@@ -465,7 +518,7 @@ static bool pool_map(CUtensorMap* map, const __nv_bfloat16* base, const Args& a,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D, int WR, bool Quad>
+template <int D, int WR, bool Quad, bool Chunk>
 static cudaError_t launch_pieces(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
   const int rows_most = std::max(a.tensor_cores ? 0 : a.n * a.group, a.own_splits > 0 ? a.max_q * a.group : 0);
   const int join_rows = WR == 4 || Quad ? 0 : std::min(16 * WR, rows_most);
@@ -474,10 +527,20 @@ static cudaError_t launch_pieces(const Args& a, const CUtensorMap& mk, const CUt
   const int items = (a.tensor_cores ? 0 : a.row_tiles * a.kv_heads * a.prefix_splits) +
                     a.batch * a.own_tiles * a.own_splits * (Quad ? ceil_div(a.kv_heads, 4) : a.kv_heads);
   static SharedMemory allowed;
-  if (const cudaError_t e = allowed.at_least(reinterpret_cast<const void*>(pieces_kernel<D, WR, Quad>), bytes); e != cudaSuccess) return e;
+  if (const cudaError_t e = allowed.at_least(reinterpret_cast<const void*>(pieces_kernel<D, WR, Quad, Chunk>), bytes); e != cudaSuccess) return e;
   const int per_sm = std::max(1, std::min(WR == 4 ? 2 : 3, 227 * 1024 / (bytes + 1024 + 64)));
-  pieces_kernel<D, WR, Quad><<<std::min(items, 148 * per_sm), kThreads, bytes, stream>>>(a, mk, mv, items, join_rows, known);
+  pieces_kernel<D, WR, Quad, Chunk><<<std::min(items, 148 * per_sm), kThreads, bytes, stream>>>(a, mk, mv, items, join_rows, known);
   return cudaGetLastError();
+}
+
+template <int D, bool Chunk>
+static cudaError_t launch_pieces_of(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
+  if (a.quad) return launch_pieces<D, 1, true, Chunk>(a, mk, mv, stream);
+  switch (a.tile_rows) {
+    case 16: return launch_pieces<D, 1, false, Chunk>(a, mk, mv, stream);
+    case 32: return launch_pieces<D, 2, false, Chunk>(a, mk, mv, stream);
+    default: return launch_pieces<D, 4, false, Chunk>(a, mk, mv, stream);
+  }
 }
 
 template <int D>
@@ -486,12 +549,9 @@ static cudaError_t launch_for(const Args& a, cudaStream_t stream) {
   CUtensorMap mk, mv;
   const bool by_warps = a.own_splits > 0 || (a.prefix_splits > 0 && !a.tensor_cores);
   if (by_warps) {
-    const int w = a.tile_rows / 16, tokens = a.quad ? 16 : kKeys;
+    const int tokens = a.quad ? 16 : kKeys;
     if (!pool_map(&mk, a.k, a, D, tokens) || !pool_map(&mv, a.v, a, D, tokens)) return cudaErrorInvalidValue;
-    e = a.quad ? launch_pieces<D, 1, true>(a, mk, mv, stream)
-        : w == 1 ? launch_pieces<D, 1, false>(a, mk, mv, stream)
-        : w == 2 ? launch_pieces<D, 2, false>(a, mk, mv, stream)
-                 : launch_pieces<D, 4, false>(a, mk, mv, stream);
+    e = a.max_q > 1 ? launch_pieces_of<D, true>(a, mk, mv, stream) : launch_pieces_of<D, false>(a, mk, mv, stream);
     if (e != cudaSuccess) return e;
   }
   if (a.tensor_cores && a.prefix_splits > 0) {

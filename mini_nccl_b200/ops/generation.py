@@ -148,7 +148,11 @@ def shared_prefix_attention(
         s.masked_fill_((torch.arange(k.shape[1]) >= seen[:, None])[:, None, None], -math.inf)
         m = torch.logsumexp(s, -1, keepdim=True)
         p = torch.exp(s - torch.where(m == -math.inf, 0.0, m))
-        o[offsets[b]: offsets[b + 1]] = torch.einsum("nhgk,hkd->nhgd", p, v).reshape(n, H, D).to(q.dtype)
+        if n > 1 and not torch.isfinite(v).all():  # a weight of 0 times a hidden value that is no number would be NaN
+            y = torch.stack([torch.einsum("hgk,hkd->hgd", p[t, ..., :e], v[:, :e]) for t, e in enumerate(seen.tolist())])
+        else:
+            y = torch.einsum("nhgk,hkd->nhgd", p, v)
+        o[offsets[b]: offsets[b + 1]] = y.reshape(n, H, D).to(q.dtype)
         lse[offsets[b]: offsets[b + 1]] = m.reshape(n, H)
     return (o, lse) if return_lse else o
 

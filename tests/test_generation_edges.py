@@ -275,3 +275,34 @@ def test_attention_shows_nan_in_queries_and_visible_keys(device, dim, rows, pref
     hit = torch.zeros(rows, 2, dtype=torch.bool)
     hit[2, 0] = True
     assert torch.equal(o.isnan().all(-1).cpu(), hit) and torch.equal(lse.isnan().cpu(), hit)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("lens,new,kv_heads,group,dim,page,prefix", [
+    ([7, 5], [7, 5], 1, 1, 32, 8, 0),
+    ([70, 33, 0, 5], [33, 1, 0, 5], 2, 2, 64, 16, 100),
+    ([130, 7, 129], [130, 7, 2], 1, 3, 128, 8, 0),
+    ([90, 31], [77, 31], 1, 1, 128, 64, 191),
+    ([9 + i % 5 for i in range(230)], [4] * 230, 5, 2, 64, 8, 40),
+    ([9 + i % 5 for i in range(230)], [4] * 230, 4, 1, 128, 8, 0),
+])
+def test_attention_leaves_out_hidden_values(device, bad, lens, new, kv_heads, group, dim, page, prefix):
+    """A query's result does not depend on tokens behind it, whatever they hold; those that see the token show it."""
+    p = Problem(lens, new, kv_heads=kv_heads, group=group, dim=dim, page=page, prefix=prefix, device=device)
+    want, want_lse = (t.cpu() for t in p.run())
+    first = torch.tensor([0] + new).cumsum(0).tolist()
+    sees = torch.zeros(sum(new), dtype=torch.bool)
+    for b, (m, n) in enumerate(zip(lens, new)):
+        if n < 2:
+            continue
+        at = m - n + n // 2  # the place of query n // 2
+        page_id = p.rows[b][at // page]
+        p.pool[1, page_id, at % page, 0, 1::2] = bad
+        p.pool[0, page_id, at % page, kv_heads - 1, 0] = bad  # and its key in another head
+        sees[first[b] + n // 2: first[b + 1]] = True
+    o, lse = (t.cpu() for t in p.run())
+    # (the rows that see it are checked below: here they get what they were without it)
+    p.check(torch.where(sees[:, None, None], want, o), torch.where(sees[:, None], want_lse, lse))
+    values = o[sees][:, :group] if kv_heads > 1 else o[sees][:0]
+    assert not values[..., 1::2].isfinite().any()
