@@ -291,6 +291,8 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(
     check_int32(*q_offsets, 1, q, "q_offsets");
     TORCH_CHECK_VALUE(q_offsets->size(0) == B + 1, "q_offsets: one more entry than page_table has rows");
     TORCH_CHECK_VALUE(max_q_len >= 0, "max_q_len: needed with q_offsets");
+    TORCH_CHECK_VALUE(N == 0 || B > 0, "q_offsets: no sequence for the ", N, " tokens");
+    TORCH_CHECK_VALUE(N == 0 || max_q_len > 0, "max_q_len: at least 1 for ", N, " tokens");
   } else {
     TORCH_CHECK_VALUE(N == B, "without q_offsets there is one token for each of the ", B, " sequences, got ", N);
     max_q_len = 1;
@@ -337,9 +339,10 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(
   TORCH_CHECK_VALUE(B * a.own_tiles * a.own_splits * Hk < (1ll << 31), "too many sequences times max_q_len");
   torch::Tensor part;
   if (pieces > 0) {
-    part = at::empty({pieces * rows * (D + 2)}, q.options().dtype(at::kFloat));
+    part = at::empty({pieces * rows * (D + 2) + 1}, q.options().dtype(at::kFloat));
     a.part_o = part.data_ptr<float>();
     a.part_ml = reinterpret_cast<float2*>(a.part_o + pieces * rows * D);
+    if (q_offsets && a.own_splits > 0) a.sound = reinterpret_cast<int*>(a.part_ml + pieces * rows);
   }
   C10_CUDA_CHECK(prefix::launch_attention(a, static_cast<int>(D), at::cuda::getCurrentCUDAStream()));
   return {o, lse};

@@ -112,11 +112,20 @@ struct Args {
   int own_tiles, own_splits, own_chunk;
   float* part_o;    // [pieces][n][heads][head_dim]
   float2* part_ml;  // [pieces][n][heads]: maximum (log2 units) and sum
+  int* sound;  // or null, without q_offsets: whether they give every row to one sequence; if not, the rows of the own
+               // keys' pieces are in part unwritten, and nobody reads them
   __nv_bfloat16* o;
   float* lse;  // or null
   int* status;  // of waits
   int* errors;  // of bad indices
 };
+
+#ifdef __CUDACC__
+// Partial results of a row's own keys that a kernel may read, behind those that write them.
+__device__ __forceinline__ int own_pieces(const Args& a) {
+  return a.sound && *const_cast<volatile int*>(a.sound) == 0 ? 0 : a.own_splits;
+}
+#endif
 
 // Splits the keys into pieces; returns how many partial results each row gets.
 int plan(Args& a, int head_dim);

@@ -74,6 +74,18 @@ constexpr int kUnlimited = 1 << 30;
 
 MNB_DEVICE void flag(const Args& a) { atomicCAS(a.errors, 0, kErrBadIndex); }
 
+// Whether q_offsets ascend from 0 to n in steps of at most max_q; for all threads of a block.
+MNB_DEVICE bool offsets_sound(const Args& a, const int* q_offsets) {
+  bool bad = false;
+  for (int b = threadIdx.x; b <= a.batch; b += blockDim.x) {
+    const long long from = q_offsets[b];
+    if (b == 0) bad = bad || from != 0;
+    if (b == a.batch) bad = bad || from != a.n;
+    else bad = bad || q_offsets[b + 1] < from || q_offsets[b + 1] - from > a.max_q;
+  }
+  return !__syncthreads_or(bad);
+}
+
 // Item i of the list: first the prefix's (split, kv head, row tile; the row tiles of the same keys side by side), then
 // the sequences' own (sequence, row tile, split, kv head).
 // With `heads` of 4 an own piece is that of four kv heads, from p.h on.
@@ -102,19 +114,17 @@ MNB_DEVICE Piece piece_of(const Args& a, const int* seq_lens, const int* q_offse
   p.n0 = b;
   int q_len = 1;
   if (a.q_offsets) {
+    // (within the rows whatever the offsets say: offsets_sound() has the word on them)
     p.n0 = min(max(q_offsets[b], 0), a.n);
-    q_len = min(max(q_offsets[b + 1] - p.n0, 0), a.n - p.n0);
-    if (q_len > a.max_q) {
-      flag(a);
-      q_len = a.max_q;
-    }
+    q_len = min(min(max(q_offsets[b + 1], 0), a.n) - p.n0, a.max_q);
+    q_len = max(q_len, 0);
   }
   p.r0 = rt * tile_rows;
   p.n_rows = min(tile_rows, q_len * a.group - p.r0);
   int len = seq_lens[b];
   if (len < 0 || len > a.max_len) {
     flag(a);
-    len = min(max(len, 0), a.max_len);
+    len = 0;  // the sequence's own tokens are left out
   }
   p.limit0 = len - q_len + 1;
   p.k0 = split * a.own_chunk;
@@ -211,6 +221,13 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
   __syncthreads();
   int pos = 0;  // stages filled, or used, so far
   let_next_start();
+  if (a.sound && blockIdx.x == 0) {
+    const bool sound = offsets_sound(a, q_offsets);
+    if (threadIdx.x == 0) {
+      *a.sound = sound;
+      if (!sound) flag(a);
+    }
+  }
 
   if (warp == 4) {
     const int per = min(1 << a.page_shift, kStep);  // tokens of a box
@@ -441,6 +458,13 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
   }
 }
 
+// A call without pieces of own keys (a bound of 0 for the lengths): reports what the other kernels do not look at.
+__global__ void __launch_bounds__(256) check_kernel(const __grid_constant__ Args a) {
+  bool bad = a.q_offsets && !offsets_sound(a, a.q_offsets);
+  for (int b = threadIdx.x; b < a.batch; b += blockDim.x) bad = bad || a.seq_lens[b] != 0;
+  if (bad) flag(a);
+}
+
 // Joins the pieces of each (token, head).  With many pieces a block takes a row and its warps the pieces in turn, because
 // one warp would wait for one piece after another (512 rows of 20 pieces: 6 us, 9 with a warp each); with few a warp takes
 // a row (76,000 rows of one piece: 57 us less than with a block each).
@@ -453,7 +477,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args 
   const long long row = Together ? blockIdx.x : blockIdx.x * 4ll + warp, rows = static_cast<long long>(a.n) * a.heads;
   wait_for_previous();
   if (row >= rows) return;
-  const int pieces = a.prefix_splits + a.own_splits;
+  const int pieces = a.prefix_splits + own_pieces(a);
   float m = -INFINITY;
   for (int p = lane; p < pieces; p += 32) m = fmaxf(m, a.part_ml[p * rows + row].x);
   m = warp_max(m);
@@ -547,6 +571,10 @@ template <int D>
 static cudaError_t launch_for(const Args& a, cudaStream_t stream) {
   cudaError_t e = cudaSuccess;
   CUtensorMap mk, mv;
+  if (a.own_splits == 0 && a.batch > 0) {
+    check_kernel<<<1, 256, 0, stream>>>(a);
+    if (e = cudaGetLastError(); e != cudaSuccess) return e;
+  }
   const bool by_warps = a.own_splits > 0 || (a.prefix_splits > 0 && !a.tensor_cores);
   if (by_warps) {
     const int tokens = a.quad ? 16 : kKeys;

@@ -466,6 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     using Part = typename Vec<kPer>::type;
     const long long rows = static_cast<long long>(a.n) * a.heads;
     wait_for_previous();  // the own keys' pieces
+    const int own = own_pieces(a);
     const bool alone = a.prefix_splits == 1;  // then this block joins the rows with their own keys' pieces and finishes them
     if (const int i = s * kTile + r; i < n_rows && half == 0) {  // (without `shared`, the first stream's threads)
       const int j = r0 + i, token = j / a.group;
@@ -479,10 +480,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (alone) {
         const float prefix_top = x.top;
-        for (int p = 1; p < 1 + a.own_splits; ++p) x.top = fmaxf(x.top, a.part_ml[p * rows + x.at].x);
+        for (int p = 1; p < 1 + own; ++p) x.top = fmaxf(x.top, a.part_ml[p * rows + x.at].x);
         const float base = x.top == -INFINITY ? 0.f : x.top, f = ex2_approx(prefix_top - base);
         l *= f;
-        for (int p = 1; p < 1 + a.own_splits; ++p) {
+        for (int p = 1; p < 1 + own; ++p) {
           const float2 ml = a.part_ml[p * rows + x.at];
           l = fmaf(ex2_approx(ml.x - base), ml.y, l);
         }
@@ -515,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (i0 + e < n_rows) *reinterpret_cast<Part*>(a.part_o + (split * rows + x[e].at) * D + lane * kPer) = o[e];
         continue;
       }
-      for (int p = 1; p < 1 + a.own_splits; ++p) {
+      for (int p = 1; p < 1 + own; ++p) {
         float top[kBatch];
         Part y[kBatch];
 #pragma unroll

@@ -87,6 +87,11 @@ def shared_prefix_attention(
     Returns ``o`` like ``q`` (contiguous) and, with ``return_lse``, the natural
     log-sum-exp of the scaled scores, fp32 ``[tokens, heads]``.  Head dims 32,
     64 and 128; page sizes 8 to 256, powers of two.
+
+    On the device, a page id outside the pool reads as zeros, a sequence whose
+    length is negative or above its bound has no tokens of its own, and with
+    ``q_offsets`` that do not give every token to one sequence no token has;
+    all are reported.
     """
     if scale is None:
         scale = 1.0 / math.sqrt(max(1, q.shape[-1]))
@@ -118,6 +123,8 @@ def shared_prefix_attention(
         _ints(q_offsets, 1, "q_offsets")
         _need(q_offsets.shape[0] == B + 1, "q_offsets: one more entry than page_table has rows")
         _need(max_q_len is not None and max_q_len >= 0, "max_q_len: needed with q_offsets")
+        _need(N == 0 or B > 0, "q_offsets: no sequence for the tokens")
+        _need(N == 0 or max_q_len > 0, "max_q_len: at least 1 where there are tokens")
         offsets = q_offsets.tolist()
         if offsets[0] != 0 or offsets[-1] != N or any(not 0 <= b - a <= max_q_len for a, b in zip(offsets, offsets[1:])):
             raise RuntimeError("q_offsets: ascending from 0 to the number of tokens, in steps of at most max_q_len")

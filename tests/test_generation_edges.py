@@ -306,3 +306,68 @@ def test_attention_leaves_out_hidden_values(device, bad, lens, new, kv_heads, gr
     p.check(torch.where(sees[:, None, None], want, o), torch.where(sees[:, None], want_lse, lse))
     values = o[sees][:, :group] if kv_heads > 1 else o[sees][:0]
     assert not values[..., 1::2].isfinite().any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim,prefix", [(32, 0), (32, 40), (64, 0), (64, 40), (64, 3000), (128, 200)])
+@pytest.mark.parametrize("offsets,most,limit", [
+    ([3, 40, 60, 70], 60, 90),    # the first rows belong to nobody
+    ([0, 40, 60, 65], 60, 90),    # nor do the last
+    ([0, 50, 40, 70], 60, 90),    # a descent
+    ([0, 40, 60, 90], 60, 90),    # past the rows
+    ([-4, 40, 60, 70], 60, 90),
+    ([0, 40, 60, 70], 25, 90),    # longer than max_q_len
+    ([0, 40, 60, 70], 60, 50),    # lengths beyond max_seq_len
+    ([0, 40, 60, 70], 60, 0),
+    ([0, 40, 69, 70], 60, 0),
+])
+def test_attention_reports_offsets_and_bounds_that_do_not_hold(device, dim, prefix, offsets, most, limit):
+    p = Problem([60, 90, 33], [40, 20, 10], kv_heads=2, group=1, dim=dim, page=16, prefix=prefix, device=device)
+    if device == "cuda":  # what the allocator hands out next holds NaN
+        stale = torch.full((32 << 20,), math.nan, device=device)
+        del stale
+
+    def call():
+        return G.shared_prefix_attention(p.q, p.pool[0], p.pool[1], ints(p.prefix_pages, device), prefix, ints(p.rows, device),
+                                         ints(p.lens, device), q_offsets=ints(offsets, device), max_q_len=most, max_seq_len=limit,
+                                         return_lse=True)
+
+    out = out_of_range(device, call)
+    if out is None:
+        return
+    o, lse = out
+    if limit == 90:  # rows without a sequence of their own: the own tokens of the whole call are left out
+        p.lens, p.own, p.new = [0] * 3, [t[:, :0] for t in p.own], [40, 20, 10]
+        p.check(o, lse)
+    else:
+        assert not o.isnan().any() and not lse.isnan().any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_attention_bounds_that_no_call_can_keep(device):
+    p = Problem([20, 5], [3, 2], kv_heads=1, group=1, dim=64, page=16, prefix=10, device=device)
+    args = (p.q, p.pool[0], p.pool[1], ints(p.prefix_pages, device), 10)
+    with pytest.raises(ValueError, match="max_q_len"):
+        G.shared_prefix_attention(*args, ints(p.rows, device), ints(p.lens, device), q_offsets=ints([0, 3, 5], device), max_q_len=0)
+    with pytest.raises(ValueError, match="q_offsets"):
+        G.shared_prefix_attention(*args, torch.empty(0, 2, dtype=torch.int32, device=device), ints([], device),
+                                  q_offsets=ints([0], device), max_q_len=5)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_attention_over_the_prefix_alone(device):
+    # a bound of 0 with lengths of 0 is a sound request
+    for rows in (3, 60):
+        p = Problem([0] * rows, [1] * rows, kv_heads=2, group=1, dim=64, page=16, prefix=140, device=device)
+        p.check(*p.run(max_seq_len=0))
+
+
+@pytest.mark.gpu
+def test_attention_leaves_out_a_sequence_with_a_bad_length():
+    for lens, bound in (([20, -3, 30], 48), ([20, 49, 30], 48)):
+        p = Problem([20, 48, 30], [1, 1, 1], kv_heads=2, group=1, dim=64, page=16, prefix=40, device="cuda")
+        o, lse = out_of_range("cuda", lambda: G.shared_prefix_attention(
+            p.q, p.pool[0], p.pool[1], ints(p.prefix_pages, "cuda"), 40, ints(p.rows, "cuda"), ints(lens, "cuda"), max_seq_len=bound,
+            return_lse=True))
+        p.lens[1], p.own[1] = 0, p.own[1][:, :0]
+        p.check(o, lse)
