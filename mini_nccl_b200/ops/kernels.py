@@ -79,10 +79,11 @@ def check_status(device: torch.device | None = None) -> None:
         v, _, left_out, _ = st.tolist()
         if v or left_out:
             st.zero_()
+        reports = [f"GEMM kernel on cuda:{idx} reported pipeline status {v}"] if v else []
         if left_out:
-            raise RuntimeError(f"request left out on cuda:{idx}: {_REQUEST_STATUS.get(left_out, left_out)}")
-        if v:
-            raise RuntimeError(f"GEMM kernel on cuda:{idx} reported pipeline status {v}")
+            reports.append(f"request left out on cuda:{idx}: {_REQUEST_STATUS.get(left_out, left_out)}")
+        if reports:
+            raise RuntimeError("; ".join(reports))
 
 
 def supports_gemm(x: torch.Tensor, w: torch.Tensor) -> bool:

@@ -371,3 +371,20 @@ def test_attention_leaves_out_a_sequence_with_a_bad_length():
             return_lse=True))
         p.lens[1], p.own[1] = 0, p.own[1][:, :0]
         p.check(o, lse)
+
+
+# ---- status ------------------------------------------------------------------------------
+
+
+def test_check_status_reports_a_pipeline_and_a_request_at_once(monkeypatch):
+    from mini_nccl_b200.ops import kernels as K
+
+    word = torch.zeros(4, dtype=torch.int32)
+    monkeypatch.setattr(K, "_STATUS", {0: word})
+    K.check_status()
+    for value, match in (([2, 0, 4, 0], "pipeline status 2.*too few free pages"), ([2, 0, 0, 0], "pipeline status 2$"),
+                         ([0, 0, 5, 0], "^request left out on cuda:0.*outside its tensor")):
+        word.copy_(torch.tensor(value))
+        with pytest.raises(RuntimeError, match=match):
+            K.check_status()
+        K.check_status()  # the words were cleared
