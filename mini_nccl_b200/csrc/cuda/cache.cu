@@ -86,7 +86,8 @@ MNB_DEVICE void claim(const int* slot_of, int n, int slots, int* owner) {
 // part-filled last one gets a page of its own (src / dst / tokens name the copy).
 // Few requests keep their state in shared memory: what is left of the time is
 // three trips to memory, one after another (the requests, their lengths, the rows):
-// 6.6 us for 4 requests with cold caches.
+// 6.6 us for 4 requests with cold caches.  That a parent's row names no page of the pool shows only when the child's is
+// written, so such a request is taken back then (the page that it had been given stays free, also for later requests).
 constexpr int kFew = 256;
 __global__ void __launch_bounds__(kThreads) fork_plan_kernel(Table t, const int* __restrict__ parents,
                                                              const int* __restrict__ children, int n, int* owner,
@@ -144,36 +145,62 @@ __global__ void __launch_bounds__(kThreads) fork_plan_kernel(Table t, const int*
     if (of_dst[i] >= have) of_tokens[i] = of_dst[i] = -1;  // no page left: the child stays empty
   }
   __syncthreads();
-  // entries of the children's rows, request by request (i and col advance without divisions)
-  int i = threadIdx.x / t.columns, col = threadIdx.x % t.columns;
-  const int step_i = kThreads / t.columns, step_col = kThreads % t.columns;
-  for (; i < n; i += step_i, col += step_col) {
-    if (col >= t.columns) {
-      col -= t.columns;
-      if (++i >= n) break;
+  // f(request, column, the parent's row, its full pages) for the entries of the children's rows, request by request (i and
+  // col advance without divisions)
+  auto entries = [&](auto f) {
+    int i = threadIdx.x / t.columns, col = threadIdx.x % t.columns;
+    const int step_i = kThreads / t.columns, step_col = kThreads % t.columns;
+    for (; i < n; i += step_i, col += step_col) {
+      if (col >= t.columns) {
+        col -= t.columns;
+        if (++i >= n) break;
+      }
+      if (of_tokens[i] < 0) continue;
+      const int p = few ? few_parent[i] : parents[i];
+      f(i, col, t.table + p * t.ld, (few ? few_len[i] : t.lens[p]) / t.page_size);
     }
-    if (of_tokens[i] < 0) continue;
-    const int p = few ? few_parent[i] : parents[i], full = (few ? few_len[i] : t.lens[p]) / t.page_size;
+  };
+  auto child_row = [&](int i) { return t.table + (few ? few_child[i] : children[i]) * t.ld; };
+  auto of_pool = [&](int page) { return page >= 0 && page < t.pages; };
+  bool damaged = false;
+  entries([&](int i, int col, const int* row, int full) {
     int page = -1;
     if (col <= full) {
-      page = t.table[p * t.ld + col];
+      page = row[col];
       if (col == full) {
-        if (of_tokens[i] > 0 && page >= 0 && page < t.pages) of_src[i] = page;
+        if (of_tokens[i] > 0 && of_pool(page)) of_src[i] = page;
+        damaged = damaged || (of_tokens[i] > 0 && !of_pool(page));
         page = of_tokens[i] > 0 ? of_ids[of_dst[i]] : -1;
         if (page >= 0) t.refs[page] = 1;
-      } else if (page < 0 || page >= t.pages) {
-        flag(status, kErrBadIndex);
-        page = -1;
-      } else {
+      } else if (of_pool(page)) {
         atomicAdd(t.refs + page, 1);
+      } else {
+        damaged = true;
       }
     }
-    t.table[(few ? few_child[i] : children[i]) * t.ld + col] = page;
+    child_row(i)[col] = page;
+  });
+  if (__syncthreads_or(damaged)) {
+    entries([&](int i, int col, const int* row, int full) {  // which requests it is (-2)
+      if (col < full ? !of_pool(row[col]) : col == full && of_tokens[i] > 0 && !of_pool(row[col])) of_src[i] = -2;
+    });
+    __syncthreads();
+    entries([&](int i, int col, const int* row, int full) {
+      if (of_src[i] != -2) return;
+      if (col < full && of_pool(row[col])) atomicSub(t.refs + row[col], 1);
+      if (col == full && of_tokens[i] > 0) t.refs[of_ids[of_dst[i]]] = 0;
+      child_row(i)[col] = -1;
+    });
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads)
+      if (of_src[i] == -2) {
+        of_tokens[i] = of_dst[i] = -1;
+        flag(status, kErrBadIndex);
+      }
+    __syncthreads();
   }
-  __syncthreads();
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const int to = of_tokens[i] >= 0 && of_dst[i] >= 0 ? of_ids[of_dst[i]] : -1;
-    if (to >= 0 && of_src[i] < 0) flag(status, kErrBadIndex);  // the parent's last page is not in the pool
     if (of_tokens[i] >= 0) t.lens[few ? few_child[i] : children[i]] = few ? few_len[i] : t.lens[parents[i]];
     src[i] = of_src[i];
     dst[i] = to;

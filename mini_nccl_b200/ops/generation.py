@@ -353,7 +353,8 @@ def fork_sequences(
     own, so appending to either never touches the other.  New pages are the
     lowest free ids, in the order of the requests.  Children are distinct,
     empty (length 0) and nobody's parent in the same call; a request that
-    breaks this, or finds no free page, is left out and reported.
+    breaks this, finds no free page, or whose parent's row names a page outside
+    the pool, is left out and reported.
     """
     if kv.is_cuda:
         K = _kernels()
@@ -368,6 +369,9 @@ def fork_sequences(
         if not (0 <= p < S and 0 <= c < S and cs.index(c) == i and p not in cs and int(lens[c]) == 0
                 and 0 <= int(lens[p]) <= W * page):
             raise RuntimeError(f"fork {i}: sequence {p} to {c} (children are distinct, empty and nobody's parent)")
+        held = page_table[p, : -(-int(lens[p]) // page)]
+        if held.numel() and (int(held.min()) < 0 or int(held.max()) >= pool.shape[1]):
+            raise RuntimeError(f"fork {i}: the row of sequence {p} names a page outside the pool")
     free = _free_ids(refs)
     if sum(int(lens[p]) % page > 0 for p in ps) > len(free):
         raise RuntimeError("the pool has too few free pages")

@@ -388,3 +388,32 @@ def test_check_status_reports_a_pipeline_and_a_request_at_once(monkeypatch):
         with pytest.raises(RuntimeError, match=match):
             K.check_status()
         K.check_status()  # the words were cleared
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("bad", [-1, 10 ** 6, -(1 << 31)])
+@pytest.mark.parametrize("column", [0, 1, 2])
+def test_fork_of_a_damaged_sequence_is_left_out(device, bad, column, many):
+    """A parent whose row names no page of the pool: in the middle, or where the part-filled last page is."""
+    lens = [20, 13, 17] + [9] * (300 if many else 2)
+    b = Books(device, lens, slots=2 * len(lens), columns=4, pages=1300)
+    want = [b.tokens(s) for s in range(len(lens))]
+    b.table[2, column] = bad
+    table, n, refs = b.table.clone(), b.lens.clone(), b.refs.clone()
+    at = len(lens)
+    parents = [0, 2, 1] + list(range(3, len(lens)))
+    children = list(range(at, 2 * at))
+    out_of_range(device, lambda: G.fork_sequences(b.kv, b.table, b.lens, b.refs, ints(parents, device), ints(children, device)))
+    assert torch.equal(b.table[:at], table[:at]) and torch.equal(b.lens[:at], n[:at])
+    if device == "cpu":
+        assert torch.equal(b.table, table) and torch.equal(b.lens, n) and torch.equal(b.refs, refs)
+        return
+    assert int(b.lens[at + 1]) == 0 and torch.all(b.table[at + 1] == -1)
+    for p, c in zip(parents, children):
+        if p != 2:
+            assert torch.equal(b.tokens(c), want[p])
+    held = b.table[(b.table >= 0) & (b.table < 1300)].long()
+    missing = torch.bincount(held, minlength=1300).int()
+    gap = b.refs - missing
+    assert int(gap.sum()) == 1 and int(gap.min()) == 0, "only the page that the damaged row no longer names"
