@@ -414,11 +414,11 @@ def reserve_pages(
         if not (0 <= s < S and n >= 0 and ss.index(s) == i and int(lens[s]) + n <= min(W * page_size, 2 ** 31 - 1)):
             raise RuntimeError(f"reserve {i}: {n} tokens for sequence {s}")
     free = _free_ids(refs)
-    for s, n in zip(ss, ns):
-        first, last = -(-int(lens[s]) // page_size), -(-(int(lens[s]) + n) // page_size)
-        if last - first > len(free):
-            raise RuntimeError("the pool has too few free pages")
-        for column in range(first, last):
+    new = [range(-(-int(lens[s]) // page_size), -(-(int(lens[s]) + n) // page_size)) for s, n in zip(ss, ns)]
+    if sum(map(len, new)) > len(free):
+        raise RuntimeError("the pool has too few free pages")
+    for s, n, columns in zip(ss, ns, new):
+        for column in columns:
             page_table[s, column] = free.pop(0)
             refs[page_table[s, column]] = 1
         lens[s] += n

@@ -417,3 +417,14 @@ def test_fork_of_a_damaged_sequence_is_left_out(device, bad, column, many):
     missing = torch.bincount(held, minlength=1300).int()
     gap = b.refs - missing
     assert int(gap.sum()) == 1 and int(gap.min()) == 0, "only the page that the damaged row no longer names"
+
+
+def test_reserve_without_room_changes_nothing_on_the_cpu():
+    c = G.PagedKVCache(1, 4, 8, 1, 32, max_seqs=3, max_seq_len=32, device="cpu")
+    c.extend([0], [9])
+    with pytest.raises(RuntimeError, match="too few free pages"):
+        c.extend([1, 2], [16, 8])
+    assert c.lengths == [9, 0, 0] and c.lens.tolist() == c.lengths and c.pages_in_use() == 2
+    assert torch.all(c.page_table[1:] == -1)
+    c.extend([2], [16])
+    assert c.lens.tolist() == c.lengths == [9, 0, 16]
