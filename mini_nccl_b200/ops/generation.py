@@ -18,7 +18,8 @@ runs out of pages -- cannot raise without waiting for the GPU: the kernels
 leave such a request out, never touch memory outside the tensors, and set the
 device's status word, which :func:`mini_nccl_b200.ops.kernels.check_status`
 turns into an error (the CPU path raises at once).  Nothing here has a
-gradient: these operators serve, they do not train.
+gradient on CUDA: these operators serve, they do not train, and a backward pass
+through an output or a log-probability raises.
 """
 
 from __future__ import annotations
@@ -48,6 +49,25 @@ def _need(ok: bool, message: str) -> None:
 
 def _ints(t: torch.Tensor, dim: int, what: str) -> None:
     _need(t.dtype == torch.int32 and t.dim() == dim, f"{what}: a {dim}-d int32 tensor")
+
+
+class _NoGradient(torch.autograd.Function):
+    """A kernel's result as a function of its inputs, for inputs that want a gradient: asking for it raises."""
+
+    @staticmethod
+    def forward(ctx, name, out, *inputs):
+        ctx.name = name
+        return out.view_as(out)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.name} has no gradient on CUDA: it serves, it does not train")
+
+
+def _of(name: str, out: torch.Tensor, *inputs: torch.Tensor) -> torch.Tensor:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in inputs):
+        return _NoGradient.apply(name, out, *inputs)
+    return out
 
 
 # ---- attention -----------------------------------------------------------------------
@@ -101,7 +121,8 @@ def shared_prefix_attention(
             q, k_pages, v_pages, prefix_pages, prefix_len, page_table, seq_lens, q_offsets,
             -1 if max_q_len is None else max_q_len, -1 if max_seq_len is None else max_seq_len, scale, return_lse,
             K.status_word(q.device))
-        return (o, lse) if return_lse else o
+        o = _of("shared_prefix_attention", o, q, k_pages, v_pages)
+        return (o, _of("shared_prefix_attention", lse, q, k_pages, v_pages)) if return_lse else o
     _need(q.dim() == 3 and k_pages.dim() == 4 and k_pages.shape == v_pages.shape,
           "q: [tokens, heads, head_dim]; k_pages and v_pages: [num_pages, page_size, kv_heads, head_dim]")
     _ints(prefix_pages, 1, "prefix_pages")
@@ -209,7 +230,10 @@ def sample(
         token, logprob = K.ext().sample(
             logits, noise, *split(temperature, float), *split(top_k, int), *split(top_p, float), *split(min_p, float),
             return_logprob, K.status_word(logits.device))
-        return (token, logprob) if return_logprob else token
+        if not return_logprob:
+            return token
+        settings = (t for t in (temperature, top_p, min_p) if isinstance(t, torch.Tensor))
+        return token, _of("sample", logprob, logits, noise, *settings)
     _need(logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32),
           "logits: a bf16 or fp32 tensor [rows, vocabulary]")
     R, V = logits.shape

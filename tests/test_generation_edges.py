@@ -428,3 +428,22 @@ def test_reserve_without_room_changes_nothing_on_the_cpu():
     assert torch.all(c.page_table[1:] == -1)
     c.extend([2], [16])
     assert c.lens.tolist() == c.lengths == [9, 0, 16]
+
+
+@pytest.mark.gpu
+def test_gradients_are_refused_not_lost():
+    p = Problem([20, 5], [1, 1], kv_heads=2, group=1, dim=64, page=16, prefix=40, device="cuda")
+    want, want_lse = p.run()
+    p.q = p.q.detach().requires_grad_()
+    o, lse = p.run()
+    assert torch.equal(o, want) and torch.equal(lse, want_lse) and o.requires_grad and lse.requires_grad
+    for out in (o, lse):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            out.float().sum().backward()
+    with torch.no_grad():
+        assert not p.run()[0].requires_grad
+    x = torch.randn(3, 100, device="cuda", requires_grad=True)
+    token, logprob = G.sample(x, torch.zeros(3, 100, device="cuda"), return_logprob=True)
+    assert not token.requires_grad and logprob.requires_grad
+    with pytest.raises(RuntimeError, match="no gradient"):
+        logprob.sum().backward()
