@@ -30,16 +30,18 @@ cudaError_t launch_after(void (*kernel)(P...), int blocks, int threads, int byte
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// A kernel's limit of dynamic shared memory on each device, raised when a launch needs more than any before.
+// A kernel's limit of dynamic shared memory on each device, raised when a launch needs more than any before, and then to
+// all that the kernel can have (`most`): every call sets the same value, so that calls from several threads agree.
 struct SharedMemory {
   static constexpr int kDevices = 64;
   std::atomic<int> limit[kDevices] = {};
-  cudaError_t at_least(const void* kernel, int bytes) {
+  cudaError_t at_least(const void* kernel, int bytes, int most = 227 * 1024 - 4096) {
     int dev = 0;
     if (const cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
     if (dev < kDevices && bytes <= limit[dev].load(std::memory_order_acquire)) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 4096 > bytes ? 227 * 1024 - 4096 : bytes);
-    if (e == cudaSuccess && dev < kDevices) limit[dev].store(227 * 1024 - 4096 > bytes ? 227 * 1024 - 4096 : bytes, std::memory_order_release);
+    if (most < bytes) most = bytes;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e == cudaSuccess && dev < kDevices) limit[dev].store(most, std::memory_order_release);
     return e;
   }
 };

@@ -41,6 +41,7 @@
 
 #include "common.cuh"
 #include "generation.h"
+#include "launch.cuh"
 
 namespace mnb {
 
@@ -1029,8 +1030,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 
 template <typename T, bool Staged, bool Multi>
 static cudaError_t launch_with(const Sample& a, int cluster, int bytes, cudaStream_t stream) {
+  static SharedMemory allowed;
   if (Staged)
-    if (const cudaError_t e = cudaFuncSetAttribute(sample_kernel<T, Staged, Multi>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (const cudaError_t e = allowed.at_least(reinterpret_cast<const void*>(sample_kernel<T, Staged, Multi>), bytes,
+                                               227 * 1024 - 1024 - static_cast<int>(sizeof(Shared<Multi>)));
         e != cudaSuccess)
       return e;
   cudaLaunchConfig_t cfg{};

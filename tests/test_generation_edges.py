@@ -447,3 +447,26 @@ def test_gradients_are_refused_not_lost():
     assert not token.requires_grad and logprob.requires_grad
     with pytest.raises(RuntimeError, match="no gradient"):
         logprob.sum().backward()
+
+
+# ---- sampling ----------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+def test_sample_from_several_threads():
+    """Rows of very different lengths at once, each thread on a stream of its own: a launch may not lower another's limits."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    def work(vocab):
+        x, noise = (t.cuda() for t in logits_of(3, vocab, torch.float32, seed=vocab))
+        want = G.sample(x, noise, top_p=0.9)
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            got = [G.sample(x, noise, top_p=0.9) for _ in range(60)]
+        stream.synchronize()
+        return all(torch.equal(t, want) for t in got)
+
+    with ThreadPoolExecutor(4) as pool:
+        assert all(pool.map(work, [300, 50304, 9001, 130003, 20000, 40000]))
+    settle("cuda")
