@@ -64,12 +64,6 @@ class _NoGradient(torch.autograd.Function):
         raise RuntimeError(f"{ctx.name} has no gradient on CUDA: it serves, it does not train")
 
 
-def _of(name: str, out: torch.Tensor, *inputs: torch.Tensor) -> torch.Tensor:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in inputs):
-        return _NoGradient.apply(name, out, *inputs)
-    return out
-
-
 # ---- attention -----------------------------------------------------------------------
 
 
@@ -121,8 +115,9 @@ def shared_prefix_attention(
             q, k_pages, v_pages, prefix_pages, prefix_len, page_table, seq_lens, q_offsets,
             -1 if max_q_len is None else max_q_len, -1 if max_seq_len is None else max_seq_len, scale, return_lse,
             K.status_word(q.device))
-        o = _of("shared_prefix_attention", o, q, k_pages, v_pages)
-        return (o, _of("shared_prefix_attention", lse, q, k_pages, v_pages)) if return_lse else o
+        if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
+            o, lse = (None if t is None else _NoGradient.apply("shared_prefix_attention", t, q, k_pages, v_pages) for t in (o, lse))
+        return (o, lse) if return_lse else o
     _need(q.dim() == 3 and k_pages.dim() == 4 and k_pages.shape == v_pages.shape,
           "q: [tokens, heads, head_dim]; k_pages and v_pages: [num_pages, page_size, kv_heads, head_dim]")
     _ints(prefix_pages, 1, "prefix_pages")
@@ -227,13 +222,14 @@ def sample(
             return (x, whole(0)) if isinstance(x, torch.Tensor) else (None, whole(x))
 
         K = _kernels()
-        token, logprob = K.ext().sample(
-            logits, noise, *split(temperature, float), *split(top_k, int), *split(top_p, float), *split(min_p, float),
-            return_logprob, K.status_word(logits.device))
-        if not return_logprob:
-            return token
-        settings = (t for t in (temperature, top_p, min_p) if isinstance(t, torch.Tensor))
-        return token, _of("sample", logprob, logits, noise, *settings)
+        heat, nucleus, least = split(temperature, float), split(top_p, float), split(min_p, float)
+        token, logprob = K.ext().sample(logits, noise, *heat, *split(top_k, int), *nucleus, *least, return_logprob,
+                                        K.status_word(logits.device))
+        if return_logprob and torch.is_grad_enabled() and (
+                logits.requires_grad or noise.requires_grad or (heat[0] is not None and heat[0].requires_grad)
+                or (nucleus[0] is not None and nucleus[0].requires_grad) or (least[0] is not None and least[0].requires_grad)):
+            logprob = _NoGradient.apply("sample", logprob, logits, noise, heat[0], nucleus[0], least[0])
+        return (token, logprob) if return_logprob else token
     _need(logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32),
           "logits: a bf16 or fp32 tensor [rows, vocabulary]")
     R, V = logits.shape
