@@ -444,7 +444,6 @@ cudaError_t launch_compact(const Pool& p, const int* table, long long table_ld, 
                            int* new_table, int* new_refs, int* scratch, int* status, cudaStream_t stream) {
   int* s = scratch;
   const long long all = static_cast<long long>(rows) * columns;
-  constexpr int kSmallTable = 16 * kThreads;  // the planning block does 16 entries a thread in less time than a launch takes
   const bool small = all <= kSmallTable;
   compact_plan_kernel<<<1, kThreads, 0, stream>>>(refs, p.pages, new_refs, s, s + p.pages, s + 2 * p.pages, s + 3 * p.pages,
                                                   table, table_ld, columns, small ? static_cast<int>(all) : 0, new_table);

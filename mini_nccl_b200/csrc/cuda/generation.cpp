@@ -14,6 +14,8 @@ namespace {
 
 constexpr double kLog2e = 1.4426950408889634;
 
+thread_local int64_t launched = 0;  // kernels of the last call
+
 void check_int32(const torch::Tensor& t, int64_t dim, const torch::Tensor& like, const char* what) {
   TORCH_CHECK_VALUE(t.is_cuda() && t.device() == like.device() && t.scalar_type() == at::kInt && t.dim() == dim &&
                         (t.numel() == 0 || t.stride(dim - 1) == 1),
@@ -85,7 +87,10 @@ S setting(const c10::optional<torch::Tensor>& each, double all, int64_t rows, at
 
 }  // namespace
 
+int64_t generation_launches() { return launched; }
+
 void copy_pages(const torch::Tensor& kv, const torch::Tensor& src, const torch::Tensor& dst, const torch::Tensor& status) {
+  launched = 0;
   const auto p = pool_of(kv);
   check_int32(src, 1, kv, "src");
   check_int32(dst, 1, kv, "dst");
@@ -94,10 +99,12 @@ void copy_pages(const torch::Tensor& kv, const torch::Tensor& src, const torch::
   const c10::cuda::CUDAGuard guard(kv.device());
   C10_CUDA_CHECK(cache::launch_copy(p, src.data_ptr<int>(), dst.data_ptr<int>(), nullptr, nullptr,
                                     static_cast<int>(src.size(0)), errors_of(status), at::cuda::getCurrentCUDAStream()));
+  launched = src.size(0) > 0;
 }
 
 void fork_sequences(const torch::Tensor& kv, const torch::Tensor& page_table, const torch::Tensor& lens, const torch::Tensor& refs,
                     const torch::Tensor& parents, const torch::Tensor& children, const torch::Tensor& status) {
+  launched = 0;
   const auto p = pool_of(kv);
   const auto t = table_of(page_table, lens, refs, p.page_size);
   check_int32(parents, 1, kv, "parents");
@@ -113,10 +120,12 @@ void fork_sequences(const torch::Tensor& kv, const torch::Tensor& page_table, co
   auto scratch = at::empty({4 * n + t.slots}, parents.options());
   C10_CUDA_CHECK(cache::launch_fork(p, t, parents.data_ptr<int>(), children.data_ptr<int>(), static_cast<int>(n),
                                     scratch.data_ptr<int>(), errors_of(status), at::cuda::getCurrentCUDAStream()));
+  launched = 2;
 }
 
 void reserve_pages(const torch::Tensor& page_table, const torch::Tensor& lens, const torch::Tensor& refs, const torch::Tensor& slots,
                    const torch::Tensor& counts, int64_t page_size, const torch::Tensor& status) {
+  launched = 0;
   TORCH_CHECK_VALUE(page_size >= 1 && page_size < (1 << 30), "page_size: at least 1");
   const auto t = table_of(page_table, lens, refs, static_cast<int>(page_size));
   check_int32(slots, 1, page_table, "slots");
@@ -129,10 +138,12 @@ void reserve_pages(const torch::Tensor& page_table, const torch::Tensor& lens, c
   auto scratch = at::empty({t.pages + n + t.slots}, slots.options());
   C10_CUDA_CHECK(cache::launch_reserve(t, slots.data_ptr<int>(), counts.data_ptr<int>(), static_cast<int>(n),
                                        scratch.data_ptr<int>(), errors_of(status), at::cuda::getCurrentCUDAStream()));
+  launched = 1;
 }
 
 void free_sequences(const torch::Tensor& page_table, const torch::Tensor& lens, const torch::Tensor& refs, const torch::Tensor& slots,
                     const torch::Tensor& status) {
+  launched = 0;
   const auto t = table_of(page_table, lens, refs, 1);
   check_int32(slots, 1, page_table, "slots");
   check_status_word(status);
@@ -140,10 +151,12 @@ void free_sequences(const torch::Tensor& page_table, const torch::Tensor& lens, 
   if (n == 0 || t.columns == 0) return;
   const c10::cuda::CUDAGuard guard(page_table.device());
   C10_CUDA_CHECK(cache::launch_free(t, slots.data_ptr<int>(), n, errors_of(status), at::cuda::getCurrentCUDAStream()));
+  launched = 1;
 }
 
 std::tuple<torch::Tensor, torch::Tensor> compact_pages(const torch::Tensor& kv, const torch::Tensor& page_table, const torch::Tensor& refs,
                                                        const torch::Tensor& status) {
+  launched = 0;
   const auto p = pool_of(kv);
   check_int32(page_table, 2, kv, "page_table");
   check_int32(refs, 1, kv, "refs");
@@ -157,11 +170,13 @@ std::tuple<torch::Tensor, torch::Tensor> compact_pages(const torch::Tensor& kv, 
                                        static_cast<int>(page_table.size(0)), static_cast<int>(page_table.size(1)),
                                        refs.data_ptr<int>(), new_table.data_ptr<int>(), new_refs.data_ptr<int>(),
                                        scratch.data_ptr<int>(), errors_of(status), at::cuda::getCurrentCUDAStream()));
+  launched = page_table.numel() > cache::kSmallTable ? 3 : 2;
   return {new_table, new_refs};
 }
 
 void append_kv(const torch::Tensor& k_pages, const torch::Tensor& v_pages, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& page_table,
                const torch::Tensor& positions, const c10::optional<torch::Tensor>& slots, const torch::Tensor& status) {
+  launched = 0;
   TORCH_CHECK_VALUE(k_pages.is_cuda() && k_pages.dim() == 4 && k_pages.scalar_type() == at::kBFloat16 &&
                         v_pages.scalar_type() == at::kBFloat16 && v_pages.sizes() == k_pages.sizes() &&
                         v_pages.strides() == k_pages.strides() && v_pages.device() == k_pages.device(),
@@ -211,12 +226,14 @@ void append_kv(const torch::Tensor& k_pages, const torch::Tensor& v_pages, const
   a.heads = static_cast<int>(H);
   a.chunks = static_cast<int>(D / 8);
   C10_CUDA_CHECK(cache::launch_append(a, errors_of(status), at::cuda::getCurrentCUDAStream()));
+  launched = 1;
 }
 
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>> sample(
     const torch::Tensor& logits, const torch::Tensor& noise, const c10::optional<torch::Tensor>& temperature, double temperature_all,
     const c10::optional<torch::Tensor>& top_k, int64_t top_k_all, const c10::optional<torch::Tensor>& top_p, double top_p_all,
     const c10::optional<torch::Tensor>& min_p, double min_p_all, bool return_logprob, const torch::Tensor& status) {
+  launched = 0;
   using sampling::Setting;
   TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() == 2 &&
                         (logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kFloat),
@@ -251,6 +268,7 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> sample(
   a.token = reinterpret_cast<long long*>(token.data_ptr<int64_t>());
   a.logprob = logprob ? logprob->data_ptr<float>() : nullptr;
   C10_CUDA_CHECK(sampling::launch_sample(a, at::cuda::getCurrentCUDAStream()));
+  launched = 1;
   return {token, logprob};
 }
 
@@ -258,6 +276,7 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(
     const torch::Tensor& q, const torch::Tensor& k_pages, const torch::Tensor& v_pages, const torch::Tensor& prefix_pages, int64_t prefix_len,
     const torch::Tensor& page_table, const torch::Tensor& seq_lens, const c10::optional<torch::Tensor>& q_offsets, int64_t max_q_len,
     int64_t max_seq_len, double scale, bool return_lse, const torch::Tensor& status) {
+  launched = 0;
   TORCH_CHECK_VALUE(q.is_cuda() && q.scalar_type() == at::kBFloat16 && q.dim() == 3,
                     "q: a bf16 CUDA tensor [tokens, heads, head_dim]");
   TORCH_CHECK_VALUE(k_pages.device() == q.device() && v_pages.device() == q.device() &&
@@ -345,6 +364,7 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(
     if (q_offsets && a.own_splits > 0) a.sound = reinterpret_cast<int*>(a.part_ml + pieces * rows);
   }
   C10_CUDA_CHECK(prefix::launch_attention(a, static_cast<int>(D), at::cuda::getCurrentCUDAStream()));
+  launched = prefix::kernels(a);
   return {o, lse};
 }
 

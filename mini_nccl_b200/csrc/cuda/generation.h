@@ -48,6 +48,7 @@ cudaError_t launch_reserve(const Table& t, const int* slots, const int* counts, 
                            cudaStream_t stream);
 cudaError_t launch_free(const Table& t, const int* slots, int n, int* status, cudaStream_t stream);
 // scratch: 3 pages + 1 ints
+constexpr int kSmallTable = 16 * 1024;  // entries that the planning block remaps itself, in less time than a launch takes
 cudaError_t launch_compact(const Pool& p, const int* table, long long table_ld, int rows, int columns, const int* refs,
                            int* new_table, int* new_refs, int* scratch, int* status, cudaStream_t stream);
 cudaError_t launch_append(const Append& a, int* status, cudaStream_t stream);
@@ -132,6 +133,7 @@ int plan(Args& a, int head_dim);
 // head dims 64 and 128; with one prefix piece, joins the rows and finishes them
 cudaError_t launch_prefix_tc(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, int head_dim, cudaStream_t stream);
 cudaError_t launch_attention(const Args& a, int head_dim, cudaStream_t stream);
+int kernels(const Args& a);  // that launch_attention() launches
 
 }  // namespace prefix
 

@@ -567,25 +567,31 @@ static cudaError_t launch_pieces_of(const Args& a, const CUtensorMap& mk, const 
   }
 }
 
+// Which kernels a call takes.
+static bool checks(const Args& a) { return a.own_splits == 0 && a.batch > 0; }
+static bool by_warps(const Args& a) { return a.own_splits > 0 || (a.prefix_splits > 0 && !a.tensor_cores); }
+static bool by_tensor_cores(const Args& a) { return a.tensor_cores && a.prefix_splits > 0; }
+static bool joins(const Args& a) { return !(by_tensor_cores(a) && a.prefix_splits == 1); }
+int kernels(const Args& a) { return checks(a) + by_warps(a) + by_tensor_cores(a) + joins(a); }
+
 template <int D>
 static cudaError_t launch_for(const Args& a, cudaStream_t stream) {
   cudaError_t e = cudaSuccess;
   CUtensorMap mk, mv;
-  if (a.own_splits == 0 && a.batch > 0) {
+  if (checks(a)) {
     check_kernel<<<1, 256, 0, stream>>>(a);
     if (e = cudaGetLastError(); e != cudaSuccess) return e;
   }
-  const bool by_warps = a.own_splits > 0 || (a.prefix_splits > 0 && !a.tensor_cores);
-  if (by_warps) {
+  if (by_warps(a)) {
     const int tokens = a.quad ? 16 : kKeys;
     if (!pool_map(&mk, a.k, a, D, tokens) || !pool_map(&mv, a.v, a, D, tokens)) return cudaErrorInvalidValue;
     e = a.max_q > 1 ? launch_pieces_of<D, true>(a, mk, mv, stream) : launch_pieces_of<D, false>(a, mk, mv, stream);
     if (e != cudaSuccess) return e;
   }
-  if (a.tensor_cores && a.prefix_splits > 0) {
-    if ((!by_warps || a.quad) && (!pool_map(&mk, a.k, a, D, kKeys) || !pool_map(&mv, a.v, a, D, kKeys))) return cudaErrorInvalidValue;
+  if (by_tensor_cores(a)) {
+    if ((!by_warps(a) || a.quad) && (!pool_map(&mk, a.k, a, D, kKeys) || !pool_map(&mv, a.v, a, D, kKeys))) return cudaErrorInvalidValue;
     e = launch_prefix_tc(a, mk, mv, D, stream);
-    if (e != cudaSuccess || a.prefix_splits == 1) return e;
+    if (e != cudaSuccess || !joins(a)) return e;
   }
   const int rows = a.n * a.heads;
   if (a.prefix_splits + a.own_splits > 4) return launch_after(join_kernel<D, true>, rows, 128, 0, stream, a);

@@ -30,14 +30,6 @@ KERNELS_PER_CALL = {
     "flash_attn_fwd_tc": 1,
     "flash_attn_bwd": 3,
     "flash_attn_bwd_tc": 3,
-    "copy_pages": 1,
-    "fork_sequences": 2,
-    "reserve_pages": 1,
-    "free_sequences": 1,
-    "compact_pages": 2,
-    "append_kv": 1,
-    "sample": 1,
-    "shared_prefix_attention": 2,
     "all_reduce": 1,
     "reduce_scatter": 1,
     "move": 1,
@@ -47,6 +39,11 @@ KERNELS_PER_CALL = {
     "reduce_scatter_adamw": 1,
     "ag_gemm": 1,
 }
+
+
+# Entry points whose number of kernels depends on the call: the extension says how many the last one launched.
+ASKED = {"copy_pages", "fork_sequences", "reserve_pages", "free_sequences", "compact_pages", "append_kv", "sample",
+         "shared_prefix_attention"}
 
 
 def add(n: int) -> None:
@@ -78,9 +75,17 @@ class CountingProxy:
     def __getattr__(self, name):
         attr = getattr(self._t, name)
         per = KERNELS_PER_CALL.get(name)
-        if per is None or not callable(attr):
+        if (per is None and name not in ASKED) or not callable(attr):
             return attr
-        if name == "gemm":
+        if name in ASKED:
+            launched = self._t.generation_launches
+
+            def call(*args, **kwargs):
+                global _count
+                out = attr(*args, **kwargs)
+                _count += launched()
+                return out
+        elif name == "gemm":
             def call(*args, **kwargs):
                 global _count
                 out = attr(*args, **kwargs)

@@ -470,3 +470,46 @@ def test_sample_from_several_threads():
     with ThreadPoolExecutor(4) as pool:
         assert all(pool.map(work, [300, 50304, 9001, 130003, 20000, 40000]))
     settle("cuda")
+
+
+# ---- counted launches --------------------------------------------------------------------
+
+
+def test_launch_counts_follow_what_the_extension_says():
+    from types import SimpleNamespace
+
+    from mini_nccl_b200.utils import launches
+
+    last = []
+    target = SimpleNamespace(sample=lambda n: last.append(n) or n, gelu_fwd=lambda: None, generation_launches=lambda: last[-1])
+    proxy = launches.CountingProxy(target)
+    before = launches.count()
+    assert proxy.sample(3) == 3 and proxy.sample(0) == 0 and proxy.gelu_fwd() is None
+    assert launches.count() - before == 4
+
+
+@pytest.mark.gpu
+def test_launch_counts_of_the_forms_of_a_call():
+    from mini_nccl_b200.utils import launches
+
+    def kernels(call):
+        before = launches.count()
+        call()
+        return launches.count() - before
+
+    def attention(rows, prefix, lens=5, dim=64, **more):
+        p = Problem([lens] * rows, [1] * rows, kv_heads=2, group=1, dim=dim, page=16, prefix=prefix, device="cuda")
+        return kernels(lambda: p.run(**more))
+
+    assert attention(3, 40) == 2  # pieces, join
+    assert attention(60, 40) == 2  # own pieces, and the prefix on tensor cores, which joins them
+    assert attention(60, 9000) == 3  # the prefix in several pieces
+    assert attention(60, 40, lens=0, max_seq_len=0) == 2  # the check of the lengths, and the prefix
+    assert attention(3, 0, lens=0, max_seq_len=0) == 2  # the check, and the join that writes zeros
+    b = Books("cuda", [9, 20], slots=4, columns=4, pages=40)
+    assert kernels(lambda: b.fork([0], [2])) == 2 and kernels(lambda: b.fork([], [])) == 0
+    assert kernels(lambda: G.compact_pages(b.kv, b.table, b.refs)) == 2
+    assert kernels(lambda: G.compact_pages(b.kv, b.table.repeat(1100, 1), b.refs)) == 3
+    assert kernels(lambda: G.copy_pages(b.kv, ints([], "cuda"), ints([], "cuda"))) == 0
+    x = torch.zeros(2, 9, device="cuda")
+    assert kernels(lambda: G.sample(x, x)) == 1 and kernels(lambda: G.sample(x[:0], x[:0])) == 0
