@@ -40,6 +40,7 @@ void flash_attn_bwd_tc(torch::Tensor qkv, torch::Tensor o, torch::Tensor dout, t
 void exp2_poly_eval(torch::Tensor x, torch::Tensor y);
 // generation.cpp
 int64_t generation_launches();
+void prefix_exp2_eval(const torch::Tensor& x, const torch::Tensor& y);
 void copy_pages(const torch::Tensor& kv, const torch::Tensor& src, const torch::Tensor& dst, const torch::Tensor& status);
 void fork_sequences(const torch::Tensor& kv, const torch::Tensor& page_table, const torch::Tensor& lens, const torch::Tensor& refs,
                     const torch::Tensor& parents, const torch::Tensor& children, const torch::Tensor& status);
@@ -85,6 +86,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("flash_attn_bwd_tc", &mnb::flash_attn_bwd_tc, "tcgen05 flash attention backward");
   m.def("exp2_poly_eval", &mnb::exp2_poly_eval, "the attention softmax's FMA-pipe exp2, over a tensor");
   m.def("generation_launches", &mnb::generation_launches, "kernels that this thread's last call of the operators below launched");
+  m.def("prefix_exp2_eval", &mnb::prefix_exp2_eval, "the shared-prefix attention's FMA-pipe exp2, over a tensor");
   m.def("copy_pages", &mnb::copy_pages);
   m.def("fork_sequences", &mnb::fork_sequences);
   m.def("reserve_pages", &mnb::reserve_pages);

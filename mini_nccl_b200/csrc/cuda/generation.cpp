@@ -89,6 +89,16 @@ S setting(const c10::optional<torch::Tensor>& each, double all, int64_t rows, at
 
 int64_t generation_launches() { return launched; }
 
+void prefix_exp2_eval(const torch::Tensor& x, const torch::Tensor& y) {
+  TORCH_CHECK_VALUE(x.is_cuda() && x.scalar_type() == at::kFloat && x.is_contiguous() && x.numel() % 2 == 0 &&
+                        x.numel() < (1ll << 31) && y.device() == x.device() && y.sizes() == x.sizes() &&
+                        y.scalar_type() == at::kFloat && y.is_contiguous(),
+                    "prefix_exp2_eval: contiguous fp32 CUDA tensors of one shape, an even number of entries");
+  const c10::cuda::CUDAGuard guard(x.device());
+  C10_CUDA_CHECK(prefix::launch_exp2(x.data_ptr<float>(), y.data_ptr<float>(), static_cast<int>(x.numel() / 2),
+                                     at::cuda::getCurrentCUDAStream()));
+}
+
 void copy_pages(const torch::Tensor& kv, const torch::Tensor& src, const torch::Tensor& dst, const torch::Tensor& status) {
   launched = 0;
   const auto p = pool_of(kv);

@@ -132,6 +132,8 @@ __device__ __forceinline__ int own_pieces(const Args& a) {
 int plan(Args& a, int head_dim);
 // head dims 64 and 128; with one prefix piece, joins the rows and finishes them
 cudaError_t launch_prefix_tc(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, int head_dim, cudaStream_t stream);
+// the tensor-core kernel's own 2^x, on 2 * pairs numbers
+cudaError_t launch_exp2(const float* x, float* y, int pairs, cudaStream_t stream);
 cudaError_t launch_attention(const Args& a, int head_dim, cudaStream_t stream);
 int kernels(const Args& a);  // that launch_attention() launches
 

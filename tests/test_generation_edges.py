@@ -513,3 +513,49 @@ def test_launch_counts_of_the_forms_of_a_call():
     assert kernels(lambda: G.copy_pages(b.kv, ints([], "cuda"), ints([], "cuda"))) == 0
     x = torch.zeros(2, 9, device="cuda")
     assert kernels(lambda: G.sample(x, x)) == 1 and kernels(lambda: G.sample(x[:0], x[:0])) == 0
+
+
+# ---- forms that few calls reach ----------------------------------------------------------
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lens,new,kv_heads,group,dim,page,prefix", [
+    # more sequences than a block keeps the lengths of
+    ([i % 23 for i in range(1100)], [1] * 1100, 1, 1, 64, 8, 40),
+    ([i % 9 for i in range(1030)], [i % 3 for i in range(1030)], 2, 1, 32, 8, 0),
+    # four kv heads to a piece at head dim 32, the last of them fewer
+    ([(3 * i) % 31 for i in range(300)], [1] * 300, 7, 1, 32, 8, 0),
+    ([(3 * i) % 31 for i in range(300)], [1] * 300, 4, 4, 32, 64, 0),
+])
+def test_attention_many_sequences(device, lens, new, kv_heads, group, dim, page, prefix):
+    p = Problem(lens, new, kv_heads=kv_heads, group=group, dim=dim, page=page, prefix=prefix, device=device)
+    p.check(*p.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,new,kv_heads,group,dim,prefix", [
+    ([17, 300, 5, 90], [1] * 4, 12, 1, 64, 300),
+    ([(11 * i) % 400 for i in range(96)], [1] * 96, 8, 1, 128, 3000),
+    ([(11 * i) % 700 for i in range(16)], [1] * 16, 8, 4, 128, 9000),
+    ([200, 77, 300, 150], [200, 60, 150, 1], 4, 2, 128, 1500),
+    ([4] * 200, [1] * 200, 8, 1, 64, 64),
+])
+def test_attention_repeats_itself_to_the_bit(lens, new, kv_heads, group, dim, prefix):
+    p = Problem(lens, new, kv_heads=kv_heads, group=group, dim=dim, page=16, prefix=prefix, device="cuda")
+    o, lse = p.run()
+    for _ in range(10):
+        again, lse_again = p.run()
+        assert torch.equal(again, o) and torch.equal(lse_again, lse)
+
+
+@pytest.mark.gpu
+def test_attention_exponential_on_the_fma_pipe():
+    """The polynomial is off by 1.1e-7 at most; its last rounding adds 2^-24 and the earlier ones together less than 2^-25."""
+    from mini_nccl_b200.ops import kernels as K
+
+    x = torch.cat([torch.linspace(-126, 20, 1 << 20), torch.arange(-126.0, 20), torch.tensor([-126.5, -1e30, -math.inf, -0.0])]).cuda()
+    y = torch.empty_like(x)
+    K.ext().prefix_exp2_eval(x, y)
+    want = torch.exp2(x.double().clamp(min=-126))
+    assert float(((y.double() - want).abs() / want).max()) <= 1.1e-7 + 2.0 ** -24 + 2.0 ** -25
+    whole = y[1 << 20: -4]
+    assert torch.equal(whole, torch.exp2(torch.arange(-126.0, 20).double()).float().cuda()), "exact at whole numbers"
