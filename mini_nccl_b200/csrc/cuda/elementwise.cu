@@ -1225,6 +1225,8 @@ void embed_fwd(torch::Tensor idx, torch::Tensor wte, torch::Tensor wpe, torch::T
   check_bf16(wpe, "wpe");
   TORCH_CHECK(idx.scalar_type() == at::kLong && idx.is_contiguous(), "idx must be int64");
   TORCH_CHECK(status.is_cuda() && status.scalar_type() == at::kInt && status.numel() >= 3, "status: int32 on the device");
+  TORCH_CHECK(wpe.size(0) >= idx.size(-1) && wpe.size(1) == wte.size(1), "wpe: a row of ", wte.size(1), " for each of the ",
+              idx.size(-1), " positions, got ", wpe.sizes());
   const int T = static_cast<int>(idx.size(-1));
   const int C = static_cast<int>(wte.size(1));
   const int tokens = static_cast<int>(idx.numel());
@@ -1238,6 +1240,7 @@ void embed_fwd(torch::Tensor idx, torch::Tensor wte, torch::Tensor wpe, torch::T
 
 void embed_bwd(torch::Tensor idx, torch::Tensor dy, torch::Tensor dwte, torch::Tensor dwpe, bool accumulate_pos) {
   check_bf16(dy, "dy");
+  TORCH_CHECK(idx.scalar_type() == at::kLong && idx.is_contiguous(), "idx must be int64");
   const int B = static_cast<int>(idx.size(0));
   const int T = static_cast<int>(idx.size(1));
   const int C = static_cast<int>(dwte.size(1));

@@ -485,7 +485,8 @@ class Embedding(torch.autograd.Function):
     def forward(ctx, idx, wte, wpe):
         B, T = idx.shape
         y = torch.empty((B, T, wte.shape[1]), dtype=wte.dtype, device=wte.device)
-        ext().embed_fwd(idx.contiguous(), wte, wpe, y, status_word(wte.device))
+        idx = idx.contiguous()
+        ext().embed_fwd(idx, wte, wpe, y, status_word(wte.device))
         ctx.save_for_backward(idx)
         ctx.shapes = (wte.shape, wpe.shape)
         return y

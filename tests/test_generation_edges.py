@@ -559,3 +559,23 @@ def test_attention_exponential_on_the_fma_pipe():
     assert float(((y.double() - want).abs() / want).max()) <= 1.1e-7 + 2.0 ** -24 + 2.0 ** -25
     whole = y[1 << 20: -4]
     assert torch.equal(whole, torch.exp2(torch.arange(-126.0, 20).double()).float().cuda()), "exact at whole numbers"
+
+
+# ---- the embedding's other arguments -----------------------------------------------------
+
+
+@pytest.mark.gpu
+def test_embedding_of_strided_ids_and_of_too_many_positions():
+    from mini_nccl_b200.ops import kernels as K
+
+    wte = torch.randn(40, 24, device="cuda").to(torch.bfloat16).requires_grad_()
+    wpe = torch.randn(6, 24, device="cuda").to(torch.bfloat16).requires_grad_()
+    flat = torch.arange(12, device="cuda")
+    for idx in (flat.view(4, 3).t(), flat[:4].expand(3, 4), flat.view(3, 4)[:, ::2]):
+        wte.grad = None
+        K.Embedding.apply(idx, wte, wpe).sum().backward()
+        count = torch.bincount(idx.reshape(-1), minlength=40)
+        assert torch.equal(wte.grad.float(), count[:, None].float().expand(40, 24))
+    with pytest.raises(RuntimeError, match="positions"):
+        K.Embedding.apply(flat.view(1, 12), wte, wpe)
+    settle("cuda")
