@@ -107,11 +107,11 @@ class BranchedGeneration:
             raise ValueError(f"the branches hold {self.max_new_tokens} tokens already")
         c, P = self.cache, self.prompt_len
         ids = self._ids(self.branches)
+        x = _embed(self.model, tokens[:, None], P + self.length)[:, 0]  # (first: it refuses tokens that are none)
         c.extend(self.branches, [1] * n, ids, torch.ones_like(ids))
         place = torch.full_like(ids, self.length)
         table, lens = c.page_table[ids.long()], c.lens[ids.long()]
         prefix = c.page_table[0, : -(-P // c.page_size)]
-        x = _embed(self.model, tokens[:, None], P + self.length)[:, 0]
         self.length += 1
         for layer, block in enumerate(self._blocks):
             h = F.layer_norm(x, block.ln1.weight, block.ln1.bias, block.ln1.eps)

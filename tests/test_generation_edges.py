@@ -579,3 +579,25 @@ def test_embedding_of_strided_ids_and_of_too_many_positions():
     with pytest.raises(RuntimeError, match="positions"):
         K.Embedding.apply(flat.view(1, 12), wte, wpe)
     settle("cuda")
+
+
+# ---- after an error ----------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_step_that_was_refused_changes_nothing(device):
+    from mini_nccl_b200.models.generation import BranchedGeneration
+    from mini_nccl_b200.models.gpt import GPT
+
+    torch.manual_seed(0)
+    m = GPT(96, 64, 2, 2, 64)
+    m = m.to(device, torch.bfloat16) if device == "cuda" else m
+    prompt, good = torch.arange(20, device=device), torch.tensor([5], device=device)
+    # a dtype that the embedding does not take, and (seen on the CPU only) a token that is none
+    for bad in [good.float()] + ([good + 1000] if device == "cpu" else []):
+        states = [BranchedGeneration(m, prompt, max_branches=1, max_new_tokens=4) for _ in range(2)]
+        with pytest.raises((RuntimeError, IndexError)):
+            states[0].step(bad)
+        assert states[0].length == 0 and states[0].cache.lengths == [20, 0] and states[0].cache.lens.tolist() == [20, 0]
+        assert torch.equal(states[0].step(good), states[1].step(good))
+    settle(device)
