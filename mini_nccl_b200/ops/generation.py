@@ -242,6 +242,8 @@ def sample(
             return x[:, None]
         return torch.full((R, 1), x, dtype=dtype)
 
+    if not isinstance(top_k, torch.Tensor):
+        top_k = min(max(int(top_k), 0), V)
     T, k = column(temperature, torch.float32, "temperature"), column(top_k, torch.int32, "top_k")
     p, least = column(top_p, torch.float32, "top_p"), column(min_p, torch.float32, "min_p").clamp(max=1)
     x = logits.float()

@@ -601,3 +601,14 @@ def test_a_step_that_was_refused_changes_nothing(device):
         assert states[0].length == 0 and states[0].cache.lengths == [20, 0] and states[0].cache.lens.tolist() == [20, 0]
         assert torch.equal(states[0].step(good), states[1].step(good))
     settle(device)
+
+
+# ---- sizes at the ends of their types ----------------------------------------------------
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_sample_top_k_beyond_32_bits_keeps_all(device):
+    x, noise = (t.to(device) for t in logits_of(2, 300, torch.float32, seed=1))
+    want = G.sample(x, noise)
+    for k in (1 << 40, (1 << 31) - 1, 300, 0, -1, -(1 << 40)):
+        assert torch.equal(G.sample(x, noise, top_k=k), want)
