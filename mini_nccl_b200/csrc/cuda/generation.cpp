@@ -18,7 +18,7 @@ thread_local int64_t launched = 0;  // kernels of the last call
 
 void check_int32(const torch::Tensor& t, int64_t dim, const torch::Tensor& like, const char* what) {
   TORCH_CHECK_VALUE(t.is_cuda() && t.device() == like.device() && t.scalar_type() == at::kInt && t.dim() == dim &&
-                        (t.numel() == 0 || t.stride(dim - 1) == 1),
+                        (t.numel() == 0 || t.size(dim - 1) == 1 || t.stride(dim - 1) == 1),
                     what, ": a ", dim, "-d int32 tensor on ", like.device(), " with its last axis contiguous");
   TORCH_CHECK_VALUE(t.numel() < (1ll << 31), what, ": too many entries");
 }

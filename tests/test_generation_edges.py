@@ -612,3 +612,15 @@ def test_sample_top_k_beyond_32_bits_keeps_all(device):
     want = G.sample(x, noise)
     for k in (1 << 40, (1 << 31) - 1, 300, 0, -1, -(1 << 40)):
         assert torch.equal(G.sample(x, noise, top_k=k), want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_single_entries_of_strided_tensors(device):
+    """An axis of one entry has any stride: a column of a wider table, an entry of a wider list."""
+    p = Problem([7], [1], kv_heads=2, group=1, dim=64, page=8, prefix=5, device=device)
+    want, _ = p.run()
+    table = ints([[p.rows[0][0], 9, 9]] * 2, device)
+    lens, prefix = ints([7, 0, 3, 0], device), ints([p.prefix_pages[0], 4, 4], device)
+    got = G.shared_prefix_attention(p.q, p.pool[0], p.pool[1], prefix[::3], 5, table[:1, ::3], lens[::4])
+    assert torch.equal(got, want)
+    settle(device)
