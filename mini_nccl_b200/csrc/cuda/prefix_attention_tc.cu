@@ -22,7 +22,7 @@
 //
 // Measured: 16 sequences of 4 grouped heads (64 rows) over 65,537 keys of 8 kv
 // heads, 268 MB: 48 us, 5.6 TB/s, bound by the bytes.  2388 rows of 32 heads
-// over 4001 keys, 157 GFLOP: 187 us, 0.84 PFLOP/s (0.51 of the measured bf16
+// over 4001 keys, 157 GFLOP: about 185 us, 0.85 PFLOP/s (0.52 of the measured bf16
 // peak).  A step of both streams (256 rows, 128 keys) takes some 3300 cycles,
 // of which the products take 2048 and the exponentials as long on their unit;
 // what is left is the chain S -> maximum -> P -> O -> next S of each stream,

@@ -23,7 +23,8 @@
 //     above the band, scores it, and lists the band; the sorted list gives the
 //     exact cut.  A band with too many tokens is counted again in finer bins.
 //   - what is left (thousands of equal logits at the cut, infinite logits) is
-//     found by bisection over the pairs, slowly.
+//     found by bisection over the pairs, slowly: 1 x 50304 bf16 around 20 with
+//     a spread of 1, top-p 0.9, 167 us where the same around 0 takes 22.
 // Measured (GPU time): 1 x 50304 bf16, top-k 50: 11 us; 64 x 50304 fp32 with
 // mixed settings 26 us; 512 x 50304 bf16, top-p 0.9 to 0.95: 80 us (52 MB of
 // logits and about as much noise); 129 x 130003 fp32, min-p: 43 us (67 MB).

@@ -450,7 +450,8 @@ def free_sequences(page_table: torch.Tensor, lens: torch.Tensor, refs: torch.Ten
     """Empty the sequences ``slots``: each of their pages loses one holder.
 
     A page without holders is free (``refs`` 0).  Naming a slot twice frees it
-    once.
+    once.  On the device a row is emptied also where it names a page that is
+    none, or that nobody holds: that entry is dropped and reported.
     """
     if page_table.is_cuda:
         K = _kernels()
