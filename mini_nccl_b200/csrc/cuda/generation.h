@@ -122,10 +122,9 @@ struct Args {
 };
 
 #ifdef __CUDACC__
-// Partial results of a row's own keys that a kernel may read, behind those that write them.
-__device__ __forceinline__ int own_pieces(const Args& a) {
-  return a.sound && *const_cast<volatile int*>(a.sound) == 0 ? 0 : a.own_splits;
-}
+// Whether the partial results of own keys count, for a kernel behind those that write them.  (The word comes by way of L1:
+// fetched from L2 by every warp of the join, it made 16 x 512 tokens of 16 heads of 64 7 % slower.)
+__device__ __forceinline__ bool own_count(const Args& a) { return !a.sound || *a.sound != 0; }
 #endif
 
 // Splits the keys into pieces; returns how many partial results each row gets.

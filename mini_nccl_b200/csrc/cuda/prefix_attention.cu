@@ -74,16 +74,16 @@ constexpr int kUnlimited = 1 << 30;
 
 MNB_DEVICE void flag(const Args& a) { atomicCAS(a.errors, 0, kErrBadIndex); }
 
-// Whether q_offsets ascend from 0 to n in steps of at most max_q; for all threads of a block.
+// Whether q_offsets ascend from 0 to n in steps of at most max_q; for all lanes of a warp.
 MNB_DEVICE bool offsets_sound(const Args& a, const int* q_offsets) {
   bool bad = false;
-  for (int b = threadIdx.x; b <= a.batch; b += blockDim.x) {
+  for (int b = threadIdx.x % 32; b <= a.batch; b += 32) {
     const long long from = q_offsets[b];
     if (b == 0) bad = bad || from != 0;
     if (b == a.batch) bad = bad || from != a.n;
     else bad = bad || q_offsets[b + 1] < from || q_offsets[b + 1] - from > a.max_q;
   }
-  return !__syncthreads_or(bad);
+  return !__any_sync(0xffffffffu, bad);
 }
 
 // Item i of the list: first the prefix's (split, kv head, row tile; the row tiles of the same keys side by side), then
@@ -135,39 +135,42 @@ MNB_DEVICE Piece piece_of(const Args& a, const int* seq_lens, const int* q_offse
   return p;
 }
 
-// The outputs of a warp's 16 rows from row0 on once more, key by key: keys first to first + width - 1 of every `step`.  A
-// product over a tile gives a hidden key weight 0, and 0 times a value that is no number is NaN; here each row takes
-// only what it sees.  `m0` and `m1` are the maxima of this lane's rows (lane / 4, and 8 more); the rows are those of
-// `rows` in shared memory, `pitch` apart, or without it their places among the partial results.
+// The rows of a block's pieces that are not finite, computed again key by key.  A product over a tile gives a hidden key
+// weight 0, and 0 times a value that is no number is NaN; here each row takes only what it sees.  (A row that sees such a
+// value comes out as it was.)  Maxima and sums are right already.
 template <int D>
-__device__ __noinline__ void rows_key_by_key(const Args& a, Piece p, int head, int row0, int first, int width, int step, float m0,
-                                             float m1, float* rows, int pitch) {
+__device__ __noinline__ void rows_again(const Args& a, const int* seq_lens, const int* q_offsets, int items, int tile_rows, int heads) {
   constexpr int kPer = D / 32;
-  const int lane = threadIdx.x % 32;
-  __syncwarp();
-  for (int x = 0; x < 16; ++x) {
-    const int r = row0 + x;
-    if (r >= p.n_rows) break;
-    const float m = __shfl_sync(0xffffffffu, x < 8 ? m0 : m1, x % 8 * 4), base = m == -INFINITY ? 0.f : m;
-    const int j = p.r0 + r, token = j / a.group, limit = min(p.k1, p.limit0 + token), in_group = j - token * a.group;
-    const __nv_bfloat16* q = a.q + (p.n0 + token) * a.q_ld + (head * a.group + in_group) * a.q_head + lane * kPer;
-    float o[kPer] = {};
-    for (int t0 = p.k0 + first; t0 < limit; t0 += step)
-      for (int key = t0; key < min(t0 + width, limit); ++key) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  for (int i = blockIdx.x; i < items; i += gridDim.x) {
+    const Piece p = piece_of(a, seq_lens, q_offsets, i, tile_rows, heads);
+    if (p.limit0 + p.r0 / a.group >= p.k1) continue;  // every row sees every key
+    for (int x = warp; x < p.n_rows * heads; x += kWorkers / 32) {
+      const int r = x / heads, head = p.h + x % heads, j = p.r0 + r, token = j / a.group, in_group = j - token * a.group;
+      if (head >= a.kv_heads) continue;
+      const long long out = (static_cast<long long>(p.slot) * a.n + p.n0 + token) * a.heads + head * a.group + in_group;
+      float* to = a.part_o + out * D + lane * kPer;
+      float zero = 0.f;
+#pragma unroll
+      for (int c = 0; c < kPer; ++c) zero = fmaf(to[c], 0.f, zero);
+      if (!__any_sync(0xffffffffu, zero != 0.f)) continue;
+      const float m = a.part_ml[out].x, base = m == -INFINITY ? 0.f : m;
+      const __nv_bfloat16* q = a.q + (p.n0 + token) * a.q_ld + (head * a.group + in_group) * a.q_head + lane * kPer;
+      float o[kPer] = {};
+      for (int key = p.k0; key < min(p.k1, p.limit0 + token); ++key) {
         const int page = p.ids[key >> a.page_shift];
         if (page < 0 || page >= a.pages) continue;  // reads as zeros
         const long long at = page * a.page_ld + (key & ((1 << a.page_shift) - 1)) * a.token_ld + head * a.head_ld + lane * kPer;
         float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) s = fmaf(bf16_to_f32(q[i]), bf16_to_f32(a.k[at + i]), s);
+        for (int c = 0; c < kPer; ++c) s = fmaf(bf16_to_f32(q[c]), bf16_to_f32(a.k[at + c]), s);
         const float w = ex2_approx(warp_sum(s) * a.scale_log2 - base);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) o[i] = fmaf(w, bf16_to_f32(a.v[at + i]), o[i]);
+        for (int c = 0; c < kPer; ++c) o[c] = fmaf(w, bf16_to_f32(a.v[at + c]), o[c]);
       }
-    const long long out = (static_cast<long long>(p.slot) * a.n + p.n0 + token) * a.heads + head * a.group + in_group;
-    float* to = rows ? rows + r * pitch : a.part_o + out * D;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) to[lane * kPer + i] = o[i];
+      for (int c = 0; c < kPer; ++c) to[c] = o[c];
+    }
   }
 }
 
@@ -185,8 +188,7 @@ __device__ __noinline__ void rows_key_by_key(const Args& a, Piece p, int head, i
 // are short (2048 sequences of 4 tokens, 16 heads, behind a prefix of 64: the
 // call 261 us without, 86 with).
 //
-// Chunk: sequences may have several new tokens, and rows not see all the keys of their piece.  (Its own kernel because the
-// registers for rows_key_by_key cost single tokens 1 %.)
+// Chunk: sequences may have several new tokens, and rows not see all the keys of their piece.
 template <int D, int WR, bool Quad, bool Chunk>
 __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
     pieces_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap map_k,
@@ -201,9 +203,11 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t bars[2 * kStages];
+  __shared__ int again;  // some row has to be computed again
   const uint32_t ring = smem_u32(sm), full0 = smem_u32(bars), empty0 = full0 + 8 * kStages;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
+    again = 0;
     for (int s = 0; s < kStages; ++s) {
       mbar_init(full0 + 8 * s, 1);
       mbar_init(empty0 + 8 * s, 4);
@@ -221,18 +225,12 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
   __syncthreads();
   int pos = 0;  // stages filled, or used, so far
   let_next_start();
-  if (a.sound && blockIdx.x == 0) {
-    const bool sound = offsets_sound(a, q_offsets);
-    if (threadIdx.x == 0) {
-      *a.sound = sound;
-      if (!sound) flag(a);
-    }
-  }
 
   if (warp == 4) {
     const int per = min(1 << a.page_shift, kStep);  // tokens of a box
     const int box = lane / kHeads, head = lane % kHeads;
-    for (int i = blockIdx.x; i < items; i += gridDim.x) {
+    bool ok = true;
+    for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
       const Piece p = piece_of(a, seq_lens, q_offsets, i, 16 * WR, kHeads);
       const int heads = min(kHeads, a.kv_heads - p.h);
       for (int j0 = p.k0; j0 < p.k1; j0 += kStep, ++pos) {
@@ -247,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
             page = a.no_page;
           }
         }
-        if (!mbar_wait(empty0 + 8 * st, ((pos / kStages) & 1) ^ 1, a.status)) return;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * st, ((pos / kStages) & 1) ^ 1, a.status)))) break;
         if (lane == 0) mbar_arrive_expect_tx(full0 + 8 * st, boxes * per * heads * D * 4);
         __syncwarp();
         if (mine) {
@@ -259,6 +257,13 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
             tma_load_4d(to + R::tile + c * (kKeys * 128), &map_v, c * 64, p.h + head, token, page, full0 + 8 * st);
           }
         }
+      }
+    }
+    if (a.sound && blockIdx.x == 0) {  // (here because nobody waits for this warp any more)
+      const bool sound = offsets_sound(a, q_offsets);
+      if (lane == 0) {
+        *a.sound = sound;
+        if (!sound) flag(a);
       }
     }
     return;
@@ -394,17 +399,16 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
       l_r[e] += __shfl_xor_sync(0xffffffffu, l_r[e], 1);
       l_r[e] += __shfl_xor_sync(0xffffffffu, l_r[e], 2);
     }
-    // Whether some row does not see all the keys here, and the warp's outputs hold something that is no number.
-    bool again = false;
-    if (Chunk && p.limit0 + p.r0 / a.group < p.k1 && !idle) {
-      float zero = 0.f;
+    // A row that does not see all the keys here and holds something that is no number is computed again.
+    if (Chunk && __any_sync(0xffffffffu, min(lim[0], lim[1]) < p.k1) && !idle) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         if (e == 1 && !lower) break;
+        float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int d = 0; d < D / 8; ++d) zero = fmaf(acc[d][2 * e], 0.f, fmaf(acc[d][2 * e + 1], 0.f, zero));
+        for (int d = 0; d < D / 8; ++d) sum = add2(sum, make_float2(acc[d][2 * e], acc[d][2 * e + 1]));
+        if (lim[e] < p.k1 && !(fabsf(sum.x + sum.y) < INFINITY)) again = 1;
       }
-      again = __any_sync(0xffffffffu, zero != 0.f);
     }
     if constexpr (WK > 1) {
       // the key groups of a row join through shared memory
@@ -419,7 +423,6 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
         for (int d = 0; d < D / 8; ++d)
           *reinterpret_cast<float2*>(so + (wk * join_rows + r) * kPitch + d * 8 + 2 * tg) = make_float2(acc[d][2 * e], acc[d][2 * e + 1]);
       }
-      if (again) rows_key_by_key<D>(a, p, head, wr * 16, wk * KW, KW, kStep, m_r[0], m_r[1], so + wk * join_rows * kPitch, kPitch);
       workers_sync();
       for (int x = threadIdx.x; x < p.n_rows * (D / 4); x += kWorkers) {
         const int r = x / (D / 4), c = x % (D / 4) * 4;
@@ -453,14 +456,17 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
           *reinterpret_cast<float2*>(a.part_o + out * D + d * 8 + 2 * tg) = make_float2(acc[d][2 * e], acc[d][2 * e + 1]);
         if (tg == 0) a.part_ml[out] = make_float2(m_r[e], l_r[e]);
       }
-      if (again) rows_key_by_key<D>(a, p, head, wr * 16, 0, kStep, kStep, m_r[0], m_r[1], nullptr, 0);
     }
+  }
+  if constexpr (Chunk) {
+    workers_sync();
+    if (again) rows_again<D>(a, seq_lens, q_offsets, items, 16 * WR, kHeads);
   }
 }
 
 // A call without pieces of own keys (a bound of 0 for the lengths): reports what the other kernels do not look at.
 __global__ void __launch_bounds__(256) check_kernel(const __grid_constant__ Args a) {
-  bool bad = a.q_offsets && !offsets_sound(a, a.q_offsets);
+  bool bad = a.q_offsets && threadIdx.x < 32 && !offsets_sound(a, a.q_offsets);
   for (int b = threadIdx.x; b < a.batch; b += blockDim.x) bad = bad || a.seq_lens[b] != 0;
   if (bad) flag(a);
 }
@@ -468,7 +474,8 @@ __global__ void __launch_bounds__(256) check_kernel(const __grid_constant__ Args
 // Joins the pieces of each (token, head).  With many pieces a block takes a row and its warps the pieces in turn, because
 // one warp would wait for one piece after another (512 rows of 20 pieces: 6 us, 9 with a warp each); with few a warp takes
 // a row (76,000 rows of one piece: 57 us less than with a block each).
-template <int D, bool Together>
+// Checked: the call has offsets, which may not hold.
+template <int D, bool Together, bool Checked>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args a) {
   constexpr int kPer = D / 32, kStep = Together ? 4 : 1;
   __shared__ float so[4][D];
@@ -477,15 +484,22 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args 
   const long long row = Together ? blockIdx.x : blockIdx.x * 4ll + warp, rows = static_cast<long long>(a.n) * a.heads;
   wait_for_previous();
   if (row >= rows) return;
-  const int pieces = a.prefix_splits + own_pieces(a);
+  // Own pieces that do not count are read as empty, so that their loads do not wait for the word on them (16 x 512 tokens of
+  // 16 heads of 64: 97.7 us for the call if they do, 88.8 so).
+  const int pieces = a.prefix_splits + a.own_splits;
+  const bool own = !Checked || own_count(a);
+  auto part = [&](int p) {
+    const float2 ml = a.part_ml[p * rows + row];
+    return !Checked || p < a.prefix_splits || own ? ml : make_float2(-INFINITY, 0.f);
+  };
   float m = -INFINITY;
-  for (int p = lane; p < pieces; p += 32) m = fmaxf(m, a.part_ml[p * rows + row].x);
+  for (int p = lane; p < pieces; p += 32) m = fmaxf(m, part(p).x);
   m = warp_max(m);
   const float base = m == -INFINITY ? 0.f : m;
   float l = 0.f, o[kPer] = {};
 #pragma unroll 4
   for (int p = Together ? warp : 0; p < pieces; p += kStep) {
-    const float2 ml = a.part_ml[p * rows + row];
+    const float2 ml = part(p);
     const float f = ex2_approx(ml.x - base);
     l = fmaf(f, ml.y, l);
     const float* po = a.part_o + (p * rows + row) * D + lane * kPer;
@@ -594,8 +608,9 @@ static cudaError_t launch_for(const Args& a, cudaStream_t stream) {
     if (e != cudaSuccess || !joins(a)) return e;
   }
   const int rows = a.n * a.heads;
-  if (a.prefix_splits + a.own_splits > 4) return launch_after(join_kernel<D, true>, rows, 128, 0, stream, a);
-  return launch_after(join_kernel<D, false>, ceil_div(rows, 4), 128, 0, stream, a);
+  if (a.prefix_splits + a.own_splits > 4)
+    return launch_after(a.sound ? join_kernel<D, true, true> : join_kernel<D, true, false>, rows, 128, 0, stream, a);
+  return launch_after(a.sound ? join_kernel<D, false, true> : join_kernel<D, false, false>, ceil_div(rows, 4), 128, 0, stream, a);
 }
 
 // Splits of the tensor-core kernel: whole waves of one block per SM, each taking its tiles and a fixed part, and the

@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     using Part = typename Vec<kPer>::type;
     const long long rows = static_cast<long long>(a.n) * a.heads;
     wait_for_previous();  // the own keys' pieces
-    const int own = own_pieces(a);
+    const int own = own_count(a) ? a.own_splits : 0;
     const bool alone = a.prefix_splits == 1;  // then this block joins the rows with their own keys' pieces and finishes them
     if (const int i = s * kTile + r; i < n_rows && half == 0) {  // (without `shared`, the first stream's threads)
       const int j = r0 + i, token = j / a.group;

@@ -26,7 +26,7 @@
 //     found by bisection over the pairs, slowly: 1 x 50304 bf16 around 20 with
 //     a spread of 1, top-p 0.9, 167 us where the same around 0 takes 22.
 // Measured (GPU time): 1 x 50304 bf16, top-k 50: 11 us; 64 x 50304 fp32 with
-// mixed settings 26 us; 512 x 50304 bf16, top-p 0.9 to 0.95: 80 us (52 MB of
+// mixed settings 27 us; 512 x 50304 bf16, top-p 0.9 to 0.95: 80 us (52 MB of
 // logits and about as much noise); 129 x 130003 fp32, min-p: 43 us (67 MB).
 // None is bound by its bytes: a row is a chain of passes, and the instructions
 // of the passes (12 an element to count, 13 to split, 11 to score) fill the
