@@ -259,6 +259,8 @@ __global__ void __launch_bounds__(kThreads, WR == 4 ? 2 : 3)
         }
       }
     }
+    // The block does not end before its last copies have arrived, also where a worker's wait was given up.
+    for (int k = max(0, pos - kStages); k < pos; ++k) mbar_wait(full0 + 8 * (k % kStages), (k / kStages) & 1, nullptr);
     if (a.sound && blockIdx.x == 0) {  // (here because nobody waits for this warp any more)
       const bool sound = offsets_sound(a, q_offsets);
       if (lane == 0) {

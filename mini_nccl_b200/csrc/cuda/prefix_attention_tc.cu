@@ -58,7 +58,7 @@ struct Smem {
   static constexpr int stages = D == 128 ? 5 : 8;
   static constexpr uint32_t q_off = 0, kv_off = 2 * q_tile;
   static constexpr uint32_t bar_off = kv_off + stages * kv_tile;
-  static constexpr int n_bars = 2 * stages + 9;
+  static constexpr int n_bars = 2 * stages + 10;
   static constexpr uint32_t max_off = bar_off + n_bars * 8 + 16;  // row maxima so far: [stream][row], as order_of()
   static constexpr uint32_t total = max_off + 2 * kTile * 4 + 1024;
   static_assert(total <= 227 * 1024, "a block's shared memory");
@@ -113,6 +113,8 @@ MNB_DEVICE int order_of(float x) {
   return i ^ ((i >> 31) & 0x7fffffff);
 }
 MNB_DEVICE float of_order(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
+// A warp's wait, given up by all of its lanes or by none.
+MNB_DEVICE bool warp_wait(uint32_t bar, uint32_t parity, int* abort) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort)); }
 MNB_DEVICE void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kSoftmax) : "memory"); }
 MNB_DEVICE void stream_sync(int s) { asm volatile("bar.sync %0, %1;" ::"r"(2 + s), "n"(kSoftmax / 2) : "memory"); }
 
@@ -138,7 +140,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + S::bar_off);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + S::n_bars);
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * kStages, q_full = empty0 + 8 * kStages,
-                 s_full0 = q_full + 8, o_full0 = s_full0 + 16, p_full0 = o_full0 + 16;  // (p_full: two halves per stream)
+                 s_full0 = q_full + 8, o_full0 = s_full0 + 16, p_full0 = o_full0 + 16,  // (p_full: two halves per stream)
+                 drained = p_full0 + 32;
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   // The first `whole` blocks take 256 rows, the others half as many: a last wave that fills less than half of the SMs
@@ -166,6 +169,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(empty0 + 8 * s, 1);
     }
     mbar_init(q_full, kSoftmax);
+    mbar_init(drained, 1);
     for (int s = 0; s < 2; ++s) {
       mbar_init(s_full0 + 8 * s, 1);
       mbar_init(p_full0 + 16 * s, 128);
@@ -191,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int pos = 0;
     auto load = [&](const CUtensorMap* map, int tile) -> bool {
       const int st = pos % kStages;
-      if (!mbar_wait(empty0 + 8 * st, ((pos / kStages) & 1) ^ 1, a.status)) return false;
+      if (!warp_wait(empty0 + 8 * st, ((pos / kStages) & 1) ^ 1, a.status)) return false;
       ++pos;
       const int j0 = k0 + tile * kTile;
       const int per = min(1 << a.page_shift, 64);  // tokens of a box
@@ -219,9 +223,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = load(&map_k, 0) && (n_tiles < 2 || load(&map_k, 1));
       for (int t = 0; t < n_tiles && ok; ++t) ok = load(&map_v, t) && (t + 2 >= n_tiles || load(&map_k, t + 2));
     }
+    // The block does not end before its last copies have arrived, also where another warp's wait was given up.
+    for (int p = max(0, pos - kStages); p < pos; ++p) mbar_wait(full0 + 8 * (p % kStages), (p / kStages) & 1, nullptr);
   } else if (warp == 1) {
     int pos = 0;
-    auto wait_full = [&](int p) { return mbar_wait(full0 + 8 * (p % kStages), (p / kStages) & 1, a.status); };
+    // Whether this lane's waits have all ended well.  The lanes agree on it once a step (`settle`): a vote at each wait made
+    // the kernel 2 % slower, and what a step computes past a wait that was given up is in bounds.
+    bool good = true;
+    auto settle = [&] { return __all_sync(0xffffffffu, good); };
+    auto wait_full = [&](int p) { good = mbar_wait(full0 + 8 * (p % kStages), (p / kStages) & 1, a.status) && good; };
     // (adding bytes / 16 to a descriptor moves its address: the tiles lie below 256 KB, so nothing carries)
     const uint64_t q_desc = smem_desc_sw128(sbase + S::q_off, 16, 1024);
     const uint64_t k_desc = smem_desc_sw128(sbase + S::kv_off, 16, 1024);
@@ -241,11 +251,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
     };
     // O_s (+)= P_s V, the first half of the keys while the second half's probabilities are still computed
-    auto values = [&](int s, int p, int step) -> bool {
+    auto values = [&](int s, int p, int step) {
       const uint64_t vb = v_desc + tile_of(p);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        if (!mbar_wait(p_full0 + 16 * s + 8 * half, step & 1, a.status)) return false;
+        good = mbar_wait(p_full0 + 16 * s + 8 * half, step & 1, a.status) && good;
         tc_fence_after();
         if (elected()) {
 #pragma unroll
@@ -255,7 +265,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
       }
-      return true;
     };
     auto done_with = [&](int p) {
       if (elected()) tc_commit(empty0 + 8 * (p % kStages));
@@ -273,28 +282,30 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_async_smem();
       __syncwarp();
     };
-    bool ok = mbar_wait(q_full, 0, a.status);
+    bool ok = warp_wait(q_full, 0, a.status);
     tc_fence_after();
     if (shared) {
-      if (ok && (ok = wait_full(pos))) {
+      if (ok) {
+        wait_full(pos);
         scores(0, pos);
         scores(1, pos);
         done_with(pos++);
+        ok = settle();
       }
       for (int t = 0; t < n_tiles && ok; ++t) {
         const int v = pos++, k = pos;
         const bool more = t + 1 < n_tiles;
         if (more) ++pos;
-        if (!(ok = wait_full(v))) break;
+        wait_full(v);
         clean(t, v);
-        if (!(ok = values(0, v, t))) break;
+        values(0, v, t);
         if (more) {
-          if (!(ok = wait_full(k))) break;
+          wait_full(k);
           scores(0, k);
         } else if (elected()) {
           tc_commit(o_full0);
         }
-        if (!(ok = values(1, v, t))) break;
+        values(1, v, t);
         done_with(v);
         if (more) {
           scores(1, k);
@@ -302,27 +313,35 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else if (elected()) {
           tc_commit(o_full0 + 8);
         }
+        ok = settle();
       }
     } else {
-      for (int s = 0; s < 2 && s < n_tiles && ok; ++s)
-        if ((ok = wait_full(pos))) {
-          scores(s, pos);
-          done_with(pos++);
-        }
+      for (int s = 0; s < 2 && s < n_tiles && ok; ++s) {
+        wait_full(pos);
+        scores(s, pos);
+        done_with(pos++);
+        ok = settle();
+      }
       for (int t = 0; t < n_tiles && ok; ++t) {
         const int s = t & 1;
-        if (!(ok = wait_full(pos))) break;
+        wait_full(pos);
         clean(t, pos);
-        if (!(ok = values(s, pos, t >> 1))) break;
+        values(s, pos, t >> 1);
         done_with(pos++);
         if (t + 2 < n_tiles) {
-          if (!(ok = wait_full(pos))) break;
+          wait_full(pos);
           scores(s, pos);
           done_with(pos++);
         } else if (elected()) {
           tc_commit(o_full0 + 8 * s);
         }
+        ok = settle();
       }
+    }
+    if (!ok) {  // a wait was given up: nor do products end after their TMEM is freed
+      if (elected()) tc_commit(drained);
+      __syncwarp();
+      mbar_wait(drained, 0, nullptr);
     }
   } else {
     const int s = (warp - 2) / 8, half = (warp - 2) / 4 % 2, quad = warp % 4;

@@ -619,7 +619,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 
   float mine = -INFINITY;
   for (int c = tid, j = 0; c < row.count; ++j) {  // a chunk holds two of a thread's pieces
-    if (Staged && !mbar_wait(smem_u32(sh.arrived + j), 0, a.status)) break;
+    // (not given up because another wait of the device has run out: a block may not end before its copies have)
+    if (Staged && !mbar_wait(smem_u32(sh.arrived + j), 0, nullptr)) {
+      atomicCAS(a.status, 0, kErrPipelineTimeout);
+      break;
+    }
 #pragma unroll
     for (int e = 0; e < kChunk / kThreads; ++e, c += kThreads)
       if (c < row.count) mine = R::widest(row.piece(c), mine);
