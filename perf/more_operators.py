@@ -19,7 +19,7 @@ own = False
 DEV = "cuda"
 
 TOP = {"int8": 127.0, "float8_e4m3fn": 448.0}  # the largest code
-LEAST = -100  # the scales' least exponent
+LEAST = -60  # the scales' least exponent
 
 
 # ---- cases -----------------------------------------------------------------------------
