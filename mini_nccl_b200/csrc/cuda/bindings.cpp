@@ -41,17 +41,24 @@ void exp2_poly_eval(torch::Tensor x, torch::Tensor y);
 // generation.cpp
 int64_t generation_launches();
 void prefix_exp2_eval(const torch::Tensor& x, const torch::Tensor& y);
-void copy_pages(const torch::Tensor& kv, const torch::Tensor& src, const torch::Tensor& dst, const torch::Tensor& status);
+using OptionalTensor = c10::optional<torch::Tensor>;
+void copy_pages(const torch::Tensor& kv, const torch::Tensor& src, const torch::Tensor& dst, const OptionalTensor& scales,
+                const torch::Tensor& status);
 void fork_sequences(const torch::Tensor& kv, const torch::Tensor& page_table, const torch::Tensor& lens, const torch::Tensor& refs,
-                    const torch::Tensor& parents, const torch::Tensor& children, const torch::Tensor& status);
+                    const torch::Tensor& parents, const torch::Tensor& children, const OptionalTensor& scales, const torch::Tensor& status);
 void reserve_pages(const torch::Tensor& page_table, const torch::Tensor& lens, const torch::Tensor& refs, const torch::Tensor& slots,
                    const torch::Tensor& counts, int64_t page_size, const torch::Tensor& status);
 void free_sequences(const torch::Tensor& page_table, const torch::Tensor& lens, const torch::Tensor& refs, const torch::Tensor& slots,
                     const torch::Tensor& status);
 std::tuple<torch::Tensor, torch::Tensor> compact_pages(const torch::Tensor& kv, const torch::Tensor& page_table, const torch::Tensor& refs,
-                                                       const torch::Tensor& status);
+                                                       const OptionalTensor& scales, const torch::Tensor& status);
 void append_kv(const torch::Tensor& k_pages, const torch::Tensor& v_pages, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& page_table,
-               const torch::Tensor& positions, const c10::optional<torch::Tensor>& slots, const torch::Tensor& status);
+               const torch::Tensor& positions, const c10::optional<torch::Tensor>& slots,
+               const OptionalTensor& k_scales, const OptionalTensor& v_scales, const torch::Tensor& status);
+void adjust_logits(const torch::Tensor& in, const torch::Tensor& out, const OptionalTensor& prompt, const OptionalTensor& history,
+                   const OptionalTensor& history_lens, const OptionalTensor& repetition, double repetition_all, const OptionalTensor& presence,
+                   double presence_all, const OptionalTensor& frequency, double frequency_all, const OptionalTensor& bias_tokens,
+                   const OptionalTensor& bias, const OptionalTensor& allowed, const OptionalTensor& mask_of, const torch::Tensor& status);
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>> sample(
     const torch::Tensor& logits, const torch::Tensor& noise, const c10::optional<torch::Tensor>& temperature, double temperature_all,
     const c10::optional<torch::Tensor>& top_k, int64_t top_k_all, const c10::optional<torch::Tensor>& top_p, double top_p_all,
@@ -59,7 +66,8 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> sample(
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(
     const torch::Tensor& q, const torch::Tensor& k_pages, const torch::Tensor& v_pages, const torch::Tensor& prefix_pages, int64_t prefix_len,
     const torch::Tensor& page_table, const torch::Tensor& seq_lens, const c10::optional<torch::Tensor>& q_offsets, int64_t max_q_len,
-    int64_t max_seq_len, double scale, bool return_lse, const torch::Tensor& status);
+    int64_t max_seq_len, double scale, bool return_lse, const OptionalTensor& k_scales, const OptionalTensor& v_scales,
+    const torch::Tensor& status);
 // comm.cu
 void register_comm(pybind11::module_& m);
 }  // namespace mnb
@@ -93,6 +101,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("free_sequences", &mnb::free_sequences);
   m.def("compact_pages", &mnb::compact_pages);
   m.def("append_kv", &mnb::append_kv);
+  m.def("adjust_logits", &mnb::adjust_logits, "penalties, biases and masks on logits");
   m.def("sample", &mnb::sample, "temperature / top-k / top-p / min-p sampling from given noise");
   m.def("shared_prefix_attention", &mnb::shared_prefix_attention,
         "paged attention over a shared prefix and each sequence's own tokens");

@@ -330,14 +330,15 @@ __global__ void __launch_bounds__(kThreads) compact_plan_kernel(const int* __res
 
 // 16-byte chunks of the named pages, in every plane: [planes][moves][chunks].
 // Eight loads in flight per thread: 83 us for 477 MB (5.8 TB/s; four 97, two 88).
-// `tokens` (or null) gives the leading tokens of each page that hold data.
+// `tokens` (or null) gives the leading tokens of each page that hold data.  A page of codes in 8 bits takes its scales along.
 // The kernel may start while the one that plans the copies still writes src,
 // dst, tokens and count, so those are neither const nor __restrict__: nothing
 // may read them ahead of wait_for_previous().
 constexpr int kPer = 8;
 __global__ void __launch_bounds__(256) copy_pages_kernel(uint4* __restrict__ pool, long long plane_chunks,
                                                          int page_chunks, int token_chunks, int planes, int pages,
-                                                         int* src, int* dst, int* tokens, int* count, int n_max, int* status) {
+                                                         int* src, int* dst, int* tokens, int* count, int n_max, int* status,
+                                                         float* scales, int heads) {
   wait_for_previous();
   const int n = count ? min(*count, n_max) : n_max;
   const int runs = (page_chunks + 256 * kPer - 1) / (256 * kPer);
@@ -364,6 +365,9 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(uint4* __restrict__ poo
 #pragma unroll
     for (int k = 0; k < kPer; ++k)
       if (c0 + k * 256 < valid) into[c0 + k * 256] = w[k];
+    if (scales && run == 0)
+      for (int h = threadIdx.x; h < heads; h += 256)
+        scales[(static_cast<long long>(plane) * pages + b) * heads + h] = scales[(static_cast<long long>(plane) * pages + a) * heads + h];
   }
 }
 
@@ -417,7 +421,7 @@ cudaError_t launch_copy(const Pool& p, int* src, int* dst, int* tokens, int* cou
   const long long runs = (p.page_chunks + 256 * kPer - 1) / (256 * kPer);
   return launch_after(copy_pages_kernel, copy_blocks(static_cast<long long>(n) * p.planes * runs), 256, 0, stream,
                       static_cast<uint4*>(p.base), p.plane_chunks, p.page_chunks, p.token_chunks, p.planes, p.pages, src, dst,
-                      tokens, count, n, status);
+                      tokens, count, n, status, p.scales, p.heads);
 }
 
 cudaError_t launch_fork(const Pool& p, const Table& t, const int* parents, const int* children, int n, int* scratch,

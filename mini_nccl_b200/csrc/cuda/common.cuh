@@ -25,6 +25,7 @@ enum : int {
   kErrBadArgument = 3,
   kErrNoPages = 4,         // the key / value cache's pool has too few free pages
   kErrBadIndex = 5,        // a token, page, slot, position or length outside its tensor
+  kErrNotANumber = 6,      // NaN among values that are to be held as int8
 };
 
 // ---------------------------------------------------------------------------

@@ -35,13 +35,33 @@ int* errors_of(const torch::Tensor& status) { return status.data_ptr<int>() + 2;
 // 16-byte accesses along the last axis work at every index.
 bool rows_aligned(const torch::Tensor& t) {
   bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-  for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) * t.element_size() % 16 == 0);
   return ok;
 }
 
 __nv_bfloat16* bf16(const torch::Tensor& t) { return reinterpret_cast<__nv_bfloat16*>(t.data_ptr()); }
+uint8_t* bytes(const torch::Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
 
-cache::Pool pool_of(const torch::Tensor& kv) {
+using Scales = c10::optional<torch::Tensor>;
+
+// The kind of a cache's pages; those in 8 bits come with a scale for each page and kv head.
+prefix::Codes codes_of(const torch::Tensor& k_pages, const torch::Tensor& v_pages, const Scales& k_scales, const Scales& v_scales) {
+  const auto type = k_pages.scalar_type();
+  const auto codes = type == at::kChar ? prefix::kInt8 : type == at::kFloat8_e4m3fn ? prefix::kE4m3 : prefix::kNoCodes;
+  TORCH_CHECK_VALUE((codes || type == at::kBFloat16) && v_pages.scalar_type() == type && k_pages.is_cuda() && k_pages.dim() == 4 &&
+                        v_pages.sizes() == k_pages.sizes() && v_pages.strides() == k_pages.strides() && v_pages.device() == k_pages.device(),
+                    "k_pages and v_pages: bf16, int8 or float8_e4m3fn CUDA tensors [num_pages, page_size, kv_heads, head_dim] of one layout");
+  TORCH_CHECK_VALUE(codes ? k_scales && v_scales : !k_scales && !v_scales,
+                    "k_scales and v_scales: needed with pages of int8 or float8_e4m3fn, and only with them");
+  if (codes)
+    for (const auto* s : {&*k_scales, &*v_scales})
+      TORCH_CHECK_VALUE(s->device() == k_pages.device() && s->scalar_type() == at::kFloat && s->dim() == 2 && s->size(0) == k_pages.size(0) &&
+                            s->size(1) == k_pages.size(2) && s->strides() == k_scales->strides(),
+                        "k_scales and v_scales: fp32 tensors [num_pages, kv_heads] of one layout, on the pages' device");
+  return codes;
+}
+
+cache::Pool pool_of(const torch::Tensor& kv, const Scales& scales) {
   TORCH_CHECK_VALUE(kv.is_cuda() && kv.dim() >= 4 && kv.is_contiguous(),
                     "kv: a contiguous CUDA tensor [..., num_pages, page_size, kv_heads, head_dim]");
   TORCH_CHECK_VALUE(kv.numel() > 0, "kv: an empty pool");
@@ -59,6 +79,15 @@ cache::Pool pool_of(const torch::Tensor& kv) {
   p.planes = static_cast<int>(kv.numel() * kv.element_size() / (page * pages));
   p.pages = static_cast<int>(pages);
   p.page_size = static_cast<int>(kv.size(d - 3));
+  p.scales = nullptr;
+  p.heads = 0;
+  if (scales) {
+    bool fits = scales->device() == kv.device() && scales->scalar_type() == at::kFloat && scales->is_contiguous() && scales->dim() == d - 2;
+    for (int64_t i = 0; fits && i < d - 2; ++i) fits = scales->size(i) == kv.size(i < d - 3 ? i : d - 2);
+    TORCH_CHECK_VALUE(fits, "scales: a contiguous fp32 tensor [..., num_pages, kv_heads] with the leading axes of kv");
+    p.scales = scales->data_ptr<float>();
+    p.heads = static_cast<int>(kv.size(d - 2));
+  }
   return p;
 }
 
@@ -99,9 +128,9 @@ void prefix_exp2_eval(const torch::Tensor& x, const torch::Tensor& y) {
                                      at::cuda::getCurrentCUDAStream()));
 }
 
-void copy_pages(const torch::Tensor& kv, const torch::Tensor& src, const torch::Tensor& dst, const torch::Tensor& status) {
+void copy_pages(const torch::Tensor& kv, const torch::Tensor& src, const torch::Tensor& dst, const Scales& scales, const torch::Tensor& status) {
   launched = 0;
-  const auto p = pool_of(kv);
+  const auto p = pool_of(kv, scales);
   check_int32(src, 1, kv, "src");
   check_int32(dst, 1, kv, "dst");
   check_status_word(status);
@@ -113,9 +142,9 @@ void copy_pages(const torch::Tensor& kv, const torch::Tensor& src, const torch::
 }
 
 void fork_sequences(const torch::Tensor& kv, const torch::Tensor& page_table, const torch::Tensor& lens, const torch::Tensor& refs,
-                    const torch::Tensor& parents, const torch::Tensor& children, const torch::Tensor& status) {
+                    const torch::Tensor& parents, const torch::Tensor& children, const Scales& scales, const torch::Tensor& status) {
   launched = 0;
-  const auto p = pool_of(kv);
+  const auto p = pool_of(kv, scales);
   const auto t = table_of(page_table, lens, refs, p.page_size);
   check_int32(parents, 1, kv, "parents");
   check_int32(children, 1, kv, "children");
@@ -165,9 +194,9 @@ void free_sequences(const torch::Tensor& page_table, const torch::Tensor& lens, 
 }
 
 std::tuple<torch::Tensor, torch::Tensor> compact_pages(const torch::Tensor& kv, const torch::Tensor& page_table, const torch::Tensor& refs,
-                                                       const torch::Tensor& status) {
+                                                       const Scales& scales, const torch::Tensor& status) {
   launched = 0;
-  const auto p = pool_of(kv);
+  const auto p = pool_of(kv, scales);
   check_int32(page_table, 2, kv, "page_table");
   check_int32(refs, 1, kv, "refs");
   check_status_word(status);
@@ -185,18 +214,16 @@ std::tuple<torch::Tensor, torch::Tensor> compact_pages(const torch::Tensor& kv, 
 }
 
 void append_kv(const torch::Tensor& k_pages, const torch::Tensor& v_pages, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& page_table,
-               const torch::Tensor& positions, const c10::optional<torch::Tensor>& slots, const torch::Tensor& status) {
+               const torch::Tensor& positions, const c10::optional<torch::Tensor>& slots,
+               const Scales& k_scales, const Scales& v_scales, const torch::Tensor& status) {
   launched = 0;
-  TORCH_CHECK_VALUE(k_pages.is_cuda() && k_pages.dim() == 4 && k_pages.scalar_type() == at::kBFloat16 &&
-                        v_pages.scalar_type() == at::kBFloat16 && v_pages.sizes() == k_pages.sizes() &&
-                        v_pages.strides() == k_pages.strides() && v_pages.device() == k_pages.device(),
-                    "k_pages and v_pages: bf16 CUDA tensors [num_pages, page_size, kv_heads, head_dim] of one layout");
+  const auto codes = codes_of(k_pages, v_pages, k_scales, v_scales);
   TORCH_CHECK_VALUE(k.dim() == 3 && v.dim() == 3 && k.sizes() == v.sizes() && k.scalar_type() == at::kBFloat16 &&
                         v.scalar_type() == at::kBFloat16 && k.device() == k_pages.device() && v.device() == k.device(),
                     "k and v: bf16 tensors [tokens, kv_heads, head_dim] on the pages' device");
   const int64_t H = k_pages.size(2), D = k_pages.size(3), n = k.size(0);
   TORCH_CHECK_VALUE(k.size(1) == H && k.size(2) == D, "k and v: ", H, " heads of ", D, " as in the pages");
-  TORCH_CHECK_VALUE(D % 8 == 0, "head_dim: a multiple of 8");
+  TORCH_CHECK_VALUE(codes ? D % 16 == 0 && D <= 256 : D % 8 == 0, "head_dim: a multiple of 8 (in 8 bits: of 16, and at most 256)");
   TORCH_CHECK_VALUE(n == 0 || k_pages.numel() == 0 ||
                         (rows_aligned(k) && rows_aligned(v) && rows_aligned(k_pages) && rows_aligned(v_pages)),
                     "k, v and the pages: last axis contiguous, rows 16-byte aligned");
@@ -212,28 +239,47 @@ void append_kv(const torch::Tensor& k_pages, const torch::Tensor& v_pages, const
   }
   if (n * H * D == 0 || k_pages.size(1) == 0) return;
   const c10::cuda::CUDAGuard guard(k_pages.device());
+  TORCH_CHECK_VALUE(n < (1ll << 31), "too many tokens");
+  auto fill = [&](auto& a) {
+    a.page_ld = k_pages.stride(0);
+    a.token_ld = k_pages.stride(1);
+    a.head_ld = k_pages.stride(2);
+    a.k = bf16(k);
+    a.v = bf16(v);
+    a.k_ld = k.stride(0);
+    a.k_head = k.stride(1);
+    a.v_ld = v.stride(0);
+    a.v_head = v.stride(1);
+    a.table = page_table.data_ptr<int>();
+    a.table_ld = page_table.stride(0);
+    a.slots = static_cast<int>(page_table.size(0));
+    a.columns = static_cast<int>(page_table.size(1));
+    a.pages = static_cast<int>(k_pages.size(0));
+    a.page_size = static_cast<int>(k_pages.size(1));
+    a.positions = positions.data_ptr<int>();
+    a.slot_of = slots ? slots->data_ptr<int>() : nullptr;
+    a.n = static_cast<int>(n);
+    a.heads = static_cast<int>(H);
+  };
+  if (codes) {
+    cache::Append8 a{};
+    a.e4m3 = codes == prefix::kE4m3;
+    a.k_pool = bytes(k_pages);
+    a.v_pool = bytes(v_pages);
+    a.k_scales = k_scales->data_ptr<float>();
+    a.v_scales = v_scales->data_ptr<float>();
+    a.scale_ld = k_scales->stride(0);
+    a.scale_head = k_scales->stride(1);
+    a.dim = static_cast<int>(D);
+    fill(a);
+    C10_CUDA_CHECK(cache::launch_append8(a, errors_of(status), at::cuda::getCurrentCUDAStream()));
+    launched = 1;
+    return;
+  }
   cache::Append a{};
   a.k_pool = bf16(k_pages);
   a.v_pool = bf16(v_pages);
-  a.page_ld = k_pages.stride(0);
-  a.token_ld = k_pages.stride(1);
-  a.head_ld = k_pages.stride(2);
-  a.k = bf16(k);
-  a.v = bf16(v);
-  a.k_ld = k.stride(0);
-  a.k_head = k.stride(1);
-  a.v_ld = v.stride(0);
-  a.v_head = v.stride(1);
-  a.table = page_table.data_ptr<int>();
-  a.table_ld = page_table.stride(0);
-  a.slots = static_cast<int>(page_table.size(0));
-  a.columns = static_cast<int>(page_table.size(1));
-  a.pages = static_cast<int>(k_pages.size(0));
-  a.page_size = static_cast<int>(k_pages.size(1));
-  a.positions = positions.data_ptr<int>();
-  a.slot_of = slots ? slots->data_ptr<int>() : nullptr;
-  a.n = static_cast<int>(n);
-  a.heads = static_cast<int>(H);
+  fill(a);
   a.chunks = static_cast<int>(D / 8);
   C10_CUDA_CHECK(cache::launch_append(a, errors_of(status), at::cuda::getCurrentCUDAStream()));
   launched = 1;
@@ -282,17 +328,108 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> sample(
   return {token, logprob};
 }
 
+namespace {
+
+// A list of tokens for each row, or one for all of them.
+logits::Ids ids_of(const c10::optional<torch::Tensor>& t, int64_t rows, const torch::Tensor& like, bool shared, const char* what) {
+  logits::Ids ids{};
+  if (!t) return ids;
+  TORCH_CHECK_VALUE(t->device() == like.device() && (t->scalar_type() == at::kLong || t->scalar_type() == at::kInt) &&
+                        ((t->dim() == 2 && t->size(0) == rows) || (shared && t->dim() == 1)) &&
+                        (t->numel() == 0 || t->size(-1) == 1 || t->stride(-1) == 1),
+                    what, ": int64 or int32 tokens [", rows, " rows, n]", shared ? " or [n]" : "", " on the logits' device, last axis contiguous");
+  ids.ids = t->data_ptr();
+  ids.wide = t->scalar_type() == at::kLong;
+  ids.ld = t->dim() == 2 ? t->stride(0) : 0;
+  ids.n = t->size(-1);
+  return ids;
+}
+
+}  // namespace
+
+void adjust_logits(const torch::Tensor& in, const torch::Tensor& out, const c10::optional<torch::Tensor>& prompt,
+                   const c10::optional<torch::Tensor>& history, const c10::optional<torch::Tensor>& history_lens,
+                   const c10::optional<torch::Tensor>& repetition, double repetition_all, const c10::optional<torch::Tensor>& presence,
+                   double presence_all, const c10::optional<torch::Tensor>& frequency, double frequency_all,
+                   const c10::optional<torch::Tensor>& bias_tokens, const c10::optional<torch::Tensor>& bias,
+                   const c10::optional<torch::Tensor>& allowed, const c10::optional<torch::Tensor>& mask_of, const torch::Tensor& status) {
+  launched = 0;
+  using sampling::Setting;
+  TORCH_CHECK_VALUE(in.is_cuda() && in.dim() == 2 && (in.scalar_type() == at::kBFloat16 || in.scalar_type() == at::kFloat),
+                    "logits: a bf16 or fp32 tensor [rows, vocabulary]");
+  const int64_t R = in.size(0), V = in.size(1);
+  TORCH_CHECK_VALUE(V >= 1 && V <= (1 << sampling::kIndexBits), "vocabulary: 1 to 1048576 tokens, got ", V);
+  TORCH_CHECK_VALUE(in.stride(1) == 1 || V == 1, "logits: last axis contiguous");
+  TORCH_CHECK_VALUE(out.device() == in.device() && out.scalar_type() == in.scalar_type() && out.sizes() == in.sizes() &&
+                        (out.stride(1) == 1 || V == 1) && (R <= 1 || out.stride(0) >= V),
+                    "out: a tensor like logits, last axis contiguous, rows apart");
+  check_status_word(status);
+  logits::Adjust a{};
+  a.prompt = ids_of(prompt, R, in, true, "prompt");
+  a.history = ids_of(history, R, in, false, "history");
+  a.bias_tokens = ids_of(bias_tokens, R, in, true, "bias_tokens");
+  TORCH_CHECK_VALUE(a.history.n < (1 << logits::kCountBits) && a.prompt.n < (1ll << 31), "history: at most ", (1 << logits::kCountBits) - 1, " tokens a row");
+  if (history_lens) {
+    check_int32(*history_lens, 1, in, "history_lens");
+    TORCH_CHECK_VALUE(history && history_lens->size(0) == R, "history_lens: one length for each row of history");
+    TORCH_CHECK_VALUE(history_lens->is_contiguous(), "history_lens: contiguous");
+    a.history_lens = history_lens->data_ptr<int>();
+  }
+  TORCH_CHECK_VALUE(bias_tokens.has_value() == bias.has_value(), "bias_tokens and bias: one needs the other");
+  if (bias) {
+    TORCH_CHECK_VALUE(bias->device() == in.device() && bias->scalar_type() == at::kFloat && bias->sizes() == bias_tokens->sizes() &&
+                          bias->is_contiguous() && bias_tokens->is_contiguous(),
+                      "bias_tokens and bias: contiguous, fp32 biases of the tokens' shape");
+    TORCH_CHECK_VALUE(a.bias_tokens.n <= logits::kMostBiases, "bias_tokens: at most ", logits::kMostBiases, " a row");
+    a.bias = bias->data_ptr<float>();
+  }
+  a.repetition = setting<Setting>(repetition, repetition_all, R, at::kFloat, in, "repetition");
+  a.presence = setting<Setting>(presence, presence_all, R, at::kFloat, in, "presence");
+  a.frequency = setting<Setting>(frequency, frequency_all, R, at::kFloat, in, "frequency");
+  if (allowed) {
+    check_int32(*allowed, 2, in, "allowed");
+    TORCH_CHECK_VALUE(allowed->size(1) == (V + 31) / 32, "allowed: ", (V + 31) / 32, " words of 32 tokens a mask");
+    a.allowed = reinterpret_cast<const uint32_t*>(allowed->data_ptr<int>());
+    a.mask_ld = allowed->stride(0);
+    a.masks = static_cast<int>(allowed->size(0));
+    if (mask_of) {
+      check_int32(*mask_of, 1, in, "mask_of");
+      TORCH_CHECK_VALUE(mask_of->size(0) == R && mask_of->is_contiguous(), "mask_of: contiguous, one mask for each row");
+      a.mask_of = mask_of->data_ptr<int>();
+    } else {
+      TORCH_CHECK_VALUE(a.masks == 1 || a.masks == R, "allowed: without mask_of one mask, or one for each row");
+    }
+  } else {
+    TORCH_CHECK_VALUE(!mask_of, "mask_of: needs allowed");
+  }
+  if (R == 0) return;
+  TORCH_CHECK_VALUE(R * ((V + 2047) / 2048 + 1) < (1ll << 31), "too many rows");
+  const c10::cuda::CUDAGuard guard(in.device());
+  a.in = in.data_ptr();
+  a.out = out.data_ptr();
+  a.bf16 = in.scalar_type() == at::kBFloat16;
+  a.in_ld = in.stride(0);
+  a.out_ld = out.stride(0);
+  a.in_place = a.in == a.out && (a.in_ld == a.out_ld || R == 1);
+  auto end_of = [&](const torch::Tensor& t) { return static_cast<const char*>(t.data_ptr()) + ((R - 1) * t.stride(0) + V) * t.element_size(); };
+  TORCH_CHECK_VALUE(a.in_place || end_of(in) <= static_cast<const char*>(out.data_ptr()) || end_of(out) <= static_cast<const char*>(in.data_ptr()),
+                    "out: logits itself, or memory that does not overlap it");
+  a.rows = static_cast<int>(R);
+  a.vocab = static_cast<int>(V);
+  a.status = errors_of(status);
+  C10_CUDA_CHECK(logits::launch_adjust(a, at::cuda::getCurrentCUDAStream()));
+  launched = 1;
+}
+
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(
     const torch::Tensor& q, const torch::Tensor& k_pages, const torch::Tensor& v_pages, const torch::Tensor& prefix_pages, int64_t prefix_len,
     const torch::Tensor& page_table, const torch::Tensor& seq_lens, const c10::optional<torch::Tensor>& q_offsets, int64_t max_q_len,
-    int64_t max_seq_len, double scale, bool return_lse, const torch::Tensor& status) {
+    int64_t max_seq_len, double scale, bool return_lse, const Scales& k_scales, const Scales& v_scales, const torch::Tensor& status) {
   launched = 0;
   TORCH_CHECK_VALUE(q.is_cuda() && q.scalar_type() == at::kBFloat16 && q.dim() == 3,
                     "q: a bf16 CUDA tensor [tokens, heads, head_dim]");
-  TORCH_CHECK_VALUE(k_pages.device() == q.device() && v_pages.device() == q.device() &&
-                        k_pages.scalar_type() == at::kBFloat16 && v_pages.scalar_type() == at::kBFloat16 &&
-                        k_pages.dim() == 4 && k_pages.sizes() == v_pages.sizes() && k_pages.strides() == v_pages.strides(),
-                    "k_pages and v_pages: bf16 tensors [num_pages, page_size, kv_heads, head_dim] of one layout, on q's device");
+  const auto codes = codes_of(k_pages, v_pages, k_scales, v_scales);
+  TORCH_CHECK_VALUE(k_pages.device() == q.device(), "k_pages and v_pages: on q's device");
   const int64_t N = q.size(0), H = q.size(1), D = q.size(2);
   const int64_t pages = k_pages.size(0), page = k_pages.size(1), Hk = k_pages.size(2);
   TORCH_CHECK_VALUE(D == 32 || D == 64 || D == 128, "head_dim: 32, 64 or 128, got ", D);
@@ -338,8 +475,20 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(
   a.q = bf16(q);
   a.q_ld = q.stride(0);
   a.q_head = q.stride(1);
-  a.k = bf16(pages > 0 ? k_pages : q);  // (a map needs an address, also where nothing will be read)
-  a.v = bf16(pages > 0 ? v_pages : q);
+  // (a map needs an address, also where nothing will be read)
+  const torch::Tensor &k_of = pages > 0 ? k_pages : q, &v_of = pages > 0 ? v_pages : q;
+  a.codes = codes;
+  if (codes) {
+    a.k8 = bytes(k_of);
+    a.v8 = bytes(v_of);
+    a.k_scales = k_scales->data_ptr<float>();
+    a.v_scales = v_scales->data_ptr<float>();
+    a.scale_ld = k_scales->stride(0);
+    a.scale_head = k_scales->stride(1);
+  } else {
+    a.k = bf16(k_of);
+    a.v = bf16(v_of);
+  }
   a.page_ld = k_pages.stride(0);
   a.token_ld = k_pages.stride(1);
   a.head_ld = k_pages.stride(2);
@@ -365,7 +514,8 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(
   a.o = bf16(o);
   a.lse = lse ? lse->data_ptr<float>() : nullptr;
   const int64_t pieces = prefix::plan(a, static_cast<int>(D)), rows = N * H;
-  TORCH_CHECK_VALUE(B * a.own_tiles * a.own_splits * Hk < (1ll << 31), "too many sequences times max_q_len");
+  TORCH_CHECK_VALUE(B * a.own_tiles * a.own_splits * Hk < (1ll << 30), "too many sequences times max_q_len");
+  TORCH_CHECK_VALUE(static_cast<int64_t>(a.row_tiles) * a.prefix_splits * Hk < (1ll << 30), "too many rows");
   torch::Tensor part;
   if (pieces > 0) {
     part = at::empty({pieces * rows * (D + 2) + 1}, q.options().dtype(at::kFloat));

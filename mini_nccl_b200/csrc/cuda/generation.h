@@ -6,6 +6,7 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+#include <stdint.h>
 
 namespace mnb {
 
@@ -16,6 +17,8 @@ struct Pool {
   void* base;
   long long plane_chunks;
   int page_chunks, token_chunks, planes, pages, page_size;
+  float* scales;  // [planes][pages][heads] of codes in 8 bits, or null
+  int heads;
 };
 
 struct Table {
@@ -53,6 +56,23 @@ cudaError_t launch_compact(const Pool& p, const int* table, long long table_ld, 
                            int* new_table, int* new_refs, int* scratch, int* status, cudaStream_t stream);
 cudaError_t launch_append(const Append& a, int* status, cudaStream_t stream);
 
+struct Append8 {
+  bool e4m3;  // or int8
+  uint8_t *k_pool, *v_pool;
+  long long page_ld, token_ld, head_ld;
+  float *k_scales, *v_scales;  // one for each page and head
+  long long scale_ld, scale_head;
+  const __nv_bfloat16 *k, *v;
+  long long k_ld, k_head, v_ld, v_head;
+  const int* table;
+  long long table_ld;
+  int slots, columns, pages, page_size;
+  const int* positions;
+  const int* slot_of;  // or null: token i belongs to row i
+  int n, heads, dim;
+};
+cudaError_t launch_append8(const Append8& a, int* status, cudaStream_t stream);
+
 }  // namespace cache
 
 namespace sampling {
@@ -87,12 +107,52 @@ cudaError_t launch_sample(const Sample& a, cudaStream_t stream);
 
 }  // namespace sampling
 
+namespace logits {
+
+constexpr int kCountBits = 19;                    // a row's history is shorter than 2^19 tokens
+constexpr int kMostBiases = (1 << (31 - kCountBits)) - 1;  // that a row names
+
+// Lists of tokens, int64 or int32; one list for all rows has ld 0.
+struct Ids {
+  const void* ids;
+  bool wide;
+  long long ld, n;
+};
+
+struct Adjust {
+  const void* in;
+  void* out;
+  bool bf16, in_place;
+  long long in_ld, out_ld;
+  int rows, vocab;
+  Ids prompt, history;
+  const int* history_lens;  // or null: all of them
+  sampling::Setting repetition, presence, frequency;
+  Ids bias_tokens;
+  const float* bias;  // as bias_tokens
+  const uint32_t* allowed;
+  long long mask_ld;
+  int masks;
+  const int* mask_of;  // or null: mask r for row r, or the only one
+  int* status;
+};
+
+cudaError_t launch_adjust(const Adjust& a, cudaStream_t stream);
+
+}  // namespace logits
+
 namespace prefix {
+
+enum Codes { kNoCodes, kInt8, kE4m3 };
 
 struct Args {
   const __nv_bfloat16* q;
   long long q_ld, q_head;
   const __nv_bfloat16 *k, *v;
+  Codes codes;             // of a cache in 8 bits: then the pages are these, with a scale for each page and kv head
+  const uint8_t *k8, *v8;
+  const float *k_scales, *v_scales;
+  long long scale_ld, scale_head;
   long long page_ld, token_ld, head_ld;  // of the page pools, in elements
   int pages, page_shift;
   int no_page;  // an index outside the pool's tensor map, where TMA reads zeros: for ids that name no page
@@ -133,6 +193,9 @@ int plan(Args& a, int head_dim);
 cudaError_t launch_prefix_tc(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, int head_dim, cudaStream_t stream);
 // the tensor-core kernel's own 2^x, on 2 * pairs numbers
 cudaError_t launch_exp2(const float* x, float* y, int pairs, cudaStream_t stream);
+// of a cache in 8 bits (prefix_attention_8bit.cu)
+int plan8(Args& a, int head_dim);
+cudaError_t launch_pieces8(const Args& a, int head_dim, cudaStream_t stream);
 cudaError_t launch_attention(const Args& a, int head_dim, cudaStream_t stream);
 int kernels(const Args& a);  // that launch_attention() launches
 

@@ -1,0 +1,518 @@
+// The paged attention over a cache in 8 bits: codes (int8 or e4m3) and one fp32
+// scale for each page and kv head; a code stands for code * scale.
+// prefix_attention.cu has the mathematics, the pieces and the kernel that joins
+// them; prefix_attention_8bit_tc.cu takes the prefix where there are many rows.
+//
+// With codes c, scales a (keys) and b (values), s_j = scale q . k_j = (scale a_j) (q . c_j),
+// and with w_j = b_j exp(s_j) = exp(s_j + log b_j) a part's output is sum w_j c_j: the
+// scale of the values rides in the exponent, so weights and codes are both what the
+// product takes as f16.  A row's base is the running maximum of s_j + log2 b_j less
+// 15, so the largest weight is 2^15 and f16 holds weights down to 2^-39 of it (to 11
+// bits down to 2^-29).  The sum of exp(s_j) gets w_j / b_j in fp32.  Codes are exact in
+// f16.  So are queries but for values below 2^-31 of their row's largest: each row is
+// scaled by a power of two, which the scores' factor takes back.
+//
+// What bounds it: the codes' bytes are half of a bf16 cache's, and what is spent on each
+// key (widening the codes, products, exponentials) has to fit in half the time.  So the
+// products have the keys as their rows: S^T = K Q^T and O^T = V^T P^T (mma.sync
+// m16n8k16) for eight or sixteen query rows, where the usual orientation pads one
+// query row of a head to sixteen; a warp takes pieces by itself (no barriers between
+// warps, no partial results to join in a block) and widens codes in registers: an
+// int8 pair by one byte permutation and one subtraction (0x6400 | u is 1024 + u in f16),
+// an e4m3 pair by one conversion.
+#include <algorithm>
+#include <type_traits>
+
+#include "launch.cuh"
+#include "prefix_attention.cuh"
+#include "warp_mma.cuh"
+
+namespace mnb {
+
+namespace prefix {
+
+namespace q8 {
+
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kStep = 32;  // keys of a stage
+constexpr float kLeastScale = 8.673617379884035e-19f;  // 2^-60
+
+template <int D>
+struct Ring {
+  static constexpr int stages = 3;
+  static constexpr int blocks = D == 128 ? 2 : 4;    // per SM
+  static constexpr uint32_t tile = kStep * D;        // of K; V follows
+  static constexpr uint32_t bytes = stages * 2 * tile;  // of a warp
+  // 16-byte chunk c of row r, as TMA's swizzle leaves it
+  MNB_DEVICE static uint32_t at(int r, int c) {
+    const int x = D == 128 ? r & 7 : D == 64 ? (r >> 1) & 3 : (r >> 2) & 1;
+    return r * D + ((c ^ x) << 4);
+  }
+};
+
+// Where row i of the products' 8 keys lies among them: rows next to one another meet no bank conflicts when threads read
+// 16 bytes each.
+template <int D>
+MNB_DEVICE int key_of(int i) {
+  return D == 128 ? (i >> 1) | ((i & 1) << 2) : i;
+}
+
+MNB_DEVICE void mma_f16(float* c, const uint32_t* a, const uint32_t* b) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+MNB_DEVICE uint32_t transposed(uint32_t x) {  // of an 8 x 8 matrix of 16-bit values, a row's pair in each lane
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+MNB_DEVICE uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t y;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+  return y;
+}
+MNB_DEVICE uint32_t sub_f16x2(uint32_t a, uint32_t b) {
+  uint32_t y;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
+MNB_DEVICE uint32_t f16_of_e4m3(uint16_t x) {
+  uint32_t y;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(y) : "h"(x));
+  return y;
+}
+// Four codes as f16: of bytes 0 and 2 (lo), and 1 and 3 (hi).
+template <bool kFloat>
+MNB_DEVICE void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (kFloat) {
+    w = __byte_perm(w, 0, 0x3120);
+    lo = f16_of_e4m3(static_cast<uint16_t>(w)), hi = f16_of_e4m3(static_cast<uint16_t>(w >> 16));
+  } else {
+    w ^= 0x80808080u;
+    lo = sub_f16x2(__byte_perm(w, 0x64646464u, 0x4240), 0x64806480u);
+    hi = sub_f16x2(__byte_perm(w, 0x64646464u, 0x4341), 0x64806480u);
+  }
+}
+// The same as whichever pairs are cheapest: bytes (0, 1), (2, 3) of e4m3, (0, 2), (1, 3) of int8.
+template <bool kFloat>
+MNB_DEVICE void widen_any(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (kFloat)
+    lo = f16_of_e4m3(static_cast<uint16_t>(w)), hi = f16_of_e4m3(static_cast<uint16_t>(w >> 16));
+  else
+    widen<false>(w, lo, hi);
+}
+MNB_DEVICE void copy_float(uint32_t dst, const float* src, bool there) {  // zero where not
+  const int n = there ? 4 : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+MNB_DEVICE void arrive_after_copies(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// NT: eights of query rows.
+template <int D, int NT, bool kFloat>
+__global__ void __launch_bounds__(kThreads, Ring<D>::blocks)
+    pieces8_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap map_k,
+                   const __grid_constant__ CUtensorMap map_v, int items, int known) {
+  using R = Ring<D>;
+  constexpr int kStages = R::stages, kU = kStep / 16, kRows = 8 * NT, kMt = D / 16;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t bars[kWarps][kStages];
+  __shared__ float scale_of[kWarps][kStages][2][4];  // of a stage's pages: keys, values
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  const uint32_t ring = smem_u32(sm) + warp * R::bytes, bar0 = smem_u32(bars[warp]), sc0 = smem_u32(scale_of[warp]);
+  if (lane < kStages) mbar_init(bar0 + 8 * lane, 33);  // the expected bytes, and every lane's copies of scales
+  fence_mbar_init();
+  if (lane < kStages * 8) (&scale_of[warp][0][0][0])[lane] = 1.f;  // (a stage's pages may be fewer than it has room for)
+  int* lens = reinterpret_cast<int*>(sm + kWarps * R::bytes);
+  int* offsets = lens + known;
+  for (int b = threadIdx.x; b < known; b += kThreads) lens[b] = a.seq_lens[b];
+  if (a.q_offsets)
+    for (int b = threadIdx.x; b < known + (known > 0); b += kThreads) offsets[b] = a.q_offsets[b];
+  const int* const seq_lens = known ? lens : a.seq_lens;
+  const int* const q_offsets = known ? offsets : a.q_offsets;
+  __syncthreads();
+  let_next_start();
+
+  // Items in turn over the warps of all blocks.
+  const int first = blockIdx.x + warp * gridDim.x, stride = kWarps * gridDim.x;
+
+  // Loading runs ahead of the work by the stages of the ring, on into the next pieces.
+  const int per = min(1 << a.page_shift, kStep);  // tokens of a box
+  int load_item = first - stride, load_key = 0, load_end = 0, load_head = 0, batch = 0, ids_end = 0, issued = 0;
+  int ids_now = 0, ids_next = 0;  // this lane's of 32 pages from `batch` on, and of the 32 after them
+  const int* ids = nullptr;
+  auto fetch = [&](int from) { return from + lane < ids_end ? ids[from + lane] : 0; };
+  auto next_piece = [&] {
+    for (load_item += stride; load_item < items; load_item += stride) {
+      const Piece p = piece_of(a, seq_lens, q_offsets, load_item, kRows, 1);
+      if (p.k1 <= p.k0) continue;
+      load_key = p.k0, load_end = p.k1, load_head = p.h, ids = p.ids;
+      batch = p.k0 >> a.page_shift;
+      ids_end = ((p.k1 - 1) >> a.page_shift) + 1;
+      ids_now = fetch(batch);
+      ids_next = fetch(batch + 32);
+      return;
+    }
+  };
+  auto issue = [&] {
+    if (load_item >= items) return;
+    if ((load_key >> a.page_shift) - batch >= 32) {
+      batch += 32;
+      ids_now = ids_next;
+      ids_next = fetch(batch + 32);
+    }
+    const int st = issued % kStages, boxes = (min(kStep, load_end - load_key) + per - 1) / per;
+    const uint32_t bar = bar0 + 8 * st;
+    // lanes 0 to 3 fetch the keys of a box each, 4 to 7 the values
+    const int box = lane & 3, part = lane >> 2;
+    int page = __shfl_sync(0xffffffffu, ids_now, (load_key >> a.page_shift) - batch + min(box, boxes - 1));
+    if (lane == 0) mbar_arrive_expect_tx(bar, boxes * per * D * 2);
+    __syncwarp();
+    if (lane < 8 && box < boxes) {
+      const bool there = page >= 0 && page < a.pages;
+      if (!there) {
+        flag(a);
+        page = a.no_page;  // reads as zeros
+      }
+      const int key = load_key + box * per;
+      tma_load_4d(ring + (st * 2 + part) * R::tile + box * per * D, part ? &map_v : &map_k, 0, load_head,
+                  key & ((1 << a.page_shift) - 1), page, bar);
+      const float* s = part ? a.v_scales : a.k_scales;
+      copy_float(sc0 + ((st * 2 + part) * 4 + box) * 4, there ? s + page * a.scale_ld + load_head * a.scale_head : s, there);
+    }
+    arrive_after_copies(bar);
+    ++issued;
+    load_key += kStep;
+    if (load_key >= load_end) next_piece();
+  };
+  next_piece();
+  for (int s = 0; s < kStages; ++s) issue();
+
+  // Where this lane reads: row g (and g + 8) of 16 keys as the first operand of K Q^T, and the rows of ldmatrix for V^T P^T
+  const uint32_t at_k = D == 32 ? R::at(g, t >> 1) + (t & 1) * 8 : R::at(key_of<D>(g), t);
+  const uint32_t at_v = R::at(((lane >> 3) & 1) * 8 + key_of<D>(lane & 7), lane >> 4);
+  int pos = 0;  // stages used so far
+  for (int i = first; i < items; i += stride) {
+    const Piece p = piece_of(a, seq_lens, q_offsets, i, kRows, 1);
+    if (p.n_rows <= 0) continue;
+    auto out_of = [&](int r) {
+      const int j = p.r0 + r, token = j / a.group;
+      return (static_cast<long long>(p.slot) * a.n + p.n0 + token) * a.heads + p.h * a.group + j - token * a.group;
+    };
+    if (p.k1 <= p.k0) {  // nothing here: the join skips the piece
+      if (lane < p.n_rows) a.part_ml[out_of(lane)] = make_float2(-INFINITY, 0.f);
+      continue;
+    }
+    // Queries as the products' second operand: row n * 8 + g, four dims (those of a word of codes) for each 16-wide step.
+    uint32_t qf[NT][kMt][2];
+    float back[NT][2];  // what rows n * 8 + 2 t and + 1 were scaled by, taken back
+    int lim[NT][2];     // the keys that they see
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = n * 8 + g, j = p.r0 + r, token = j / a.group;
+      const bool in = r < p.n_rows;
+      const __nv_bfloat16* q = a.q + (p.n0 + token) * a.q_ld + (p.h * a.group + j - token * a.group) * a.q_head;
+      uint4 w[kMt / 2];
+#pragma unroll
+      for (int x = 0; x < kMt / 2; ++x) {
+        const int dim = D == 32 ? 8 * t : (x / 2) * 64 + 16 * t + (x % 2) * 8;
+        w[x] = in ? ld_v4(q + dim) : make_uint4(0, 0, 0, 0);
+      }
+      uint32_t most = 0;  // of the finite values, as bits
+#pragma unroll
+      for (int x = 0; x < kMt / 2; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t v = (&w[x].x)[e], lo = v & 0x7fffu, hi = (v >> 16) & 0x7fffu;
+          most = max(most, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+        }
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      const int shift = min(141 - static_cast<int>(most >> 7), 126);  // the largest becomes 2^14 to 2^15
+      const float up = __int_as_float((127 + shift) << 23);
+#pragma unroll
+      for (int x = 0; x < kMt / 2; ++x)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float2 u = unpack_bf16x2((&w[x].x)[2 * e]), v = unpack_bf16x2((&w[x].x)[2 * e + 1]);
+          u = mul2(u, splat2(up)), v = mul2(v, splat2(up));
+          qf[n][2 * x + e][0] = kFloat ? pack_f16x2(u.x, u.y) : pack_f16x2(u.x, v.x);
+          qf[n][2 * x + e][1] = kFloat ? pack_f16x2(v.x, v.y) : pack_f16x2(u.y, v.y);
+        }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = n * 8 + 2 * t + e;
+        back[n][e] = __int_as_float((127 - __shfl_sync(0xffffffffu, shift, (2 * t + e) * 4)) << 23);
+        lim[n][e] = row < p.n_rows ? min(p.k1, p.limit0 + (p.r0 + row) / a.group) : p.k0;
+      }
+    }
+    const int whole = min(p.k1, p.limit0 + p.r0 / a.group);  // keys before this are seen by every row
+    float o[NT][kMt][4], base[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      base[n][0] = base[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int m = 0; m < kMt; ++m) o[n][m][0] = o[n][m][1] = o[n][m][2] = o[n][m][3] = 0.f;
+    }
+
+    for (int t0 = p.k0; t0 < p.k1; t0 += kStep, ++pos) {
+      const int st = pos % kStages;
+      mbar_wait(bar0 + 8 * st, (pos / kStages) & 1, a.status);  // (a wait that gave up is in the status word)
+      __syncwarp();
+      const uint32_t sK = ring + st * 2 * R::tile, sV = sK + R::tile;
+      float s[NT][kU][4];
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n][u][0] = s[n][u][1] = s[n][u][2] = s[n][u][3] = 0.f;
+#pragma unroll
+        for (int x = 0; x < (D + 63) / 64; ++x) {
+          uint4 ka, kb;  // a row's words: two of them at head dim 32
+          const uint32_t from = (sK + u * 16 * D + at_k) ^ (x * 64);
+          if (D == 32) {
+            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(ka.x), "=r"(ka.y) : "r"(from));
+            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(kb.x), "=r"(kb.y) : "r"(from + 8 * D));
+          } else {
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(ka.x), "=r"(ka.y), "=r"(ka.z), "=r"(ka.w) : "r"(from));
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(kb.x), "=r"(kb.y), "=r"(kb.z), "=r"(kb.w) : "r"(from + 8 * D));
+          }
+#pragma unroll
+          for (int j = 0; j < (D == 32 ? 2 : 4); ++j) {
+            uint32_t f[4];
+            widen_any<kFloat>((&ka.x)[j], f[0], f[2]);
+            widen_any<kFloat>((&kb.x)[j], f[1], f[3]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_f16(s[n][u], f, qf[n][x * 4 + j]);
+          }
+        }
+      }
+      // Each eight keys lie in one page: its factor of the scores, the logarithm of its values' scale, and what turns a
+      // weight into its part of the sum (times 2^15, so that nothing leaves the range of fp32).
+      const int box = min((lane & 3) * 8 >> a.page_shift, 3);
+      const float mine_v = fmaxf(scale_of[warp][st][1][box], kLeastScale);  // (a page of zeros may have any scale)
+      const float mine_k = scale_of[warp][st][0][box] * a.scale_log2, mine_b = __log2f(mine_v), mine_r = ex2_approx(15.f - mine_b);
+      const bool masked = t0 + kStep > whole;
+      float top[NT][2];
+      float sum_of[kU][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float fk = __shfl_sync(0xffffffffu, mine_k, 2 * u + h), fb = __shfl_sync(0xffffffffu, mine_b, 2 * u + h);
+          sum_of[u][h] = __shfl_sync(0xffffffffu, mine_r, 2 * u + h);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              // (towards zero: a factor past fp32's range stays finite, and 0 times it stays 0)
+              float x = fmaf(s[n][u][2 * h + e], __fmul_rz(fk, back[n][e]), fb);
+              if (masked && t0 + u * 16 + h * 8 + key_of<D>(g) >= lim[n][e]) x = -INFINITY;
+              s[n][u][2 * h + e] = x;
+              top[n][e] = fmaxf(top[n][e], x);
+            }
+        }
+      uint32_t pf[NT][kU][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float from[2];
+        bool moved = false;
+        float alpha[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], 4));
+          top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], 8));
+          top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], 16));
+          const float to = fmaxf(base[n][e], top[n][e] - 15.f);
+          from[e] = to == -INFINITY ? 0.f : to;  // no key yet: every weight is exp2(-inf) = 0
+          alpha[e] = ex2_approx(base[n][e] - from[e]);
+          moved = moved || alpha[e] != 1.f;
+          base[n][e] = to;
+        }
+        if (__any_sync(0xffffffffu, moved)) {  // some row of the warp has a new maximum
+          l[n][0] *= alpha[0], l[n][1] *= alpha[1];
+#pragma unroll
+          for (int m = 0; m < kMt; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][m][e] *= alpha[e & 1];
+        }
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float w0 = ex2_approx(s[n][u][2 * h] - from[0]), w1 = ex2_approx(s[n][u][2 * h + 1] - from[1]);
+            l[n][0] = fmaf(w0, sum_of[u][h], l[n][0]);
+            l[n][1] = fmaf(w1, sum_of[u][h], l[n][1]);
+            pf[n][u][h] = transposed(pack_f16x2(w0, w1));
+          }
+      }
+      // A key that a row does not see has weight 0, and 0 times a value that is no number (e4m3 has one; also past the end of
+      // the keys, where a page holds anything) would be NaN: such codes count as zeros here, and rows that see one are told.
+      auto values = [&](auto careful) {
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+#pragma unroll
+          for (int c = 0; c < kMt / 2; ++c) {
+            uint32_t w[4];
+            ldsm_x4_t(w, (sV + u * 16 * D + at_v) ^ (c * 32));
+            if constexpr (decltype(careful)::value) {
+              uint32_t nan[4], any = 0;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                nan[k] = (((w[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;  // 1 in each byte that is NaN
+                w[k] &= ~(nan[k] * 0xffu);
+                any |= nan[k];
+              }
+              if (__any_sync(0xffffffffu, any != 0)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                  uint32_t sees[2];
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    const int key = t0 + u * 16 + h * 8 + key_of<D>(g);
+                    sees[h] = transposed((key < lim[n][0] ? 0x3c00u : 0u) | (key < lim[n][1] ? 0x3c000000u : 0u));
+                  }
+#pragma unroll
+                  for (int m = 0; m < 2; ++m) {
+                    // (0x3c00 is 1 in f16)
+                    const uint32_t f[4] = {(nan[2 * m] & 0x10001u) * 0x3c00u, ((nan[2 * m] >> 8) & 0x10001u) * 0x3c00u,
+                                           (nan[2 * m + 1] & 0x10001u) * 0x3c00u, ((nan[2 * m + 1] >> 8) & 0x10001u) * 0x3c00u};
+                    float count[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma_f16(count, f, sees);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                      if (count[e] > 0.f) o[n][2 * c + m][e] = NAN;
+                  }
+                }
+              }
+            }
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+              uint32_t f[4];
+              widen<kFloat>(w[2 * m], f[0], f[1]);
+              widen<kFloat>(w[2 * m + 1], f[2], f[3]);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * c + m], f, pf[n][u]);
+            }
+          }
+      };
+      if (kFloat && masked)
+        values(std::bool_constant<kFloat>{});
+      else
+        values(std::false_type{});
+      __syncwarp();
+      issue();
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float sum = l[n][e];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        const int r = n * 8 + 2 * t + e;
+        if (r >= p.n_rows) continue;
+        const long long out = out_of(r);
+#pragma unroll
+        for (int m = 0; m < kMt; ++m)
+          *reinterpret_cast<float2*>(a.part_o + out * D + m * 16 + 2 * g) = make_float2(o[n][m][e], o[n][m][2 + e]);
+        if (g == 0) a.part_ml[out] = make_float2(base[n][e], sum * 3.0517578125e-5f);  // 2^-15
+      }
+  }
+  // The block does not end before its last copies have arrived, also where a wait was given up.
+  for (int k = max(0, issued - kStages); k < issued; ++k) mbar_wait(bar0 + 8 * (k % kStages), (k / kStages) & 1, nullptr);
+  if (a.sound && blockIdx.x == 0 && warp == 0) {
+    const bool sound = offsets_sound(a, q_offsets);
+    if (lane == 0) {
+      *a.sound = sound;
+      if (!sound) flag(a);
+    }
+  }
+}
+
+// A pool of codes as (head_dim, heads, tokens, pages) in boxes of up to `tokens` of one page and head.
+static bool codes_map(CUtensorMap* map, const uint8_t* base, const Args& a, int head_dim, int tokens) {
+  if (!encode_fn()) return false;
+  const int page = 1 << a.page_shift;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(a.kv_heads),
+                              static_cast<cuuint64_t>(page), static_cast<cuuint64_t>(std::max(1, a.pages))};
+  // an axis of one entry may have any stride: give the map one that it accepts
+  auto stride = [](long long n, long long ld) { return static_cast<cuuint64_t>(n > 1 ? ld : 16); };
+  const cuuint64_t strides[3] = {stride(a.kv_heads, a.head_ld), stride(page, a.token_ld), stride(a.pages, a.page_ld)};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(head_dim), 1, static_cast<cuuint32_t>(std::min(page, tokens)), 1};
+  const cuuint32_t each[4] = {1, 1, 1, 1};
+  const CUtensorMapSwizzle swizzle = head_dim == 32 ? CU_TENSOR_MAP_SWIZZLE_32B
+                                     : head_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+  return encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t*>(base), dims, strides, box, each,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, int NT, bool kFloat>
+static cudaError_t launch(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
+  using R = Ring<D>;
+  const int known = a.own_splits > 0 && a.batch <= 1024 ? a.batch : 0;
+  const int bytes = kWarps * R::bytes + (known ? (2 * known + 1) * 4 : 0) + 1024;
+  const int items = (a.tensor_cores ? 0 : a.row_tiles * a.kv_heads * a.prefix_splits) + a.batch * a.own_tiles * a.own_splits * a.kv_heads;
+  static SharedMemory allowed;
+  if (const cudaError_t e = allowed.at_least(reinterpret_cast<const void*>(pieces8_kernel<D, NT, kFloat>), bytes); e != cudaSuccess) return e;
+  const int per_sm = std::max(1, std::min(R::blocks, 227 * 1024 / (bytes + 1024 + 512)));
+  pieces8_kernel<D, NT, kFloat><<<std::min(items, 148 * per_sm), kThreads, bytes, stream>>>(a, mk, mv, items, known);
+  return cudaGetLastError();
+}
+
+template <int D>
+static cudaError_t launch_for(const Args& a, cudaStream_t stream) {
+  CUtensorMap mk, mv;
+  if (!codes_map(&mk, a.k8, a, D, kStep) || !codes_map(&mv, a.v8, a, D, kStep)) return cudaErrorInvalidValue;
+  if (a.codes == kE4m3) return a.tile_rows == 8 ? launch<D, 1, true>(a, mk, mv, stream) : launch<D, 2, true>(a, mk, mv, stream);
+  return a.tile_rows == 8 ? launch<D, 1, false>(a, mk, mv, stream) : launch<D, 2, false>(a, mk, mv, stream);
+}
+
+}  // namespace q8
+
+cudaError_t launch_pieces8(const Args& a, int head_dim, cudaStream_t stream) {
+  switch (head_dim) {
+    case 32: return q8::launch_for<32>(a, stream);
+    case 64: return q8::launch_for<64>(a, stream);
+    default: return q8::launch_for<128>(a, stream);
+  }
+}
+
+int plan8(Args& a, int head_dim) {
+  using q8::kStep;
+  // Pieces until every warp has about three.
+  const int want = 148 * q8::kWarps * (head_dim == 128 ? 2 : 4) * 3;
+  a.prefix_splits = a.own_splits = 0;
+  a.quad = a.tensor_cores = false;
+  const long long rows = static_cast<long long>(a.n) * a.group;
+  const long long most = a.prefix_len > 0 ? std::max(rows, static_cast<long long>(a.max_q) * a.group) : static_cast<long long>(a.max_q) * a.group;
+  a.tile_rows = most <= 8 ? 8 : 16;
+  if (a.prefix_len > 0) {
+    a.row_tiles = ceil_div(rows, a.tile_rows);
+    const int tiles = ceil_div(a.prefix_len, kStep);
+    const int splits = std::max(1, std::min({tiles, 64, ceil_div(want, static_cast<long long>(a.row_tiles) * a.kv_heads)}));
+    a.prefix_chunk = ceil_div(tiles, splits) * kStep;
+    a.prefix_splits = ceil_div(a.prefix_len, a.prefix_chunk);
+  }
+  if (a.max_len > 0 && a.max_q > 0 && a.batch > 0) {
+    a.own_tiles = ceil_div(static_cast<long long>(a.max_q) * a.group, a.tile_rows);
+    const int tiles = ceil_div(a.max_len, kStep);
+    const int splits = std::max(1, std::min({tiles, 64, ceil_div(want, static_cast<long long>(a.batch) * a.own_tiles * a.kv_heads)}));
+    a.own_chunk = ceil_div(tiles, splits) * kStep;
+    a.own_splits = ceil_div(a.max_len, a.own_chunk);
+  }
+  return a.prefix_splits + a.own_splits;
+}
+
+}  // namespace prefix
+
+}  // namespace mnb

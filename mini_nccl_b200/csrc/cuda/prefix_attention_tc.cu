@@ -34,9 +34,8 @@
 // (head_dim, heads, tokens, pages) into a ring of 128-byte-swizzled stages, in
 // the order in which the products use them.  The MMA warp zeroes V rows past
 // the prefix's end (pages hold anything there); keys past it are masked.
-#include "common.cuh"
-#include "generation.h"
 #include "launch.cuh"
+#include "prefix_attention.cuh"
 #include "warp_mma.cuh"
 
 namespace mnb {
@@ -65,12 +64,6 @@ struct Smem {
 };
 
 MNB_DEVICE void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-MNB_DEVICE void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
-      : "memory");
-}
 // 2^x of a pair on the FMA and integer pipes.  x = n + f with n the nearest whole number (adding and subtracting
 // 1.5 * 2^23 rounds to it; shifted left by 23 the sum's bits are n in the exponent's place, the rest shifted out) and
 // 2^f from 1 + c1 f + ... + c5 f^5, a least-squares fit of the relative error on [-1/2, 1/2] reweighted until level

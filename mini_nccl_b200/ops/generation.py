@@ -3,12 +3,19 @@
 * :func:`shared_prefix_attention` -- attention of new tokens over a prefix that
   the whole batch shares (computed once for all rows) and over each
   sequence's own tokens, both in a paged cache;
+* :func:`adjust_logits` -- penalties for repeated tokens, biases and masks (of a
+  grammar) on logits, before :func:`sample`;
 * :func:`sample` -- temperature, top-k, top-p and min-p sampling from given
   random numbers;
 * :func:`append_kv`, :func:`copy_pages`, :func:`fork_sequences`,
   :func:`reserve_pages`, :func:`free_sequences`, :func:`compact_pages` -- the
   page operations, and :class:`PagedKVCache`, which holds the tensors they
   work on.
+
+A cache is held in bf16, or in 8 bits: codes (int8 or float8_e4m3fn) and one
+fp32 scale for each page and kv head, a power of two.  A code stands for
+``code * scale``; :func:`append_kv` chooses the scales, and the functions that
+take pages take the scales with them.
 
 As in :mod:`mini_nccl_b200.ops.functional`, a CUDA tensor runs the sm_100a
 kernel (and raises where the extension is missing), a CPU tensor the plain
@@ -51,6 +58,38 @@ def _ints(t: torch.Tensor, dim: int, what: str) -> None:
     _need(t.dtype == torch.int32 and t.dim() == dim, f"{what}: a {dim}-d int32 tensor")
 
 
+#: The largest code of each type that an 8-bit cache may have.
+TOP_CODE = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
+_LEAST_EXPONENT = -60  # of a scale
+
+
+def _held_in_8_bits(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor | None, v_scales: torch.Tensor | None) -> bool:
+    _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.dtype == v_pages.dtype,
+          "k_pages and v_pages: [num_pages, page_size, kv_heads, head_dim] of one type")
+    coded = k_pages.dtype in TOP_CODE
+    _need((k_scales is not None and v_scales is not None) if coded else (k_scales is None and v_scales is None),
+          "k_scales and v_scales: needed with pages of int8 or float8_e4m3fn, and only with them")
+    for s in (k_scales, v_scales):
+        _need(s is None or (s.dtype == torch.float32 and s.shape == (k_pages.shape[0], k_pages.shape[2])),
+              "k_scales and v_scales: fp32 tensors [num_pages, kv_heads]")
+    return coded
+
+
+def _values(pages: torch.Tensor, scales: torch.Tensor | None, ids: torch.Tensor) -> torch.Tensor:
+    """What the pages ``ids`` hold, in fp32 (CPU)."""
+    if scales is None:
+        return pages[ids].float()
+    return pages.view(torch.uint8)[ids].view(pages.dtype).float() * scales[ids][:, None, :, None]
+
+
+def _code(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """The nearest code to each of ``x``, of two the even one (CPU)."""
+    top = TOP_CODE[dtype]
+    if dtype == torch.int8:
+        return torch.round(x.clamp(-top, top)).to(torch.int8)
+    return x.clamp(-top, top).to(dtype)
+
+
 class _NoGradient(torch.autograd.Function):
     """A kernel's result as a function of its inputs, for inputs that want a gradient: asking for it raises."""
 
@@ -81,6 +120,8 @@ def shared_prefix_attention(
     max_seq_len: int | None = None,
     scale: float | None = None,
     return_lse: bool = False,
+    k_scales: torch.Tensor | None = None,
+    v_scales: torch.Tensor | None = None,
 ) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
     """``softmax(scale q k^T) v`` over a shared prefix and each sequence's own tokens.
 
@@ -98,6 +139,13 @@ def shared_prefix_attention(
     log-sum-exp of ``-inf``.  ``max_seq_len`` bounds ``seq_lens`` (default:
     what ``page_table`` can hold); a tight bound means fewer idle blocks.
 
+    Pages of int8 or float8_e4m3fn come with ``k_scales`` and ``v_scales``, fp32
+    ``[num_pages, kv_heads]`` of one layout: page p's keys of head h are
+    ``k_pages[p, :, h] * k_scales[p, h]``.  Scales are powers of two from
+    ``2 ** -60`` on (a smaller or no positive scale of values counts as
+    ``2 ** -60``), as :func:`append_kv` leaves them, or 0 where nothing was
+    written; others only cost accuracy.
+
     Returns ``o`` like ``q`` (contiguous) and, with ``return_lse``, the natural
     log-sum-exp of the scaled scores, fp32 ``[tokens, heads]``.  Head dims 32,
     64 and 128; page sizes 8 to 256, powers of two.
@@ -113,13 +161,14 @@ def shared_prefix_attention(
         K = _kernels()
         o, lse = K.ext().shared_prefix_attention(
             q, k_pages, v_pages, prefix_pages, prefix_len, page_table, seq_lens, q_offsets,
-            -1 if max_q_len is None else max_q_len, -1 if max_seq_len is None else max_seq_len, scale, return_lse,
+            -1 if max_q_len is None else max_q_len, -1 if max_seq_len is None else max_seq_len, scale, return_lse, k_scales, v_scales,
             K.status_word(q.device))
         if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
             o, lse = (None if t is None else _NoGradient.apply("shared_prefix_attention", t, q, k_pages, v_pages) for t in (o, lse))
         return (o, lse) if return_lse else o
     _need(q.dim() == 3 and k_pages.dim() == 4 and k_pages.shape == v_pages.shape,
           "q: [tokens, heads, head_dim]; k_pages and v_pages: [num_pages, page_size, kv_heads, head_dim]")
+    _held_in_8_bits(k_pages, v_pages, k_scales, v_scales)
     _ints(prefix_pages, 1, "prefix_pages")
     _ints(page_table, 2, "page_table")
     _ints(seq_lens, 1, "seq_lens")
@@ -149,7 +198,7 @@ def shared_prefix_attention(
     def tokens(ids: torch.Tensor, n: int) -> tuple[torch.Tensor, torch.Tensor]:
         if n and (int(ids.min()) < 0 or int(ids.max()) >= pages):
             raise RuntimeError("a page id outside the pool")
-        k, v = (p[ids.long()].reshape(-1, Hk, D)[:n].float().transpose(0, 1) for p in (k_pages, v_pages))
+        k, v = (_values(p, s, ids.long()).reshape(-1, Hk, D)[:n].transpose(0, 1) for p, s in ((k_pages, k_scales), (v_pages, v_scales)))
         return k, v
 
     o = torch.zeros(N, H, D, dtype=q.dtype)
@@ -272,15 +321,145 @@ def sample(
     return token, torch.where(token < 0, -math.inf, logprob)
 
 
+def adjust_logits(
+    logits: torch.Tensor,
+    *,
+    prompt: torch.Tensor | None = None,
+    history: torch.Tensor | None = None,
+    history_lens: torch.Tensor | None = None,
+    repetition: Setting = 1.0,
+    presence: Setting = 0.0,
+    frequency: Setting = 0.0,
+    bias_tokens: torch.Tensor | None = None,
+    bias: torch.Tensor | None = None,
+    allowed: torch.Tensor | None = None,
+    mask_of: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Penalties, biases and masks on ``logits`` ``[rows, vocabulary]`` (bf16 or fp32), for :func:`sample`.
+
+    With x the logit of token v in row r, and c the number of times that v is
+    among the row's ``history``, in this order and in fp32, rounded once:
+
+    * ``x = x / repetition`` if x is above 0, else ``x * repetition``, where v is
+      in the history or in the ``prompt``;
+    * ``x = x - (frequency * c + presence)`` where v is in the history;
+    * ``x = x + bias[r, i]`` where ``bias_tokens[r, i]`` is v (of a token that is
+      named twice the later one);
+    * ``x = -inf`` where the row's mask does not allow v.
+
+    ``history`` is ``[rows, n]``, its first ``history_lens`` (int32, one for each
+    row; default all) tokens counting; ``prompt`` ``[rows, n]``, or ``[n]`` for
+    all rows, as are ``bias_tokens`` and ``bias`` (fp32).  Tokens are int64 or
+    int32; negative ones are padding.  ``repetition`` (above 0), ``presence`` and
+    ``frequency`` are numbers or fp32 tensors with one entry for each row.
+    ``allowed`` holds masks, int32 ``[masks, (vocabulary + 31) // 32]``: bit
+    ``v % 32`` of word ``v // 32`` allows token v.  Row r has mask
+    ``mask_of[r]`` (int32, a negative one is no mask); without ``mask_of`` mask r,
+    or the only one.
+
+    Returns a new tensor, or ``out``, which may be ``logits`` itself (then tokens
+    that nothing names are neither read nor written) but no other memory that
+    overlaps it.  A token or a mask that there is none of, and a length outside
+    the history (the history then counts for nothing), are reported.
+    """
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if logits.is_cuda:
+
+        def split(x):
+            return (x, 0.0) if isinstance(x, torch.Tensor) else (None, float(x))
+
+        K = _kernels()
+        given = (logits, *(t for t in (repetition, presence, frequency, bias) if isinstance(t, torch.Tensor)))
+        wanted = torch.is_grad_enabled() and any(t.requires_grad for t in given)
+        _need(not (wanted and out is logits), "out: not in place where a gradient is wanted")
+        K.ext().adjust_logits(logits, out, prompt, history, history_lens, *split(repetition), *split(presence), *split(frequency),
+                              bias_tokens, bias, allowed, mask_of, K.status_word(logits.device))
+        return _NoGradient.apply("adjust_logits", out, *given) if wanted else out
+    _need(logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32),
+          "logits: a bf16 or fp32 tensor [rows, vocabulary]")
+    R, V = logits.shape
+    _need(1 <= V <= 1 << 20, f"vocabulary: 1 to 1048576 tokens, got {V}")
+    _need(out.shape == logits.shape and out.dtype == logits.dtype, "out: a tensor like logits")
+
+    def column(x, what):
+        if isinstance(x, torch.Tensor):
+            _need(x.dtype == torch.float32 and x.shape == (R,), f"{what}: a number, or an fp32 tensor with one entry for each row")
+            return x[:, None]
+        return torch.full((R, 1), float(x))
+
+    def listed(t, shared, what):
+        _need(t.dtype in (torch.int64, torch.int32) and ((t.dim() == 2 and t.shape[0] == R) or (shared and t.dim() == 1)),
+              f"{what}: int64 or int32 tokens [rows, n]" + (" or [n]" if shared else ""))
+        if t.numel() and int(t.max()) >= V:
+            raise RuntimeError(f"{what}: a token outside the vocabulary")
+        return t.long().expand(R, t.shape[-1])
+
+    rho, alpha, phi = column(repetition, "repetition"), column(presence, "presence"), column(frequency, "frequency")
+    count, seen = torch.zeros(R, V + 1), torch.zeros(R, V + 1, dtype=torch.bool)  # (the last one is padding's)
+    _need(history_lens is None or history is not None, "history_lens: needs history")
+    if history is not None:
+        ids = listed(history, False, "history")
+        _need(ids.shape[1] < 1 << 19, "history: at most 524287 tokens a row")
+        if history_lens is not None:
+            _ints(history_lens, 1, "history_lens")
+            _need(history_lens.shape[0] == R, "history_lens: one length for each row of history")
+            if R and (int(history_lens.min()) < 0 or int(history_lens.max()) > ids.shape[1]):
+                raise RuntimeError("history_lens: a length outside the history")
+            ids = torch.where(torch.arange(ids.shape[1]) < history_lens[:, None], ids, -1)
+        count.scatter_add_(1, torch.where(ids < 0, V, ids), torch.ones(ids.shape))
+    if prompt is not None:
+        ids = listed(prompt, True, "prompt")
+        seen.scatter_(1, torch.where(ids < 0, V, ids), True)
+    count, seen = count[:, :V], seen[:, :V]
+    x = logits.float()
+    x = torch.where((count > 0) | seen, torch.where(x > 0, x / rho, x * rho), x)
+    x = torch.where(count > 0, x - (phi * count + alpha), x)
+    _need((bias is None) == (bias_tokens is None), "bias_tokens and bias: one needs the other")
+    if bias is not None:
+        _need(bias.dtype == torch.float32 and bias.shape == bias_tokens.shape, "bias: fp32, of the tokens' shape")
+        ids = listed(bias_tokens, True, "bias_tokens")
+        _need(ids.shape[1] <= 4095, "bias_tokens: at most 4095 a row")
+        last = torch.full((R, V + 1), -1).scatter_reduce_(
+            1, torch.where(ids < 0, V, ids), torch.arange(ids.shape[1]).expand(R, -1), "amax")[:, :V]
+        if ids.shape[1]:
+            x = torch.where(last >= 0, x + bias.expand(R, -1).gather(1, last.clamp(min=0)), x)
+    _need(mask_of is None or allowed is not None, "mask_of: needs allowed")
+    if allowed is not None:
+        _ints(allowed, 2, "allowed")
+        _need(allowed.shape[1] == -(-V // 32), f"allowed: {-(-V // 32)} words of 32 tokens a mask")
+        if mask_of is None:
+            _need(allowed.shape[0] in (1, R), "allowed: without mask_of one mask, or one for each row")
+            of = torch.arange(R) if allowed.shape[0] == R else torch.zeros(R, dtype=torch.long)
+        else:
+            _ints(mask_of, 1, "mask_of")
+            _need(mask_of.shape[0] == R, "mask_of: one mask for each row")
+            of = mask_of.long()
+            if R and int(of.max()) >= allowed.shape[0]:
+                raise RuntimeError("mask_of: a mask that there is none of")
+        if allowed.shape[0]:
+            v = torch.arange(V)
+            bits = (allowed[of.clamp(min=0)][:, v // 32] >> (v % 32).int()) & 1
+            x = torch.where((bits != 0) | (of < 0)[:, None], x, -math.inf)
+    return out.copy_(x)
+
+
 # ---- pages ---------------------------------------------------------------------------
 
 
-def _pool(kv: torch.Tensor) -> torch.Tensor:
-    """The pool as ``[planes, num_pages, page_size, kv_heads, head_dim]``."""
+def _pool(kv: torch.Tensor, scales: torch.Tensor | None = None) -> tuple[torch.Tensor, ...]:
+    """The pool as ``[planes, num_pages, page_size, kv_heads, head_dim]``, and its scales, if any, as ``[planes, num_pages, kv_heads]``."""
     _need(kv.dim() >= 4 and kv.is_contiguous() and kv.numel() > 0,
           "kv: a contiguous tensor [..., num_pages, page_size, kv_heads, head_dim]")
     _need(kv.shape[-1] * kv.shape[-2] * kv.element_size() % 16 == 0, "kv: a token's keys must be a multiple of 16 bytes")
-    return kv.view(-1, *kv.shape[-4:])
+    if kv.dtype == torch.float8_e4m3fn:
+        kv = kv.view(torch.uint8)
+    if scales is None:
+        return (kv.view(-1, *kv.shape[-4:]),)
+    _need(scales.dtype == torch.float32 and scales.is_contiguous() and scales.shape == (*kv.shape[:-3], kv.shape[-2]),
+          "scales: a contiguous fp32 tensor [..., num_pages, kv_heads] with the leading axes of kv")
+    return kv.view(-1, *kv.shape[-4:]), scales.view(-1, *scales.shape[-2:])
 
 
 def _state(page_table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor) -> None:
@@ -309,6 +488,9 @@ def append_kv(
     page_table: torch.Tensor,
     positions: torch.Tensor,
     slots: torch.Tensor | None = None,
+    *,
+    k_scales: torch.Tensor | None = None,
+    v_scales: torch.Tensor | None = None,
 ) -> None:
     """Write the keys and values of tokens into their sequences' pages.
 
@@ -316,13 +498,28 @@ def append_kv(
     ``positions[i]`` of the sequence in row ``slots[i]`` of ``page_table`` (row
     i without ``slots``); a negative position is padding and is left out.  The
     pages have to be there (:func:`reserve_pages`) and must not be shared.
+
+    Pages of int8 or float8_e4m3fn come with ``k_scales`` and ``v_scales``, fp32
+    ``[num_pages, kv_heads]``, which are written too.  A page's values of one
+    head share a scale, the least power of two (from ``2 ** -60`` on) whose
+    multiple by the largest code (127 or 448) is at least the largest of them;
+    each value becomes the nearest code, of two the even one.  Writing a page's
+    first place begins the page: its scale then comes from this call's tokens
+    alone.  Otherwise the scale only grows, and the codes that are there are
+    rounded to the new one.  Values that are not finite do not count for the
+    scale; an infinite one is stored as the largest code, NaN as float8_e4m3fn's
+    NaN, or as int8 zero (and reported).  In a call the tokens of one page follow
+    one another (padding aside), in any order; a place that is named twice gets
+    the later one.  Head dims that are multiples of 16, up to 256.
     """
     if k_pages.is_cuda:
         K = _kernels()
-        K.ext().append_kv(k_pages, v_pages, k, v, page_table, positions, slots, K.status_word(k_pages.device))
+        K.ext().append_kv(k_pages, v_pages, k, v, page_table, positions, slots, k_scales, v_scales, K.status_word(k_pages.device))
         return
     _need(k_pages.dim() == 4 and v_pages.shape == k_pages.shape and k.shape == v.shape and k.dim() == 3
           and k.shape[1:] == k_pages.shape[2:], "k, v: [tokens, kv_heads, head_dim] as in the pages")
+    coded = _held_in_8_bits(k_pages, v_pages, k_scales, v_scales)
+    _need(not coded or (k.shape[2] % 16 == 0 and k.shape[2] <= 256), "head_dim: in 8 bits a multiple of 16, at most 256")
     _ints(page_table, 2, "page_table")
     named = [(positions, "positions")] + ([(slots, "slots")] if slots is not None else [])
     where = _ids(*named)
@@ -330,34 +527,63 @@ def append_kv(
     _need(slots is not None or k.shape[0] <= page_table.shape[0],
           "without slots, token i belongs to row i of page_table: too many tokens")
     page, rows = k_pages.shape[1], page_table.tolist()
+    runs: list[tuple[int, dict[int, int], list[int]]] = []  # a page, which token its places get, and all that the call has for it
     for i, pos in enumerate(where[0]):
         if pos < 0:
             continue
         s = where[1][i] if slots is not None else i
         if not (0 <= s < len(rows) and pos // page < len(rows[s]) and 0 <= rows[s][pos // page] < k_pages.shape[0]):
             raise RuntimeError(f"token {i}: no page for place {pos} of sequence {s}")
-        k_pages[rows[s][pos // page], pos % page] = k[i]
-        v_pages[rows[s][pos // page], pos % page] = v[i]
+        if not coded:
+            k_pages[rows[s][pos // page], pos % page] = k[i]
+            v_pages[rows[s][pos // page], pos % page] = v[i]
+            continue
+        if not runs or runs[-1][0] != rows[s][pos // page]:
+            _need(all(r[0] != rows[s][pos // page] for r in runs), "positions: in 8 bits, a page's tokens follow one another")
+            runs.append((rows[s][pos // page], {}, []))
+        runs[-1][1][pos % page] = i
+        runs[-1][2].append(i)
+    if coded and k_pages.dtype == torch.int8 and any(bool(x[r[2]].isnan().any()) for r in runs for x in (k, v)):
+        raise RuntimeError("NaN cannot be held as int8")
+    for p, places, tokens in runs:
+        for pages, scales, x in ((k_pages, k_scales, k.float()), (v_pages, v_scales, v.float())):
+            most = torch.where(x[tokens].isfinite(), x[tokens].abs(), 0.0).amax((0, 2))
+            m, e = torch.frexp(most)
+            top, shift = math.frexp(TOP_CODE[pages.dtype])
+            e = torch.where(most > 0, e - shift + (m > top).int(), _LEAST_EXPONENT).clamp(min=_LEAST_EXPONENT)
+            held = torch.zeros_like(scales[p]) if 0 in places else scales[p].clone()
+            need = torch.ldexp(torch.ones_like(held), e)
+            now = torch.where(held > need, held, need)
+            if 0 not in places:
+                ratio = torch.where(held > 0, held / now, 0.0)[:, None]
+                again = _code(pages[p].float() * ratio, pages.dtype)
+                pages.view(torch.uint8)[p] = torch.where((now != held)[:, None], again.view(torch.uint8), pages[p].view(torch.uint8))
+            scales[p] = now
+            code = _code(x[list(places.values())] / now[:, None], pages.dtype)
+            pages.view(torch.uint8)[p, list(places)] = code.view(torch.uint8)
 
 
-def copy_pages(kv: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
+def copy_pages(kv: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, scales: torch.Tensor | None = None) -> None:
     """Copy page ``src[i]`` to page ``dst[i]`` in every plane of ``kv``.
 
     ``kv`` is ``[..., num_pages, page_size, kv_heads, head_dim]``, of any
     dtype; the leading axes are the planes.  Pairs with a negative id are left
-    out; no destination may be named twice or be a source as well.
+    out; no destination may be named twice or be a source as well.  ``scales``,
+    fp32 ``[..., num_pages, kv_heads]``, are those of a cache in 8 bits and go
+    with their pages (here and in the functions below).
     """
     if kv.is_cuda:
         K = _kernels()
-        K.ext().copy_pages(kv, src, dst, K.status_word(kv.device))
+        K.ext().copy_pages(kv, src, dst, scales, K.status_word(kv.device))
         return
-    pool = _pool(kv)
+    pools = _pool(kv, scales)
     for a, b in zip(*_ids((src, "src"), (dst, "dst"))):
         if a < 0 or b < 0:
             continue
-        if max(a, b) >= pool.shape[1]:
+        if max(a, b) >= pools[0].shape[1]:
             raise RuntimeError("a page id outside the pool")
-        pool[:, b] = pool[:, a]
+        for pool in pools:
+            pool[:, b] = pool[:, a]
 
 
 def fork_sequences(
@@ -367,6 +593,7 @@ def fork_sequences(
     refs: torch.Tensor,
     parents: torch.Tensor,
     children: torch.Tensor,
+    scales: torch.Tensor | None = None,
 ) -> None:
     """Make the empty sequence ``children[i]`` a copy of sequence ``parents[i]``.
 
@@ -380,9 +607,9 @@ def fork_sequences(
     """
     if kv.is_cuda:
         K = _kernels()
-        K.ext().fork_sequences(kv, page_table, lens, refs, parents, children, K.status_word(kv.device))
+        K.ext().fork_sequences(kv, page_table, lens, refs, parents, children, scales, K.status_word(kv.device))
         return
-    pool = _pool(kv)
+    pool, *of_scales = _pool(kv, scales)
     _state(page_table, lens, refs)
     _need(refs.shape[0] == pool.shape[1], "refs: one count for each page of kv")
     ps, cs = _ids((parents, "parents"), (children, "children"))
@@ -405,6 +632,8 @@ def fork_sequences(
         if part:
             row[full] = free.pop(0)
             pool[:, row[full], :part] = pool[:, page_table[p, full], :part]
+            for t in of_scales:
+                t[:, row[full]] = t[:, page_table[p, full]]
             refs[row[full]] = 1
         page_table[c], lens[c] = row, lens[p]
 
@@ -470,7 +699,7 @@ def free_sequences(page_table: torch.Tensor, lens: torch.Tensor, refs: torch.Ten
 
 
 def compact_pages(
-    kv: torch.Tensor, page_table: torch.Tensor, refs: torch.Tensor
+    kv: torch.Tensor, page_table: torch.Tensor, refs: torch.Tensor, scales: torch.Tensor | None = None
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Move the pages in use to the front of the pool; returns the new ``(page_table, refs)``.
 
@@ -480,15 +709,16 @@ def compact_pages(
     """
     if kv.is_cuda:
         K = _kernels()
-        return K.ext().compact_pages(kv, page_table, refs, K.status_word(kv.device))
-    pool = _pool(kv)
+        return K.ext().compact_pages(kv, page_table, refs, scales, K.status_word(kv.device))
+    pool, *of_scales = _pool(kv, scales)
     _ints(page_table, 2, "page_table")
     _ints(refs, 1, "refs")
     _need(refs.shape[0] == pool.shape[1], "refs: one count for each page of kv")
     live = refs > 0
     n, at = int(live.sum()), torch.arange(refs.shape[0])
     src, dst = at[live & (at >= n)], at[~live & (at < n)]
-    pool[:, dst] = pool[:, src]
+    for t in (pool, *of_scales):
+        t[:, dst] = t[:, src]
     to = torch.where(live, at, -1)
     to[src] = dst
     moved = torch.zeros_like(refs)
@@ -514,6 +744,7 @@ class PagedKVCache:
         _need(8 <= page_size <= 256 and page_size & (page_size - 1) == 0, "page_size: a power of two from 8 to 256")
         self.page_size = page_size
         self.kv = torch.zeros(n_layer, 2, num_pages, page_size, n_kv_head, head_dim, dtype=dtype, device=device)
+        self.scales = torch.zeros(n_layer, 2, num_pages, n_kv_head, device=device) if dtype in TOP_CODE else None
         ints = dict(dtype=torch.int32, device=device)
         self.page_table = torch.full((max_seqs, -(-max_seq_len // page_size)), -1, **ints)
         self.lens = torch.zeros(max_seqs, **ints)
@@ -543,7 +774,11 @@ class PagedKVCache:
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
                slots: torch.Tensor | None = None) -> None:
         """Keys and values of one layer, for places that :meth:`extend` made (see :func:`append_kv`)."""
-        append_kv(self.kv[layer, 0], self.kv[layer, 1], k, v, self.page_table, positions, slots)
+        append_kv(self.kv[layer, 0], self.kv[layer, 1], k, v, self.page_table, positions, slots, **self.scales_of(layer))
+
+    def scales_of(self, layer: int) -> dict[str, torch.Tensor]:
+        """One layer's scales as the operators' arguments (none for a cache that has none)."""
+        return {} if self.scales is None else {"k_scales": self.scales[layer, 0], "v_scales": self.scales[layer, 1]}
 
     def fork(self, parents: Sequence[int], children: Sequence[int]) -> None:
         """Each child, an empty slot, becomes a copy of its parent (see :func:`fork_sequences`)."""
@@ -554,7 +789,8 @@ class PagedKVCache:
               "children: one for each parent, distinct, empty and nobody's parent")
         if not children:
             return
-        fork_sequences(self.kv, self.page_table, self.lens, self.refs, self._tensor(parents), self._tensor(children))
+        fork_sequences(self.kv, self.page_table, self.lens, self.refs, self._tensor(parents), self._tensor(children),
+                       self.scales)
         for p, c in zip(parents, children):
             self.lengths[c] = self.lengths[p]
 
@@ -569,7 +805,7 @@ class PagedKVCache:
 
     def compact(self) -> None:
         """Move the pages in use to the front of the pool (see :func:`compact_pages`)."""
-        self.page_table, self.refs = compact_pages(self.kv, self.page_table, self.refs)
+        self.page_table, self.refs = compact_pages(self.kv, self.page_table, self.refs, self.scales)
 
     def pages_in_use(self) -> int:
         """Number of pages that some sequence holds (waits for the device)."""

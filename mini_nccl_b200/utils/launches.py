@@ -43,7 +43,7 @@ KERNELS_PER_CALL = {
 
 # Entry points whose number of kernels depends on the call: the extension says how many the last one launched.
 ASKED = {"copy_pages", "fork_sequences", "reserve_pages", "free_sequences", "compact_pages", "append_kv", "sample",
-         "shared_prefix_attention"}
+         "shared_prefix_attention", "adjust_logits"}
 
 
 def add(n: int) -> None:
