@@ -73,7 +73,8 @@ MNB_DEVICE uint32_t rescaled(uint32_t w, float by) {
 
 }  // namespace
 
-template <bool kFloat>
+// kKeep: 16-byte parts of tokens that a lane keeps between the two looks at them.
+template <bool kFloat, int kKeep>
 __global__ void __launch_bounds__(32 * kWarps) append8_kernel(const __grid_constant__ Append8 a, int window, int* status) {
   constexpr int kTop = kFloat ? 8 : 6;                        // the largest code is kMantissa 2^kTop
   constexpr uint32_t kMantissa = kFloat ? 0x600000 : 0x7e0000;  // 448 = 1.75 * 2^8, 127 = 1.984375 * 2^6
@@ -137,25 +138,60 @@ __global__ void __launch_bounds__(32 * kWarps) append8_kernel(const __grid_const
         if (end) return;
       }
     };
-    uint32_t most = 0;  // of the finite values, as bits
-    bool anew = false;  // the first place is written: the page begins
+    // The run: how far it goes, whether it has the page's first place, and whether it is nothing but places one after another.
+    long long end = i0;
+    bool anew = false, plain = true;
+    const int at0 = __shfl_sync(0xffffffffu, place, of);
     run([&](long long c0, int count, int q, int at) {
+      end = c0 + count;
       anew = anew || __any_sync(0xffffffffu, lane < count && q == p && at == 0);
-#pragma unroll 4
-      for (int b = 0; b < count; b += together) {
-        const int j = b + token;
-        const bool in = token < together && j < count;
-        const int of_page = __shfl_sync(0xffffffffu, q, min(j, 31));
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (in && of_page == p) w = ld_v4(x + (c0 + j) * x_ld + chunk);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t v = (&w.x)[e], lo = v & 0x7fffu, hi = v >> 16 & 0x7fffu;
-          most = max(most, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
-        }
-      }
+      plain = plain && __all_sync(0xffffffffu, lane >= count || (q == p && at == at0 + c0 + lane - i0));
     });
-    most = __reduce_max_sync(0xffffffffu, most) << 16;
+    const int count = static_cast<int>(end - i0);
+    // The tokens in rounds of kKeep for each lane; those of the last round stay in registers (for pages of 32 tokens and head
+    // dim 128 that is all of them).
+    uint4 w[kKeep];
+    auto load = [&](int from) {
+#pragma unroll
+      for (int r = 0; r < kKeep; ++r) {
+        const int j = from + r * together + token;
+        w[r] = make_uint4(0, 0, 0, 0);
+        if (token < together && j < count) w[r] = ld_v4(x + (i0 + j) * x_ld + chunk);
+      }
+    };
+    auto largest = [&](uint32_t m) {  // of both halves of a word, with every lane's
+      m = max(m & 0xffffu, m >> 16);
+      return __reduce_max_sync(0xffffffffu, m);
+    };
+    const int round = kKeep * together, last = count > 0 ? (count - 1) / round * round : 0;
+    uint32_t most = 0;  // pairs, as bits
+    if (plain)
+      for (int from = 0; from <= last; from += round) {
+        load(from);
+#pragma unroll
+        for (int r = 0; r < kKeep; ++r)
+          most = __vmaxu2(most, __vmaxu2(__vmaxu2(w[r].x & 0x7fff7fffu, w[r].y & 0x7fff7fffu), __vmaxu2(w[r].z & 0x7fff7fffu, w[r].w & 0x7fff7fffu)));
+      }
+    most = largest(most);
+    if (!plain || most >= 0x7f80u) {  // padding in between, or something that is no finite number, which does not count
+      plain = false;
+      most = 0;
+      run([&](long long c0, int n, int q, int at) {
+        for (int b = 0; b < n; b += together) {
+          const int j = b + token;
+          const int of_page = __shfl_sync(0xffffffffu, q, min(j, 31));
+          if (token >= together || j >= n || of_page != p) continue;
+          const uint4 u = ld_v4(x + (c0 + j) * x_ld + chunk);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t v = (&u.x)[e], lo = v & 0x7fffu, hi = v >> 16 & 0x7fffu;
+            most = max(most, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+          }
+        }
+      });
+      most = largest(most);
+    }
+    most <<= 16;
     const int e = max(static_cast<int>(most >> 23) - 127 - kTop + ((most & 0x7fffff) > kMantissa), -60);
     const float need = __int_as_float((e + 127) << 23);
     float* const scale_at = scales + p * a.scale_ld;
@@ -166,43 +202,47 @@ __global__ void __launch_bounds__(32 * kWarps) append8_kernel(const __grid_const
       for (int b = 0; b < a.page_size; b += together) {
         if (token >= together || b + token >= a.page_size) continue;
         uint2* const c = reinterpret_cast<uint2*>(to + (b + token) * a.token_ld + chunk);
-        const uint2 w = *c;
-        *c = make_uint2(rescaled<kFloat>(w.x, by), rescaled<kFloat>(w.y, by));
+        const uint2 u = *c;
+        *c = make_uint2(rescaled<kFloat>(u.x, by), rescaled<kFloat>(u.y, by));
       }
     }
     __syncwarp();  // (also: every lane has read the scale)
     if (lane == 0) *scale_at = now;
     const float by = 1.f / now;
-    run([&](long long c0, int count, int q, int at) {
-#pragma unroll 4
-      for (int b = 0; b < count; b += together) {
+    if (plain) {
+      for (int from = last; from >= 0; from -= round) {
+        if (from != last) load(from);
+#pragma unroll
+        for (int r = 0; r < kKeep; ++r) {
+          const int j = from + r * together + token;
+          if (token < together && j < count)
+            *reinterpret_cast<uint2*>(to + (at0 + j) * a.token_ld + chunk) =
+                make_uint2(codes_of<kFloat>(w[r].x, w[r].y, by), codes_of<kFloat>(w[r].z, w[r].w, by));
+        }
+      }
+      continue;
+    }
+    run([&](long long c0, int n, int q, int at) {
+      for (int b = 0; b < n; b += together) {
         const int j = b + token;
         const int of_page = __shfl_sync(0xffffffffu, q, min(j, 31)), of_place = __shfl_sync(0xffffffffu, at, min(j, 31));
-        bool in = token < together && j < count && of_page == p;
+        bool in = token < together && j < n && of_page == p;
         for (int d = 1; d < together; ++d) {  // a place that is named twice gets the later token
           const int other = __shfl_down_sync(0xffffffffu, in ? of_place : -1, d * lanes);
           if (token + d < together && other == of_place) in = false;
         }
         if (in) {
-          const uint4 w = ld_v4(x + (c0 + j) * x_ld + chunk);
-          uint2 c = make_uint2(codes_of<kFloat>(w.x, w.y, by), codes_of<kFloat>(w.z, w.w, by));
+          const uint4 u = ld_v4(x + (c0 + j) * x_ld + chunk);
+          uint2 c = make_uint2(codes_of<kFloat>(u.x, u.y, by), codes_of<kFloat>(u.z, u.w, by));
           if constexpr (!kFloat) {
-            bool odd = false;  // something that is no finite number
+            uint32_t code[8];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const uint32_t v = (&w.x)[k];
-              odd = odd || (v & 0x7f80u) == 0x7f80u || (v & 0x7f800000u) == 0x7f800000u;
+              const float2 v = unpack_bf16x2((&u.x)[k]);
+              if (v.x != v.x || v.y != v.y) atomicCAS(status, 0, kErrNotANumber);
+              code[2 * k] = nearest(within(v.x * by), 1.f), code[2 * k + 1] = nearest(within(v.y * by), 1.f);
             }
-            if (odd) {
-              uint32_t code[8];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float2 v = unpack_bf16x2((&w.x)[k]);
-                if (v.x != v.x || v.y != v.y) atomicCAS(status, 0, kErrNotANumber);
-                code[2 * k] = nearest(within(v.x * by), 1.f), code[2 * k + 1] = nearest(within(v.y * by), 1.f);
-              }
-              c = make_uint2(bytes_of(code[0], code[1], code[2], code[3]), bytes_of(code[4], code[5], code[6], code[7]));
-            }
+            c = make_uint2(bytes_of(code[0], code[1], code[2], code[3]), bytes_of(code[4], code[5], code[6], code[7]));
           }
           *reinterpret_cast<uint2*>(to + of_place * a.token_ld + chunk) = c;
         }
@@ -219,10 +259,9 @@ cudaError_t launch_append8(const Append8& a, int* status, cudaStream_t stream) {
   while (window < 32 && (a.n + window - 1ll) / window * a.heads * 2 > 148 * 48) window *= 2;
   const long long warps = (a.n + window - 1ll) / window * a.heads * 2;
   const unsigned blocks = static_cast<unsigned>((warps + kWarps - 1) / kWarps);
-  if (a.e4m3)
-    append8_kernel<true><<<blocks, 32 * kWarps, 0, stream>>>(a, window, status);
-  else
-    append8_kernel<false><<<blocks, 32 * kWarps, 0, stream>>>(a, window, status);
+  const auto kernel = a.e4m3 ? (window == 1 ? append8_kernel<true, 2> : append8_kernel<true, 16>)
+                             : (window == 1 ? append8_kernel<false, 2> : append8_kernel<false, 16>);
+  kernel<<<blocks, 32 * kWarps, 0, stream>>>(a, window, status);
   return cudaGetLastError();
 }
 

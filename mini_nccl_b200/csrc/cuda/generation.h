@@ -171,6 +171,7 @@ struct Args {
   bool quad;          // it takes four kv heads of a sequence at once
   int row_tiles, prefix_splits, prefix_chunk;
   int own_tiles, own_splits, own_chunk;
+  int least_share;  // of a cache in 8 bits, or 0: warps take equal shares of the keys instead of pieces of these chunks
   float* part_o;    // [pieces][n][heads][head_dim]
   float2* part_ml;  // [pieces][n][heads]: maximum (log2 units) and sum
   int* sound;  // or null, without q_offsets: whether they give every row to one sequence; if not, the rows of the own

@@ -8,11 +8,14 @@
 // in fp32, one IEEE operation after another, rounded once to the logits' type.
 //
 // Bound by the bytes of the logits, once in and once out.  A block takes a run of a
-// row's tokens, whose logits wait in registers while the tokens that the row names are
-// counted in shared memory (whole numbers, so their order does not matter): one word for
-// each token (its count, whether the prompt has it, and which bias it gets) and one bit,
-// by which the pass over the logits passes over the many tokens that nobody named.
-// Logits of tokens that the mask forbids are not read.
+// row's tokens: it copies their logits under the mask (those of tokens that the mask
+// forbids are not read), and then rewrites the few that the row's lists name.  For
+// that, one word of shared memory for each token counts it (whole numbers, so the order
+// does not matter), remembers whether the prompt has it and which bias it gets; whoever
+// takes the word out first writes the token.  Only words of named tokens are ever
+// touched.  (Penalties applied on the way, in the copying pass, cost every warp the
+// arithmetic of each of its lanes' tokens in turn: 512 x 50304 with 1300 tokens named in
+// a row, 63 us.)
 #include <algorithm>
 
 #include "common.cuh"
@@ -42,10 +45,13 @@ MNB_DEVICE float adjusted(float x, uint32_t named, float repetition, float prese
 
 // Groups of 16 bytes (8 or 4 tokens) of a row, kPer for each thread, one chunk for each block.
 template <bool kBf16, int kPer>
-__global__ void __launch_bounds__(kThreads) adjust_kernel(const __grid_constant__ Adjust a, int chunks) {
+__global__ void __launch_bounds__(kThreads, 5) adjust_kernel(const __grid_constant__ Adjust a, int chunks) {
   constexpr int kGroup = kBf16 ? 8 : 4, kSize = kBf16 ? 2 : 4, kTokens = kThreads * kPer * kGroup;
-  __shared__ uint32_t named[kTokens];
-  __shared__ uint32_t touched[kTokens / 32];
+  constexpr int kBatch = kPer < 4 ? kPer : 4;  // groups whose loads are under way together
+  constexpr int kList = 1024;
+  static_assert(kTokens <= 1 << 14, "a place's bits");
+  __shared__ uint32_t named[kTokens], list[kList];
+  __shared__ int listed;
   const int row = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
   const char* const in = static_cast<const char*>(a.in) + row * a.in_ld * kSize;
   char* const out = static_cast<char*>(a.out) + row * a.out_ld * kSize;
@@ -65,131 +71,152 @@ __global__ void __launch_bounds__(kThreads) adjust_kernel(const __grid_constant_
   const uint32_t* const mask = of >= 0 ? a.allowed + of * a.mask_ld : nullptr;
   const int words = (a.vocab + 31) / 32;
 
-  // token of the thread's group k, and which of its tokens exist and are allowed
-  auto token_of = [&](int k) { return first + (k * kThreads + static_cast<int>(threadIdx.x)) * kGroup; };
-  uint32_t allowed[kPer];
-#pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    const int v = token_of(k);
-    uint32_t bits = (1u << kGroup) - 1;
-    if (mask && v < a.vocab && v + kGroup > 0) {
-      const int at = max(v, 0), w = at >> 5;
-      const uint32_t lo = mask[w], hi = w + 1 < words && (at & 31) + kGroup > 32 ? mask[w + 1] : 0u;
-      bits = (__funnelshift_r(lo, hi, at & 31) << (at - v)) & bits;
+  // The tokens of the row's lists that lie in the chunk: place, list (0 history, 1 prompt, 2 biases) and, of a bias, which.
+  int held = static_cast<int>(a.history.n);
+  if (a.history_lens) {
+    held = a.history_lens[row];
+    if (held < 0 || held > a.history.n) {
+      if (threadIdx.x == 0) atomicCAS(a.status, 0, kErrBadIndex);
+      held = 0;
     }
-    allowed[k] = bits;
   }
-  uint4 x[kPer];
-  auto load = [&](int k) {
-    const int v = token_of(k);
-    if (in_aligned && v >= 0 && v + kGroup <= a.vocab) {
-      x[k] = ld_v4(in + static_cast<long long>(v) * kSize);
-      return;
-    }
-    x[k] = make_uint4(0, 0, 0, 0);
+  const int prompts = static_cast<int>(a.prompt.n), biases = static_cast<int>(a.bias_tokens.n);
+  const bool names = prompts > 0 || held > 0 || biases > 0;
+  auto scan = [&](const Ids& t, int n, uint32_t kind, auto f) {
+    constexpr int kAhead = 4;
+    for (int i0 = threadIdx.x; i0 < n; i0 += kAhead * kThreads) {
+      long long v[kAhead];
 #pragma unroll
-    for (int e = 0; e < kGroup; ++e)
-      if (v + e >= 0 && v + e < a.vocab) {
-        if constexpr (kBf16)
-          (&x[k].x)[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(in)[v + e]) << (e % 2 * 16);
-        else
-          (&x[k].x)[e] = reinterpret_cast<const uint32_t*>(in)[v + e];
+      for (int k = 0; k < kAhead; ++k) v[k] = i0 + k * kThreads < n ? id_at(t, row * t.ld + i0 + k * kThreads) : -1;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        if (v[k] >= a.vocab && chunk == 0) atomicCAS(a.status, 0, kErrBadIndex);
+        const long long at = v[k] - first;
+        if (v[k] >= 0 && v[k] < a.vocab && at >= 0 && at < kTokens) f(static_cast<uint32_t>(at) | kind << 14 | (kind == 2 ? i0 + k * kThreads : 0) << 16);
       }
+    }
   };
-  if (!a.in_place) {
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      x[k] = make_uint4(0, 0, 0, 0);
-      if (allowed[k] && token_of(k) < a.vocab) load(k);
-    }
-  }
-
-  float repetition = 1.f, presence = 0.f, frequency = 0.f;
-  const bool names = a.prompt.n > 0 || a.history.n > 0 || a.bias_tokens.n > 0;
+  auto scan_all = [&](auto f) {
+    scan(a.prompt, prompts, 1, f);
+    scan(a.history, held, 0, f);
+    scan(a.bias_tokens, biases, 2, f);
+  };
+  // (more of them than the list has room for are looked for again each time)
+  auto each = [&](auto f) {
+    const int n = listed;
+    if (n > kList) scan_all(f);
+    else
+      for (int i = threadIdx.x; i < n; i += kThreads) f(list[i]);
+  };
+  auto place = [](uint32_t x) { return x & 0x3fffu; };
+  auto kind = [](uint32_t x) { return x >> 14 & 3u; };
   if (names) {
-    repetition = a.repetition.each ? a.repetition.each[row] : a.repetition.all;
-    presence = a.presence.each ? a.presence.each[row] : a.presence.all;
-    frequency = a.frequency.each ? a.frequency.each[row] : a.frequency.all;
-    for (int i = threadIdx.x; i < kTokens / 4; i += kThreads) reinterpret_cast<uint4*>(named)[i] = make_uint4(0, 0, 0, 0);
-    for (int i = threadIdx.x; i < kTokens / 32; i += kThreads) touched[i] = 0;
-    int held = static_cast<int>(a.history.n);
-    if (a.history_lens) {
-      held = a.history_lens[row];
-      if (held < 0 || held > a.history.n) {
-        if (threadIdx.x == 0) atomicCAS(a.status, 0, kErrBadIndex);
-        held = 0;
-      }
-    }
+    if (threadIdx.x == 0) listed = 0;
     __syncthreads();
-    // f(place in the chunk, which one it is) for the tokens of a list
-    auto each = [&](const Ids& t, int n, auto f) {
-      for (int i = threadIdx.x; i < n; i += kThreads) {
-        const long long v = id_at(t, row * t.ld + i);
-        if (v >= a.vocab && chunk == 0) atomicCAS(a.status, 0, kErrBadIndex);
-        const long long at = v - first;
-        if (v < 0 || v >= a.vocab || at < 0 || at >= kTokens) continue;
-        f(static_cast<int>(at), i);
-        atomicOr(touched + (at >> 5), 1u << (at & 31));
-      }
-    };
-    if (a.bias_tokens.n > 0) {  // (the later one of a token that is named twice)
-      each(a.bias_tokens, static_cast<int>(a.bias_tokens.n), [&](int at, int i) { atomicMax(named + at, static_cast<uint32_t>(i + 1) << kBiasShift); });
+    scan_all([&](uint32_t x) {
+      named[place(x)] = 0;
+      const int i = atomicAdd(&listed, 1);
+      if (i < kList) list[i] = x;
+    });
+    __syncthreads();
+    if (biases > 0) {  // (the later one of a token that is named twice)
+      each([&](uint32_t x) {
+        if (kind(x) == 2) atomicMax(named + place(x), ((x >> 16) + 1) << kBiasShift);
+      });
       __syncthreads();
     }
-    each(a.prompt, static_cast<int>(a.prompt.n), [&](int at, int) { atomicOr(named + at, kPrompt); });
-    each(a.history, held, [&](int at, int) { atomicAdd(named + at, 1u); });
-    __syncthreads();
+    each([&](uint32_t x) {
+      if (kind(x) == 0) atomicAdd(named + place(x), 1u);
+      if (kind(x) == 1) atomicOr(named + place(x), kPrompt);
+    });
   }
-  const float* const bias = a.bias + row * a.bias_tokens.ld;
 
+  // The copy, under the mask
+  constexpr uint32_t kAll = (1u << kGroup) - 1;
+  if (!a.in_place || mask) {
+#pragma unroll 1
+    for (int b = 0; b < kPer; b += kBatch) {
+      auto token_of = [&](int k) { return first + ((b + k) * kThreads + static_cast<int>(threadIdx.x)) * kGroup; };
+      uint32_t allowed[kBatch];
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    const int v = token_of(k), at = v - first;
-    if (v >= a.vocab) continue;
-    const uint32_t here = names ? touched[at >> 5] >> (at & 31) & ((1u << kGroup) - 1) & allowed[k] : 0u;
-    const bool all = allowed[k] == (1u << kGroup) - 1;
-    if (a.in_place) {
-      if (all && !here) continue;
-      if (allowed[k]) load(k);
-    }
-    if (here) {
+      for (int k = 0; k < kBatch; ++k) {
+        const int v = token_of(k);
+        allowed[k] = kAll;
+        if (mask && v < a.vocab && v + kGroup > 0) {
+          const int at = max(v, 0), w = at >> 5;
+          const uint32_t lo = mask[w], hi = w + 1 < words && (at & 31) + kGroup > 32 ? mask[w + 1] : 0u;
+          allowed[k] = (__funnelshift_r(lo, hi, at & 31) << (at - v)) & kAll;
+        }
+      }
+      uint4 x[kBatch];
 #pragma unroll
-      for (int e = 0; e < kGroup; ++e)
-        if (here >> e & 1) {
-          uint32_t& w = (&x[k].x)[kBf16 ? e / 2 : e];
-          if constexpr (kBf16) {
-            const float y = adjusted(__uint_as_float(e % 2 ? w & 0xffff0000u : w << 16), named[at + e], repetition, presence, frequency, bias);
-            const uint32_t b = __bfloat16_as_ushort(f32_to_bf16(y));
-            w = e % 2 ? (w & 0xffffu) | b << 16 : (w & 0xffff0000u) | b;
-          } else {
-            w = __float_as_uint(adjusted(__uint_as_float(w), named[at + e], repetition, presence, frequency, bias));
+      for (int k = 0; k < kBatch; ++k) {
+        const int v = token_of(k);
+        x[k] = make_uint4(0, 0, 0, 0);
+        if (v >= a.vocab || !allowed[k] || (a.in_place && allowed[k] == kAll)) continue;
+        if (in_aligned && v >= 0 && v + kGroup <= a.vocab) {
+          x[k] = ld_v4(in + static_cast<long long>(v) * kSize);
+          continue;
+        }
+#pragma unroll
+        for (int e = 0; e < kGroup; ++e)
+          if (v + e >= 0 && v + e < a.vocab) {
+            if constexpr (kBf16)
+              (&x[k].x)[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(in)[v + e]) << (e % 2 * 16);
+            else
+              (&x[k].x)[e] = reinterpret_cast<const uint32_t*>(in)[v + e];
           }
-        }
-    }
-    if (!all) {
+      }
 #pragma unroll
-      for (int e = 0; e < kGroup; ++e)
-        if (!(allowed[k] >> e & 1)) {
-          uint32_t& w = (&x[k].x)[kBf16 ? e / 2 : e];
-          if constexpr (kBf16)
-            w = e % 2 ? (w & 0xffffu) | 0xff800000u : (w & 0xffff0000u) | 0xff80u;
-          else
-            w = 0xff800000u;
-        }
-    }
-    if (v >= 0 && v + kGroup <= a.vocab) {
-      st_v4(out + static_cast<long long>(v) * kSize, x[k]);
-    } else {
+      for (int k = 0; k < kBatch; ++k) {
+        const int v = token_of(k);
+        if (v >= a.vocab || (a.in_place && allowed[k] == kAll)) continue;
+        if (allowed[k] != kAll) {
 #pragma unroll
-      for (int e = 0; e < kGroup; ++e)
-        if (v + e >= 0 && v + e < a.vocab) {
-          if constexpr (kBf16)
-            reinterpret_cast<uint16_t*>(out)[v + e] = static_cast<uint16_t>((&x[k].x)[e / 2] >> (e % 2 * 16));
-          else
-            reinterpret_cast<uint32_t*>(out)[v + e] = (&x[k].x)[e];
+          for (int e = 0; e < kGroup; ++e)
+            if (!(allowed[k] >> e & 1)) {
+              uint32_t& w = (&x[k].x)[kBf16 ? e / 2 : e];
+              if constexpr (kBf16)
+                w = e % 2 ? (w & 0xffffu) | 0xff800000u : (w & 0xffff0000u) | 0xff80u;
+              else
+                w = 0xff800000u;
+            }
         }
+        if (v >= 0 && v + kGroup <= a.vocab) {
+          st_v4(out + static_cast<long long>(v) * kSize, x[k]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kGroup; ++e)
+            if (v + e >= 0 && v + e < a.vocab) {
+              if constexpr (kBf16)
+                reinterpret_cast<uint16_t*>(out)[v + e] = static_cast<uint16_t>((&x[k].x)[e / 2] >> (e % 2 * 16));
+              else
+                reinterpret_cast<uint32_t*>(out)[v + e] = (&x[k].x)[e];
+            }
+        }
+      }
     }
   }
+  if (!names) return;
+
+  // The tokens that the lists name
+  const float repetition = a.repetition.each ? a.repetition.each[row] : a.repetition.all;
+  const float presence = a.presence.each ? a.presence.each[row] : a.presence.all;
+  const float frequency = a.frequency.each ? a.frequency.each[row] : a.frequency.all;
+  const float* const bias = a.bias + row * a.bias_tokens.ld;
+  __syncthreads();  // (the counts are done, and the block's copies in place)
+  each([&](uint32_t x) {
+    const uint32_t of_token = atomicExch(named + place(x), 0u);
+    if (!of_token) return;
+    const int v = first + static_cast<int>(place(x));
+    if (mask && !(mask[v >> 5] >> (v & 31) & 1)) return;
+    if constexpr (kBf16) {
+      const float y = bf16_to_f32(reinterpret_cast<const __nv_bfloat16*>(in)[v]);
+      reinterpret_cast<__nv_bfloat16*>(out)[v] = f32_to_bf16(adjusted(y, of_token, repetition, presence, frequency, bias));
+    } else {
+      reinterpret_cast<float*>(out)[v] = adjusted(reinterpret_cast<const float*>(in)[v], of_token, repetition, presence, frequency, bias);
+    }
+  });
 }
 
 template <bool kBf16, int kPer>
@@ -203,10 +230,11 @@ cudaError_t launch(const Adjust& a, cudaStream_t stream) {
 }  // namespace
 
 cudaError_t launch_adjust(const Adjust& a, cudaStream_t stream) {
-  // 8192 tokens to a block, so that few blocks read a row's lists; 2048 where that would leave SMs without one
-  const bool few = static_cast<long long>(a.rows) * ((a.vocab + 8191) / 8192) < 148;
+  // 16 KB of a row to a block, so that few blocks read a row's lists; 4 KB where that would leave SMs without one
+  const int size = a.bf16 ? 2 : 4;
+  const bool few = static_cast<long long>(a.rows) * ((a.vocab * size + 16383) / 16384) < 148;
   if (a.bf16) return few ? launch<true, 1>(a, stream) : launch<true, 4>(a, stream);
-  return few ? launch<false, 2>(a, stream) : launch<false, 8>(a, stream);
+  return few ? launch<false, 1>(a, stream) : launch<false, 4>(a, stream);
 }
 
 }  // namespace logits

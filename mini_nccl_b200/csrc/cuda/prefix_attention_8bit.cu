@@ -35,12 +35,14 @@ namespace q8 {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kStep = 32;  // keys of a stage
+constexpr int kMostKnown = 1024;  // sequences whose lengths a block keeps
 constexpr float kLeastScale = 8.673617379884035e-19f;  // 2^-60
 
-template <int D>
+template <int D, int NT>
 struct Ring {
-  static constexpr int stages = 3;
-  static constexpr int blocks = D == 128 ? 2 : 4;    // per SM
+  // (sixteen rows need more registers)
+  static constexpr int blocks = (D == 128 ? 3 : 4) - (NT == 2 && D > 32);  // per SM
+  static constexpr int stages = D == 128 && NT == 1 ? 2 : 3;
   static constexpr uint32_t tile = kStep * D;        // of K; V follows
   static constexpr uint32_t bytes = stages * 2 * tile;  // of a warp
   // 16-byte chunk c of row r, as TMA's swizzle leaves it
@@ -114,10 +116,10 @@ MNB_DEVICE void arrive_after_copies(uint32_t bar) {
 
 // NT: eights of query rows.
 template <int D, int NT, bool kFloat>
-__global__ void __launch_bounds__(kThreads, Ring<D>::blocks)
+__global__ void __launch_bounds__(kThreads, Ring<D, NT>::blocks)
     pieces8_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap map_k,
-                   const __grid_constant__ CUtensorMap map_v, int items, int known) {
-  using R = Ring<D>;
+                   const __grid_constant__ CUtensorMap map_v, int items, int known, int least) {
+  using R = Ring<D, NT>;
   constexpr int kStages = R::stages, kU = kStep / 16, kRows = 8 * NT, kMt = D / 16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -130,6 +132,7 @@ __global__ void __launch_bounds__(kThreads, Ring<D>::blocks)
   if (lane < kStages * 8) (&scale_of[warp][0][0][0])[lane] = 1.f;  // (a stage's pages may be fewer than it has room for)
   int* lens = reinterpret_cast<int*>(sm + kWarps * R::bytes);
   int* offsets = lens + known;
+  int* tiles_before = offsets + known + 1;  // of 32 keys, of the sequences before each one
   for (int b = threadIdx.x; b < known; b += kThreads) lens[b] = a.seq_lens[b];
   if (a.q_offsets)
     for (int b = threadIdx.x; b < known + (known > 0); b += kThreads) offsets[b] = a.q_offsets[b];
@@ -137,20 +140,106 @@ __global__ void __launch_bounds__(kThreads, Ring<D>::blocks)
   const int* const q_offsets = known ? offsets : a.q_offsets;
   __syncthreads();
   let_next_start();
+  const int warps = kWarps * gridDim.x, self = blockIdx.x + warp * gridDim.x;
 
-  // Items in turn over the warps of all blocks.
-  const int first = blockIdx.x + warp * gridDim.x, stride = kWarps * gridDim.x;
+  // Shares (least > 0: single new tokens).  The tiles of 32 keys of all (part, row tile, kv head), the prefix first, lie in
+  // one row, and every warp takes as many of them, `share`, as every other: a part whose tiles several warps have gets
+  // partial results in slots one after another.  (`least` keeps them as few as there are slots.)
+  // Otherwise items, pieces of one (part, row tile, kv head, range of keys), in turn over the warps.
+  const int own_units = a.own_splits > 0 ? a.own_tiles * a.kv_heads : 0;
+  const int prefix_tiles = a.tensor_cores ? 0 : (a.prefix_len + kStep - 1) / kStep, prefix_units = a.row_tiles * a.kv_heads;
+  long long of_prefix = 0, from = 0, end = 0, share = 1;
+  if (least > 0) {
+    if (warp == 0) {
+      int sum = 0;
+      for (int b0 = 0; b0 < known; b0 += 32) {
+        const int len = b0 + lane < known ? lens[b0 + lane] : 0;
+        int x = len > 0 && len <= a.max_len ? (len + kStep - 1) / kStep : 0;
+        const int mine = x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, x, o);
+          if (lane >= o) x += y;
+        }
+        if (b0 + lane < known) tiles_before[b0 + lane] = sum + x - mine;
+        sum += __shfl_sync(0xffffffffu, x, 31);
+      }
+      if (lane == 0) tiles_before[known] = sum;
+    }
+    __syncthreads();
+    of_prefix = static_cast<long long>(prefix_tiles) * prefix_units;
+    const long long all = of_prefix + static_cast<long long>(known ? tiles_before[known] : 0) * own_units;
+    share = max((all + warps - 1) / warps, static_cast<long long>(least));
+    from = min(all, self * share), end = min(all, from + share);
+  }
+  // The piece of this warp that begins at `at` (a tile, or an item), or else the first one behind it; `at` moves past it.
+  auto next = [&](long long& at, Piece& p, int& part_end) {
+    if (least == 0) {
+      if (at >= items) return false;
+      p = piece_of(a, seq_lens, q_offsets, static_cast<int>(at), kRows, 1);
+      part_end = 0;  // (nobody asks)
+      at += warps;
+      return true;
+    }
+    if (at >= end) return false;
+    int unit, tile, tiles, b = -1;
+    if (at < of_prefix) {
+      tiles = prefix_tiles;
+      unit = static_cast<int>(at / tiles), tile = static_cast<int>(at - static_cast<long long>(unit) * tiles);
+    } else {
+      const long long own = at - of_prefix;
+      int lo = 0, hi = known - 1;  // the last sequence whose tiles begin at or before it (those without any come before it)
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (static_cast<long long>(tiles_before[mid]) * own_units <= own) lo = mid;
+        else hi = mid - 1;
+      }
+      b = lo;
+      tiles = tiles_before[b + 1] - tiles_before[b];
+      const long long in = own - static_cast<long long>(tiles_before[b]) * own_units;
+      unit = static_cast<int>(in / tiles), tile = static_cast<int>(in - static_cast<long long>(unit) * tiles);
+    }
+    const int len = b < 0 ? a.prefix_len : lens[b], most = static_cast<int>(min(end - at, static_cast<long long>(tiles - tile)));
+    const int segment = self - static_cast<int>((at - tile) / share);
+    part_end = len;
+    p.h = unit % a.kv_heads;
+    p.r0 = unit / a.kv_heads * kRows;
+    p.k0 = tile * kStep;
+    p.k1 = min(len, p.k0 + most * kStep);
+    p.limit0 = kUnlimited;
+    if (b < 0) {
+      p.n0 = 0;
+      p.n_rows = min(kRows, a.n * a.group - p.r0);
+      p.slot = segment;
+      p.ids = a.prefix_pages;
+    } else {
+      int rows = a.group;
+      p.n0 = b;
+      if (a.q_offsets) {  // (within the rows whatever the offsets say: offsets_sound() has the word on them)
+        p.n0 = min(max(q_offsets[b], 0), a.n);
+        rows = max(0, min(min(max(q_offsets[b + 1], 0), a.n) - p.n0, 1)) * a.group;
+      }
+      p.n_rows = min(kRows, rows - p.r0);
+      p.slot = a.prefix_splits + segment;
+      p.ids = a.page_table + b * a.table_ld;
+    }
+    at += most;
+    return true;
+  };
 
   // Loading runs ahead of the work by the stages of the ring, on into the next pieces.
   const int per = min(1 << a.page_shift, kStep);  // tokens of a box
-  int load_item = first - stride, load_key = 0, load_end = 0, load_head = 0, batch = 0, ids_end = 0, issued = 0;
+  long long load_at = least ? from : self;
+  bool loading = true;
+  int load_key = 0, load_end = 0, load_head = 0, batch = 0, ids_end = 0, issued = 0;
   int ids_now = 0, ids_next = 0;  // this lane's of 32 pages from `batch` on, and of the 32 after them
   const int* ids = nullptr;
-  auto fetch = [&](int from) { return from + lane < ids_end ? ids[from + lane] : 0; };
+  auto fetch = [&](int first) { return first + lane < ids_end ? ids[first + lane] : 0; };
   auto next_piece = [&] {
-    for (load_item += stride; load_item < items; load_item += stride) {
-      const Piece p = piece_of(a, seq_lens, q_offsets, load_item, kRows, 1);
-      if (p.k1 <= p.k0) continue;
+    Piece p;
+    int unused;
+    while ((loading = next(load_at, p, unused))) {
+      if (p.k1 <= p.k0 || p.n_rows <= 0) continue;
       load_key = p.k0, load_end = p.k1, load_head = p.h, ids = p.ids;
       batch = p.k0 >> a.page_shift;
       ids_end = ((p.k1 - 1) >> a.page_shift) + 1;
@@ -160,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, Ring<D>::blocks)
     }
   };
   auto issue = [&] {
-    if (load_item >= items) return;
+    if (!loading) return;
     if ((load_key >> a.page_shift) - batch >= 32) {
       batch += 32;
       ids_now = ids_next;
@@ -197,8 +286,10 @@ __global__ void __launch_bounds__(kThreads, Ring<D>::blocks)
   const uint32_t at_k = D == 32 ? R::at(g, t >> 1) + (t & 1) * 8 : R::at(key_of<D>(g), t);
   const uint32_t at_v = R::at(((lane >> 3) & 1) * 8 + key_of<D>(lane & 7), lane >> 4);
   int pos = 0;  // stages used so far
-  for (int i = first; i < items; i += stride) {
-    const Piece p = piece_of(a, seq_lens, q_offsets, i, kRows, 1);
+  long long work_at = least ? from : self;
+  Piece p;
+  int part_end;
+  while (next(work_at, p, part_end)) {
     if (p.n_rows <= 0) continue;
     auto out_of = [&](int r) {
       const int j = p.r0 + r, token = j / a.group;
@@ -425,8 +516,23 @@ __global__ void __launch_bounds__(kThreads, Ring<D>::blocks)
         for (int m = 0; m < kMt; ++m)
           *reinterpret_cast<float2*>(a.part_o + out * D + m * 16 + 2 * g) = make_float2(o[n][m][e], o[n][m][2 + e]);
         if (g == 0) a.part_ml[out] = make_float2(base[n][e], sum * 3.0517578125e-5f);  // 2^-15
+        if (least > 0 && p.k1 == part_end) {  // of shares: the part's other slots have nothing
+          const long long step = static_cast<long long>(a.n) * a.heads;
+          const int slots = p.slot < a.prefix_splits ? a.prefix_splits : a.prefix_splits + a.own_splits;
+          for (int x = p.slot + 1 + g; x < slots; x += 8) a.part_ml[out + (x - p.slot) * step] = make_float2(-INFINITY, 0.f);
+        }
       }
   }
+  // Sequences without tokens have no partial results at all.
+  if (least > 0)
+    for (int b = self; b < known; b += warps)
+      if (tiles_before[b + 1] == tiles_before[b]) {
+        if (lane == 0 && lens[b] != 0) flag(a);  // (a length out of its bounds)
+        const int n0 = a.q_offsets ? min(max(q_offsets[b], 0), a.n) : b;
+        const int rows = a.q_offsets ? max(0, min(min(max(q_offsets[b + 1], 0), a.n) - n0, 1)) : 1;
+        for (int x = lane; x < rows * a.own_splits * a.heads; x += 32)
+          a.part_ml[(static_cast<long long>(a.prefix_splits + x / a.heads) * a.n + n0) * a.heads + x % a.heads] = make_float2(-INFINITY, 0.f);
+      }
   // The block does not end before its last copies have arrived, also where a wait was given up.
   for (int k = max(0, issued - kStages); k < issued; ++k) mbar_wait(bar0 + 8 * (k % kStages), (k / kStages) & 1, nullptr);
   if (a.sound && blockIdx.x == 0 && warp == 0) {
@@ -458,14 +564,16 @@ static bool codes_map(CUtensorMap* map, const uint8_t* base, const Args& a, int 
 
 template <int D, int NT, bool kFloat>
 static cudaError_t launch(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
-  using R = Ring<D>;
-  const int known = a.own_splits > 0 && a.batch <= 1024 ? a.batch : 0;
-  const int bytes = kWarps * R::bytes + (known ? (2 * known + 1) * 4 : 0) + 1024;
-  const int items = (a.tensor_cores ? 0 : a.row_tiles * a.kv_heads * a.prefix_splits) + a.batch * a.own_tiles * a.own_splits * a.kv_heads;
+  using R = Ring<D, NT>;
+  const int known = a.own_splits > 0 && a.batch <= kMostKnown ? a.batch : 0;
+  const int bytes = kWarps * R::bytes + (known ? (3 * known + 2) * 4 : 0) + 1024;
+  long long items = a.batch * static_cast<long long>(a.own_tiles) * a.own_splits * a.kv_heads;
+  if (!a.tensor_cores) items += static_cast<long long>(a.row_tiles) * a.kv_heads * a.prefix_splits;
   static SharedMemory allowed;
   if (const cudaError_t e = allowed.at_least(reinterpret_cast<const void*>(pieces8_kernel<D, NT, kFloat>), bytes); e != cudaSuccess) return e;
   const int per_sm = std::max(1, std::min(R::blocks, 227 * 1024 / (bytes + 1024 + 512)));
-  pieces8_kernel<D, NT, kFloat><<<std::min(items, 148 * per_sm), kThreads, bytes, stream>>>(a, mk, mv, items, known);
+  const int blocks = static_cast<int>(std::min<long long>(items, 148 * per_sm));
+  pieces8_kernel<D, NT, kFloat><<<blocks, kThreads, bytes, stream>>>(a, mk, mv, static_cast<int>(items), known, a.least_share);
   return cudaGetLastError();
 }
 
@@ -489,27 +597,45 @@ cudaError_t launch_pieces8(const Args& a, int head_dim, cudaStream_t stream) {
 
 int plan8(Args& a, int head_dim) {
   using q8::kStep;
-  // Pieces until every warp has about three.
-  const int want = 148 * q8::kWarps * (head_dim == 128 ? 2 : 4) * 3;
-  a.prefix_splits = a.own_splits = 0;
+  a.prefix_splits = a.own_splits = a.least_share = 0;
   a.quad = a.tensor_cores = false;
-  const long long rows = static_cast<long long>(a.n) * a.group;
-  const long long most = a.prefix_len > 0 ? std::max(rows, static_cast<long long>(a.max_q) * a.group) : static_cast<long long>(a.max_q) * a.group;
-  a.tile_rows = most <= 8 ? 8 : 16;
+  const long long rows = static_cast<long long>(a.n) * a.group, own_rows = static_cast<long long>(a.max_q) * a.group;
+  const bool own = a.max_len > 0 && a.max_q > 0 && a.batch > 0;
+  a.tile_rows = std::max(a.prefix_len > 0 ? rows : 0, own ? own_rows : 0) <= 8 ? 8 : 16;
+  const int warps = 148 * q8::kWarps * ((head_dim == 128 ? 3 : 4) - (a.tile_rows == 16 && head_dim > 32));
+  const int prefix_tiles = ceil_div(a.prefix_len, kStep), own_tiles = ceil_div(a.max_len, kStep);
+  if (a.prefix_len > 0) a.row_tiles = ceil_div(rows, a.tile_rows);
+  if (own) a.own_tiles = ceil_div(own_rows, a.tile_rows);
+  // Single new tokens: shares of the tiles, the same for every warp (48 sequences of up to 6001 tokens, 8 heads: 89 us with
+  // pieces of 608 keys in turn).  A part of t tiles has at most 1 + ceil((t - 1) / share) warps, and as many slots.  Parts of
+  // the average length need one for each warp that it takes to fill the GPU, longer ones (here: up to twice) more.
+  const bool shares = a.max_q == 1 && (!own || (a.batch <= q8::kMostKnown && static_cast<long long>(a.batch) * own_tiles < (1ll << 31)));
+  auto slots = [&](int tiles, long long units, int times) {
+    return std::min({tiles, 64, times * ceil_div(warps, units) + (times == 1 ? 2 : 1)});
+  };
   if (a.prefix_len > 0) {
-    a.row_tiles = ceil_div(rows, a.tile_rows);
-    const int tiles = ceil_div(a.prefix_len, kStep);
-    const int splits = std::max(1, std::min({tiles, 64, ceil_div(want, static_cast<long long>(a.row_tiles) * a.kv_heads)}));
-    a.prefix_chunk = ceil_div(tiles, splits) * kStep;
-    a.prefix_splits = ceil_div(a.prefix_len, a.prefix_chunk);
+    const long long units = static_cast<long long>(a.row_tiles) * a.kv_heads;
+    if (shares) {
+      a.prefix_splits = slots(prefix_tiles, units, 1);
+      if (prefix_tiles > 1) a.least_share = ceil_div(prefix_tiles - 1, a.prefix_splits - 1);
+    } else {  // pieces until every warp has about three
+      const int splits = std::max(1, std::min({prefix_tiles, 64, ceil_div(3 * warps, units)}));
+      a.prefix_chunk = ceil_div(prefix_tiles, splits) * kStep;
+      a.prefix_splits = ceil_div(a.prefix_len, a.prefix_chunk);
+    }
   }
-  if (a.max_len > 0 && a.max_q > 0 && a.batch > 0) {
-    a.own_tiles = ceil_div(static_cast<long long>(a.max_q) * a.group, a.tile_rows);
-    const int tiles = ceil_div(a.max_len, kStep);
-    const int splits = std::max(1, std::min({tiles, 64, ceil_div(want, static_cast<long long>(a.batch) * a.own_tiles * a.kv_heads)}));
-    a.own_chunk = ceil_div(tiles, splits) * kStep;
-    a.own_splits = ceil_div(a.max_len, a.own_chunk);
+  if (own) {
+    const long long units = static_cast<long long>(a.batch) * a.own_tiles * a.kv_heads;
+    if (shares) {
+      a.own_splits = slots(own_tiles, units, 2);
+      if (own_tiles > 1) a.least_share = std::max(a.least_share, ceil_div(own_tiles - 1, a.own_splits - 1));
+    } else {
+      const int splits = std::max(1, std::min({own_tiles, 64, ceil_div(3 * warps, units)}));
+      a.own_chunk = ceil_div(own_tiles, splits) * kStep;
+      a.own_splits = ceil_div(a.max_len, a.own_chunk);
+    }
   }
+  if (shares) a.least_share = std::max(a.least_share, 1);
   return a.prefix_splits + a.own_splits;
 }
 
