@@ -196,6 +196,8 @@ cudaError_t launch_prefix_tc(const Args& a, const CUtensorMap& mk, const CUtenso
 cudaError_t launch_exp2(const float* x, float* y, int pairs, cudaStream_t stream);
 // of a cache in 8 bits (prefix_attention_8bit.cu)
 int plan8(Args& a, int head_dim);
+void plan_prefix_tc(Args& a, int head_dim);  // the prefix's pieces, where it goes to the tensor cores
+cudaError_t launch_prefix_tc8(const Args& a, int head_dim, cudaStream_t stream);
 cudaError_t launch_pieces8(const Args& a, int head_dim, cudaStream_t stream);
 cudaError_t launch_attention(const Args& a, int head_dim, cudaStream_t stream);
 int kernels(const Args& a);  // that launch_attention() launches

@@ -527,7 +527,8 @@ static cudaError_t launch_for(const Args& a, cudaStream_t stream) {
   }
   if (a.codes) {
     if (by_warps(a) && (e = launch_pieces8(a, D, stream)) != cudaSuccess) return e;
-    return launch_join_of<D>(a, stream);
+    if (by_tensor_cores(a) && (e = launch_prefix_tc8(a, D, stream)) != cudaSuccess) return e;
+    return joins(a) ? launch_join_of<D>(a, stream) : e;
   }
   if (by_warps(a)) {
     const int tokens = a.quad ? 16 : kKeys;
@@ -561,6 +562,15 @@ static int tc_splits(int blocks, int tiles, long long rows, int head_dim, bool w
   return best;
 }
 
+void plan_prefix_tc(Args& a, int head_dim) {
+  const long long rows = static_cast<long long>(a.n) * a.group;
+  a.row_tiles = ceil_div(rows, 256);
+  const int tiles = ceil_div(a.prefix_len, 128);
+  const int splits = tc_splits(a.row_tiles * a.kv_heads, tiles, rows * a.kv_heads, head_dim, rows > 128);
+  a.prefix_chunk = ceil_div(tiles, splits) * 128;
+  a.prefix_splits = ceil_div(a.prefix_len, a.prefix_chunk);
+}
+
 int plan(Args& a, int head_dim) {
   if (a.codes) return plan8(a, head_dim);
   // Without tensor cores, pieces until every SM has about six, so that the last ones are short against the whole.
@@ -573,10 +583,7 @@ int plan(Args& a, int head_dim) {
   a.tile_rows = 16 * row_warps(static_cast<int>(a.tensor_cores || a.prefix_len == 0 ? static_cast<long long>(a.max_q) * a.group : rows));
   if (a.prefix_len > 0) {
     if (a.tensor_cores) {
-      a.row_tiles = ceil_div(rows, 256);
-      const int tiles = ceil_div(a.prefix_len, 128);
-      const int splits = tc_splits(a.row_tiles * a.kv_heads, tiles, rows * a.kv_heads, head_dim, rows > 128);
-      a.prefix_chunk = ceil_div(tiles, splits) * 128;
+      plan_prefix_tc(a, head_dim);
     } else {
       a.row_tiles = ceil_div(rows, a.tile_rows);
       const int tiles = ceil_div(a.prefix_len, kKeys);

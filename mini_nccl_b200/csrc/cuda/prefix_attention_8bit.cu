@@ -24,7 +24,7 @@
 #include <type_traits>
 
 #include "launch.cuh"
-#include "prefix_attention.cuh"
+#include "prefix_attention_8bit.cuh"
 #include "warp_mma.cuh"
 
 namespace mnb {
@@ -35,8 +35,8 @@ namespace q8 {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kStep = 32;  // keys of a stage
+constexpr int kTensorCoreRows = 16;  // more rows of a kv head than this go to the tensor-core kernel
 constexpr int kMostKnown = 1024;  // sequences whose lengths a block keeps
-constexpr float kLeastScale = 8.673617379884035e-19f;  // 2^-60
 
 template <int D, int NT>
 struct Ring {
@@ -71,49 +71,6 @@ MNB_DEVICE uint32_t transposed(uint32_t x) {  // of an 8 x 8 matrix of 16-bit va
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-MNB_DEVICE uint32_t pack_f16x2(float lo, float hi) {
-  uint32_t y;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
-  return y;
-}
-MNB_DEVICE uint32_t sub_f16x2(uint32_t a, uint32_t b) {
-  uint32_t y;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
-  return y;
-}
-MNB_DEVICE uint32_t f16_of_e4m3(uint16_t x) {
-  uint32_t y;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(y) : "h"(x));
-  return y;
-}
-// Four codes as f16: of bytes 0 and 2 (lo), and 1 and 3 (hi).
-template <bool kFloat>
-MNB_DEVICE void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if constexpr (kFloat) {
-    w = __byte_perm(w, 0, 0x3120);
-    lo = f16_of_e4m3(static_cast<uint16_t>(w)), hi = f16_of_e4m3(static_cast<uint16_t>(w >> 16));
-  } else {
-    w ^= 0x80808080u;
-    lo = sub_f16x2(__byte_perm(w, 0x64646464u, 0x4240), 0x64806480u);
-    hi = sub_f16x2(__byte_perm(w, 0x64646464u, 0x4341), 0x64806480u);
-  }
-}
-// The same as whichever pairs are cheapest: bytes (0, 1), (2, 3) of e4m3, (0, 2), (1, 3) of int8.
-template <bool kFloat>
-MNB_DEVICE void widen_any(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if constexpr (kFloat)
-    lo = f16_of_e4m3(static_cast<uint16_t>(w)), hi = f16_of_e4m3(static_cast<uint16_t>(w >> 16));
-  else
-    widen<false>(w, lo, hi);
-}
-MNB_DEVICE void copy_float(uint32_t dst, const float* src, bool there) {  // zero where not
-  const int n = there ? 4 : 0;
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-MNB_DEVICE void arrive_after_copies(uint32_t bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
-
 // NT: eights of query rows.
 template <int D, int NT, bool kFloat>
 __global__ void __launch_bounds__(kThreads, Ring<D, NT>::blocks)
@@ -544,24 +501,6 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NT>::blocks)
   }
 }
 
-// A pool of codes as (head_dim, heads, tokens, pages) in boxes of up to `tokens` of one page and head.
-static bool codes_map(CUtensorMap* map, const uint8_t* base, const Args& a, int head_dim, int tokens) {
-  if (!encode_fn()) return false;
-  const int page = 1 << a.page_shift;
-  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(a.kv_heads),
-                              static_cast<cuuint64_t>(page), static_cast<cuuint64_t>(std::max(1, a.pages))};
-  // an axis of one entry may have any stride: give the map one that it accepts
-  auto stride = [](long long n, long long ld) { return static_cast<cuuint64_t>(n > 1 ? ld : 16); };
-  const cuuint64_t strides[3] = {stride(a.kv_heads, a.head_ld), stride(page, a.token_ld), stride(a.pages, a.page_ld)};
-  const cuuint32_t box[4] = {static_cast<cuuint32_t>(head_dim), 1, static_cast<cuuint32_t>(std::min(page, tokens)), 1};
-  const cuuint32_t each[4] = {1, 1, 1, 1};
-  const CUtensorMapSwizzle swizzle = head_dim == 32 ? CU_TENSOR_MAP_SWIZZLE_32B
-                                     : head_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
-  return encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t*>(base), dims, strides, box, each,
-                     CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int D, int NT, bool kFloat>
 static cudaError_t launch(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
   using R = Ring<D, NT>;
@@ -598,13 +537,16 @@ cudaError_t launch_pieces8(const Args& a, int head_dim, cudaStream_t stream) {
 int plan8(Args& a, int head_dim) {
   using q8::kStep;
   a.prefix_splits = a.own_splits = a.least_share = 0;
-  a.quad = a.tensor_cores = false;
+  a.quad = false;
   const long long rows = static_cast<long long>(a.n) * a.group, own_rows = static_cast<long long>(a.max_q) * a.group;
   const bool own = a.max_len > 0 && a.max_q > 0 && a.batch > 0;
-  a.tile_rows = std::max(a.prefix_len > 0 ? rows : 0, own ? own_rows : 0) <= 8 ? 8 : 16;
+  // (the tensor-core kernel takes maxima before it scales)
+  a.tensor_cores = a.prefix_len > 0 && head_dim != 32 && rows > q8::kTensorCoreRows && a.scale_log2 > 0.f;
+  a.tile_rows = std::max(a.prefix_len > 0 && !a.tensor_cores ? rows : 0, own ? own_rows : 0) <= 8 ? 8 : 16;
   const int warps = 148 * q8::kWarps * ((head_dim == 128 ? 3 : 4) - (a.tile_rows == 16 && head_dim > 32));
   const int prefix_tiles = ceil_div(a.prefix_len, kStep), own_tiles = ceil_div(a.max_len, kStep);
-  if (a.prefix_len > 0) a.row_tiles = ceil_div(rows, a.tile_rows);
+  if (a.tensor_cores) plan_prefix_tc(a, head_dim);
+  else if (a.prefix_len > 0) a.row_tiles = ceil_div(rows, a.tile_rows);
   if (own) a.own_tiles = ceil_div(own_rows, a.tile_rows);
   // Single new tokens: shares of the tiles, the same for every warp (48 sequences of up to 6001 tokens, 8 heads: 89 us with
   // pieces of 608 keys in turn).  A part of t tiles has at most 1 + ceil((t - 1) / share) warps, and as many slots.  Parts of
@@ -613,7 +555,7 @@ int plan8(Args& a, int head_dim) {
   auto slots = [&](int tiles, long long units, int times) {
     return std::min({tiles, 64, times * ceil_div(warps, units) + (times == 1 ? 2 : 1)});
   };
-  if (a.prefix_len > 0) {
+  if (a.prefix_len > 0 && !a.tensor_cores) {
     const long long units = static_cast<long long>(a.row_tiles) * a.kv_heads;
     if (shares) {
       a.prefix_splits = slots(prefix_tiles, units, 1);

@@ -1,0 +1,529 @@
+// The shared prefix's part of the paged attention on the 5th-generation tensor
+// cores over a cache in 8 bits.  prefix_attention_tc.cu has the scheme (two
+// streams of 128 rows, scores, P and O in TMEM) and prefix_attention_8bit.cu the
+// mathematics of scales and weights; here the two meet.
+//
+// Codes come page by page into a ring of raw tiles (128 keys, or their values); four
+// warps widen each into the swizzled f16 tile that the products read.  An f16 tile holds
+// code * scale / R, with R the largest scale of the tile's pages: exact while the pages
+// of 128 tokens next to one another have scales within a factor of 2^15 (2^17 for int8);
+// a value of a page further below R is rounded to a multiple of R 2^-24.  R of the keys
+// goes into the factor of the tile's scores, R of the values into their exponent,
+//   s'_j = s_j + log2 R_v,  O = sum 2^(s'_j - base) (v_j / R_v),  sum_j 2^(s_j - base) = sum_j 2^(s'_j - base) / R_v,
+// one number each for a tile, so the softmax costs what it costs without scales.  The base
+// lies 7 below a maximum that scores may pass by 8, so a weight in f16 is at most 2^15.
+// Both R come with a tile's keys, before its scores.
+//
+// What bounds it: with few rows the bytes (raw tiles then also lie where the second
+// stream's queries would be, so that 64 KB are under way), with many the softmax, beside
+// which the widening warps take a fifth of the issue slots.
+#include <type_traits>
+
+#include "launch.cuh"
+#include "prefix_attention_8bit.cuh"
+#include "prefix_attention_tc.cuh"
+#include "warp_mma.cuh"
+
+namespace mnb {
+
+namespace prefix {
+
+namespace tc8 {
+
+using namespace tc;
+using namespace q8;
+
+constexpr int kWiden = 128;                       // threads that widen codes, a row of a tile each
+// Warps 0 and 1 load and issue products (2 and 3 only fill their warpgroup), 4 to 19 do the softmax, 20 to 23 widen.  768
+// threads can have 80 registers each; the softmax takes over what the others do not need.
+constexpr int kThreads = 128 + kSoftmax + kWiden, kFirst = 4;
+constexpr int kLaunched = 80, kSmall = 48, kLarge = 96;
+static_assert((kThreads - kSoftmax) * kSmall + kSoftmax * kLarge <= kThreads * kLaunched, "registers");
+constexpr float kBelow = 7.f, kPass = 15.f;       // the base below the maximum, and what a score may lie above the base
+constexpr int kInfo = 8;                          // tiles whose factors are kept
+
+template <int D>
+struct Smem {
+  static constexpr uint32_t q_tile = kTile * D * 2;
+  static constexpr uint32_t kv_tile = kTile * D * 2;
+  static constexpr uint32_t raw_tile = kTile * D;
+  static constexpr int stages = D == 128 ? 4 : 6;
+  static constexpr int raws = D == 128 ? 2 : 4, more_raws = q_tile / raw_tile;  // with one tile of queries these many more
+  static constexpr uint32_t q_off = 0, kv_off = 2 * q_tile, raw_off = kv_off + stages * kv_tile;
+  static constexpr uint32_t bar_off = raw_off + raws * raw_tile;
+  static constexpr int n_bars = 2 * stages + 2 * (raws + more_raws) + 10;
+  static constexpr uint32_t max_off = bar_off + n_bars * 8 + 16;    // row maxima so far: [stream][row], as order_of()
+  static constexpr uint32_t scale_off = max_off + 2 * kTile * 4;    // of the raw tiles' pages: [raw][keys, values][16]
+  static constexpr uint32_t info_off = scale_off + (raws + more_raws) * 2 * 16 * 4;  // of tiles: a float4 each
+  static constexpr uint32_t total = info_off + kInfo * 16 + 1024;
+  static_assert(total <= 227 * 1024, "a block's shared memory");
+  static_assert(max_off % 16 == 0, "alignment");
+  static_assert(kMeeting<D> <= stages * kv_tile + raws * raw_tile, "the meeting place fits the rings");
+};
+
+// Instruction descriptor for kind::f16 with f16 A/B and fp32 D.
+constexpr uint32_t idesc_f16(int m, int n, bool a_mn, bool b_mn) { return idesc_bf16(m, n, a_mn, b_mn) & ~((1u << 7) | (1u << 10)); }
+
+// The order in which the products use the tiles: (keys or values, which).
+struct Step {
+  bool keys;
+  int tile;
+};
+MNB_DEVICE Step step_of(int pos, int n_tiles, bool shared) {
+  if (shared || n_tiles == 1) return {(pos & 1) == 0, pos >> 1};
+  if (pos < 2) return {true, pos};
+  const int j = pos - 2;
+  if (j < 2 * (n_tiles - 2)) return {(j & 1) == 1, (j >> 1) + 2 * (j & 1)};
+  return {false, j - (n_tiles - 2)};
+}
+
+template <int D, bool kFloat>
+__global__ void __launch_bounds__(kThreads, 1)
+    prefix8_tc_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap map_k,
+                      const __grid_constant__ CUtensorMap map_v, int whole) {
+  using S = Smem<D>;
+  constexpr int kStages = S::stages;
+  constexpr uint32_t kIdescS = idesc_f16(kTile, kTile, false, false);
+  constexpr uint32_t kIdescO = idesc_f16(kTile, D, false, true);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(sm);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + S::bar_off);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + S::n_bars);
+  constexpr int kMostRaws = S::raws + S::more_raws;
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * kStages, raw_full0 = empty0 + 8 * kStages,
+                 raw_empty0 = raw_full0 + 8 * kMostRaws, q_full = raw_empty0 + 8 * kMostRaws, s_full0 = q_full + 8,
+                 o_full0 = s_full0 + 16, p_full0 = o_full0 + 16,  // (p_full: two halves per stream)
+                 drained = p_full0 + 32;
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  // The first `whole` blocks take 256 rows, the others half as many (a short last wave: prefix_attention_tc.cu).
+  int unit = blockIdx.x, most = 2 * kTile, skip = 0;
+  if (unit >= whole) {
+    skip = (unit - whole) % 2 * kTile;
+    most = kTile;
+    unit = whole + (unit - whole) / 2;
+  }
+  const int rt = unit % a.row_tiles;
+  const int h = (unit / a.row_tiles) % a.kv_heads;
+  const int split = unit / (a.row_tiles * a.kv_heads);
+  const int r0 = rt * 2 * kTile + skip;
+  const int n_rows = min(most, a.n * a.group - r0);
+  if (n_rows <= 0) return;
+  const bool shared = n_rows > kTile;  // both streams use every key tile
+  const int k0 = split * a.prefix_chunk, k1 = min(a.prefix_len, k0 + a.prefix_chunk);
+  const int n_tiles = (k1 - k0 + kTile - 1) / kTile, loads = 2 * n_tiles;
+  const int raws = shared ? S::raws : kMostRaws;
+  const int per = min(1 << a.page_shift, kTile);  // tokens of a box
+  auto raw_at = [&](int r) { return r < S::raws ? S::raw_off + r * S::raw_tile : S::q_off + S::q_tile + (r - S::raws) * S::raw_tile; };
+  auto valid_of = [&](int tile) { return min(kTile, k1 - k0 - tile * kTile); };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full0 + 8 * s, kWiden / 32);
+      mbar_init(empty0 + 8 * s, 1);
+    }
+    for (int r = 0; r < kMostRaws; ++r) {
+      mbar_init(raw_full0 + 8 * r, 33);  // the expected bytes, and every lane's copies of scales
+      mbar_init(raw_empty0 + 8 * r, kWiden / 32);
+    }
+    mbar_init(q_full, kSoftmax);
+    mbar_init(drained, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(s_full0 + 8 * s, 1);
+      mbar_init(p_full0 + 16 * s, 128);
+      mbar_init(p_full0 + 16 * s + 8, 128);
+      mbar_init(o_full0 + 8 * s, 1);
+    }
+    fence_mbar_init();
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  let_next_start();
+  const uint32_t tmem = *tmem_slot;  // S_0, S_1: 128 columns each, then O_0, O_1
+
+  if (warp < kFirst) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSmall));
+    if (warp == 0) {
+      int pos = 0;
+      for (bool ok = true; ok && pos < loads; ++pos) {
+        const Step step = step_of(pos, n_tiles, shared);
+        const int r = pos % raws, j0 = k0 + step.tile * kTile, boxes = (valid_of(step.tile) + per - 1) / per;
+        const uint32_t bar = raw_full0 + 8 * r;
+        int page = 0;
+        if (lane < boxes) page = a.prefix_pages[(j0 + lane * per) >> a.page_shift];
+        ok = warp_wait(raw_empty0 + 8 * r, ((pos / raws) & 1) ^ 1, a.status);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(bar, boxes * per * D);
+        __syncwarp();
+        if (lane < boxes) {
+          const bool there = page >= 0 && page < a.pages;
+          if (!there) {
+            atomicCAS(a.errors, 0, kErrBadIndex);
+            page = a.no_page;  // reads as zeros
+          }
+          tma_load_4d(sbase + raw_at(r) + lane * per * D, step.keys ? &map_k : &map_v, 0, h, (j0 + lane * per) & ((1 << a.page_shift) - 1), page, bar);
+          const long long at = there ? page * a.scale_ld + h * a.scale_head : 0;
+          const uint32_t to = sbase + S::scale_off + (r * 2 * 16 + lane) * 4;
+          if (step.keys) copy_float(to, a.k_scales + at, there);
+          copy_float(to + 64, a.v_scales + at, there);
+        }
+        arrive_after_copies(bar);
+      }
+      // The block does not end before its last copies have arrived, also where another warp's wait was given up.
+      for (int p = max(0, pos - raws); p < pos; ++p) mbar_wait(raw_full0 + 8 * (p % raws), (p / raws) & 1, nullptr);
+    } else if (warp == 1) {
+      int pos = 0;
+      // Whether this lane's waits have all ended well.  The lanes agree on it once a step (`settle`): a vote at each wait made
+      // the bf16 kernel 2 % slower, and what a step computes past a wait that was given up is in bounds.
+      bool good = true;
+      auto settle = [&] { return __all_sync(0xffffffffu, good); };
+      auto wait_full = [&](int p) {
+        good = mbar_wait(full0 + 8 * (p % kStages), (p / kStages) & 1, a.status) && good;
+        tc_fence_after();
+      };
+      // (adding bytes / 16 to a descriptor moves its address: the tiles lie below 256 KB, so nothing carries)
+      const uint64_t q_desc = smem_desc_sw128(sbase + S::q_off, 16, 1024);
+      const uint64_t k_desc = smem_desc_sw128(sbase + S::kv_off, 16, 1024);
+      const uint64_t v_desc = smem_desc_sw128(sbase + S::kv_off, kTile * 128, 1024);
+      auto tile_of = [&](int p) { return static_cast<uint64_t>(p % kStages) * (S::kv_tile / 16); };
+      // S_s = Q_s K^T
+      auto scores = [&](int s, int p) {
+        const uint64_t qa = q_desc + (shared ? s : 0) * (S::q_tile / 16), kb = k_desc + tile_of(p);
+        if (elected()) {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t at = ((kk / 4) * (kTile * 128) + (kk % 4) * 32) / 16;
+            tc_mma(tmem + s * kTile, qa + at, kb + at, kIdescS, kk > 0 ? 1u : 0u);
+          }
+          tc_commit(s_full0 + 8 * s);
+        }
+        __syncwarp();
+      };
+      // O_s (+)= P_s V, the first half of the keys while the second half's probabilities are still computed
+      auto values = [&](int s, int p, int step) {
+        const uint64_t vb = v_desc + tile_of(p);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          good = mbar_wait(p_full0 + 16 * s + 8 * half, step & 1, a.status) && good;
+          tc_fence_after();
+          if (elected()) {
+#pragma unroll
+            for (int kk = half * kTile / 32; kk < (half + 1) * kTile / 32; ++kk)
+              tc_mma_tmem_a(tmem + 2 * kTile + s * D, tmem + s * kTile + kk * 8, vb + kk * (2048 / 16), kIdescO,
+                            step == 0 && kk == 0 ? 0u : 1u);
+          }
+          __syncwarp();
+        }
+      };
+      auto done_with = [&](int p) {
+        if (elected()) tc_commit(empty0 + 8 * (p % kStages));
+        __syncwarp();
+      };
+      bool ok = warp_wait(q_full, 0, a.status);
+      tc_fence_after();
+      if (shared) {
+        if (ok) {
+          wait_full(pos);
+          scores(0, pos);
+          scores(1, pos);
+          done_with(pos++);
+          ok = settle();
+        }
+        for (int t = 0; t < n_tiles && ok; ++t) {
+          const int v = pos++, k = pos;
+          const bool more = t + 1 < n_tiles;
+          if (more) ++pos;
+          wait_full(v);
+          values(0, v, t);
+          if (more) {
+            wait_full(k);
+            scores(0, k);
+          } else if (elected()) {
+            tc_commit(o_full0);
+          }
+          values(1, v, t);
+          done_with(v);
+          if (more) {
+            scores(1, k);
+            done_with(k);
+          } else if (elected()) {
+            tc_commit(o_full0 + 8);
+          }
+          ok = settle();
+        }
+      } else {
+        for (int s = 0; s < 2 && s < n_tiles && ok; ++s) {
+          wait_full(pos);
+          scores(s, pos);
+          done_with(pos++);
+          ok = settle();
+        }
+        for (int t = 0; t < n_tiles && ok; ++t) {
+          const int s = t & 1;
+          wait_full(pos);
+          values(s, pos, t >> 1);
+          done_with(pos++);
+          if (t + 2 < n_tiles) {
+            wait_full(pos);
+            scores(s, pos);
+            done_with(pos++);
+          } else if (elected()) {
+            tc_commit(o_full0 + 8 * s);
+          }
+          ok = settle();
+        }
+      }
+      if (!ok) {  // a wait was given up: nor do products end after their TMEM is freed
+        if (elected()) tc_commit(drained);
+        __syncwarp();
+        mbar_wait(drained, 0, nullptr);
+      }
+    }
+  } else if (warp >= kFirst + kSoftmax / 32) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSmall));
+    // Widening: a lane has a row of the tile, so one scale.
+    const int row = threadIdx.x - (kThreads - kWiden);
+    bool ok = true;
+    for (int pos = 0; ok && pos < loads; ++pos) {
+      const Step step = step_of(pos, n_tiles, shared);
+      const int r = pos % raws, st = pos % kStages, valid = valid_of(step.tile), boxes = (valid + per - 1) / per;
+      ok = warp_wait(raw_full0 + 8 * r, (pos / raws) & 1, a.status) && warp_wait(empty0 + 8 * st, ((pos / kStages) & 1) ^ 1, a.status);
+      if (!ok) break;
+      const float* scales = reinterpret_cast<const float*>(sm + S::scale_off) + r * 2 * 16;
+      auto largest = [&](float x) {  // of the pages' scales, and at least the least
+        const float mine = lane < boxes ? fmaxf(x, kLeastScale) : kLeastScale;  // (also for what is no number)
+        return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mine)));
+      };
+      const int box = min(row, valid - 1) / per;
+      float factor;
+      if (step.keys) {
+        const float top_k = largest(scales[lane & 15]), top_v = largest(scales[16 + (lane & 15)]);
+        factor = scales[box] / top_k;
+        if (row == 0) {
+          const float b = __log2f(top_v);
+          *reinterpret_cast<float4*>(sm + S::info_off + step.tile % kInfo * 16) =
+              make_float4(fminf(top_k, 3.4e38f) * a.scale_log2, b, ex2_approx(15.f - b), 0.f);
+        }
+      } else {
+        factor = fmaxf(scales[16 + box], kLeastScale) / largest(scales[16 + (lane & 15)]);
+      }
+      uint32_t by;  // as an f16 pair
+      by = pack_f16x2(factor, factor);
+      const bool there = row < valid;
+      const uint32_t from = sbase + raw_at(r) + row * D, to = sbase + S::kv_off + st * S::kv_tile + row * 128;
+      const int turn_in = D == 128 ? row & 7 : (row >> 1) & 3, turn_out = row & 7;
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) {
+        uint4 w;
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(from + ((c ^ turn_in) << 4)));
+        uint32_t y[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          widen_in_order<kFloat>((&w.x)[k], y[2 * k], y[2 * k + 1]);
+          y[2 * k] = mul_f16x2(y[2 * k], by), y[2 * k + 1] = mul_f16x2(y[2 * k + 1], by);
+        }
+        if (!there)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) y[k] = 0;  // past the end a page holds anything
+        const uint32_t at = to + (2 * c / 8) * (kTile * 128);
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at + (((2 * c % 8) ^ turn_out) << 4)), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at + (((2 * c % 8 + 1) ^ turn_out) << 4)), "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7]) : "memory");
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(full0 + 8 * st);
+        mbar_arrive(raw_empty0 + 8 * r);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kLarge));
+    const int s = (warp - kFirst) / 8, half = (warp - kFirst) / 4 % 2, quad = warp % 4;
+    const int r = quad * 32 + lane;                 // row of the stream's tile
+    float* const row_back = reinterpret_cast<float*>(sm + S::max_off);
+    {  // Q as f16, each row times a power of two, swizzled as TMA would leave it; rows past the last are zeros
+      constexpr int kChunks = D / 8, kStep = kSoftmax / kChunks, kAhead = 4;  // a thread keeps its chunk and goes through the rows
+      const int c = (threadIdx.x - 32 * kFirst) % kChunks, rows_end = shared ? 2 * kTile : kTile;
+      for (int i0 = (threadIdx.x - 32 * kFirst) / kChunks; i0 < rows_end; i0 += kStep * kAhead) {
+        uint4 w[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const int i = i0 + k * kStep, j = r0 + i;
+          w[k] = i < n_rows ? ld_v4(a.q + (j / a.group) * a.q_ld + (h * a.group + j % a.group) * a.q_head + c * 8) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const int i = i0 + k * kStep, x = i % kTile;
+          uint32_t top = 0;  // of the finite values, as bits
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t v = (&w[k].x)[e], lo = v & 0x7fffu, hi = v >> 16 & 0x7fffu;
+            top = max(top, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+          }
+#pragma unroll
+          for (int o = 1; o < kChunks; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const int shift = min(141 - static_cast<int>(top >> 7), 126);  // the largest becomes 2^14 to 2^15
+          const float up = __int_as_float((127 + shift) << 23);
+          uint32_t y[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 v = mul2(unpack_bf16x2((&w[k].x)[e]), splat2(up));
+            y[e] = pack_f16x2(v.x, v.y);
+          }
+          if (i < rows_end) {
+            *reinterpret_cast<uint4*>(sm + S::q_off + (i / kTile) * S::q_tile + (c / 8) * (kTile * 128) + x * 128 + (((c % 8) ^ (x % 8)) << 4)) =
+                make_uint4(y[0], y[1], y[2], y[3]);
+            if (c == 0) row_back[i] = __int_as_float((127 - shift) << 23);
+          }
+        }
+      }
+      fence_async_smem();
+      mbar_arrive(q_full);
+    }
+    softmax_sync();
+    const float back = row_back[(shared ? s * kTile : 0) + r];
+    softmax_sync();
+    volatile int* seen = reinterpret_cast<int*>(sm + S::max_off) + s * kTile + r;
+    if (half == 0) *seen = order_of(-INFINITY);
+    stream_sync(s);
+    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t t_s = tmem + s * kTile + lanes, t_o = tmem + 2 * kTile + s * D + lanes;
+    const int steps = shared ? n_tiles : (n_tiles - s + 1) / 2;
+    const bool padding = (shared ? s * kTile : 0) + quad * 32 >= n_rows;  // a warp without rows leaves P as it is
+    float m = -INFINITY, l = 0.f;  // the base, and the sum (times 2^15)
+    for (int t = 0; t < steps; ++t) {
+      // (a wait that gave up is in the status word; the loop goes on, because the other warps meet this one at barriers)
+      mbar_wait(s_full0 + 8 * s, t & 1, a.status);
+      __syncwarp();
+      tc_fence_after();
+      if (padding) {
+        tc_fence_before();
+        stream_sync(s);
+        mbar_arrive(p_full0 + 16 * s + 8 * half);
+        continue;
+      }
+      const int tile = shared ? t : 2 * t + s;
+      const int valid = k1 - k0 - tile * kTile - half * 64;  // keys of this half tile (or more, or none)
+      const float4 info = *reinterpret_cast<const float4*>(sm + S::info_off + tile % kInfo * 16);
+      // (towards zero, so that past fp32's range it stays finite and 0 times it 0; above 0, so that masked scores stay -inf)
+        const float factor = fmaxf(__fmul_rz(info.x, back), 1.2e-38f);
+      float v[64];
+      tmem_ld_32(t_s + half * 64, v);
+      tmem_ld_32(t_s + half * 64 + 32, v + 32);
+      if (valid < 64) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i)
+          if (i >= valid) v[i] = -INFINITY;
+      }
+      float mx = v[0], mx2 = v[1];
+#pragma unroll
+      for (int i = 2; i < 64; i += 4) {
+        mx = max3_or_nan(mx, v[i], v[i + 1]);
+        if (i + 3 < 64) mx2 = max3_or_nan(mx2, v[i + 2], v[i + 3]);
+      }
+      mx = max3_or_nan(mx, mx2, mx2);  // (a score of NaN makes the row NaN, by its base)
+      // The halves' maxima meet in the row's maximum so far.  Past this barrier both halves' scores are in registers, so
+      // P may go over them.  (Neither half is ahead: S of a step was issued after both halves of the last one had read
+      // their maximum and written P.)
+      atomicMax(const_cast<int*>(seen), order_of(valid > 0 ? fmaf(mx, factor, info.y) : -INFINITY));
+      tc_fence_before();
+      stream_sync(s);
+      tc_fence_after();
+      mx = of_order(*seen);
+      const bool grows = !(mx <= m + kPass) || m == -INFINITY;
+      if (__any_sync(0xffffffffu, grows)) {
+        const float to = grows ? mx - kBelow : m;
+        const float alpha = ex2_approx(m - (to == -INFINITY ? 0.f : to));
+        if (t > 0 && half == 0) {
+          // The first half's threads rescale O: the products of this step wait for their probabilities.  Every product
+          // issued so far has finished: S of this step was issued after them.
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) {
+            float x[16];
+            uint32_t w[16];
+            tmem_ld_16(t_o + c * 16, x);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(x[i] * alpha);
+            tmem_st_16(t_o + c * 16, w);
+          }
+        }
+        l *= alpha;
+        m = to;
+      }
+      float2 scale2 = splat2(factor);
+      float2 base2 = splat2(m == -INFINITY ? 0.f : info.y - m);
+      if (__any_sync(0xffffffffu, fabsf(m) >= 16777216.f)) {
+        // Here rounding a scaled score moves it by whole units, and by more than a float's range later: round the scores as
+        // their maximum was.
+#pragma unroll
+        for (int i = 0; i < 64; ++i) v[i] = i >= valid ? -INFINITY : fmaf(v[i], factor, info.y);
+        scale2 = splat2(1.f);
+        base2 = splat2(m == -INFINITY ? 0.f : -m);
+      }
+      float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const float2 y = fma2(make_float2(v[c * 16 + i], v[c * 16 + i + 1]), scale2, base2);
+          // one pair of eight on the FMA pipe, as in the bf16 kernel
+          const float2 p = i == 6 ? exp2_fma(y) : make_float2(ex2_approx(y.x), ex2_approx(y.y));
+          sum = add2(sum, p);
+          w[i / 2] = pack_f16x2(p.x, p.y);
+        }
+        tmem_st_8(t_s + half * 32 + c * 8, w);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(p_full0 + 16 * s + 8 * half);
+      l = fmaf(sum.x + sum.y, info.z, l);
+    }
+    if (steps > 0) {
+      mbar_wait(o_full0 + 8 * s, 0, a.status);
+      __syncwarp();
+      tc_fence_after();
+    }
+    finish_rows<D>(a, sm + S::kv_off, t_o, m, l * 3.0517578125e-5f, steps, s, half, r, warp - kFirst, n_rows, r0, h, split, shared);
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int D, bool kFloat>
+static cudaError_t launch(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
+  constexpr int bytes = Smem<D>::total;
+  static SharedMemory allowed;
+  if (const cudaError_t e = allowed.at_least(reinterpret_cast<const void*>(prefix8_tc_kernel<D, kFloat>), bytes); e != cudaSuccess) return e;
+  const int units = a.row_tiles * a.kv_heads * a.prefix_splits, last = units % 148;
+  const int whole = a.prefix_splits == 1 && 2 * last <= 148 ? units - last : units;
+  const int blocks = whole + 2 * (units - whole);
+  if (a.own_splits > 0) return launch_after(prefix8_tc_kernel<D, kFloat>, blocks, kThreads, bytes, stream, a, mk, mv, whole);
+  prefix8_tc_kernel<D, kFloat><<<blocks, kThreads, bytes, stream>>>(a, mk, mv, whole);
+  return cudaGetLastError();
+}
+
+}  // namespace tc8
+
+cudaError_t launch_prefix_tc8(const Args& a, int head_dim, cudaStream_t stream) {
+  CUtensorMap mk, mv;
+  if (!q8::codes_map(&mk, a.k8, a, head_dim, tc::kTile) || !q8::codes_map(&mv, a.v8, a, head_dim, tc::kTile)) return cudaErrorInvalidValue;
+  if (a.codes == kE4m3) return head_dim == 64 ? tc8::launch<64, true>(a, mk, mv, stream) : tc8::launch<128, true>(a, mk, mv, stream);
+  return head_dim == 64 ? tc8::launch<64, false>(a, mk, mv, stream) : tc8::launch<128, false>(a, mk, mv, stream);
+}
+
+}  // namespace prefix
+
+}  // namespace mnb
