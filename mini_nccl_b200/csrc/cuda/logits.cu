@@ -20,6 +20,7 @@
 
 #include "common.cuh"
 #include "generation.h"
+#include "launch.cuh"
 
 namespace mnb {
 
@@ -27,7 +28,6 @@ namespace logits {
 
 namespace {
 
-constexpr int kThreads = 256;
 constexpr uint32_t kCount = (1u << kCountBits) - 1, kPrompt = 1u << kCountBits;  // and the bias' index + 1 above
 constexpr int kBiasShift = kCountBits + 1;
 
@@ -43,19 +43,18 @@ MNB_DEVICE float adjusted(float x, uint32_t named, float repetition, float prese
   return x;
 }
 
-// Groups of 16 bytes (8 or 4 tokens) of a row, kPer for each thread, one chunk for each block.
-template <bool kBf16, int kPer>
-__global__ void __launch_bounds__(kThreads, 5) adjust_kernel(const __grid_constant__ Adjust a, int chunks) {
-  constexpr int kGroup = kBf16 ? 8 : 4, kSize = kBf16 ? 2 : 4, kTokens = kThreads * kPer * kGroup;
-  constexpr int kBatch = kPer < 4 ? kPer : 4;  // groups whose loads are under way together
-  constexpr int kList = 1024;
+// A block takes kThreads * kPer groups of eight tokens of a row.
+template <bool kBf16, int kThreads, int kPer>
+__global__ void __launch_bounds__(kThreads, kThreads == 512 ? 3 : 6) adjust_kernel(const __grid_constant__ Adjust a, int chunks) {
+  constexpr int kSize = kBf16 ? 2 : 4, kWords = kBf16 ? 4 : 8, kTokens = kThreads * kPer * 8, kList = 1024;
   static_assert(kTokens <= 1 << 14, "a place's bits");
-  __shared__ uint32_t named[kTokens], list[kList];
+  extern __shared__ uint32_t named[];  // [kTokens], where some list names tokens
+  __shared__ uint32_t list[kList];
   __shared__ int listed;
   const int row = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
   const char* const in = static_cast<const char*>(a.in) + row * a.in_ld * kSize;
   char* const out = static_cast<char*>(a.out) + row * a.out_ld * kSize;
-  // The groups follow the output's alignment: the row's first token is number `skip` of the first group.
+  // The groups follow the output's alignment to 16 bytes: the row's first token is number `skip` of the first group.
   const int skip = static_cast<int>(reinterpret_cast<uintptr_t>(out) % 16) / kSize;
   const int first = chunk * kTokens - skip;  // the chunk's first token (below 0: before the row)
   const bool in_aligned = reinterpret_cast<uintptr_t>(in + first * kSize) % 16 == 0;
@@ -90,9 +89,12 @@ __global__ void __launch_bounds__(kThreads, 5) adjust_kernel(const __grid_consta
       for (int k = 0; k < kAhead; ++k) v[k] = i0 + k * kThreads < n ? id_at(t, row * t.ld + i0 + k * kThreads) : -1;
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
-        if (v[k] >= a.vocab && chunk == 0) atomicCAS(a.status, 0, kErrBadIndex);
-        const long long at = v[k] - first;
-        if (v[k] >= 0 && v[k] < a.vocab && at >= 0 && at < kTokens) f(static_cast<uint32_t>(at) | kind << 14 | (kind == 2 ? i0 + k * kThreads : 0) << 16);
+        const uint32_t at = static_cast<uint32_t>(v[k]) - static_cast<uint32_t>(first);
+        if (static_cast<unsigned long long>(v[k]) >= static_cast<unsigned long long>(a.vocab)) {
+          if (v[k] >= 0 && chunk == 0) atomicCAS(a.status, 0, kErrBadIndex);
+        } else if (at < kTokens) {
+          f(at | kind << 14 | (kind == 2 ? i0 + k * kThreads : 0) << 16);
+        }
       }
     }
   };
@@ -132,68 +134,71 @@ __global__ void __launch_bounds__(kThreads, 5) adjust_kernel(const __grid_consta
   }
 
   // The copy, under the mask
-  constexpr uint32_t kAll = (1u << kGroup) - 1;
   if (!a.in_place || mask) {
-#pragma unroll 1
-    for (int b = 0; b < kPer; b += kBatch) {
-      auto token_of = [&](int k) { return first + ((b + k) * kThreads + static_cast<int>(threadIdx.x)) * kGroup; };
-      uint32_t allowed[kBatch];
+    auto token_of = [&](int k) { return first + (k * kThreads + static_cast<int>(threadIdx.x)) * 8; };
+    uint32_t allowed[kPer];  // of each group's tokens
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const int v = token_of(k);
-        allowed[k] = kAll;
-        if (mask && v < a.vocab && v + kGroup > 0) {
-          const int at = max(v, 0), w = at >> 5;
-          const uint32_t lo = mask[w], hi = w + 1 < words && (at & 31) + kGroup > 32 ? mask[w + 1] : 0u;
-          allowed[k] = (__funnelshift_r(lo, hi, at & 31) << (at - v)) & kAll;
+    for (int k = 0; k < kPer; ++k) {
+      const int v = token_of(k);
+      allowed[k] = 0xff;
+      if (mask && v < a.vocab && v + 8 > 0) {
+        const int at = max(v, 0), w = at >> 5;
+        const uint32_t lo = mask[w], hi = w + 1 < words && (at & 31) > 24 ? mask[w + 1] : 0u;
+        allowed[k] = (__funnelshift_r(lo, hi, at & 31) << (at - v)) & 0xff;
+      }
+    }
+    uint32_t x[kPer][kWords];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int v = token_of(k);
+#pragma unroll
+      for (int e = 0; e < kWords; ++e) x[k][e] = 0;
+      if (v >= a.vocab || !allowed[k] || (a.in_place && allowed[k] == 0xff)) continue;
+      if (in_aligned && v >= 0 && v + 8 <= a.vocab) {
+#pragma unroll
+        for (int q = 0; q < kWords / 4; ++q) {
+          const uint4 y = ld_v4(in + static_cast<long long>(v) * kSize + 16 * q);
+          x[k][4 * q] = y.x, x[k][4 * q + 1] = y.y, x[k][4 * q + 2] = y.z, x[k][4 * q + 3] = y.w;
+        }
+        continue;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (v + e >= 0 && v + e < a.vocab) {
+          if constexpr (kBf16)
+            x[k][e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(in)[v + e]) << (e % 2 * 16);
+          else
+            x[k][e] = reinterpret_cast<const uint32_t*>(in)[v + e];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int v = token_of(k);
+      if (v >= a.vocab || (a.in_place && allowed[k] == 0xff)) continue;
+      if (allowed[k] != 0xff) {
+#pragma unroll
+        for (int e = 0; e < kWords; ++e) {
+          if constexpr (kBf16) {
+            const uint32_t two = allowed[k] >> 2 * e, keep = (two & 1u) * 0xffffu | (two >> 1 & 1u) * 0xffff0000u;
+            x[k][e] = (x[k][e] & keep) | (0xff80ff80u & ~keep);
+          } else {
+            x[k][e] = allowed[k] >> e & 1 ? x[k][e] : 0xff800000u;
+          }
         }
       }
-      uint4 x[kBatch];
+      if (v >= 0 && v + 8 <= a.vocab) {
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const int v = token_of(k);
-        x[k] = make_uint4(0, 0, 0, 0);
-        if (v >= a.vocab || !allowed[k] || (a.in_place && allowed[k] == kAll)) continue;
-        if (in_aligned && v >= 0 && v + kGroup <= a.vocab) {
-          x[k] = ld_v4(in + static_cast<long long>(v) * kSize);
-          continue;
-        }
+        for (int q = 0; q < kWords / 4; ++q)
+          st_v4(out + static_cast<long long>(v) * kSize + 16 * q, make_uint4(x[k][4 * q], x[k][4 * q + 1], x[k][4 * q + 2], x[k][4 * q + 3]));
+      } else {
 #pragma unroll
-        for (int e = 0; e < kGroup; ++e)
+        for (int e = 0; e < 8; ++e)
           if (v + e >= 0 && v + e < a.vocab) {
             if constexpr (kBf16)
-              (&x[k].x)[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(in)[v + e]) << (e % 2 * 16);
+              reinterpret_cast<uint16_t*>(out)[v + e] = static_cast<uint16_t>(x[k][e / 2] >> (e % 2 * 16));
             else
-              (&x[k].x)[e] = reinterpret_cast<const uint32_t*>(in)[v + e];
+              reinterpret_cast<uint32_t*>(out)[v + e] = x[k][e];
           }
-      }
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const int v = token_of(k);
-        if (v >= a.vocab || (a.in_place && allowed[k] == kAll)) continue;
-        if (allowed[k] != kAll) {
-#pragma unroll
-          for (int e = 0; e < kGroup; ++e)
-            if (!(allowed[k] >> e & 1)) {
-              uint32_t& w = (&x[k].x)[kBf16 ? e / 2 : e];
-              if constexpr (kBf16)
-                w = e % 2 ? (w & 0xffffu) | 0xff800000u : (w & 0xffff0000u) | 0xff80u;
-              else
-                w = 0xff800000u;
-            }
-        }
-        if (v >= 0 && v + kGroup <= a.vocab) {
-          st_v4(out + static_cast<long long>(v) * kSize, x[k]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < kGroup; ++e)
-            if (v + e >= 0 && v + e < a.vocab) {
-              if constexpr (kBf16)
-                reinterpret_cast<uint16_t*>(out)[v + e] = static_cast<uint16_t>((&x[k].x)[e / 2] >> (e % 2 * 16));
-              else
-                reinterpret_cast<uint32_t*>(out)[v + e] = (&x[k].x)[e];
-            }
-        }
       }
     }
   }
@@ -219,22 +224,26 @@ __global__ void __launch_bounds__(kThreads, 5) adjust_kernel(const __grid_consta
   });
 }
 
-template <bool kBf16, int kPer>
+template <bool kBf16, int kThreads, int kPer>
 cudaError_t launch(const Adjust& a, cudaStream_t stream) {
-  constexpr int kGroup = kBf16 ? 8 : 4, kTokens = kThreads * kPer * kGroup;
-  const int chunks = (a.vocab + kGroup - 1 + kTokens - 1) / kTokens;  // (a row may begin inside its first group)
-  adjust_kernel<kBf16, kPer><<<static_cast<unsigned>(a.rows) * chunks, kThreads, 0, stream>>>(a, chunks);
+  constexpr int kTokens = kThreads * kPer * 8;
+  const int chunks = (a.vocab + 7 + kTokens - 1) / kTokens;  // (a row may begin inside its first group)
+  const bool names = a.prompt.n > 0 || a.history.n > 0 || a.bias_tokens.n > 0;
+  const int bytes = names ? kTokens * 4 : 0;
+  static SharedMemory allowed;
+  if (const cudaError_t e = allowed.at_least(reinterpret_cast<const void*>(adjust_kernel<kBf16, kThreads, kPer>), bytes, kTokens * 4); e != cudaSuccess) return e;
+  adjust_kernel<kBf16, kThreads, kPer><<<static_cast<unsigned>(a.rows) * chunks, kThreads, bytes, stream>>>(a, chunks);
   return cudaGetLastError();
 }
 
 }  // namespace
 
 cudaError_t launch_adjust(const Adjust& a, cudaStream_t stream) {
-  // 16 KB of a row to a block, so that few blocks read a row's lists; 4 KB where that would leave SMs without one
+  // 32 KB of a row to a block, so that few blocks read a row's lists; 4 KB (fp32: 8) where that would leave SMs without one
   const int size = a.bf16 ? 2 : 4;
-  const bool few = static_cast<long long>(a.rows) * ((a.vocab * size + 16383) / 16384) < 148;
-  if (a.bf16) return few ? launch<true, 1>(a, stream) : launch<true, 4>(a, stream);
-  return few ? launch<false, 1>(a, stream) : launch<false, 4>(a, stream);
+  const bool few = static_cast<long long>(a.rows) * ((a.vocab * size + 32767) / 32768) < 148;
+  if (a.bf16) return few ? launch<true, 256, 1>(a, stream) : launch<true, 512, 4>(a, stream);
+  return few ? launch<false, 256, 1>(a, stream) : launch<false, 512, 2>(a, stream);
 }
 
 }  // namespace logits

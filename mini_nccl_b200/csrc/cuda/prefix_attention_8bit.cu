@@ -6,9 +6,10 @@
 // With codes c, scales a (keys) and b (values), s_j = scale q . k_j = (scale a_j) (q . c_j),
 // and with w_j = b_j exp(s_j) = exp(s_j + log b_j) a part's output is sum w_j c_j: the
 // scale of the values rides in the exponent, so weights and codes are both what the
-// product takes as f16.  A row's base is the running maximum of s_j + log2 b_j less
-// 15, so the largest weight is 2^15 and f16 holds weights down to 2^-39 of it (to 11
-// bits down to 2^-29).  The sum of exp(s_j) gets w_j / b_j in fp32.  Codes are exact in
+// product takes as f16.  A row's base lies 9 below a maximum of s_j + log2 b_j and moves
+// when one passes it by 15, so the largest weight is at most 2^15 and f16 holds weights
+// down to 2^-33 of the largest (to 11 bits down to 2^-23).  The sum of exp(s_j) gets
+// w_j / b_j in fp32.  Codes are exact in
 // f16.  So are queries but for values below 2^-31 of their row's largest: each row is
 // scaled by a power of two, which the scores' factor takes back.
 //
@@ -34,7 +35,8 @@ namespace prefix {
 namespace q8 {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
-constexpr int kStep = 32;  // keys of a stage
+constexpr int kStep = 64;  // keys of a stage (2^6)
+constexpr float kBelow = 9.f, kPass = 15.f;  // the base below the maximum, and what a score may lie above the base
 constexpr int kTensorCoreRows = 16;  // more rows of a kv head than this go to the tensor-core kernel
 constexpr int kMostKnown = 1024;  // sequences whose lengths a block keeps
 
@@ -42,8 +44,10 @@ template <int D, int NT>
 struct Ring {
   // (sixteen rows need more registers)
   static constexpr int blocks = (D == 128 ? 3 : 4) - (NT == 2 && D > 32);  // per SM
-  static constexpr int stages = D == 128 && NT == 1 ? 2 : 3;
-  static constexpr uint32_t tile = kStep * D;        // of K; V follows
+  // A stage's keys and its values each have a place of their own, which the next ones take as soon as it is free: at head dim
+  // 128 the keys come while the weights and values are worked on, and the values while the next scores are.
+  static constexpr int stages = D == 128 ? 1 : 2;
+  static constexpr uint32_t tile = kStep * D;           // of keys, or values
   static constexpr uint32_t bytes = stages * 2 * tile;  // of a warp
   // 16-byte chunk c of row r, as TMA's swizzle leaves it
   MNB_DEVICE static uint32_t at(int r, int c) {
@@ -59,12 +63,16 @@ MNB_DEVICE int key_of(int i) {
   return D == 128 ? (i >> 1) | ((i & 1) << 2) : i;
 }
 
+// (not volatile, as the widening: they may move between the loads)
 MNB_DEVICE void mma_f16(float* c, const uint32_t* a, const uint32_t* b) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+MNB_DEVICE uint32_t nan_bytes(uint32_t w) {  // 1 in each byte that is e4m3's NaN
+  return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
 }
 MNB_DEVICE uint32_t transposed(uint32_t x) {  // of an 8 x 8 matrix of 16-bit values, a row's pair in each lane
   uint32_t y;
@@ -80,16 +88,22 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NT>::blocks)
   constexpr int kStages = R::stages, kU = kStep / 16, kRows = 8 * NT, kMt = D / 16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t bars[kWarps][kStages];
-  __shared__ float scale_of[kWarps][kStages][2][4];  // of a stage's pages: keys, values
+  __shared__ uint64_t bars[kWarps][2 * kStages];
+  __shared__ float scale_of[kWarps][kStages][2][8];  // of a stage's pages: keys, values
+  __shared__ float4 factor_of[kWarps][8];            // of each eight keys of the stage that is worked on
+  __shared__ uint32_t nan_at[kFloat ? kWarps : 1][kRows][D / 32];  // outputs that have to become NaN, a bit each
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-  const uint32_t ring = smem_u32(sm) + warp * R::bytes, bar0 = smem_u32(bars[warp]), sc0 = smem_u32(scale_of[warp]);
-  if (lane < kStages) mbar_init(bar0 + 8 * lane, 33);  // the expected bytes, and every lane's copies of scales
+  const uint32_t ring = smem_u32(sm) + warp * R::bytes, full_k = smem_u32(bars[warp]), full_v = full_k + 8 * kStages,
+                 sc0 = smem_u32(scale_of[warp]);
+  if (lane < kStages) {
+    mbar_init(full_k + 8 * lane, 33);  // the expected bytes, and every lane's copies of scales
+    mbar_init(full_v + 8 * lane, 1);
+  }
   fence_mbar_init();
-  if (lane < kStages * 8) (&scale_of[warp][0][0][0])[lane] = 1.f;  // (a stage's pages may be fewer than it has room for)
+  for (int x = lane; x < kStages * 16; x += 32) (&scale_of[warp][0][0][0])[x] = 1.f;  // (a stage's pages may be fewer than it has room for)
   int* lens = reinterpret_cast<int*>(sm + kWarps * R::bytes);
   int* offsets = lens + known;
-  int* tiles_before = offsets + known + 1;  // of 32 keys, of the sequences before each one
+  int* tiles_before = offsets + known + 1;  // of 64 keys, of the sequences before each one
   for (int b = threadIdx.x; b < known; b += kThreads) lens[b] = a.seq_lens[b];
   if (a.q_offsets)
     for (int b = threadIdx.x; b < known + (known > 0); b += kThreads) offsets[b] = a.q_offsets[b];
@@ -97,14 +111,16 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NT>::blocks)
   const int* const q_offsets = known ? offsets : a.q_offsets;
   __syncthreads();
   let_next_start();
-  const int warps = kWarps * gridDim.x, self = blockIdx.x + warp * gridDim.x;
-
-  // Shares (least > 0: single new tokens).  The tiles of 32 keys of all (part, row tile, kv head), the prefix first, lie in
-  // one row, and every warp takes as many of them, `share`, as every other: a part whose tiles several warps have gets
-  // partial results in slots one after another.  (`least` keeps them as few as there are slots.)
+  // Shares (least > 0: single new tokens).  The tiles of 64 keys of all (part, row tile, kv heads), the prefix first, lie in
+  // one row, and every worker takes as many of them, `share`, as every other: a part whose tiles several workers have gets
+  // partial results in slots one after another.  (`least` keeps them as few as there are slots.)  A worker is as many warps
+  // of a block as heads are taken at once: then they load what lies together in memory (48 sequences of up to 6001 tokens,
+  // 8 kv heads: 75 us for a warp and one head each).
   // Otherwise items, pieces of one (part, row tile, kv head, range of keys), in turn over the warps.
-  const int own_units = a.own_splits > 0 ? a.own_tiles * a.kv_heads : 0;
-  const int prefix_tiles = a.tensor_cores ? 0 : (a.prefix_len + kStep - 1) / kStep, prefix_units = a.row_tiles * a.kv_heads;
+  const int at_once = least == 0 ? 1 : a.kv_heads % 4 == 0 ? 4 : a.kv_heads % 2 == 0 ? 2 : 1, head_groups = a.kv_heads / at_once;
+  const int warps = kWarps / at_once * gridDim.x, self = blockIdx.x + warp / at_once * gridDim.x;
+  const int own_units = a.own_splits > 0 ? a.own_tiles * head_groups : 0;
+  const int prefix_tiles = a.tensor_cores ? 0 : (a.prefix_len + kStep - 1) / kStep, prefix_units = a.row_tiles * head_groups;
   long long of_prefix = 0, from = 0, end = 0, share = 1;
   if (least > 0) {
     if (warp == 0) {
@@ -129,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NT>::blocks)
     share = max((all + warps - 1) / warps, static_cast<long long>(least));
     from = min(all, self * share), end = min(all, from + share);
   }
-  // The piece of this warp that begins at `at` (a tile, or an item), or else the first one behind it; `at` moves past it.
+  // This warp's piece that begins at `at` (a tile, or an item), or else the first one behind it; `at` moves past it.
   auto next = [&](long long& at, Piece& p, int& part_end) {
     if (least == 0) {
       if (at >= items) return false;
@@ -159,8 +175,8 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NT>::blocks)
     const int len = b < 0 ? a.prefix_len : lens[b], most = static_cast<int>(min(end - at, static_cast<long long>(tiles - tile)));
     const int segment = self - static_cast<int>((at - tile) / share);
     part_end = len;
-    p.h = unit % a.kv_heads;
-    p.r0 = unit / a.kv_heads * kRows;
+    p.h = unit % head_groups * at_once + warp % at_once;
+    p.r0 = unit / head_groups * kRows;
     p.k0 = tile * kStep;
     p.k1 = min(len, p.k0 + most * kStep);
     p.limit0 = kUnlimited;
@@ -184,8 +200,8 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NT>::blocks)
     return true;
   };
 
-  // Loading runs ahead of the work by the stages of the ring, on into the next pieces.
-  const int per = min(1 << a.page_shift, kStep);  // tokens of a box
+  // Loading runs ahead of the work, on into the next pieces.
+  const int per_shift = min(a.page_shift, 6), per = 1 << per_shift;  // tokens of a box
   long long load_at = least ? from : self;
   bool loading = true;
   int load_key = 0, load_end = 0, load_head = 0, batch = 0, ids_end = 0, issued = 0;
@@ -205,39 +221,52 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NT>::blocks)
       return;
     }
   };
-  auto issue = [&] {
+  // The keys of the next stage, a box for each of the first lanes, and the scales of both; its values follow.
+  int box_page = 0, box_token = 0, box_head = 0, boxes = 0;
+  auto issue_keys = [&] {
+    boxes = 0;
     if (!loading) return;
     if ((load_key >> a.page_shift) - batch >= 32) {
       batch += 32;
       ids_now = ids_next;
       ids_next = fetch(batch + 32);
     }
-    const int st = issued % kStages, boxes = (min(kStep, load_end - load_key) + per - 1) / per;
-    const uint32_t bar = bar0 + 8 * st;
-    // lanes 0 to 3 fetch the keys of a box each, 4 to 7 the values
-    const int box = lane & 3, part = lane >> 2;
-    int page = __shfl_sync(0xffffffffu, ids_now, (load_key >> a.page_shift) - batch + min(box, boxes - 1));
-    if (lane == 0) mbar_arrive_expect_tx(bar, boxes * per * D * 2);
+    const int st = issued % kStages;
+    const uint32_t bar = full_k + 8 * st;
+    boxes = (min(kStep, load_end - load_key) + per - 1) >> per_shift;
+    box_page = __shfl_sync(0xffffffffu, ids_now, ((load_key >> a.page_shift) - batch + lane) & 31);
+    box_token = (load_key + lane * per) & ((1 << a.page_shift) - 1), box_head = load_head;
+    if (lane == 0) mbar_arrive_expect_tx(bar, boxes * per * D);
     __syncwarp();
-    if (lane < 8 && box < boxes) {
-      const bool there = page >= 0 && page < a.pages;
+    if (lane < boxes) {
+      const bool there = box_page >= 0 && box_page < a.pages;
+      const long long at = there ? box_page * a.scale_ld + load_head * a.scale_head : 0;
       if (!there) {
         flag(a);
-        page = a.no_page;  // reads as zeros
+        box_page = a.no_page;  // reads as zeros
       }
-      const int key = load_key + box * per;
-      tma_load_4d(ring + (st * 2 + part) * R::tile + box * per * D, part ? &map_v : &map_k, 0, load_head,
-                  key & ((1 << a.page_shift) - 1), page, bar);
-      const float* s = part ? a.v_scales : a.k_scales;
-      copy_float(sc0 + ((st * 2 + part) * 4 + box) * 4, there ? s + page * a.scale_ld + load_head * a.scale_head : s, there);
+      tma_load_4d(ring + st * 2 * R::tile + lane * per * D, &map_k, 0, load_head, box_token, box_page, bar);
+      copy_float(sc0 + (st * 16 + lane) * 4, a.k_scales + at, there);
+      copy_float(sc0 + (st * 16 + 8 + lane) * 4, a.v_scales + at, there);
     }
     arrive_after_copies(bar);
-    ++issued;
     load_key += kStep;
     if (load_key >= load_end) next_piece();
   };
+  auto issue_values = [&] {
+    if (boxes == 0) return;
+    const int st = issued % kStages;
+    const uint32_t bar = full_v + 8 * st;
+    if (lane == 0) mbar_arrive_expect_tx(bar, boxes * per * D);
+    __syncwarp();
+    if (lane < boxes) tma_load_4d(ring + (st * 2 + 1) * R::tile + lane * per * D, &map_v, 0, box_head, box_token, box_page, bar);
+    ++issued;
+  };
   next_piece();
-  for (int s = 0; s < kStages; ++s) issue();
+  for (int s = 0; s < kStages; ++s) {
+    issue_keys();
+    issue_values();
+  }
 
   // Where this lane reads: row g (and g + 8) of 16 keys as the first operand of K Q^T, and the rows of ldmatrix for V^T P^T
   const uint32_t at_k = D == 32 ? R::at(g, t >> 1) + (t & 1) * 8 : R::at(key_of<D>(g), t);
@@ -311,9 +340,17 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NT>::blocks)
 
     for (int t0 = p.k0; t0 < p.k1; t0 += kStep, ++pos) {
       const int st = pos % kStages;
-      mbar_wait(bar0 + 8 * st, (pos / kStages) & 1, a.status);  // (a wait that gave up is in the status word)
+      const uint32_t phase = (pos / kStages) & 1;
+      mbar_wait(full_k + 8 * st, phase, a.status);  // (a wait that gave up is in the status word)
       __syncwarp();
       const uint32_t sK = ring + st * 2 * R::tile, sV = sK + R::tile;
+      // Each eight keys lie in one page: its factor of the scores, the logarithm of its values' scale, and what turns a
+      // weight into its part of the sum (times 2^15, so that nothing leaves the range of fp32).
+      if (lane < 8) {
+        const int box = (lane * 8) >> a.page_shift;
+        const float b = __log2f(fmaxf(scale_of[warp][st][1][box], kLeastScale));  // (a page of zeros may have any scale)
+        factor_of[warp][lane] = make_float4(scale_of[warp][st][0][box] * a.scale_log2, b, ex2_approx(15.f - b), 0.f);
+      }
       float s[NT][kU][4];
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
@@ -340,123 +377,142 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NT>::blocks)
           }
         }
       }
-      // Each eight keys lie in one page: its factor of the scores, the logarithm of its values' scale, and what turns a
-      // weight into its part of the sum (times 2^15, so that nothing leaves the range of fp32).
-      const int box = min((lane & 3) * 8 >> a.page_shift, 3);
-      const float mine_v = fmaxf(scale_of[warp][st][1][box], kLeastScale);  // (a page of zeros may have any scale)
-      const float mine_k = scale_of[warp][st][0][box] * a.scale_log2, mine_b = __log2f(mine_v), mine_r = ex2_approx(15.f - mine_b);
-      const bool masked = t0 + kStep > whole;
-      float top[NT][2];
+      __syncwarp();  // (the keys and scales have been read)
+      issue_keys();
       float sum_of[kU][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
 #pragma unroll
       for (int u = 0; u < kU; ++u)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float fk = __shfl_sync(0xffffffffu, mine_k, 2 * u + h), fb = __shfl_sync(0xffffffffu, mine_b, 2 * u + h);
-          sum_of[u][h] = __shfl_sync(0xffffffffu, mine_r, 2 * u + h);
+          const float4 f = factor_of[warp][2 * u + h];
+          sum_of[u][h] = f.z;
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
+            for (int e = 0; e < 2; ++e)
               // (towards zero: a factor past fp32's range stays finite, and 0 times it stays 0)
-              float x = fmaf(s[n][u][2 * h + e], __fmul_rz(fk, back[n][e]), fb);
-              if (masked && t0 + u * 16 + h * 8 + key_of<D>(g) >= lim[n][e]) x = -INFINITY;
-              s[n][u][2 * h + e] = x;
-              top[n][e] = fmaxf(top[n][e], x);
-            }
+              s[n][u][2 * h + e] = fmaf(s[n][u][2 * h + e], __fmul_rz(f.x, back[n][e]), f.y);
         }
-      uint32_t pf[NT][kU][2];
+      const bool masked = t0 + kStep > whole;
+      if (masked) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float from[2];
-        bool moved = false;
-        float alpha[2];
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int u = 0; u < kU; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (t0 + u * 16 + e / 2 * 8 + key_of<D>(g) >= lim[n][e & 1]) s[n][u][e] = -INFINITY;
+      }
+      float top[NT][2];
+      bool grows = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], 4));
-          top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], 8));
-          top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], 16));
-          const float to = fmaxf(base[n][e], top[n][e] - 15.f);
-          from[e] = to == -INFINITY ? 0.f : to;  // no key yet: every weight is exp2(-inf) = 0
-          alpha[e] = ex2_approx(base[n][e] - from[e]);
-          moved = moved || alpha[e] != 1.f;
-          base[n][e] = to;
+          float x = fmaxf(s[n][0][e], s[n][0][2 + e]);
+#pragma unroll
+          for (int u = 1; u < kU; ++u) x = max3f(x, s[n][u][e], s[n][u][2 + e]);
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          top[n][e] = x;
+          grows = grows || x > base[n][e] + kPass || (base[n][e] == -INFINITY && x > -INFINITY);
         }
-        if (__any_sync(0xffffffffu, moved)) {  // some row of the warp has a new maximum
-          l[n][0] *= alpha[0], l[n][1] *= alpha[1];
+      if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float alpha[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float to = top[n][e] > base[n][e] + kPass || base[n][e] == -INFINITY ? top[n][e] - kBelow : base[n][e];
+            alpha[e] = to == base[n][e] ? 1.f : ex2_approx(base[n][e] - to);
+            l[n][e] *= alpha[e];
+            base[n][e] = to;
+          }
 #pragma unroll
           for (int m = 0; m < kMt; ++m)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[n][m][e] *= alpha[e & 1];
         }
+      }
+      uint32_t pf[NT][kU][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        // (no key yet: every weight is exp2(-inf) = 0)
+        const float from0 = base[n][0] == -INFINITY ? 0.f : base[n][0], from1 = base[n][1] == -INFINITY ? 0.f : base[n][1];
 #pragma unroll
         for (int u = 0; u < kU; ++u)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float w0 = ex2_approx(s[n][u][2 * h] - from[0]), w1 = ex2_approx(s[n][u][2 * h + 1] - from[1]);
+            const float w0 = ex2_approx(s[n][u][2 * h] - from0), w1 = ex2_approx(s[n][u][2 * h + 1] - from1);
             l[n][0] = fmaf(w0, sum_of[u][h], l[n][0]);
             l[n][1] = fmaf(w1, sum_of[u][h], l[n][1]);
             pf[n][u][h] = transposed(pack_f16x2(w0, w1));
           }
       }
-      // A key that a row does not see has weight 0, and 0 times a value that is no number (e4m3 has one; also past the end of
-      // the keys, where a page holds anything) would be NaN: such codes count as zeros here, and rows that see one are told.
-      auto values = [&](auto careful) {
-#pragma unroll
-        for (int u = 0; u < kU; ++u)
-#pragma unroll
-          for (int c = 0; c < kMt / 2; ++c) {
-            uint32_t w[4];
-            ldsm_x4_t(w, (sV + u * 16 * D + at_v) ^ (c * 32));
-            if constexpr (decltype(careful)::value) {
-              uint32_t nan[4], any = 0;
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                nan[k] = (((w[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;  // 1 in each byte that is NaN
-                w[k] &= ~(nan[k] * 0xffu);
-                any |= nan[k];
-              }
-              if (__any_sync(0xffffffffu, any != 0)) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                  uint32_t sees[2];
-#pragma unroll
-                  for (int h = 0; h < 2; ++h) {
-                    const int key = t0 + u * 16 + h * 8 + key_of<D>(g);
-                    sees[h] = transposed((key < lim[n][0] ? 0x3c00u : 0u) | (key < lim[n][1] ? 0x3c000000u : 0u));
-                  }
-#pragma unroll
-                  for (int m = 0; m < 2; ++m) {
-                    // (0x3c00 is 1 in f16)
-                    const uint32_t f[4] = {(nan[2 * m] & 0x10001u) * 0x3c00u, ((nan[2 * m] >> 8) & 0x10001u) * 0x3c00u,
-                                           (nan[2 * m + 1] & 0x10001u) * 0x3c00u, ((nan[2 * m + 1] >> 8) & 0x10001u) * 0x3c00u};
-                    float count[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma_f16(count, f, sees);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                      if (count[e] > 0.f) o[n][2 * c + m][e] = NAN;
-                  }
-                }
-              }
-            }
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-              uint32_t f[4];
-              widen<kFloat>(w[2 * m], f[0], f[1]);
-              widen<kFloat>(w[2 * m + 1], f[2], f[3]);
-#pragma unroll
-              for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * c + m], f, pf[n][u]);
-            }
-          }
-      };
-      if (kFloat && masked)
-        values(std::bool_constant<kFloat>{});
-      else
-        values(std::false_type{});
+      mbar_wait(full_v + 8 * st, phase, a.status);
       __syncwarp();
-      issue();
+      bool spoiled = false;
+      if constexpr (kFloat) {
+        // A key that a row does not see has weight 0, and 0 times NaN (which e4m3 has, also past the end of the keys, where
+        // a page holds anything) would be NaN: such codes become zeros here, and rows that do see one become NaN below.
+        if (masked) {
+          uint32_t some = 0;
+          for (int x = lane; x < kStep * D / 16; x += 32) {
+            uint4 w;
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(sV + x * 16));
+            some |= nan_bytes(w.x) | nan_bytes(w.y) | nan_bytes(w.z) | nan_bytes(w.w);
+          }
+          spoiled = __any_sync(0xffffffffu, some != 0);
+          if (spoiled) {
+            for (int x = lane; x < kRows * (D / 32); x += 32) (&nan_at[warp][0][0])[x] = 0;
+            __syncwarp();
+#pragma unroll 1
+            for (int x = lane; x < kStep * D / 4; x += 32) {  // word by word
+              const int key = x / (D / 4), word = x % (D / 4);
+              const uint32_t at = sV + R::at(key, word / 4) + word % 4 * 4;
+              uint32_t w;
+              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at));
+              const uint32_t odd = nan_bytes(w);
+              if (!odd) continue;
+              asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(w & ~(odd * 0xffu)) : "memory");
+              const uint32_t bits = ((odd & 1u) | (odd >> 7 & 2u) | (odd >> 14 & 4u) | (odd >> 21 & 8u)) << (word % 8 * 4);
+              for (int row = 0; row < p.n_rows; ++row)
+                if (t0 + key < min(p.k1, p.limit0 + (p.r0 + row) / a.group)) atomicOr(&nan_at[warp][row][word / 8], bits);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // TMA writes here next
+            __syncwarp();
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+#pragma unroll
+        for (int c = 0; c < kMt / 2; ++c) {
+          uint32_t w[4];
+          ldsm_x4_t(w, (sV + u * 16 * D + at_v) ^ (c * 32));
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            uint32_t f[4];
+            widen<kFloat>(w[2 * m], f[0], f[1]);
+            widen<kFloat>(w[2 * m + 1], f[2], f[3]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * c + m], f, pf[n][u]);
+          }
+        }
+      if (kFloat && spoiled) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int m = 0; m < kMt; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int dim = m * 16 + 2 * g + e / 2;
+              if (nan_at[warp][n * 8 + 2 * t + e % 2][dim / 32] >> (dim % 32) & 1) o[n][m][e] = NAN;
+            }
+      }
+      __syncwarp();
+      issue_values();
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -481,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NT>::blocks)
       }
   }
   // Sequences without tokens have no partial results at all.
-  if (least > 0)
+  if (least > 0 && warp % at_once == 0)
     for (int b = self; b < known; b += warps)
       if (tiles_before[b + 1] == tiles_before[b]) {
         if (lane == 0 && lens[b] != 0) flag(a);  // (a length out of its bounds)
@@ -491,7 +547,10 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NT>::blocks)
           a.part_ml[(static_cast<long long>(a.prefix_splits + x / a.heads) * a.n + n0) * a.heads + x % a.heads] = make_float2(-INFINITY, 0.f);
       }
   // The block does not end before its last copies have arrived, also where a wait was given up.
-  for (int k = max(0, issued - kStages); k < issued; ++k) mbar_wait(bar0 + 8 * (k % kStages), (k / kStages) & 1, nullptr);
+  for (int k = max(0, issued - kStages); k < issued; ++k) {
+    mbar_wait(full_k + 8 * (k % kStages), (k / kStages) & 1, nullptr);
+    mbar_wait(full_v + 8 * (k % kStages), (k / kStages) & 1, nullptr);
+  }
   if (a.sound && blockIdx.x == 0 && warp == 0) {
     const bool sound = offsets_sound(a, q_offsets);
     if (lane == 0) {
@@ -510,7 +569,7 @@ static cudaError_t launch(const Args& a, const CUtensorMap& mk, const CUtensorMa
   if (!a.tensor_cores) items += static_cast<long long>(a.row_tiles) * a.kv_heads * a.prefix_splits;
   static SharedMemory allowed;
   if (const cudaError_t e = allowed.at_least(reinterpret_cast<const void*>(pieces8_kernel<D, NT, kFloat>), bytes); e != cudaSuccess) return e;
-  const int per_sm = std::max(1, std::min(R::blocks, 227 * 1024 / (bytes + 1024 + 512)));
+  const int per_sm = std::max(1, std::min(R::blocks, 227 * 1024 / (bytes + 1024 + 2048)));
   const int blocks = static_cast<int>(std::min<long long>(items, 148 * per_sm));
   pieces8_kernel<D, NT, kFloat><<<blocks, kThreads, bytes, stream>>>(a, mk, mv, static_cast<int>(items), known, a.least_share);
   return cudaGetLastError();

@@ -49,20 +49,14 @@ MNB_DEVICE void widen_any(uint32_t w, uint32_t& lo, uint32_t& hi) {
   else
     widen<false>(w, lo, hi);
 }
-// The same in the bytes' order.
-template <bool kFloat>
-MNB_DEVICE void widen_in_order(uint32_t w, uint32_t& first, uint32_t& second) {
-  if constexpr (kFloat) {
-    widen_any<true>(w, first, second);
-  } else {
-    w ^= 0x80808080u;
-    first = sub_f16x2(__byte_perm(w, 0x64646464u, 0x4140), 0x64806480u);
-    second = sub_f16x2(__byte_perm(w, 0x64646464u, 0x4342), 0x64806480u);
-  }
-}
 MNB_DEVICE uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   uint32_t y;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
+MNB_DEVICE uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t y;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(a), "r"(b), "r"(c));
   return y;
 }
 MNB_DEVICE void copy_float(uint32_t dst, const float* src, bool there) {  // zero where not

@@ -33,11 +33,11 @@ namespace tc8 {
 using namespace tc;
 using namespace q8;
 
-constexpr int kWiden = 128;                       // threads that widen codes, a row of a tile each
-// Warps 0 and 1 load and issue products (2 and 3 only fill their warpgroup), 4 to 19 do the softmax, 20 to 23 widen.  768
-// threads can have 80 registers each; the softmax takes over what the others do not need.
+constexpr int kWiden = 256;  // threads that widen codes: two groups, every other tile each, a thread a row of it
+// Warps 0 and 1 load and issue products (2 and 3 only fill their warpgroup), 4 to 19 do the softmax, 20 to 27 widen.  896
+// threads can have 72 registers each; the softmax takes over what the others do not need.
 constexpr int kThreads = 128 + kSoftmax + kWiden, kFirst = 4;
-constexpr int kLaunched = 80, kSmall = 48, kLarge = 96;
+constexpr int kLaunched = 72, kSmall = 48, kLarge = 88;
 static_assert((kThreads - kSoftmax) * kSmall + kSoftmax * kLarge <= kThreads * kLaunched, "registers");
 constexpr float kBelow = 7.f, kPass = 15.f;       // the base below the maximum, and what a score may lie above the base
 constexpr int kInfo = 8;                          // tiles whose factors are kept
@@ -58,6 +58,7 @@ struct Smem {
   static constexpr uint32_t total = info_off + kInfo * 16 + 1024;
   static_assert(total <= 227 * 1024, "a block's shared memory");
   static_assert(max_off % 16 == 0, "alignment");
+  static_assert(stages % 2 == 0 && raws % 2 == 0 && more_raws % 2 == 0, "two groups take turns");
   static_assert(kMeeting<D> <= stages * kv_tile + raws * raw_tile, "the meeting place fits the rings");
 };
 
@@ -114,18 +115,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int k0 = split * a.prefix_chunk, k1 = min(a.prefix_len, k0 + a.prefix_chunk);
   const int n_tiles = (k1 - k0 + kTile - 1) / kTile, loads = 2 * n_tiles;
   const int raws = shared ? S::raws : kMostRaws;
-  const int per = min(1 << a.page_shift, kTile);  // tokens of a box
+  const int per_shift = min(a.page_shift, 7), per = 1 << per_shift;  // tokens of a box
   auto raw_at = [&](int r) { return r < S::raws ? S::raw_off + r * S::raw_tile : S::q_off + S::q_tile + (r - S::raws) * S::raw_tile; };
   auto valid_of = [&](int tile) { return min(kTile, k1 - k0 - tile * kTile); };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(full0 + 8 * s, kWiden / 32);
+      mbar_init(full0 + 8 * s, kTile / 32);
       mbar_init(empty0 + 8 * s, 1);
     }
     for (int r = 0; r < kMostRaws; ++r) {
       mbar_init(raw_full0 + 8 * r, 33);  // the expected bytes, and every lane's copies of scales
-      mbar_init(raw_empty0 + 8 * r, kWiden / 32);
+      mbar_init(raw_empty0 + 8 * r, kTile / 32);
     }
     mbar_init(q_full, kSoftmax);
     mbar_init(drained, 1);
@@ -152,15 +153,26 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp < kFirst) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSmall));
     if (warp == 0) {
-      int pos = 0;
-      for (bool ok = true; ok && pos < loads; ++pos) {
+      int pos = 0, r = 0;
+      uint32_t phase = 1;
+      // Page ids, 32 from `batch` on and the 32 after them (a value's tile is up to two behind the keys'): asked for long
+      // before they are needed, because a trip to memory takes as long as a tile.
+      const int ids_end = ((k1 - 1) >> a.page_shift) + 1;
+      auto fetch = [&](int from) { return from + lane < ids_end ? a.prefix_pages[from + lane] : 0; };
+      int batch = k0 >> a.page_shift, ids_now = fetch(batch), ids_next = fetch(batch + 32);
+      for (; pos < loads; ++pos) {
         const Step step = step_of(pos, n_tiles, shared);
-        const int r = pos % raws, j0 = k0 + step.tile * kTile, boxes = (valid_of(step.tile) + per - 1) / per;
+        const int j0 = k0 + step.tile * kTile, boxes = (valid_of(step.tile) + per - 1) >> per_shift;
         const uint32_t bar = raw_full0 + 8 * r;
-        int page = 0;
-        if (lane < boxes) page = a.prefix_pages[(j0 + lane * per) >> a.page_shift];
-        ok = warp_wait(raw_empty0 + 8 * r, ((pos / raws) & 1) ^ 1, a.status);
-        if (!ok) break;
+        if (!step.keys && (j0 >> a.page_shift) - batch >= 32) {
+          batch += 32;
+          ids_now = ids_next;
+          ids_next = fetch(batch + 32);
+        }
+        const int at_id = ((j0 + lane * per) >> a.page_shift) - batch;
+        const int of_now = __shfl_sync(0xffffffffu, ids_now, at_id & 31), of_next = __shfl_sync(0xffffffffu, ids_next, at_id & 31);
+        int page = at_id < 32 ? of_now : of_next;
+        if (!warp_wait(raw_empty0 + 8 * r, phase, a.status)) break;
         if (lane == 0) mbar_arrive_expect_tx(bar, boxes * per * D);
         __syncwarp();
         if (lane < boxes) {
@@ -176,6 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           copy_float(to + 64, a.v_scales + at, there);
         }
         arrive_after_copies(bar);
+        if (++r == raws) r = 0, phase ^= 1;
       }
       // The block does not end before its last copies have arrived, also where another warp's wait was given up.
       for (int p = max(0, pos - raws); p < pos; ++p) mbar_wait(raw_full0 + 8 * (p % raws), (p / raws) & 1, nullptr);
@@ -289,60 +302,81 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp >= kFirst + kSoftmax / 32) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSmall));
-    // Widening: a lane has a row of the tile, so one scale.
-    const int row = threadIdx.x - (kThreads - kWiden);
-    bool ok = true;
-    for (int pos = 0; ok && pos < loads; ++pos) {
+    // Widening: a thread has a row of the tile, so one scale.
+    const int self = threadIdx.x - (kThreads - kWiden), row = self % kTile, group = self / kTile;
+    int r = group, st = group;
+    uint32_t raw_phase = 0, phase = 1;
+    for (int pos = group; pos < loads; pos += 2) {
       const Step step = step_of(pos, n_tiles, shared);
-      const int r = pos % raws, st = pos % kStages, valid = valid_of(step.tile), boxes = (valid + per - 1) / per;
-      ok = warp_wait(raw_full0 + 8 * r, (pos / raws) & 1, a.status) && warp_wait(empty0 + 8 * st, ((pos / kStages) & 1) ^ 1, a.status);
-      if (!ok) break;
+      const int valid = valid_of(step.tile), boxes = (valid + per - 1) >> per_shift;
+      if (!warp_wait(raw_full0 + 8 * r, raw_phase, a.status) || !warp_wait(empty0 + 8 * st, phase, a.status)) break;
       const float* scales = reinterpret_cast<const float*>(sm + S::scale_off) + r * 2 * 16;
       auto largest = [&](float x) {  // of the pages' scales, and at least the least
         const float mine = lane < boxes ? fmaxf(x, kLeastScale) : kLeastScale;  // (also for what is no number)
         return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mine)));
       };
-      const int box = min(row, valid - 1) / per;
-      float factor;
+      const float* const mine = scales + (step.keys ? 0 : 16);
+      const float top = largest(mine[lane & 15]), own = mine[min(row, valid - 1) >> per_shift];
+      const float factor = (step.keys ? own : fmaxf(own, kLeastScale)) * rcp_approx(top);
       if (step.keys) {
-        const float top_k = largest(scales[lane & 15]), top_v = largest(scales[16 + (lane & 15)]);
-        factor = scales[box] / top_k;
-        if (row == 0) {
-          const float b = __log2f(top_v);
+        const float b = __log2f(largest(scales[16 + (lane & 15)]));
+        if (row == 0)
           *reinterpret_cast<float4*>(sm + S::info_off + step.tile % kInfo * 16) =
-              make_float4(fminf(top_k, 3.4e38f) * a.scale_log2, b, ex2_approx(15.f - b), 0.f);
-        }
-      } else {
-        factor = fmaxf(scales[16 + box], kLeastScale) / largest(scales[16 + (lane & 15)]);
+              make_float4(fminf(top, 3.4e38f) * a.scale_log2, b, ex2_approx(15.f - b), 0.f);
       }
-      uint32_t by;  // as an f16 pair
-      by = pack_f16x2(factor, factor);
+      const uint32_t by = pack_f16x2(factor, factor);
+      // int8: (1024 + u) by - 1152 by in one step, which is exact where `by` is a power of two
+      const uint32_t less = mul_f16x2(by, 0xe480e480u);
+      const bool powers = kFloat || __all_sync(0xffffffffu, (__float_as_uint(factor) & 0x7fffff) == 0);
       const bool there = row < valid;
-      const uint32_t from = sbase + raw_at(r) + row * D, to = sbase + S::kv_off + st * S::kv_tile + row * 128;
+      const uint8_t* const from = sm + raw_at(r) + row * D;
+      uint8_t* const to = sm + S::kv_off + st * S::kv_tile + row * 128;
       const int turn_in = D == 128 ? row & 7 : (row >> 1) & 3, turn_out = row & 7;
+      auto widen_row = [&](auto by_powers) {
 #pragma unroll
-      for (int c = 0; c < D / 16; ++c) {
-        uint4 w;
-        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(from + ((c ^ turn_in) << 4)));
-        uint32_t y[8];
+        for (int c0 = 0; c0 < D / 16; c0 += 4) {
+          uint4 w[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          widen_in_order<kFloat>((&w.x)[k], y[2 * k], y[2 * k + 1]);
-          y[2 * k] = mul_f16x2(y[2 * k], by), y[2 * k + 1] = mul_f16x2(y[2 * k + 1], by);
+          for (int k = 0; k < 4; ++k) w[k] = ld_v4(from + (((c0 + k) ^ turn_in) << 4));
+          if (!there) w[0] = w[1] = w[2] = w[3] = make_uint4(0, 0, 0, 0);  // past the end a page holds anything
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t y[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t v = (&w[k].x)[e];
+              if constexpr (kFloat) {
+                widen_any<true>(v, y[2 * e], y[2 * e + 1]);  // (in the bytes' order)
+                y[2 * e] = mul_f16x2(y[2 * e], by), y[2 * e + 1] = mul_f16x2(y[2 * e + 1], by);
+              } else {
+                v ^= 0x80808080u;
+                y[2 * e] = __byte_perm(v, 0x64646464u, 0x4140), y[2 * e + 1] = __byte_perm(v, 0x64646464u, 0x4342);
+                if constexpr (decltype(by_powers)::value) {
+                  y[2 * e] = fma_f16x2(y[2 * e], by, less), y[2 * e + 1] = fma_f16x2(y[2 * e + 1], by, less);
+                } else {
+                  y[2 * e] = mul_f16x2(sub_f16x2(y[2 * e], 0x64806480u), by);
+                  y[2 * e + 1] = mul_f16x2(sub_f16x2(y[2 * e + 1], 0x64806480u), by);
+                }
+              }
+            }
+            // (dims 16 c on: chunks 2 c and 2 c + 1 of 8 values, eight of them to a 128-byte row)
+            uint8_t* const at = to + c0 / 4 * (kTile * 128);
+            const int first = (2 * k) ^ turn_out;
+            st_v4(at + (first << 4), make_uint4(y[0], y[1], y[2], y[3]));
+            st_v4(at + ((first ^ 1) << 4), make_uint4(y[4], y[5], y[6], y[7]));
+          }
         }
-        if (!there)
-#pragma unroll
-          for (int k = 0; k < 8; ++k) y[k] = 0;  // past the end a page holds anything
-        const uint32_t at = to + (2 * c / 8) * (kTile * 128);
-        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at + (((2 * c % 8) ^ turn_out) << 4)), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
-        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at + (((2 * c % 8 + 1) ^ turn_out) << 4)), "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7]) : "memory");
-      }
+      };
+      if (kFloat || powers) widen_row(std::true_type{});
+      else widen_row(std::false_type{});
       fence_async_smem();
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(full0 + 8 * st);
         mbar_arrive(raw_empty0 + 8 * r);
       }
+      if ((r += 2) >= raws) r -= raws, raw_phase ^= 1;
+      if ((st += 2) >= kStages) st -= kStages, phase ^= 1;
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kLarge));
