@@ -446,6 +446,69 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args 
   if (a.lse && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : kLn2 * (m + log2f(l));
 }
 
+// The same for a cache in 8 bits, where a row has many slots for pieces and most of them may be empty: the warps of a row
+// look at all maxima and take the pieces that are there in turn.  kWarps: of a row.
+template <int D, int kWarps, bool Checked>
+__global__ void __launch_bounds__(kWarps == 1 ? 128 : 32 * kWarps) join8_kernel(const __grid_constant__ Args a) {
+  constexpr int kPer = D / 32, kRows = kWarps == 1 ? 4 : 1, kBatch = 4;
+  __shared__ float so[kWarps][D];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, self = kWarps == 1 ? 0 : warp;
+  const long long row = static_cast<long long>(blockIdx.x) * kRows + (kWarps == 1 ? warp : 0), rows = static_cast<long long>(a.n) * a.heads;
+  wait_for_previous();
+  if (row >= rows) return;  // (with one row to a block there is none such)
+  const bool own = !Checked || own_count(a);
+  const int pieces = a.prefix_splits + (own ? a.own_splits : 0);
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int p = lane; p < pieces; p += 32) m = fmaxf(m, a.part_ml[p * rows + row].x);
+  m = warp_max(m);
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o[kPer] = {};
+  int turn = 0;  // pieces before these that are there
+  for (int p0 = 0; p0 < pieces; p0 += 32) {
+    const float2 ml = p0 + lane < pieces ? a.part_ml[(p0 + lane) * rows + row] : make_float2(-INFINITY, 0.f);
+    const float f = ex2_approx(ml.x - base);
+    l = fmaf(f, ml.y, l);
+    const unsigned there = __ballot_sync(0xffffffffu, ml.x > -INFINITY);
+    const int rank = turn + __popc(there & ((1u << lane) - 1));
+    unsigned mine = __ballot_sync(0xffffffffu, ml.x > -INFINITY && rank % kWarps == self);
+    turn += __popc(there);
+    while (mine) {
+      float part[kBatch][kPer], by[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int which = mine ? __ffs(mine) - 1 : 0;
+        by[k] = mine ? __shfl_sync(0xffffffffu, f, which) : 0.f;
+        const float* po = a.part_o + ((p0 + which) * rows + row) * D + lane * kPer;
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) part[k][c] = mine ? po[c] : 0.f;
+        mine &= mine - 1;
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) o[c] = fmaf(by[k], part[k][c], o[c]);
+    }
+  }
+  l = warp_sum(l);
+  if (kWarps > 1) {
+#pragma unroll
+    for (int c = 0; c < kPer; ++c) so[warp][lane * kPer + c] = o[c];
+    __syncthreads();
+    if (self > 0) return;
+#pragma unroll
+    for (int k = 1; k < kWarps; ++k)
+#pragma unroll
+      for (int c = 0; c < kPer; ++c) o[c] += so[k][lane * kPer + c];
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // a row without keys is zero; one with a score of NaN stays NaN
+  __nv_bfloat16* out = a.o + row * D + lane * kPer;
+  if constexpr (kPer == 1) *out = f32_to_bf16(o[0] * inv);
+#pragma unroll
+  for (int c = 0; c + 1 < kPer; c += 2) *reinterpret_cast<uint32_t*>(out + c) = pack_bf16x2(o[c] * inv, o[c + 1] * inv);
+  if (a.lse && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : kLn2 * (m + log2f(l));
+}
+
 int row_warps(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -512,6 +575,15 @@ int kernels(const Args& a) { return checks(a) + by_warps(a) + by_tensor_cores(a)
 template <int D>
 static cudaError_t launch_join_of(const Args& a, cudaStream_t stream) {
   const int rows = a.n * a.heads;
+  if (a.codes) {
+    // eight warps to a row where there are many slots, four where there are some; with many rows a warp each fills the GPU
+    const int pieces = a.prefix_splits + a.own_splits;
+    if (pieces > 32 && rows <= 148 * 32)
+      return launch_after(a.sound ? join8_kernel<D, 8, true> : join8_kernel<D, 8, false>, rows, 256, 0, stream, a);
+    if (pieces > 4 && rows <= 148 * 64)
+      return launch_after(a.sound ? join8_kernel<D, 4, true> : join8_kernel<D, 4, false>, rows, 128, 0, stream, a);
+    return launch_after(a.sound ? join8_kernel<D, 1, true> : join8_kernel<D, 1, false>, ceil_div(rows, 4), 128, 0, stream, a);
+  }
   if (a.prefix_splits + a.own_splits > 4)
     return launch_after(a.sound ? join_kernel<D, true, true> : join_kernel<D, true, false>, rows, 128, 0, stream, a);
   return launch_after(a.sound ? join_kernel<D, false, true> : join_kernel<D, false, false>, ceil_div(rows, 4), 128, 0, stream, a);

@@ -85,12 +85,19 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NT>::blocks)
     pieces8_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap map_k,
                    const __grid_constant__ CUtensorMap map_v, int items, int known, int least) {
   using R = Ring<D, NT>;
-  constexpr int kStages = R::stages, kU = kStep / 16, kRows = 8 * NT, kMt = D / 16;
+  // The work takes half a stage at a time: with whole ones the code is so long that fetching it bounds short calls (and
+  // sixteen rows lack registers).
+  constexpr int kStages = R::stages, kPart = kStep / 2, kU = kPart / 16, kQueue = 4, kRows = 8 * NT, kMt = D / 16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t bars[kWarps][2 * kStages];
   __shared__ float scale_of[kWarps][kStages][2][8];  // of a stage's pages: keys, values
   __shared__ float4 factor_of[kWarps][8];            // of each eight keys of the stage that is worked on
+  struct Queued {
+    Piece p;
+    int part_end;
+  };
+  __shared__ Queued queue[kWarps][kQueue];  // pieces whose loads have begun
   __shared__ uint32_t nan_at[kFloat ? kWarps : 1][kRows][D / 32];  // outputs that have to become NaN, a bit each
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   const uint32_t ring = smem_u32(sm) + warp * R::bytes, full_k = smem_u32(bars[warp]), full_v = full_k + 8 * kStages,
@@ -208,19 +215,32 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NT>::blocks)
   int ids_now = 0, ids_next = 0;  // this lane's of 32 pages from `batch` on, and of the 32 after them
   const int* ids = nullptr;
   auto fetch = [&](int first) { return first + lane < ids_end ? ids[first + lane] : 0; };
+  auto out_of = [&](const Piece& p, int r) {  // where row r's partial results go
+    const int j = p.r0 + r, token = j / a.group;
+    return (static_cast<long long>(p.slot) * a.n + p.n0 + token) * a.heads + p.h * a.group + j - token * a.group;
+  };
+  int queued = 0;
   auto next_piece = [&] {
     Piece p;
-    int unused;
-    while ((loading = next(load_at, p, unused))) {
-      if (p.k1 <= p.k0 || p.n_rows <= 0) continue;
+    int part_end;
+    while ((loading = next(load_at, p, part_end))) {
+      if (p.n_rows <= 0) continue;
+      if (p.k1 <= p.k0) {  // nothing here: the join skips the piece
+        if (lane < p.n_rows) a.part_ml[out_of(p, lane)] = make_float2(-INFINITY, 0.f);
+        continue;
+      }
       load_key = p.k0, load_end = p.k1, load_head = p.h, ids = p.ids;
       batch = p.k0 >> a.page_shift;
       ids_end = ((p.k1 - 1) >> a.page_shift) + 1;
       ids_now = fetch(batch);
       ids_next = fetch(batch + 32);
+      // (pieces ahead of the one that is worked on: at most one for each stage, and this)
+      if (lane == 0) queue[warp][queued % kQueue] = Queued{p, part_end};
+      ++queued;
       return;
     }
   };
+  static_assert(kStages + 1 < kQueue, "pieces under way");
   // The keys of the next stage, a box for each of the first lanes, and the scales of both; its values follow.
   int box_page = 0, box_token = 0, box_head = 0, boxes = 0;
   auto issue_keys = [&] {
@@ -262,33 +282,27 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NT>::blocks)
     if (lane < boxes) tma_load_4d(ring + (st * 2 + 1) * R::tile + lane * per * D, &map_v, 0, box_head, box_token, box_page, bar);
     ++issued;
   };
-  next_piece();
-  for (int s = 0; s < kStages; ++s) {
-    issue_keys();
-    issue_values();
-  }
-
   // Where this lane reads: row g (and g + 8) of 16 keys as the first operand of K Q^T, and the rows of ldmatrix for V^T P^T
   const uint32_t at_k = D == 32 ? R::at(g, t >> 1) + (t & 1) * 8 : R::at(key_of<D>(g), t);
   const uint32_t at_v = R::at(((lane >> 3) & 1) * 8 + key_of<D>(lane & 7), lane >> 4);
-  int pos = 0;  // stages used so far
-  long long work_at = least ? from : self;
+  next_piece();
+  uint32_t qf[NT][kMt][2];
+  float back[NT][2];         // what rows n * 8 + 2 t and + 1 were scaled by, taken back
+  int lim[NT][2], whole = 0;  // the keys that they see, and those that every row does
+  float o[NT][kMt][4], base[NT][2], l[NT][2];
   Piece p;
-  int part_end;
-  while (next(work_at, p, part_end)) {
-    if (p.n_rows <= 0) continue;
-    auto out_of = [&](int r) {
-      const int j = p.r0 + r, token = j / a.group;
-      return (static_cast<long long>(p.slot) * a.n + p.n0 + token) * a.heads + p.h * a.group + j - token * a.group;
-    };
-    if (p.k1 <= p.k0) {  // nothing here: the join skips the piece
-      if (lane < p.n_rows) a.part_ml[out_of(lane)] = make_float2(-INFINITY, 0.f);
-      continue;
-    }
+  int part_end = 0, t0 = 0, taken = 0;
+  p.k1 = 0;
+  // Stage by stage, the first kStages steps only load.
+  for (int pos = -kStages;; ++pos) {
+  const bool work = pos >= 0;
+  if (work && t0 >= p.k1) {  // the next piece
+    if (taken == queued) break;
+    __syncwarp();
+    p = queue[warp][taken % kQueue].p, part_end = queue[warp][taken % kQueue].part_end;
+    ++taken;
+    t0 = p.k0;
     // Queries as the products' second operand: row n * 8 + g, four dims (those of a word of codes) for each 16-wide step.
-    uint32_t qf[NT][kMt][2];
-    float back[NT][2];  // what rows n * 8 + 2 t and + 1 were scaled by, taken back
-    int lim[NT][2];     // the keys that they see
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int r = n * 8 + g, j = p.r0 + r, token = j / a.group;
@@ -328,8 +342,7 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NT>::blocks)
         lim[n][e] = row < p.n_rows ? min(p.k1, p.limit0 + (p.r0 + row) / a.group) : p.k0;
       }
     }
-    const int whole = min(p.k1, p.limit0 + p.r0 / a.group);  // keys before this are seen by every row
-    float o[NT][kMt][4], base[NT][2], l[NT][2];
+    whole = min(p.k1, p.limit0 + p.r0 / a.group);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       base[n][0] = base[n][1] = -INFINITY;
@@ -338,182 +351,197 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NT>::blocks)
       for (int m = 0; m < kMt; ++m) o[n][m][0] = o[n][m][1] = o[n][m][2] = o[n][m][3] = 0.f;
     }
 
-    for (int t0 = p.k0; t0 < p.k1; t0 += kStep, ++pos) {
-      const int st = pos % kStages;
+  }
+      const int st = max(pos, 0) % kStages;
       const uint32_t phase = (pos / kStages) & 1;
-      mbar_wait(full_k + 8 * st, phase, a.status);  // (a wait that gave up is in the status word)
+      if (work) mbar_wait(full_k + 8 * st, phase, a.status);  // (a wait that gave up is in the status word)
       __syncwarp();
       const uint32_t sK = ring + st * 2 * R::tile, sV = sK + R::tile;
       // Each eight keys lie in one page: its factor of the scores, the logarithm of its values' scale, and what turns a
       // weight into its part of the sum (times 2^15, so that nothing leaves the range of fp32).
-      if (lane < 8) {
+      if (work && lane < 8) {
         const int box = (lane * 8) >> a.page_shift;
         const float b = __log2f(fmaxf(scale_of[warp][st][1][box], kLeastScale));  // (a page of zeros may have any scale)
         factor_of[warp][lane] = make_float4(scale_of[warp][st][0][box] * a.scale_log2, b, ex2_approx(15.f - b), 0.f);
       }
-      float s[NT][kU][4];
+      __syncwarp();
+      bool spoiled = false;
+#pragma unroll 1
+      for (int part = 0; part < kStep / kPart; ++part) {
+        const int t1 = t0 + part * kPart;
+        const bool live = work && (part == 0 || t1 < p.k1);
+        float s[NT][kU][4];
+        if (live) {
 #pragma unroll
-      for (int u = 0; u < kU; ++u) {
+          for (int u = 0; u < kU; ++u) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) s[n][u][0] = s[n][u][1] = s[n][u][2] = s[n][u][3] = 0.f;
+            for (int n = 0; n < NT; ++n) s[n][u][0] = s[n][u][1] = s[n][u][2] = s[n][u][3] = 0.f;
 #pragma unroll
-        for (int x = 0; x < (D + 63) / 64; ++x) {
-          uint4 ka, kb;  // a row's words: two of them at head dim 32
-          const uint32_t from = (sK + u * 16 * D + at_k) ^ (x * 64);
-          if (D == 32) {
-            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(ka.x), "=r"(ka.y) : "r"(from));
-            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(kb.x), "=r"(kb.y) : "r"(from + 8 * D));
-          } else {
-            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(ka.x), "=r"(ka.y), "=r"(ka.z), "=r"(ka.w) : "r"(from));
-            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(kb.x), "=r"(kb.y), "=r"(kb.z), "=r"(kb.w) : "r"(from + 8 * D));
+            for (int x = 0; x < (D + 63) / 64; ++x) {
+              uint4 ka, kb;  // a row's words: two of them at head dim 32
+              const uint32_t from = (sK + (part * kPart + u * 16) * D + at_k) ^ (x * 64);
+              if (D == 32) {
+                asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(ka.x), "=r"(ka.y) : "r"(from));
+                asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(kb.x), "=r"(kb.y) : "r"(from + 8 * D));
+              } else {
+                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(ka.x), "=r"(ka.y), "=r"(ka.z), "=r"(ka.w) : "r"(from));
+                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(kb.x), "=r"(kb.y), "=r"(kb.z), "=r"(kb.w) : "r"(from + 8 * D));
+              }
+#pragma unroll
+              for (int j = 0; j < (D == 32 ? 2 : 4); ++j) {
+                uint32_t f[4];
+                widen_any<kFloat>((&ka.x)[j], f[0], f[2]);
+                widen_any<kFloat>((&kb.x)[j], f[1], f[3]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma_f16(s[n][u], f, qf[n][x * 4 + j]);
+              }
+            }
           }
-#pragma unroll
-          for (int j = 0; j < (D == 32 ? 2 : 4); ++j) {
-            uint32_t f[4];
-            widen_any<kFloat>((&ka.x)[j], f[0], f[2]);
-            widen_any<kFloat>((&kb.x)[j], f[1], f[3]);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma_f16(s[n][u], f, qf[n][x * 4 + j]);
-          }
         }
-      }
-      __syncwarp();  // (the keys and scales have been read)
-      issue_keys();
-      float sum_of[kU][2];
-#pragma unroll
-      for (int u = 0; u < kU; ++u)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float4 f = factor_of[warp][2 * u + h];
-          sum_of[u][h] = f.z;
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              // (towards zero: a factor past fp32's range stays finite, and 0 times it stays 0)
-              s[n][u][2 * h + e] = fmaf(s[n][u][2 * h + e], __fmul_rz(f.x, back[n][e]), f.y);
+        if (part == kStep / kPart - 1) {
+          __syncwarp();  // (the keys and scales have been read)
+          issue_keys();
         }
-      const bool masked = t0 + kStep > whole;
-      if (masked) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int u = 0; u < kU; ++u)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (t0 + u * 16 + e / 2 * 8 + key_of<D>(g) >= lim[n][e & 1]) s[n][u][e] = -INFINITY;
-      }
-      float top[NT][2];
-      bool grows = false;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float x = fmaxf(s[n][0][e], s[n][0][2 + e]);
-#pragma unroll
-          for (int u = 1; u < kU; ++u) x = max3f(x, s[n][u][e], s[n][u][2 + e]);
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          top[n][e] = x;
-          grows = grows || x > base[n][e] + kPass || (base[n][e] == -INFINITY && x > -INFINITY);
-        }
-      if (__any_sync(0xffffffffu, grows)) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float alpha[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float to = top[n][e] > base[n][e] + kPass || base[n][e] == -INFINITY ? top[n][e] - kBelow : base[n][e];
-            alpha[e] = to == base[n][e] ? 1.f : ex2_approx(base[n][e] - to);
-            l[n][e] *= alpha[e];
-            base[n][e] = to;
-          }
-#pragma unroll
-          for (int m = 0; m < kMt; ++m)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][m][e] *= alpha[e & 1];
-        }
-      }
-      uint32_t pf[NT][kU][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        // (no key yet: every weight is exp2(-inf) = 0)
-        const float from0 = base[n][0] == -INFINITY ? 0.f : base[n][0], from1 = base[n][1] == -INFINITY ? 0.f : base[n][1];
+        if (!live) continue;
+        float sum_of[kU][2];
 #pragma unroll
         for (int u = 0; u < kU; ++u)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float w0 = ex2_approx(s[n][u][2 * h] - from0), w1 = ex2_approx(s[n][u][2 * h + 1] - from1);
-            l[n][0] = fmaf(w0, sum_of[u][h], l[n][0]);
-            l[n][1] = fmaf(w1, sum_of[u][h], l[n][1]);
-            pf[n][u][h] = transposed(pack_f16x2(w0, w1));
+            const float4 f = factor_of[warp][2 * (part * kU + u) + h];
+            sum_of[u][h] = f.z;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                // (towards zero: a factor past fp32's range stays finite, and 0 times it stays 0)
+                s[n][u][2 * h + e] = fmaf(s[n][u][2 * h + e], __fmul_rz(f.x, back[n][e]), f.y);
           }
-      }
-      mbar_wait(full_v + 8 * st, phase, a.status);
-      __syncwarp();
-      bool spoiled = false;
-      if constexpr (kFloat) {
-        // A key that a row does not see has weight 0, and 0 times NaN (which e4m3 has, also past the end of the keys, where
-        // a page holds anything) would be NaN: such codes become zeros here, and rows that do see one become NaN below.
+        const bool masked = t1 + kPart > whole;
         if (masked) {
-          uint32_t some = 0;
-          for (int x = lane; x < kStep * D / 16; x += 32) {
-            uint4 w;
-            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(sV + x * 16));
-            some |= nan_bytes(w.x) | nan_bytes(w.y) | nan_bytes(w.z) | nan_bytes(w.w);
-          }
-          spoiled = __any_sync(0xffffffffu, some != 0);
-          if (spoiled) {
-            for (int x = lane; x < kRows * (D / 32); x += 32) (&nan_at[warp][0][0])[x] = 0;
-            __syncwarp();
-#pragma unroll 1
-            for (int x = lane; x < kStep * D / 4; x += 32) {  // word by word
-              const int key = x / (D / 4), word = x % (D / 4);
-              const uint32_t at = sV + R::at(key, word / 4) + word % 4 * 4;
-              uint32_t w;
-              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at));
-              const uint32_t odd = nan_bytes(w);
-              if (!odd) continue;
-              asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(w & ~(odd * 0xffu)) : "memory");
-              const uint32_t bits = ((odd & 1u) | (odd >> 7 & 2u) | (odd >> 14 & 4u) | (odd >> 21 & 8u)) << (word % 8 * 4);
-              for (int row = 0; row < p.n_rows; ++row)
-                if (t0 + key < min(p.k1, p.limit0 + (p.r0 + row) / a.group)) atomicOr(&nan_at[warp][row][word / 8], bits);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // TMA writes here next
-            __syncwarp();
-          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int u = 0; u < kU; ++u)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (t1 + u * 16 + e / 2 * 8 + key_of<D>(g) >= lim[n][e & 1]) s[n][u][e] = -INFINITY;
         }
-      }
-#pragma unroll
-      for (int u = 0; u < kU; ++u)
-#pragma unroll
-        for (int c = 0; c < kMt / 2; ++c) {
-          uint32_t w[4];
-          ldsm_x4_t(w, (sV + u * 16 * D + at_v) ^ (c * 32));
-#pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            uint32_t f[4];
-            widen<kFloat>(w[2 * m], f[0], f[1]);
-            widen<kFloat>(w[2 * m + 1], f[2], f[3]);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * c + m], f, pf[n][u]);
-          }
-        }
-      if (kFloat && spoiled) {
+        float top[NT][2];
+        bool grows = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int m = 0; m < kMt; ++m)
+          for (int e = 0; e < 2; ++e) {
+            float x = fmaxf(s[n][0][e], s[n][0][2 + e]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int dim = m * 16 + 2 * g + e / 2;
-              if (nan_at[warp][n * 8 + 2 * t + e % 2][dim / 32] >> (dim % 32) & 1) o[n][m][e] = NAN;
+            for (int u = 1; u < kU; ++u) x = max3f(x, s[n][u][e], s[n][u][2 + e]);
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            top[n][e] = x;
+            grows = grows || x > base[n][e] + kPass || (base[n][e] == -INFINITY && x > -INFINITY);
+          }
+        if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float alpha[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float to = top[n][e] > base[n][e] + kPass || base[n][e] == -INFINITY ? top[n][e] - kBelow : base[n][e];
+              alpha[e] = to == base[n][e] ? 1.f : ex2_approx(base[n][e] - to);
+              l[n][e] *= alpha[e];
+              base[n][e] = to;
             }
+#pragma unroll
+            for (int m = 0; m < kMt; ++m)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[n][m][e] *= alpha[e & 1];
+          }
+        }
+        uint32_t pf[NT][kU][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          // (no key yet: every weight is exp2(-inf) = 0)
+          const float from0 = base[n][0] == -INFINITY ? 0.f : base[n][0], from1 = base[n][1] == -INFINITY ? 0.f : base[n][1];
+#pragma unroll
+          for (int u = 0; u < kU; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float w0 = ex2_approx(s[n][u][2 * h] - from0), w1 = ex2_approx(s[n][u][2 * h + 1] - from1);
+              l[n][0] = fmaf(w0, sum_of[u][h], l[n][0]);
+              l[n][1] = fmaf(w1, sum_of[u][h], l[n][1]);
+              pf[n][u][h] = transposed(pack_f16x2(w0, w1));
+            }
+        }
+        if (part == 0) {
+          mbar_wait(full_v + 8 * st, phase, a.status);
+          __syncwarp();
+        }
+        if constexpr (kFloat) {
+          // A key that a row does not see has weight 0, and 0 times NaN (which e4m3 has, also past the end of the keys, where
+          // a page holds anything) would be NaN: such codes become zeros here, and rows that do see one become NaN below.
+          if (part == 0 && t0 + kStep > whole) {
+            uint32_t some = 0;
+            for (int x = lane; x < kStep * D / 16; x += 32) {
+              uint4 w;
+              asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(sV + x * 16));
+              some |= nan_bytes(w.x) | nan_bytes(w.y) | nan_bytes(w.z) | nan_bytes(w.w);
+            }
+            spoiled = __any_sync(0xffffffffu, some != 0);
+            if (spoiled) {
+              for (int x = lane; x < kRows * (D / 32); x += 32) (&nan_at[warp][0][0])[x] = 0;
+              __syncwarp();
+#pragma unroll 1
+              for (int x = lane; x < kStep * D / 4; x += 32) {  // word by word
+                const int key = x / (D / 4), word = x % (D / 4);
+                const uint32_t at = sV + R::at(key, word / 4) + word % 4 * 4;
+                uint32_t w;
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at));
+                const uint32_t odd = nan_bytes(w);
+                if (!odd) continue;
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(w & ~(odd * 0xffu)) : "memory");
+                const uint32_t bits = ((odd & 1u) | (odd >> 7 & 2u) | (odd >> 14 & 4u) | (odd >> 21 & 8u)) << (word % 8 * 4);
+                for (int row = 0; row < p.n_rows; ++row)
+                  if (t0 + key < min(p.k1, p.limit0 + (p.r0 + row) / a.group)) atomicOr(&nan_at[warp][row][word / 8], bits);
+              }
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // TMA writes here next
+              __syncwarp();
+            }
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+#pragma unroll
+          for (int c = 0; c < kMt / 2; ++c) {
+            uint32_t w[4];
+            ldsm_x4_t(w, (sV + (part * kPart + u * 16) * D + at_v) ^ (c * 32));
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+              uint32_t f[4];
+              widen<kFloat>(w[2 * m], f[0], f[1]);
+              widen<kFloat>(w[2 * m + 1], f[2], f[3]);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * c + m], f, pf[n][u]);
+            }
+          }
+        if (kFloat && spoiled) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int m = 0; m < kMt; ++m)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int dim = m * 16 + 2 * g + e / 2;
+                if (nan_at[warp][n * 8 + 2 * t + e % 2][dim / 32] >> (dim % 32) & 1) o[n][m][e] = NAN;
+              }
+        }
       }
       __syncwarp();
       issue_values();
-    }
+      if (!work) continue;
+      t0 += kStep;
+      if (t0 < p.k1) continue;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -524,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NT>::blocks)
         sum += __shfl_xor_sync(0xffffffffu, sum, 16);
         const int r = n * 8 + 2 * t + e;
         if (r >= p.n_rows) continue;
-        const long long out = out_of(r);
+        const long long out = out_of(p, r);
 #pragma unroll
         for (int m = 0; m < kMt; ++m)
           *reinterpret_cast<float2*>(a.part_o + out * D + m * 16 + 2 * g) = make_float2(o[n][m][e], o[n][m][2 + e]);
@@ -611,8 +639,9 @@ int plan8(Args& a, int head_dim) {
   // pieces of 608 keys in turn).  A part of t tiles has at most 1 + ceil((t - 1) / share) warps, and as many slots.  Parts of
   // the average length need one for each warp that it takes to fill the GPU, longer ones (here: up to twice) more.
   const bool shares = a.max_q == 1 && (!own || (a.batch <= q8::kMostKnown && static_cast<long long>(a.batch) * own_tiles < (1ll << 31)));
+  constexpr int kMostSlots = 256;
   auto slots = [&](int tiles, long long units, int times) {
-    return std::min({tiles, 64, times * ceil_div(warps, units) + (times == 1 ? 2 : 1)});
+    return std::min({tiles, kMostSlots, times * ceil_div(warps, units) + (times == 1 ? 2 : 1)});
   };
   if (a.prefix_len > 0 && !a.tensor_cores) {
     const long long units = static_cast<long long>(a.row_tiles) * a.kv_heads;

@@ -33,9 +33,8 @@ namespace tc8 {
 using namespace tc;
 using namespace q8;
 
-constexpr int kWiden = 256;  // threads that widen codes: two groups, every other tile each, a thread a row of it
-// Warps 0 and 1 load and issue products (2 and 3 only fill their warpgroup), 4 to 19 do the softmax, 20 to 27 widen.  896
-// threads can have 72 registers each; the softmax takes over what the others do not need.
+constexpr int kWiden = 256;  // threads that widen codes: a thread a row of a tile, a warp 32 of them
+// Warp 0 loads keys, 2 values, 1 issues the products (3 only fills its warpgroup), 4 to 19 do the softmax, 20 to 27 widen.  896 threads can have 72 registers each; the softmax takes over what the others do not need.
 constexpr int kThreads = 128 + kSoftmax + kWiden, kFirst = 4;
 constexpr int kLaunched = 72, kSmall = 48, kLarge = 88;
 static_assert((kThreads - kSoftmax) * kSmall + kSoftmax * kLarge <= kThreads * kLaunched, "registers");
@@ -48,35 +47,22 @@ struct Smem {
   static constexpr uint32_t kv_tile = kTile * D * 2;
   static constexpr uint32_t raw_tile = kTile * D;
   static constexpr int stages = D == 128 ? 4 : 6;
-  static constexpr int raws = D == 128 ? 2 : 4, more_raws = q_tile / raw_tile;  // with one tile of queries these many more
+  static constexpr int raws = D == 128 ? 2 : 8, more_raws = D == 128 ? 2 : 0;  // (with one tile of queries there is more room)
   static constexpr uint32_t q_off = 0, kv_off = 2 * q_tile, raw_off = kv_off + stages * kv_tile;
   static constexpr uint32_t bar_off = raw_off + raws * raw_tile;
   static constexpr int n_bars = 2 * stages + 2 * (raws + more_raws) + 10;
   static constexpr uint32_t max_off = bar_off + n_bars * 8 + 16;    // row maxima so far: [stream][row], as order_of()
   static constexpr uint32_t scale_off = max_off + 2 * kTile * 4;    // of the raw tiles' pages: [raw][keys, values][16]
   static constexpr uint32_t info_off = scale_off + (raws + more_raws) * 2 * 16 * 4;  // of tiles: a float4 each
-  static constexpr uint32_t total = info_off + kInfo * 16 + 1024;
+  static constexpr uint32_t total = info_off + kInfo * 16 + 16 + 1024;  // (and the count of widening jobs)
+  static_assert(more_raws * raw_tile <= q_tile, "room");
   static_assert(total <= 227 * 1024, "a block's shared memory");
   static_assert(max_off % 16 == 0, "alignment");
-  static_assert(stages % 2 == 0 && raws % 2 == 0 && more_raws % 2 == 0, "two groups take turns");
   static_assert(kMeeting<D> <= stages * kv_tile + raws * raw_tile, "the meeting place fits the rings");
 };
 
 // Instruction descriptor for kind::f16 with f16 A/B and fp32 D.
 constexpr uint32_t idesc_f16(int m, int n, bool a_mn, bool b_mn) { return idesc_bf16(m, n, a_mn, b_mn) & ~((1u << 7) | (1u << 10)); }
-
-// The order in which the products use the tiles: (keys or values, which).
-struct Step {
-  bool keys;
-  int tile;
-};
-MNB_DEVICE Step step_of(int pos, int n_tiles, bool shared) {
-  if (shared || n_tiles == 1) return {(pos & 1) == 0, pos >> 1};
-  if (pos < 2) return {true, pos};
-  const int j = pos - 2;
-  if (j < 2 * (n_tiles - 2)) return {(j & 1) == 1, (j >> 1) + 2 * (j & 1)};
-  return {false, j - (n_tiles - 2)};
-}
 
 template <int D, bool kFloat>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -113,8 +99,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (n_rows <= 0) return;
   const bool shared = n_rows > kTile;  // both streams use every key tile
   const int k0 = split * a.prefix_chunk, k1 = min(a.prefix_len, k0 + a.prefix_chunk);
-  const int n_tiles = (k1 - k0 + kTile - 1) / kTile, loads = 2 * n_tiles;
-  const int raws = shared ? S::raws : kMostRaws;
+  const int n_tiles = (k1 - k0 + kTile - 1) / kTile;
+  // Rings of raw and of widened tiles: keys have the even places, values the odd ones.
+  const int raw_shift = D == 64 ? 2 : shared ? 0 : 1, raws = 1 << raw_shift;
+  constexpr int kRing = kStages / 2;
+  static_assert(S::raws == (D == 64 ? 8 : 2) && kMostRaws == (D == 64 ? 8 : 4), "keys and values have half of them each");
+  int* const jobs = reinterpret_cast<int*>(sm + S::info_off + kInfo * 16);
   const int per_shift = min(a.page_shift, 7), per = 1 << per_shift;  // tokens of a box
   auto raw_at = [&](int r) { return r < S::raws ? S::raw_off + r * S::raw_tile : S::q_off + S::q_tile + (r - S::raws) * S::raw_tile; };
   auto valid_of = [&](int tile) { return min(kTile, k1 - k0 - tile * kTile); };
@@ -136,6 +126,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(p_full0 + 16 * s + 8, 128);
       mbar_init(o_full0 + 8 * s, 1);
     }
+    *jobs = 0;
     fence_mbar_init();
     tma_prefetch_desc(&map_k);
     tma_prefetch_desc(&map_v);
@@ -152,64 +143,64 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < kFirst) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSmall));
-    if (warp == 0) {
-      int pos = 0, r = 0;
-      uint32_t phase = 1;
-      // Page ids, 32 from `batch` on and the 32 after them (a value's tile is up to two behind the keys'): asked for long
-      // before they are needed, because a trip to memory takes as long as a tile.
-      const int ids_end = ((k1 - 1) >> a.page_shift) + 1;
+    if (warp % 2 == 0) {
+      const bool keys = warp == 0;
+      const CUtensorMap* const map = keys ? &map_k : &map_v;
+      // Page ids, 32 from `batch` on and the 32 after them, asked for long before they are needed: a trip to memory takes as
+      // long as a tile.
+      const int ids_end = ((k1 - 1) >> a.page_shift) + 1, in_page = (1 << a.page_shift) - 1;
       auto fetch = [&](int from) { return from + lane < ids_end ? a.prefix_pages[from + lane] : 0; };
       int batch = k0 >> a.page_shift, ids_now = fetch(batch), ids_next = fetch(batch + 32);
-      for (; pos < loads; ++pos) {
-        const Step step = step_of(pos, n_tiles, shared);
-        const int j0 = k0 + step.tile * kTile, boxes = (valid_of(step.tile) + per - 1) >> per_shift;
+      int r = warp / 2;  // the raw tile's place
+      uint32_t phase = 1;
+      int t = 0;
+      for (; t < n_tiles; ++t) {
+        const int j0 = k0 + t * kTile, boxes = (valid_of(t) + per - 1) >> per_shift;
         const uint32_t bar = raw_full0 + 8 * r;
-        if (!step.keys && (j0 >> a.page_shift) - batch >= 32) {
+        if ((j0 >> a.page_shift) - batch >= 32) {
           batch += 32;
           ids_now = ids_next;
           ids_next = fetch(batch + 32);
         }
-        const int at_id = ((j0 + lane * per) >> a.page_shift) - batch;
-        const int of_now = __shfl_sync(0xffffffffu, ids_now, at_id & 31), of_next = __shfl_sync(0xffffffffu, ids_next, at_id & 31);
-        int page = at_id < 32 ? of_now : of_next;
+        int page = __shfl_sync(0xffffffffu, ids_now, ((j0 >> a.page_shift) - batch + lane) & 31);
         if (!warp_wait(raw_empty0 + 8 * r, phase, a.status)) break;
         if (lane == 0) mbar_arrive_expect_tx(bar, boxes * per * D);
         __syncwarp();
         if (lane < boxes) {
           const bool there = page >= 0 && page < a.pages;
+          const long long at = there ? page * a.scale_ld + h * a.scale_head : 0;
+          const uint32_t to = sbase + S::scale_off + (r * 2 * 16 + lane) * 4;
           if (!there) {
             atomicCAS(a.errors, 0, kErrBadIndex);
             page = a.no_page;  // reads as zeros
           }
-          tma_load_4d(sbase + raw_at(r) + lane * per * D, step.keys ? &map_k : &map_v, 0, h, (j0 + lane * per) & ((1 << a.page_shift) - 1), page, bar);
-          const long long at = there ? page * a.scale_ld + h * a.scale_head : 0;
-          const uint32_t to = sbase + S::scale_off + (r * 2 * 16 + lane) * 4;
-          if (step.keys) copy_float(to, a.k_scales + at, there);
+          tma_load_4d(sbase + raw_at(r) + lane * per * D, map, 0, h, (j0 + lane * per) & in_page, page, bar);
+          if (keys) copy_float(to, a.k_scales + at, there);
           copy_float(to + 64, a.v_scales + at, there);
         }
         arrive_after_copies(bar);
-        if (++r == raws) r = 0, phase ^= 1;
+        if ((r += 2) >= 2 * raws) r -= 2 * raws, phase ^= 1;
       }
       // The block does not end before its last copies have arrived, also where another warp's wait was given up.
-      for (int p = max(0, pos - raws); p < pos; ++p) mbar_wait(raw_full0 + 8 * (p % raws), (p / raws) & 1, nullptr);
+      for (int x = max(0, t - raws); x < t; ++x) mbar_wait(raw_full0 + 8 * (2 * (x % raws) + warp / 2), (x / raws) & 1, nullptr);
     } else if (warp == 1) {
-      int pos = 0;
       // Whether this lane's waits have all ended well.  The lanes agree on it once a step (`settle`): a vote at each wait made
       // the bf16 kernel 2 % slower, and what a step computes past a wait that was given up is in bounds.
       bool good = true;
       auto settle = [&] { return __all_sync(0xffffffffu, good); };
-      auto wait_full = [&](int p) {
-        good = mbar_wait(full0 + 8 * (p % kStages), (p / kStages) & 1, a.status) && good;
+      auto keys_at = [&](int t) { return 2 * (t % kRing); };
+      auto values_at = [&](int t) { return 2 * (t % kRing) + 1; };
+      auto wait_full = [&](int st, int t) {
+        good = mbar_wait(full0 + 8 * st, (t / kRing) & 1, a.status) && good;
         tc_fence_after();
       };
       // (adding bytes / 16 to a descriptor moves its address: the tiles lie below 256 KB, so nothing carries)
       const uint64_t q_desc = smem_desc_sw128(sbase + S::q_off, 16, 1024);
       const uint64_t k_desc = smem_desc_sw128(sbase + S::kv_off, 16, 1024);
       const uint64_t v_desc = smem_desc_sw128(sbase + S::kv_off, kTile * 128, 1024);
-      auto tile_of = [&](int p) { return static_cast<uint64_t>(p % kStages) * (S::kv_tile / 16); };
       // S_s = Q_s K^T
-      auto scores = [&](int s, int p) {
-        const uint64_t qa = q_desc + (shared ? s : 0) * (S::q_tile / 16), kb = k_desc + tile_of(p);
+      auto scores = [&](int s, int t) {
+        const uint64_t qa = q_desc + (shared ? s : 0) * (S::q_tile / 16), kb = k_desc + static_cast<uint64_t>(keys_at(t)) * (S::kv_tile / 16);
         if (elected()) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
@@ -221,8 +212,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
       };
       // O_s (+)= P_s V, the first half of the keys while the second half's probabilities are still computed
-      auto values = [&](int s, int p, int step) {
-        const uint64_t vb = v_desc + tile_of(p);
+      auto values = [&](int s, int t, int step) {
+        const uint64_t vb = v_desc + static_cast<uint64_t>(values_at(t)) * (S::kv_tile / 16);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           good = mbar_wait(p_full0 + 16 * s + 8 * half, step & 1, a.status) && good;
@@ -236,92 +227,96 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
         }
       };
-      auto done_with = [&](int p) {
-        if (elected()) tc_commit(empty0 + 8 * (p % kStages));
+      auto commit = [&](uint32_t bar) {
+        if (elected()) tc_commit(bar);
         __syncwarp();
       };
       bool ok = warp_wait(q_full, 0, a.status);
       tc_fence_after();
       if (shared) {
         if (ok) {
-          wait_full(pos);
-          scores(0, pos);
-          scores(1, pos);
-          done_with(pos++);
+          wait_full(keys_at(0), 0);
+          scores(0, 0);
+          scores(1, 0);
+          commit(empty0 + 8 * keys_at(0));
           ok = settle();
         }
         for (int t = 0; t < n_tiles && ok; ++t) {
-          const int v = pos++, k = pos;
           const bool more = t + 1 < n_tiles;
-          if (more) ++pos;
-          wait_full(v);
-          values(0, v, t);
+          wait_full(values_at(t), t);
+          values(0, t, t);
           if (more) {
-            wait_full(k);
-            scores(0, k);
-          } else if (elected()) {
-            tc_commit(o_full0);
+            wait_full(keys_at(t + 1), t + 1);
+            scores(0, t + 1);
+          } else {
+            commit(o_full0);
           }
-          values(1, v, t);
-          done_with(v);
+          values(1, t, t);
+          commit(empty0 + 8 * values_at(t));
           if (more) {
-            scores(1, k);
-            done_with(k);
-          } else if (elected()) {
-            tc_commit(o_full0 + 8);
+            scores(1, t + 1);
+            commit(empty0 + 8 * keys_at(t + 1));
+          } else {
+            commit(o_full0 + 8);
           }
           ok = settle();
         }
       } else {
-        for (int s = 0; s < 2 && s < n_tiles && ok; ++s) {
-          wait_full(pos);
-          scores(s, pos);
-          done_with(pos++);
-          ok = settle();
-        }
+        auto next_scores = [&](int t) {
+          wait_full(keys_at(t), t);
+          scores(t & 1, t);
+          commit(empty0 + 8 * keys_at(t));
+        };
+        if (ok) next_scores(0);
+        if (n_tiles > 1 && ok) next_scores(1);
+        ok = settle() && ok;
         for (int t = 0; t < n_tiles && ok; ++t) {
           const int s = t & 1;
-          wait_full(pos);
-          values(s, pos, t >> 1);
-          done_with(pos++);
-          if (t + 2 < n_tiles) {
-            wait_full(pos);
-            scores(s, pos);
-            done_with(pos++);
-          } else if (elected()) {
-            tc_commit(o_full0 + 8 * s);
-          }
+          wait_full(values_at(t), t);
+          values(s, t, t >> 1);
+          commit(empty0 + 8 * values_at(t));
+          if (t + 2 < n_tiles) next_scores(t + 2);
+          else commit(o_full0 + 8 * s);
           ok = settle();
         }
       }
       if (!ok) {  // a wait was given up: nor do products end after their TMEM is freed
-        if (elected()) tc_commit(drained);
-        __syncwarp();
+        commit(drained);
         mbar_wait(drained, 0, nullptr);
       }
     }
   } else if (warp >= kFirst + kSoftmax / 32) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSmall));
-    // Widening: a thread has a row of the tile, so one scale.
-    const int self = threadIdx.x - (kThreads - kWiden), row = self % kTile, group = self / kTile;
-    int r = group, st = group;
-    uint32_t raw_phase = 0, phase = 1;
-    for (int pos = group; pos < loads; pos += 2) {
-      const Step step = step_of(pos, n_tiles, shared);
-      const int valid = valid_of(step.tile), boxes = (valid + per - 1) >> per_shift;
-      if (!warp_wait(raw_full0 + 8 * r, raw_phase, a.status) || !warp_wait(empty0 + 8 * st, phase, a.status)) break;
+    // Widening: a thread has a row of the tile, so one scale.  The warps take 32 rows of a tile as they come, in the order in
+    // which the products use the tiles: with few rows of queries only some of the SM's four schedulers have softmax warps to
+    // serve, and the warps of the others widen more.
+    int next_job = lane == 0 ? atomicAdd(jobs, 1) : 0;
+    for (;;) {
+      const int job = __shfl_sync(0xffffffffu, next_job, 0), turn = job / 4;
+      if (turn >= 2 * n_tiles) break;
+      if (lane == 0) next_job = atomicAdd(jobs, 1);
+      bool keys = turn % 2 == 0;
+      int t = turn / 2;
+      if (!shared && n_tiles > 1) {  // keys 0, keys 1, values 0, keys 2, values 1, ...
+        keys = turn < 2 || (turn % 2 == 1 && turn < 2 * n_tiles - 2);
+        t = turn < 2 ? turn : keys ? (turn + 1) / 2 : turn < 2 * n_tiles - 2 ? turn / 2 - 1 : turn - n_tiles;
+      }
+      const int row = job % 4 * 32 + lane;
+      const int r = 2 * (t & (raws - 1)) + !keys, st = 2 * (t % kRing) + !keys;
+      const int valid = valid_of(t), boxes = (valid + per - 1) >> per_shift;
+      if (!warp_wait(raw_full0 + 8 * r, (t >> raw_shift) & 1, a.status) || !warp_wait(empty0 + 8 * st, ((t / kRing) & 1) ^ 1, a.status)) break;
       const float* scales = reinterpret_cast<const float*>(sm + S::scale_off) + r * 2 * 16;
       auto largest = [&](float x) {  // of the pages' scales, and at least the least
         const float mine = lane < boxes ? fmaxf(x, kLeastScale) : kLeastScale;  // (also for what is no number)
         return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mine)));
       };
-      const float* const mine = scales + (step.keys ? 0 : 16);
+      const float* const mine = scales + (keys ? 0 : 16);
       const float top = largest(mine[lane & 15]), own = mine[min(row, valid - 1) >> per_shift];
-      const float factor = (step.keys ? own : fmaxf(own, kLeastScale)) * rcp_approx(top);
-      if (step.keys) {
+      const float factor = (keys ? own : fmaxf(own, kLeastScale)) * rcp_approx(top);
+      if (keys) {
         const float b = __log2f(largest(scales[16 + (lane & 15)]));
         if (row == 0)
-          *reinterpret_cast<float4*>(sm + S::info_off + step.tile % kInfo * 16) =
+          *reinterpret_cast<float4*>(sm + S::info_off + t % kInfo * 16) =
               make_float4(fminf(top, 3.4e38f) * a.scale_log2, b, ex2_approx(15.f - b), 0.f);
       }
       const uint32_t by = pack_f16x2(factor, factor);
@@ -375,8 +370,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(full0 + 8 * st);
         mbar_arrive(raw_empty0 + 8 * r);
       }
-      if ((r += 2) >= raws) r -= raws, raw_phase ^= 1;
-      if ((st += 2) >= kStages) st -= kStages, phase ^= 1;
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kLarge));
@@ -509,8 +502,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
           const float2 y = fma2(make_float2(v[c * 16 + i], v[c * 16 + i + 1]), scale2, base2);
-          // one pair of eight on the FMA pipe, as in the bf16 kernel
-          const float2 p = i == 6 ? exp2_fma(y) : make_float2(ex2_approx(y.x), ex2_approx(y.y));
+          // one pair of eight on the FMA pipe, as in the bf16 kernel, where both streams keep the exponential unit busy
+          const float2 p = i == 6 && shared ? exp2_fma(y) : make_float2(ex2_approx(y.x), ex2_approx(y.y));
           sum = add2(sum, p);
           w[i / 2] = pack_f16x2(p.x, p.y);
         }
