@@ -37,7 +37,6 @@ namespace q8 {
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kStep = 64;  // keys of a stage (2^6)
 constexpr float kBelow = 9.f, kPass = 15.f;  // the base below the maximum, and what a score may lie above the base
-constexpr int kTensorCoreRows = 16;  // more rows of a kv head than this go to the tensor-core kernel
 constexpr int kMostKnown = 1024;  // sequences whose lengths a block keeps
 
 template <int D, int NT>
@@ -627,8 +626,11 @@ int plan8(Args& a, int head_dim) {
   a.quad = false;
   const long long rows = static_cast<long long>(a.n) * a.group, own_rows = static_cast<long long>(a.max_q) * a.group;
   const bool own = a.max_len > 0 && a.max_q > 0 && a.batch > 0;
-  // (the tensor-core kernel takes maxima before it scales)
-  a.tensor_cores = a.prefix_len > 0 && head_dim != 32 && rows > q8::kTensorCoreRows && a.scale_log2 > 0.f;
+  // The tensor-core kernel for more rows than a warp takes, where that comes to enough steps of 16 rows and 64 keys: its blocks
+  // take 10 us before and after their tiles, in which the warps do some 2000 steps (20 rows of 16 kv heads over 4096 keys 22
+  // us, on tensor cores 25; 160 rows over 4096 keys 72 and 43).  (It takes maxima before it scales.)
+  const double steps = static_cast<double>(ceil_div(rows, 16)) * ceil_div(a.prefix_len, kStep) * a.kv_heads;
+  a.tensor_cores = a.prefix_len > 0 && head_dim != 32 && rows > 16 && steps > 2048 && a.scale_log2 > 0.f;
   a.tile_rows = std::max(a.prefix_len > 0 && !a.tensor_cores ? rows : 0, own ? own_rows : 0) <= 8 ? 8 : 16;
   const int warps = 148 * q8::kWarps * ((head_dim == 128 ? 3 : 4) - (a.tile_rows == 16 && head_dim > 32));
   const int prefix_tiles = ceil_div(a.prefix_len, kStep), own_tiles = ceil_div(a.max_len, kStep);

@@ -12,7 +12,7 @@
 //   s'_j = s_j + log2 R_v,  O = sum 2^(s'_j - base) (v_j / R_v),  sum_j 2^(s_j - base) = sum_j 2^(s'_j - base) / R_v,
 // one number each for a tile, so the softmax costs what it costs without scales.  The base
 // lies 7 below a maximum that scores may pass by 8, so a weight in f16 is at most 2^15.
-// Both R come with a tile's keys, before its scores.
+// Both R come with a tile's keys, before its scores, and one warp makes factors of them.
 //
 // What bounds it: with few rows the bytes (raw tiles then also lie where the second
 // stream's queries would be, so that 64 KB are under way), with many the softmax, beside
@@ -33,8 +33,8 @@ namespace tc8 {
 using namespace tc;
 using namespace q8;
 
-constexpr int kWiden = 256;  // threads that widen codes: a thread a row of a tile, a warp 32 of them
-// Warp 0 loads keys, 2 values, 1 issues the products (3 only fills its warpgroup), 4 to 19 do the softmax, 20 to 27 widen.  896 threads can have 72 registers each; the softmax takes over what the others do not need.
+constexpr int kWiden = 256;  // threads that widen codes: keys and values by a group each, a thread a row of a tile
+// Warp 0 loads keys, 2 values, 1 issues the products, 3 looks at scales, 4 to 19 do the softmax, 20 to 27 widen.  896 threads can have 72 registers each; the softmax takes over what the others do not need.
 constexpr int kThreads = 128 + kSoftmax + kWiden, kFirst = 4;
 constexpr int kLaunched = 72, kSmall = 48, kLarge = 88;
 static_assert((kThreads - kSoftmax) * kSmall + kSoftmax * kLarge <= kThreads * kLaunched, "registers");
@@ -47,14 +47,14 @@ struct Smem {
   static constexpr uint32_t kv_tile = kTile * D * 2;
   static constexpr uint32_t raw_tile = kTile * D;
   static constexpr int stages = D == 128 ? 4 : 6;
-  static constexpr int raws = D == 128 ? 2 : 8, more_raws = D == 128 ? 2 : 0;  // (with one tile of queries there is more room)
+  static constexpr int raws = D == 128 ? 2 : 4, more_raws = D == 128 ? 2 : 0;  // (with one tile of queries there is more room)
   static constexpr uint32_t q_off = 0, kv_off = 2 * q_tile, raw_off = kv_off + stages * kv_tile;
   static constexpr uint32_t bar_off = raw_off + raws * raw_tile;
-  static constexpr int n_bars = 2 * stages + 2 * (raws + more_raws) + 10;
+  static constexpr int n_bars = 2 * stages + 3 * (raws + more_raws) + 10;
   static constexpr uint32_t max_off = bar_off + n_bars * 8 + 16;    // row maxima so far: [stream][row], as order_of()
   static constexpr uint32_t scale_off = max_off + 2 * kTile * 4;    // of the raw tiles' pages: [raw][keys, values][16]
   static constexpr uint32_t info_off = scale_off + (raws + more_raws) * 2 * 16 * 4;  // of tiles: a float4 each
-  static constexpr uint32_t total = info_off + kInfo * 16 + 16 + 1024;  // (and the count of widening jobs)
+  static constexpr uint32_t total = info_off + kInfo * 16 + 1024;
   static_assert(more_raws * raw_tile <= q_tile, "room");
   static_assert(total <= 227 * 1024, "a block's shared memory");
   static_assert(max_off % 16 == 0, "alignment");
@@ -79,7 +79,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + S::n_bars);
   constexpr int kMostRaws = S::raws + S::more_raws;
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * kStages, raw_full0 = empty0 + 8 * kStages,
-                 raw_empty0 = raw_full0 + 8 * kMostRaws, q_full = raw_empty0 + 8 * kMostRaws, s_full0 = q_full + 8,
+                 raw_empty0 = raw_full0 + 8 * kMostRaws, scaled0 = raw_empty0 + 8 * kMostRaws, q_full = scaled0 + 8 * kMostRaws,
+                 s_full0 = q_full + 8,
                  o_full0 = s_full0 + 16, p_full0 = o_full0 + 16,  // (p_full: two halves per stream)
                  drained = p_full0 + 32;
 
@@ -101,10 +102,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int k0 = split * a.prefix_chunk, k1 = min(a.prefix_len, k0 + a.prefix_chunk);
   const int n_tiles = (k1 - k0 + kTile - 1) / kTile;
   // Rings of raw and of widened tiles: keys have the even places, values the odd ones.
-  const int raw_shift = D == 64 ? 2 : shared ? 0 : 1, raws = 1 << raw_shift;
+  const int raw_shift = D == 128 && shared ? 0 : 1, raws = 1 << raw_shift;
   constexpr int kRing = kStages / 2;
-  static_assert(S::raws == (D == 64 ? 8 : 2) && kMostRaws == (D == 64 ? 8 : 4), "keys and values have half of them each");
-  int* const jobs = reinterpret_cast<int*>(sm + S::info_off + kInfo * 16);
+  static_assert(S::raws == (D == 64 ? 4 : 2) && kMostRaws == 4 && kRing >= 2, "keys and values have half of them each");
   const int per_shift = min(a.page_shift, 7), per = 1 << per_shift;  // tokens of a box
   auto raw_at = [&](int r) { return r < S::raws ? S::raw_off + r * S::raw_tile : S::q_off + S::q_tile + (r - S::raws) * S::raw_tile; };
   auto valid_of = [&](int tile) { return min(kTile, k1 - k0 - tile * kTile); };
@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int r = 0; r < kMostRaws; ++r) {
       mbar_init(raw_full0 + 8 * r, 33);  // the expected bytes, and every lane's copies of scales
       mbar_init(raw_empty0 + 8 * r, kTile / 32);
+      mbar_init(scaled0 + 8 * r, 1);
     }
     mbar_init(q_full, kSoftmax);
     mbar_init(drained, 1);
@@ -126,7 +127,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(p_full0 + 16 * s + 8, 128);
       mbar_init(o_full0 + 8 * s, 1);
     }
-    *jobs = 0;
     fence_mbar_init();
     tma_prefetch_desc(&map_k);
     tma_prefetch_desc(&map_v);
@@ -284,41 +284,51 @@ __global__ void __launch_bounds__(kThreads, 1)
         commit(drained);
         mbar_wait(drained, 0, nullptr);
       }
+    } else {
+      // Scales become the factors of the pages' codes, in place, and the tile's own go to its info.
+      int r = 0;
+      uint32_t phase = 0;
+      float top_v = 0.f;
+      for (int t = 0, part = 0; t < n_tiles;) {
+        if (!warp_wait(raw_full0 + 8 * (r + part), phase, a.status)) break;
+        float* const scales = reinterpret_cast<float*>(sm + S::scale_off) + (r + part) * 2 * 16;
+        const int boxes = (valid_of(t) + per - 1) >> per_shift;
+        auto largest = [&](float x) {  // of the pages' scales, and at least the least
+          const float mine = lane < boxes ? fmaxf(x, kLeastScale) : kLeastScale;  // (also for what is no number)
+          return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mine)));
+        };
+        const float x = scales[part * 16 + (lane & 15)];
+        const float top = part ? top_v : largest(x);
+        if (!part) top_v = largest(scales[16 + (lane & 15)]);
+        __syncwarp();
+        if (lane < boxes) scales[part * 16 + lane] = (part ? fmaxf(x, kLeastScale) : x) * rcp_approx(top);
+        if (!part && lane == 0) {
+          const float b = __log2f(top_v);
+          *reinterpret_cast<float4*>(sm + S::info_off + t % kInfo * 16) = make_float4(fminf(top, 3.4e38f) * a.scale_log2, b, ex2_approx(15.f - b), 0.f);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(scaled0 + 8 * (r + part));
+        part ^= 1;
+        if (part == 0) {
+          ++t;
+          if ((r += 2) >= 2 * raws) r = 0, phase ^= 1;
+        }
+      }
     }
   } else if (warp >= kFirst + kSoftmax / 32) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSmall));
-    // Widening: a thread has a row of the tile, so one scale.  The warps take 32 rows of a tile as they come, in the order in
-    // which the products use the tiles: with few rows of queries only some of the SM's four schedulers have softmax warps to
-    // serve, and the warps of the others widen more.
-    int next_job = lane == 0 ? atomicAdd(jobs, 1) : 0;
-    for (;;) {
-      const int job = __shfl_sync(0xffffffffu, next_job, 0), turn = job / 4;
-      if (turn >= 2 * n_tiles) break;
-      if (lane == 0) next_job = atomicAdd(jobs, 1);
-      bool keys = turn % 2 == 0;
-      int t = turn / 2;
-      if (!shared && n_tiles > 1) {  // keys 0, keys 1, values 0, keys 2, values 1, ...
-        keys = turn < 2 || (turn % 2 == 1 && turn < 2 * n_tiles - 2);
-        t = turn < 2 ? turn : keys ? (turn + 1) / 2 : turn < 2 * n_tiles - 2 ? turn / 2 - 1 : turn - n_tiles;
-      }
-      const int row = job % 4 * 32 + lane;
-      const int r = 2 * (t & (raws - 1)) + !keys, st = 2 * (t % kRing) + !keys;
-      const int valid = valid_of(t), boxes = (valid + per - 1) >> per_shift;
-      if (!warp_wait(raw_full0 + 8 * r, (t >> raw_shift) & 1, a.status) || !warp_wait(empty0 + 8 * st, ((t / kRing) & 1) ^ 1, a.status)) break;
-      const float* scales = reinterpret_cast<const float*>(sm + S::scale_off) + r * 2 * 16;
-      auto largest = [&](float x) {  // of the pages' scales, and at least the least
-        const float mine = lane < boxes ? fmaxf(x, kLeastScale) : kLeastScale;  // (also for what is no number)
-        return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mine)));
-      };
-      const float* const mine = scales + (keys ? 0 : 16);
-      const float top = largest(mine[lane & 15]), own = mine[min(row, valid - 1) >> per_shift];
-      const float factor = (keys ? own : fmaxf(own, kLeastScale)) * rcp_approx(top);
-      if (keys) {
-        const float b = __log2f(largest(scales[16 + (lane & 15)]));
-        if (row == 0)
-          *reinterpret_cast<float4*>(sm + S::info_off + t % kInfo * 16) =
-              make_float4(fminf(top, 3.4e38f) * a.scale_log2, b, ex2_approx(15.f - b), 0.f);
-      }
+    // Widening: a thread has a row of the tile, so one scale.  (Every warp meets every phase of its barriers: one that took
+    // tiles out of turn could take a barrier two phases behind for one that is done.)
+    const int self = threadIdx.x - (kThreads - kWiden), row = self % kTile, group = self / kTile;
+    int r = group, st = group;
+    uint32_t raw_phase = 0, phase = 1;
+    for (int t = 0; t < n_tiles; ++t) {
+      const int valid = valid_of(t);
+      if (!warp_wait(raw_full0 + 8 * r, raw_phase, a.status) || !warp_wait(scaled0 + 8 * r, raw_phase, a.status) ||
+          !warp_wait(empty0 + 8 * st, phase, a.status))
+        break;
+      const float* const factors = reinterpret_cast<const float*>(sm + S::scale_off) + (r * 2 + group) * 16;
+      const float factor = factors[min(row, valid - 1) >> per_shift];
       const uint32_t by = pack_f16x2(factor, factor);
       // int8: (1024 + u) by - 1152 by in one step, which is exact where `by` is a power of two
       const uint32_t less = mul_f16x2(by, 0xe480e480u);
@@ -370,6 +380,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(full0 + 8 * st);
         mbar_arrive(raw_empty0 + 8 * r);
       }
+      if ((r += 2) >= 2 * raws) r -= 2 * raws, raw_phase ^= 1;
+      if ((st += 2) >= kStages) st -= kStages, phase ^= 1;
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kLarge));

@@ -354,6 +354,12 @@ SHAPES = [
     ([(5 * i) % 21 for i in range(450)], [i % 3 for i in range(450)], 6, 3, 32, 16, 40),
     ([1200, 3], [1, 1], 1, 1, 128, 128, 4500),
     ([33] * 1100, [1] * 1100, 1, 1, 32, 8, 0),  # more sequences than a block keeps the lengths of
+    # enough of a prefix for the tensor cores: rows in both streams, and in one; ends inside a tile and a page
+    ([2] * 180, [1] * 180, 12, 1, 128, 16, 1491),
+    ([i % 3 for i in range(40)], [1] * 40, 8, 4, 64, 64, 2500),
+    ([5, 0, 9] * 4, [1] * 12, 8, 4, 128, 8, 6001),
+    ([7] * 30, [1] * 30, 16, 1, 64, 128, 4100),
+    ([70, 90, 64], [60, 90, 34], 4, 3, 128, 32, 1000),
 ]
 
 
