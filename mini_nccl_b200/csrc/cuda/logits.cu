@@ -15,7 +15,10 @@
 // takes the word out first writes the token.  Only words of named tokens are ever
 // touched.  (Penalties applied on the way, in the copying pass, cost every warp the
 // arithmetic of each of its lanes' tokens in turn: 512 x 50304 with 1300 tokens named in
-// a row, 63 us.)
+// a row, 63 us.)  Measured: 512 x 50304 in bf16 34 us (3.0 TB/s; the lists are read by
+// each of a row's seven blocks), 129 x 130003 in fp32 under a mask and biases each
+// 34 us (4.0 TB/s), 64 x 50304 in fp32 under masks that leave a twenty-fifth 11 us, one
+// row 4 us.
 #include <algorithm>
 
 #include "common.cuh"
@@ -45,7 +48,7 @@ MNB_DEVICE float adjusted(float x, uint32_t named, float repetition, float prese
 
 // A block takes kThreads * kPer groups of eight tokens of a row.
 template <bool kBf16, int kThreads, int kPer>
-__global__ void __launch_bounds__(kThreads, kThreads == 512 ? 3 : 6) adjust_kernel(const __grid_constant__ Adjust a, int chunks) {
+__global__ void __launch_bounds__(kThreads, 5) adjust_kernel(const __grid_constant__ Adjust a, int chunks) {
   constexpr int kSize = kBf16 ? 2 : 4, kWords = kBf16 ? 4 : 8, kTokens = kThreads * kPer * 8, kList = 1024;
   static_assert(kTokens <= 1 << 14, "a place's bits");
   extern __shared__ uint32_t named[];  // [kTokens], where some list names tokens
@@ -69,6 +72,47 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 ? 3 : 6) adjust_kern
   }
   const uint32_t* const mask = of >= 0 ? a.allowed + of * a.mask_ld : nullptr;
   const int words = (a.vocab + 31) / 32;
+
+  // The copy, under the mask: its loads are on their way while the lists are looked through.
+  const bool copies = !a.in_place || mask;
+  auto token_of = [&](int k) { return first + (k * kThreads + static_cast<int>(threadIdx.x)) * 8; };
+  uint32_t allowed[kPer];  // of each group's tokens
+  uint32_t x[kPer][kWords];
+  if (copies) {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int v = token_of(k);
+      allowed[k] = 0xff;
+      if (mask && v < a.vocab && v + 8 > 0) {
+        const int at = max(v, 0), w = at >> 5;
+        const uint32_t lo = mask[w], hi = w + 1 < words && (at & 31) > 24 ? mask[w + 1] : 0u;
+        allowed[k] = (__funnelshift_r(lo, hi, at & 31) << (at - v)) & 0xff;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int v = token_of(k);
+#pragma unroll
+      for (int e = 0; e < kWords; ++e) x[k][e] = 0;
+      if (v >= a.vocab || !allowed[k] || (a.in_place && allowed[k] == 0xff)) continue;
+      if (in_aligned && v >= 0 && v + 8 <= a.vocab) {
+#pragma unroll
+        for (int q = 0; q < kWords / 4; ++q) {
+          const uint4 y = ld_v4(in + static_cast<long long>(v) * kSize + 16 * q);
+          x[k][4 * q] = y.x, x[k][4 * q + 1] = y.y, x[k][4 * q + 2] = y.z, x[k][4 * q + 3] = y.w;
+        }
+        continue;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (v + e >= 0 && v + e < a.vocab) {
+          if constexpr (kBf16)
+            x[k][e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(in)[v + e]) << (e % 2 * 16);
+          else
+            x[k][e] = reinterpret_cast<const uint32_t*>(in)[v + e];
+        }
+    }
+  }
 
   // The tokens of the row's lists that lie in the chunk: place, list (0 history, 1 prompt, 2 biases) and, of a bias, which.
   int held = static_cast<int>(a.history.n);
@@ -133,44 +177,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 ? 3 : 6) adjust_kern
     });
   }
 
-  // The copy, under the mask
-  if (!a.in_place || mask) {
-    auto token_of = [&](int k) { return first + (k * kThreads + static_cast<int>(threadIdx.x)) * 8; };
-    uint32_t allowed[kPer];  // of each group's tokens
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const int v = token_of(k);
-      allowed[k] = 0xff;
-      if (mask && v < a.vocab && v + 8 > 0) {
-        const int at = max(v, 0), w = at >> 5;
-        const uint32_t lo = mask[w], hi = w + 1 < words && (at & 31) > 24 ? mask[w + 1] : 0u;
-        allowed[k] = (__funnelshift_r(lo, hi, at & 31) << (at - v)) & 0xff;
-      }
-    }
-    uint32_t x[kPer][kWords];
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const int v = token_of(k);
-#pragma unroll
-      for (int e = 0; e < kWords; ++e) x[k][e] = 0;
-      if (v >= a.vocab || !allowed[k] || (a.in_place && allowed[k] == 0xff)) continue;
-      if (in_aligned && v >= 0 && v + 8 <= a.vocab) {
-#pragma unroll
-        for (int q = 0; q < kWords / 4; ++q) {
-          const uint4 y = ld_v4(in + static_cast<long long>(v) * kSize + 16 * q);
-          x[k][4 * q] = y.x, x[k][4 * q + 1] = y.y, x[k][4 * q + 2] = y.z, x[k][4 * q + 3] = y.w;
-        }
-        continue;
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (v + e >= 0 && v + e < a.vocab) {
-          if constexpr (kBf16)
-            x[k][e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(in)[v + e]) << (e % 2 * 16);
-          else
-            x[k][e] = reinterpret_cast<const uint32_t*>(in)[v + e];
-        }
-    }
+  // The copy's end
+  if (copies) {
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
       const int v = token_of(k);
@@ -239,11 +247,11 @@ cudaError_t launch(const Adjust& a, cudaStream_t stream) {
 }  // namespace
 
 cudaError_t launch_adjust(const Adjust& a, cudaStream_t stream) {
-  // 32 KB of a row to a block, so that few blocks read a row's lists; 4 KB (fp32: 8) where that would leave SMs without one
+  // 16 KB of a row to a block, so that few blocks read a row's lists (32 KB: 39 us where 16 KB take 34); 4 KB (fp32: 8) where that would leave SMs without one
   const int size = a.bf16 ? 2 : 4;
-  const bool few = static_cast<long long>(a.rows) * ((a.vocab * size + 32767) / 32768) < 148;
-  if (a.bf16) return few ? launch<true, 256, 1>(a, stream) : launch<true, 512, 4>(a, stream);
-  return few ? launch<false, 256, 1>(a, stream) : launch<false, 512, 2>(a, stream);
+  const bool few = static_cast<long long>(a.rows) * ((a.vocab * size + 16383) / 16384) < 148;
+  if (a.bf16) return few ? launch<true, 256, 1>(a, stream) : launch<true, 256, 4>(a, stream);
+  return few ? launch<false, 256, 1>(a, stream) : launch<false, 256, 2>(a, stream);
 }
 
 }  // namespace logits
