@@ -2,10 +2,13 @@
 
     python examples/sample_gpt.py --steps 200 --branches 8
     python examples/sample_gpt.py --device cuda --branches 64 --top-p 0.95 --resample-every 16
+    python examples/sample_gpt.py --cache-dtype e4m3 --repetition 1.2 --only "abcdefghijklmnopqrstuvwxyz .,"
 
 The prompt runs through the model once; the continuations share its keys and
 values in a paged cache.  With ``--resample-every`` the likelier half of the
 branches replaces the other half every so many tokens (fork, free, compact).
+``--cache-dtype`` holds the cache in 8 bits; ``--repetition``, ``--presence``,
+``--frequency`` and ``--only`` change the scores before a token is drawn.
 """
 
 from __future__ import annotations
@@ -40,6 +43,11 @@ def main() -> None:
     ap.add_argument("--top-p", type=float, default=0.95)
     ap.add_argument("--min-p", type=float, default=0.0)
     ap.add_argument("--resample-every", type=int, default=0)
+    ap.add_argument("--cache-dtype", choices=["same", "int8", "e4m3"], default="same", help="type of the cache's keys and values")
+    ap.add_argument("--repetition", type=float, default=1.0)
+    ap.add_argument("--presence", type=float, default=0.0)
+    ap.add_argument("--frequency", type=float, default=0.0)
+    ap.add_argument("--only", help="characters that may be drawn")
     args = ap.parse_args()
 
     data, vocab = encode(load_corpus(args.data))
@@ -64,10 +72,19 @@ def main() -> None:
 
     prompt = torch.tensor([vocab.index(ch) for ch in args.prompt if ch in vocab], device=dev)
     gen = torch.Generator(device=dev).manual_seed(1)
+    allowed = None
+    if args.only:
+        words = [0] * -(-size // 32)
+        for i, ch in enumerate(vocab):
+            if ch in args.only:
+                words[i // 32] |= 1 << i % 32
+        allowed = torch.tensor([w - (w >> 31 << 32) for w in words], dtype=torch.int32, device=dev)[None]
     start = time.perf_counter()
     tokens, logprobs = sample_continuations(
         model, prompt, args.branches, args.new_tokens, temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
-        min_p=args.min_p, generator=gen, resample_every=args.resample_every)
+        min_p=args.min_p, generator=gen, resample_every=args.resample_every,
+        cache_dtype={"same": None, "int8": torch.int8, "e4m3": torch.float8_e4m3fn}[args.cache_dtype], repetition=args.repetition,
+        presence=args.presence, frequency=args.frequency, allowed=allowed)
     tokens, mean = tokens.tolist(), logprobs.mean(1).tolist()
     seconds = time.perf_counter() - start
     if dev.type == "cuda":

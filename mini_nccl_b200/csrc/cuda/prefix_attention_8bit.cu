@@ -294,253 +294,253 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NT>::blocks)
   p.k1 = 0;
   // Stage by stage, the first kStages steps only load.
   for (int pos = -kStages;; ++pos) {
-  const bool work = pos >= 0;
-  if (work && t0 >= p.k1) {  // the next piece
-    if (taken == queued) break;
-    __syncwarp();
-    p = queue[warp][taken % kQueue].p, part_end = queue[warp][taken % kQueue].part_end;
-    ++taken;
-    t0 = p.k0;
-    // Queries as the products' second operand: row n * 8 + g, four dims (those of a word of codes) for each 16-wide step.
+    const bool work = pos >= 0;
+    if (work && t0 >= p.k1) {  // the next piece
+      if (taken == queued) break;
+      __syncwarp();
+      p = queue[warp][taken % kQueue].p, part_end = queue[warp][taken % kQueue].part_end;
+      ++taken;
+      t0 = p.k0;
+      // Queries as the products' second operand: row n * 8 + g, four dims (those of a word of codes) for each 16-wide step.
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int r = n * 8 + g, j = p.r0 + r, token = j / a.group;
-      const bool in = r < p.n_rows;
-      const __nv_bfloat16* q = a.q + (p.n0 + token) * a.q_ld + (p.h * a.group + j - token * a.group) * a.q_head;
-      uint4 w[kMt / 2];
+      for (int n = 0; n < NT; ++n) {
+        const int r = n * 8 + g, j = p.r0 + r, token = j / a.group;
+        const bool in = r < p.n_rows;
+        const __nv_bfloat16* q = a.q + (p.n0 + token) * a.q_ld + (p.h * a.group + j - token * a.group) * a.q_head;
+        uint4 w[kMt / 2];
 #pragma unroll
-      for (int x = 0; x < kMt / 2; ++x) {
-        const int dim = D == 32 ? 8 * t : (x / 2) * 64 + 16 * t + (x % 2) * 8;
-        w[x] = in ? ld_v4(q + dim) : make_uint4(0, 0, 0, 0);
-      }
-      uint32_t most = 0;  // of the finite values, as bits
-#pragma unroll
-      for (int x = 0; x < kMt / 2; ++x)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t v = (&w[x].x)[e], lo = v & 0x7fffu, hi = (v >> 16) & 0x7fffu;
-          most = max(most, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+        for (int x = 0; x < kMt / 2; ++x) {
+          const int dim = D == 32 ? 8 * t : (x / 2) * 64 + 16 * t + (x % 2) * 8;
+          w[x] = in ? ld_v4(q + dim) : make_uint4(0, 0, 0, 0);
         }
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      const int shift = min(141 - static_cast<int>(most >> 7), 126);  // the largest becomes 2^14 to 2^15
-      const float up = __int_as_float((127 + shift) << 23);
+        uint32_t most = 0;  // of the finite values, as bits
 #pragma unroll
-      for (int x = 0; x < kMt / 2; ++x)
+        for (int x = 0; x < kMt / 2; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t v = (&w[x].x)[e], lo = v & 0x7fffu, hi = (v >> 16) & 0x7fffu;
+            most = max(most, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+          }
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const int shift = min(141 - static_cast<int>(most >> 7), 126);  // the largest becomes 2^14 to 2^15
+        const float up = __int_as_float((127 + shift) << 23);
+#pragma unroll
+        for (int x = 0; x < kMt / 2; ++x)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float2 u = unpack_bf16x2((&w[x].x)[2 * e]), v = unpack_bf16x2((&w[x].x)[2 * e + 1]);
+            u = mul2(u, splat2(up)), v = mul2(v, splat2(up));
+            qf[n][2 * x + e][0] = kFloat ? pack_f16x2(u.x, u.y) : pack_f16x2(u.x, v.x);
+            qf[n][2 * x + e][1] = kFloat ? pack_f16x2(v.x, v.y) : pack_f16x2(u.y, v.y);
+          }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float2 u = unpack_bf16x2((&w[x].x)[2 * e]), v = unpack_bf16x2((&w[x].x)[2 * e + 1]);
-          u = mul2(u, splat2(up)), v = mul2(v, splat2(up));
-          qf[n][2 * x + e][0] = kFloat ? pack_f16x2(u.x, u.y) : pack_f16x2(u.x, v.x);
-          qf[n][2 * x + e][1] = kFloat ? pack_f16x2(v.x, v.y) : pack_f16x2(u.y, v.y);
+          const int row = n * 8 + 2 * t + e;
+          back[n][e] = __int_as_float((127 - __shfl_sync(0xffffffffu, shift, (2 * t + e) * 4)) << 23);
+          lim[n][e] = row < p.n_rows ? min(p.k1, p.limit0 + (p.r0 + row) / a.group) : p.k0;
         }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int row = n * 8 + 2 * t + e;
-        back[n][e] = __int_as_float((127 - __shfl_sync(0xffffffffu, shift, (2 * t + e) * 4)) << 23);
-        lim[n][e] = row < p.n_rows ? min(p.k1, p.limit0 + (p.r0 + row) / a.group) : p.k0;
       }
-    }
-    whole = min(p.k1, p.limit0 + p.r0 / a.group);
+      whole = min(p.k1, p.limit0 + p.r0 / a.group);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      base[n][0] = base[n][1] = -INFINITY;
-      l[n][0] = l[n][1] = 0.f;
+      for (int n = 0; n < NT; ++n) {
+        base[n][0] = base[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = 0.f;
 #pragma unroll
-      for (int m = 0; m < kMt; ++m) o[n][m][0] = o[n][m][1] = o[n][m][2] = o[n][m][3] = 0.f;
-    }
+        for (int m = 0; m < kMt; ++m) o[n][m][0] = o[n][m][1] = o[n][m][2] = o[n][m][3] = 0.f;
+      }
 
-  }
-      const int st = max(pos, 0) % kStages;
-      const uint32_t phase = (pos / kStages) & 1;
-      if (work) mbar_wait(full_k + 8 * st, phase, a.status);  // (a wait that gave up is in the status word)
-      __syncwarp();
-      const uint32_t sK = ring + st * 2 * R::tile, sV = sK + R::tile;
-      // Each eight keys lie in one page: its factor of the scores, the logarithm of its values' scale, and what turns a
-      // weight into its part of the sum (times 2^15, so that nothing leaves the range of fp32).
-      if (work && lane < 8) {
-        const int box = (lane * 8) >> a.page_shift;
-        const float b = __log2f(fmaxf(scale_of[warp][st][1][box], kLeastScale));  // (a page of zeros may have any scale)
-        factor_of[warp][lane] = make_float4(scale_of[warp][st][0][box] * a.scale_log2, b, ex2_approx(15.f - b), 0.f);
-      }
-      __syncwarp();
-      bool spoiled = false;
+    }
+    const int st = max(pos, 0) % kStages;
+    const uint32_t phase = (pos / kStages) & 1;
+    if (work) mbar_wait(full_k + 8 * st, phase, a.status);  // (a wait that gave up is in the status word)
+    __syncwarp();
+    const uint32_t sK = ring + st * 2 * R::tile, sV = sK + R::tile;
+    // Each eight keys lie in one page: its factor of the scores, the logarithm of its values' scale, and what turns a
+    // weight into its part of the sum (times 2^15, so that nothing leaves the range of fp32).
+    if (work && lane < 8) {
+      const int box = (lane * 8) >> a.page_shift;
+      const float b = __log2f(fmaxf(scale_of[warp][st][1][box], kLeastScale));  // (a page of zeros may have any scale)
+      factor_of[warp][lane] = make_float4(scale_of[warp][st][0][box] * a.scale_log2, b, ex2_approx(15.f - b), 0.f);
+    }
+    __syncwarp();
+    bool spoiled = false;
 #pragma unroll 1
-      for (int part = 0; part < kStep / kPart; ++part) {
-        const int t1 = t0 + part * kPart;
-        const bool live = work && (part == 0 || t1 < p.k1);
-        float s[NT][kU][4];
-        if (live) {
+    for (int part = 0; part < kStep / kPart; ++part) {
+      const int t1 = t0 + part * kPart;
+      const bool live = work && (part == 0 || t1 < p.k1);
+      float s[NT][kU][4];
+      if (live) {
 #pragma unroll
-          for (int u = 0; u < kU; ++u) {
+        for (int u = 0; u < kU; ++u) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) s[n][u][0] = s[n][u][1] = s[n][u][2] = s[n][u][3] = 0.f;
+          for (int n = 0; n < NT; ++n) s[n][u][0] = s[n][u][1] = s[n][u][2] = s[n][u][3] = 0.f;
 #pragma unroll
-            for (int x = 0; x < (D + 63) / 64; ++x) {
-              uint4 ka, kb;  // a row's words: two of them at head dim 32
-              const uint32_t from = (sK + (part * kPart + u * 16) * D + at_k) ^ (x * 64);
-              if (D == 32) {
-                asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(ka.x), "=r"(ka.y) : "r"(from));
-                asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(kb.x), "=r"(kb.y) : "r"(from + 8 * D));
-              } else {
-                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(ka.x), "=r"(ka.y), "=r"(ka.z), "=r"(ka.w) : "r"(from));
-                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(kb.x), "=r"(kb.y), "=r"(kb.z), "=r"(kb.w) : "r"(from + 8 * D));
-              }
+          for (int x = 0; x < (D + 63) / 64; ++x) {
+            uint4 ka, kb;  // a row's words: two of them at head dim 32
+            const uint32_t from = (sK + (part * kPart + u * 16) * D + at_k) ^ (x * 64);
+            if (D == 32) {
+              asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(ka.x), "=r"(ka.y) : "r"(from));
+              asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(kb.x), "=r"(kb.y) : "r"(from + 8 * D));
+            } else {
+              asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(ka.x), "=r"(ka.y), "=r"(ka.z), "=r"(ka.w) : "r"(from));
+              asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(kb.x), "=r"(kb.y), "=r"(kb.z), "=r"(kb.w) : "r"(from + 8 * D));
+            }
 #pragma unroll
-              for (int j = 0; j < (D == 32 ? 2 : 4); ++j) {
-                uint32_t f[4];
-                widen_any<kFloat>((&ka.x)[j], f[0], f[2]);
-                widen_any<kFloat>((&kb.x)[j], f[1], f[3]);
+            for (int j = 0; j < (D == 32 ? 2 : 4); ++j) {
+              uint32_t f[4];
+              widen_any<kFloat>((&ka.x)[j], f[0], f[2]);
+              widen_any<kFloat>((&kb.x)[j], f[1], f[3]);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma_f16(s[n][u], f, qf[n][x * 4 + j]);
-              }
+              for (int n = 0; n < NT; ++n) mma_f16(s[n][u], f, qf[n][x * 4 + j]);
             }
           }
         }
-        if (part == kStep / kPart - 1) {
-          __syncwarp();  // (the keys and scales have been read)
-          issue_keys();
+      }
+      if (part == kStep / kPart - 1) {
+        __syncwarp();  // (the keys and scales have been read)
+        issue_keys();
+      }
+      if (!live) continue;
+      float sum_of[kU][2];
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float4 f = factor_of[warp][2 * (part * kU + u) + h];
+          sum_of[u][h] = f.z;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              // (towards zero: a factor past fp32's range stays finite, and 0 times it stays 0)
+              s[n][u][2 * h + e] = fmaf(s[n][u][2 * h + e], __fmul_rz(f.x, back[n][e]), f.y);
         }
-        if (!live) continue;
-        float sum_of[kU][2];
+      const bool masked = t1 + kPart > whole;
+      if (masked) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int u = 0; u < kU; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (t1 + u * 16 + e / 2 * 8 + key_of<D>(g) >= lim[n][e & 1]) s[n][u][e] = -INFINITY;
+      }
+      float top[NT][2];
+      bool grows = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = fmaxf(s[n][0][e], s[n][0][2 + e]);
+#pragma unroll
+          for (int u = 1; u < kU; ++u) x = max3f(x, s[n][u][e], s[n][u][2 + e]);
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          top[n][e] = x;
+          grows = grows || x > base[n][e] + kPass || (base[n][e] == -INFINITY && x > -INFINITY);
+        }
+      if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float alpha[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float to = top[n][e] > base[n][e] + kPass || base[n][e] == -INFINITY ? top[n][e] - kBelow : base[n][e];
+            alpha[e] = to == base[n][e] ? 1.f : ex2_approx(base[n][e] - to);
+            l[n][e] *= alpha[e];
+            base[n][e] = to;
+          }
+#pragma unroll
+          for (int m = 0; m < kMt; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][m][e] *= alpha[e & 1];
+        }
+      }
+      uint32_t pf[NT][kU][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        // (no key yet: every weight is exp2(-inf) = 0)
+        const float from0 = base[n][0] == -INFINITY ? 0.f : base[n][0], from1 = base[n][1] == -INFINITY ? 0.f : base[n][1];
 #pragma unroll
         for (int u = 0; u < kU; ++u)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float4 f = factor_of[warp][2 * (part * kU + u) + h];
-            sum_of[u][h] = f.z;
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                // (towards zero: a factor past fp32's range stays finite, and 0 times it stays 0)
-                s[n][u][2 * h + e] = fmaf(s[n][u][2 * h + e], __fmul_rz(f.x, back[n][e]), f.y);
+            const float w0 = ex2_approx(s[n][u][2 * h] - from0), w1 = ex2_approx(s[n][u][2 * h + 1] - from1);
+            l[n][0] = fmaf(w0, sum_of[u][h], l[n][0]);
+            l[n][1] = fmaf(w1, sum_of[u][h], l[n][1]);
+            pf[n][u][h] = transposed(pack_f16x2(w0, w1));
           }
-        const bool masked = t1 + kPart > whole;
-        if (masked) {
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int u = 0; u < kU; ++u)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (t1 + u * 16 + e / 2 * 8 + key_of<D>(g) >= lim[n][e & 1]) s[n][u][e] = -INFINITY;
+      }
+      if (part == 0) {
+        mbar_wait(full_v + 8 * st, phase, a.status);
+        __syncwarp();
+      }
+      if constexpr (kFloat) {
+        // A key that a row does not see has weight 0, and 0 times NaN (which e4m3 has, also past the end of the keys, where
+        // a page holds anything) would be NaN: such codes become zeros here, and rows that do see one become NaN below.
+        if (part == 0 && t0 + kStep > whole) {
+          uint32_t some = 0;
+          for (int x = lane; x < kStep * D / 16; x += 32) {
+            uint4 w;
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(sV + x * 16));
+            some |= nan_bytes(w.x) | nan_bytes(w.y) | nan_bytes(w.z) | nan_bytes(w.w);
+          }
+          spoiled = __any_sync(0xffffffffu, some != 0);
+          if (spoiled) {
+            for (int x = lane; x < kRows * (D / 32); x += 32) (&nan_at[warp][0][0])[x] = 0;
+            __syncwarp();
+#pragma unroll 1
+            for (int x = lane; x < kStep * D / 4; x += 32) {  // word by word
+              const int key = x / (D / 4), word = x % (D / 4);
+              const uint32_t at = sV + R::at(key, word / 4) + word % 4 * 4;
+              uint32_t w;
+              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at));
+              const uint32_t odd = nan_bytes(w);
+              if (!odd) continue;
+              asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(w & ~(odd * 0xffu)) : "memory");
+              const uint32_t bits = ((odd & 1u) | (odd >> 7 & 2u) | (odd >> 14 & 4u) | (odd >> 21 & 8u)) << (word % 8 * 4);
+              for (int row = 0; row < p.n_rows; ++row)
+                if (t0 + key < min(p.k1, p.limit0 + (p.r0 + row) / a.group)) atomicOr(&nan_at[warp][row][word / 8], bits);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // TMA writes here next
+            __syncwarp();
+          }
         }
-        float top[NT][2];
-        bool grows = false;
+      }
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+#pragma unroll
+        for (int c = 0; c < kMt / 2; ++c) {
+          uint32_t w[4];
+          ldsm_x4_t(w, (sV + (part * kPart + u * 16) * D + at_v) ^ (c * 32));
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            uint32_t f[4];
+            widen<kFloat>(w[2 * m], f[0], f[1]);
+            widen<kFloat>(w[2 * m + 1], f[2], f[3]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * c + m], f, pf[n][u]);
+          }
+        }
+      if (kFloat && spoiled) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float x = fmaxf(s[n][0][e], s[n][0][2 + e]);
+          for (int m = 0; m < kMt; ++m)
 #pragma unroll
-            for (int u = 1; u < kU; ++u) x = max3f(x, s[n][u][e], s[n][u][2 + e]);
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-            top[n][e] = x;
-            grows = grows || x > base[n][e] + kPass || (base[n][e] == -INFINITY && x > -INFINITY);
-          }
-        if (__any_sync(0xffffffffu, grows)) {
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float alpha[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float to = top[n][e] > base[n][e] + kPass || base[n][e] == -INFINITY ? top[n][e] - kBelow : base[n][e];
-              alpha[e] = to == base[n][e] ? 1.f : ex2_approx(base[n][e] - to);
-              l[n][e] *= alpha[e];
-              base[n][e] = to;
+            for (int e = 0; e < 4; ++e) {
+              const int dim = m * 16 + 2 * g + e / 2;
+              if (nan_at[warp][n * 8 + 2 * t + e % 2][dim / 32] >> (dim % 32) & 1) o[n][m][e] = NAN;
             }
-#pragma unroll
-            for (int m = 0; m < kMt; ++m)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[n][m][e] *= alpha[e & 1];
-          }
-        }
-        uint32_t pf[NT][kU][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          // (no key yet: every weight is exp2(-inf) = 0)
-          const float from0 = base[n][0] == -INFINITY ? 0.f : base[n][0], from1 = base[n][1] == -INFINITY ? 0.f : base[n][1];
-#pragma unroll
-          for (int u = 0; u < kU; ++u)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float w0 = ex2_approx(s[n][u][2 * h] - from0), w1 = ex2_approx(s[n][u][2 * h + 1] - from1);
-              l[n][0] = fmaf(w0, sum_of[u][h], l[n][0]);
-              l[n][1] = fmaf(w1, sum_of[u][h], l[n][1]);
-              pf[n][u][h] = transposed(pack_f16x2(w0, w1));
-            }
-        }
-        if (part == 0) {
-          mbar_wait(full_v + 8 * st, phase, a.status);
-          __syncwarp();
-        }
-        if constexpr (kFloat) {
-          // A key that a row does not see has weight 0, and 0 times NaN (which e4m3 has, also past the end of the keys, where
-          // a page holds anything) would be NaN: such codes become zeros here, and rows that do see one become NaN below.
-          if (part == 0 && t0 + kStep > whole) {
-            uint32_t some = 0;
-            for (int x = lane; x < kStep * D / 16; x += 32) {
-              uint4 w;
-              asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(sV + x * 16));
-              some |= nan_bytes(w.x) | nan_bytes(w.y) | nan_bytes(w.z) | nan_bytes(w.w);
-            }
-            spoiled = __any_sync(0xffffffffu, some != 0);
-            if (spoiled) {
-              for (int x = lane; x < kRows * (D / 32); x += 32) (&nan_at[warp][0][0])[x] = 0;
-              __syncwarp();
-#pragma unroll 1
-              for (int x = lane; x < kStep * D / 4; x += 32) {  // word by word
-                const int key = x / (D / 4), word = x % (D / 4);
-                const uint32_t at = sV + R::at(key, word / 4) + word % 4 * 4;
-                uint32_t w;
-                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at));
-                const uint32_t odd = nan_bytes(w);
-                if (!odd) continue;
-                asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(w & ~(odd * 0xffu)) : "memory");
-                const uint32_t bits = ((odd & 1u) | (odd >> 7 & 2u) | (odd >> 14 & 4u) | (odd >> 21 & 8u)) << (word % 8 * 4);
-                for (int row = 0; row < p.n_rows; ++row)
-                  if (t0 + key < min(p.k1, p.limit0 + (p.r0 + row) / a.group)) atomicOr(&nan_at[warp][row][word / 8], bits);
-              }
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // TMA writes here next
-              __syncwarp();
-            }
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < kU; ++u)
-#pragma unroll
-          for (int c = 0; c < kMt / 2; ++c) {
-            uint32_t w[4];
-            ldsm_x4_t(w, (sV + (part * kPart + u * 16) * D + at_v) ^ (c * 32));
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-              uint32_t f[4];
-              widen<kFloat>(w[2 * m], f[0], f[1]);
-              widen<kFloat>(w[2 * m + 1], f[2], f[3]);
-#pragma unroll
-              for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * c + m], f, pf[n][u]);
-            }
-          }
-        if (kFloat && spoiled) {
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int m = 0; m < kMt; ++m)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int dim = m * 16 + 2 * g + e / 2;
-                if (nan_at[warp][n * 8 + 2 * t + e % 2][dim / 32] >> (dim % 32) & 1) o[n][m][e] = NAN;
-              }
-        }
       }
-      __syncwarp();
-      issue_values();
-      if (!work) continue;
-      t0 += kStep;
-      if (t0 < p.k1) continue;
+    }
+    __syncwarp();
+    issue_values();
+    if (!work) continue;
+    t0 += kStep;
+    if (t0 < p.k1) continue;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll

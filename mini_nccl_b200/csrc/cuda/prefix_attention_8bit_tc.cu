@@ -4,7 +4,9 @@
 // mathematics of scales and weights; here the two meet.
 //
 // Codes come page by page into a ring of raw tiles (128 keys, or their values); four
-// warps widen each into the swizzled f16 tile that the products read.  An f16 tile holds
+// warps widen those of keys and four those of values into the swizzled f16 tiles that the
+// products read.  (Each group meets every phase of its barriers, in order: a wait by
+// parity takes a barrier that is two phases behind for done.)  An f16 tile holds
 // code * scale / R, with R the largest scale of the tile's pages: exact while the pages
 // of 128 tokens next to one another have scales within a factor of 2^15 (2^17 for int8);
 // a value of a page further below R is rounded to a multiple of R 2^-24.  R of the keys
@@ -14,9 +16,12 @@
 // lies 7 below a maximum that scores may pass by 8, so a weight in f16 is at most 2^15.
 // Both R come with a tile's keys, before its scores, and one warp makes factors of them.
 //
-// What bounds it: with few rows the bytes (raw tiles then also lie where the second
-// stream's queries would be, so that 64 KB are under way), with many the softmax, beside
-// which the widening warps take a fifth of the issue slots.
+// What bounds it: the widening and the softmax, which share the issue slots and the shared
+// memory's bandwidth: 1.4 us for a tile of 128 keys whether one stream has rows or both,
+// and 20 us before the first and after the last.  (With few rows raw tiles also lie where
+// the second stream's queries would be, so that 64 KB are under way.)  Measured: 48 rows of
+// 8 kv heads behind 100003 tokens 93 us (2.4 TB/s of codes), 160 rows of 16 heads behind
+// 8003 tokens 87 us with their own keys, 2400 ragged rows of 32 heads 211 us with theirs.
 #include <type_traits>
 
 #include "launch.cuh"
@@ -34,7 +39,8 @@ using namespace tc;
 using namespace q8;
 
 constexpr int kWiden = 256;  // threads that widen codes: keys and values by a group each, a thread a row of a tile
-// Warp 0 loads keys, 2 values, 1 issues the products, 3 looks at scales, 4 to 19 do the softmax, 20 to 27 widen.  896 threads can have 72 registers each; the softmax takes over what the others do not need.
+// Warp 0 loads keys, 2 values, 1 issues the products, 3 looks at scales, 4 to 19 do the softmax, 20 to 27 widen.  896 threads
+// can have 72 registers each; the softmax takes over what the others do not need.
 constexpr int kThreads = 128 + kSoftmax + kWiden, kFirst = 4;
 constexpr int kLaunched = 72, kSmall = 48, kLarge = 88;
 static_assert((kThreads - kSoftmax) * kSmall + kSoftmax * kLarge <= kThreads * kLaunched, "registers");
@@ -453,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int valid = k1 - k0 - tile * kTile - half * 64;  // keys of this half tile (or more, or none)
       const float4 info = *reinterpret_cast<const float4*>(sm + S::info_off + tile % kInfo * 16);
       // (towards zero, so that past fp32's range it stays finite and 0 times it 0; above 0, so that masked scores stay -inf)
-        const float factor = fmaxf(__fmul_rz(info.x, back), 1.2e-38f);
+      const float factor = fmaxf(__fmul_rz(info.x, back), 1.2e-38f);
       float v[64];
       tmem_ld_32(t_s + half * 64, v);
       tmem_ld_32(t_s + half * 64 + 32, v + 32);

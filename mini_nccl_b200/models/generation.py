@@ -4,9 +4,13 @@ The prompt runs through the model once and its keys and values stay in a paged
 cache; every continuation ("branch") adds pages of its own.  A step feeds one
 token per branch: the attention reads the prompt's pages once for all branches
 (:func:`~mini_nccl_b200.ops.generation.shared_prefix_attention`), the next
-tokens are drawn by :func:`~mini_nccl_b200.ops.generation.sample`, and branches
-are copied, dropped and moved together by the page operations.  A CUDA model
-(bf16) runs the sm_100a kernels, a CPU model the plain PyTorch path.
+tokens' scores are penalised and masked by
+:func:`~mini_nccl_b200.ops.generation.adjust_logits` where that is asked for and
+drawn by :func:`~mini_nccl_b200.ops.generation.sample`, and branches are copied,
+dropped and moved together by the page operations.  The cache holds the
+weights' type, or 8 bits (``cache_dtype``: int8 or float8_e4m3fn), which is half
+the memory and half of what the attention reads.  A CUDA model (bf16) runs the
+sm_100a kernels, a CPU model the plain PyTorch path.
 """
 
 from __future__ import annotations
@@ -48,10 +52,13 @@ class BranchedGeneration:
     ``branches``; at first there is one branch, which holds nothing yet.
     The model is a plain :class:`GPT`: one whose blocks are wrapped (sharded
     by ``FullyShardedDataParallel``) is refused with ``ValueError``.
+    ``cache_dtype`` is the weights' type (the default), int8 or float8_e4m3fn;
+    the prompt's own pass through the model does not read the cache.
     """
 
     @torch.no_grad()
-    def __init__(self, model: GPT, prompt: torch.Tensor, *, max_branches: int, max_new_tokens: int, page_size: int = 16) -> None:
+    def __init__(self, model: GPT, prompt: torch.Tensor, *, max_branches: int, max_new_tokens: int, page_size: int = 16,
+                 cache_dtype: torch.dtype | None = None) -> None:
         prompt = prompt.reshape(-1)
         P, self._blocks = prompt.numel(), _plain_blocks(model)
         if P < 1 or max_branches < 1 or max_new_tokens < 1:
@@ -60,11 +67,13 @@ class BranchedGeneration:
             raise ValueError(f"{P} + {max_new_tokens} tokens are more than the model's {model.block_size} positions")
         self.model, self.prompt_len, self.max_new_tokens = model, P, max_new_tokens
         cfg, w = model.config, model.tok_emb.weight
+        if cache_dtype is not None and cache_dtype != w.dtype and cache_dtype not in G.TOP_CODE:
+            raise ValueError(f"cache_dtype: the weights' {w.dtype}, int8 or float8_e4m3fn, not {cache_dtype}")
         self.heads, self.head_dim = cfg.n_head, cfg.n_embd // cfg.n_head
         pages = -(-P // page_size) + max_branches * -(-max_new_tokens // page_size)
         # slot 0 is the prompt's
         self.cache = G.PagedKVCache(cfg.n_layer, pages, page_size, self.heads, self.head_dim, max_seqs=max_branches + 1,
-                                    max_seq_len=max(P, max_new_tokens), device=w.device, dtype=w.dtype)
+                                    max_seq_len=max(P, max_new_tokens), device=w.device, dtype=cache_dtype or w.dtype)
         self.branches = [1]
         self.length = 0  # tokens of each branch
         self._device_ids: dict[tuple[int, ...], torch.Tensor] = {}
@@ -117,7 +126,8 @@ class BranchedGeneration:
             h = F.layer_norm(x, block.ln1.weight, block.ln1.bias, block.ln1.eps)
             q, k, v = F.linear(h, block.qkv.weight, block.qkv.bias).view(n, 3, self.heads, self.head_dim).unbind(1)
             c.append(layer, k, v, place, ids)
-            y = G.shared_prefix_attention(q, c.kv[layer, 0], c.kv[layer, 1], prefix, P, table, lens, max_seq_len=self.length)
+            y = G.shared_prefix_attention(q, c.kv[layer, 0], c.kv[layer, 1], prefix, P, table, lens, max_seq_len=self.length,
+                                          **c.scales_of(layer))
             x = self._rest(block, y.reshape(n, -1), x)
         self.logits = self._head(x)
         return self.logits
@@ -180,6 +190,13 @@ def sample_continuations(
     resample_every: int = 0,
     score: Callable[[torch.Tensor, torch.Tensor], torch.Tensor] | None = None,
     page_size: int = 16,
+    cache_dtype: torch.dtype | None = None,
+    repetition: float = 1.0,
+    presence: float = 0.0,
+    frequency: float = 0.0,
+    bias_tokens: torch.Tensor | None = None,
+    bias: torch.Tensor | None = None,
+    allowed: torch.Tensor | Callable[[torch.Tensor], torch.Tensor] | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Draw ``n`` continuations of ``prompt``; returns ``(tokens, logprobs)``, ``[n, max_new_tokens]`` each.
 
@@ -188,8 +205,19 @@ def sample_continuations(
     ``resample_every``, after every so many tokens the better half of the
     branches, by ``score(tokens, logprobs)`` (default: the mean
     log-probability; larger is better), is copied over the other half.
+
+    ``repetition`` counts the prompt's tokens and the branch's own, ``presence``
+    and ``frequency`` the branch's own; ``bias_tokens`` and ``bias`` are added
+    before the temperature, and only tokens that ``allowed`` has are drawn (see
+    :func:`~mini_nccl_b200.ops.generation.adjust_logits`).  ``allowed`` is one
+    mask, one for each branch, or a function that makes them from the tokens
+    drawn so far, ``[n, t]``.
     """
-    state = BranchedGeneration(model, prompt, max_branches=n, max_new_tokens=max_new_tokens, page_size=page_size)
+    if not repetition > 0:
+        raise ValueError("repetition: above 0 (1: no penalty)")
+    adjusted = repetition != 1 or presence != 0 or frequency != 0 or bias is not None or bias_tokens is not None or allowed is not None
+    state = BranchedGeneration(model, prompt, max_branches=n, max_new_tokens=max_new_tokens, page_size=page_size,
+                               cache_dtype=cache_dtype)
     state.select([0] * n)
     device = state.logits.device
     tokens = torch.empty(n, max_new_tokens, dtype=torch.long, device=device)
@@ -197,7 +225,12 @@ def sample_continuations(
     for t in range(max_new_tokens):
         noise = torch.empty(state.logits.shape, dtype=torch.float32, device=device)
         noise.exponential_(generator=generator).log_().neg_()
-        tokens[:, t], logprobs[:, t] = G.sample(state.logits, noise, temperature=temperature, top_k=top_k, top_p=top_p,
+        logits = state.logits
+        if adjusted:
+            masks = allowed(tokens[:, :t]) if callable(allowed) else allowed
+            logits = G.adjust_logits(logits, prompt=prompt.reshape(-1), history=tokens[:, :t], repetition=repetition, presence=presence,
+                                     frequency=frequency, bias_tokens=bias_tokens, bias=bias, allowed=masks)
+        tokens[:, t], logprobs[:, t] = G.sample(logits, noise, temperature=temperature, top_k=top_k, top_p=top_p,
                                                 min_p=min_p, return_logprob=True)
         if t + 1 == max_new_tokens:
             break

@@ -142,9 +142,11 @@ def shared_prefix_attention(
     Pages of int8 or float8_e4m3fn come with ``k_scales`` and ``v_scales``, fp32
     ``[num_pages, kv_heads]`` of one layout: page p's keys of head h are
     ``k_pages[p, :, h] * k_scales[p, h]``.  Scales are powers of two from
-    ``2 ** -60`` on (a smaller or no positive scale of values counts as
-    ``2 ** -60``), as :func:`append_kv` leaves them, or 0 where nothing was
-    written; others only cost accuracy.
+    ``2 ** -60`` to ``2 ** 60`` (a smaller or no positive scale of values
+    counts as ``2 ** -60``), as :func:`append_kv` leaves them for values up to
+    1e20, or 0 where nothing was written; others only cost accuracy, as do
+    scales more than ``2 ** 15`` apart within 128 tokens of the prefix, of which
+    the smaller ones' values lose their lowest bits.
 
     Returns ``o`` like ``q`` (contiguous) and, with ``return_lse``, the natural
     log-sum-exp of the scaled scores, fp32 ``[tokens, heads]``.  Head dims 32,

@@ -5,7 +5,11 @@ rounding that its definition has, so codes and scales have to be equal.  In
 the attention the weights are rounded to f16 (2^-11 of each) and the outputs to
 bf16 (2^-8 of the value); a score is an fp32 sum of D products, off by at most
 D 2^-24 sum |q_i k_i|, and is held in fp32 beside the logarithm of a scale
-(2^-24 of their sum, in log2 units), as is the row's base.  The adjustment of
+(2^-24 of their sum, in log2 units), as is the row's base.  Codes may be 0, so a
+column of the output may come from tokens of next to no weight alone: f16 holds
+a weight to 2^-25 absolutely where the largest of its row, times its scale (or
+the largest scale near it), is held as 2^7 or more, so a weight may also be off
+by 2^-32 of that, times each token's code.  The adjustment of
 logits is a chain of at most five fp32 operations, each off by 2^-24 of its
 result, and a rounding to the logits' type.
 """
@@ -281,10 +285,13 @@ class Problem:
             for t in range(n):
                 pool[:, pages[t // page], t % page] = code[:, t]
             of = scales[:, [pages[t // page] for t in range(n)]].double()
+            self.largest = max(self.largest, float(of[1].max()) if n else 0.0)
             return code.view(dtype).double() * of[..., None]
 
+        self.largest = 0.0  # of the values' scales
         self.head = fill(self.prefix_pages, prefix)
         self.own = [fill(r, m) for r, m in zip(self.rows, lens)]
+        self.top = TOP[dtype]
         self.lens, self.new, self.prefix, self.dim, self.group, self.least = lens, new, prefix, dim, group, exponents[0]
         wide = (torch.randn(sum(new), (H + 1) * dim, generator=gen) * scale_q).to(torch.bfloat16).to(device)
         self.q = wide[:, dim:].view(-1, H, dim)  # a slice of a wider projection
@@ -327,7 +334,8 @@ class Problem:
                     off = self.dim * U * (torch.einsum("hd,hkd->hk", qt.abs(), k[:, :seen].abs()) * abs(scale)).amax(-1) \
                         + 8 * U * (s.abs().amax(-1) + abs(self.least) + 40)
                     assert torch.all((lse[at] - torch.logsumexp(s, -1)).abs() <= off), ((lse[at] - torch.logsumexp(s, -1)).abs() / off).max()
-                    bound = 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2 * off[:, None]) * spread
+                    lost = 2.0 ** -32 * self.largest * self.top * (v[:, :seen] != 0).sum(1) * p.amax(1)
+                    bound = 2.0 ** -8 * (want.abs() + lost) + (2.0 ** -11 + 2 * off[:, None]) * spread + lost
                     assert torch.all((o[at] - want).abs() <= bound), ((o[at] - want).abs() / bound).max()
                 at += 1
 
