@@ -55,7 +55,7 @@ std::tuple<torch::Tensor, torch::Tensor> compact_pages(const torch::Tensor& kv, 
 void append_kv(const torch::Tensor& k_pages, const torch::Tensor& v_pages, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& page_table,
                const torch::Tensor& positions, const c10::optional<torch::Tensor>& slots,
                const OptionalTensor& k_scales, const OptionalTensor& v_scales, const torch::Tensor& status);
-void adjust_logits(const torch::Tensor& in, const torch::Tensor& out, const OptionalTensor& prompt, const OptionalTensor& history,
+torch::Tensor adjust_logits(const torch::Tensor& in, const OptionalTensor& given, const OptionalTensor& prompt, const OptionalTensor& history,
                    const OptionalTensor& history_lens, const OptionalTensor& repetition, double repetition_all, const OptionalTensor& presence,
                    double presence_all, const OptionalTensor& frequency, double frequency_all, const OptionalTensor& bias_tokens,
                    const OptionalTensor& bias, const OptionalTensor& allowed, const OptionalTensor& mask_of, const torch::Tensor& status);

@@ -347,7 +347,7 @@ logits::Ids ids_of(const c10::optional<torch::Tensor>& t, int64_t rows, const to
 
 }  // namespace
 
-void adjust_logits(const torch::Tensor& in, const torch::Tensor& out, const c10::optional<torch::Tensor>& prompt,
+torch::Tensor adjust_logits(const torch::Tensor& in, const c10::optional<torch::Tensor>& given, const c10::optional<torch::Tensor>& prompt,
                    const c10::optional<torch::Tensor>& history, const c10::optional<torch::Tensor>& history_lens,
                    const c10::optional<torch::Tensor>& repetition, double repetition_all, const c10::optional<torch::Tensor>& presence,
                    double presence_all, const c10::optional<torch::Tensor>& frequency, double frequency_all,
@@ -360,6 +360,7 @@ void adjust_logits(const torch::Tensor& in, const torch::Tensor& out, const c10:
   const int64_t R = in.size(0), V = in.size(1);
   TORCH_CHECK_VALUE(V >= 1 && V <= (1 << sampling::kIndexBits), "vocabulary: 1 to 1048576 tokens, got ", V);
   TORCH_CHECK_VALUE(in.stride(1) == 1 || V == 1, "logits: last axis contiguous");
+  const torch::Tensor out = given ? *given : at::empty(in.sizes(), in.options());
   TORCH_CHECK_VALUE(out.device() == in.device() && out.scalar_type() == in.scalar_type() && out.sizes() == in.sizes() &&
                         (out.stride(1) == 1 || V == 1) && (R <= 1 || out.stride(0) >= V),
                     "out: a tensor like logits, last axis contiguous, rows apart");
@@ -402,7 +403,7 @@ void adjust_logits(const torch::Tensor& in, const torch::Tensor& out, const c10:
   } else {
     TORCH_CHECK_VALUE(!mask_of, "mask_of: needs allowed");
   }
-  if (R == 0) return;
+  if (R == 0) return out;
   TORCH_CHECK_VALUE(R * ((V + 2047) / 2048 + 1) < (1ll << 31), "too many rows");
   const c10::cuda::CUDAGuard guard(in.device());
   a.in = in.data_ptr();
@@ -419,6 +420,7 @@ void adjust_logits(const torch::Tensor& in, const torch::Tensor& out, const c10:
   a.status = errors_of(status);
   C10_CUDA_CHECK(logits::launch_adjust(a, at::cuda::getCurrentCUDAStream()));
   launched = 1;
+  return out;
 }
 
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(

@@ -365,24 +365,24 @@ def adjust_logits(
     overlaps it.  A token or a mask that there is none of, and a length outside
     the history (the history then counts for nothing), are reported.
     """
-    if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     if logits.is_cuda:
-
-        def split(x):
-            return (x, 0.0) if isinstance(x, torch.Tensor) else (None, float(x))
-
-        K = _kernels()
-        given = (logits, *(t for t in (repetition, presence, frequency, bias) if isinstance(t, torch.Tensor)))
-        wanted = torch.is_grad_enabled() and any(t.requires_grad for t in given)
-        _need(not (wanted and out is logits), "out: not in place where a gradient is wanted")
-        K.ext().adjust_logits(logits, out, prompt, history, history_lens, *split(repetition), *split(presence), *split(frequency),
-                              bias_tokens, bias, allowed, mask_of, K.status_word(logits.device))
-        return _NoGradient.apply("adjust_logits", out, *given) if wanted else out
+        K, tensor = _kernels(), torch.Tensor
+        rho, by_rho = (repetition, 0.0) if isinstance(repetition, tensor) else (None, repetition)
+        alpha, by_alpha = (presence, 0.0) if isinstance(presence, tensor) else (None, presence)
+        phi, by_phi = (frequency, 0.0) if isinstance(frequency, tensor) else (None, frequency)
+        wanted = torch.is_grad_enabled() and (
+            logits.requires_grad or (rho is not None and rho.requires_grad) or (alpha is not None and alpha.requires_grad)
+            or (phi is not None and phi.requires_grad) or (bias is not None and bias.requires_grad))
+        _need(not wanted or out is not logits, "out: not in place where a gradient is wanted")
+        y = K.ext().adjust_logits(logits, out, prompt, history, history_lens, rho, by_rho, alpha, by_alpha, phi, by_phi, bias_tokens, bias,
+                                  allowed, mask_of, K.status_word(logits.device))
+        return _NoGradient.apply("adjust_logits", y, logits, rho, alpha, phi, bias) if wanted else y if out is None else out
     _need(logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32),
           "logits: a bf16 or fp32 tensor [rows, vocabulary]")
     R, V = logits.shape
     _need(1 <= V <= 1 << 20, f"vocabulary: 1 to 1048576 tokens, got {V}")
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype)
     _need(out.shape == logits.shape and out.dtype == logits.dtype, "out: a tensor like logits")
 
     def column(x, what):
