@@ -21,7 +21,7 @@
 // and 20 us before the first and after the last.  (With few rows raw tiles also lie where
 // the second stream's queries would be, so that 64 KB are under way.)  Measured: 48 rows of
 // 8 kv heads behind 100003 tokens 93 us (2.4 TB/s of codes), 160 rows of 16 heads behind
-// 8003 tokens 87 us with their own keys, 2400 ragged rows of 32 heads 211 us with theirs.
+// 8003 tokens 87 us with their own keys, 1504 ragged rows of 32 heads 199 us with theirs.
 #include <type_traits>
 
 #include "launch.cuh"
