@@ -237,6 +237,10 @@ void append_kv(const torch::Tensor& k_pages, const torch::Tensor& v_pages, const
   } else {
     TORCH_CHECK_VALUE(n <= page_table.size(0), "without slots, token i belongs to row i of page_table: too many tokens");
   }
+  if (codes)
+    TORCH_CHECK_VALUE(k_pages.numel() == 0 || (k_scales->data_ptr() != v_scales->data_ptr() && (k_scales->size(0) <= 1 || k_scales->stride(0) != 0) &&
+                                               (H <= 1 || k_scales->stride(1) != 0)),
+                      "k_scales and v_scales: memory of their own for each page and head");
   if (n * H * D == 0 || k_pages.size(1) == 0) return;
   const c10::cuda::CUDAGuard guard(k_pages.device());
   TORCH_CHECK_VALUE(n < (1ll << 31), "too many tokens");
@@ -483,8 +487,9 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> shared_prefix_attention(
   if (codes) {
     a.k8 = bytes(k_of);
     a.v8 = bytes(v_of);
-    a.k_scales = k_scales->data_ptr<float>();
-    a.v_scales = v_scales->data_ptr<float>();
+    // (an address also where there are no pages and nothing will be read)
+    a.k_scales = pages > 0 ? k_scales->data_ptr<float>() : reinterpret_cast<const float*>(q.data_ptr());
+    a.v_scales = pages > 0 ? v_scales->data_ptr<float>() : a.k_scales;
     a.scale_ld = k_scales->stride(0);
     a.scale_head = k_scales->stride(1);
   } else {

@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(kThreads, 5) adjust_kernel(const __grid_consta
   const bool in_aligned = reinterpret_cast<uintptr_t>(in + first * kSize) % 16 == 0;
 
   int of = -1;  // the row's mask
-  if (a.masks > 0) {
+  if (a.mask_of || a.masks > 0) {
     of = a.mask_of ? a.mask_of[row] : a.masks > 1 ? row : 0;
     if (of >= a.masks) {
       if (threadIdx.x == 0) atomicCAS(a.status, 0, kErrBadIndex);

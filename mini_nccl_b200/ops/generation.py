@@ -165,8 +165,10 @@ def shared_prefix_attention(
             q, k_pages, v_pages, prefix_pages, prefix_len, page_table, seq_lens, q_offsets,
             -1 if max_q_len is None else max_q_len, -1 if max_seq_len is None else max_seq_len, scale, return_lse, k_scales, v_scales,
             K.status_word(q.device))
-        if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
-            o, lse = (None if t is None else _NoGradient.apply("shared_prefix_attention", t, q, k_pages, v_pages) for t in (o, lse))
+        if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad
+                                        or (k_scales is not None and (k_scales.requires_grad or v_scales.requires_grad))):
+            o, lse = (None if t is None else _NoGradient.apply("shared_prefix_attention", t, q, k_pages, v_pages, k_scales, v_scales)
+                      for t in (o, lse))
         return (o, lse) if return_lse else o
     _need(q.dim() == 3 and k_pages.dim() == 4 and k_pages.shape == v_pages.shape,
           "q: [tokens, heads, head_dim]; k_pages and v_pages: [num_pages, page_size, kv_heads, head_dim]")
@@ -502,11 +504,11 @@ def append_kv(
     pages have to be there (:func:`reserve_pages`) and must not be shared.
 
     Pages of int8 or float8_e4m3fn come with ``k_scales`` and ``v_scales``, fp32
-    ``[num_pages, kv_heads]``, which are written too.  A page's values of one
-    head share a scale, the least power of two (from ``2 ** -60`` on) whose
-    multiple by the largest code (127 or 448) is at least the largest of them;
-    each value becomes the nearest code, of two the even one.  Writing a page's
-    first place begins the page: its scale then comes from this call's tokens
+    ``[num_pages, kv_heads]``, which are written too (so they do not share
+    memory).  A page's values of one head share a scale, the least power of two
+    (from ``2 ** -60`` on) whose multiple by the largest code (127 or 448) is at
+    least the largest of them; each value becomes the nearest code, of two the
+    even one.  Writing a page's first place begins the page: its scale then comes from this call's tokens
     alone.  Otherwise the scale only grows, and the codes that are there are
     rounded to the new one.  Values that are not finite do not count for the
     scale; an infinite one is stored as the largest code, NaN as float8_e4m3fn's
@@ -522,6 +524,10 @@ def append_kv(
           and k.shape[1:] == k_pages.shape[2:], "k, v: [tokens, kv_heads, head_dim] as in the pages")
     coded = _held_in_8_bits(k_pages, v_pages, k_scales, v_scales)
     _need(not coded or (k.shape[2] % 16 == 0 and k.shape[2] <= 256), "head_dim: in 8 bits a multiple of 16, at most 256")
+    _need(not coded or k_pages.numel() == 0 or (
+        k_scales.data_ptr() != v_scales.data_ptr()
+        and all(s.shape[i] <= 1 or s.stride(i) != 0 for s in (k_scales, v_scales) for i in (0, 1))),
+        "k_scales and v_scales: memory of their own for each page and head")
     _ints(page_table, 2, "page_table")
     named = [(positions, "positions")] + ([(slots, "slots")] if slots is not None else [])
     where = _ids(*named)

@@ -204,6 +204,36 @@ def test_attention_no_rows_and_no_tokens(device, dtype):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lens,new,kv_heads,group,dim,page,prefix", [
+    ([5, 70, 0], [1, 1, 1], 1, 71, 64, 16, 50),
+    ([5, 70, 3], [2, 9, 1], 1, 40, 128, 16, 50),
+    ([5, 70, 3], [1, 1, 1], 2, 64, 32, 8, 0),
+    pytest.param([5, 70, 3], [2, 9, 1], 1, 64, 128, 16, 5000, marks=pytest.mark.gpu),
+    ([300], [300], 1, 1, 64, 256, 0),
+])
+def test_attention_many_heads_to_one(device, lens, new, kv_heads, group, dim, page, prefix):
+    p = Problem(lens, new, kv_heads=kv_heads, group=group, dim=dim, page=page, prefix=prefix, device=device, dtype=torch.int8)
+    p.check(*p.run())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_on_a_pool_without_pages(device, dtype):
+    pool, scales = torch.zeros(0, 8, 2, 64, device=device).to(dtype), torch.zeros(0, 2, device=device)
+    q = torch.randn(3, 4, 64, device=device).to(torch.bfloat16)
+
+    def call(prefix, lens):
+        return G.shared_prefix_attention(q, pool, pool, ints([0], device), prefix, ints([[-1], [-1], [0]], device), ints(lens, device),
+                                         k_scales=scales, v_scales=scales)
+
+    assert torch.all(call(0, [0, 0, 0]) == 0)
+    settle(device)
+    for prefix, lens in ((5, [0, 0, 0]), (0, [0, 0, 3])):
+        o = out_of_range(device, lambda: call(prefix, lens))
+        assert o is None or torch.all(o == 0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_attention_refusals(device):
     def call(dtype=torch.int8, v_dtype=None, scales=(4, 2), of=torch.float32, only_k=False, q=(3, 4, 64), rows=3, **more):
         pool = [torch.zeros(4, 8, 2, 64, device=device).to(t) for t in (dtype, v_dtype or dtype)]
@@ -350,6 +380,10 @@ def test_gradients_are_refused_not_lost():
     for out in (o, lse):
         with pytest.raises(RuntimeError, match="no gradient"):
             out.float().sum().backward()
+    p.q = p.q.detach()
+    p.scales.requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        p.run()[0].float().sum().backward()
     x, b = torch.randn(2, 50, device="cuda", requires_grad=True), torch.randn(1, device="cuda", requires_grad=True)
     for y in (G.adjust_logits(x, repetition=2.0, prompt=ints([3], "cuda")),
               G.adjust_logits(x.detach(), bias_tokens=ints([3], "cuda"), bias=b)):
@@ -413,6 +447,17 @@ def test_page_operations_take_the_scales_along(device, dtype):
             G.compact_pages(c.kv, c.page_table, c.refs, bad)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_append_refuses_scales_that_share_memory(device):
+    pool, scales = torch.zeros(2, 4, 8, 2, 16, dtype=torch.int8, device=device), torch.zeros(2, 4, 2, device=device)
+    k, v = tokens_of(1, 2, 16, device, 0)
+    for a, b in ((scales[0], scales[0]), (scales[0, :, :1].expand(4, 2), scales[1, :, :1].expand(4, 2)),
+                 (scales[0, :1].expand(4, 2), scales[1, :1].expand(4, 2))):
+        with pytest.raises(ValueError, match="of their own"):
+            G.append_kv(pool[0], pool[1], k, v, ints([[1]], device), ints([0], device), k_scales=a, v_scales=b)
+    settle(device)
+
+
 # ---- logits ------------------------------------------------------------------------------
 
 
@@ -459,6 +504,10 @@ def test_adjust_logits_reports_what_there_is_not(device):
     assert y is None or torch.equal(y, want)
     y = bad(allowed=torch.full((2, 3), -1, dtype=torch.int32, device=device), mask_of=ints([0, 2, -1], device))
     assert y is None or torch.equal(y[[0, 2]], want[[0, 2]])
+    none = torch.empty(0, 3, dtype=torch.int32, device=device)
+    y = bad(allowed=none, mask_of=ints([-1, 0, -1], device))
+    assert y is None or torch.equal(y, want)
+    assert torch.equal(G.adjust_logits(x, **good, allowed=none, mask_of=ints([-1, -1, -1], device)), want)
     settle(device)
 
 
