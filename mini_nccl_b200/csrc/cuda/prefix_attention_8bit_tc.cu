@@ -330,9 +330,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t raw_phase = 0, phase = 1;
     for (int t = 0; t < n_tiles; ++t) {
       const int valid = valid_of(t);
-      if (!warp_wait(raw_full0 + 8 * r, raw_phase, a.status) || !warp_wait(scaled0 + 8 * r, raw_phase, a.status) ||
-          !warp_wait(empty0 + 8 * st, phase, a.status))
-        break;
+      // (the factors come from a warp that has waited for the codes)
+      if (!warp_wait(scaled0 + 8 * r, raw_phase, a.status)) break;
       const float* const factors = reinterpret_cast<const float*>(sm + S::scale_off) + (r * 2 + group) * 16;
       const float factor = factors[min(row, valid - 1) >> per_shift];
       const uint32_t by = pack_f16x2(factor, factor);
@@ -343,13 +342,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint8_t* const from = sm + raw_at(r) + row * D;
       uint8_t* const to = sm + S::kv_off + st * S::kv_tile + row * 128;
       const int turn_in = D == 128 ? row & 7 : (row >> 1) & 3, turn_out = row & 7;
+      uint4 w[4];
+      auto load = [&](int c0) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = ld_v4(from + (((c0 + k) ^ turn_in) << 4));
+        if (!there) w[0] = w[1] = w[2] = w[3] = make_uint4(0, 0, 0, 0);  // past the end a page holds anything
+      };
+      load(0);  // (on their way while the f16 tile's place is waited for)
+      if (!warp_wait(empty0 + 8 * st, phase, a.status)) break;
       auto widen_row = [&](auto by_powers) {
 #pragma unroll
         for (int c0 = 0; c0 < D / 16; c0 += 4) {
-          uint4 w[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) w[k] = ld_v4(from + (((c0 + k) ^ turn_in) << 4));
-          if (!there) w[0] = w[1] = w[2] = w[3] = make_uint4(0, 0, 0, 0);  // past the end a page holds anything
+          if (c0 > 0) load(c0);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             uint32_t y[8];
