@@ -15,9 +15,9 @@
 // takes the word out first writes the token.  Only words of named tokens are ever
 // touched.  (Penalties applied on the way, in the copying pass, cost every warp the
 // arithmetic of each of its lanes' tokens in turn: 512 x 50304 with 1300 tokens named in
-// a row, 63 us.)  Measured: 512 x 50304 in bf16 34 us (3.0 TB/s; the lists are read by
+// a row, 63 us.)  Measured: 512 x 50304 in bf16 33 us (3.1 TB/s; the lists are read by
 // each of a row's seven blocks), 129 x 130003 in fp32 under a mask and biases each
-// 34 us (4.0 TB/s), 64 x 50304 in fp32 under masks that leave a twenty-fifth 11 us, one
+// 33 us (4.1 TB/s), 64 x 50304 in fp32 under masks that leave a twenty-fifth 9 us, one
 // row 4 us.
 #include <algorithm>
 
@@ -46,13 +46,16 @@ MNB_DEVICE float adjusted(float x, uint32_t named, float repetition, float prese
   return x;
 }
 
-// A block takes kThreads * kPer groups of eight tokens of a row.
+// A block takes kThreads * kPer groups of eight tokens of a row.  (Six blocks to an SM fit fp32, 34 -> 32 us at 129 x 130003, at
+// the price of some registers spilled; with bf16 their shared memory would take too much of L1, 34 -> 37 us at 512 x 50304.)
 template <bool kBf16, int kThreads, int kPer>
-__global__ void __launch_bounds__(kThreads, 5) adjust_kernel(const __grid_constant__ Adjust a, int chunks) {
-  constexpr int kSize = kBf16 ? 2 : 4, kWords = kBf16 ? 4 : 8, kTokens = kThreads * kPer * 8, kList = 1024;
+__global__ void __launch_bounds__(kThreads, kBf16 ? 5 : 6) adjust_kernel(const __grid_constant__ Adjust a, int chunks) {
+  constexpr int kSize = kBf16 ? 2 : 4, kWords = kBf16 ? 4 : 8, kTokens = kThreads * kPer * 8, kList = 2048;
   static_assert(kTokens <= 1 << 14, "a place's bits");
   extern __shared__ uint32_t named[];  // [kTokens], where some list names tokens
-  __shared__ uint32_t list[kList];
+  // Places, and which list names them.  (32 bits each would be room for half as many: 82 rows with a prompt of 2232 tokens 17
+  // us, so 11.  More room takes it from L1: 512 x 50304 35 us, so 33.)
+  __shared__ uint16_t list[kList];
   __shared__ int listed;
   const int row = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
   const char* const in = static_cast<const char*>(a.in) + row * a.in_ld * kSize;
@@ -152,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, 5) adjust_kernel(const __grid_consta
     const int n = listed;
     if (n > kList) scan_all(f);
     else
-      for (int i = threadIdx.x; i < n; i += kThreads) f(list[i]);
+      for (int i = threadIdx.x; i < n; i += kThreads) f(static_cast<uint32_t>(list[i]));
   };
   auto place = [](uint32_t x) { return x & 0x3fffu; };
   auto kind = [](uint32_t x) { return x >> 14 & 3u; };
@@ -162,13 +165,11 @@ __global__ void __launch_bounds__(kThreads, 5) adjust_kernel(const __grid_consta
     scan_all([&](uint32_t x) {
       named[place(x)] = 0;
       const int i = atomicAdd(&listed, 1);
-      if (i < kList) list[i] = x;
+      if (i < kList) list[i] = static_cast<uint16_t>(x);
     });
     __syncthreads();
     if (biases > 0) {  // (the later one of a token that is named twice)
-      each([&](uint32_t x) {
-        if (kind(x) == 2) atomicMax(named + place(x), ((x >> 16) + 1) << kBiasShift);
-      });
+      scan(a.bias_tokens, biases, 2, [&](uint32_t x) { atomicMax(named + place(x), ((x >> 16) + 1) << kBiasShift); });
       __syncthreads();
     }
     each([&](uint32_t x) {
