@@ -20,8 +20,10 @@
 // memory's bandwidth: 1.4 us for a tile of 128 keys whether one stream has rows or both,
 // and 20 us before the first and after the last.  (With few rows raw tiles also lie where
 // the second stream's queries would be, so that 64 KB are under way.)  Measured: 48 rows of
-// 8 kv heads behind 100003 tokens 93 us (2.4 TB/s of codes), 160 rows of 16 heads behind
-// 8003 tokens 87 us with their own keys, 1504 ragged rows of 32 heads 199 us with theirs.
+// 8 kv heads behind 100003 tokens 92 us (2.4 TB/s of codes), 160 rows of 16 heads behind
+// 8003 tokens 86 us with their own keys, 1504 ragged rows of 32 heads 194 us with theirs.
+// (The keys' raw tiles two or three deep, with one f16 tile of values less, changed nothing:
+// 202 and 96 us.  The two halves of a row meeting alone, not their whole stream, neither.)
 #include <type_traits>
 
 #include "launch.cuh"
@@ -399,14 +401,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int r = quad * 32 + lane;                 // row of the stream's tile
     float* const row_back = reinterpret_cast<float*>(sm + S::max_off);
     {  // Q as f16, each row times a power of two, swizzled as TMA would leave it; rows past the last are zeros
-      constexpr int kChunks = D / 8, kStep = kSoftmax / kChunks, kAhead = 4;  // a thread keeps its chunk and goes through the rows
+      constexpr int kChunks = D / 8, kStep = kSoftmax / kChunks, kAhead = 8;  // a thread keeps its chunk and goes through the rows
       const int c = (threadIdx.x - 32 * kFirst) % kChunks, rows_end = shared ? 2 * kTile : kTile;
-      for (int i0 = (threadIdx.x - 32 * kFirst) / kChunks; i0 < rows_end; i0 += kStep * kAhead) {
+      // (a row's token and which head of the group: kStep rows further without a division each)
+      int i0 = (threadIdx.x - 32 * kFirst) / kChunks, token = (r0 + i0) / a.group, member = r0 + i0 - token * a.group;
+      const int tokens_on = kStep / a.group, members_on = kStep - tokens_on * a.group;
+      for (; i0 < rows_end; i0 += kStep * kAhead) {
         uint4 w[kAhead];
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
-          const int i = i0 + k * kStep, j = r0 + i;
-          w[k] = i < n_rows ? ld_v4(a.q + (j / a.group) * a.q_ld + (h * a.group + j % a.group) * a.q_head + c * 8) : make_uint4(0, 0, 0, 0);
+          w[k] = make_uint4(0, 0, 0, 0);
+          if (i0 + k * kStep < n_rows) w[k] = ld_v4(a.q + token * a.q_ld + (h * a.group + member) * a.q_head + c * 8);
+          token += tokens_on, member += members_on;
+          if (member >= a.group) ++token, member -= a.group;
         }
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
@@ -541,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       tc_fence_after();
     }
-    finish_rows<D>(a, sm + S::kv_off, t_o, m, l * 3.0517578125e-5f, steps, s, half, r, warp - kFirst, n_rows, r0, h, split, shared);
+    finish_rows<D, 4>(a, sm + S::kv_off, t_o, m, l * 3.0517578125e-5f, steps, s, half, r, warp - kFirst, n_rows, r0, h, split, shared);
     tc_fence_before();
   }
   __syncthreads();

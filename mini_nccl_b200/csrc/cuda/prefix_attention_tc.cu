@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       tc_fence_after();
     }
-    finish_rows<D>(a, sm + S::kv_off, t_o, m, l, steps, s, half, r, warp - 2, n_rows, r0, h, split, shared);
+    finish_rows<D, 2>(a, sm + S::kv_off, t_o, m, l, steps, s, half, r, warp - 2, n_rows, r0, h, split, shared);
     tc_fence_before();
   }
   __syncthreads();

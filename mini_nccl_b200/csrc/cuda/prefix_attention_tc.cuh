@@ -76,8 +76,9 @@ template <int D>
 constexpr int kMeeting = 2 * kTile * ((D + 4) * 4 + 8 + 20 + 4);
 
 // The end of a block's softmax warps (number `self` of 16): row r of stream s has its base m, its half's sum l and its output
-// at t_o in TMEM.  With one prefix piece the rows are joined with their own keys' pieces and finished.
-template <int D>
+// at t_o in TMEM.  With one prefix piece the rows are joined with their own keys' pieces and finished.  kBatch: rows of a warp
+// whose loads are under way together.
+template <int D, int kBatch>
 MNB_DEVICE void finish_rows(const Args& a, uint8_t* ring, uint32_t t_o, float m, float l, int steps, int s, int half, int r, int self,
                             int n_rows, int r0, int h, int split, bool shared) {
   const int lane = threadIdx.x % 32;
@@ -143,7 +144,6 @@ MNB_DEVICE void finish_rows(const Args& a, uint8_t* ring, uint32_t t_o, float m,
     info[i] = x;
   }
   softmax_sync();
-  constexpr int kBatch = 2;  // rows whose loads are under way together
   for (int i0 = self * kBatch; i0 < n_rows; i0 += kSoftmax / 32 * kBatch) {
     Part o[kBatch];
     Row x[kBatch];
