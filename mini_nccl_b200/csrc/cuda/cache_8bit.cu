@@ -133,6 +133,11 @@ __global__ void __launch_bounds__(32 * kWarps) append8_kernel(const __grid_const
     const int of = __ffs(begins) - 1;
     const long long i0 = w0 + window - 32 + of;
     const int p = __shfl_sync(0xffffffffu, page, of);
+    // A run of a page that had one before it would meet that one's warp there: left out, where it can be seen from here.
+    if (__ballot_sync(0xffffffffu, page == p) & ((1u << of) - 1)) {
+      if (lane == 0) atomicCAS(status, 0, kErrScattered);
+      continue;
+    }
     // f(the run's tokens from c0 on: how many of 32 to look at, this lane's page and place)
     auto run = [&](auto f) {
       for (long long c0 = i0;; c0 += 32) {

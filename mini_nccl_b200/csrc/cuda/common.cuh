@@ -26,6 +26,7 @@ enum : int {
   kErrNoPages = 4,         // the key / value cache's pool has too few free pages
   kErrBadIndex = 5,        // a token, page, slot, position or length outside its tensor
   kErrNotANumber = 6,      // NaN among values that are to be held as int8
+  kErrScattered = 7,       // tokens of one page of a cache in 8 bits that do not follow one another
 };
 
 // ---------------------------------------------------------------------------

@@ -514,7 +514,9 @@ def append_kv(
     scale; an infinite one is stored as the largest code, NaN as float8_e4m3fn's
     NaN, or as int8 zero (and reported).  In a call the tokens of one page follow
     one another (padding aside), in any order; a place that is named twice gets
-    the later one.  Head dims that are multiples of 16, up to 256.
+    the later one.  Tokens that come back to a page are left out and reported
+    where a kernel sees it (among 32 tokens one after another, in calls of few);
+    further apart what the page then holds is undefined.  Head dims that are multiples of 16, up to 256.
     """
     if k_pages.is_cuda:
         K = _kernels()

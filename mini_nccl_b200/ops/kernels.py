@@ -69,7 +69,8 @@ def fold_accumulator(device: torch.device, n: int) -> torch.Tensor:
 #: Status codes of the page operations, the paged attention and the embedding (csrc/cuda/common.cuh).
 _REQUEST_STATUS = {4: "the key / value cache's pool has too few free pages",
                    5: "a token, page, slot, position or length outside its tensor",
-                   6: "NaN among keys or values that are held as int8"}
+                   6: "NaN among keys or values that are held as int8",
+                   7: "tokens of one page of a cache in 8 bits that do not follow one another"}
 
 
 def check_status(device: torch.device | None = None) -> None:

@@ -240,6 +240,26 @@ def test_append_refuses_scattered_pages_on_the_cpu():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_append_leaves_out_tokens_that_come_back_to_a_page(dtype):
+    from mini_nccl_b200.ops import kernels as K
+
+    k, v = tokens_of(5, 2, 64, "cuda", 0)
+    held = []
+    for positions, slots in (([0, 8, 1, 9, 2], [0, 1, 0, 1, 0]), ([0, 8], [0, 1])):
+        c = Cache(6, 8, 2, 64, dtype, "cuda")
+        n = len(positions)
+        G.append_kv(c.kv[0], c.kv[1], k[:n], v[:n], ints([[4, 0], [2, 5]], "cuda"), ints(positions, "cuda"), ints(slots, "cuda"),
+                    k_scales=c.scales[0], v_scales=c.scales[1])
+        held.append(c)
+        if n == 5:
+            with pytest.raises(RuntimeError, match="do not follow one another"):
+                K.check_status()
+    settle("cuda")
+    assert torch.equal(held[0].kv.view(torch.uint8), held[1].kv.view(torch.uint8)) and torch.equal(held[0].scales, held[1].scales)
+
+
+@pytest.mark.gpu
 def test_append_leaves_bad_requests_out():
     from mini_nccl_b200.ops import kernels as K
 
